@@ -58,6 +58,7 @@ extern "C" {
 #define MJ_DEV_BAD_PAGE 1    /* block-table entry or slot page outside [0, num_pages) */
 #define MJ_DEV_BAD_SPLIT 2   /* work item split >= max_splits or seq >= part_seqs */
 #define MJ_DEV_TIMEOUT 3     /* a bounded wait in a pipelined kernel gave up */
+#define MJ_DEV_BAD_POSITION 4 /* a position outside the cos / sin table */
 
 /* KV formats. e2m3 / e3m2: 6-bit codes (sign | exponent | mantissa, biases
  * 1 / 3, maxima 7.5 / 28, no inf or NaN) packed 4 per 3 bytes little-endian;
@@ -74,6 +75,20 @@ extern "C" {
 #define MJ_KV_E3M2 2
 #define MJ_KV_E2M1 3
 #define MJ_KV_NVFP4 4
+/* Block-scaled fp8: e4m3 codes with one power-of-two scale per (block of G
+ * consecutive tokens of a page, KV head), G = 16, 32, 64 or 128 (a divisor of
+ * the page size). The scale tensors hold exponent bytes e of the scale
+ * 2^(e - 127), logical (num_pages, page_size / G, h_k); a cached value is
+ * code * 2^(e - 127). Written by mj_block_write, read by mj_block_read,
+ * mj_block_attention and mj_decode. Writers produce e in
+ * [MJ_BLOCK_E_MIN, MJ_BLOCK_E_MAX]; readers take a byte outside as the nearest
+ * of the two. */
+#define MJ_KV_FP8_B16 5
+#define MJ_KV_FP8_B32 6
+#define MJ_KV_FP8_B64 7
+#define MJ_KV_FP8_B128 8
+#define MJ_BLOCK_E_MIN 95  /* 2^-32 */
+#define MJ_BLOCK_E_MAX 159 /* 2^32 */
 
 /* element types of Q / O / new K,V rows */
 #define MJ_DT_BF16 0
@@ -320,6 +335,126 @@ int mj_expand_pages(const mj_expand_args* args, void* stream);
  * (nothing in it needs to start at zero); calls that overlap on the GPU
  * race on it and must be ordered. */
 int mj_decode_noalloc(const mj_decode_args* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* RMS norm of every Q and K head row with the position rotation, one pass.  */
+/* y = x * rsqrt(mean(x^2) + eps) * weight (no norm where the weight pointer */
+/* is null), then for i < rot_dim / 2 the pair (a, b) -- elements (i, i +     */
+/* rot_dim / 2), or (2 i, 2 i + 1) when interleaved -- becomes                */
+/* (a cos - b sin, b cos + a sin) with cos = cos_sin[position][i], sin =      */
+/* cos_sin[position][rot_dim / 2 + i]; elements from rot_dim on keep y. All   */
+/* of it in fp32, rounded once. Q and K are read and written through token    */
+/* and head strides; the outputs may be the inputs (in place) but must not    */
+/* overlap them otherwise. A position outside [0, num_positions) flags        */
+/* MJ_DEV_BAD_POSITION and leaves that token's rows untouched.                */
+typedef struct mj_qk_norm_rope_args {
+  const void* q;                /* (num_tokens, h_q, head_size), head dim contiguous; may be null with h_q = 0 */
+  const void* k;                /* (num_tokens, h_k, head_size); may be null with h_k = 0 */
+  void* q_out;
+  void* k_out;
+  int dtype;                    /* MJ_DT_* of q, k and the outputs */
+  int64_t num_tokens;
+  int h_q, h_k;
+  int head_size;                /* a multiple of 16, at most 512 */
+  int rot_dim;                  /* a multiple of 16, at most head_size; 0 = no rotation */
+  int interleaved;
+  int64_t q_stride_tok, q_stride_head, k_stride_tok, k_stride_head;     /* elements */
+  int64_t qo_stride_tok, qo_stride_head, ko_stride_tok, ko_stride_head; /* elements */
+  const int64_t* positions;     /* (num_tokens,) */
+  const void* cos_sin;          /* (num_positions, rot_dim): cos | sin halves, rows contiguous */
+  int cos_sin_dtype;            /* MJ_DT_* */
+  int64_t cos_sin_stride;       /* elements between rows */
+  int64_t num_positions;
+  const void* q_weight;         /* optional (head_size,) of weight_dtype */
+  const void* k_weight;
+  int weight_dtype;             /* MJ_DT_* */
+  float eps;
+  int32_t* status;              /* optional device status word (MJ_DEV_*) */
+} mj_qk_norm_rope_args;
+
+int mj_qk_norm_rope(const mj_qk_norm_rope_args* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Quantising write into a block-scaled cache (kv_format MJ_KV_FP8_B16 ..     */
+/* _B128 of a mj_cache_write_args; k_scale / v_scale and their modes are not  */
+/* read, ks_stride_row / vs_stride_row are the byte strides between blocks,   */
+/* head_size 128 or 256). Of the rows that this call writes into a block, the */
+/* largest finite magnitude amax asks for the smallest e in [95, 159] with    */
+/* amax <= 448 * 2^(e - 127). A call that writes row 0 of a block opens it    */
+/* and takes that e. Otherwise the block keeps the larger of its e and the    */
+/* new one, and when its e grows, its rows that this call does not write      */
+/* follow: code <- e4m3(code * 2^(e_old - e_new)), exact but for codes that   */
+/* become subnormal. New codes are e4m3(x * 2^(127 - e)), to nearest even,    */
+/* saturating at +-448 (infinities too); NaN stays NaN. slot_mapping as in    */
+/* mj_cache_write; the tokens that one call writes into one block stand       */
+/* together in it (only negative entries between them) and their slots        */
+/* differ. Where they do not, that block's contents are unspecified.          */
+int mj_block_write(const mj_cache_write_args* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Tokens of a block-scaled cache back as contiguous rows: output rows        */
+/* offsets[s] .. offsets[s + 1] - 1 receive tokens starts[s], starts[s] + 1,  */
+/* ... of sequence s, K into k_out and V into v_out: code * 2^(e - 127)       */
+/* rounded to out_dtype. A page outside [0, num_pages), or a token past the   */
+/* block table's columns, flags MJ_DEV_BAD_PAGE and leaves its rows           */
+/* untouched, as rows from offsets[num_seqs] on are.                          */
+typedef struct mj_block_read_args {
+  const void* k_cache;          /* logical (num_pages, page_size, h_k, head_size) e4m3 codes */
+  const void* v_cache;
+  int64_t k_stride_page, k_stride_row, k_stride_head; /* bytes */
+  int64_t v_stride_page, v_stride_row, v_stride_head; /* bytes */
+  const void* k_scales;         /* logical (num_pages, page_size / G, h_k) exponent bytes */
+  const void* v_scales;
+  int64_t ks_stride_page, ks_stride_block, ks_stride_head; /* bytes */
+  int64_t vs_stride_page, vs_stride_block, vs_stride_head; /* bytes */
+  int64_t num_pages;
+  int page_size, h_k, head_size; /* head_size 128 or 256 */
+  int kv_format;                /* MJ_KV_FP8_B16 .. _B128 */
+  const int32_t* block_table; int64_t block_table_stride; int block_table_cols;
+  const int32_t* starts;        /* (num_seqs,), >= 0 */
+  const int32_t* offsets;       /* (num_seqs + 1,), ascending from 0 */
+  int num_seqs;
+  int64_t num_rows;             /* rows of the outputs */
+  void* k_out;                  /* (num_rows, h_k, head_size), head dim contiguous */
+  void* v_out;
+  int out_dtype;                /* MJ_DT_* */
+  int64_t ko_stride_tok, ko_stride_head, vo_stride_tok, vo_stride_head; /* elements */
+  int32_t* status;              /* optional device status word (MJ_DEV_*) */
+} mj_block_read_args;
+
+int mj_block_read(const mj_block_read_args* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Attention of ragged query chunks over a block-scaled cache. Query rows     */
+/* q_start[s] .. q_start[s + 1] - 1 are the last n_s tokens of sequence s     */
+/* (seq_lens[s] INCLUDES them); with causal != 0 query i of n_s sees keys     */
+/* 0 .. seq_lens[s] - n_s + i, otherwise all seq_lens[s]. A query that sees   */
+/* no key gets O = 0 and LSE = -inf. Masked and unwritten cache rows may hold */
+/* any bytes. q and o share a dtype (bf16 or fp16).                           */
+typedef struct mj_block_attn_args {
+  int num_seqs, h_q, h_k, head_size; /* head_size 128 or 256 */
+  int page_size, kv_format;          /* page 16, 32, 64 or 128; MJ_KV_FP8_B16 .. _B128 */
+  int dtype;                         /* MJ_DT_BF16 or MJ_DT_FP16 */
+  const void* q; int64_t q_stride_tok, q_stride_head; /* elements */
+  void* o; int64_t o_stride_tok, o_stride_head;       /* elements */
+  int64_t num_tokens;                /* rows of q and o */
+  const void* k_cache; const void* v_cache;
+  int64_t k_stride_page, k_stride_row, k_stride_head; /* bytes */
+  int64_t v_stride_page, v_stride_row, v_stride_head; /* bytes */
+  const void* k_scales; const void* v_scales;
+  int64_t ks_stride_page, ks_stride_block, ks_stride_head; /* bytes */
+  int64_t vs_stride_page, vs_stride_block, vs_stride_head; /* bytes */
+  int64_t num_pages;
+  const int32_t* block_table; int64_t block_table_stride; int block_table_cols;
+  const int32_t* seq_lens;           /* (num_seqs,) */
+  const int32_t* q_start;            /* (num_seqs + 1,), ascending from 0 */
+  float* lse;                        /* optional (num_tokens, h_q) natural-log LSE */
+  float softmax_scale;
+  int causal;
+  int32_t* status;                   /* optional device status word (MJ_DEV_*) */
+} mj_block_attn_args;
+
+int mj_block_attention(const mj_block_attn_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -23,6 +23,7 @@ MJ_DEV_OK = 0
 MJ_DEV_BAD_PAGE = 1
 MJ_DEV_BAD_SPLIT = 2
 MJ_DEV_TIMEOUT = 3
+MJ_DEV_BAD_POSITION = 4
 
 MJ_KV_FP8_E4M3 = 0
 MJ_KV_E2M3 = 1
@@ -31,6 +32,9 @@ MJ_KV_E2M1 = 3
 MJ_KV_NVFP4 = 4
 KV_FORMATS = {"fp8": MJ_KV_FP8_E4M3, "e2m3": MJ_KV_E2M3, "e3m2": MJ_KV_E3M2, "e2m1": MJ_KV_E2M1,
               "nvfp4": MJ_KV_NVFP4}
+
+# block-scaled fp8 by tokens per scale block
+BLOCK_FORMATS = {16: 5, 32: 6, 64: 7, 128: 8}
 
 MJ_DT_BF16 = 0
 MJ_DT_FP16 = 1
@@ -48,7 +52,8 @@ MJ_SCALE_SEQ_HEAD = 3
 
 EXPORTED = ("mj_last_error", "mj_abi_version", "mj_row_bytes", "mj_cache_write", "mj_decode", "mj_combine",
             "mj_decode_noalloc", "mj_decode_kernel", "mj_expand_pages", "mj_plan_split_kv", "mj_create", "mj_plan",
-            "mj_runner_fill", "mj_runner_status", "mj_destroy", "mj_tc_fallbacks")
+            "mj_runner_fill", "mj_runner_status", "mj_destroy", "mj_tc_fallbacks", "mj_qk_norm_rope", "mj_block_write",
+            "mj_block_read", "mj_block_attention")
 
 _i64, _i32, _vp, _f32 = C.c_int64, C.c_int, C.c_void_p, C.c_float
 
@@ -124,6 +129,56 @@ class DecodeArgs(C.Structure):
     ]
 
 
+class QkNormRopeArgs(C.Structure):
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("q_out", _vp), ("k_out", _vp),
+        ("dtype", _i32), ("num_tokens", _i64), ("h_q", _i32), ("h_k", _i32),
+        ("head_size", _i32), ("rot_dim", _i32), ("interleaved", _i32),
+        ("q_stride_tok", _i64), ("q_stride_head", _i64), ("k_stride_tok", _i64), ("k_stride_head", _i64),
+        ("qo_stride_tok", _i64), ("qo_stride_head", _i64), ("ko_stride_tok", _i64), ("ko_stride_head", _i64),
+        ("positions", _vp), ("cos_sin", _vp), ("cos_sin_dtype", _i32), ("cos_sin_stride", _i64),
+        ("num_positions", _i64),
+        ("q_weight", _vp), ("k_weight", _vp), ("weight_dtype", _i32), ("eps", _f32),
+        ("status", _vp),
+    ]
+
+
+_BLOCK_CACHE_FIELDS = [
+    ("k_stride_page", _i64), ("k_stride_row", _i64), ("k_stride_head", _i64),
+    ("v_stride_page", _i64), ("v_stride_row", _i64), ("v_stride_head", _i64),
+    ("k_scales", _vp), ("v_scales", _vp),
+    ("ks_stride_page", _i64), ("ks_stride_block", _i64), ("ks_stride_head", _i64),
+    ("vs_stride_page", _i64), ("vs_stride_block", _i64), ("vs_stride_head", _i64),
+    ("num_pages", _i64),
+]
+
+
+class BlockReadArgs(C.Structure):
+    _fields_ = [
+        ("k_cache", _vp), ("v_cache", _vp), *_BLOCK_CACHE_FIELDS,
+        ("page_size", _i32), ("h_k", _i32), ("head_size", _i32), ("kv_format", _i32),
+        ("block_table", _vp), ("block_table_stride", _i64), ("block_table_cols", _i32),
+        ("starts", _vp), ("offsets", _vp), ("num_seqs", _i32), ("num_rows", _i64),
+        ("k_out", _vp), ("v_out", _vp), ("out_dtype", _i32),
+        ("ko_stride_tok", _i64), ("ko_stride_head", _i64), ("vo_stride_tok", _i64), ("vo_stride_head", _i64),
+        ("status", _vp),
+    ]
+
+
+class BlockAttnArgs(C.Structure):
+    _fields_ = [
+        ("num_seqs", _i32), ("h_q", _i32), ("h_k", _i32), ("head_size", _i32),
+        ("page_size", _i32), ("kv_format", _i32), ("dtype", _i32),
+        ("q", _vp), ("q_stride_tok", _i64), ("q_stride_head", _i64),
+        ("o", _vp), ("o_stride_tok", _i64), ("o_stride_head", _i64),
+        ("num_tokens", _i64),
+        ("k_cache", _vp), ("v_cache", _vp), *_BLOCK_CACHE_FIELDS,
+        ("block_table", _vp), ("block_table_stride", _i64), ("block_table_cols", _i32),
+        ("seq_lens", _vp), ("q_start", _vp), ("lse", _vp),
+        ("softmax_scale", _f32), ("causal", _i32), ("status", _vp),
+    ]
+
+
 class MjolnirError(RuntimeError):
     def __init__(self, code: int, msg: str):
         super().__init__(f"mjolnir_b200 status {code}: {msg}")
@@ -162,6 +217,10 @@ def load():
         lib.mj_tc_fallbacks.restype = C.c_int
         lib.mj_expand_pages.argtypes = [C.POINTER(ExpandArgs), _vp]
         lib.mj_expand_pages.restype = C.c_int
+        for fn, args in (("mj_qk_norm_rope", QkNormRopeArgs), ("mj_block_write", CacheWriteArgs),
+                         ("mj_block_read", BlockReadArgs), ("mj_block_attention", BlockAttnArgs)):
+            getattr(lib, fn).argtypes = [C.POINTER(args), _vp]
+            getattr(lib, fn).restype = C.c_int
         _pi = C.POINTER(C.c_int32)
         lib.mj_plan_split_kv.argtypes = [_pi, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                                          C.c_float, _pi, C.c_int, _pi, C.POINTER(C.c_int), C.POINTER(C.c_int)]
@@ -215,6 +274,22 @@ def decode_noalloc(args: DecodeArgs, stream: int) -> None:
 def expand_pages(args: ExpandArgs, stream: int) -> None:
     """e2m3 -> e4m3 expansion of cache pages into a fallback's scratch."""
     check(load().mj_expand_pages(C.byref(args), _vp(stream)))
+
+
+def qk_norm_rope(args: QkNormRopeArgs, stream: int) -> None:
+    check(load().mj_qk_norm_rope(C.byref(args), _vp(stream)))
+
+
+def block_write(args: CacheWriteArgs, stream: int) -> None:
+    check(load().mj_block_write(C.byref(args), _vp(stream)))
+
+
+def block_read(args: BlockReadArgs, stream: int) -> None:
+    check(load().mj_block_read(C.byref(args), _vp(stream)))
+
+
+def block_attention(args: BlockAttnArgs, stream: int) -> None:
+    check(load().mj_block_attention(C.byref(args), _vp(stream)))
 
 
 def plan_split_kv(seq_lens, h_k: int, n_q_tiles: int, sm_count: int, ctas_per_sm: int = 1, max_splits: int = 16,

@@ -1,0 +1,208 @@
+// The block-scaled cache: quantising write and read-back.
+//
+// A block is G consecutive tokens of a page for one KV head; its e4m3 codes
+// share the scale 2^(e - 127). Powers of two keep x / scale, and the codes'
+// move to a larger scale, exact in fp32 (only a code that becomes subnormal
+// rounds), so a block filled token by token holds what one write of all its
+// tokens would. e4m3 is a floating type: the shared exponent costs no
+// precision until a value is 2^14 below its block's largest.
+#include "block_cache.cuh"
+
+namespace mj {
+
+// The smallest e with amax <= 448 * 2^(e - 127), 448 = 1.75 * 2^8.
+__device__ __forceinline__ int block_exponent(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  const int e = (int)(u >> 23) - 8 + ((u & 0x7FFFFFu) > 0x600000u);
+  return min(max(e, MJ_BLOCK_E_MIN), MJ_BLOCK_E_MAX);
+}
+
+// One warp per (tile of tokens, KV head, side). A lane per token finds the
+// tokens that begin a block's run in slot_mapping; the warp then takes those
+// blocks in turn: the run's largest magnitude, the scale, the codes, and (only
+// where an open block's scale grew) the rows already there.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) block_write_kernel(mj_cache_write_args a, int lg, int tile) {
+  griddep_wait();
+  constexpr int CPR = D / 8;  // 8-element chunks of a row
+  __shared__ int members_all[4][128];
+  const int wid = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int* members = members_all[wid];  // run's tokens, as offsets from its first
+  const int64_t tiles = (a.num_tokens + tile - 1) / tile;
+  const int64_t w = blockIdx.x * (int64_t)4 + wid;
+  if (w >= tiles * a.h_k * 2) return;  // whole warps
+  const int side = (int)(w & 1);
+  const int h = (int)((w >> 1) % a.h_k);
+  const int64_t t0 = ((w >> 1) / a.h_k) * tile;
+  const int64_t* slots = a.slot_mapping;
+  const T* src = static_cast<const T*>(side ? a.value : a.key) + h * (side ? a.value_stride_head : a.key_stride_head);
+  const int64_t st = side ? a.value_stride_tok : a.key_stride_tok;
+  unsigned char* cache = static_cast<unsigned char*>(side ? a.v_cache : a.k_cache) + h * (side ? a.v_stride_head : a.k_stride_head);
+  const int64_t sp = side ? a.v_stride_page : a.k_stride_page, sr = side ? a.v_stride_row : a.k_stride_row;
+  unsigned char* scales = static_cast<unsigned char*>(side ? a.v_scales : a.k_scales) + h * (side ? a.vs_stride_head : a.ks_stride_head);
+  const int64_t ssp = side ? a.vs_stride_page : a.ks_stride_page, ssb = side ? a.vs_stride_row : a.ks_stride_row;
+  const int G = 1 << lg;
+
+  // lane i < tile: does token t0 + i begin its block's run?
+  bool first = false;
+  const int64_t t = t0 + lane;
+  if (lane < tile && t < a.num_tokens) {
+    const int64_t s = slots[t];
+    first = s >= 0;
+    if (first) {
+      int64_t u = t - 1;
+      while (u >= 0 && slots[u] < 0) --u;
+      first = u < 0 || (slots[u] >> lg) != (s >> lg);
+    }
+  }
+  for (uint32_t todo = __ballot_sync(0xffffffffu, first); todo; todo &= todo - 1) {
+    const int64_t tb = t0 + __ffs(todo) - 1;
+    const int64_t block = slots[tb] >> lg;
+    const int per_page = a.page_size >> lg;
+    const int64_t page = block / per_page;
+    const int sub = (int)(block % per_page);
+    if (page >= a.num_pages) {
+      if (lane == 0) flag(a.status, MJ_DEV_BAD_PAGE);
+      continue;
+    }
+    // the run: its tokens in order, and which rows of the block they fill
+    int count = 0;
+    uint32_t rows[4] = {0, 0, 0, 0};
+    for (int64_t u0 = tb; u0 < a.num_tokens; u0 += 32) {
+      const int64_t u = u0 + lane;
+      const int64_t s = u < a.num_tokens ? slots[u] : -1;
+      const bool same = s >= 0 && (s >> lg) == block;
+      const uint32_t stop = __ballot_sync(0xffffffffu, s >= 0 && !same);
+      const uint32_t before = stop ? (stop & -stop) - 1u : 0xffffffffu;  // lanes before the next block's token
+      const uint32_t in = __ballot_sync(0xffffffffu, same) & before;
+      const bool take = (in >> lane) & 1u;
+      const int at = count + __popc(in & ((1u << lane) - 1u));
+      if (take && at < G) members[at] = (int)(u - tb);
+      const int r = take ? (int)(s & (G - 1)) : 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) rows[k] |= __reduce_or_sync(0xffffffffu, take && (r >> 5) == k ? 1u << (r & 31) : 0u);
+      count += __popc(in);
+      if (stop || count >= G) break;
+    }
+    if (count > G) count = G;
+    __syncwarp();
+    float amax = 0.f;
+    for (int c = lane; c < count * CPR; c += 32) {
+      float v[8];
+      load8(src + (tb + members[c / CPR]) * st + (c % CPR) * 8, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float m = fabsf(v[i]);
+        amax = m <= 3.402823466e38f ? fmaxf(amax, m) : amax;  // finite values only
+      }
+    }
+    amax = warp_allmax(amax);
+    unsigned char* sb = scales + page * ssp + sub * ssb;
+    int e = block_exponent(amax);
+    const bool opened = rows[0] & 1u;
+    unsigned char* base = cache + page * sp + (int64_t)(sub << lg) * sr;
+    if (!opened) {
+      const int old = min(max((int)*sb, MJ_BLOCK_E_MIN), MJ_BLOCK_E_MAX);
+      __syncwarp();
+      if (e > old) {  // the rows already there follow
+        const float f = __uint_as_float((uint32_t)(127 + old - e) << 23);
+        for (int c = lane; c < G * CPR; c += 32) {
+          const int r = c / CPR;
+          if ((rows[r >> 5] >> (r & 31)) & 1u) continue;
+          uint2* q = reinterpret_cast<uint2*>(base + r * sr + (c % CPR) * 8);
+          const uint2 codes = *q;
+          *q = make_uint2(scale4(codes.x, f), scale4(codes.y, f));
+        }
+      } else {
+        e = old;
+      }
+    }
+    if (lane == 0) *sb = (unsigned char)e;
+    const float inv = __uint_as_float((uint32_t)(254 - e) << 23);  // 2^(127 - e)
+    for (int c = lane; c < count * CPR; c += 32) {
+      const int64_t u = tb + members[c / CPR];
+      float v[8];
+      load8(src + u * st + (c % CPR) * 8, v);
+      *reinterpret_cast<uint2*>(base + (slots[u] & (G - 1)) * sr + (c % CPR) * 8) = quantize8(v, inv);
+    }
+    __syncwarp();  // members is rewritten for the next block
+  }
+}
+
+template <typename T>
+static cudaError_t write_t(const mj_cache_write_args& a, int lg, cudaStream_t stream) {
+  const int tile = 16;
+  const int64_t warps = (a.num_tokens + tile - 1) / tile * a.h_k * 2;
+  const dim3 grid((unsigned)((warps + 3) / 4));
+  if (a.head_size == 256) return launch_kernel(block_write_kernel<T, 256>, grid, dim3(128), 0, stream, a, lg, tile);
+  return launch_kernel(block_write_kernel<T, 128>, grid, dim3(128), 0, stream, a, lg, tile);
+}
+
+cudaError_t launch_block_write(const mj_cache_write_args& a, cudaStream_t stream) {
+  const int lg = block_log2(a.kv_format);
+  if (a.src_dtype == MJ_DT_FP32) return write_t<float>(a, lg, stream);
+  if (a.src_dtype == MJ_DT_FP16) return write_t<__half>(a, lg, stream);
+  return write_t<__nv_bfloat16>(a, lg, stream);
+}
+
+// One warp per (output row, group of up to 8 KV heads): the row's sequence and
+// page are looked up once, then each pass moves 256 codes (K and V of a head at
+// head_size 128).
+template <typename T, int D>
+__global__ void __launch_bounds__(256) block_read_kernel(mj_block_read_args a, int lg) {
+  griddep_wait();
+  const int lane = threadIdx.x & 31;
+  const int groups = (a.h_k + 7) / 8;
+  const int64_t w = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5;
+  const int64_t row = w / groups;
+  if (row >= a.num_rows || row >= a.offsets[a.num_seqs]) return;
+  int lo = 0, hi = a.num_seqs - 1;  // the last sequence whose rows begin at or before this one
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.offsets[mid] <= row) lo = mid;
+    else hi = mid - 1;
+  }
+  const int64_t pos = row - a.offsets[lo] + a.starts[lo];
+  const int64_t col = pos / a.page_size;
+  const int r = (int)(pos % a.page_size);
+  int page = -1;
+  if (pos >= 0 && col < a.block_table_cols) page = a.block_table[lo * a.block_table_stride + col];
+  if (page < 0 || page >= a.num_pages) {
+    if (lane == 0) flag(a.status, MJ_DEV_BAD_PAGE);
+    return;
+  }
+  const int h0 = (int)(w % groups) * 8, h1 = min(h0 + 8, a.h_k);
+  constexpr int CPR = D / 8;
+  for (int c = lane; c < (h1 - h0) * 2 * CPR; c += 32) {
+    const int h = h0 + c / (2 * CPR), side = (c / CPR) & 1, at = (c % CPR) * 8;
+    const unsigned char* in = static_cast<const unsigned char*>(side ? a.v_cache : a.k_cache) +
+                              page * (side ? a.v_stride_page : a.k_stride_page) + r * (side ? a.v_stride_row : a.k_stride_row) +
+                              h * (side ? a.v_stride_head : a.k_stride_head) + at;
+    const unsigned char* sc = static_cast<const unsigned char*>(side ? a.v_scales : a.k_scales) +
+                              page * (side ? a.vs_stride_page : a.ks_stride_page) +
+                              (r >> lg) * (side ? a.vs_stride_block : a.ks_stride_block) +
+                              h * (side ? a.vs_stride_head : a.ks_stride_head);
+    T* out = static_cast<T*>(side ? a.v_out : a.k_out) + row * (side ? a.vo_stride_tok : a.ko_stride_tok) +
+             h * (side ? a.vo_stride_head : a.ko_stride_head) + at;
+    float v[8];
+    dequantize8(*reinterpret_cast<const uint2*>(in), block_scale(*sc), v);
+    store8(out, v);
+  }
+}
+
+template <typename T>
+static cudaError_t read_t(const mj_block_read_args& a, int lg, cudaStream_t stream) {
+  const int64_t warps = a.num_rows * ((a.h_k + 7) / 8);
+  const dim3 grid((unsigned)((warps + 7) / 8));
+  if (a.head_size == 256) return launch_kernel(block_read_kernel<T, 256>, grid, dim3(256), 0, stream, a, lg);
+  return launch_kernel(block_read_kernel<T, 128>, grid, dim3(256), 0, stream, a, lg);
+}
+
+cudaError_t launch_block_read(const mj_block_read_args& a, cudaStream_t stream) {
+  const int lg = block_log2(a.kv_format);
+  if (a.out_dtype == MJ_DT_FP32) return read_t<float>(a, lg, stream);
+  if (a.out_dtype == MJ_DT_FP16) return read_t<__half>(a, lg, stream);
+  return read_t<__nv_bfloat16>(a, lg, stream);
+}
+
+}  // namespace mj

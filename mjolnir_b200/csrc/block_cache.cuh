@@ -1,0 +1,84 @@
+// Device helpers of the block-scaled cache (e4m3 codes, scale 2^(e - 127)).
+#pragma once
+
+#include "common.cuh"
+#include "sm100.cuh"
+
+namespace mj {
+
+__host__ __device__ __forceinline__ bool is_block_format(int kv_format) {
+  return kv_format >= MJ_KV_FP8_B16 && kv_format <= MJ_KV_FP8_B128;
+}
+// log2 of the tokens of a block
+__host__ __device__ __forceinline__ int block_log2(int kv_format) { return kv_format - MJ_KV_FP8_B16 + 4; }
+
+// e as a reader takes it
+__device__ __forceinline__ int block_e(unsigned char b) {
+  return min(max((int)b, MJ_BLOCK_E_MIN), MJ_BLOCK_E_MAX);
+}
+__device__ __forceinline__ float block_scale(unsigned char b) { return __uint_as_float((uint32_t)block_e(b) << 23); }
+
+// 8 elements, 16-byte aligned for the 16-bit types and fp32
+__device__ __forceinline__ void load8(const float* p, float* v) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float* v) {
+  const uint4 raw = *reinterpret_cast<const uint4*>(p);
+  const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&raw);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __bfloat1622float2(e[i]);
+    v[2 * i] = f.x, v[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void load8(const __half* p, float* v) {
+  const uint4 raw = *reinterpret_cast<const uint4*>(p);
+  const __half2* e = reinterpret_cast<const __half2*>(&raw);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(e[i]);
+    v[2 * i] = f.x, v[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void store8(float* p, const float* v) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float* v) {
+  uint4 raw;
+  __nv_bfloat162* e = reinterpret_cast<__nv_bfloat162*>(&raw);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) e[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+  *reinterpret_cast<uint4*>(p) = raw;
+}
+__device__ __forceinline__ void store8(__half* p, const float* v) {
+  uint4 raw;
+  __half2* e = reinterpret_cast<__half2*>(&raw);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) e[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+  *reinterpret_cast<uint4*>(p) = raw;
+}
+
+// 8 values times f -> e4m3 codes: nearest even, saturating, NaN stays NaN
+__device__ __forceinline__ uint2 quantize8(const float* v, float f) {
+  uint16_t c[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c[i] = sm100::f2_to_e4m3x2(v[2 * i] * f, v[2 * i + 1] * f);
+  return make_uint2(c[0] | ((uint32_t)c[1] << 16), c[2] | ((uint32_t)c[3] << 16));
+}
+__device__ __forceinline__ void dequantize8(uint2 codes, float f, float* v) {
+  const uint16_t c[4] = {(uint16_t)codes.x, (uint16_t)(codes.x >> 16), (uint16_t)codes.y, (uint16_t)(codes.y >> 16)};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 p = sm100::e4m3x2_to_f2(c[i]);
+    v[2 * i] = p.x * f, v[2 * i + 1] = p.y * f;
+  }
+}
+// 4 codes times f, as codes
+__device__ __forceinline__ uint32_t scale4(uint32_t codes, float f) {
+  const float2 a = sm100::e4m3x2_to_f2((uint16_t)codes), b = sm100::e4m3x2_to_f2((uint16_t)(codes >> 16));
+  return sm100::f2_to_e4m3x2(a.x * f, a.y * f) | ((uint32_t)sm100::f2_to_e4m3x2(b.x * f, b.y * f) << 16);
+}
+
+}  // namespace mj

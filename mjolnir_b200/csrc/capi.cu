@@ -5,6 +5,7 @@
 #include <stdio.h>
 #include <stdlib.h>
 
+#include "block_cache.cuh"
 #include "common.cuh"
 
 namespace mj {
@@ -14,6 +15,10 @@ cudaError_t launch_combine(const mj_decode_args& a, cudaStream_t stream);
 cudaError_t launch_decode_tc(const mj_decode_args& a, cudaStream_t stream, bool* handled, bool dry);
 const char* tc_ineligible(const mj_decode_args& a);
 cudaError_t launch_expand_pages(const mj_expand_args& a, cudaStream_t stream);
+cudaError_t launch_qk_norm_rope(const mj_qk_norm_rope_args& a, bool vec, cudaStream_t stream);
+cudaError_t launch_block_write(const mj_cache_write_args& a, cudaStream_t stream);
+cudaError_t launch_block_read(const mj_block_read_args& a, cudaStream_t stream);
+cudaError_t launch_block_attention(const mj_block_attn_args& a, cudaStream_t stream);
 }  // namespace mj
 
 static thread_local char g_err[512] = "";
@@ -57,7 +62,7 @@ int mj_abi_version(void) { return MJ_ABI_VERSION; }
 
 int mj_row_bytes(int head_size, int kv_format) {
   if (head_size <= 0 || head_size % 16) return -1;
-  if (kv_format == MJ_KV_FP8_E4M3) return head_size;
+  if (kv_format == MJ_KV_FP8_E4M3 || mj::is_block_format(kv_format)) return head_size;
   if (kv_format == MJ_KV_E2M3 || kv_format == MJ_KV_E3M2) return head_size * 3 / 4;
   if (kv_format == MJ_KV_E2M1 || kv_format == MJ_KV_NVFP4) return head_size / 2;
   return -1;
@@ -84,7 +89,9 @@ int mj_cache_write(const mj_cache_write_args* args, void* stream) {
     return MJ_OK;
   }
   const int rb = mj_row_bytes(a.head_size, a.kv_format);
-  if (rb < 0) return fail(MJ_ERR_UNSUPPORTED, "mj_cache_write: head_size %d / kv_format %d", a.head_size, a.kv_format);
+  if (rb < 0 || mj::is_block_format(a.kv_format))
+    return fail(MJ_ERR_UNSUPPORTED, "mj_cache_write: head_size %d / kv_format %d%s", a.head_size, a.kv_format,
+                rb < 0 ? "" : " (block-scaled formats: mj_block_write)");
   if (a.src_dtype < MJ_DT_BF16 || a.src_dtype > MJ_DT_FP32) return fail(MJ_ERR_INVALID, "mj_cache_write: src_dtype %d", a.src_dtype);
   if (!a.key || !a.value || !a.k_cache || !a.v_cache || !a.slot_mapping || !a.k_scale || !a.v_scale)
     return fail(MJ_ERR_INVALID, "mj_cache_write: null pointer argument");
@@ -232,6 +239,136 @@ int mj_expand_pages(const mj_expand_args* args, void* stream) {
   if (a.num_out_pages * a.page_size * a.h_k > (int64_t)INT32_MAX)
     return fail(MJ_ERR_UNSUPPORTED, "mj_expand_pages: too many rows");
   return cuda_status(mj::launch_expand_pages(a, (cudaStream_t)stream), "mj_expand_pages launch");
+}
+
+// Shape, layout and scale tensors of a block-scaled cache (nullptr = valid):
+// st = the six cache strides, ss the six scale strides, in bytes.
+static const char* block_cache_problem(int head_size, int kv_format, int page_size, int h_k, int64_t num_pages,
+                                       const void* k, const void* v, const int64_t* st, const void* ks, const void* vs,
+                                       const int64_t* ss, uintptr_t align) {
+  if (!mj::is_block_format(kv_format)) return "kv_format is not block-scaled (MJ_KV_FP8_B16 .. _B128)";
+  if (head_size != 128 && head_size != 256) return "head_size must be 128 or 256";
+  if (page_size <= 0 || page_size % (1 << mj::block_log2(kv_format))) return "a block must divide the page";
+  if (page_size > (1 << 20)) return "page_size";
+  if (h_k <= 0 || num_pages <= 0 || num_pages > INT32_MAX) return "h_k / num_pages";
+  if (!k || !v || !ks || !vs) return "null cache or scale pointer";
+  for (int i = 0; i < 6; ++i)
+    if (st[i] < 0 || st[i] % (int64_t)align || ss[i] < 0) return "cache strides must be multiples of the row alignment";
+  if (!aligned(k, align) || !aligned(v, align)) return "cache rows must be aligned";
+  return nullptr;
+}
+
+int mj_qk_norm_rope(const mj_qk_norm_rope_args* args, void* stream) {
+  if (!args) return fail(MJ_ERR_INVALID, "mj_qk_norm_rope: null args");
+  const mj_qk_norm_rope_args& a = *args;
+  if (a.num_tokens < 0 || a.h_q < 0 || a.h_k < 0)
+    return fail(MJ_ERR_INVALID, "mj_qk_norm_rope: num_tokens %lld h_q %d h_k %d", (long long)a.num_tokens, a.h_q, a.h_k);
+  if (a.head_size <= 0 || a.head_size % 16 || a.head_size > 512)
+    return fail(MJ_ERR_UNSUPPORTED, "mj_qk_norm_rope: head_size %d (a multiple of 16, at most 512)", a.head_size);
+  if (a.rot_dim < 0 || a.rot_dim % 16 || a.rot_dim > a.head_size)
+    return fail(MJ_ERR_UNSUPPORTED, "mj_qk_norm_rope: rot_dim %d (a multiple of 16, at most head_size)", a.rot_dim);
+  for (int dt : {a.dtype, a.cos_sin_dtype, a.weight_dtype})
+    if (dt < MJ_DT_BF16 || dt > MJ_DT_FP32) return fail(MJ_ERR_INVALID, "mj_qk_norm_rope: dtype %d", dt);
+  if (a.num_tokens == 0 || a.h_q + a.h_k == 0) {
+    g_err[0] = 0;
+    return MJ_OK;
+  }
+  if ((a.h_q && (!a.q || !a.q_out)) || (a.h_k && (!a.k || !a.k_out)))
+    return fail(MJ_ERR_INVALID, "mj_qk_norm_rope: null q / k pointer");
+  if (a.rot_dim && (!a.positions || !a.cos_sin || a.num_positions <= 0))
+    return fail(MJ_ERR_INVALID, "mj_qk_norm_rope: rotation needs positions and the cos / sin table");
+  if (!(a.eps >= 0.f)) return fail(MJ_ERR_INVALID, "mj_qk_norm_rope: eps %g", (double)a.eps);
+  if (a.num_tokens * (a.h_q + a.h_k) > (int64_t)1 << 34) return fail(MJ_ERR_UNSUPPORTED, "mj_qk_norm_rope: too many rows");
+  // 16-byte accesses where every row allows them
+  const int64_t es = a.dtype == MJ_DT_FP32 ? 4 : 2;
+  bool vec = true;
+  if (a.h_q) {
+    vec = vec && aligned(a.q, 16) && aligned(a.q_out, 16);
+    for (int64_t s : {a.q_stride_tok, a.q_stride_head, a.qo_stride_tok, a.qo_stride_head}) vec = vec && (s * es) % 16 == 0;
+  }
+  if (a.h_k) {
+    vec = vec && aligned(a.k, 16) && aligned(a.k_out, 16);
+    for (int64_t s : {a.k_stride_tok, a.k_stride_head, a.ko_stride_tok, a.ko_stride_head}) vec = vec && (s * es) % 16 == 0;
+  }
+  return cuda_status(mj::launch_qk_norm_rope(a, vec, (cudaStream_t)stream), "mj_qk_norm_rope launch");
+}
+
+int mj_block_write(const mj_cache_write_args* args, void* stream) {
+  if (!args) return fail(MJ_ERR_INVALID, "mj_block_write: null args");
+  const mj_cache_write_args& a = *args;
+  if (a.num_tokens < 0) return fail(MJ_ERR_INVALID, "mj_block_write: num_tokens %lld", (long long)a.num_tokens);
+  const int64_t st[6] = {a.k_stride_page, a.k_stride_row, a.k_stride_head, a.v_stride_page, a.v_stride_row, a.v_stride_head};
+  const int64_t ss[6] = {a.ks_stride_page, a.ks_stride_row, a.ks_stride_head, a.vs_stride_page, a.vs_stride_row, a.vs_stride_head};
+  if (const char* why = block_cache_problem(a.head_size, a.kv_format, a.page_size, a.h_k, a.num_pages, a.k_cache, a.v_cache,
+                                            st, a.k_scales, a.v_scales, ss, 8))
+    return fail(MJ_ERR_UNSUPPORTED, "mj_block_write: %s (head_size %d, kv_format %d, page_size %d; 8-byte aligned rows)", why,
+                a.head_size, a.kv_format, a.page_size);
+  if (a.src_dtype < MJ_DT_BF16 || a.src_dtype > MJ_DT_FP32) return fail(MJ_ERR_INVALID, "mj_block_write: src_dtype %d", a.src_dtype);
+  if (a.num_tokens == 0) {
+    g_err[0] = 0;
+    return MJ_OK;
+  }
+  if (!a.key || !a.value || !a.slot_mapping) return fail(MJ_ERR_INVALID, "mj_block_write: null pointer argument");
+  const int64_t es = a.src_dtype == MJ_DT_FP32 ? 4 : 2;
+  bool ok = aligned(a.key, 16) && aligned(a.value, 16);
+  for (int64_t s : {a.key_stride_tok, a.key_stride_head, a.value_stride_tok, a.value_stride_head}) ok = ok && (s * es) % 16 == 0;
+  if (!ok) return fail(MJ_ERR_UNSUPPORTED, "mj_block_write: key / value rows must be 16-byte aligned");
+  if (a.num_tokens > INT32_MAX || a.num_tokens * a.h_k > (int64_t)1 << 33) return fail(MJ_ERR_UNSUPPORTED, "mj_block_write: too many rows");
+  return cuda_status(mj::launch_block_write(a, (cudaStream_t)stream), "mj_block_write launch");
+}
+
+int mj_block_read(const mj_block_read_args* args, void* stream) {
+  if (!args) return fail(MJ_ERR_INVALID, "mj_block_read: null args");
+  const mj_block_read_args& a = *args;
+  if (a.num_seqs < 0 || a.num_rows < 0) return fail(MJ_ERR_INVALID, "mj_block_read: num_seqs %d num_rows %lld", a.num_seqs, (long long)a.num_rows);
+  const int64_t st[6] = {a.k_stride_page, a.k_stride_row, a.k_stride_head, a.v_stride_page, a.v_stride_row, a.v_stride_head};
+  const int64_t ss[6] = {a.ks_stride_page, a.ks_stride_block, a.ks_stride_head, a.vs_stride_page, a.vs_stride_block, a.vs_stride_head};
+  if (const char* why = block_cache_problem(a.head_size, a.kv_format, a.page_size, a.h_k, a.num_pages, a.k_cache, a.v_cache,
+                                            st, a.k_scales, a.v_scales, ss, 8))
+    return fail(MJ_ERR_UNSUPPORTED, "mj_block_read: %s (head_size %d, kv_format %d, page_size %d; 8-byte aligned rows)", why,
+                a.head_size, a.kv_format, a.page_size);
+  if (a.out_dtype < MJ_DT_BF16 || a.out_dtype > MJ_DT_FP32) return fail(MJ_ERR_INVALID, "mj_block_read: out_dtype %d", a.out_dtype);
+  if (a.num_seqs == 0 || a.num_rows == 0) {
+    g_err[0] = 0;
+    return MJ_OK;
+  }
+  if (!a.block_table || a.block_table_cols <= 0 || !a.starts || !a.offsets || !a.k_out || !a.v_out)
+    return fail(MJ_ERR_INVALID, "mj_block_read: null pointer argument");
+  const int64_t es = a.out_dtype == MJ_DT_FP32 ? 4 : 2;
+  bool ok = aligned(a.k_out, 16) && aligned(a.v_out, 16);
+  for (int64_t s : {a.ko_stride_tok, a.ko_stride_head, a.vo_stride_tok, a.vo_stride_head}) ok = ok && (s * es) % 16 == 0;
+  if (!ok) return fail(MJ_ERR_UNSUPPORTED, "mj_block_read: output rows must be 16-byte aligned");
+  if (a.num_rows > INT32_MAX) return fail(MJ_ERR_UNSUPPORTED, "mj_block_read: too many rows");
+  return cuda_status(mj::launch_block_read(a, (cudaStream_t)stream), "mj_block_read launch");
+}
+
+int mj_block_attention(const mj_block_attn_args* args, void* stream) {
+  if (!args) return fail(MJ_ERR_INVALID, "mj_block_attention: null args");
+  const mj_block_attn_args& a = *args;
+  if (a.num_seqs < 0 || a.num_tokens < 0 || a.h_k <= 0 || a.h_q <= 0 || a.h_q % a.h_k)
+    return fail(MJ_ERR_INVALID, "mj_block_attention: num_seqs %d num_tokens %lld h_q %d h_k %d", a.num_seqs,
+                (long long)a.num_tokens, a.h_q, a.h_k);
+  const int64_t st[6] = {a.k_stride_page, a.k_stride_row, a.k_stride_head, a.v_stride_page, a.v_stride_row, a.v_stride_head};
+  const int64_t ss[6] = {a.ks_stride_page, a.ks_stride_block, a.ks_stride_head, a.vs_stride_page, a.vs_stride_block, a.vs_stride_head};
+  if (const char* why = block_cache_problem(a.head_size, a.kv_format, a.page_size, a.h_k, a.num_pages, a.k_cache, a.v_cache,
+                                            st, a.k_scales, a.v_scales, ss, 16))
+    return fail(MJ_ERR_UNSUPPORTED, "mj_block_attention: %s (head_size %d, kv_format %d, page_size %d; 16-byte aligned rows)",
+                why, a.head_size, a.kv_format, a.page_size);
+  if (a.page_size != 16 && a.page_size != 32 && a.page_size != 64 && a.page_size != 128)
+    return fail(MJ_ERR_UNSUPPORTED, "mj_block_attention: page_size %d (16, 32, 64 or 128)", a.page_size);
+  if (a.dtype != MJ_DT_BF16 && a.dtype != MJ_DT_FP16)
+    return fail(MJ_ERR_UNSUPPORTED, "mj_block_attention: dtype %d (bf16 or fp16)", a.dtype);
+  if (a.num_seqs == 0 || a.num_tokens == 0) {
+    g_err[0] = 0;
+    return MJ_OK;
+  }
+  if (!a.q || !a.o || !a.block_table || a.block_table_cols <= 0 || !a.seq_lens || !a.q_start)
+    return fail(MJ_ERR_INVALID, "mj_block_attention: null pointer argument");
+  bool ok = aligned(a.q, 16) && aligned(a.o, 16);
+  for (int64_t s : {a.q_stride_tok, a.q_stride_head, a.o_stride_tok, a.o_stride_head}) ok = ok && s % 8 == 0;
+  if (!ok) return fail(MJ_ERR_UNSUPPORTED, "mj_block_attention: q / o rows must be 16-byte aligned");
+  if (a.num_tokens * a.h_q > (int64_t)INT32_MAX) return fail(MJ_ERR_UNSUPPORTED, "mj_block_attention: too many rows");
+  return cuda_status(mj::launch_block_attention(a, (cudaStream_t)stream), "mj_block_attention launch");
 }
 
 }  // extern "C"
