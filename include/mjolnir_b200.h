@@ -451,10 +451,36 @@ typedef struct mj_block_attn_args {
   float* lse;                        /* optional (num_tokens, h_q) natural-log LSE */
   float softmax_scale;
   int causal;
+  /* The plan (mj_block_plan writes it on the host): num_work items of 8 int32
+   * (seq, first row, tile begin, tile end, partial slot or -1, 0, 0, 0). A
+   * row is (query token, head of the KV head's group), token-major; an item
+   * covers MJ_BLOCK_ROWS(head_size) rows from its first and the keys of its
+   * tiles of MJ_BLOCK_KEYS(head_size). Items with a slot leave normalised
+   * partials in o_part / lse_part at [slot][KV head][row]; num_merges entries
+   * of 4 int32 (seq, first row, first slot, slots) say which to join. */
+  const int32_t* work; int num_work;
+  const int32_t* merges; int num_merges;
+  float* o_part;                     /* (num_slots, h_k, rows, head_size) fp32 */
+  float* lse_part;                   /* (num_slots, h_k, rows) fp32 */
+  int num_slots;
   int32_t* status;                   /* optional device status word (MJ_DEV_*) */
 } mj_block_attn_args;
 
+#define MJ_BLOCK_ROWS(head_size) ((head_size) == 256 ? 128 : 256)
+#define MJ_BLOCK_KEYS(head_size) ((head_size) == 256 ? 64 : 128)
+
 int mj_block_attention(const mj_block_attn_args* args, void* stream);
+
+/* Host plan of a step: every sequence with query_lens[s] > 0 is cut into items
+ * of MJ_BLOCK_ROWS rows; an item longer than an equal share of the step's key
+ * tiles per SM is split along its keys, so that few rows over a long context
+ * still fill the GPU. Items come longest first. work_out: work_capacity x 8
+ * int32, merges_out: merges_capacity x 4, at most max_slots partial slots (0 =
+ * never split). MJ_ERR_UNSUPPORTED when a capacity is too small. Pure host
+ * code, no CUDA call. */
+int mj_block_plan(const int32_t* query_lens, const int32_t* seq_lens, int num_seqs, int h_q, int h_k, int head_size,
+                  int causal, int sm_count, int max_slots, int32_t* work_out, int work_capacity, int32_t* merges_out,
+                  int merges_capacity, int* num_work, int* num_merges, int* num_slots);
 
 #ifdef __cplusplus
 }

@@ -53,7 +53,7 @@ MJ_SCALE_SEQ_HEAD = 3
 EXPORTED = ("mj_last_error", "mj_abi_version", "mj_row_bytes", "mj_cache_write", "mj_decode", "mj_combine",
             "mj_decode_noalloc", "mj_decode_kernel", "mj_expand_pages", "mj_plan_split_kv", "mj_create", "mj_plan",
             "mj_runner_fill", "mj_runner_status", "mj_destroy", "mj_tc_fallbacks", "mj_qk_norm_rope", "mj_block_write",
-            "mj_block_read", "mj_block_attention")
+            "mj_block_read", "mj_block_attention", "mj_block_plan")
 
 _i64, _i32, _vp, _f32 = C.c_int64, C.c_int, C.c_void_p, C.c_float
 
@@ -175,7 +175,9 @@ class BlockAttnArgs(C.Structure):
         ("k_cache", _vp), ("v_cache", _vp), *_BLOCK_CACHE_FIELDS,
         ("block_table", _vp), ("block_table_stride", _i64), ("block_table_cols", _i32),
         ("seq_lens", _vp), ("q_start", _vp), ("lse", _vp),
-        ("softmax_scale", _f32), ("causal", _i32), ("status", _vp),
+        ("softmax_scale", _f32), ("causal", _i32),
+        ("work", _vp), ("num_work", _i32), ("merges", _vp), ("num_merges", _i32),
+        ("o_part", _vp), ("lse_part", _vp), ("num_slots", _i32), ("status", _vp),
     ]
 
 
@@ -225,6 +227,8 @@ def load():
         lib.mj_plan_split_kv.argtypes = [_pi, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                                          C.c_float, _pi, C.c_int, _pi, C.POINTER(C.c_int), C.POINTER(C.c_int)]
         lib.mj_plan_split_kv.restype = C.c_int
+        lib.mj_block_plan.argtypes = [_pi, _pi, *[C.c_int] * 7, _pi, C.c_int, _pi, C.c_int, *[C.POINTER(C.c_int)] * 3]
+        lib.mj_block_plan.restype = C.c_int
         lib.mj_create.argtypes = [C.c_int] * 10
         lib.mj_create.restype = _vp
         lib.mj_plan.argtypes = [_vp, _pi, C.c_int, C.c_int, C.c_int, C.c_int, _vp]
@@ -290,6 +294,21 @@ def block_read(args: BlockReadArgs, stream: int) -> None:
 
 def block_attention(args: BlockAttnArgs, stream: int) -> None:
     check(load().mj_block_attention(C.byref(args), _vp(stream)))
+
+
+def block_plan(query_lens, seq_lens, h_q: int, h_k: int, head_size: int, causal: bool, sm_count: int, max_slots: int,
+               work, merges) -> tuple[int, int, int]:
+    """mj_block_plan into the int32 arrays ``work`` (n, 8) and ``merges`` (m,
+    4): (work items, merges, partial slots)."""
+    import numpy as np
+
+    q, kv = np.ascontiguousarray(query_lens, dtype=np.int32), np.ascontiguousarray(seq_lens, dtype=np.int32)
+    _pi = C.POINTER(C.c_int32)
+    n = [C.c_int(0) for _ in range(3)]
+    check(load().mj_block_plan(q.ctypes.data_as(_pi), kv.ctypes.data_as(_pi), len(q), h_q, h_k, head_size, int(causal),
+                               sm_count, max_slots, work.ctypes.data_as(_pi), len(work), merges.ctypes.data_as(_pi),
+                               len(merges), *[C.byref(x) for x in n]))
+    return n[0].value, n[1].value, n[2].value
 
 
 def plan_split_kv(seq_lens, h_k: int, n_q_tiles: int, sm_count: int, ctas_per_sm: int = 1, max_splits: int = 16,

@@ -368,6 +368,10 @@ int mj_block_attention(const mj_block_attn_args* args, void* stream) {
   for (int64_t s : {a.q_stride_tok, a.q_stride_head, a.o_stride_tok, a.o_stride_head}) ok = ok && s % 8 == 0;
   if (!ok) return fail(MJ_ERR_UNSUPPORTED, "mj_block_attention: q / o rows must be 16-byte aligned");
   if (a.num_tokens * a.h_q > (int64_t)INT32_MAX) return fail(MJ_ERR_UNSUPPORTED, "mj_block_attention: too many rows");
+  if (a.num_work < 0 || a.num_merges < 0 || a.num_slots < 0 || (a.num_work && (!a.work || !aligned(a.work, 16))) ||
+      (a.num_merges && (!a.merges || !aligned(a.merges, 16))) || (a.num_slots && (!a.o_part || !a.lse_part || !aligned(a.o_part, 16))))
+    return fail(MJ_ERR_INVALID, "mj_block_attention: plan or partial buffers");
+  if ((int64_t)a.num_work * a.h_k > (int64_t)INT32_MAX) return fail(MJ_ERR_UNSUPPORTED, "mj_block_attention: too many work items");
   return cuda_status(mj::launch_block_attention(a, (cudaStream_t)stream), "mj_block_attention launch");
 }
 

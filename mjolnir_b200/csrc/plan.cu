@@ -20,6 +20,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <exception>
 #include <set>
 #include <vector>
 
@@ -139,6 +140,67 @@ int mj_plan_split_kv(const int32_t* seq_lens, int num_seqs, int h_k, int n_q_til
   }
   *num_work_out = total;
   if (chunk_tiles_out) *chunk_tiles_out = chunk;
+  return MJ_OK;
+}
+
+// ---- block attention -------------------------------------------------------
+
+// Splitting: an equal share of the step's key tiles per SM bounds an item, but
+// a piece keeps at least kMinPiece tiles (its prologue and epilogue cost about
+// as much as two). Where the pieces would need more than max_slots partials,
+// the bound doubles until they do not.
+int mj_block_plan(const int32_t* query_lens, const int32_t* seq_lens, int num_seqs, int h_q, int h_k, int head_size,
+                  int causal, int sm_count, int max_slots, int32_t* work_out, int work_capacity, int32_t* merges_out,
+                  int merges_capacity, int* num_work, int* num_merges, int* num_slots) {
+  if (num_seqs < 0 || h_k <= 0 || h_q <= 0 || h_q % h_k || (head_size != 128 && head_size != 256) || sm_count <= 0 ||
+      max_slots < 0 || (num_seqs && (!query_lens || !seq_lens)) || !num_work || !num_merges || !num_slots)
+    return mj::set_last_error(MJ_ERR_INVALID, "mj_block_plan: invalid argument");
+  constexpr int kMinPiece = 4;
+  const int h_r = h_q / h_k, rows = MJ_BLOCK_ROWS(head_size), keys = MJ_BLOCK_KEYS(head_size);
+  struct Block {
+    int32_t seq, row0, tiles;
+  };
+  try {
+    std::vector<Block> blocks;
+    int64_t total = 0;
+    for (int s = 0; s < num_seqs; ++s) {
+      const int64_t n = query_lens[s], L = seq_lens[s], all = n * h_r;
+      if (n < 0 || L < 0 || all > INT32_MAX) return mj::set_last_error(MJ_ERR_INVALID, "mj_block_plan: a length");
+      for (int64_t r = 0; r < all; r += rows) {
+        const int64_t last = causal ? L - n + (std::min(r + rows, all) - 1) / h_r : L - 1;  // last key seen
+        blocks.push_back({s, (int32_t)r, last < 0 ? 0 : (int32_t)(last / keys + 1)});
+        total += blocks.back().tiles;
+      }
+    }
+    std::stable_sort(blocks.begin(), blocks.end(), [](const Block& x, const Block& y) { return x.tiles > y.tiles; });
+    int64_t bound = std::max<int64_t>(kMinPiece, ceil_div(total * h_k, sm_count));
+    auto pieces = [&](const Block& b) { return b.tiles > bound ? ceil_div(b.tiles, bound) : 1; };
+    for (;; bound *= 2) {
+      int64_t slots = 0;
+      for (const Block& b : blocks) slots += pieces(b) > 1 ? pieces(b) : 0;
+      if (slots <= max_slots) break;
+    }
+    int64_t nw = 0, nm = 0, ns = 0;
+    for (const Block& b : blocks) {
+      const int k = pieces(b);
+      if (nw + k > work_capacity || (k > 1 && nm >= merges_capacity) || !work_out || (k > 1 && !merges_out))
+        return mj::set_last_error(MJ_ERR_UNSUPPORTED, "mj_block_plan: more items than the capacity");
+      if (k > 1) {
+        const int32_t m[4] = {b.seq, b.row0, (int32_t)ns, k};
+        std::copy(m, m + 4, merges_out + 4 * nm++);
+      }
+      for (int i = 0; i < k; ++i) {  // pieces of equal length, to a tile
+        const int32_t w[8] = {b.seq, b.row0, (int32_t)((int64_t)b.tiles * i / k), (int32_t)((int64_t)b.tiles * (i + 1) / k),
+                              k > 1 ? (int32_t)ns++ : -1, 0, 0, 0};
+        std::copy(w, w + 8, work_out + 8 * nw++);
+      }
+    }
+    *num_work = (int)nw;
+    *num_merges = (int)nm;
+    *num_slots = (int)ns;
+  } catch (const std::exception&) {
+    return mj::set_last_error(MJ_ERR_INVALID, "mj_block_plan: out of memory");
+  }
   return MJ_OK;
 }
 

@@ -19,6 +19,7 @@ from __future__ import annotations
 
 from dataclasses import dataclass
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -184,6 +185,9 @@ class BlockPlan:
     block_table: torch.Tensor
     seq_lens: torch.Tensor
     q_start: torch.Tensor  # (num_seqs + 1,) int32, device
+    work: torch.Tensor  # (items, 8) int32, device
+    merges: torch.Tensor  # (merges, 4) int32, device
+    num_slots: int
     causal: bool = True
 
 
@@ -203,7 +207,16 @@ class BlockAttention:
         self.max_num_seqs, self.max_num_tokens = max_num_seqs, max_num_tokens
         self.device = torch.device(device)
         _lib.load()  # fail at construction, not at the first step
-        self.q_start = torch.zeros(max_num_seqs + 1, dtype=torch.int32, device=self.device)
+        self.sm_count = torch.cuda.get_device_properties(self.device).multi_processor_count
+        # rows of a work item, and the partial slots that splitting for every SM can ask for
+        self.rows = 128 if head_size == 256 else 256
+        self.max_slots = 2 * -(-self.sm_count // num_kv_heads)
+        self.max_work = max_num_tokens * (num_heads // num_kv_heads) // self.rows + max_num_seqs + self.max_slots
+        # the plan: q_start | merges | work, one fixed-address buffer and one copy a step
+        self._at = (-(-(max_num_seqs + 1) // 4) * 4, -(-(max_num_seqs + 1) // 4) * 4 + 4 * self.max_slots)
+        self.plan_buf = torch.zeros(self._at[1] + 8 * self.max_work, dtype=torch.int32, device=self.device)
+        self.o_part = torch.empty(self.max_slots * num_kv_heads * self.rows * head_size, dtype=torch.float32, device=self.device)
+        self.lse_part = torch.empty(self.max_slots * num_kv_heads * self.rows, dtype=torch.float32, device=self.device)
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
 
     def plan(self, query_lens, seq_lens_cpu, block_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -214,16 +227,24 @@ class BlockAttention:
         q = [int(x) for x in query_lens]
         if len(q) > self.max_num_seqs or sum(q) > self.max_num_tokens:
             raise ValueError(f"{len(q)} sequences / {sum(q)} tokens beyond the runner's capacity")
-        if len(q) != len(list(seq_lens_cpu)) or any(x < 0 for x in q):
+        kv = [int(x) for x in seq_lens_cpu]
+        if len(q) != len(kv) or min(q, default=0) < 0 or min(kv, default=0) < 0:
             raise ValueError("query_lens and seq_lens_cpu must pair up, without negative lengths")
         _table(block_table, len(q))
         if seq_lens.dtype != torch.int32 or seq_lens.dim() != 1 or seq_lens.shape[0] < len(q) or not seq_lens.is_contiguous():
             raise ValueError("seq_lens must be a contiguous int32 tensor of every sequence")
-        _on(self.q_start.device, block_table, seq_lens)
-        start = torch.zeros(len(q) + 1, dtype=torch.int32)
-        torch.cumsum(torch.tensor(q, dtype=torch.int32), 0, out=start[1:]) if q else None
-        self.q_start[: len(q) + 1].copy_(start.pin_memory() if self.device.type == "cuda" else start, non_blocking=True)
-        return BlockPlan(q, sum(q), block_table, seq_lens, self.q_start[: len(q) + 1], causal)
+        _on(self.status.device, block_table, seq_lens)
+        n, (m0, w0) = len(q), self._at
+        stage = torch.empty(self.plan_buf.shape[0], dtype=torch.int32, pin_memory=True)
+        host = stage.numpy()
+        host[0] = 0
+        np.cumsum(q, out=host[1:n + 1])
+        work, merges = host[w0:].reshape(-1, 8), host[m0:w0].reshape(-1, 4)
+        nw, nm, slots = _lib.block_plan(q, kv, self.h_q, self.h_k, self.d, causal, self.sm_count, self.max_slots, work, merges)
+        used = w0 + 8 * nw
+        self.plan_buf[:used].copy_(stage[:used], non_blocking=True)
+        return BlockPlan(q, sum(q), block_table, seq_lens, self.plan_buf[:n + 1], self.plan_buf[w0:used].view(-1, 8),
+                         self.plan_buf[m0:m0 + 4 * nm].view(-1, 4), slots, causal)
 
     def run(
         self,
@@ -250,7 +271,7 @@ class BlockAttention:
         if lse is not None and (lse.dtype != torch.float32 or lse.shape[0] < plan.num_tokens or lse.shape[1:] != (self.h_q,)
                                 or not lse.is_contiguous()):
             raise ValueError("lse must be a contiguous fp32 (tokens, h_q)")
-        _on(self.q_start.device, query, out, k_cache, lse)
+        _on(self.status.device, query, out, k_cache, lse)
         a.num_seqs, a.h_q, a.num_tokens, a.dtype = len(plan.query_lens), self.h_q, plan.num_tokens, dtype_code(query.dtype)
         a.q, a.q_stride_tok, a.q_stride_head = query.data_ptr(), query.stride(0), query.stride(1)
         a.o, a.o_stride_tok, a.o_stride_head = out.data_ptr(), out.stride(0), out.stride(1)
@@ -258,8 +279,10 @@ class BlockAttention:
         a.block_table, a.block_table_stride, a.block_table_cols = bt.data_ptr(), bt.stride(0), bt.shape[1]
         a.seq_lens, a.q_start, a.lse = plan.seq_lens.data_ptr(), plan.q_start.data_ptr(), _ptr(lse)
         a.softmax_scale, a.causal, a.status = float(softmax_scale), int(plan.causal), self.status.data_ptr()
-        with torch.cuda.device(self.q_start.device):
-            _lib.block_attention(a, _stream(self.q_start.device))
+        a.work, a.num_work, a.merges, a.num_merges = plan.work.data_ptr(), len(plan.work), plan.merges.data_ptr(), len(plan.merges)
+        a.o_part, a.lse_part, a.num_slots = self.o_part.data_ptr(), self.lse_part.data_ptr(), plan.num_slots
+        with torch.cuda.device(self.status.device):
+            _lib.block_attention(a, _stream(self.status.device))
         return out
 
     def check_status(self) -> None:
