@@ -35,6 +35,7 @@ KV_FORMATS = {"fp8": MJ_KV_FP8_E4M3, "e2m3": MJ_KV_E2M3, "e3m2": MJ_KV_E3M2, "e2
 
 # block-scaled fp8 by tokens per scale block
 BLOCK_FORMATS = {16: 5, 32: 6, 64: 7, 128: 8}
+KV_FORMATS |= {f"fp8b{g}": code for g, code in BLOCK_FORMATS.items()}
 
 MJ_DT_BF16 = 0
 MJ_DT_FP16 = 1

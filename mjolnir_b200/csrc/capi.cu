@@ -116,8 +116,11 @@ static int validate_decode(const mj_decode_args& a, const char* who) {
     return fail(MJ_ERR_INVALID, "%s: num_seqs %d q_len %d h_q %d h_k %d", who, a.num_seqs, a.q_len, a.h_q, a.h_k);
   if (a.head_size != 128 && a.head_size != 256)
     return fail(MJ_ERR_UNSUPPORTED, "%s: head_size %d (128 or 256)", who, a.head_size);
-  if (a.kv_format < MJ_KV_FP8_E4M3 || a.kv_format > MJ_KV_NVFP4)
+  if (a.kv_format < MJ_KV_FP8_E4M3 || a.kv_format > MJ_KV_FP8_B128)
     return fail(MJ_ERR_INVALID, "%s: kv_format %d", who, a.kv_format);
+  if (mj::is_block_format(a.kv_format) && (!a.k_scales || !a.v_scales || a.kernel == MJ_KERNEL_SIMT || mj::tc_ineligible(a)))
+    return fail(MJ_ERR_UNSUPPORTED, "%s: block-scaled formats need k_scales and v_scales and run the tensor-core kernel only (%s)",
+                who, a.kernel == MJ_KERNEL_SIMT ? "kernel" : mj::tc_ineligible(a) ? mj::tc_ineligible(a) : "scales");
   if (a.kv_format == MJ_KV_NVFP4) {
     const int64_t st[6] = {a.ks_stride_page, a.ks_stride_row, a.ks_stride_head, a.vs_stride_page, a.vs_stride_row, a.vs_stride_head};
     if (const char* why = nvfp4_scales_problem(a.k_scales, a.v_scales, st, false))
@@ -176,6 +179,8 @@ int mj_decode(const mj_decode_args* args, void* stream) {
     e = mj::launch_decode_tc(a, s, &handled, false);
     if (e != cudaSuccess) return cuda_status(e, "mj_decode launch (tensor-core kernel)");
   }
+  if (!handled && mj::is_block_format(a.kv_format))
+    return fail(MJ_ERR_UNSUPPORTED, "mj_decode: no tensor-core variant fits this build for the block-scaled formats");
   if (!handled) {
     e = mj::launch_decode_simt(a, s);
     if (e != cudaSuccess) return cuda_status(e, "mj_decode launch");

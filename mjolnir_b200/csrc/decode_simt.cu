@@ -2,6 +2,7 @@
 // per KV format, inst_<format>.cu) and the LSE combine kernel.
 #include <math.h>
 
+#include "block_cache.cuh"
 #include "common.cuh"
 
 namespace mj {
@@ -36,11 +37,18 @@ __global__ void __launch_bounds__(128) combine_kernel(const mj_decode_args a) {
   float m = -INFINITY;
   for (int s = lane; s < ns; s += 32) m = fmaxf(m, a.lse_part[s * stride_split + row]);
   m = warp_allmax(m);
+  // block-scaled formats: a NaN partial makes its row NaN (the max ignores it)
+  const bool block = is_block_format(a.kv_format);
+  if (block) {
+    bool nan = false;
+    for (int s = lane; s < ns; s += 32) nan |= isnan(a.lse_part[s * stride_split + row]);
+    if (__any_sync(0xffffffffu, nan)) m = __int_as_float(0x7FFFFFFF);
+  }
   float den = 0.f;
   if (m != -INFINITY)
     for (int s = lane; s < ns; s += 32) den += expf(a.lse_part[s * stride_split + row] - m);
   den = warp_allsum(den);
-  const float inv = den > 0.f ? 1.f / den : 0.f;
+  const float inv = (block ? den != 0.f : den > 0.f) ? 1.f / den : 0.f;
   const int qi = r / h_r, rr = r % h_r;
   const int64_t tok = (int64_t)seq * q_len + qi;
   const int qh = h * h_r + rr;
@@ -70,7 +78,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const mj_decode_args a) {
       store_elem(a.o, tok * a.o_stride_tok + qh * a.o_stride_head + c + k, a.o_dtype, v);
     }
   }
-  if (lane == 0 && a.lse) a.lse[tok * a.h_q + qh] = (m != -INFINITY && den > 0.f) ? m + logf(den) : -INFINITY;
+  if (lane == 0 && a.lse) a.lse[tok * a.h_q + qh] = (m != -INFINITY && (block ? den != 0.f : den > 0.f)) ? m + logf(den) : -INFINITY;
 }
 
 cudaError_t launch_decode_simt(const mj_decode_args& a, cudaStream_t stream) {

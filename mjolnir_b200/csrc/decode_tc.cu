@@ -9,6 +9,7 @@
 #include <atomic>
 #include <mutex>
 
+#include "block_cache.cuh"
 #include "common.cuh"
 
 namespace mj {
@@ -54,10 +55,14 @@ const char* tc_ineligible(const mj_decode_args& a) {
     for (int i = 0; i < 6; ++i)
       if (ss[i] % 8) return "nvfp4 scale stride alignment";
   }
+  if (is_block_format(a.kv_format)) {
+    if (!a.k_scales || !a.v_scales) return "block scales";
+    if (a.page_size % (1 << block_log2(a.kv_format))) return "a block must divide the page";
+  }
   if (a.head_size != 128 && a.head_size != 256) return "head_size not 128 or 256";
   if (a.page_size != 16 && a.page_size != 32 && a.page_size != 64 && a.page_size != 128) return "page size";
   if (a.num_pages >= (int64_t)INT32_MAX) return "num_pages";
-  const uintptr_t al = a.kv_format == MJ_KV_FP8_E4M3 ? 16 : 32;
+  const uintptr_t al = a.kv_format == MJ_KV_FP8_E4M3 || is_block_format(a.kv_format) ? 16 : 32;
   if ((uintptr_t)a.k_cache % al || (uintptr_t)a.v_cache % al) return "KV view alignment";
   const int64_t st[6] = {a.k_stride_page, a.k_stride_row, a.k_stride_head, a.v_stride_page, a.v_stride_row, a.v_stride_head};
   for (int i = 0; i < 6; ++i)
@@ -80,7 +85,7 @@ static CUtensorMapDataType tma_type(int kv_format) {
 // (codes, half, rows, h_k, pages), one box per half.
 static bool make_map(CUtensorMap* m, const void* base, int64_t s_page, int64_t s_row, int64_t s_head,
                      const mj_decode_args& a) {
-  const bool narrow = a.kv_format != MJ_KV_FP8_E4M3;
+  const bool narrow = a.kv_format != MJ_KV_FP8_E4M3 && !is_block_format(a.kv_format);
   // a dimension of extent 1 never moves its coordinate; give it any legal stride
   const int64_t fill = narrow ? 32 : 16;
   const cuuint64_t sr = (cuuint64_t)(s_row ? s_row : fill), sh = (cuuint64_t)(s_head ? s_head : fill),
@@ -153,6 +158,10 @@ static cudaError_t dispatch_nq(const mj_decode_args& a, int n_q, bool fused, con
     case MJ_KV_E3M2: return launch_tc_fmt<MJ_KV_E3M2>(a, n_q, fused, mk, mv, stream, dry);
     case MJ_KV_E2M1: return launch_tc_fmt<MJ_KV_E2M1>(a, n_q, fused, mk, mv, stream, dry);
     case MJ_KV_NVFP4: return launch_tc_fmt<MJ_KV_NVFP4>(a, n_q, fused, mk, mv, stream, dry);
+    case MJ_KV_FP8_B16:
+    case MJ_KV_FP8_B32:
+    case MJ_KV_FP8_B64:
+    case MJ_KV_FP8_B128: return launch_tc_fmt<MJ_KV_FP8_B16>(a, n_q, fused, mk, mv, stream, dry);
     default: return launch_tc_fmt<MJ_KV_FP8_E4M3>(a, n_q, fused, mk, mv, stream, dry);
   }
 }

@@ -24,6 +24,11 @@
 //                      A = V (e4m3, MN-major), B = P; O accumulates in TMEM
 //                      over the job's tiles and is rescaled in place on the
 //                      rare max raise, read out once at the job's end
+//   Block-scaled e4m3 is used as stored: the softmax thread of a KV row reads
+//   the row's two block exponents one tile ahead, K's goes into the score
+//   (s c 2^ek) and V's into the exponent (z = s + ev; P' = 2^(z - m') is what
+//   multiplies V's codes, the row sums take P' 2^-ev), so the max runs over
+//   what enters O and one tensor's large scale cannot push P out of e4m3.
 //   e2m3 V cannot be an MN-major MMA operand, so converter warps (a whole
 //   warpgroup in the one-warpgroup variants) rewrite each 16-code slot in
 //   place as 16 e4m3 bytes of value code * 2^-6 (exact; the 2^6 is folded
@@ -50,6 +55,7 @@
 #include <atomic>
 #include <mutex>
 
+#include "block_cache.cuh"
 #include "common.cuh"
 #include "sm100.cuh"
 
@@ -163,11 +169,19 @@ __device__ __forceinline__ uint2 nvfp4x8_to_e4m3(uint32_t w, uint2 t) {
 // Per-format constants of the tensor-core path.
 template <int FMT>
 struct Fmt {
-  static constexpr bool NARROW = FMT != MJ_KV_FP8_E4M3;  // V needs a conversion to e4m3
+  // block-scaled e4m3 (one instantiation, MJ_KV_FP8_B16, serves every block size)
+  static constexpr bool BLOCK = FMT == MJ_KV_FP8_B16;
+  static constexpr bool NARROW = FMT != MJ_KV_FP8_E4M3 && !BLOCK;  // V needs a conversion to e4m3
   static constexpr bool SCALED = FMT == MJ_KV_NVFP4;     // group scales: K is converted too
   // kind::f8f6f4 operand format of K (nvfp4 K is converted to e4m3)
   static constexpr uint32_t MMA_FMT = FMT == MJ_KV_E2M3 ? 3u : FMT == MJ_KV_E3M2 ? 4u : FMT == MJ_KV_E2M1 ? 5u : 0u;
   static constexpr uint32_t ROW = (FMT == MJ_KV_E2M1 || SCALED) ? 64u : NARROW ? 96u : 128u;  // packed bytes per 128-code row
+  // block-scaled: the max moves once a P' would pass 2^2 of it, so that the
+  // largest P' stays in [112, 448] and the split's floor (2^-18) is 2^-25 of it
+  // rather than 2^-19: a head-dim element that the large weights multiply with
+  // zeros keeps its precision
+  static constexpr float RESCALE = BLOCK ? 2.f : kRescaleLog2;
+  static constexpr float LOG2P = BLOCK ? 6.80735492205760410f : kLog2PScale;  // log2(448) - RESCALE
   static constexpr float V_UNSCALE = FMT == MJ_KV_E3M2 ? 16.f : SCALED ? 1.f : NARROW ? 64.f : 1.f;  // undoes the conversion's shift
   static __device__ __forceinline__ uint4 convert(uint4 raw) {
     if constexpr (FMT == MJ_KV_E3M2) return e3m2x16_to_e4m3(raw);
@@ -823,6 +837,27 @@ __global__ void __launch_bounds__(Cfg<FMT, NQP, NWG, CVTW, DH>::THREADS, Cfg<FMT
       const int L = a.seq_lens[seq];
       const int nsp = a.n_splits[seq];
       const int row0 = g * RT + col0;
+      // block scales: this thread's KV row of tile i is in page_nx's block; the
+      // page is looked up two tiles ahead, the exponent bytes (K low, V << 8)
+      // one tile ahead
+      const int blk_lg = Fmt<FMT>::BLOCK ? block_log2(a.kv_format) : 0;
+      auto scale_page = [&](int tile) -> int {  // -1: no such row, or a bad entry (the producer flags it)
+        const int row = tile * kTileRows + t;
+        if (tile >= te || row >= L) return -1;
+        const int pg = __ldg(a.block_table + (int64_t)seq * a.block_table_stride + row / a.page_size);
+        return pg < 0 || pg >= a.num_pages ? -1 : pg;
+      };
+      auto scale_bytes = [&](int tile, int pg) -> uint32_t {
+        if (pg < 0) return 127u | (127u << 8);  // scales of 1 (such rows are zeros or masked)
+        const int b = ((tile * kTileRows + t) & (a.page_size - 1)) >> blk_lg;
+        return __ldg(static_cast<const unsigned char*>(a.k_scales) + pg * a.ks_stride_page + b * a.ks_stride_row + h * a.ks_stride_head) |
+               ((uint32_t)__ldg(static_cast<const unsigned char*>(a.v_scales) + pg * a.vs_stride_page + b * a.vs_stride_row + h * a.vs_stride_head) << 8);
+      };
+      int page_cur = -1, page_nx = -1;
+      if constexpr (Fmt<FMT>::BLOCK) {
+        page_cur = scale_page(tb);
+        page_nx = scale_page(tb + 1);
+      }
       float qv[DH][NQP], qm[DH][NQP];
       const int64_t qbase = (int64_t)seq * q_len * a.q_stride_tok + (int64_t)h * h_r * a.q_stride_head + t;
       auto qoff = [&](int r) {  // element offset of row r's head-dim element t
@@ -859,13 +894,20 @@ __global__ void __launch_bounds__(Cfg<FMT, NQP, NWG, CVTW, DH>::THREADS, Cfg<FMT
 #pragma unroll
         for (int r = 0; r < NQP; ++r) {
           qv[dh][r] = row0 + r < n_q ? qv[dh][r] * qm[dh][r] : 0.f;
+          if constexpr (Fmt<FMT>::BLOCK) {  // an infinity makes its row NaN, and only its row
+            if (fabsf(qv[dh][r]) > 3.402823466e38f) qv[dh][r] = __int_as_float(0x7FFFFFFF);
+          }
           qmax = fmaxf(qmax, fabsf(qv[dh][r]));
         }
       qmax = warp_max_f32(qmax);
       if (lane == 0) red[wq] = qmax;
       if (named_bar_or(bar_id, 128, *abort_flag != 0)) break;
       qmax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-      const float qs = qmax > 0.f ? 224.f / qmax : 1.f;  // |q * qs| <= 224
+      float qs = qmax > 0.f ? 224.f / qmax : 1.f;  // |q * qs| <= 224
+      if constexpr (Fmt<FMT>::BLOCK) {  // a power of two, |q * qs| < 256: 16-bit queries stay exact in the three terms
+        const int k = min(max(134 - (int)(__float_as_uint(qmax) >> 23), -120), 120);
+        qs = qmax > 0.f ? __uint_as_float((uint32_t)(127 + k) << 23) : 1.f;
+      }
 #pragma unroll
       for (int dh = 0; dh < DH; ++dh) {
         unsigned char* qb = qbuf(jc & 1, dh);
@@ -880,6 +922,7 @@ __global__ void __launch_bounds__(Cfg<FMT, NQP, NWG, CVTW, DH>::THREADS, Cfg<FMT
       const float kd = descale_at(a.k_descale, a.k_descale_mode, seq, h, h_k);
       const float vd = descale_at(a.v_descale, a.v_descale_mode, seq, h, h_k);
       const float c2 = a.softmax_scale * kd * kLog2e / qs;  // S (in q*qs units) -> log2 units
+      uint32_t sc_nx = Fmt<FMT>::BLOCK ? scale_bytes(tb, page_cur) : 0u;
       if (named_bar_or(bar_id, 128, *abort_flag != 0)) break;  // Q written and fenced, red[] read
       if (t == 0) mbar_arrive(&b.q_full[jc & 1]);
       ++jc;
@@ -914,6 +957,17 @@ __global__ void __launch_bounds__(Cfg<FMT, NQP, NWG, CVTW, DH>::THREADS, Cfg<FMT
       // written, and PV_t (PV_{t+1}) needs P_t (P_{t+1}), not yet written.
       const int n = te - tb;
       for (int i = 0; i < n; ++i, ++it) {
+        // this tile's scale of the scores, addend of the exponents and factor of the row sums
+        float2 c2t = c2v, ev2 = make_float2(0.f, 0.f), inv2 = make_float2(1.f, 1.f);
+        if constexpr (Fmt<FMT>::BLOCK) {
+          const int ek = block_e((unsigned char)sc_nx), ev = block_e((unsigned char)(sc_nx >> 8));
+          const float c = c2 * __uint_as_float((uint32_t)ek << 23), v = (float)(ev - 127), u = __uint_as_float((uint32_t)(254 - ev) << 23);
+          c2t = make_float2(c, c);
+          ev2 = make_float2(v, v);
+          inv2 = make_float2(u, u);
+          sc_nx = scale_bytes(tb + i + 1, page_nx);
+          page_nx = scale_page(tb + i + 2);
+        }
         if (!mbar_wait(&b.s_full[it & 1], (it >> 1) & 1, abort_flag, wait_ns) && !*abort_flag) give_up();
         tc_fence_after();
         float2 x2[NP];
@@ -924,7 +978,8 @@ __global__ void __launch_bounds__(Cfg<FMT, NQP, NWG, CVTW, DH>::THREADS, Cfg<FMT
           tmem_ld_cols<NS>(s_taddr, sv);
           tmem_wait_ld();
 #pragma unroll
-          for (int q = 0; q < NP; ++q) x2[q] = fmul2(combine3x2<NQP>(sv, 2 * q), c2v);
+          for (int q = 0; q < NP; ++q)
+            x2[q] = Fmt<FMT>::BLOCK ? ffma2(combine3x2<NQP>(sv, 2 * q), c2t, ev2) : fmul2(combine3x2<NQP>(sv, 2 * q), c2v);
         } else {  // this warpgroup's columns r, RT + r, 2 RT + r of 16 query rows: one wait
           static_assert(NQP == 16, "wide variants run 16 rows per warpgroup");
           float hv[16], mv[16], lv[16];
@@ -936,8 +991,8 @@ __global__ void __launch_bounds__(Cfg<FMT, NQP, NWG, CVTW, DH>::THREADS, Cfg<FMT
           for (int k = 0; k < 16; k += 2) {
             const float2 hi = make_float2(hv[k], hv[k + 1]), mid = make_float2(mv[k], mv[k + 1]),
                          lo = make_float2(lv[k], lv[k + 1]);
-            x2[k / 2] = fmul2(
-                ffma2(lo, make_float2(0.00390625f, 0.00390625f), ffma2(mid, make_float2(0.0625f, 0.0625f), hi)), c2v);
+            const float2 sum = ffma2(lo, make_float2(0.00390625f, 0.00390625f), ffma2(mid, make_float2(0.0625f, 0.0625f), hi));
+            x2[k / 2] = Fmt<FMT>::BLOCK ? ffma2(sum, c2t, ev2) : fmul2(sum, c2v);
           }
         }
         tc_fence_before();
@@ -961,7 +1016,7 @@ __global__ void __launch_bounds__(Cfg<FMT, NQP, NWG, CVTW, DH>::THREADS, Cfg<FMT
             x2[q] = fadd2(x2[q], nm2[q]);
             dmax = fmaxf(dmax, fmaxf(x2[q].x, x2[q].y));
           }
-          grow = dmax > kRescaleLog2 + kLog2PScale;
+          grow = dmax > Fmt<FMT>::RESCALE + Fmt<FMT>::LOG2P;
         }
         // one barrier per tile: a uniform vote on "some score outgrew its row's
         // max" (or abort); only then do the rows exchange their tile maxima
@@ -991,7 +1046,7 @@ __global__ void __launch_bounds__(Cfg<FMT, NQP, NWG, CVTW, DH>::THREADS, Cfg<FMT
           float cc[NQP];  // correction of each row's earlier sums: 2^(m_old - m_new)
 #pragma unroll
           for (int r = 0; r < NQP; ++r) {
-            const float mt = __shfl_sync(0xffffffffu, mine, r) - kLog2PScale;
+            const float mt = __shfl_sync(0xffffffffu, mine, r) - Fmt<FMT>::LOG2P;
             float& nmr = (r & 1) ? nm2[r >> 1].y : nm2[r >> 1].x;
             float& lr = (r & 1) ? l2[r >> 1].y : l2[r >> 1].x;
             cc[r] = 1.f;
@@ -1046,7 +1101,7 @@ __global__ void __launch_bounds__(Cfg<FMT, NQP, NWG, CVTW, DH>::THREADS, Cfg<FMT
 #pragma unroll
         for (int q = 0; q < NP; ++q) {
           const float2 pv = make_float2(exp2_approx(x2[q].x), exp2_approx(x2[q].y));
-          l2[q] = fadd2(l2[q], pv);
+          l2[q] = Fmt<FMT>::BLOCK ? ffma2(pv, inv2, l2[q]) : fadd2(l2[q], pv);
           uint16_t hb, mb, lb;
           split3x2(pv, hb, mb, lb);
           const int r = 2 * q, sh = 16 * (q & 1);
@@ -1152,7 +1207,8 @@ __global__ void __launch_bounds__(Cfg<FMT, NQP, NWG, CVTW, DH>::THREADS, Cfg<FMT
 #pragma unroll
           for (int r = 0; r < NQP; ++r) {
             const float lt = lred[r] + lred[NQP + r] + lred[2 * NQP + r] + lred[3 * NQP + r];
-            o[r] = lt > 0.f ? orow[dh][r] * __fdividef(vscale, lt) : 0.f;
+            if constexpr (Fmt<FMT>::BLOCK) o[r] = lt == 0.f ? 0.f : orow[dh][r] * (vscale / lt);  // NaN sums stay NaN; lt may pass 2^126
+            else o[r] = lt > 0.f ? orow[dh][r] * __fdividef(vscale, lt) : 0.f;
           }
           if (final_out && a.o_mul) {
             float om[NQP];
@@ -1187,7 +1243,7 @@ __global__ void __launch_bounds__(Cfg<FMT, NQP, NWG, CVTW, DH>::THREADS, Cfg<FMT
               lt = lred[r] + lred[NQP + r] + lred[2 * NQP + r] + lred[3 * NQP + r];
               mr = -((r & 1) ? nm2[r >> 1].y : nm2[r >> 1].x);
             }
-          const float lse = lt > 0.f ? (mr + log2f(lt)) * kLn2 : -INFINITY;
+          const float lse = (Fmt<FMT>::BLOCK ? lt != 0.f : lt > 0.f) ? (mr + log2f(lt)) * kLn2 : -INFINITY;
           if (!final_out) a.lse_part[(((int64_t)split * a.part_seqs + seq) * h_k + h) * n_q + row0 + t] = lse;
           else if (a.lse) a.lse[tok_of(t) * a.h_q + qh_of(t)] = lse;
         }
@@ -1227,7 +1283,7 @@ __global__ void __launch_bounds__(Cfg<FMT, NQP, NWG, CVTW, DH>::THREADS, Cfg<FMT
             for (int r = 0; r < NQP; ++r) {
               if (row0 + r >= n_q) break;
               float m = -INFINITY;
-              for (int k = 0; k < ns; ++k) m = fmaxf(m, lsm[k * NQP + r]);
+              for (int k = 0; k < ns; ++k) m = Fmt<FMT>::BLOCK ? nan_max(m, lsm[k * NQP + r]) : fmaxf(m, lsm[k * NQP + r]);
               float den = 0.f;
 #pragma unroll
               for (int dh = 0; dh < DH; ++dh) {  // head-dim element e = dh * 128 + t
@@ -1246,11 +1302,11 @@ __global__ void __launch_bounds__(Cfg<FMT, NQP, NWG, CVTW, DH>::THREADS, Cfg<FMT
                       acc = fmaf(w, ov[k], acc);
                     }
                 }
-                float o = den > 0.f ? acc / den : 0.f;
+                float o = (Fmt<FMT>::BLOCK ? den != 0.f : den > 0.f) ? acc / den : 0.f;
                 if (a.o_mul) o *= a.o_mul[(int64_t)qh_of(r) * D + e];
                 store_elem(a.o, tok_of(r) * a.o_stride_tok + qh_of(r) * a.o_stride_head + e, a.o_dtype, o);
               }
-              if (t == 0 && a.lse) a.lse[tok_of(r) * a.h_q + qh_of(r)] = den > 0.f ? m + __logf(den) : -INFINITY;
+              if (t == 0 && a.lse) a.lse[tok_of(r) * a.h_q + qh_of(r)] = (Fmt<FMT>::BLOCK ? den != 0.f : den > 0.f) ? m + __logf(den) : -INFINITY;
             }
           }
         }

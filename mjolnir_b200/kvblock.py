@@ -23,7 +23,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .runner import _ptr, _stream, dtype_code, kv_byte_strides
+from .runner import DecodeRunner, StepPlan, _ptr, _stream, dtype_code, kv_byte_strides
 
 HEAD_SIZES = (128, 256)
 BLOCK_TOKENS = tuple(_lib.BLOCK_FORMATS)
@@ -189,14 +189,20 @@ class BlockPlan:
     merges: torch.Tensor  # (merges, 4) int32, device
     num_slots: int
     causal: bool = True
+    decode: StepPlan | None = None  # the leading sequences that the decode kernel serves
 
 
 class BlockAttention:
     """Attention over a block-scaled cache for steps of any mix of lengths:
-    single tokens, drafts and prompt chunks behind cached contexts."""
+    single tokens, drafts and prompt chunks behind cached contexts.
+
+    The leading sequences of a step that share one query length of at most
+    ``max_q_len`` tokens (a batch's decodes, which schedulers put first) run on
+    the decode kernel, the others on the kernel for chunks: one query token of
+    a group of 4 heads fills 4 of the chunk kernel's 256 rows."""
 
     def __init__(self, *, num_heads: int, num_kv_heads: int, head_size: int, page_size: int, block_tokens: int = 16,
-                 max_num_seqs: int = 256, max_num_tokens: int = 8192, device: torch.device | str = "cuda"):
+                 max_num_seqs: int = 256, max_num_tokens: int = 8192, max_q_len: int = 4, device: torch.device | str = "cuda"):
         if num_heads % num_kv_heads:
             raise ValueError("num_heads must be a multiple of num_kv_heads")
         if page_size not in (16, 32, 64, 128):
@@ -207,6 +213,10 @@ class BlockAttention:
         self.max_num_seqs, self.max_num_tokens = max_num_seqs, max_num_tokens
         self.device = torch.device(device)
         _lib.load()  # fail at construction, not at the first step
+        self.max_q_len = min(max_q_len, 64 // (num_heads // num_kv_heads))
+        self.decode = None if self.max_q_len < 1 else DecodeRunner(
+            num_heads=num_heads, num_kv_heads=num_kv_heads, head_size=head_size, page_size=page_size,
+            max_num_seqs=max_num_seqs, max_q_len=self.max_q_len, kv_format=f"fp8b{block_tokens}", kernel="tc", device=device)
         self.sm_count = torch.cuda.get_device_properties(self.device).multi_processor_count
         # rows of a work item, and the partial slots that splitting for every SM can ask for
         self.rows = 128 if head_size == 256 else 256
@@ -218,6 +228,7 @@ class BlockAttention:
         self.o_part = torch.empty(self.max_slots * num_kv_heads * self.rows * head_size, dtype=torch.float32, device=self.device)
         self.lse_part = torch.empty(self.max_slots * num_kv_heads * self.rows, dtype=torch.float32, device=self.device)
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self.one = torch.ones(1, dtype=torch.float32, device=self.device)
 
     def plan(self, query_lens, seq_lens_cpu, block_table: torch.Tensor, seq_lens: torch.Tensor,
              causal: bool = True) -> BlockPlan:
@@ -234,17 +245,23 @@ class BlockAttention:
         if seq_lens.dtype != torch.int32 or seq_lens.dim() != 1 or seq_lens.shape[0] < len(q) or not seq_lens.is_contiguous():
             raise ValueError("seq_lens must be a contiguous int32 tensor of every sequence")
         _on(self.status.device, block_table, seq_lens)
+        decode, few = None, 0
+        if q and 1 <= q[0] <= self.max_q_len:
+            few = next((i for i, x in enumerate(q) if x != q[0]), len(q))
+            decode = self.decode.plan(kv, few, q[0], block_table, seq_lens, causal=causal)
+        if few == len(q):
+            return BlockPlan(q, sum(q), block_table, seq_lens, None, None, None, 0, causal, decode)
         n, (m0, w0) = len(q), self._at
         stage = torch.empty(self.plan_buf.shape[0], dtype=torch.int32, pin_memory=True)
         host = stage.numpy()
         host[0] = 0
         np.cumsum(q, out=host[1:n + 1])
         work, merges = host[w0:].reshape(-1, 8), host[m0:w0].reshape(-1, 4)
-        nw, nm, slots = _lib.block_plan(q, kv, self.h_q, self.h_k, self.d, causal, self.sm_count, self.max_slots, work, merges)
+        nw, nm, slots = _lib.block_plan([0] * few + q[few:], kv, self.h_q, self.h_k, self.d, causal, self.sm_count, self.max_slots, work, merges)
         used = w0 + 8 * nw
         self.plan_buf[:used].copy_(stage[:used], non_blocking=True)
         return BlockPlan(q, sum(q), block_table, seq_lens, self.plan_buf[:n + 1], self.plan_buf[w0:used].view(-1, 8),
-                         self.plan_buf[m0:m0 + 4 * nm].view(-1, 4), slots, causal)
+                         self.plan_buf[m0:m0 + 4 * nm].view(-1, 4), slots, causal, decode)
 
     def run(
         self,
@@ -258,6 +275,11 @@ class BlockAttention:
         softmax_scale: float,
         lse: torch.Tensor | None = None,  # optional (tokens, h_q) fp32
     ) -> torch.Tensor:
+        if plan.decode is not None:
+            self.decode.run(plan.decode, query, out, k_cache, v_cache, self.one, self.one, softmax_scale, lse=lse,
+                            k_scales=k_scales, v_scales=v_scales)
+            if plan.work is None:
+                return out
         a = _lib.BlockAttnArgs()
         g = _cache_args(a, k_cache, v_cache, k_scales, v_scales)
         if (a.page_size, g, a.h_k, a.head_size) != (self.page_size, self.block_tokens, self.h_k, self.d):
@@ -288,6 +310,8 @@ class BlockAttention:
     def check_status(self) -> None:
         """Raise if a kernel flagged a bad page or a wait that ran out
         (synchronizes); the status word is cleared."""
+        if self.decode is not None:
+            self.decode.check_status()
         code = int(self.status.item())
         if code != _lib.MJ_DEV_OK:
             self.status.zero_()

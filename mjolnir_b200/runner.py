@@ -125,10 +125,14 @@ def split_kv_cache(kv_cache: torch.Tensor, layout: str, row: int):
     return k, v
 
 
+# tokens per scale block of the block-scaled fp8 formats
+BLOCK_OF = {f"fp8b{g}": g for g in _lib.BLOCK_FORMATS}
+
+
 def row_bytes(head_size: int, kv_format: str) -> int:
     if head_size % 16:
         raise ValueError(f"head_size {head_size} must be a multiple of 16")
-    if kv_format == "fp8":
+    if kv_format == "fp8" or kv_format in BLOCK_OF:
         return head_size
     if kv_format in ("e2m3", "e3m2"):
         return head_size * 3 // 4
@@ -148,7 +152,19 @@ def scale_row_bytes(head_size: int) -> int:
 def set_scale_views(a, k_scales: torch.Tensor | None, v_scales: torch.Tensor | None, pages: int, page_size: int,
                     h_k: int, head_size: int, kv_format: str) -> None:
     """Point an args struct at the nvfp4 group-scale views (logical
-    (pages, page_size, h_k, head_size / 16) bytes, last dim contiguous)."""
+    (pages, page_size, h_k, head_size / 16) bytes, last dim contiguous), or at
+    the exponent views of a block-scaled format (logical (pages, page_size / G,
+    h_k) bytes)."""
+    if kv_format in BLOCK_OF:
+        want = (pages, page_size // BLOCK_OF[kv_format], h_k)
+        for side, t in (("k", k_scales), ("v", v_scales)):
+            if t is None or tuple(t.shape) != want or t.element_size() != 1:
+                raise ValueError(f"{kv_format} needs {side}_scales of {want} bytes, got {None if t is None else tuple(t.shape)}")
+            st = [0 if n == 1 else s for n, s in zip(t.shape, t.stride())]
+            setattr(a, f"{side}_scales", t.data_ptr())
+            for name, x in zip(("page", "row", "head"), st):
+                setattr(a, f"{side}s_stride_{name}", x)
+        return
     if kv_format != "nvfp4":
         return
     want = (page_size, h_k, scale_row_bytes(head_size))
@@ -257,6 +273,8 @@ class DecodeRunner:
             raise ValueError(f"page size {page_size} unsupported (supported: {SUPPORTED_PAGE_SIZES})")
         if kv_format not in _lib.KV_FORMATS:
             raise ValueError(f"kv_format must be one of {tuple(_lib.KV_FORMATS)}")
+        if kv_format in BLOCK_OF and page_size % BLOCK_OF[kv_format]:
+            raise ValueError(f"{kv_format}: a block must divide the page of {page_size}")
         self.h_q, self.h_k, self.d = num_heads, num_kv_heads, head_size
         self.h_r = num_heads // num_kv_heads
         if max_q_len * self.h_r > 64:
@@ -468,8 +486,8 @@ class DecodeRunner:
         q_mul: torch.Tensor | None = None,  # (h_q, d) fp32: e2m3 K channel scales folded into Q
         o_mul: torch.Tensor | None = None,  # (h_q, d) fp32: e2m3 V channel scales on O
         lse: torch.Tensor | None = None,  # optional (b*q_len, h_q) fp32
-        k_scales: torch.Tensor | None = None,  # nvfp4: (num_pages, page_size, h_k, d / 16) uint8 views
-        v_scales: torch.Tensor | None = None,
+        k_scales: torch.Tensor | None = None,  # nvfp4: (num_pages, page_size, h_k, d / 16) uint8 views; fp8bG:
+        v_scales: torch.Tensor | None = None,  # (num_pages, page_size / G, h_k) exponent bytes
     ):
         a = self.decode_args(plan, query, out, k_cache, v_cache, k_scale, v_scale, softmax_scale, q_mul, o_mul, lse,
                              k_scales, v_scales)
