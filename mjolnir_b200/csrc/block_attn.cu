@@ -28,10 +28,12 @@
 //
 // Every mbarrier wait is bounded; on a timeout the CTA flags MJ_DEV_TIMEOUT,
 // all roles stop, the MMAs in flight complete and TMEM is freed.
+#include <limits.h>
 #include <math.h>
 
 #include <atomic>
 #include <mutex>
+#include <utility>
 
 #include "block_cache.cuh"
 
@@ -71,6 +73,17 @@ struct Cfg {
 
 // byte offset of 16-byte unit u of row r in a [rows][64 f16] swizzled block
 __device__ __forceinline__ uint32_t unit_offset(uint32_t r, uint32_t u) { return r * 128 + ((u ^ (r & 7)) << 4); }
+
+template <int D, int BN, int... K>
+__device__ __forceinline__ void issue_qk(uint32_t s, uint32_t q, uint32_t k, uint32_t hi, uint32_t idesc,
+                                         std::integer_sequence<int, K...>) {
+  (mma_f16_ss<(K >> 2) * (128 * 8) + (K & 3) * 2, (K >> 2) * (BN * 8) + (K & 3) * 2>(s, q, k, hi, idesc, K > 0), ...);
+}
+template <int... K>
+__device__ __forceinline__ void issue_pv(uint32_t o, uint32_t p, uint32_t v, uint32_t hi, uint32_t idesc, bool accumulate,
+                                         std::integer_sequence<int, K...>) {
+  (mma_f16_ts<8 * K, 128 * K>(o, p, v, hi, idesc, accumulate || K > 0), ...);
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __grid_constant__ mj_block_attn_args a, int lg) {
@@ -153,20 +166,17 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
     if (warp == 0 && lane == 0) {
       // ------------------------------------------------------------ MMA issuer
       constexpr uint32_t idesc_s = idesc_f16(0, 0, BN), idesc_o = idesc_f16(0, 1, D);
-      auto qk = [&](int w, int j) {
-        const uint32_t qa = smem_addr(sm + w * C::QTILE), ka = smem_addr(sm + C::K_OFF + (j & 1) * C::KTILE);
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          mma_f16_ss(tmem + s_col(w, j), smem_desc_sw128(qa + (k >> 2) * (128 * 128) + (k & 3) * 32, 16, 1024),
-                     smem_desc_sw128(ka + (k >> 2) * (BN * 128) + (k & 3) * 32, 16, 1024), idesc_s, k > 0);
+      constexpr uint32_t hi = desc_hi_sw128(1024);
+      const uint32_t q_lo = desc_lo(smem_addr(sm), 16), k_lo = desc_lo(smem_addr(sm + C::K_OFF), 16),
+                     v_lo = desc_lo(smem_addr(sm + C::V_OFF), BN * 128);
+      auto qk = [&](int w, int j) {  // 16 head-dim elements a step, 64 a swizzled block
+        issue_qk<D, BN>(tmem + s_col(w, j), q_lo + w * (C::QTILE / 16), k_lo + (j & 1) * (C::KTILE / 16), hi, idesc_s,
+                        std::make_integer_sequence<int, D / 16>());
         mma_commit(&s_full[s_bar(w, j)]);
       };
-      auto pv = [&](int w, int j) {
-        const uint32_t va = smem_addr(sm + C::V_OFF + (j & 1) * C::KTILE);
-#pragma unroll
-        for (int k = 0; k < BN / 16; ++k)  // 16 tokens a step: two 8-row atoms
-          mma_f16_ts(tmem + C::O_COL + w * 128, tmem + s_col(w, j) + k * 8, smem_desc_sw128(va + k * 2048, BN * 128, 1024),
-                     idesc_o, j > 0 || k > 0);
+      auto pv = [&](int w, int j) {  // 16 tokens a step: two 8-row atoms of V, 8 columns of P
+        issue_pv(tmem + C::O_COL + w * 128, tmem + s_col(w, j), v_lo + (j & 1) * (C::KTILE / 16), hi, idesc_o, j > 0,
+                 std::make_integer_sequence<int, BN / 16>());
         mma_commit(&o_full[2 * w + (j & 1)]);
       };
       bool ok = n > 0 && wait(q_full, 0) && wait(&k_full[0], 0);
@@ -203,21 +213,34 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
     if constexpr (C::REG_CVT > 0) setmaxnreg_dec<C::REG_CVT>();
     const int ct = threadIdx.x - 128;
     constexpr int CPR = D / 16, STEP = 128 / CPR, NC = BN / STEP;  // 16-code chunks of a row; rows of a pass; passes
-    const int col = ct % CPR, r0 = ct / CPR;
+    const int col = ct % CPR, r0 = ct / CPR, base = tb * BN;
     const int32_t* table = a.block_table + seq * a.block_table_stride;
     const int ps_log2 = 31 - __clz(a.page_size), pmask = a.page_size - 1;
     const unsigned char* kbase = static_cast<const unsigned char*>(a.k_cache) + h * a.k_stride_head + col * 16;
     const unsigned char* vbase = static_cast<const unsigned char*>(a.v_cache) + h * a.v_stride_head + col * 16;
-    // page of token `pos`; -1 past the sequence or for a bad table entry
-    auto page_of = [&](int pos) -> int {
-      if (pos >= L) return -1;
+    // The table entry of token `pos` is loaded an operand before it is checked:
+    // checking it at once would wait a memory round trip for every row.
+    constexpr int kNone = INT_MIN;  // past the sequence
+    const int last = base + n * BN;  // tokens from here on are not this item's
+    auto entry_of = [&](int pos) -> int {
+      if (pos >= L || pos >= last) return kNone;
       const int c = pos >> ps_log2;
-      const int p = c < a.block_table_cols ? __ldg(table + c) : -1;
-      if (p < 0 || p >= a.num_pages) {
-        flag(a.status, MJ_DEV_BAD_PAGE);
-        return -1;
-      }
-      return p;
+      return c < a.block_table_cols ? __ldg(table + c) : -1;
+    };
+    auto page_of = [&](int e) -> int {  // -1: no such token, or a bad entry
+      if ((unsigned)e < (unsigned)a.num_pages) return e;
+      if (e != kNone) flag(a.status, MJ_DEV_BAD_PAGE);
+      return -1;
+    };
+    // block scales of the tile's 16-token groups: thread ct < BN / 16 looks the
+    // page up two tiles ahead and reads the two exponents one tile ahead
+    constexpr uint32_t kOne = 127u | (127u << 8);
+    const bool scaler = ct < BN / 16;
+    auto exponents = [&](int pos, int p) -> uint32_t {
+      if (p < 0) return kOne;
+      const int b = (pos & pmask) >> lg;
+      return __ldg(static_cast<const unsigned char*>(a.k_scales) + p * a.ks_stride_page + b * a.ks_stride_block + h * a.ks_stride_head) |
+             ((uint32_t)__ldg(static_cast<const unsigned char*>(a.v_scales) + p * a.vs_stride_page + b * a.vs_stride_block + h * a.vs_stride_head) << 8);
     };
     uint4 data[NC];
     int page[NC];
@@ -239,26 +262,27 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
       *reinterpret_cast<uint4*>(buf + block_at + unit_offset(r, unit + odd)) = odd ? hi : lo;
       *reinterpret_cast<uint4*>(buf + block_at + unit_offset(r, unit + 1 - odd)) = odd ? lo : hi;
     };
-    const int base = tb * BN;
+    int sc_entry = kNone;
+    uint32_t sc_next = kOne;
+    if (scaler) {
+      const int e0 = entry_of(base + ct * 16);
+      sc_entry = entry_of(base + BN + ct * 16);
+      sc_next = exponents(base + ct * 16, page_of(e0));
+    }
 #pragma unroll
-    for (int i = 0; i < NC; ++i) page[i] = page_of(base + r0 + i * STEP);
+    for (int i = 0; i < NC; ++i) page[i] = entry_of(base + r0 + i * STEP);
+#pragma unroll
+    for (int i = 0; i < NC; ++i) page[i] = page_of(page[i]);
 #pragma unroll
     for (int i = 0; i < NC; ++i) data[i] = load_k(base + r0 + i * STEP, page[i]);
     for (int j = 0; j < n; ++j) {
       const int t0 = base + j * BN;
-      if (ct < BN / 16) {  // this tile's block scales, one entry per 16 tokens
-        const int pos = t0 + ct * 16, p = page_of(pos);
-        float ek = 1.f, ev = 0.f, inv = 1.f;
-        if (p >= 0) {
-          const int b = (pos & pmask) >> lg;
-          const unsigned char* ks = static_cast<const unsigned char*>(a.k_scales) + p * a.ks_stride_page + b * a.ks_stride_block + h * a.ks_stride_head;
-          const unsigned char* vs = static_cast<const unsigned char*>(a.v_scales) + p * a.vs_stride_page + b * a.vs_stride_block + h * a.vs_stride_head;
-          ek = block_scale(*ks);
-          const int e = block_e(*vs);
-          ev = (float)(e - 127);
-          inv = __uint_as_float((uint32_t)(254 - e) << 23);
-        }
-        reinterpret_cast<float4*>(sm + C::SC_OFF)[(j & 3) * (BN / 16) + ct] = make_float4(ek, ev, inv, 0.f);
+      if (scaler) {
+        const int e = block_e((unsigned char)(sc_next >> 8));
+        reinterpret_cast<float4*>(sm + C::SC_OFF)[(j & 3) * (BN / 16) + ct] =
+            make_float4(block_scale((unsigned char)sc_next), (float)(e - 127), __uint_as_float((uint32_t)(254 - e) << 23), 0.f);
+        sc_next = exponents(t0 + BN + ct * 16, page_of(sc_entry));
+        sc_entry = entry_of(t0 + 2 * BN + ct * 16);
       }
       if (ct < 32) {
         __syncwarp();
@@ -271,7 +295,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
         const int r = r0 + i * STEP;
         store(kb, r, data[i]);
         data[i] = load_v(t0 + r, page[i]);
-        page[i] = j + 1 < n ? page_of(t0 + BN + r) : -1;
+        page[i] = entry_of(t0 + BN + r);
       }
       fence_proxy_async_smem();
       mbar_arrive(&k_full[j & 1]);
@@ -281,6 +305,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
       for (int i = 0; i < NC; ++i) {
         const int r = r0 + i * STEP;
         store(vb, r, data[i]);
+        page[i] = page_of(page[i]);
         data[i] = load_k(t0 + BN + r, page[i]);
       }
       fence_proxy_async_smem();

@@ -23,7 +23,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .runner import DecodeRunner, StepPlan, _ptr, _stream, dtype_code, kv_byte_strides
+from .runner import DecodeRunner, StepPlan, _ptr, call, dtype_code
 
 HEAD_SIZES = (128, 256)
 BLOCK_TOKENS = tuple(_lib.BLOCK_FORMATS)
@@ -54,39 +54,38 @@ def _format(block_tokens: int, page_size: int, head_size: int) -> int:
     return _lib.BLOCK_FORMATS[block_tokens]
 
 
-def _cache_args(a, k_cache, v_cache, k_scales, v_scales, row_stride: str = "block") -> int:
-    """Points an args struct at checked cache and scale views; returns the
-    tokens of a block."""
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if t.dim() != 4 or t.shape != k_cache.shape or t.element_size() != 1:
-            raise ValueError(f"{name} must be a (pages, page_size, h_k, d) byte view, got {tuple(t.shape)} {t.dtype}")
-    pages, page_size, h_k, d = k_cache.shape
-    blocks = k_scales.shape[1] if k_scales.dim() == 3 else 0
-    if blocks < 1 or page_size % blocks:
-        raise ValueError(f"k_scales {tuple(k_scales.shape)} is not (pages, page_size / G, h_k) for pages of {page_size}")
-    for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
-        if tuple(t.shape) != (pages, blocks, h_k) or t.element_size() != 1:
-            raise ValueError(f"{name} {tuple(t.shape)} {t.dtype} is not ({pages}, {blocks}, {h_k}) bytes")
-    for t in (v_cache, k_scales, v_scales):
-        if t.device != k_cache.device:
-            raise ValueError(f"cache and scales must share a device, got {k_cache.device} and {t.device}")
-    a.kv_format = _format(page_size // blocks, page_size, d)
-    a.k_cache, a.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
-    a.k_stride_page, a.k_stride_row, a.k_stride_head = kv_byte_strides(k_cache)
-    a.v_stride_page, a.v_stride_row, a.v_stride_head = kv_byte_strides(v_cache)
-    a.k_scales, a.v_scales = k_scales.data_ptr(), v_scales.data_ptr()
-    for side, t in (("ks", k_scales), ("vs", v_scales)):
-        st = [0 if n == 1 else s for n, s in zip(t.shape, t.stride())]
-        setattr(a, f"{side}_stride_page", st[0])
-        setattr(a, f"{side}_stride_{row_stride}", st[1])
-        setattr(a, f"{side}_stride_head", st[2])
-    a.num_pages, a.page_size, a.h_k, a.head_size = pages, page_size, h_k, d
-    return page_size // blocks
+def _strides(t: torch.Tensor) -> tuple:
+    """Strides of the first three dims; a dim of extent 1 may carry any."""
+    st, sh = t.stride(), t.shape
+    if 1 in sh:
+        st = [0 if n == 1 else x for n, x in zip(sh, st)]
+    return st[0], st[1], st[2]
 
 
-def _rows(name: str, t: torch.Tensor, h_k: int, d: int) -> None:
-    if t.dim() != 3 or tuple(t.shape[1:]) != (h_k, d) or t.stride(2) != 1:
-        raise ValueError(f"{name} {tuple(t.shape)} is not (rows, {h_k}, {d}) with contiguous rows")
+def _cache(k_cache, v_cache, k_scales, v_scales) -> tuple:
+    """Checks cache and scale views; returns (shape, kv_format, the six code
+    strides, the six scale strides)."""
+    shape, sshape = k_cache.shape, k_scales.shape
+    if len(shape) != 4 or v_cache.shape != shape or k_cache.itemsize != 1 or v_cache.itemsize != 1 or (
+            k_cache.stride(3) != 1 or v_cache.stride(3) != 1):
+        raise ValueError(f"k_cache {tuple(shape)} {k_cache.dtype} and v_cache {tuple(v_cache.shape)} {v_cache.dtype} must be "
+                         "(pages, page_size, h_k, d) byte views with contiguous rows")
+    pages, page_size, h_k, d = shape
+    if (len(sshape) != 3 or v_scales.shape != sshape or k_scales.itemsize != 1 or v_scales.itemsize != 1
+            or sshape[0] != pages or sshape[2] != h_k or sshape[1] < 1 or page_size % sshape[1]):
+        raise ValueError(f"k_scales {tuple(sshape)} {k_scales.dtype} and v_scales {tuple(v_scales.shape)} {v_scales.dtype} must "
+                         f"be ({pages}, {page_size} / G, {h_k}) byte views")
+    kv_format = _format(page_size // sshape[1], page_size, d)
+    _on(k_cache.device, v_cache, k_scales, v_scales)
+    return shape, kv_format, _strides(k_cache) + _strides(v_cache), _strides(k_scales) + _strides(v_scales)
+
+
+def _rows(name: str, t: torch.Tensor, h_k: int, d: int) -> tuple:
+    """(token, head) strides of checked rows."""
+    shape, st = t.shape, t.stride()
+    if len(shape) != 3 or shape[1] != h_k or shape[2] != d or st[2] != 1:
+        raise ValueError(f"{name} {tuple(shape)} is not (rows, {h_k}, {d}) with contiguous rows")
+    return st[0], st[1]
 
 
 def _on(device: torch.device, *tensors) -> None:
@@ -112,10 +111,8 @@ def write(
     T = slot_mapping.shape[0]
     if T == 0:
         return
-    a = _lib.CacheWriteArgs()
-    _cache_args(a, k_cache, v_cache, k_scales, v_scales, row_stride="row")
-    _rows("key", key, a.h_k, a.head_size)
-    _rows("value", value, a.h_k, a.head_size)
+    (pages, page_size, h_k, d), kv_format, st, ss = _cache(k_cache, v_cache, k_scales, v_scales)
+    kt, vt = _rows("key", key, h_k, d), _rows("value", value, h_k, d)
     if key.shape[0] < T or value.shape[0] < T:
         raise ValueError("fewer key / value rows than slots")
     if value.dtype != key.dtype:
@@ -123,13 +120,14 @@ def write(
     if slot_mapping.dim() != 1 or slot_mapping.dtype not in (torch.int64, torch.int32):
         raise TypeError("slot_mapping must be a 1-D int64")
     _on(k_cache.device, key, value, slot_mapping, status)
-    slots = slot_mapping.to(torch.int64).contiguous()
-    a.key, a.value, a.src_dtype, a.num_tokens = key.data_ptr(), value.data_ptr(), dtype_code(key.dtype), T
-    a.key_stride_tok, a.key_stride_head = key.stride(0), key.stride(1)
-    a.value_stride_tok, a.value_stride_head = value.stride(0), value.stride(1)
-    a.slot_mapping, a.status = slots.data_ptr(), _ptr(status)
-    with torch.cuda.device(k_cache.device):
-        _lib.block_write(a, _stream(k_cache.device))
+    slots = slot_mapping
+    if slots.dtype != torch.int64 or not slots.is_contiguous():
+        slots = slots.to(torch.int64).contiguous()
+    a = _lib.CacheWriteArgs(
+        key.data_ptr(), value.data_ptr(), dtype_code(key.dtype), T, h_k, d, *kt, *vt, k_cache.data_ptr(), v_cache.data_ptr(),
+        *st, pages, page_size, kv_format, slots.data_ptr(), None, 0, None, 0, _ptr(status),
+        k_scales.data_ptr(), v_scales.data_ptr(), *ss)
+    call(_lib.block_write, a, k_cache.device)
 
 
 def _table(block_table: torch.Tensor, num_seqs: int) -> None:
@@ -153,26 +151,21 @@ def read(
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """Read tokens ``starts[s] ..`` of each sequence into rows ``offsets[s] ..
     offsets[s + 1] - 1`` of the outputs; returns ``(k_out, v_out)``."""
-    a = _lib.BlockReadArgs()
-    _cache_args(a, k_cache, v_cache, k_scales, v_scales)
+    (pages, page_size, h_k, d), kv_format, st, ss = _cache(k_cache, v_cache, k_scales, v_scales)
     n = starts.shape[0]
     for name, t, m in (("starts", starts, n), ("offsets", offsets, n + 1)):
-        if t.dtype != torch.int32 or tuple(t.shape) != (m,) or not t.is_contiguous():
+        if t.dtype != torch.int32 or t.shape != (m,) or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous int32 ({m},), got {t.dtype} {tuple(t.shape)}")
     _table(block_table, n)
-    _rows("k_out", k_out, a.h_k, a.head_size)
-    _rows("v_out", v_out, a.h_k, a.head_size)
+    ko, vo = _rows("k_out", k_out, h_k, d), _rows("v_out", v_out, h_k, d)
     if v_out.shape != k_out.shape or v_out.dtype != k_out.dtype:
         raise ValueError("k_out and v_out must share a shape and dtype")
     _on(k_cache.device, block_table, starts, offsets, k_out, v_out, status)
-    a.block_table, a.block_table_stride, a.block_table_cols = block_table.data_ptr(), block_table.stride(0), block_table.shape[1]
-    a.starts, a.offsets, a.num_seqs, a.num_rows = starts.data_ptr(), offsets.data_ptr(), n, k_out.shape[0]
-    a.k_out, a.v_out, a.out_dtype = k_out.data_ptr(), v_out.data_ptr(), dtype_code(k_out.dtype)
-    a.ko_stride_tok, a.ko_stride_head = k_out.stride(0), k_out.stride(1)
-    a.vo_stride_tok, a.vo_stride_head = v_out.stride(0), v_out.stride(1)
-    a.status = _ptr(status)
-    with torch.cuda.device(k_cache.device):
-        _lib.block_read(a, _stream(k_cache.device))
+    a = _lib.BlockReadArgs(
+        k_cache.data_ptr(), v_cache.data_ptr(), *st, k_scales.data_ptr(), v_scales.data_ptr(), *ss, pages, page_size, h_k, d,
+        kv_format, block_table.data_ptr(), block_table.stride(0), block_table.shape[1], starts.data_ptr(), offsets.data_ptr(),
+        n, k_out.shape[0], k_out.data_ptr(), v_out.data_ptr(), dtype_code(k_out.dtype), *ko, *vo, _ptr(status))
+    call(_lib.block_read, a, k_cache.device)
     return k_out, v_out
 
 
@@ -275,36 +268,39 @@ class BlockAttention:
         softmax_scale: float,
         lse: torch.Tensor | None = None,  # optional (tokens, h_q) fp32
     ) -> torch.Tensor:
-        if plan.decode is not None:
-            self.decode.run(plan.decode, query, out, k_cache, v_cache, self.one, self.one, softmax_scale, lse=lse,
-                            k_scales=k_scales, v_scales=v_scales)
-            if plan.work is None:
-                return out
-        a = _lib.BlockAttnArgs()
-        g = _cache_args(a, k_cache, v_cache, k_scales, v_scales)
-        if (a.page_size, g, a.h_k, a.head_size) != (self.page_size, self.block_tokens, self.h_k, self.d):
-            raise ValueError(f"cache of pages {a.page_size}, blocks {g}, {a.h_k} heads of {a.head_size} is not this runner's")
-        for name, t in (("query", query), ("out", out)):
-            _rows(name, t, self.h_q, self.d)
-            if t.shape[0] < plan.num_tokens:
-                raise ValueError(f"{name} has {t.shape[0]} rows for {plan.num_tokens} tokens")
-        if out.dtype != query.dtype or query.dtype not in (torch.bfloat16, torch.float16):
+        (pages, page_size, h_k, d), kv_format, st, ss = _cache(k_cache, v_cache, k_scales, v_scales)
+        if (page_size, kv_format, h_k, d) != (self.page_size, self.kv_format, self.h_k, self.d):
+            raise ValueError(f"a cache of pages {page_size}, format {kv_format}, {h_k} heads of {d} is not this runner's")
+        qs, os_ = _rows("query", query, self.h_q, d), _rows("out", out, self.h_q, d)
+        tokens, dt = plan.num_tokens, dtype_code(query.dtype)
+        if query.shape[0] < tokens or out.shape[0] < tokens:
+            raise ValueError(f"query {tuple(query.shape)} / out {tuple(out.shape)} have fewer rows than the step's {tokens} tokens")
+        if out.dtype != query.dtype or dt == _lib.MJ_DT_FP32:
             raise TypeError(f"query and out must both be bf16 or fp16, got {query.dtype} and {out.dtype}")
-        if lse is not None and (lse.dtype != torch.float32 or lse.shape[0] < plan.num_tokens or lse.shape[1:] != (self.h_q,)
+        if lse is not None and (lse.dtype != torch.float32 or lse.shape[0] < tokens or lse.shape[1:] != (self.h_q,)
                                 or not lse.is_contiguous()):
             raise ValueError("lse must be a contiguous fp32 (tokens, h_q)")
-        _on(self.status.device, query, out, k_cache, lse)
-        a.num_seqs, a.h_q, a.num_tokens, a.dtype = len(plan.query_lens), self.h_q, plan.num_tokens, dtype_code(query.dtype)
-        a.q, a.q_stride_tok, a.q_stride_head = query.data_ptr(), query.stride(0), query.stride(1)
-        a.o, a.o_stride_tok, a.o_stride_head = out.data_ptr(), out.stride(0), out.stride(1)
-        bt = plan.block_table
-        a.block_table, a.block_table_stride, a.block_table_cols = bt.data_ptr(), bt.stride(0), bt.shape[1]
-        a.seq_lens, a.q_start, a.lse = plan.seq_lens.data_ptr(), plan.q_start.data_ptr(), _ptr(lse)
-        a.softmax_scale, a.causal, a.status = float(softmax_scale), int(plan.causal), self.status.data_ptr()
-        a.work, a.num_work, a.merges, a.num_merges = plan.work.data_ptr(), len(plan.work), plan.merges.data_ptr(), len(plan.merges)
-        a.o_part, a.lse_part, a.num_slots = self.o_part.data_ptr(), self.lse_part.data_ptr(), plan.num_slots
-        with torch.cuda.device(self.status.device):
-            _lib.block_attention(a, _stream(self.status.device))
+        dev = self.status.device
+        _on(dev, query, out, k_cache, lse)
+        bt, scale, causal = plan.block_table, float(softmax_scale), int(plan.causal)
+        cache = (k_cache.data_ptr(), v_cache.data_ptr(), *st)
+        scales = (k_scales.data_ptr(), v_scales.data_ptr())
+        if plan.decode is not None:
+            p, r = plan.decode, self.decode
+            one = self.one.data_ptr()
+            call(_lib.decode, _lib.DecodeArgs(
+                p.num_seqs, p.q_len, self.h_q, h_k, d, page_size, kv_format, query.data_ptr(), dt, *qs, out.data_ptr(), dt,
+                *os_, *cache, pages, bt.data_ptr(), bt.stride(0), plan.seq_lens.data_ptr(), p.work.data_ptr(), p.num_work,
+                p.n_splits.data_ptr(), r.max_splits, r.o_part.data_ptr(), r.lse_part.data_ptr(), self.max_num_seqs, _ptr(lse),
+                one, _lib.MJ_SCALE_TENSOR, one, _lib.MJ_SCALE_TENSOR, None, None, scale, causal, int(p.with_reduction),
+                r.kernel, r.status.data_ptr(), r.merge_counters.data_ptr() if r.merges(p) else None, *scales, *ss, 0), dev)
+        if plan.work is not None:
+            call(_lib.block_attention, _lib.BlockAttnArgs(
+                len(plan.query_lens), self.h_q, h_k, d, page_size, kv_format, dt, query.data_ptr(), *qs, out.data_ptr(), *os_,
+                tokens, *cache, *scales, *ss, pages, bt.data_ptr(), bt.stride(0), bt.shape[1], plan.seq_lens.data_ptr(),
+                plan.q_start.data_ptr(), _ptr(lse), scale, causal, plan.work.data_ptr(), plan.work.shape[0],
+                plan.merges.data_ptr(), plan.merges.shape[0], self.o_part.data_ptr(), self.lse_part.data_ptr(),
+                plan.num_slots, self.status.data_ptr()), dev)
         return out
 
     def check_status(self) -> None:

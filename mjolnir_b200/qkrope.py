@@ -11,15 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .runner import _ptr, _stream, dtype_code
-
-
-def _rows(name: str, t: torch.Tensor, like: torch.Tensor | None = None) -> torch.Tensor:
-    if t.dim() != 3 or t.stride(2) != 1:
-        raise ValueError(f"{name} must be (tokens, heads, head_size) with a contiguous head dim, got {tuple(t.shape)}")
-    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
-        raise ValueError(f"{name} {tuple(t.shape)} {t.dtype} does not match {tuple(like.shape)} {like.dtype}")
-    return t
+from .runner import _ptr, call, dtype_code
 
 
 def qk_norm_rope(
@@ -39,38 +31,40 @@ def qk_norm_rope(
     """Normalise and rotate Q and K; returns ``(q_out, k_out)``. A position
     outside the table flags ``MJ_DEV_BAD_POSITION`` in ``status`` and leaves
     its token's output rows as they were."""
-    _rows("q", q)
-    _rows("k", k)
-    T, h_q, d = q.shape
-    if k.shape[0] != T or k.shape[2] != d or k.dtype != q.dtype or k.device != q.device:
-        raise ValueError(f"k {tuple(k.shape)} {k.dtype} does not match q {tuple(q.shape)} {q.dtype}")
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else _rows("q_out", q_out, q)
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k_out is None else _rows("k_out", k_out, k)
+    shape, dtype, dev = q.shape, q.dtype, q.device
+    if len(shape) != 3 or len(k.shape) != 3:
+        raise ValueError(f"q {tuple(shape)} and k {tuple(k.shape)} must be (tokens, heads, head_size)")
+    T, h_q, d = shape
+    h_k = k.shape[1]
+    if k.shape[0] != T or k.shape[2] != d or k.dtype != dtype:
+        raise ValueError(f"k {tuple(k.shape)} {k.dtype} does not match q {tuple(shape)} {dtype}")
+    if q_out is None:
+        q_out = torch.empty(shape, dtype=dtype, device=dev)
+    if k_out is None:
+        k_out = torch.empty(k.shape, dtype=dtype, device=dev)
+    if q_out.shape != shape or q_out.dtype != dtype or k_out.shape != k.shape or k_out.dtype != dtype:
+        raise ValueError(f"q_out {tuple(q_out.shape)} {q_out.dtype} / k_out {tuple(k_out.shape)} {k_out.dtype} do not match q and k")
+    qs, ks, qos, kos = q.stride(), k.stride(), q_out.stride(), k_out.stride()
+    if qs[2] != 1 or ks[2] != 1 or qos[2] != 1 or kos[2] != 1:
+        raise ValueError("the head dim of q, k and the outputs must be contiguous")
     if positions.dtype != torch.int64 or positions.shape != (T,) or (T > 1 and positions.stride(0) != 1):
         raise ValueError(f"positions must be a contiguous int64 ({T},), got {positions.dtype} {tuple(positions.shape)}")
     if cos_sin.dim() != 2 or (cos_sin.shape[1] > 1 and cos_sin.stride(1) != 1):
         raise ValueError(f"cos_sin must be (positions, rot_dim) with contiguous rows, got {tuple(cos_sin.shape)}")
-    weights = [w for w in (q_weight, k_weight) if w is not None]
-    for w in weights:
-        if w.shape != (d,) or not w.is_contiguous() or w.dtype != weights[0].dtype:
-            raise ValueError(f"norm weights must be contiguous ({d},) of one dtype, got {tuple(w.shape)} {w.dtype}")
-    for t in (k, positions, cos_sin, *weights, *([] if status is None else [status])):
-        if t.device != q.device:
-            raise ValueError(f"every tensor must be on {q.device}, got {t.device}")
-    a = _lib.QkNormRopeArgs()
-    a.q, a.k, a.q_out, a.k_out = q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr()
-    a.dtype, a.num_tokens, a.h_q, a.h_k = dtype_code(q.dtype), T, h_q, k.shape[1]
-    a.head_size, a.rot_dim, a.interleaved = d, cos_sin.shape[1], int(interleaved)
-    a.q_stride_tok, a.q_stride_head, _ = q.stride()
-    a.k_stride_tok, a.k_stride_head, _ = k.stride()
-    a.qo_stride_tok, a.qo_stride_head, _ = q_out.stride()
-    a.ko_stride_tok, a.ko_stride_head, _ = k_out.stride()
-    a.positions, a.cos_sin, a.cos_sin_dtype = positions.data_ptr(), cos_sin.data_ptr(), dtype_code(cos_sin.dtype)
-    a.cos_sin_stride, a.num_positions = cos_sin.stride(0), cos_sin.shape[0]
-    a.q_weight, a.k_weight = _ptr(q_weight), _ptr(k_weight)
-    a.weight_dtype = dtype_code(weights[0].dtype) if weights else _lib.MJ_DT_FP32
-    a.eps = float(eps)
-    a.status = _ptr(status)
-    with torch.cuda.device(q.device):
-        _lib.qk_norm_rope(a, _stream(q.device))
+    w_dtype = torch.float32
+    for w in (q_weight, k_weight):
+        if w is not None:
+            if w.shape != (d,) or not w.is_contiguous():
+                raise ValueError(f"norm weights must be contiguous ({d},), got {tuple(w.shape)}")
+            w_dtype = w.dtype
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise ValueError(f"norm weights must share a dtype, got {q_weight.dtype} and {k_weight.dtype}")
+    for t in (k, q_out, k_out, positions, cos_sin, q_weight, k_weight, status):
+        if t is not None and t.device != dev:
+            raise ValueError(f"every tensor must be on {dev}, got {t.device}")
+    call(_lib.qk_norm_rope, _lib.QkNormRopeArgs(
+        q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), dtype_code(dtype), T, h_q, h_k, d, cos_sin.shape[1],
+        int(interleaved), qs[0], qs[1], ks[0], ks[1], qos[0], qos[1], kos[0], kos[1], positions.data_ptr(), cos_sin.data_ptr(),
+        dtype_code(cos_sin.dtype), cos_sin.stride(0), cos_sin.shape[0], _ptr(q_weight), _ptr(k_weight), dtype_code(w_dtype),
+        float(eps), _ptr(status)), dev)
     return q_out, k_out

@@ -235,6 +235,16 @@ def _stream(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def call(entry, args, device: torch.device) -> None:
+    """Run a library entry point on ``device``'s current stream, with that
+    device current."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        entry(args, _stream(device))
+    else:
+        with torch.cuda.device(device):
+            entry(args, _stream(device))
+
+
 class DecodeRunner:
     """The B200 decode runner (the counterpart of the reference's
     ``T5DecodeRunner``, ``arch/thor/runner.py:84``).
