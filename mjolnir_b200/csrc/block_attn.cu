@@ -33,7 +33,6 @@
 
 #include <atomic>
 #include <mutex>
-#include <utility>
 
 #include "block_cache.cuh"
 
@@ -73,17 +72,6 @@ struct Cfg {
 
 // byte offset of 16-byte unit u of row r in a [rows][64 f16] swizzled block
 __device__ __forceinline__ uint32_t unit_offset(uint32_t r, uint32_t u) { return r * 128 + ((u ^ (r & 7)) << 4); }
-
-template <int D, int BN, int... K>
-__device__ __forceinline__ void issue_qk(uint32_t s, uint32_t q, uint32_t k, uint32_t hi, uint32_t idesc,
-                                         std::integer_sequence<int, K...>) {
-  (mma_f16_ss<(K >> 2) * (128 * 8) + (K & 3) * 2, (K >> 2) * (BN * 8) + (K & 3) * 2>(s, q, k, hi, idesc, K > 0), ...);
-}
-template <int... K>
-__device__ __forceinline__ void issue_pv(uint32_t o, uint32_t p, uint32_t v, uint32_t hi, uint32_t idesc, bool accumulate,
-                                         std::integer_sequence<int, K...>) {
-  (mma_f16_ts<8 * K, 128 * K>(o, p, v, hi, idesc, accumulate || K > 0), ...);
-}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __grid_constant__ mj_block_attn_args a, int lg) {
@@ -146,7 +134,12 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  // all 512 columns, so the base is column 0, and TMEM addresses are constants
+  if (*tmem_slot != 0) {  // uniform, and cannot happen
+    if (threadIdx.x == 0) flag(a.status, MJ_DEV_BAD_SPLIT);
+    if (warp == 0) tmem_dealloc(*tmem_slot, C::TMEM_COLS);
+    return;
+  }
   auto give_up = [&]() {
     *abort_flag = 1;
     flag(a.status, MJ_DEV_TIMEOUT);
@@ -163,48 +156,61 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
 
   if (warp < 4) {
     if constexpr (C::REG_MMA > 0) setmaxnreg_dec<C::REG_MMA>();
-    if (warp == 0 && lane == 0) {
+    if (warp == 0) {
       // ------------------------------------------------------------ MMA issuer
-      constexpr uint32_t idesc_s = idesc_f16(0, 0, BN), idesc_o = idesc_f16(0, 1, D);
-      constexpr uint32_t hi = desc_hi_sw128(1024);
-      const uint32_t q_lo = desc_lo(smem_addr(sm), 16), k_lo = desc_lo(smem_addr(sm + C::K_OFF), 16),
-                     v_lo = desc_lo(smem_addr(sm + C::V_OFF), BN * 128);
+      // (the whole warp runs the loop, one lane issues: see elect_one)
+      const bool lead = elect_one();
       auto qk = [&](int w, int j) {  // 16 head-dim elements a step, 64 a swizzled block
-        issue_qk<D, BN>(tmem + s_col(w, j), q_lo + w * (C::QTILE / 16), k_lo + (j & 1) * (C::KTILE / 16), hi, idesc_s,
-                        std::make_integer_sequence<int, D / 16>());
-        mma_commit(&s_full[s_bar(w, j)]);
+        constexpr uint32_t idesc = idesc_f16(0, 0, BN);
+        const uint64_t q = smem_desc_sw128(smem_addr(sm + w * C::QTILE), 16, 1024),
+                       k = smem_desc_sw128(smem_addr(sm + C::K_OFF + (j & 1) * C::KTILE), 16, 1024);
+        if (lead) {
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i)
+            mma_f16_ss(s_col(w, j), q + (i >> 2) * (128 * 8) + (i & 3) * 2, k + (i >> 2) * (BN * 8) + (i & 3) * 2, idesc, i > 0);
+          mma_commit(&s_full[s_bar(w, j)]);
+        }
       };
       auto pv = [&](int w, int j) {  // 16 tokens a step: two 8-row atoms of V, 8 columns of P
-        issue_pv(tmem + C::O_COL + w * 128, tmem + s_col(w, j), v_lo + (j & 1) * (C::KTILE / 16), hi, idesc_o, j > 0,
-                 std::make_integer_sequence<int, BN / 16>());
-        mma_commit(&o_full[2 * w + (j & 1)]);
+        constexpr uint32_t idesc = idesc_f16(0, 1, D);
+        const uint64_t v = smem_desc_sw128(smem_addr(sm + C::V_OFF + (j & 1) * C::KTILE), BN * 128, 1024);
+        if (lead) {
+#pragma unroll
+          for (int i = 0; i < BN / 16; ++i)
+            mma_f16_ts(C::O_COL + w * 128, s_col(w, j) + i * 8, v + i * 128, idesc, j > 0 || i > 0);
+          mma_commit(&o_full[2 * w + (j & 1)]);
+        }
+      };
+      auto commit = [&](uint64_t* bar) {
+        if (lead) mma_commit(bar);
       };
       bool ok = n > 0 && wait(q_full, 0) && wait(&k_full[0], 0);
+      ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         tc_fence_after();
         for (int w = 0; w < na; ++w) qk(w, 0);
-        mma_commit(&k_empty[0]);
+        commit(&k_empty[0]);
       }
       for (int j = 0; ok && j < n; ++j) {
         const bool more = j + 1 < n;
-        if (more) ok = wait(&k_full[(j + 1) & 1], (j + 1) >> 1);
+        if (more) ok = __all_sync(0xffffffffu, wait(&k_full[(j + 1) & 1], (j + 1) >> 1));
         if (NT == 1 && ok && more) {
           tc_fence_after();
           qk(0, j + 1);
-          mma_commit(&k_empty[(j + 1) & 1]);
+          commit(&k_empty[(j + 1) & 1]);
         }
-        ok = ok && wait(&v_full[j & 1], j >> 1);
+        ok = ok && __all_sync(0xffffffffu, wait(&v_full[j & 1], j >> 1));
         for (int w = 0; ok && w < na; ++w) {
-          ok = wait(&p_full[s_bar(w, j)], s_phase(j));
+          ok = __all_sync(0xffffffffu, wait(&p_full[s_bar(w, j)], s_phase(j)));
           if (!ok) break;
           tc_fence_after();
           pv(w, j);
-          if (w == na - 1) mma_commit(&v_empty[j & 1]);
+          if (w == na - 1) commit(&v_empty[j & 1]);
           if (NT == 2 && more) qk(w, j + 1);  // over S and P of tile j: behind its product, in issue order
         }
-        if (NT == 2 && ok && more) mma_commit(&k_empty[(j + 1) & 1]);
+        if (NT == 2 && ok && more) commit(&k_empty[(j + 1) & 1]);
       }
-      mma_commit(drain);  // all issued MMAs complete before TMEM is released
+      commit(drain);  // all issued MMAs complete before TMEM is released
       mbar_wait(drain, 0, &never_abort, kWaitNs);
     }
     __syncwarp();
@@ -361,7 +367,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
       // first tile sees none at all (keys are a prefix) and keeps P = 0
       float nm = 0.f, l = 0.f;
       bool ok = true;
-      const uint32_t o_addr = tmem + C::O_COL + w * 128 + lane_base;
+      const uint32_t o_addr = C::O_COL + w * 128 + lane_base;
       for (int j = 0; j < n; ++j) {
         ok = wait(&sc_full[j & 3], j >> 2) && wait(&s_full[s_bar(w, j)], s_phase(j));
         // every thread leaves the loop with its warp: the collectives below
@@ -370,7 +376,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
           break;
         }
         tc_fence_after();
-        const uint32_t s_addr = tmem + s_col(w, j) + lane_base;
+        const uint32_t s_addr = s_col(w, j) + lane_base;
         float2 s[BN / 2];
 #pragma unroll
         for (int c = 0; c < BN / 32; ++c) tmem_ld32(s_addr + 32 * c, reinterpret_cast<float*>(s) + 32 * c);
@@ -480,7 +486,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
   __syncthreads();
   if (warp == 0) {
     tc_fence_after();
-    tmem_dealloc(tmem, C::TMEM_COLS);
+    tmem_dealloc(0, C::TMEM_COLS);
   }
 }
 

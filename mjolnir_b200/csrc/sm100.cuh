@@ -277,33 +277,37 @@ __device__ __forceinline__ void mma_f8f6f4(uint32_t d_tmem, uint64_t a_desc, uin
 }
 
 // kind::f16, both operands f16: A in shared memory, or in TMEM (row i in lane
-// i, two elements a column). Shared-memory descriptors as their low words (see
-// desc_lo) plus a compile-time offset in 16-byte units and the common high
-// word, put together here: built outside, the unrolled issue loops' descriptors
-// are hoisted and spilled, and each issue waits for them.
-template <int AO, int BO>
-__device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc,
+// i, two elements a column).
+__device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                            uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b32 x, y;\n\t.reg .b64 a, b;\n\t"
-      "setp.ne.b32 p, %5, 0;\n\t"
-      "add.u32 x, %1, %6;\n\tadd.u32 y, %2, %7;\n\t"
-      "mov.b64 a, {x, %3};\n\tmov.b64 b, {y, %3};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate), "n"(AO), "n"(BO)
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-template <int AO, int BO>
-__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t hi, uint32_t idesc,
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
                                            uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b32 x, y;\n\t.reg .b64 b;\n\t"
-      "setp.ne.b32 p, %5, 0;\n\t"
-      "add.u32 x, %1, %6;\n\tadd.u32 y, %2, %7;\n\t"
-      "mov.b64 b, {y, %3};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %4, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate), "n"(AO), "n"(BO)
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+
+// One lane of a converged warp. A warp that runs an issue loop as a whole and
+// issues through this keeps the loop's addresses and descriptors in uniform
+// registers; in a one-thread branch each MMA first moves them there.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
 }
 
 // Arrive on `bar` once every tcgen05.mma issued so far by this thread has completed.
@@ -337,13 +341,6 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr, uint32_t lbo
   d |= (uint64_t)2 << 61;  // SWIZZLE_128B
   return d;
 }
-
-// The same descriptor as two words: the low one holds the address and lbo, the
-// high one sbo, the version and the swizzle.
-__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) {
-  return ((saddr & 0x3FFFFu) >> 4) | (((lbo >> 4) & 0x3FFFu) << 16);
-}
-__host__ __device__ constexpr uint32_t desc_hi_sw128(uint32_t sbo) { return ((sbo >> 4) & 0x3FFFu) | (1u << 14) | (2u << 29); }
 
 // Shared-memory matrix descriptor without swizzle (canonical "interleaved"
 // layout of 8-row x 16-byte core matrices), sm_100 version 1.
