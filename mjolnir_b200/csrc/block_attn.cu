@@ -4,14 +4,19 @@
 // A CTA takes one work item of one KV head: NT tiles of 128 rows -- a row is
 // (query token, head of the KV head's group), so a group shares every key read
 // -- and a range of key tiles of BN tokens. Warp roles:
-//   converter warpgroup  page-table walk, 16-byte code loads one operand ahead
-//                        in registers, e4m3 -> f16 (exact), 128-byte swizzled
-//                        K (K-major) and V (MN-major) tiles in two-stage rings;
+//   loader warps         one for K, one for V: page-table walk, 16-byte async
+//                        copies of the next tile's codes into a staging tile
+//   converter warpgroup  staged e4m3 -> f16 (exact), 128-byte swizzled K
+//                        (K-major) and V (MN-major) tiles in two-stage rings;
 //                        also the tile's block scales
 //   MMA thread           S = Q K^T (both from shared memory), O += P V (P from
 //                        TMEM, over the columns of the S it came from)
-//   NT softmax warpgroups  thread = row: S to registers, online softmax in base
-//                        2, P back to TMEM as f16
+//   softmax warpgroups   two per row tile, a thread = a row's half of the key
+//                        tile: S to registers, online softmax in base 2, P back
+//                        to TMEM as f16. Half a row a thread puts four softmax
+//                        warps on each SM sub-partition: with a whole row a
+//                        thread (two warps) a tile's softmax took 3800 cycles of
+//                        latency beside 1024 of MMA and the tensor cores idled
 // With NT = 2 the tiles take turns: while one is in its softmax the tensor
 // cores run the other's products. With NT = 1 (head_size 256, whose O takes
 // half of TMEM) S is double-buffered and the next tile's product runs instead.
@@ -55,23 +60,34 @@ struct Cfg {
   static constexpr int BN = MJ_BLOCK_KEYS(D);
   static constexpr int ROWS = NT * 128;
   static_assert(ROWS == MJ_BLOCK_ROWS(D), "the plan's rows");
-  static constexpr int THREADS = 256 + 128 * NT;
+  static constexpr int THREADS = 256 + 256 * NT;
   static constexpr int QTILE = 128 * D * 2, KTILE = BN * D * 2;
-  static constexpr int K_OFF = NT * QTILE, V_OFF = K_OFF + 2 * KTILE, SC_OFF = V_OFF + 2 * KTILE;
+  static constexpr int RAW = BN * D;  // one operand's codes
+  static constexpr int K_OFF = NT * QTILE, V_OFF = K_OFF + 2 * KTILE, RAW_OFF = V_OFF + 2 * KTILE, SC_OFF = RAW_OFF + 2 * RAW;
   static constexpr int SC_BYTES = 4 * (BN / 16) * 16;  // four tiles' float4 per 16 tokens
   static constexpr int BAR_OFF = SC_OFF + SC_BYTES;
-  static constexpr int NBARS = 8 + 4 + 2 + 2 + 4 + 2;
+  static constexpr int NBARS = 8 + 4 + 2 + 2 + 4 + 2 + 4;
   static constexpr int MISC_OFF = BAR_OFF + NBARS * 8;
-  static constexpr int SMEM = MISC_OFF + 64;
+  static constexpr int RED_OFF = MISC_OFF + 64;  // float [2 NT][128]: what the two halves of a row exchange
+  static constexpr int SMEM = RED_OFF + 2 * NT * 128 * 4;
+  static_assert(SMEM <= 232448, "shared memory of a CTA");
   static constexpr int TMEM_COLS = 512;
   static constexpr int O_COL = 256;
-  // 512 threads share 65536 registers: the MMA warpgroup gives most of its up
-  static constexpr int REG_MMA = NT == 2 ? 40 : 0, REG_CVT = NT == 2 ? 96 : 0, REG_SM = NT == 2 ? 184 : 0;
-  static constexpr int REG_POOL = 128 * REG_MMA + 128 * REG_CVT + 128 * NT * REG_SM;
+  // 768 threads launch with 80 registers each: the MMA warpgroup gives most of its up
+  static constexpr int REG_MMA = NT == 2 ? 40 : 0, REG_CVT = NT == 2 ? 88 : 0, REG_SM = NT == 2 ? 88 : 0;
+  static constexpr int REG_LAUNCH = NT == 2 ? 80 : 0;
+  static_assert(REG_MMA <= REG_LAUNCH && REG_CVT >= REG_LAUNCH && REG_SM >= REG_LAUNCH, "directions of the changes");
+  static constexpr int REG_POOL = 128 * REG_MMA + 128 * REG_CVT + 256 * NT * REG_SM;
 };
 
 // byte offset of 16-byte unit u of row r in a [rows][64 f16] swizzled block
 __device__ __forceinline__ uint32_t unit_offset(uint32_t r, uint32_t u) { return r * 128 + ((u ^ (r & 7)) << 4); }
+
+// byte offset of 16-code chunk c of row r in a staging tile: odd rows swap the
+// halves of each 128 bytes, so four chunks of two neighbouring rows cover all
+// banks
+template <int D>
+__device__ __forceinline__ uint32_t raw_offset(uint32_t r, uint32_t c) { return r * D + ((c ^ ((r & 1) << 2)) << 4); }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __grid_constant__ mj_block_attn_args a, int lg) {
@@ -81,7 +97,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::BAR_OFF);
   uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6, *sc_full = bars + 8,
-           *s_full = bars + 12, *p_full = bars + 14, *o_full = bars + 16, *q_full = bars + 20, *drain = bars + 21;
+           *s_full = bars + 12, *p_full = bars + 14, *o_full = bars + 16, *q_full = bars + 20, *drain = bars + 21, *raw_full = bars + 22, *raw_empty = bars + 24;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::MISC_OFF);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + C::MISC_OFF + 4);
   int& never_abort = *reinterpret_cast<int*>(sm + C::MISC_OFF + 8);
@@ -115,13 +131,15 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
       mbar_init(&v_full[i], 128);
       mbar_init(&v_empty[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
+      mbar_init(&raw_full[i], 32);
+      mbar_init(&raw_empty[i], 128);
+      mbar_init(&p_full[i], 256);
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&sc_full[i], 1);
       mbar_init(&o_full[i], 1);
     }
-    mbar_init(q_full, 128 * na);
+    mbar_init(q_full, 256 * na);
     mbar_init(drain, 1);
     *abort_flag = 0;
     never_abort = 0;
@@ -153,6 +171,21 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
   auto s_col = [&](int w, int j) { return (uint32_t)(NT == 2 ? w * 128 : (j & 1) * BN); };
   auto s_bar = [&](int w, int j) { return NT == 2 ? w : j & 1; };
   auto s_phase = [&](int j) { return NT == 2 ? j : j >> 1; };
+
+  // Page-table walk. An entry is loaded before it is needed and checked then:
+  // checking it at once would wait a memory round trip.
+  constexpr int kNone = INT_MIN;  // past the sequence or the item
+  const int base = tb * BN, pmask = a.page_size - 1;
+  auto entry_of = [&](int pos) -> int {
+    if (pos >= L || pos >= base + n * BN) return kNone;
+    const int c = pos >> (31 - __clz(a.page_size));
+    return c < a.block_table_cols ? __ldg(a.block_table + seq * a.block_table_stride + c) : -1;
+  };
+  auto page_of = [&](int e) -> int {  // -1: no such token, or a bad entry
+    if ((unsigned)e < (unsigned)a.num_pages) return e;
+    if (e != kNone) flag(a.status, MJ_DEV_BAD_PAGE);
+    return -1;
+  };
 
   if (warp < 4) {
     if constexpr (C::REG_MMA > 0) setmaxnreg_dec<C::REG_MMA>();
@@ -212,32 +245,38 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
       }
       commit(drain);  // all issued MMAs complete before TMEM is released
       mbar_wait(drain, 0, &never_abort, kWaitNs);
+    } else if (warp < 3) {
+      // -------------------------------------------- loaders: warp 1 K, warp 2 V
+      const int side = warp - 1;
+      constexpr int CPR = D / 16, STEP = 32 / CPR;
+      const unsigned char* src = static_cast<const unsigned char*>(side ? a.v_cache : a.k_cache) +
+                                 h * (side ? a.v_stride_head : a.k_stride_head) + (lane % CPR) * 16;
+      const int64_t sp = side ? a.v_stride_page : a.k_stride_page, sr = side ? a.v_stride_row : a.k_stride_row;
+      unsigned char* raw = sm + C::RAW_OFF + side * C::RAW;
+      // lane i < BN / 16 holds the table entry of the tile's 16-token group i
+      auto entries = [&](int j) { return lane < BN / 16 ? entry_of(base + j * BN + lane * 16) : kNone; };
+      int next = n > 0 ? entries(0) : kNone;
+      for (int j = 0; j < n; ++j) {
+        const int page = page_of(next);
+        next = entries(j + 1);
+        const bool ok = wait(&raw_empty[side], j + 1);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        const int t0 = base + j * BN;
+#pragma unroll 4
+        for (int r = lane / CPR; r < BN; r += STEP) {
+          const int p = __shfl_sync(0xffffffffu, page, r >> 4);
+          const bool there = p >= 0 && t0 + r < L;  // rows past the sequence become zeros
+          cp_async16(raw + raw_offset<D>(r, lane % CPR), there ? src + p * sp + ((t0 + r) & pmask) * sr : src, there ? 16u : 0u);
+        }
+        cp_async_arrive_noinc(&raw_full[side]);
+      }
+      cp_async_wait_all();  // copies land before the CTA exits
     }
     __syncwarp();
   } else if (warp < 8) {
     // ------------------------------------------------------- converter warpgroup
-    if constexpr (C::REG_CVT > 0) setmaxnreg_dec<C::REG_CVT>();
+    if constexpr (C::REG_CVT > 0) setmaxnreg_inc<C::REG_CVT>();
     const int ct = threadIdx.x - 128;
-    constexpr int CPR = D / 16, STEP = 128 / CPR, NC = BN / STEP;  // 16-code chunks of a row; rows of a pass; passes
-    const int col = ct % CPR, r0 = ct / CPR, base = tb * BN;
-    const int32_t* table = a.block_table + seq * a.block_table_stride;
-    const int ps_log2 = 31 - __clz(a.page_size), pmask = a.page_size - 1;
-    const unsigned char* kbase = static_cast<const unsigned char*>(a.k_cache) + h * a.k_stride_head + col * 16;
-    const unsigned char* vbase = static_cast<const unsigned char*>(a.v_cache) + h * a.v_stride_head + col * 16;
-    // The table entry of token `pos` is loaded an operand before it is checked:
-    // checking it at once would wait a memory round trip for every row.
-    constexpr int kNone = INT_MIN;  // past the sequence
-    const int last = base + n * BN;  // tokens from here on are not this item's
-    auto entry_of = [&](int pos) -> int {
-      if (pos >= L || pos >= last) return kNone;
-      const int c = pos >> ps_log2;
-      return c < a.block_table_cols ? __ldg(table + c) : -1;
-    };
-    auto page_of = [&](int e) -> int {  // -1: no such token, or a bad entry
-      if ((unsigned)e < (unsigned)a.num_pages) return e;
-      if (e != kNone) flag(a.status, MJ_DEV_BAD_PAGE);
-      return -1;
-    };
     // block scales of the tile's 16-token groups: thread ct < BN / 16 looks the
     // page up two tiles ahead and reads the two exponents one tile ahead
     constexpr uint32_t kOne = 127u | (127u << 8);
@@ -248,26 +287,6 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
       return __ldg(static_cast<const unsigned char*>(a.k_scales) + p * a.ks_stride_page + b * a.ks_stride_block + h * a.ks_stride_head) |
              ((uint32_t)__ldg(static_cast<const unsigned char*>(a.v_scales) + p * a.vs_stride_page + b * a.vs_stride_block + h * a.vs_stride_head) << 8);
     };
-    uint4 data[NC];
-    int page[NC];
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    auto load_k = [&](int pos, int p) { return p < 0 ? zero : __ldg(reinterpret_cast<const uint4*>(kbase + p * a.k_stride_page + (pos & pmask) * a.k_stride_row)); };
-    auto load_v = [&](int pos, int p) { return p < 0 ? zero : __ldg(reinterpret_cast<const uint4*>(vbase + p * a.v_stride_page + (pos & pmask) * a.v_stride_row)); };
-    // 16 codes -> two 16-byte units of f16; the threads of odd 64-column blocks
-    // store their odd unit first, so that 8 threads of a row cover all banks
-    const uint32_t block_at = (uint32_t)(col >> 2) * (BN * 128), unit = (uint32_t)(col & 3) * 2, odd = (uint32_t)(col >> 2) & 1;
-    auto store = [&](unsigned char* buf, int r, uint4 d) {
-      const uint32_t w[4] = {d.x, d.y, d.z, d.w};
-      uint32_t o[8];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        o[2 * i] = e4m3x2_to_h2((uint16_t)w[i]);
-        o[2 * i + 1] = e4m3x2_to_h2((uint16_t)(w[i] >> 16));
-      }
-      const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
-      *reinterpret_cast<uint4*>(buf + block_at + unit_offset(r, unit + odd)) = odd ? hi : lo;
-      *reinterpret_cast<uint4*>(buf + block_at + unit_offset(r, unit + 1 - odd)) = odd ? lo : hi;
-    };
     int sc_entry = kNone;
     uint32_t sc_next = kOne;
     if (scaler) {
@@ -275,12 +294,36 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
       sc_entry = entry_of(base + BN + ct * 16);
       sc_next = exponents(base + ct * 16, page_of(e0));
     }
+    // Thread ct takes 16-code chunk `col` of rows r0, r0 + STEP, ...: eight
+    // neighbouring threads are four chunks of a 64-element block in two rows, so
+    // both their staged reads and their swizzled stores cover all banks.
+    constexpr int BLOCKS = D / 64, STEP = 32 / BLOCKS, NC = BN / STEP;
+    const int quad = ct & 3, blk = (ct >> 3) % BLOCKS, r0 = ((ct >> 2) & 1) + 2 * ((ct >> 3) / BLOCKS);
+    auto convert = [&](int side, int j, uint64_t* empty, uint64_t* full) -> bool {
+      if (!wait(&raw_full[side], j)) return false;
+      const unsigned char* raw = sm + C::RAW_OFF + side * C::RAW;
+      uint4 d[NC];
 #pragma unroll
-    for (int i = 0; i < NC; ++i) page[i] = entry_of(base + r0 + i * STEP);
+      for (int i = 0; i < NC; ++i) d[i] = *reinterpret_cast<const uint4*>(raw + raw_offset<D>(r0 + i * STEP, 4 * blk + quad));
+      mbar_arrive(&raw_empty[side]);
+      if (!wait(&empty[j & 1], (j >> 1) + 1)) return false;
+      unsigned char* out = sm + (side ? C::V_OFF : C::K_OFF) + (j & 1) * C::KTILE + blk * (BN * 128);
 #pragma unroll
-    for (int i = 0; i < NC; ++i) page[i] = page_of(page[i]);
+      for (int i = 0; i < NC; ++i) {
+        const uint32_t w[4] = {d[i].x, d[i].y, d[i].z, d[i].w};
+        uint32_t o[8];
 #pragma unroll
-    for (int i = 0; i < NC; ++i) data[i] = load_k(base + r0 + i * STEP, page[i]);
+        for (int k = 0; k < 4; ++k) {
+          o[2 * k] = e4m3x2_to_h2((uint16_t)w[k]);
+          o[2 * k + 1] = e4m3x2_to_h2((uint16_t)(w[k] >> 16));
+        }
+        *reinterpret_cast<uint4*>(out + unit_offset(r0 + i * STEP, 2 * quad)) = make_uint4(o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<uint4*>(out + unit_offset(r0 + i * STEP, 2 * quad + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&full[j & 1]);
+      return true;
+    };
     for (int j = 0; j < n; ++j) {
       const int t0 = base + j * BN;
       if (scaler) {
@@ -294,35 +337,18 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
         __syncwarp();
         if (ct == 0) mbar_arrive(&sc_full[j & 3]);
       }
-      if (!wait(&k_empty[j & 1], (j >> 1) + 1)) break;
-      unsigned char* kb = sm + C::K_OFF + (j & 1) * C::KTILE;
-#pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        const int r = r0 + i * STEP;
-        store(kb, r, data[i]);
-        data[i] = load_v(t0 + r, page[i]);
-        page[i] = entry_of(t0 + BN + r);
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(&k_full[j & 1]);
-      if (!wait(&v_empty[j & 1], (j >> 1) + 1)) break;
-      unsigned char* vb = sm + C::V_OFF + (j & 1) * C::KTILE;
-#pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        const int r = r0 + i * STEP;
-        store(vb, r, data[i]);
-        page[i] = page_of(page[i]);
-        data[i] = load_k(t0 + BN + r, page[i]);
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(&v_full[j & 1]);
+      if (!convert(0, j, k_empty, k_full) || !convert(1, j, v_empty, v_full)) break;
     }
   } else {
     if constexpr (C::REG_SM > 0) setmaxnreg_inc<C::REG_SM>();
     // ------------------------------------------------------- softmax warpgroups
-    const int w = NT == 1 ? 0 : (warp - 8) >> 2;
-    const int t = (threadIdx.x - 256) & 127;
+    const int w = NT == 1 ? 0 : (warp - 8) >> 3, half = ((warp - 8) >> 2) & 1;
+    const int t = threadIdx.x & 127;
     if (w < na) {
+      constexpr int HN = BN / 2, HD = D / 2;  // keys of a tile, and head-dim elements, of one half
+      // the two warps that share 32 rows meet in a named barrier of their own
+      const uint32_t pair = 1 + 4 * w + (warp & 3);
+      float* red = reinterpret_cast<float*>(sm + C::RED_OFF) + w * 256;
       const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
       const int R = row0 + w * 128 + t;
       const bool live = R < n_rows;
@@ -330,20 +356,24 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
       const int lim = !live ? -1 : a.causal ? L - n_tok + tok : L - 1;  // the last key this row sees
       // the first row of the warp sees the fewest keys
       const int warp_lim = __shfl_sync(0xffffffffu, lim, 0);
-      // ---- Q: this row as f16 into the K-major tile (dead rows are zeros)
+      // ---- Q: this half row as f16 into the K-major tile (dead rows are zeros)
       float c2 = a.softmax_scale * kLog2e;
       {
-        const T* q = static_cast<const T*>(a.q) + (int64_t)(q0 + tok) * a.q_stride_tok + hq * a.q_stride_head;
-        unsigned char* qs = sm + w * C::QTILE;
+        const T* q = static_cast<const T*>(a.q) + (int64_t)(q0 + tok) * a.q_stride_tok + hq * a.q_stride_head + half * HD;
+        unsigned char* qs = sm + w * C::QTILE + half * (HD / 64) * (128 * 128);
         float up = 1.f;
         if constexpr (std::is_same<T, __nv_bfloat16>::value) {
           float amax = 0.f;
-          for (int c = 0; c < D / 8; ++c) {
+#pragma unroll 4
+          for (int c = 0; c < HD / 8; ++c) {
             float v[8];
             load8(q + 8 * c, v);
 #pragma unroll
             for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[i]));
           }
+          red[half * 128 + t] = amax;
+          named_bar_sync(pair, 64);
+          amax = fmaxf(amax, red[(half ^ 1) * 128 + t]);
           // 2^k with amax 2^k in [2^14, 2^15), inside fp32's normal range
           const int ex = (int)(__float_as_uint(amax) >> 23);
           if (ex > 0 && ex < 255) {
@@ -352,7 +382,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
             c2 *= __uint_as_float((uint32_t)(127 - k) << 23);
           }
         }
-        for (int c = 0; c < D / 8; ++c) {
+#pragma unroll 4
+        for (int c = 0; c < HD / 8; ++c) {
           float v[8];
           load8(q + 8 * c, v);
           uint32_t o[4];
@@ -363,59 +394,66 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
         fence_proxy_async_smem();
         mbar_arrive(q_full);
       }
-      // nm: kHeadroom minus the running maximum; a row that sees no key of the
-      // first tile sees none at all (keys are a prefix) and keeps P = 0
+      // nm: kHeadroom minus the running maximum (the same in both halves); a
+      // row that sees no key of the first tile sees none at all (keys are a
+      // prefix) and keeps P = 0. l: this half's part of the row sum.
       float nm = 0.f, l = 0.f;
       bool ok = true;
-      const uint32_t o_addr = C::O_COL + w * 128 + lane_base;
+      const uint32_t o_addr = C::O_COL + w * 128 + half * HD + lane_base;
       for (int j = 0; j < n; ++j) {
         ok = wait(&sc_full[j & 3], j >> 2) && wait(&s_full[s_bar(w, j)], s_phase(j));
-        // every thread leaves the loop with its warp: the collectives below
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
         tc_fence_after();
         const uint32_t s_addr = s_col(w, j) + lane_base;
-        float2 s[BN / 2];
+        float2 s[HN / 2];
+        __syncwarp();
 #pragma unroll
-        for (int c = 0; c < BN / 32; ++c) tmem_ld32(s_addr + 32 * c, reinterpret_cast<float*>(s) + 32 * c);
+        for (int c = 0; c < HN / 32; ++c) tmem_ld32(s_addr + half * HN + 32 * c, reinterpret_cast<float*>(s) + 32 * c);
         tmem_wait_ld();
-        const float4* sc = reinterpret_cast<const float4*>(sm + C::SC_OFF) + (j & 3) * (BN / 16);
+        const float4* sc = reinterpret_cast<const float4*>(sm + C::SC_OFF) + (j & 3) * (BN / 16) + half * (HN / 16);
 #pragma unroll
-        for (int g = 0; g < BN / 16; ++g) {
+        for (int g = 0; g < HN / 16; ++g) {
           const float4 f = sc[g];
           const float2 m2 = make_float2(c2 * f.x, c2 * f.x), b2 = make_float2(f.y + nm, f.y + nm);
 #pragma unroll
           for (int i = 0; i < 8; ++i) s[8 * g + i] = ffma2(s[8 * g + i], m2, b2);
         }
-        const int j0 = (tb + j) * BN;
-        if (j0 + BN - 1 > warp_lim) {  // some row of the warp sees part of this tile
+        const int j0 = (tb + j) * BN + half * HN;
+        if (j0 + HN - 1 > warp_lim) {  // some row of the warp sees part of this half tile
 #pragma unroll
-          for (int i = 0; i < BN / 2; ++i) {
+          for (int i = 0; i < HN / 2; ++i) {
             if (j0 + 2 * i > lim) s[i].x = -INFINITY;
             if (j0 + 2 * i + 1 > lim) s[i].y = -INFINITY;
           }
         }
-        float mx = -INFINITY;
+        float mx4[4];
 #pragma unroll
-        for (int i = 0; i < BN / 2; ++i) mx = fmaxf(mx, fmaxf(s[i].x, s[i].y));
-        if (__any_sync(0xffffffffu, j == 0 || mx > kRaise)) {
+        for (int i = 0; i < 4; ++i) mx4[i] = fmaxf(s[i].x, s[i].y);
+#pragma unroll
+        for (int i = 4; i < HN / 2; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], fmaxf(s[i].x, s[i].y));
+        float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+        // One barrier per tile between the two halves: both hold their scores
+        // (P goes over the first half's columns), and both learn whether some
+        // row outgrew its maximum, or a wait ran out.
+        if (named_bar_or(pair, 64, j == 0 || mx > kRaise || !ok)) {
+          if (named_bar_or(pair, 64, !ok)) {
+            ok = false;
+            break;
+          }
+          red[half * 128 + t] = mx;
+          named_bar_sync(pair, 64);
+          mx = fmaxf(mx, red[(half ^ 1) * 128 + t]);
           const float up = (j == 0 ? mx > -INFINITY : mx > kRaise) ? kHeadroom - mx : 0.f;  // added to nm
           nm += up;
 #pragma unroll
-          for (int i = 0; i < BN / 2; ++i) s[i] = fadd2(s[i], make_float2(up, up));
+          for (int i = 0; i < HN / 2; ++i) s[i] = fadd2(s[i], make_float2(up, up));
           if (j > 0) {  // O and l follow, once the last product has landed
             const float f = exp2_approx(up);
             l *= f;
             ok = wait(&o_full[2 * w + ((j - 1) & 1)], (j - 1) >> 1);
-            if (!__all_sync(0xffffffffu, ok)) {
-              ok = false;
-              break;
-            }
             tc_fence_after();
+            __syncwarp();
 #pragma unroll 1
-            for (int c = 0; c < D; c += 16) {
+            for (int c = 0; c < HD; c += 16) {
               float o[16];
               tmem_ld16(o_addr + c, o);
               tmem_wait_ld();
@@ -424,9 +462,10 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
               tmem_st16(o_addr + c, reinterpret_cast<const uint32_t*>(o));
             }
           }
+          // red is read before the next raise writes it: the barrier of that tile
         }
 #pragma unroll
-        for (int c = 0; c < BN / 32; ++c) {  // 32 keys: 16 columns of P
+        for (int c = 0; c < HN / 32; ++c) {  // 32 keys: 16 columns of P
           uint32_t p[16];
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
@@ -440,25 +479,25 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
             }
             l = fmaf(sum.x + sum.y, sc[2 * c + g].z, l);
           }
-          tmem_st16(s_addr + 16 * c, p);
+          tmem_st16(s_addr + half * (HN / 2) + 16 * c, p);
         }
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&p_full[s_bar(w, j)]);
       }
-      // ---- epilogue: O / l of this row
-      if (ok && n > 0) {
-        ok = wait(&o_full[2 * w + ((n - 1) & 1)], (n - 1) >> 1);
-        ok = __all_sync(0xffffffffu, ok);
-        tc_fence_after();
-      }
-      if (ok) {
+      // ---- epilogue: this half's head-dim elements of O / l
+      if (ok && n > 0) ok = wait(&o_full[2 * w + ((n - 1) & 1)], (n - 1) >> 1);
+      tc_fence_after();
+      // both halves leave together, and know the whole sum
+      if (!named_bar_or(pair, 64, !ok)) {
+        red[half * 128 + t] = l;
+        named_bar_sync(pair, 64);
+        l += red[(half ^ 1) * 128 + t];
         const float inv = l == 0.f ? 0.f : 1.f / l;  // a NaN sum stays NaN
-        const float lse = l == 0.f ? -INFINITY : (log2f(l) - nm) * kLn2;
         const int64_t part = ((int64_t)slot * a.h_k + h) * C::ROWS + w * 128 + t;
-        T* o = static_cast<T*>(a.o) + (int64_t)(q0 + tok) * a.o_stride_tok + hq * a.o_stride_head;
+        T* o = static_cast<T*>(a.o) + (int64_t)(q0 + tok) * a.o_stride_tok + hq * a.o_stride_head + half * HD;
 #pragma unroll 1
-        for (int c = 0; c < D; c += 16) {
+        for (int c = 0; c < HD; c += 16) {
           float v[16];
           if (n > 0) {
             tmem_ld16(o_addr + c, v);
@@ -471,11 +510,12 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
             store8(o + c + 8, v + 8);
           } else if (live) {
 #pragma unroll
-            for (int i = 0; i < 16; i += 8) store8(a.o_part + part * D + c + i, v + i);
+            for (int i = 0; i < 16; i += 8) store8(a.o_part + part * D + half * HD + c + i, v + i);
           }
           __syncwarp();  // the TMEM load is a whole-warp operation
         }
-        if (live) {
+        if (live && half == 0) {
+          const float lse = l == 0.f ? -INFINITY : (log2f(l) - nm) * kLn2;
           if (slot >= 0) a.lse_part[part] = lse;
           else if (a.lse) a.lse[(int64_t)(q0 + tok) * a.h_q + hq] = lse;
         }
@@ -550,7 +590,7 @@ static cudaError_t launch_t(const mj_block_attn_args& a, cudaStream_t stream) {
     if ((e = cudaFuncGetAttributes(&fa, kern)) != cudaSuccess) return e;
     // the register split must fit the launch allocation, or the softmax
     // warpgroups would wait for registers that never come
-    if (C::REG_POOL > fa.numRegs * C::THREADS) return cudaErrorNotSupported;
+    if (C::REG_LAUNCH && (fa.numRegs != C::REG_LAUNCH || C::REG_POOL > fa.numRegs * C::THREADS)) return cudaErrorNotSupported;
     if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM)) != cudaSuccess) return e;
     ready[dev].store(1, std::memory_order_release);
   }
