@@ -4,100 +4,128 @@
 // A CTA takes one work item of one KV head: NT tiles of 128 rows -- a row is
 // (query token, head of the KV head's group), so a group shares every key read
 // -- and a range of key tiles of BN tokens. Warp roles:
-//   loader warps         one for K, one for V: page-table walk, 16-byte async
-//                        copies of the next tile's codes into a staging tile
-//   converter warpgroup  staged e4m3 -> f16 (exact), 128-byte swizzled K
-//                        (K-major) and V (MN-major) tiles in two-stage rings;
-//                        also the tile's block scales
-//   MMA thread           S = Q K^T (both from shared memory), O += P V (P from
-//                        TMEM, over the columns of the S it came from)
-//   softmax warpgroups   two per row tile, a thread = a row's half of the key
-//                        tile: S to registers, online softmax in base 2, P back
-//                        to TMEM as f16. Half a row a thread puts four softmax
-//                        warps on each SM sub-partition: with a whole row a
-//                        thread (two warps) a tile's softmax took 3800 cycles of
-//                        latency beside 1024 of MMA and the tensor cores idled
+//   K and V producers    one warp each: page-table walk, one TMA box per page
+//   converter warpgroup  staged V codes e4m3 -> f16 (exact) into the MN-major
+//                        operand tiles; also the tile's block scales
+//   MMA warp             S = Q K^T (kind::f8f6f4, K as stored), O += P V
+//                        (kind::f16, P from TMEM, over the columns of its S)
+//   softmax warpgroups   HALVES per row tile, a thread = a row's part of the
+//                        key tile: S to registers, online softmax in base 2, P
+//                        back to TMEM as f16
 // With NT = 2 the tiles take turns: while one is in its softmax the tensor
 // cores run the other's products. With NT = 1 (head_size 256, whose O takes
 // half of TMEM) S is double-buffered and the next tile's product runs instead.
 //
+// Q enters as TERMS e4m3 terms of its row scaled by a power of two to [128,
+// 256): hi + mid holds bf16's 8 bits, a third term f16's 11; what is lost is
+// below 2^-17 of the row's largest element. Two terms at fp8's rate cost what
+// one f16 product would, and K needs no conversion.
 // Scales: score_ij = c 2^ek_j (q_i . kcode_j), and V's scale is folded into the
 // exponent: z_ij = score_ij + ev_j (base 2), P' = 2^(z - m), O = sum P' vcode /
 // sum P' 2^-ev. The running maximum m is thus over what enters O, so a large V
 // scale cannot push the other rows' P out of f16's range. m moves lazily, when
 // a z exceeds it by 2^8; P' keeps 2^6 of headroom above m so that f16 holds
 // values down to 2^-31 of the maximum.
-// Q enters as f16: exact for f16; a bf16 row is scaled by a power of two that
-// puts its largest element into [2^14, 2^15), so elements down to 2^-31 of it
-// are exact.
 //
 // Every mbarrier wait is bounded; on a timeout the CTA flags MJ_DEV_TIMEOUT,
-// all roles stop, the MMAs in flight complete and TMEM is freed.
+// all roles stop, the copies and MMAs in flight complete and TMEM is freed.
 #include <limits.h>
 #include <math.h>
 
 #include <atomic>
 #include <mutex>
 
+#include <cuda.h>
+
 #include "block_cache.cuh"
 
 namespace mj {
 
 std::mutex& tc_init_mutex();
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn tensor_map_encoder();
 
 namespace ba {
 
 using namespace sm100;
 
 constexpr uint64_t kWaitNs = 500000000ull;  // per wait; a tile takes microseconds
+#ifndef MJ_BA_HALVES
+#define MJ_BA_HALVES 2
+#endif
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kHeadroom = 6.f;            // P' of the running maximum is 2^6
 constexpr float kRaise = kHeadroom + 8.f;   // raise it when a P' would pass 2^14
 
-template <int D>
+template <typename T, int D>
 struct Cfg {
   static constexpr int NT = D == 256 ? 1 : 2;
   static constexpr int BN = MJ_BLOCK_KEYS(D);
   static constexpr int ROWS = NT * 128;
   static_assert(ROWS == MJ_BLOCK_ROWS(D), "the plan's rows");
-  static constexpr int THREADS = 256 + 256 * NT;
-  static constexpr int QTILE = 128 * D * 2, KTILE = BN * D * 2;
-  static constexpr int RAW = BN * D;  // one operand's codes
-  static constexpr int K_OFF = NT * QTILE, V_OFF = K_OFF + 2 * KTILE, RAW_OFF = V_OFF + 2 * KTILE, SC_OFF = RAW_OFF + 2 * RAW;
+  static constexpr int TERMS = std::is_same<T, __half>::value ? 3 : 2;
+  static constexpr int HALVES = MJ_BA_HALVES;
+  static constexpr int THREADS = 256 + 128 * HALVES * NT;
+  static constexpr int KST = TERMS == 2 ? 3 : 2, RST = TERMS == 2 ? 2 : 1;  // stages of K, and of staged V
+  static constexpr int QTERM = 128 * D, QTILE = TERMS * QTERM;  // one row tile's e4m3 term; all its terms
+  static constexpr int RAW = BN * D, VTILE = 2 * RAW;           // a tile's codes; V as f16
+  static constexpr int K_OFF = NT * QTILE, R_OFF = K_OFF + KST * RAW, V_OFF = R_OFF + RST * RAW, SC_OFF = V_OFF + 2 * VTILE;
   static constexpr int SC_BYTES = 4 * (BN / 16) * 16;  // four tiles' float4 per 16 tokens
   static constexpr int BAR_OFF = SC_OFF + SC_BYTES;
-  static constexpr int NBARS = 8 + 4 + 2 + 2 + 4 + 2 + 4;
+  static constexpr int NBARS = 2 * KST + 2 * RST + 4 + 4 + 2 + 2 + 4 + 2;
   static constexpr int MISC_OFF = BAR_OFF + NBARS * 8;
-  static constexpr int RED_OFF = MISC_OFF + 64;  // float [2 NT][128]: what the two halves of a row exchange
-  static constexpr int SMEM = RED_OFF + 2 * NT * 128 * 4;
+  static constexpr int RED_OFF = MISC_OFF + 16;  // float [NT][HALVES][128]: what the parts of a row exchange
+  static constexpr int SMEM = RED_OFF + NT * HALVES * 128 * 4;
   static_assert(SMEM <= 232448, "shared memory of a CTA");
   static constexpr int TMEM_COLS = 512;
   static constexpr int O_COL = 256;
-  // 768 threads launch with 80 registers each: the MMA warpgroup gives most of its up
-  static constexpr int REG_MMA = NT == 2 ? 40 : 0, REG_CVT = NT == 2 ? 88 : 0, REG_SM = NT == 2 ? 88 : 0;
-  static constexpr int REG_LAUNCH = NT == 2 ? 80 : 0;
-  static_assert(REG_MMA <= REG_LAUNCH && REG_CVT >= REG_LAUNCH && REG_SM >= REG_LAUNCH, "directions of the changes");
-  static constexpr int REG_POOL = 128 * REG_MMA + 128 * REG_CVT + 256 * NT * REG_SM;
+  // The launch allocation is shared anew where the softmax warpgroups need
+  // more than their share: the MMA / producer and converter warpgroups give.
+  static constexpr int REG_LAUNCH = NT == 1 ? 0 : HALVES == 2 ? 80 : 128;
+  static constexpr int REG_MMA = NT == 1 ? 0 : HALVES == 2 ? 32 : 48, REG_CVT = NT == 1 ? 0 : HALVES == 2 ? 64 : 80;
+  static constexpr int REG_SM = NT == 1 ? 0 : HALVES == 2 ? 96 : 192;
+  static_assert(REG_MMA <= REG_LAUNCH && REG_CVT <= REG_LAUNCH && REG_SM >= REG_LAUNCH, "directions of the changes");
+  static constexpr int REG_POOL = 128 * REG_MMA + 128 * REG_CVT + 128 * HALVES * NT * REG_SM;
+  static_assert(REG_POOL <= REG_LAUNCH * THREADS, "the split draws on the launch allocation");
 };
 
-// byte offset of 16-byte unit u of row r in a [rows][64 f16] swizzled block
+// byte offset of 16-byte unit u of row r in a [rows][128 bytes] swizzled block
 __device__ __forceinline__ uint32_t unit_offset(uint32_t r, uint32_t u) { return r * 128 + ((u ^ (r & 7)) << 4); }
 
-// byte offset of 16-code chunk c of row r in a staging tile: odd rows swap the
-// halves of each 128 bytes, so four chunks of two neighbouring rows cover all
-// banks
-template <int D>
-__device__ __forceinline__ uint32_t raw_offset(uint32_t r, uint32_t c) { return r * D + ((c ^ ((r & 1) << 2)) << 4); }
+// 8 values -> TERMS rows of e4m3 codes, each the rounded rest of those before
+// (exact differences); a value that is not finite makes its first code NaN
+template <int TERMS>
+__device__ __forceinline__ void split_terms(float* v, uint2* out) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (!(fabsf(v[i]) <= 3.402823466e38f)) v[i] = __int_as_float(0x7FFFFFFF);
+#pragma unroll
+  for (int k = 0; k < TERMS; ++k) {
+    uint16_t c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      c[i] = f2_to_e4m3x2(v[2 * i], v[2 * i + 1]);
+      const float2 f = e4m3x2_to_f2(c[i]);
+      v[2 * i] -= f.x, v[2 * i + 1] -= f.y;
+    }
+    out[k] = make_uint2(c[0] | ((uint32_t)c[1] << 16), c[2] | ((uint32_t)c[3] << 16));
+  }
+}
 
 template <typename T, int D>
-__global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __grid_constant__ mj_block_attn_args a, int lg) {
-  using C = Cfg<D>;
-  constexpr int NT = C::NT, BN = C::BN;
+__global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
+    block_attn_kernel(const __grid_constant__ mj_block_attn_args a, int lg, const __grid_constant__ CUtensorMap tmk,
+                      const __grid_constant__ CUtensorMap tmv) {
+  using C = Cfg<T, D>;
+  constexpr int NT = C::NT, BN = C::BN, HALVES = C::HALVES, KST = C::KST, RST = C::RST;
   extern __shared__ __align__(1024) unsigned char sm[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::BAR_OFF);
-  uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6, *sc_full = bars + 8,
-           *s_full = bars + 12, *p_full = bars + 14, *o_full = bars + 16, *q_full = bars + 20, *drain = bars + 21, *raw_full = bars + 22, *raw_empty = bars + 24;
+  uint64_t *v_full = bars, *v_empty = bars + 2, *sc_full = bars + 4, *s_full = bars + 8, *p_full = bars + 10,
+           *o_full = bars + 12, *q_full = bars + 16, *drain = bars + 17, *k_full = bars + 18, *k_empty = k_full + KST,
+           *r_full = k_empty + KST, *r_empty = r_full + RST;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::MISC_OFF);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + C::MISC_OFF + 4);
   int& never_abort = *reinterpret_cast<int*>(sm + C::MISC_OFF + 8);
@@ -125,26 +153,32 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
   const int na = NT == 1 || row0 + 128 < n_rows ? NT : 1;  // row tiles with rows in them
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&k_full[i], 128);
+    for (int i = 0; i < KST; ++i) {
+      mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < RST; ++i) {
+      mbar_init(&r_full[i], 1);
+      mbar_init(&r_empty[i], 128);
+    }
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&v_full[i], 128);
       mbar_init(&v_empty[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&raw_full[i], 32);
-      mbar_init(&raw_empty[i], 128);
-      mbar_init(&p_full[i], 256);
+      mbar_init(&p_full[i], 128 * HALVES);
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&sc_full[i], 1);
       mbar_init(&o_full[i], 1);
     }
-    mbar_init(q_full, 256 * na);
+    mbar_init(q_full, 128 * HALVES * na);
     mbar_init(drain, 1);
     *abort_flag = 0;
     never_abort = 0;
     fence_mbar_init();
   }
+  if (warp == 1 && lane == 0) prefetch_tmap(&tmk);
+  if (warp == 2 && lane == 0) prefetch_tmap(&tmv);
   if (warp == 0) {
     tmem_alloc(tmem_slot, C::TMEM_COLS);
     tmem_relinquish();
@@ -193,20 +227,22 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
       // ------------------------------------------------------------ MMA issuer
       // (the whole warp runs the loop, one lane issues: see elect_one)
       const bool lead = elect_one();
-      auto qk = [&](int w, int j) {  // 16 head-dim elements a step, 64 a swizzled block
-        constexpr uint32_t idesc = idesc_f16(0, 0, BN);
+      auto qk = [&](int w, int j) {  // every term of Q against the same K; 32 head-dim elements a step
+        constexpr uint32_t idesc = idesc_f8f6f4(0, 0, 0, 0, BN);
         const uint64_t q = smem_desc_sw128(smem_addr(sm + w * C::QTILE), 16, 1024),
-                       k = smem_desc_sw128(smem_addr(sm + C::K_OFF + (j & 1) * C::KTILE), 16, 1024);
+                       k = smem_desc_sw128(smem_addr(sm + C::K_OFF + (j % KST) * C::RAW), 16, 1024);
         if (lead) {
 #pragma unroll
-          for (int i = 0; i < D / 16; ++i)
-            mma_f16_ss(s_col(w, j), q + (i >> 2) * (128 * 8) + (i & 3) * 2, k + (i >> 2) * (BN * 8) + (i & 3) * 2, idesc, i > 0);
+          for (int i = 0; i < C::TERMS * (D / 32); ++i) {
+            const int term = i / (D / 32), dh = i % (D / 32) / 4, x = i % 4;
+            mma_f8f6f4(s_col(w, j), q + term * (C::QTERM / 16) + dh * (128 * 8) + x * 2, k + dh * (BN * 8) + x * 2, idesc, i > 0);
+          }
           mma_commit(&s_full[s_bar(w, j)]);
         }
       };
       auto pv = [&](int w, int j) {  // 16 tokens a step: two 8-row atoms of V, 8 columns of P
         constexpr uint32_t idesc = idesc_f16(0, 1, D);
-        const uint64_t v = smem_desc_sw128(smem_addr(sm + C::V_OFF + (j & 1) * C::KTILE), BN * 128, 1024);
+        const uint64_t v = smem_desc_sw128(smem_addr(sm + C::V_OFF + (j & 1) * C::VTILE), BN * 128, 1024);
         if (lead) {
 #pragma unroll
           for (int i = 0; i < BN / 16; ++i)
@@ -226,11 +262,14 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
       }
       for (int j = 0; ok && j < n; ++j) {
         const bool more = j + 1 < n;
-        if (more) ok = __all_sync(0xffffffffu, wait(&k_full[(j + 1) & 1], (j + 1) >> 1));
+        if (more) ok = __all_sync(0xffffffffu, wait(&k_full[(j + 1) % KST], (j + 1) / KST));
+        // S goes over the P of an earlier product, and MMAs of two kinds are not
+        // ordered with each other: that product has to be complete
+        if (NT == 1 && ok && more && j > 0) ok = __all_sync(0xffffffffu, wait(&o_full[(j - 1) & 1], (j - 1) >> 1));
         if (NT == 1 && ok && more) {
           tc_fence_after();
           qk(0, j + 1);
-          commit(&k_empty[(j + 1) & 1]);
+          commit(&k_empty[(j + 1) % KST]);
         }
         ok = ok && __all_sync(0xffffffffu, wait(&v_full[j & 1], j >> 1));
         for (int w = 0; ok && w < na; ++w) {
@@ -239,43 +278,55 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
           tc_fence_after();
           pv(w, j);
           if (w == na - 1) commit(&v_empty[j & 1]);
-          if (NT == 2 && more) qk(w, j + 1);  // over S and P of tile j: behind its product, in issue order
+          if (NT == 2 && more) {
+            ok = __all_sync(0xffffffffu, wait(&o_full[2 * w + (j & 1)], j >> 1));
+            if (!ok) break;
+            tc_fence_after();
+            qk(w, j + 1);
+          }
         }
-        if (NT == 2 && ok && more) commit(&k_empty[(j + 1) & 1]);
+        if (NT == 2 && ok && more) commit(&k_empty[(j + 1) % KST]);
       }
       commit(drain);  // all issued MMAs complete before TMEM is released
       mbar_wait(drain, 0, &never_abort, kWaitNs);
     } else if (warp < 3) {
-      // -------------------------------------------- loaders: warp 1 K, warp 2 V
-      const int side = warp - 1;
-      constexpr int CPR = D / 16, STEP = 32 / CPR;
-      const unsigned char* src = static_cast<const unsigned char*>(side ? a.v_cache : a.k_cache) +
-                                 h * (side ? a.v_stride_head : a.k_stride_head) + (lane % CPR) * 16;
-      const int64_t sp = side ? a.v_stride_page : a.k_stride_page, sr = side ? a.v_stride_row : a.k_stride_row;
-      unsigned char* raw = sm + C::RAW_OFF + side * C::RAW;
-      // lane i < BN / 16 holds the table entry of the tile's 16-token group i
-      auto entries = [&](int j) { return lane < BN / 16 ? entry_of(base + j * BN + lane * 16) : kNone; };
-      int next = n > 0 ? entries(0) : kNone;
+      // ------------------------------------------ producers: warp 1 K, warp 2 V
+      const bool v = warp == 2;
+      const int st = v ? RST : KST, P = BN / a.page_size, ps = a.page_size;  // pages of a tile: 1 .. 8
+      uint64_t *full = v ? r_full : k_full, *empty = v ? r_empty : k_empty;
+      const CUtensorMap* map = v ? &tmv : &tmk;
+      unsigned char* ring = sm + (v ? C::R_OFF : C::K_OFF);
+      const uint64_t policy = l2_policy_evict_normal();  // other row blocks read the same keys
+      // lane i < P holds the table entry of the tile's page i (pages may be
+      // larger than a tile: then its only box is a part of one)
+      const int pages = P > 0 ? P : 1;
+      auto entries = [&](int j) { return lane < pages ? entry_of(base + j * BN + lane * ps) : kNone; };
+      int next = n > 0 ? entries(0) : kNone, issued = 0;
+      bool ok = true;
       for (int j = 0; j < n; ++j) {
-        const int page = page_of(next);
+        const int page = page_of(next), s = j % st;
         next = entries(j + 1);
-        const bool ok = wait(&raw_empty[side], j + 1);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        const int t0 = base + j * BN;
-#pragma unroll 4
-        for (int r = lane / CPR; r < BN; r += STEP) {
-          const int p = __shfl_sync(0xffffffffu, page, r >> 4);
-          const bool there = p >= 0 && t0 + r < L;  // rows past the sequence become zeros
-          cp_async16(raw + raw_offset<D>(r, lane % CPR), there ? src + p * sp + ((t0 + r) & pmask) * sr : src, there ? 16u : 0u);
+        ok = __all_sync(0xffffffffu, wait(&empty[s], j / st + 1));
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], C::RAW);
+        __syncwarp();
+        if (lane < pages) {
+          // an absent page is read out of range: the TMA fills zeros
+          const int rows = min(ps, BN), r = P > 0 ? 0 : (base + j * BN) & pmask;
+#pragma unroll
+          for (int dh = 0; dh < D / 128; ++dh)
+            tma_load_5d(ring + s * C::RAW + dh * (BN * 128) + lane * rows * 128, map, &full[s], 0, dh, r, h,
+                        page < 0 ? (int)a.num_pages : page, policy);
         }
-        cp_async_arrive_noinc(&raw_full[side]);
+        issued = j + 1;
       }
-      cp_async_wait_all();  // copies land before the CTA exits
+      if (!ok)  // copies in flight land before the CTA exits
+        for (int j = max(issued - st, 0); j < issued; ++j) mbar_wait(&full[j % st], (j / st) & 1, &never_abort, kWaitNs);
     }
     __syncwarp();
   } else if (warp < 8) {
     // ------------------------------------------------------- converter warpgroup
-    if constexpr (C::REG_CVT > 0) setmaxnreg_inc<C::REG_CVT>();
+    if constexpr (C::REG_CVT > 0) setmaxnreg_dec<C::REG_CVT>();
     const int ct = threadIdx.x - 128;
     // block scales of the tile's 16-token groups: thread ct < BN / 16 looks the
     // page up two tiles ahead and reads the two exponents one tile ahead
@@ -294,20 +345,26 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
       sc_entry = entry_of(base + BN + ct * 16);
       sc_next = exponents(base + ct * 16, page_of(e0));
     }
-    // Thread ct takes 16-code chunk `col` of rows r0, r0 + STEP, ...: eight
-    // neighbouring threads are four chunks of a 64-element block in two rows, so
-    // both their staged reads and their swizzled stores cover all banks.
+    // Thread ct takes 16-code chunk 4 blk + quad of rows r0, r0 + STEP, ...:
+    // eight neighbouring threads are four chunks of a 64-element block in rows
+    // r and r ^ 5, so that both their staged reads (swizzled 16-byte chunks of
+    // 16 codes) and their stores (of 8 f16) cover all banks.
     constexpr int BLOCKS = D / 64, STEP = 32 / BLOCKS, NC = BN / STEP;
-    const int quad = ct & 3, blk = (ct >> 3) % BLOCKS, r0 = ((ct >> 2) & 1) + 2 * ((ct >> 3) / BLOCKS);
-    auto convert = [&](int side, int j, uint64_t* empty, uint64_t* full) -> bool {
-      if (!wait(&raw_full[side], j)) return false;
-      const unsigned char* raw = sm + C::RAW_OFF + side * C::RAW;
+    const int quad = ct & 3, blk = (ct >> 3) % BLOCKS, pr = (ct >> 3) / BLOCKS;
+    const int r0 = ((pr & 3) ^ ((ct >> 2) & 1 ? 5 : 0)) + (pr & ~3) * 2;
+    auto convert = [&](int j) -> bool {
+      const int rows = L - (base + j * BN);  // from there on zeros: unwritten rows may hold NaN codes
+      if (!wait(&r_full[j % RST], j / RST)) return false;
+      const unsigned char* raw = sm + C::R_OFF + (j % RST) * C::RAW + (blk >> 1) * (BN * 128);
       uint4 d[NC];
 #pragma unroll
-      for (int i = 0; i < NC; ++i) d[i] = *reinterpret_cast<const uint4*>(raw + raw_offset<D>(r0 + i * STEP, 4 * blk + quad));
-      mbar_arrive(&raw_empty[side]);
-      if (!wait(&empty[j & 1], (j >> 1) + 1)) return false;
-      unsigned char* out = sm + (side ? C::V_OFF : C::K_OFF) + (j & 1) * C::KTILE + blk * (BN * 128);
+      for (int i = 0; i < NC; ++i) {
+        const int r = r0 + i * STEP;
+        d[i] = *reinterpret_cast<const uint4*>(raw + unit_offset(r, 4 * (blk & 1) + quad));
+        if (r >= rows) d[i] = make_uint4(0, 0, 0, 0);
+      }
+      if (!wait(&v_empty[j & 1], (j >> 1) + 1)) return false;
+      unsigned char* out = sm + C::V_OFF + (j & 1) * C::VTILE + blk * (BN * 128);
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
         const uint32_t w[4] = {d[i].x, d[i].y, d[i].z, d[i].w};
@@ -320,8 +377,11 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
         *reinterpret_cast<uint4*>(out + unit_offset(r0 + i * STEP, 2 * quad)) = make_uint4(o[0], o[1], o[2], o[3]);
         *reinterpret_cast<uint4*>(out + unit_offset(r0 + i * STEP, 2 * quad + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
       }
+      // the staging tile is free once every value read from it went through the
+      // stores above: arriving before them let the compiler move reads behind it
+      mbar_arrive(&r_empty[j % RST]);
       fence_proxy_async_smem();
-      mbar_arrive(&full[j & 1]);
+      mbar_arrive(&v_full[j & 1]);
       return true;
     };
     for (int j = 0; j < n; ++j) {
@@ -337,18 +397,26 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
         __syncwarp();
         if (ct == 0) mbar_arrive(&sc_full[j & 3]);
       }
-      if (!convert(0, j, k_empty, k_full) || !convert(1, j, v_empty, v_full)) break;
+      if (!convert(j)) break;
     }
   } else {
     if constexpr (C::REG_SM > 0) setmaxnreg_inc<C::REG_SM>();
     // ------------------------------------------------------- softmax warpgroups
-    const int w = NT == 1 ? 0 : (warp - 8) >> 3, half = ((warp - 8) >> 2) & 1;
+    const int w = (warp - 8) / (4 * HALVES), half = ((warp - 8) >> 2) % HALVES;
     const int t = threadIdx.x & 127;
     if (w < na) {
-      constexpr int HN = BN / 2, HD = D / 2;  // keys of a tile, and head-dim elements, of one half
-      // the two warps that share 32 rows meet in a named barrier of their own
+      constexpr int HN = BN / HALVES, HD = D / HALVES;  // keys of a tile, and head-dim elements, of one part
+      // the warps that share 32 rows meet in a named barrier of their own
       const uint32_t pair = 1 + 4 * w + (warp & 3);
-      float* red = reinterpret_cast<float*>(sm + C::RED_OFF) + w * 256;
+      float* red = reinterpret_cast<float*>(sm + C::RED_OFF) + w * HALVES * 128;
+      auto pair_or = [&](bool v) { return HALVES == 1 ? __any_sync(0xffffffffu, v) != 0 : named_bar_or(pair, 64, v); };
+      // the other part's value of this row
+      auto other = [&](float v) {
+        if (HALVES == 1) return v;
+        red[half * 128 + t] = v;
+        named_bar_sync(pair, 64);
+        return red[(half ^ 1) * 128 + t];
+      };
       const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
       const int R = row0 + w * 128 + t;
       const bool live = R < n_rows;
@@ -356,47 +424,46 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
       const int lim = !live ? -1 : a.causal ? L - n_tok + tok : L - 1;  // the last key this row sees
       // the first row of the warp sees the fewest keys
       const int warp_lim = __shfl_sync(0xffffffffu, lim, 0);
-      // ---- Q: this half row as f16 into the K-major tile (dead rows are zeros)
+      // ---- Q: this part of the row in TERMS e4m3 terms into the K-major tiles (dead rows are zeros)
       float c2 = a.softmax_scale * kLog2e;
       {
         const T* q = static_cast<const T*>(a.q) + (int64_t)(q0 + tok) * a.q_stride_tok + hq * a.q_stride_head + half * HD;
-        unsigned char* qs = sm + w * C::QTILE + half * (HD / 64) * (128 * 128);
-        float up = 1.f;
-        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-          float amax = 0.f;
-#pragma unroll 4
-          for (int c = 0; c < HD / 8; ++c) {
-            float v[8];
-            load8(q + 8 * c, v);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[i]));
-          }
-          red[half * 128 + t] = amax;
-          named_bar_sync(pair, 64);
-          amax = fmaxf(amax, red[(half ^ 1) * 128 + t]);
-          // 2^k with amax 2^k in [2^14, 2^15), inside fp32's normal range
-          const int ex = (int)(__float_as_uint(amax) >> 23);
-          if (ex > 0 && ex < 255) {
-            const int k = min(max(141 - ex, -126), 126);
-            up = __uint_as_float((uint32_t)(127 + k) << 23);
-            c2 *= __uint_as_float((uint32_t)(127 - k) << 23);
-          }
-        }
+        unsigned char* qs = sm + w * C::QTILE;
+        float amax = 0.f;
 #pragma unroll 4
         for (int c = 0; c < HD / 8; ++c) {
           float v[8];
           load8(q + 8 * c, v);
-          uint32_t o[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[i] = live ? f2_to_h2(v[2 * i] * up, v[2 * i + 1] * up) : 0u;
-          *reinterpret_cast<uint4*>(qs + (c >> 3) * (128 * 128) + unit_offset(t, c & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
+          for (int i = 0; i < 8; ++i) amax = fabsf(v[i]) <= 3.402823466e38f ? fmaxf(amax, fabsf(v[i])) : amax;
+        }
+        amax = fmaxf(amax, other(amax));
+        // 2^k with amax 2^k in [128, 256), inside fp32's normal range
+        const int k = amax > 0.f ? min(max(134 - (int)(__float_as_uint(amax) >> 23), -126), 126) : 0;
+        const float up = __uint_as_float((uint32_t)(127 + k) << 23);
+        c2 *= __uint_as_float((uint32_t)(127 - k) << 23);
+#pragma unroll 2
+        for (int c = 0; c < HD / 16; ++c) {
+          float v[16];
+          load8(q + 16 * c, v);
+          load8(q + 16 * c + 8, v + 8);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = live ? v[i] * up : 0.f;
+          uint2 lo[C::TERMS], hi[C::TERMS];
+          split_terms<C::TERMS>(v, lo);
+          split_terms<C::TERMS>(v + 8, hi);
+          const int u = half * (HD / 16) + c;  // the row's 16-byte unit
+#pragma unroll
+          for (int i = 0; i < C::TERMS; ++i)
+            *reinterpret_cast<uint4*>(qs + i * C::QTERM + (u >> 3) * (128 * 128) + unit_offset(t, u & 7)) =
+                make_uint4(lo[i].x, lo[i].y, hi[i].x, hi[i].y);
         }
         fence_proxy_async_smem();
         mbar_arrive(q_full);
       }
-      // nm: kHeadroom minus the running maximum (the same in both halves); a
+      // nm: kHeadroom minus the running maximum (the same in every part); a
       // row that sees no key of the first tile sees none at all (keys are a
-      // prefix) and keeps P = 0. l: this half's part of the row sum.
+      // prefix) and keeps P = 0. l: this part's share of the row sum.
       float nm = 0.f, l = 0.f;
       bool ok = true;
       const uint32_t o_addr = C::O_COL + w * 128 + half * HD + lane_base;
@@ -418,7 +485,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
           for (int i = 0; i < 8; ++i) s[8 * g + i] = ffma2(s[8 * g + i], m2, b2);
         }
         const int j0 = (tb + j) * BN + half * HN;
-        if (j0 + HN - 1 > warp_lim) {  // some row of the warp sees part of this half tile
+        if (j0 + HN - 1 > warp_lim) {  // some row of the warp sees only some of these keys
 #pragma unroll
           for (int i = 0; i < HN / 2; ++i) {
             if (j0 + 2 * i > lim) s[i].x = -INFINITY;
@@ -431,17 +498,15 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
 #pragma unroll
         for (int i = 4; i < HN / 2; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], fmaxf(s[i].x, s[i].y));
         float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-        // One barrier per tile between the two halves: both hold their scores
-        // (P goes over the first half's columns), and both learn whether some
+        // One vote per tile of the warps of these rows: all hold their scores
+        // (P goes over the first part's columns), and all learn whether some
         // row outgrew its maximum, or a wait ran out.
-        if (named_bar_or(pair, 64, j == 0 || mx > kRaise || !ok)) {
-          if (named_bar_or(pair, 64, !ok)) {
+        if (pair_or(j == 0 || mx > kRaise || !ok)) {
+          if (pair_or(!ok)) {
             ok = false;
             break;
           }
-          red[half * 128 + t] = mx;
-          named_bar_sync(pair, 64);
-          mx = fmaxf(mx, red[(half ^ 1) * 128 + t]);
+          mx = fmaxf(mx, other(mx));
           const float up = (j == 0 ? mx > -INFINITY : mx > kRaise) ? kHeadroom - mx : 0.f;  // added to nm
           nm += up;
 #pragma unroll
@@ -462,7 +527,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
               tmem_st16(o_addr + c, reinterpret_cast<const uint32_t*>(o));
             }
           }
-          // red is read before the next raise writes it: the barrier of that tile
+          // (the exchanged values are read before the next vote, and written after it)
         }
 #pragma unroll
         for (int c = 0; c < HN / 32; ++c) {  // 32 keys: 16 columns of P
@@ -485,14 +550,12 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) block_attn_kernel(const __
         tc_fence_before();
         mbar_arrive(&p_full[s_bar(w, j)]);
       }
-      // ---- epilogue: this half's head-dim elements of O / l
+      // ---- epilogue: this part's head-dim elements of O / l
       if (ok && n > 0) ok = wait(&o_full[2 * w + ((n - 1) & 1)], (n - 1) >> 1);
       tc_fence_after();
-      // both halves leave together, and know the whole sum
-      if (!named_bar_or(pair, 64, !ok)) {
-        red[half * 128 + t] = l;
-        named_bar_sync(pair, 64);
-        l += red[(half ^ 1) * 128 + t];
+      // the parts leave together, and know the whole sum
+      if (!pair_or(!ok)) {
+        if (HALVES > 1) l += other(l);
         const float inv = l == 0.f ? 0.f : 1.f / l;  // a NaN sum stays NaN
         const int64_t part = ((int64_t)slot * a.h_k + h) * C::ROWS + w * 128 + t;
         T* o = static_cast<T*>(a.o) + (int64_t)(q0 + tok) * a.o_stride_tok + hq * a.o_stride_head + half * HD;
@@ -575,9 +638,26 @@ __global__ void __launch_bounds__(256) block_merge_kernel(const __grid_constant_
 
 constexpr int kMaxDevices = 64;
 
+// One operand's codes as (128 codes, 128-code halves of a row, page rows, KV
+// heads, pages), boxes of one page's rows (or a tile's, where a page is larger).
+static bool make_map(CUtensorMap* m, const void* base, int64_t s_page, int64_t s_row, int64_t s_head,
+                     const mj_block_attn_args& a) {
+  auto fn = tensor_map_encoder();
+  if (!fn) return false;
+  // a dimension of extent 1 never moves its coordinate: any legal stride
+  const cuuint64_t sr = s_row ? s_row : 16, sh = s_head ? s_head : 16, sp = s_page ? s_page : 16;
+  const int keys = MJ_BLOCK_KEYS(a.head_size), rows = a.page_size < keys ? a.page_size : keys;
+  cuuint64_t dims[5] = {128, (cuuint64_t)(a.head_size / 128), (cuuint64_t)a.page_size, (cuuint64_t)a.h_k, (cuuint64_t)a.num_pages};
+  cuuint64_t strides[4] = {128, sr, sh, sp};
+  cuuint32_t box[5] = {128, 1, (cuuint32_t)rows, 1, 1}, estr[5] = {1, 1, 1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int D>
 static cudaError_t launch_t(const mj_block_attn_args& a, cudaStream_t stream) {
-  using C = Cfg<D>;
+  using C = Cfg<T, D>;
   auto kern = block_attn_kernel<T, D>;
   static std::atomic<int> ready[kMaxDevices];
   int dev = 0;
@@ -590,12 +670,16 @@ static cudaError_t launch_t(const mj_block_attn_args& a, cudaStream_t stream) {
     if ((e = cudaFuncGetAttributes(&fa, kern)) != cudaSuccess) return e;
     // the register split must fit the launch allocation, or the softmax
     // warpgroups would wait for registers that never come
-    if (C::REG_LAUNCH && (fa.numRegs != C::REG_LAUNCH || C::REG_POOL > fa.numRegs * C::THREADS)) return cudaErrorNotSupported;
+    if (C::REG_LAUNCH && fa.numRegs != C::REG_LAUNCH) return cudaErrorNotSupported;
     if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM)) != cudaSuccess) return e;
     ready[dev].store(1, std::memory_order_release);
   }
   if (a.num_work) {
-    e = launch_kernel(kern, dim3((unsigned)(a.num_work * a.h_k)), dim3(C::THREADS), C::SMEM, stream, a, block_log2(a.kv_format));
+    CUtensorMap mk, mv;
+    if (!make_map(&mk, a.k_cache, a.k_stride_page, a.k_stride_row, a.k_stride_head, a) ||
+        !make_map(&mv, a.v_cache, a.v_stride_page, a.v_stride_row, a.v_stride_head, a))
+      return cudaErrorInvalidValue;
+    e = launch_kernel(kern, dim3((unsigned)(a.num_work * a.h_k)), dim3(C::THREADS), C::SMEM, stream, a, block_log2(a.kv_format), mk, mv);
     if (e != cudaSuccess) return e;
   }
   if (a.num_merges) {

@@ -47,6 +47,8 @@ static EncodeTiledFn encode_fn() {
   return fn;
 }
 
+EncodeTiledFn tensor_map_encoder() { return encode_fn(); }
+
 // Why the tensor-core kernel cannot run these arguments (nullptr = it can).
 const char* tc_ineligible(const mj_decode_args& a) {
   if (a.kv_format == MJ_KV_NVFP4) {  // the scale rows arrive by 8-byte copies
