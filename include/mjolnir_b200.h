@@ -455,7 +455,7 @@ typedef struct mj_block_attn_args {
    * (seq, first row, tile begin, tile end, partial slot or -1, 0, 0, 0). A
    * row is (query token, head of the KV head's group), token-major; an item
    * covers MJ_BLOCK_ROWS(head_size) rows from its first and the keys of its
-   * tiles of MJ_BLOCK_KEYS(head_size). Items with a slot leave normalised
+   * tiles of MJ_BLOCK_KEYS. Items with a slot leave normalised
    * partials in o_part / lse_part at [slot][KV head][row]; num_merges entries
    * of 4 int32 (seq, first row, first slot, slots) say which to join. */
   const int32_t* work; int num_work;
@@ -467,7 +467,7 @@ typedef struct mj_block_attn_args {
 } mj_block_attn_args;
 
 #define MJ_BLOCK_ROWS(head_size) ((head_size) == 256 ? 128 : 256)
-#define MJ_BLOCK_KEYS(head_size) ((head_size) == 256 ? 64 : 128)
+#define MJ_BLOCK_KEYS 64
 
 int mj_block_attention(const mj_block_attn_args* args, void* stream);
 

@@ -9,12 +9,13 @@
 //                        operand tiles; also the tile's block scales
 //   MMA warp             S = Q K^T (kind::f8f6f4, K as stored), O += P V
 //                        (kind::f16, P from TMEM, over the columns of its S)
-//   softmax warpgroups   HALVES per row tile, a thread = a row's part of the
-//                        key tile: S to registers, online softmax in base 2, P
-//                        back to TMEM as f16
-// With NT = 2 the tiles take turns: while one is in its softmax the tensor
-// cores run the other's products. With NT = 1 (head_size 256, whose O takes
-// half of TMEM) S is double-buffered and the next tile's product runs instead.
+//   softmax warpgroups   one per row tile, a thread = a row: S to registers,
+//                        online softmax in base 2, P back to TMEM as f16
+// S is double-buffered in TMEM (64 keys a tile, two buffers and O of both row
+// tiles fill its 512 columns): the next tile's product runs beside this one's
+// softmax, so a softmax warpgroup finds its next scores waiting. With 128 keys
+// and one buffer it waited for the previous product and the next one, two
+// thousand cycles of each tile's five.
 //
 // Q enters as TERMS e4m3 terms of its row scaled by a power of two to [128,
 // 256): hi + mid holds bf16's 8 bits, a third term f16's 11; what is lost is
@@ -52,9 +53,6 @@ namespace ba {
 using namespace sm100;
 
 constexpr uint64_t kWaitNs = 500000000ull;  // per wait; a tile takes microseconds
-#ifndef MJ_BA_HALVES
-#define MJ_BA_HALVES 2
-#endif
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kHeadroom = 6.f;            // P' of the running maximum is 2^6
 constexpr float kRaise = kHeadroom + 8.f;   // raise it when a P' would pass 2^14
@@ -62,33 +60,25 @@ constexpr float kRaise = kHeadroom + 8.f;   // raise it when a P' would pass 2^1
 template <typename T, int D>
 struct Cfg {
   static constexpr int NT = D == 256 ? 1 : 2;
-  static constexpr int BN = MJ_BLOCK_KEYS(D);
+  static constexpr int BN = MJ_BLOCK_KEYS;
   static constexpr int ROWS = NT * 128;
   static_assert(ROWS == MJ_BLOCK_ROWS(D), "the plan's rows");
   static constexpr int TERMS = std::is_same<T, __half>::value ? 3 : 2;
-  static constexpr int HALVES = MJ_BA_HALVES;
-  static constexpr int THREADS = 256 + 128 * HALVES * NT;
-  static constexpr int KST = TERMS == 2 ? 3 : 2, RST = TERMS == 2 ? 2 : 1;  // stages of K, and of staged V
+  static constexpr int THREADS = 256 + 128 * NT;
+  // stages of K, of staged V codes and of V as f16
+  static constexpr int KST = D == 128 ? 4 : TERMS == 2 ? 3 : 2, RST = D == 128 ? 3 : TERMS == 2 ? 2 : 1, VST = D == 128 ? 3 : 2;
   static constexpr int QTERM = 128 * D, QTILE = TERMS * QTERM;  // one row tile's e4m3 term; all its terms
   static constexpr int RAW = BN * D, VTILE = 2 * RAW;           // a tile's codes; V as f16
-  static constexpr int K_OFF = NT * QTILE, R_OFF = K_OFF + KST * RAW, V_OFF = R_OFF + RST * RAW, SC_OFF = V_OFF + 2 * VTILE;
+  static constexpr int K_OFF = NT * QTILE, R_OFF = K_OFF + KST * RAW, V_OFF = R_OFF + RST * RAW, SC_OFF = V_OFF + VST * VTILE;
   static constexpr int SC_BYTES = 4 * (BN / 16) * 16;  // four tiles' float4 per 16 tokens
   static constexpr int BAR_OFF = SC_OFF + SC_BYTES;
-  static constexpr int NBARS = 2 * KST + 2 * RST + 4 + 4 + 2 + 2 + 4 + 2;
+  static constexpr int NBARS = 18 + 2 * KST + 2 * RST + 2 * VST;
   static constexpr int MISC_OFF = BAR_OFF + NBARS * 8;
-  static constexpr int RED_OFF = MISC_OFF + 16;  // float [NT][HALVES][128]: what the parts of a row exchange
-  static constexpr int SMEM = RED_OFF + NT * HALVES * 128 * 4;
+  static constexpr int SMEM = MISC_OFF + 16;
+  static_assert(VST <= 3, "the four scale slots cover the tiles in flight");
   static_assert(SMEM <= 232448, "shared memory of a CTA");
   static constexpr int TMEM_COLS = 512;
   static constexpr int O_COL = 256;
-  // The launch allocation is shared anew where the softmax warpgroups need
-  // more than their share: the MMA / producer and converter warpgroups give.
-  static constexpr int REG_LAUNCH = NT == 1 ? 0 : HALVES == 2 ? 80 : 128;
-  static constexpr int REG_MMA = NT == 1 ? 0 : HALVES == 2 ? 32 : 48, REG_CVT = NT == 1 ? 0 : HALVES == 2 ? 64 : 80;
-  static constexpr int REG_SM = NT == 1 ? 0 : HALVES == 2 ? 96 : 192;
-  static_assert(REG_MMA <= REG_LAUNCH && REG_CVT <= REG_LAUNCH && REG_SM >= REG_LAUNCH, "directions of the changes");
-  static constexpr int REG_POOL = 128 * REG_MMA + 128 * REG_CVT + 128 * HALVES * NT * REG_SM;
-  static_assert(REG_POOL <= REG_LAUNCH * THREADS, "the split draws on the launch allocation");
 };
 
 // byte offset of 16-byte unit u of row r in a [rows][128 bytes] swizzled block
@@ -119,13 +109,14 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
     block_attn_kernel(const __grid_constant__ mj_block_attn_args a, int lg, const __grid_constant__ CUtensorMap tmk,
                       const __grid_constant__ CUtensorMap tmv) {
   using C = Cfg<T, D>;
-  constexpr int NT = C::NT, BN = C::BN, HALVES = C::HALVES, KST = C::KST, RST = C::RST;
+  constexpr int NT = C::NT, BN = C::BN, KST = C::KST, RST = C::RST, VST = C::VST;
   extern __shared__ __align__(1024) unsigned char sm[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::BAR_OFF);
-  uint64_t *v_full = bars, *v_empty = bars + 2, *sc_full = bars + 4, *s_full = bars + 8, *p_full = bars + 10,
-           *o_full = bars + 12, *q_full = bars + 16, *drain = bars + 17, *k_full = bars + 18, *k_empty = k_full + KST,
-           *r_full = k_empty + KST, *r_empty = r_full + RST;
+  // s_full, p_full and o_full: [row tile][key tile & 1]
+  uint64_t *sc_full = bars, *s_full = bars + 4, *p_full = bars + 8, *o_full = bars + 12, *q_full = bars + 16,
+           *drain = bars + 17, *k_full = bars + 18, *k_empty = k_full + KST, *r_full = k_empty + KST, *r_empty = r_full + RST,
+           *v_full = r_empty + RST, *v_empty = v_full + VST;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::MISC_OFF);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + C::MISC_OFF + 4);
   int& never_abort = *reinterpret_cast<int*>(sm + C::MISC_OFF + 8);
@@ -161,17 +152,17 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
       mbar_init(&r_full[i], 1);
       mbar_init(&r_empty[i], 128);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < VST; ++i) {
       mbar_init(&v_full[i], 128);
       mbar_init(&v_empty[i], 1);
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128 * HALVES);
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&sc_full[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
       mbar_init(&o_full[i], 1);
     }
-    mbar_init(q_full, 128 * HALVES * na);
+    mbar_init(q_full, 128 * na);
     mbar_init(drain, 1);
     *abort_flag = 0;
     never_abort = 0;
@@ -201,10 +192,10 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
     if (!*abort_flag) give_up();
     return false;
   };
-  // S of row tile w for key tile j (P over its first columns), and its barriers
-  auto s_col = [&](int w, int j) { return (uint32_t)(NT == 2 ? w * 128 : (j & 1) * BN); };
-  auto s_bar = [&](int w, int j) { return NT == 2 ? w : j & 1; };
-  auto s_phase = [&](int j) { return NT == 2 ? j : j >> 1; };
+  // S of row tile w for key tile j, with P over its first half; the index and
+  // phase of that pair's barriers
+  auto s_col = [&](int w, int j) { return (uint32_t)(w * 128 + (j & 1) * BN); };
+  auto at = [&](int w, int j) { return 2 * w + (j & 1); };
 
   // Page-table walk. An entry is loaded before it is needed and checked then:
   // checking it at once would wait a memory round trip.
@@ -222,7 +213,6 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
   };
 
   if (warp < 4) {
-    if constexpr (C::REG_MMA > 0) setmaxnreg_dec<C::REG_MMA>();
     if (warp == 0) {
       // ------------------------------------------------------------ MMA issuer
       // (the whole warp runs the loop, one lane issues: see elect_one)
@@ -237,17 +227,17 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
             const int term = i / (D / 32), dh = i % (D / 32) / 4, x = i % 4;
             mma_f8f6f4(s_col(w, j), q + term * (C::QTERM / 16) + dh * (128 * 8) + x * 2, k + dh * (BN * 8) + x * 2, idesc, i > 0);
           }
-          mma_commit(&s_full[s_bar(w, j)]);
+          mma_commit(&s_full[at(w, j)]);
         }
       };
       auto pv = [&](int w, int j) {  // 16 tokens a step: two 8-row atoms of V, 8 columns of P
         constexpr uint32_t idesc = idesc_f16(0, 1, D);
-        const uint64_t v = smem_desc_sw128(smem_addr(sm + C::V_OFF + (j & 1) * C::VTILE), BN * 128, 1024);
+        const uint64_t v = smem_desc_sw128(smem_addr(sm + C::V_OFF + (j % VST) * C::VTILE), BN * 128, 1024);
         if (lead) {
 #pragma unroll
           for (int i = 0; i < BN / 16; ++i)
             mma_f16_ts(C::O_COL + w * 128, s_col(w, j) + i * 8, v + i * 128, idesc, j > 0 || i > 0);
-          mma_commit(&o_full[2 * w + (j & 1)]);
+          mma_commit(&o_full[at(w, j)]);
         }
       };
       auto commit = [&](uint64_t* bar) {
@@ -261,31 +251,26 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
         commit(&k_empty[0]);
       }
       for (int j = 0; ok && j < n; ++j) {
-        const bool more = j + 1 < n;
-        if (more) ok = __all_sync(0xffffffffu, wait(&k_full[(j + 1) % KST], (j + 1) / KST));
-        // S goes over the P of an earlier product, and MMAs of two kinds are not
-        // ordered with each other: that product has to be complete
-        if (NT == 1 && ok && more && j > 0) ok = __all_sync(0xffffffffu, wait(&o_full[(j - 1) & 1], (j - 1) >> 1));
-        if (NT == 1 && ok && more) {
-          tc_fence_after();
-          qk(0, j + 1);
-          commit(&k_empty[(j + 1) % KST]);
-        }
-        ok = ok && __all_sync(0xffffffffu, wait(&v_full[j & 1], j >> 1));
-        for (int w = 0; ok && w < na; ++w) {
-          ok = __all_sync(0xffffffffu, wait(&p_full[s_bar(w, j)], s_phase(j)));
-          if (!ok) break;
-          tc_fence_after();
-          pv(w, j);
-          if (w == na - 1) commit(&v_empty[j & 1]);
-          if (NT == 2 && more) {
-            ok = __all_sync(0xffffffffu, wait(&o_full[2 * w + (j & 1)], j >> 1));
+        if (j + 1 < n) {
+          ok = __all_sync(0xffffffffu, wait(&k_full[(j + 1) % KST], (j + 1) / KST));
+          for (int w = 0; ok && w < na; ++w) {
+            // S goes over the P of tile j - 1, and MMAs of two kinds are not
+            // ordered with each other: that product has to be complete
+            if (j > 0) ok = __all_sync(0xffffffffu, wait(&o_full[at(w, j - 1)], (j - 1) >> 1));
             if (!ok) break;
             tc_fence_after();
             qk(w, j + 1);
           }
+          if (ok) commit(&k_empty[(j + 1) % KST]);
         }
-        if (NT == 2 && ok && more) commit(&k_empty[(j + 1) % KST]);
+        ok = ok && __all_sync(0xffffffffu, wait(&v_full[j % VST], j / VST));
+        for (int w = 0; ok && w < na; ++w) {
+          ok = __all_sync(0xffffffffu, wait(&p_full[at(w, j)], j >> 1));
+          if (!ok) break;
+          tc_fence_after();
+          pv(w, j);
+        }
+        if (ok) commit(&v_empty[j % VST]);
       }
       commit(drain);  // all issued MMAs complete before TMEM is released
       mbar_wait(drain, 0, &never_abort, kWaitNs);
@@ -326,7 +311,6 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
     __syncwarp();
   } else if (warp < 8) {
     // ------------------------------------------------------- converter warpgroup
-    if constexpr (C::REG_CVT > 0) setmaxnreg_dec<C::REG_CVT>();
     const int ct = threadIdx.x - 128;
     // block scales of the tile's 16-token groups: thread ct < BN / 16 looks the
     // page up two tiles ahead and reads the two exponents one tile ahead
@@ -363,8 +347,8 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
         d[i] = *reinterpret_cast<const uint4*>(raw + unit_offset(r, 4 * (blk & 1) + quad));
         if (r >= rows) d[i] = make_uint4(0, 0, 0, 0);
       }
-      if (!wait(&v_empty[j & 1], (j >> 1) + 1)) return false;
-      unsigned char* out = sm + C::V_OFF + (j & 1) * C::VTILE + blk * (BN * 128);
+      if (!wait(&v_empty[j % VST], j / VST + 1)) return false;
+      unsigned char* out = sm + C::V_OFF + (j % VST) * C::VTILE + blk * (BN * 128);
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
         const uint32_t w[4] = {d[i].x, d[i].y, d[i].z, d[i].w};
@@ -381,7 +365,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
       // stores above: arriving before them let the compiler move reads behind it
       mbar_arrive(&r_empty[j % RST]);
       fence_proxy_async_smem();
-      mbar_arrive(&v_full[j & 1]);
+      mbar_arrive(&v_full[j % VST]);
       return true;
     };
     for (int j = 0; j < n; ++j) {
@@ -400,23 +384,9 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
       if (!convert(j)) break;
     }
   } else {
-    if constexpr (C::REG_SM > 0) setmaxnreg_inc<C::REG_SM>();
     // ------------------------------------------------------- softmax warpgroups
-    const int w = (warp - 8) / (4 * HALVES), half = ((warp - 8) >> 2) % HALVES;
-    const int t = threadIdx.x & 127;
+    const int w = (warp - 8) >> 2, t = threadIdx.x & 127;
     if (w < na) {
-      constexpr int HN = BN / HALVES, HD = D / HALVES;  // keys of a tile, and head-dim elements, of one part
-      // the warps that share 32 rows meet in a named barrier of their own
-      const uint32_t pair = 1 + 4 * w + (warp & 3);
-      float* red = reinterpret_cast<float*>(sm + C::RED_OFF) + w * HALVES * 128;
-      auto pair_or = [&](bool v) { return HALVES == 1 ? __any_sync(0xffffffffu, v) != 0 : named_bar_or(pair, 64, v); };
-      // the other part's value of this row
-      auto other = [&](float v) {
-        if (HALVES == 1) return v;
-        red[half * 128 + t] = v;
-        named_bar_sync(pair, 64);
-        return red[(half ^ 1) * 128 + t];
-      };
       const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
       const int R = row0 + w * 128 + t;
       const bool live = R < n_rows;
@@ -424,26 +394,25 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
       const int lim = !live ? -1 : a.causal ? L - n_tok + tok : L - 1;  // the last key this row sees
       // the first row of the warp sees the fewest keys
       const int warp_lim = __shfl_sync(0xffffffffu, lim, 0);
-      // ---- Q: this part of the row in TERMS e4m3 terms into the K-major tiles (dead rows are zeros)
+      // ---- Q: this row in TERMS e4m3 terms into the K-major tiles (dead rows are zeros)
       float c2 = a.softmax_scale * kLog2e;
       {
-        const T* q = static_cast<const T*>(a.q) + (int64_t)(q0 + tok) * a.q_stride_tok + hq * a.q_stride_head + half * HD;
+        const T* q = static_cast<const T*>(a.q) + (int64_t)(q0 + tok) * a.q_stride_tok + hq * a.q_stride_head;
         unsigned char* qs = sm + w * C::QTILE;
         float amax = 0.f;
 #pragma unroll 4
-        for (int c = 0; c < HD / 8; ++c) {
+        for (int c = 0; c < D / 8; ++c) {
           float v[8];
           load8(q + 8 * c, v);
 #pragma unroll
           for (int i = 0; i < 8; ++i) amax = fabsf(v[i]) <= 3.402823466e38f ? fmaxf(amax, fabsf(v[i])) : amax;
         }
-        amax = fmaxf(amax, other(amax));
         // 2^k with amax 2^k in [128, 256), inside fp32's normal range
         const int k = amax > 0.f ? min(max(134 - (int)(__float_as_uint(amax) >> 23), -126), 126) : 0;
         const float up = __uint_as_float((uint32_t)(127 + k) << 23);
         c2 *= __uint_as_float((uint32_t)(127 - k) << 23);
 #pragma unroll 2
-        for (int c = 0; c < HD / 16; ++c) {
+        for (int c = 0; c < D / 16; ++c) {
           float v[16];
           load8(q + 16 * c, v);
           load8(q + 16 * c + 8, v + 8);
@@ -452,42 +421,45 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
           uint2 lo[C::TERMS], hi[C::TERMS];
           split_terms<C::TERMS>(v, lo);
           split_terms<C::TERMS>(v + 8, hi);
-          const int u = half * (HD / 16) + c;  // the row's 16-byte unit
 #pragma unroll
           for (int i = 0; i < C::TERMS; ++i)
-            *reinterpret_cast<uint4*>(qs + i * C::QTERM + (u >> 3) * (128 * 128) + unit_offset(t, u & 7)) =
+            *reinterpret_cast<uint4*>(qs + i * C::QTERM + (c >> 3) * (128 * 128) + unit_offset(t, c & 7)) =
                 make_uint4(lo[i].x, lo[i].y, hi[i].x, hi[i].y);
         }
         fence_proxy_async_smem();
         mbar_arrive(q_full);
       }
-      // nm: kHeadroom minus the running maximum (the same in every part); a
+      // nm: kHeadroom minus the running maximum; a
       // row that sees no key of the first tile sees none at all (keys are a
-      // prefix) and keeps P = 0. l: this part's share of the row sum.
+      // prefix) and keeps P = 0. l: the row sum.
       float nm = 0.f, l = 0.f;
       bool ok = true;
-      const uint32_t o_addr = C::O_COL + w * 128 + half * HD + lane_base;
+      const uint32_t o_addr = C::O_COL + w * 128 + lane_base;
       for (int j = 0; j < n; ++j) {
-        ok = wait(&sc_full[j & 3], j >> 2) && wait(&s_full[s_bar(w, j)], s_phase(j));
+        ok = wait(&sc_full[j & 3], j >> 2) && wait(&s_full[at(w, j)], j >> 1);
+        // every thread leaves the loop with its warp: the TMEM loads are collective
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
         tc_fence_after();
         const uint32_t s_addr = s_col(w, j) + lane_base;
-        float2 s[HN / 2];
-        __syncwarp();
+        float2 s[BN / 2];
 #pragma unroll
-        for (int c = 0; c < HN / 32; ++c) tmem_ld32(s_addr + half * HN + 32 * c, reinterpret_cast<float*>(s) + 32 * c);
+        for (int c = 0; c < BN / 32; ++c) tmem_ld32(s_addr + 32 * c, reinterpret_cast<float*>(s) + 32 * c);
         tmem_wait_ld();
-        const float4* sc = reinterpret_cast<const float4*>(sm + C::SC_OFF) + (j & 3) * (BN / 16) + half * (HN / 16);
+        const float4* sc = reinterpret_cast<const float4*>(sm + C::SC_OFF) + (j & 3) * (BN / 16);
 #pragma unroll
-        for (int g = 0; g < HN / 16; ++g) {
+        for (int g = 0; g < BN / 16; ++g) {
           const float4 f = sc[g];
           const float2 m2 = make_float2(c2 * f.x, c2 * f.x), b2 = make_float2(f.y + nm, f.y + nm);
 #pragma unroll
           for (int i = 0; i < 8; ++i) s[8 * g + i] = ffma2(s[8 * g + i], m2, b2);
         }
-        const int j0 = (tb + j) * BN + half * HN;
-        if (j0 + HN - 1 > warp_lim) {  // some row of the warp sees only some of these keys
+        const int j0 = (tb + j) * BN;
+        if (j0 + BN - 1 > warp_lim) {  // some row of the warp sees only some of these keys
 #pragma unroll
-          for (int i = 0; i < HN / 2; ++i) {
+          for (int i = 0; i < BN / 2; ++i) {
             if (j0 + 2 * i > lim) s[i].x = -INFINITY;
             if (j0 + 2 * i + 1 > lim) s[i].y = -INFINITY;
           }
@@ -496,29 +468,20 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) mx4[i] = fmaxf(s[i].x, s[i].y);
 #pragma unroll
-        for (int i = 4; i < HN / 2; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], fmaxf(s[i].x, s[i].y));
+        for (int i = 4; i < BN / 2; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], fmaxf(s[i].x, s[i].y));
         float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-        // One vote per tile of the warps of these rows: all hold their scores
-        // (P goes over the first part's columns), and all learn whether some
-        // row outgrew its maximum, or a wait ran out.
-        if (pair_or(j == 0 || mx > kRaise || !ok)) {
-          if (pair_or(!ok)) {
-            ok = false;
-            break;
-          }
-          mx = fmaxf(mx, other(mx));
+        if (__any_sync(0xffffffffu, j == 0 || mx > kRaise)) {
           const float up = (j == 0 ? mx > -INFINITY : mx > kRaise) ? kHeadroom - mx : 0.f;  // added to nm
           nm += up;
 #pragma unroll
-          for (int i = 0; i < HN / 2; ++i) s[i] = fadd2(s[i], make_float2(up, up));
+          for (int i = 0; i < BN / 2; ++i) s[i] = fadd2(s[i], make_float2(up, up));
           if (j > 0) {  // O and l follow, once the last product has landed
             const float f = exp2_approx(up);
             l *= f;
-            ok = wait(&o_full[2 * w + ((j - 1) & 1)], (j - 1) >> 1);
+            ok = __all_sync(0xffffffffu, wait(&o_full[at(w, j - 1)], (j - 1) >> 1));
             tc_fence_after();
-            __syncwarp();
 #pragma unroll 1
-            for (int c = 0; c < HD; c += 16) {
+            for (int c = 0; c < D; c += 16) {
               float o[16];
               tmem_ld16(o_addr + c, o);
               tmem_wait_ld();
@@ -527,10 +490,9 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
               tmem_st16(o_addr + c, reinterpret_cast<const uint32_t*>(o));
             }
           }
-          // (the exchanged values are read before the next vote, and written after it)
         }
 #pragma unroll
-        for (int c = 0; c < HN / 32; ++c) {  // 32 keys: 16 columns of P
+        for (int c = 0; c < BN / 32; ++c) {  // 32 keys: 16 columns of P
           uint32_t p[16];
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
@@ -544,23 +506,22 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
             }
             l = fmaf(sum.x + sum.y, sc[2 * c + g].z, l);
           }
-          tmem_st16(s_addr + half * (HN / 2) + 16 * c, p);
+          tmem_st16(s_addr + 16 * c, p);
         }
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(&p_full[s_bar(w, j)]);
+        mbar_arrive(&p_full[at(w, j)]);
       }
-      // ---- epilogue: this part's head-dim elements of O / l
-      if (ok && n > 0) ok = wait(&o_full[2 * w + ((n - 1) & 1)], (n - 1) >> 1);
+      // ---- epilogue: O / l of this row
+      if (ok && n > 0) ok = wait(&o_full[at(w, n - 1)], (n - 1) >> 1);
+      ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
-      // the parts leave together, and know the whole sum
-      if (!pair_or(!ok)) {
-        if (HALVES > 1) l += other(l);
+      if (ok) {
         const float inv = l == 0.f ? 0.f : 1.f / l;  // a NaN sum stays NaN
         const int64_t part = ((int64_t)slot * a.h_k + h) * C::ROWS + w * 128 + t;
-        T* o = static_cast<T*>(a.o) + (int64_t)(q0 + tok) * a.o_stride_tok + hq * a.o_stride_head + half * HD;
+        T* o = static_cast<T*>(a.o) + (int64_t)(q0 + tok) * a.o_stride_tok + hq * a.o_stride_head;
 #pragma unroll 1
-        for (int c = 0; c < HD; c += 16) {
+        for (int c = 0; c < D; c += 16) {
           float v[16];
           if (n > 0) {
             tmem_ld16(o_addr + c, v);
@@ -573,11 +534,11 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
             store8(o + c + 8, v + 8);
           } else if (live) {
 #pragma unroll
-            for (int i = 0; i < 16; i += 8) store8(a.o_part + part * D + half * HD + c + i, v + i);
+            for (int i = 0; i < 16; i += 8) store8(a.o_part + part * D + c + i, v + i);
           }
           __syncwarp();  // the TMEM load is a whole-warp operation
         }
-        if (live && half == 0) {
+        if (live) {
           const float lse = l == 0.f ? -INFINITY : (log2f(l) - nm) * kLn2;
           if (slot >= 0) a.lse_part[part] = lse;
           else if (a.lse) a.lse[(int64_t)(q0 + tok) * a.h_q + hq] = lse;
@@ -646,7 +607,7 @@ static bool make_map(CUtensorMap* m, const void* base, int64_t s_page, int64_t s
   if (!fn) return false;
   // a dimension of extent 1 never moves its coordinate: any legal stride
   const cuuint64_t sr = s_row ? s_row : 16, sh = s_head ? s_head : 16, sp = s_page ? s_page : 16;
-  const int keys = MJ_BLOCK_KEYS(a.head_size), rows = a.page_size < keys ? a.page_size : keys;
+  const int keys = MJ_BLOCK_KEYS, rows = a.page_size < keys ? a.page_size : keys;
   cuuint64_t dims[5] = {128, (cuuint64_t)(a.head_size / 128), (cuuint64_t)a.page_size, (cuuint64_t)a.h_k, (cuuint64_t)a.num_pages};
   cuuint64_t strides[4] = {128, sr, sh, sp};
   cuuint32_t box[5] = {128, 1, (cuuint32_t)rows, 1, 1}, estr[5] = {1, 1, 1, 1, 1};
@@ -666,11 +627,6 @@ static cudaError_t launch_t(const mj_block_attn_args& a, cudaStream_t stream) {
   if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
   if (!ready[dev].load(std::memory_order_acquire)) {
     std::lock_guard<std::mutex> lock(tc_init_mutex());
-    cudaFuncAttributes fa;
-    if ((e = cudaFuncGetAttributes(&fa, kern)) != cudaSuccess) return e;
-    // the register split must fit the launch allocation, or the softmax
-    // warpgroups would wait for registers that never come
-    if (C::REG_LAUNCH && fa.numRegs != C::REG_LAUNCH) return cudaErrorNotSupported;
     if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM)) != cudaSuccess) return e;
     ready[dev].store(1, std::memory_order_release);
   }

@@ -155,8 +155,8 @@ int mj_block_plan(const int32_t* query_lens, const int32_t* seq_lens, int num_se
   if (num_seqs < 0 || h_k <= 0 || h_q <= 0 || h_q % h_k || (head_size != 128 && head_size != 256) || sm_count <= 0 ||
       max_slots < 0 || (num_seqs && (!query_lens || !seq_lens)) || !num_work || !num_merges || !num_slots)
     return mj::set_last_error(MJ_ERR_INVALID, "mj_block_plan: invalid argument");
-  constexpr int kMinPiece = 4;
-  const int h_r = h_q / h_k, rows = MJ_BLOCK_ROWS(head_size), keys = MJ_BLOCK_KEYS(head_size);
+  constexpr int kMinPiece = 8;
+  const int h_r = h_q / h_k, rows = MJ_BLOCK_ROWS(head_size), keys = MJ_BLOCK_KEYS;
   struct Block {
     int32_t seq, row0, tiles;
   };
