@@ -7,8 +7,10 @@
 //   K and V producers    one warp each: page-table walk, one TMA box per page
 //   converter warpgroup  staged V codes e4m3 -> f16 (exact) into the MN-major
 //                        operand tiles; also the tile's block scales
-//   MMA warp             S = Q K^T (kind::f8f6f4, K as stored), O += P V
-//                        (kind::f16, P from TMEM, over the columns of its S)
+//   two MMA warps        S = Q K^T (kind::f8f6f4, K as stored), and O += P V
+//                        (kind::f16, P from TMEM, over the columns of its S);
+//                        a wait costs its warp 100 to 200 cycles even when it
+//                        finds the phase complete, so each has its own
 //   softmax warpgroups   one per row tile, a thread = a row: S to registers,
 //                        online softmax in base 2, P back to TMEM as f16
 // S is double-buffered in TMEM (64 keys a tile, two buffers and O of both row
@@ -25,8 +27,10 @@
 // exponent: z_ij = score_ij + ev_j (base 2), P' = 2^(z - m), O = sum P' vcode /
 // sum P' 2^-ev. The running maximum m is thus over what enters O, so a large V
 // scale cannot push the other rows' P out of f16's range. m moves lazily, when
-// a z exceeds it by 2^8; P' keeps 2^6 of headroom above m so that f16 holds
-// values down to 2^-31 of the maximum.
+// a z exceeds it by 15: moving it means waiting for the last product and
+// rescaling O in TMEM, two thousand cycles of a tile's softmax, and a warp pays
+// for each of its 32 rows (a threshold of 8 did so on most tiles of random
+// scores). f16 holds P' down to 2^-25 of the maximum.
 //
 // Every mbarrier wait is bounded; on a timeout the CTA flags MJ_DEV_TIMEOUT,
 // all roles stop, the copies and MMAs in flight complete and TMEM is freed.
@@ -54,8 +58,7 @@ using namespace sm100;
 
 constexpr uint64_t kWaitNs = 500000000ull;  // per wait; a tile takes microseconds
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kHeadroom = 6.f;            // P' of the running maximum is 2^6
-constexpr float kRaise = kHeadroom + 8.f;   // raise it when a P' would pass 2^14
+constexpr float kRaise = 15.f;  // the running maximum moves when a P' would pass 2^15 (f16's end is 2^16)
 
 template <typename T, int D>
 struct Cfg {
@@ -163,7 +166,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
       mbar_init(&o_full[i], 1);
     }
     mbar_init(q_full, 128 * na);
-    mbar_init(drain, 1);
+    mbar_init(drain, 2);
     *abort_flag = 0;
     never_abort = 0;
     fence_mbar_init();
@@ -213,66 +216,54 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
   };
 
   if (warp < 4) {
-    if (warp == 0) {
-      // ------------------------------------------------------------ MMA issuer
-      // (the whole warp runs the loop, one lane issues: see elect_one)
+    if (warp == 0 || warp == 3) {
+      // ------------------------------------- MMA issuers: warp 0 S, warp 3 O
+      // (a whole warp runs the loop, one lane issues: see elect_one)
       const bool lead = elect_one();
-      auto qk = [&](int w, int j) {  // every term of Q against the same K; 32 head-dim elements a step
+      bool ok = n > 0;
+      if (warp == 0) {
         constexpr uint32_t idesc = idesc_f8f6f4(0, 0, 0, 0, BN);
-        const uint64_t q = smem_desc_sw128(smem_addr(sm + w * C::QTILE), 16, 1024),
-                       k = smem_desc_sw128(smem_addr(sm + C::K_OFF + (j % KST) * C::RAW), 16, 1024);
-        if (lead) {
-#pragma unroll
-          for (int i = 0; i < C::TERMS * (D / 32); ++i) {
-            const int term = i / (D / 32), dh = i % (D / 32) / 4, x = i % 4;
-            mma_f8f6f4(s_col(w, j), q + term * (C::QTERM / 16) + dh * (128 * 8) + x * 2, k + dh * (BN * 8) + x * 2, idesc, i > 0);
-          }
-          mma_commit(&s_full[at(w, j)]);
-        }
-      };
-      auto pv = [&](int w, int j) {  // 16 tokens a step: two 8-row atoms of V, 8 columns of P
-        constexpr uint32_t idesc = idesc_f16(0, 1, D);
-        const uint64_t v = smem_desc_sw128(smem_addr(sm + C::V_OFF + (j % VST) * C::VTILE), BN * 128, 1024);
-        if (lead) {
-#pragma unroll
-          for (int i = 0; i < BN / 16; ++i)
-            mma_f16_ts(C::O_COL + w * 128, s_col(w, j) + i * 8, v + i * 128, idesc, j > 0 || i > 0);
-          mma_commit(&o_full[at(w, j)]);
-        }
-      };
-      auto commit = [&](uint64_t* bar) {
-        if (lead) mma_commit(bar);
-      };
-      bool ok = n > 0 && wait(q_full, 0) && wait(&k_full[0], 0);
-      ok = __all_sync(0xffffffffu, ok);
-      if (ok) {
-        tc_fence_after();
-        for (int w = 0; w < na; ++w) qk(w, 0);
-        commit(&k_empty[0]);
-      }
-      for (int j = 0; ok && j < n; ++j) {
-        if (j + 1 < n) {
-          ok = __all_sync(0xffffffffu, wait(&k_full[(j + 1) % KST], (j + 1) / KST));
+        ok = ok && __all_sync(0xffffffffu, wait(q_full, 0));
+        for (int j = 0; ok && j < n; ++j) {
+          ok = __all_sync(0xffffffffu, wait(&k_full[j % KST], j / KST));
+          const uint64_t k = smem_desc_sw128(smem_addr(sm + C::K_OFF + (j % KST) * C::RAW), 16, 1024);
           for (int w = 0; ok && w < na; ++w) {
-            // S goes over the P of tile j - 1, and MMAs of two kinds are not
-            // ordered with each other: that product has to be complete
-            if (j > 0) ok = __all_sync(0xffffffffu, wait(&o_full[at(w, j - 1)], (j - 1) >> 1));
+            // S goes over the P of tile j - 2: its product has to be complete
+            if (j > 1) ok = __all_sync(0xffffffffu, wait(&o_full[at(w, j)], (j - 2) >> 1));
             if (!ok) break;
             tc_fence_after();
-            qk(w, j + 1);
+            const uint64_t q = smem_desc_sw128(smem_addr(sm + w * C::QTILE), 16, 1024);
+            if (lead) {  // every term of Q against the same K; 32 head-dim elements a step
+#pragma unroll
+              for (int i = 0; i < C::TERMS * (D / 32); ++i) {
+                const int term = i / (D / 32), dh = i % (D / 32) / 4, x = i % 4;
+                mma_f8f6f4(s_col(w, j), q + term * (C::QTERM / 16) + dh * (128 * 8) + x * 2, k + dh * (BN * 8) + x * 2, idesc, i > 0);
+              }
+              mma_commit(&s_full[at(w, j)]);
+            }
           }
-          if (ok) commit(&k_empty[(j + 1) % KST]);
+          if (ok && lead) mma_commit(&k_empty[j % KST]);
         }
-        ok = ok && __all_sync(0xffffffffu, wait(&v_full[j % VST], j / VST));
-        for (int w = 0; ok && w < na; ++w) {
-          ok = __all_sync(0xffffffffu, wait(&p_full[at(w, j)], j >> 1));
-          if (!ok) break;
-          tc_fence_after();
-          pv(w, j);
+      } else {
+        constexpr uint32_t idesc = idesc_f16(0, 1, D);
+        for (int j = 0; ok && j < n; ++j) {
+          ok = __all_sync(0xffffffffu, wait(&v_full[j % VST], j / VST));
+          const uint64_t v = smem_desc_sw128(smem_addr(sm + C::V_OFF + (j % VST) * C::VTILE), BN * 128, 1024);
+          for (int w = 0; ok && w < na; ++w) {
+            ok = __all_sync(0xffffffffu, wait(&p_full[at(w, j)], j >> 1));
+            if (!ok) break;
+            tc_fence_after();
+            if (lead) {  // 16 tokens a step: two 8-row atoms of V, 8 columns of P
+#pragma unroll
+              for (int i = 0; i < BN / 16; ++i)
+                mma_f16_ts(C::O_COL + w * 128, s_col(w, j) + i * 8, v + i * 128, idesc, j > 0 || i > 0);
+              mma_commit(&o_full[at(w, j)]);
+            }
+          }
+          if (ok && lead) mma_commit(&v_empty[j % VST]);
         }
-        if (ok) commit(&v_empty[j % VST]);
       }
-      commit(drain);  // all issued MMAs complete before TMEM is released
+      if (lead) mma_commit(drain);  // all issued MMAs complete before TMEM is released
       mbar_wait(drain, 0, &never_abort, kWaitNs);
     } else if (warp < 3) {
       // ------------------------------------------ producers: warp 1 K, warp 2 V
@@ -429,7 +420,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
         fence_proxy_async_smem();
         mbar_arrive(q_full);
       }
-      // nm: kHeadroom minus the running maximum; a
+      // nm: minus the running maximum; a
       // row that sees no key of the first tile sees none at all (keys are a
       // prefix) and keeps P = 0. l: the row sum.
       float nm = 0.f, l = 0.f;
@@ -471,7 +462,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
         for (int i = 4; i < BN / 2; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], fmaxf(s[i].x, s[i].y));
         float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
         if (__any_sync(0xffffffffu, j == 0 || mx > kRaise)) {
-          const float up = (j == 0 ? mx > -INFINITY : mx > kRaise) ? kHeadroom - mx : 0.f;  // added to nm
+          const float up = (j == 0 ? mx > -INFINITY : mx > kRaise) ? -mx : 0.f;  // added to nm
           nm += up;
 #pragma unroll
           for (int i = 0; i < BN / 2; ++i) s[i] = fadd2(s[i], make_float2(up, up));
