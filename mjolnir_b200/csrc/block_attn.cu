@@ -4,13 +4,15 @@
 // A CTA takes one work item of one KV head: NT tiles of 128 rows -- a row is
 // (query token, head of the KV head's group), so a group shares every key read
 // -- and a range of key tiles of BN tokens. Warp roles:
-//   K and V producers    one warp each: page-table walk, one TMA box per page
+//   producer warp        page-table walk, one TMA box per page of K and of V;
+//                        also the tile's block scales
 //   converter warpgroup  staged V codes e4m3 -> f16 (exact) into the MN-major
-//                        operand tiles; also the tile's block scales
-//   two MMA warps        S = Q K^T (kind::f8f6f4, K as stored), and O += P V
-//                        (kind::f16, P from TMEM, over the columns of its S);
-//                        a wait costs its warp 100 to 200 cycles even when it
-//                        finds the phase complete, so each has its own
+//                        operand tiles
+//   MMA warps            S = Q K^T (kind::f8f6f4, K as stored), one warp for
+//                        each row tile, and O += P V (kind::f16, P from TMEM,
+//                        over the columns of its S). A wait costs its warp 100
+//                        to 200 cycles even when it finds the phase complete,
+//                        so a single issuing warp left the tensor cores idle
 //   softmax warpgroups   one per row tile, a thread = a row: S to registers,
 //                        online softmax in base 2, P back to TMEM as f16
 // S is double-buffered in TMEM (64 keys a tile, two buffers and O of both row
@@ -73,12 +75,14 @@ struct Cfg {
   static constexpr int QTERM = 128 * D, QTILE = TERMS * QTERM;  // one row tile's e4m3 term; all its terms
   static constexpr int RAW = BN * D, VTILE = 2 * RAW;           // a tile's codes; V as f16
   static constexpr int K_OFF = NT * QTILE, R_OFF = K_OFF + KST * RAW, V_OFF = R_OFF + RST * RAW, SC_OFF = V_OFF + VST * VTILE;
-  static constexpr int SC_BYTES = 4 * (BN / 16) * 16;  // four tiles' float4 per 16 tokens
+  static constexpr int SC_SLOTS = 8, SC_BYTES = SC_SLOTS * (BN / 16) * 16;  // a tile's float4 per 16 tokens
   static constexpr int BAR_OFF = SC_OFF + SC_BYTES;
-  static constexpr int NBARS = 18 + 2 * KST + 2 * RST + 2 * VST;
+  static constexpr int NBARS = 14 + 2 * KST + 2 * RST + 2 * VST;
   static constexpr int MISC_OFF = BAR_OFF + NBARS * 8;
   static constexpr int SMEM = MISC_OFF + 16;
-  static_assert(VST <= 3, "the four scale slots cover the tiles in flight");
+  // a slot is written again once K's stage is free, S of KST tiles before: then
+  // the softmax of two tiles before that one is over
+  static_assert(SC_SLOTS >= KST + 2, "scale slots");
   static_assert(SMEM <= 232448, "shared memory of a CTA");
   static constexpr int TMEM_COLS = 512;
   static constexpr int O_COL = 256;
@@ -117,8 +121,8 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::BAR_OFF);
   // s_full, p_full and o_full: [row tile][key tile & 1]
-  uint64_t *sc_full = bars, *s_full = bars + 4, *p_full = bars + 8, *o_full = bars + 12, *q_full = bars + 16,
-           *drain = bars + 17, *k_full = bars + 18, *k_empty = k_full + KST, *r_full = k_empty + KST, *r_empty = r_full + RST,
+  uint64_t *s_full = bars, *p_full = bars + 4, *o_full = bars + 8, *q_full = bars + 12, *drain = bars + 13,
+           *k_full = bars + 14, *k_empty = k_full + KST, *r_full = k_empty + KST, *r_empty = r_full + RST,
            *v_full = r_empty + RST, *v_empty = v_full + VST;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::MISC_OFF);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + C::MISC_OFF + 4);
@@ -149,7 +153,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < KST; ++i) {
       mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 1);
+      mbar_init(&k_empty[i], na);
     }
     for (int i = 0; i < RST; ++i) {
       mbar_init(&r_full[i], 1);
@@ -160,19 +164,20 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
       mbar_init(&v_empty[i], 1);
     }
     for (int i = 0; i < 4; ++i) {
-      mbar_init(&sc_full[i], 1);
-      mbar_init(&s_full[i], 1);
+      mbar_init(&s_full[i], 2);  // the product, and its issuer (who saw the tile's scales)
       mbar_init(&p_full[i], 128);
       mbar_init(&o_full[i], 1);
     }
     mbar_init(q_full, 128 * na);
-    mbar_init(drain, 2);
+    mbar_init(drain, 1 + NT);
     *abort_flag = 0;
     never_abort = 0;
     fence_mbar_init();
   }
-  if (warp == 1 && lane == 0) prefetch_tmap(&tmk);
-  if (warp == 2 && lane == 0) prefetch_tmap(&tmv);
+  if (warp == 1 && lane == 0) {
+    prefetch_tmap(&tmk);
+    prefetch_tmap(&tmv);
+  }
   if (warp == 0) {
     tmem_alloc(tmem_slot, C::TMEM_COLS);
     tmem_relinquish();
@@ -216,35 +221,12 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
   };
 
   if (warp < 4) {
-    if (warp == 0 || warp == 3) {
-      // ------------------------------------- MMA issuers: warp 0 S, warp 3 O
+    if (warp != 1 && (warp == 3 || NT == 2 || warp == 0)) {
+      // ------------------- MMA issuers: warps 0 and 2 S of a row tile, warp 3 O
       // (a whole warp runs the loop, one lane issues: see elect_one)
       const bool lead = elect_one();
       bool ok = n > 0;
-      if (warp == 0) {
-        constexpr uint32_t idesc = idesc_f8f6f4(0, 0, 0, 0, BN);
-        ok = ok && __all_sync(0xffffffffu, wait(q_full, 0));
-        for (int j = 0; ok && j < n; ++j) {
-          ok = __all_sync(0xffffffffu, wait(&k_full[j % KST], j / KST));
-          const uint64_t k = smem_desc_sw128(smem_addr(sm + C::K_OFF + (j % KST) * C::RAW), 16, 1024);
-          for (int w = 0; ok && w < na; ++w) {
-            // S goes over the P of tile j - 2: its product has to be complete
-            if (j > 1) ok = __all_sync(0xffffffffu, wait(&o_full[at(w, j)], (j - 2) >> 1));
-            if (!ok) break;
-            tc_fence_after();
-            const uint64_t q = smem_desc_sw128(smem_addr(sm + w * C::QTILE), 16, 1024);
-            if (lead) {  // every term of Q against the same K; 32 head-dim elements a step
-#pragma unroll
-              for (int i = 0; i < C::TERMS * (D / 32); ++i) {
-                const int term = i / (D / 32), dh = i % (D / 32) / 4, x = i % 4;
-                mma_f8f6f4(s_col(w, j), q + term * (C::QTERM / 16) + dh * (128 * 8) + x * 2, k + dh * (BN * 8) + x * 2, idesc, i > 0);
-              }
-              mma_commit(&s_full[at(w, j)]);
-            }
-          }
-          if (ok && lead) mma_commit(&k_empty[j % KST]);
-        }
-      } else {
+      if (warp == 3) {
         constexpr uint32_t idesc = idesc_f16(0, 1, D);
         for (int j = 0; ok && j < n; ++j) {
           ok = __all_sync(0xffffffffu, wait(&v_full[j % VST], j / VST));
@@ -262,64 +244,106 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
           }
           if (ok && lead) mma_commit(&v_empty[j % VST]);
         }
+      } else if (warp / 2 < na) {
+        const int w = warp / 2;
+        constexpr uint32_t idesc = idesc_f8f6f4(0, 0, 0, 0, BN);
+        const uint64_t q = smem_desc_sw128(smem_addr(sm + w * C::QTILE), 16, 1024);
+        ok = ok && __all_sync(0xffffffffu, wait(&q_full[0], 0));
+        for (int j = 0; ok && j < n; ++j) {
+          ok = wait(&k_full[j % KST], j / KST);
+          // S goes over the P of tile j - 2: its product has to be complete
+          if (j > 1) ok = ok && wait(&o_full[at(w, j)], (j - 2) >> 1);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t k = smem_desc_sw128(smem_addr(sm + C::K_OFF + (j % KST) * C::RAW), 16, 1024);
+          if (lead) {  // every term of Q against the same K; 32 head-dim elements a step
+#pragma unroll
+            for (int i = 0; i < C::TERMS * (D / 32); ++i) {
+              const int term = i / (D / 32), dh = i % (D / 32) / 4, x = i % 4;
+              mma_f8f6f4(s_col(w, j), q + term * (C::QTERM / 16) + dh * (128 * 8) + x * 2, k + dh * (BN * 8) + x * 2, idesc, i > 0);
+            }
+            mma_commit(&s_full[at(w, j)]);
+            mbar_arrive(&s_full[at(w, j)]);
+            mma_commit(&k_empty[j % KST]);
+          }
+        }
       }
       if (lead) mma_commit(drain);  // all issued MMAs complete before TMEM is released
       mbar_wait(drain, 0, &never_abort, kWaitNs);
-    } else if (warp < 3) {
-      // ------------------------------------------ producers: warp 1 K, warp 2 V
-      const bool v = warp == 2;
-      const int st = v ? RST : KST, P = BN / a.page_size, ps = a.page_size;  // pages of a tile: 1 .. 8
-      uint64_t *full = v ? r_full : k_full, *empty = v ? r_empty : k_empty;
-      const CUtensorMap* map = v ? &tmv : &tmk;
-      unsigned char* ring = sm + (v ? C::R_OFF : C::K_OFF);
+    } else if (warp == 1) {
+      // --------------------------------------------------------------- producer
+      const int P = BN / a.page_size, ps = a.page_size;
       const uint64_t policy = l2_policy_evict_normal();  // other row blocks read the same keys
       // lane i < P holds the table entry of the tile's page i (pages may be
       // larger than a tile: then its only box is a part of one)
-      const int pages = P > 0 ? P : 1;
+      const int pages = P > 0 ? P : 1, rows = min(ps, BN);
       auto entries = [&](int j) { return lane < pages ? entry_of(base + j * BN + lane * ps) : kNone; };
       int next = n > 0 ? entries(0) : kNone, issued = 0;
+      // block scales of the tile's 16-token groups: lane i < BN / 16 looks the
+      // page up two tiles ahead and reads the two exponents one tile ahead
+      constexpr uint32_t kOne = 127u | (127u << 8);
+      auto group_entry = [&](int j) { return lane < BN / 16 ? entry_of(base + j * BN + lane * 16) : kNone; };
+      auto exponents = [&](int j, int p) -> uint32_t {
+        if (p < 0) return kOne;
+        const int b = ((base + j * BN + lane * 16) & pmask) >> lg;
+        return __ldg(static_cast<const unsigned char*>(a.k_scales) + p * a.ks_stride_page + b * a.ks_stride_block + h * a.ks_stride_head) |
+               ((uint32_t)__ldg(static_cast<const unsigned char*>(a.v_scales) + p * a.vs_stride_page + b * a.vs_stride_block + h * a.vs_stride_head) << 8);
+      };
+      uint32_t sc_next = kOne;
+      int sc_entry = kNone;
+      if (n > 0) {
+        const int e0 = group_entry(0);
+        sc_entry = group_entry(1);
+        sc_next = exponents(0, page_of(e0));
+      }
       bool ok = true;
       for (int j = 0; j < n; ++j) {
-        const int page = page_of(next), s = j % st;
+        const int page = page_of(next);
+        // an absent page is read out of range: the TMA fills zeros
+        const int where = page < 0 ? (int)a.num_pages : page, r = P > 0 ? 0 : (base + j * BN) & pmask;
         next = entries(j + 1);
-        ok = __all_sync(0xffffffffu, wait(&empty[s], j / st + 1));
+        ok = __all_sync(0xffffffffu, wait(&k_empty[j % KST], j / KST + 1));
         if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(&full[s], C::RAW);
+        if (lane < BN / 16) {
+          const int e = block_e((unsigned char)(sc_next >> 8));
+          reinterpret_cast<float4*>(sm + C::SC_OFF)[(j % C::SC_SLOTS) * (BN / 16) + lane] =
+              make_float4(block_scale((unsigned char)sc_next), (float)(e - 127), __uint_as_float((uint32_t)(254 - e) << 23), 0.f);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(&k_full[j % KST], C::RAW);
         __syncwarp();
         if (lane < pages) {
-          // an absent page is read out of range: the TMA fills zeros
-          const int rows = min(ps, BN), r = P > 0 ? 0 : (base + j * BN) & pmask;
 #pragma unroll
           for (int dh = 0; dh < D / 128; ++dh)
-            tma_load_5d(ring + s * C::RAW + dh * (BN * 128) + lane * rows * 128, map, &full[s], 0, dh, r, h,
-                        page < 0 ? (int)a.num_pages : page, policy);
+            tma_load_5d(sm + C::K_OFF + (j % KST) * C::RAW + dh * (BN * 128) + lane * rows * 128, &tmk, &k_full[j % KST], 0, dh, r, h,
+                        where, policy);
         }
-        issued = j + 1;
+        issued = 2 * j + 1;
+        sc_next = exponents(j + 1, page_of(sc_entry));
+        sc_entry = group_entry(j + 2);
+        ok = __all_sync(0xffffffffu, wait(&r_empty[j % RST], j / RST + 1));
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&r_full[j % RST], C::RAW);
+        __syncwarp();
+        if (lane < pages) {
+#pragma unroll
+          for (int dh = 0; dh < D / 128; ++dh)
+            tma_load_5d(sm + C::R_OFF + (j % RST) * C::RAW + dh * (BN * 128) + lane * rows * 128, &tmv, &r_full[j % RST], 0, dh, r, h,
+                        where, policy);
+        }
+        issued = 2 * j + 2;
       }
-      if (!ok)  // copies in flight land before the CTA exits
-        for (int j = max(issued - st, 0); j < issued; ++j) mbar_wait(&full[j % st], (j / st) & 1, &never_abort, kWaitNs);
+      if (!ok) {  // copies in flight land before the CTA exits
+        const int nk = (issued + 1) / 2, nv = issued / 2;
+        for (int j = max(nk - KST, 0); j < nk; ++j) mbar_wait(&k_full[j % KST], (j / KST) & 1, &never_abort, kWaitNs);
+        for (int j = max(nv - RST, 0); j < nv; ++j) mbar_wait(&r_full[j % RST], (j / RST) & 1, &never_abort, kWaitNs);
+      }
     }
     __syncwarp();
   } else if (warp < 8) {
     // ------------------------------------------------------- converter warpgroup
     const int ct = threadIdx.x - 128;
-    // block scales of the tile's 16-token groups: thread ct < BN / 16 looks the
-    // page up two tiles ahead and reads the two exponents one tile ahead
-    constexpr uint32_t kOne = 127u | (127u << 8);
-    const bool scaler = ct < BN / 16;
-    auto exponents = [&](int pos, int p) -> uint32_t {
-      if (p < 0) return kOne;
-      const int b = (pos & pmask) >> lg;
-      return __ldg(static_cast<const unsigned char*>(a.k_scales) + p * a.ks_stride_page + b * a.ks_stride_block + h * a.ks_stride_head) |
-             ((uint32_t)__ldg(static_cast<const unsigned char*>(a.v_scales) + p * a.vs_stride_page + b * a.vs_stride_block + h * a.vs_stride_head) << 8);
-    };
-    int sc_entry = kNone;
-    uint32_t sc_next = kOne;
-    if (scaler) {
-      const int e0 = entry_of(base + ct * 16);
-      sc_entry = entry_of(base + BN + ct * 16);
-      sc_next = exponents(base + ct * 16, page_of(e0));
-    }
     // Thread ct takes 16-code chunk 4 blk + quad of rows r0, r0 + STEP, ...:
     // eight neighbouring threads are four chunks of a 64-element block in rows
     // r and r ^ 5, so that both their staged reads (swizzled 16-byte chunks of
@@ -359,21 +383,8 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
       mbar_arrive(&v_full[j % VST]);
       return true;
     };
-    for (int j = 0; j < n; ++j) {
-      const int t0 = base + j * BN;
-      if (scaler) {
-        const int e = block_e((unsigned char)(sc_next >> 8));
-        reinterpret_cast<float4*>(sm + C::SC_OFF)[(j & 3) * (BN / 16) + ct] =
-            make_float4(block_scale((unsigned char)sc_next), (float)(e - 127), __uint_as_float((uint32_t)(254 - e) << 23), 0.f);
-        sc_next = exponents(t0 + BN + ct * 16, page_of(sc_entry));
-        sc_entry = entry_of(t0 + 2 * BN + ct * 16);
-      }
-      if (ct < 32) {
-        __syncwarp();
-        if (ct == 0) mbar_arrive(&sc_full[j & 3]);
-      }
+    for (int j = 0; j < n; ++j)
       if (!convert(j)) break;
-    }
   } else {
     // ------------------------------------------------------- softmax warpgroups
     const int w = (warp - 8) >> 2, t = threadIdx.x & 127;
@@ -427,7 +438,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
       bool ok = true;
       const uint32_t o_addr = C::O_COL + w * 128 + lane_base;
       for (int j = 0; j < n; ++j) {
-        ok = wait(&sc_full[j & 3], j >> 2) && wait(&s_full[at(w, j)], j >> 1);
+        ok = wait(&s_full[at(w, j)], j >> 1);
         // every thread leaves the loop with its warp: the TMEM loads are collective
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
@@ -439,7 +450,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
 #pragma unroll
         for (int c = 0; c < BN / 32; ++c) tmem_ld32(s_addr + 32 * c, reinterpret_cast<float*>(s) + 32 * c);
         tmem_wait_ld();
-        const float4* sc = reinterpret_cast<const float4*>(sm + C::SC_OFF) + (j & 3) * (BN / 16);
+        const float4* sc = reinterpret_cast<const float4*>(sm + C::SC_OFF) + (j % C::SC_SLOTS) * (BN / 16);
 #pragma unroll
         for (int g = 0; g < BN / 16; ++g) {
           const float4 f = sc[g];
