@@ -4,15 +4,16 @@
 // A CTA takes one work item of one KV head: NT tiles of 128 rows -- a row is
 // (query token, head of the KV head's group), so a group shares every key read
 // -- and a range of key tiles of BN tokens. Warp roles:
-//   producer warp        page-table walk, one TMA box per page of K and of V;
-//                        also the tile's block scales
+//   producer warps       one for K and the tile's block scales, one for V:
+//                        page-table walk, one TMA box per page
 //   converter warpgroup  staged V codes e4m3 -> f16 (exact) into the MN-major
 //                        operand tiles
-//   MMA warps            S = Q K^T (kind::f8f6f4, K as stored), one warp for
-//                        each row tile, and O += P V (kind::f16, P from TMEM,
-//                        over the columns of its S). A wait costs its warp 100
-//                        to 200 cycles even when it finds the phase complete,
-//                        so a single issuing warp left the tensor cores idle
+//   MMA warps            one per row tile: S = Q K^T (kind::f8f6f4, K as
+//                        stored) of the next key tile, then O += P V of this
+//                        one (kind::f16, P from TMEM, over the columns of its
+//                        S). A wait costs its warp 100 to 200 cycles even when
+//                        it finds the phase complete: one issuing warp for both
+//                        row tiles left the tensor cores idle
 //   softmax warpgroups   one per row tile, a thread = a row: S to registers,
 //                        online softmax in base 2, P back to TMEM as f16
 // S is double-buffered in TMEM (64 keys a tile, two buffers and O of both row
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
     }
     for (int i = 0; i < VST; ++i) {
       mbar_init(&v_full[i], 128);
-      mbar_init(&v_empty[i], 1);
+      mbar_init(&v_empty[i], na);
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 2);  // the product, and its issuer (who saw the tile's scales)
@@ -169,7 +170,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
       mbar_init(&o_full[i], 1);
     }
     mbar_init(q_full, 128 * na);
-    mbar_init(drain, 1 + NT);
+    mbar_init(drain, na);
     *abort_flag = 0;
     never_abort = 0;
     fence_mbar_init();
@@ -220,125 +221,116 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
     return -1;
   };
 
+  // Producer loop over one operand's ring: wait for the stage, `before`, then a
+  // TMA box per page. Lane i < pages holds the table entry of the tile's page i
+  // (a page may be larger than a tile: then the only box is a part of one).
+  auto produce = [&](const CUtensorMap& map, int off, int stages, uint64_t* full, uint64_t* empty, auto before) {
+    const uint64_t policy = l2_policy_evict_normal();  // other row blocks read the same keys
+    const int ps = a.page_size, pages = max(BN / ps, 1), rows = min(ps, BN);
+    auto entries = [&](int j) { return lane < pages ? entry_of(base + j * BN + lane * ps) : kNone; };
+    int next = n > 0 ? entries(0) : kNone, j = 0;
+    bool ok = true;
+    for (; j < n; ++j) {
+      // an absent page is read out of range: the TMA fills zeros
+      const int page = page_of(next), where = page < 0 ? (int)a.num_pages : page;
+      const int row = ps > BN ? (base + j * BN) & pmask : 0, s = j % stages;
+      next = entries(j + 1);
+      ok = __all_sync(0xffffffffu, wait(&empty[s], j / stages + 1));
+      if (!ok) break;
+      before(j);
+      if (lane == 0) mbar_arrive_expect_tx(&full[s], C::RAW);
+      __syncwarp();
+      if (lane < pages) {
+#pragma unroll
+        for (int dh = 0; dh < D / 128; ++dh)
+          tma_load_5d(sm + off + s * C::RAW + dh * (BN * 128) + lane * rows * 128, &map, &full[s], 0, dh, row, h, where, policy);
+      }
+    }
+    if (!ok)  // copies in flight land before the CTA exits
+      for (int i = max(j - stages, 0); i < j; ++i) mbar_wait(&full[i % stages], (i / stages) & 1, &never_abort, kWaitNs);
+  };
+
   if (warp < 4) {
-    if (warp != 1 && (warp == 3 || NT == 2 || warp == 0)) {
-      // ------------------- MMA issuers: warps 0 and 2 S of a row tile, warp 3 O
-      // (a whole warp runs the loop, one lane issues: see elect_one)
+    const int w = warp >> 1;
+    if (!(warp & 1) && w < na) {
+      // --------------------------------------------------- MMAs of row tile w
+      // (the whole warp runs the loop, one lane issues: see elect_one)
       const bool lead = elect_one();
-      bool ok = n > 0;
-      if (warp == 3) {
-        constexpr uint32_t idesc = idesc_f16(0, 1, D);
-        for (int j = 0; ok && j < n; ++j) {
-          ok = __all_sync(0xffffffffu, wait(&v_full[j % VST], j / VST));
-          const uint64_t v = smem_desc_sw128(smem_addr(sm + C::V_OFF + (j % VST) * C::VTILE), BN * 128, 1024);
-          for (int w = 0; ok && w < na; ++w) {
-            ok = __all_sync(0xffffffffu, wait(&p_full[at(w, j)], j >> 1));
-            if (!ok) break;
-            tc_fence_after();
-            if (lead) {  // 16 tokens a step: two 8-row atoms of V, 8 columns of P
-#pragma unroll
-              for (int i = 0; i < BN / 16; ++i)
-                mma_f16_ts(C::O_COL + w * 128, s_col(w, j) + i * 8, v + i * 128, idesc, j > 0 || i > 0);
-              mma_commit(&o_full[at(w, j)]);
-            }
-          }
-          if (ok && lead) mma_commit(&v_empty[j % VST]);
-        }
-      } else if (warp / 2 < na) {
-        const int w = warp / 2;
+      const uint64_t q = smem_desc_sw128(smem_addr(sm + w * C::QTILE), 16, 1024);
+      auto scores = [&](int j) -> bool {  // every term of Q against the same K; 32 head-dim elements a step
         constexpr uint32_t idesc = idesc_f8f6f4(0, 0, 0, 0, BN);
-        const uint64_t q = smem_desc_sw128(smem_addr(sm + w * C::QTILE), 16, 1024);
-        ok = ok && __all_sync(0xffffffffu, wait(&q_full[0], 0));
-        for (int j = 0; ok && j < n; ++j) {
-          ok = wait(&k_full[j % KST], j / KST);
-          // S goes over the P of tile j - 2: its product has to be complete
-          if (j > 1) ok = ok && wait(&o_full[at(w, j)], (j - 2) >> 1);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          tc_fence_after();
-          const uint64_t k = smem_desc_sw128(smem_addr(sm + C::K_OFF + (j % KST) * C::RAW), 16, 1024);
-          if (lead) {  // every term of Q against the same K; 32 head-dim elements a step
+        bool ok = wait(&k_full[j % KST], j / KST);
+        // S goes over the P of tile j - 2, and MMAs of two kinds are not ordered
+        // with each other: that product has to be complete
+        if (j > 1) ok = ok && wait(&o_full[at(w, j)], (j - 2) >> 1);
+        if (!__all_sync(0xffffffffu, ok)) return false;
+        tc_fence_after();
+        const uint64_t k = smem_desc_sw128(smem_addr(sm + C::K_OFF + (j % KST) * C::RAW), 16, 1024);
+        if (lead) {
 #pragma unroll
-            for (int i = 0; i < C::TERMS * (D / 32); ++i) {
-              const int term = i / (D / 32), dh = i % (D / 32) / 4, x = i % 4;
-              mma_f8f6f4(s_col(w, j), q + term * (C::QTERM / 16) + dh * (128 * 8) + x * 2, k + dh * (BN * 8) + x * 2, idesc, i > 0);
-            }
-            mma_commit(&s_full[at(w, j)]);
-            mbar_arrive(&s_full[at(w, j)]);
-            mma_commit(&k_empty[j % KST]);
+          for (int i = 0; i < C::TERMS * (D / 32); ++i) {
+            const int term = i / (D / 32), dh = i % (D / 32) / 4, x = i % 4;
+            mma_f8f6f4(s_col(w, j), q + term * (C::QTERM / 16) + dh * (128 * 8) + x * 2, k + dh * (BN * 8) + x * 2, idesc, i > 0);
           }
+          mma_commit(&s_full[at(w, j)]);
+          mbar_arrive(&s_full[at(w, j)]);
+          mma_commit(&k_empty[j % KST]);
+        }
+        return true;
+      };
+      bool ok = n > 0 && __all_sync(0xffffffffu, wait(q_full, 0)) && scores(0);
+      for (int j = 0; ok && j < n; ++j) {
+        if (j + 1 < n) ok = scores(j + 1);
+        ok = ok && wait(&v_full[j % VST], j / VST) && wait(&p_full[at(w, j)], j >> 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t v = smem_desc_sw128(smem_addr(sm + C::V_OFF + (j % VST) * C::VTILE), BN * 128, 1024);
+        if (lead) {  // 16 tokens a step: two 8-row atoms of V, 8 columns of P
+          constexpr uint32_t idesc = idesc_f16(0, 1, D);
+#pragma unroll
+          for (int i = 0; i < BN / 16; ++i)
+            mma_f16_ts(C::O_COL + w * 128, s_col(w, j) + i * 8, v + i * 128, idesc, j > 0 || i > 0);
+          mma_commit(&o_full[at(w, j)]);
+          mma_commit(&v_empty[j % VST]);
         }
       }
       if (lead) mma_commit(drain);  // all issued MMAs complete before TMEM is released
       mbar_wait(drain, 0, &never_abort, kWaitNs);
     } else if (warp == 1) {
-      // --------------------------------------------------------------- producer
-      const int P = BN / a.page_size, ps = a.page_size;
-      const uint64_t policy = l2_policy_evict_normal();  // other row blocks read the same keys
-      // lane i < P holds the table entry of the tile's page i (pages may be
-      // larger than a tile: then its only box is a part of one)
-      const int pages = P > 0 ? P : 1, rows = min(ps, BN);
-      auto entries = [&](int j) { return lane < pages ? entry_of(base + j * BN + lane * ps) : kNone; };
-      int next = n > 0 ? entries(0) : kNone, issued = 0;
-      // block scales of the tile's 16-token groups: lane i < BN / 16 looks the
+      // -------------------------------------------------- producer: K and scales
+      // Block scales of the tile's 16-token groups: lane i < BN / 16 looks the
       // page up two tiles ahead and reads the two exponents one tile ahead
-      constexpr uint32_t kOne = 127u | (127u << 8);
+      // (into registers that nothing combines before their tile: a use of them
+      // would wait the memory round trip).
       auto group_entry = [&](int j) { return lane < BN / 16 ? entry_of(base + j * BN + lane * 16) : kNone; };
-      auto exponents = [&](int j, int p) -> uint32_t {
-        if (p < 0) return kOne;
+      unsigned char next_k = 127, next_v = 127;
+      auto exponents = [&](int j, int p) {
+        next_k = next_v = 127;
+        if (p < 0) return;
         const int b = ((base + j * BN + lane * 16) & pmask) >> lg;
-        return __ldg(static_cast<const unsigned char*>(a.k_scales) + p * a.ks_stride_page + b * a.ks_stride_block + h * a.ks_stride_head) |
-               ((uint32_t)__ldg(static_cast<const unsigned char*>(a.v_scales) + p * a.vs_stride_page + b * a.vs_stride_block + h * a.vs_stride_head) << 8);
+        next_k = __ldg(static_cast<const unsigned char*>(a.k_scales) + p * a.ks_stride_page + b * a.ks_stride_block + h * a.ks_stride_head);
+        next_v = __ldg(static_cast<const unsigned char*>(a.v_scales) + p * a.vs_stride_page + b * a.vs_stride_block + h * a.vs_stride_head);
       };
-      uint32_t sc_next = kOne;
       int sc_entry = kNone;
       if (n > 0) {
         const int e0 = group_entry(0);
         sc_entry = group_entry(1);
-        sc_next = exponents(0, page_of(e0));
+        exponents(0, page_of(e0));
       }
-      bool ok = true;
-      for (int j = 0; j < n; ++j) {
-        const int page = page_of(next);
-        // an absent page is read out of range: the TMA fills zeros
-        const int where = page < 0 ? (int)a.num_pages : page, r = P > 0 ? 0 : (base + j * BN) & pmask;
-        next = entries(j + 1);
-        ok = __all_sync(0xffffffffu, wait(&k_empty[j % KST], j / KST + 1));
-        if (!ok) break;
+      produce(tmk, C::K_OFF, KST, k_full, k_empty, [&](int j) {
         if (lane < BN / 16) {
-          const int e = block_e((unsigned char)(sc_next >> 8));
+          const int e = block_e(next_v);
           reinterpret_cast<float4*>(sm + C::SC_OFF)[(j % C::SC_SLOTS) * (BN / 16) + lane] =
-              make_float4(block_scale((unsigned char)sc_next), (float)(e - 127), __uint_as_float((uint32_t)(254 - e) << 23), 0.f);
+              make_float4(block_scale(next_k), (float)(e - 127), __uint_as_float((uint32_t)(254 - e) << 23), 0.f);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive_expect_tx(&k_full[j % KST], C::RAW);
-        __syncwarp();
-        if (lane < pages) {
-#pragma unroll
-          for (int dh = 0; dh < D / 128; ++dh)
-            tma_load_5d(sm + C::K_OFF + (j % KST) * C::RAW + dh * (BN * 128) + lane * rows * 128, &tmk, &k_full[j % KST], 0, dh, r, h,
-                        where, policy);
-        }
-        issued = 2 * j + 1;
-        sc_next = exponents(j + 1, page_of(sc_entry));
+        exponents(j + 1, page_of(sc_entry));
         sc_entry = group_entry(j + 2);
-        ok = __all_sync(0xffffffffu, wait(&r_empty[j % RST], j / RST + 1));
-        if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(&r_full[j % RST], C::RAW);
-        __syncwarp();
-        if (lane < pages) {
-#pragma unroll
-          for (int dh = 0; dh < D / 128; ++dh)
-            tma_load_5d(sm + C::R_OFF + (j % RST) * C::RAW + dh * (BN * 128) + lane * rows * 128, &tmv, &r_full[j % RST], 0, dh, r, h,
-                        where, policy);
-        }
-        issued = 2 * j + 2;
-      }
-      if (!ok) {  // copies in flight land before the CTA exits
-        const int nk = (issued + 1) / 2, nv = issued / 2;
-        for (int j = max(nk - KST, 0); j < nk; ++j) mbar_wait(&k_full[j % KST], (j / KST) & 1, &never_abort, kWaitNs);
-        for (int j = max(nv - RST, 0); j < nv; ++j) mbar_wait(&r_full[j % RST], (j / RST) & 1, &never_abort, kWaitNs);
-      }
+        __syncwarp();  // the scales are written before lane 0 arrives on k_full
+      });
+    } else if (warp == 3) {
+      // ------------------------------------------------------------ producer: V
+      produce(tmv, C::R_OFF, RST, r_full, r_empty, [](int) {});
     }
     __syncwarp();
   } else if (warp < 8) {

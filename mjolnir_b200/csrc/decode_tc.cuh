@@ -838,8 +838,7 @@ __global__ void __launch_bounds__(Cfg<FMT, NQP, NWG, CVTW, DH>::THREADS, Cfg<FMT
       const int nsp = a.n_splits[seq];
       const int row0 = g * RT + col0;
       // block scales: this thread's KV row of tile i is in page_nx's block; the
-      // page is looked up two tiles ahead, the exponent bytes (K low, V << 8)
-      // one tile ahead
+      // page is looked up two tiles ahead, the exponent bytes one tile ahead
       const int blk_lg = Fmt<FMT>::BLOCK ? block_log2(a.kv_format) : 0;
       auto scale_page = [&](int tile) -> int {  // -1: no such row, or a bad entry (the producer flags it)
         const int row = tile * kTileRows + t;
@@ -847,11 +846,13 @@ __global__ void __launch_bounds__(Cfg<FMT, NQP, NWG, CVTW, DH>::THREADS, Cfg<FMT
         const int pg = __ldg(a.block_table + (int64_t)seq * a.block_table_stride + row / a.page_size);
         return pg < 0 || pg >= a.num_pages ? -1 : pg;
       };
-      auto scale_bytes = [&](int tile, int pg) -> uint32_t {
-        if (pg < 0) return 127u | (127u << 8);  // scales of 1 (such rows are zeros or masked)
+      unsigned char sck_nx = 127, scv_nx = 127;
+      auto scale_bytes = [&](int tile, int pg) {  // into registers that nothing combines before their tile: a use would wait for them
+        sck_nx = scv_nx = 127;  // scales of 1 where there is no row (such rows are zeros or masked)
+        if (pg < 0) return;
         const int b = ((tile * kTileRows + t) & (a.page_size - 1)) >> blk_lg;
-        return __ldg(static_cast<const unsigned char*>(a.k_scales) + pg * a.ks_stride_page + b * a.ks_stride_row + h * a.ks_stride_head) |
-               ((uint32_t)__ldg(static_cast<const unsigned char*>(a.v_scales) + pg * a.vs_stride_page + b * a.vs_stride_row + h * a.vs_stride_head) << 8);
+        sck_nx = __ldg(static_cast<const unsigned char*>(a.k_scales) + pg * a.ks_stride_page + b * a.ks_stride_row + h * a.ks_stride_head);
+        scv_nx = __ldg(static_cast<const unsigned char*>(a.v_scales) + pg * a.vs_stride_page + b * a.vs_stride_row + h * a.vs_stride_head);
       };
       int page_cur = -1, page_nx = -1;
       if constexpr (Fmt<FMT>::BLOCK) {
@@ -922,7 +923,7 @@ __global__ void __launch_bounds__(Cfg<FMT, NQP, NWG, CVTW, DH>::THREADS, Cfg<FMT
       const float kd = descale_at(a.k_descale, a.k_descale_mode, seq, h, h_k);
       const float vd = descale_at(a.v_descale, a.v_descale_mode, seq, h, h_k);
       const float c2 = a.softmax_scale * kd * kLog2e / qs;  // S (in q*qs units) -> log2 units
-      uint32_t sc_nx = Fmt<FMT>::BLOCK ? scale_bytes(tb, page_cur) : 0u;
+      if constexpr (Fmt<FMT>::BLOCK) scale_bytes(tb, page_cur);
       if (named_bar_or(bar_id, 128, *abort_flag != 0)) break;  // Q written and fenced, red[] read
       if (t == 0) mbar_arrive(&b.q_full[jc & 1]);
       ++jc;
@@ -960,12 +961,12 @@ __global__ void __launch_bounds__(Cfg<FMT, NQP, NWG, CVTW, DH>::THREADS, Cfg<FMT
         // this tile's scale of the scores, addend of the exponents and factor of the row sums
         float2 c2t = c2v, ev2 = make_float2(0.f, 0.f), inv2 = make_float2(1.f, 1.f);
         if constexpr (Fmt<FMT>::BLOCK) {
-          const int ek = block_e((unsigned char)sc_nx), ev = block_e((unsigned char)(sc_nx >> 8));
+          const int ek = block_e(sck_nx), ev = block_e(scv_nx);
           const float c = c2 * __uint_as_float((uint32_t)ek << 23), v = (float)(ev - 127), u = __uint_as_float((uint32_t)(254 - ev) << 23);
           c2t = make_float2(c, c);
           ev2 = make_float2(v, v);
           inv2 = make_float2(u, u);
-          sc_nx = scale_bytes(tb + i + 1, page_nx);
+          scale_bytes(tb + i + 1, page_nx);
           page_nx = scale_page(tb + i + 2);
         }
         if (!mbar_wait(&b.s_full[it & 1], (it >> 1) & 1, abort_flag, wait_ns) && !*abort_flag) give_up();
