@@ -93,24 +93,35 @@ struct Cfg {
 __device__ __forceinline__ uint32_t unit_offset(uint32_t r, uint32_t u) { return r * 128 + ((u ^ (r & 7)) << 4); }
 
 // 8 values -> TERMS rows of e4m3 codes, each the rounded rest of those before
-// (exact differences); a value that is not finite makes its first code NaN
+// (exact differences; NaN stays NaN in the first)
 template <int TERMS>
-__device__ __forceinline__ void split_terms(float* v, uint2* out) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (!(fabsf(v[i]) <= 3.402823466e38f)) v[i] = __int_as_float(0x7FFFFFFF);
+__device__ __forceinline__ void split_terms(float2* v, uint2* out) {
 #pragma unroll
   for (int k = 0; k < TERMS; ++k) {
     uint16_t c[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      c[i] = f2_to_e4m3x2(v[2 * i], v[2 * i + 1]);
+      c[i] = f2_to_e4m3x2(v[i].x, v[i].y);
       const float2 f = e4m3x2_to_f2(c[i]);
-      v[2 * i] -= f.x, v[2 * i + 1] -= f.y;
+      v[i] = fadd2(v[i], make_float2(-f.x, -f.y));
     }
     out[k] = make_uint2(c[0] | ((uint32_t)c[1] << 16), c[2] | ((uint32_t)c[3] << 16));
   }
 }
+
+// two packed 16-bit values
+__device__ __forceinline__ float2 up2(__nv_bfloat162 v) { return __bfloat1622float2(v); }
+__device__ __forceinline__ float2 up2(__half2 v) { return __half22float2(v); }
+template <typename T>
+struct Pair;
+template <>
+struct Pair<__half> {
+  typedef __half2 type;
+};
+template <>
+struct Pair<__nv_bfloat16> {
+  typedef __nv_bfloat162 type;
+};
 
 template <typename T, int D>
 __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
@@ -388,38 +399,49 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
       const int lim = !live ? -1 : a.causal ? L - n_tok + tok : L - 1;  // the last key this row sees
       // the first row of the warp sees the fewest keys
       const int warp_lim = __shfl_sync(0xffffffffu, lim, 0);
-      // ---- Q: this row in TERMS e4m3 terms into the K-major tiles (dead rows are zeros)
+      // ---- Q: the warp's rows in TERMS e4m3 terms into the K-major tiles. D / 8
+      // lanes read a row, eight reads of each lane in flight; the row's owner
+      // hands its address round and gets its power of two back.
       float c2 = a.softmax_scale * kLog2e;
       {
-        const T* q = static_cast<const T*>(a.q) + (int64_t)(q0 + tok) * a.q_stride_tok + hq * a.q_stride_head;
+        typedef typename Pair<T>::type T2;
+        constexpr int LPR = D / 8, RPI = 32 / LPR, BATCH = 8;  // lanes of a row, rows of a pass, passes in flight
+        const int c = lane % LPR, wr = (warp & 3) * 32;
+        const int64_t q_off = (int64_t)(q0 + tok) * a.q_stride_tok + hq * a.q_stride_head;
         unsigned char* qs = sm + w * C::QTILE;
-        float amax = 0.f;
-#pragma unroll 4
-        for (int c = 0; c < D / 8; ++c) {
-          float v[8];
-          load8(q + 8 * c, v);
+        int mine = 0;  // the power of two of this thread's row
+#pragma unroll 1
+        for (int i0 = 0; i0 < 32 / RPI; i0 += BATCH) {
+          uint4 raw[BATCH];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) amax = fabsf(v[i]) <= 3.402823466e38f ? fmaxf(amax, fabsf(v[i])) : amax;
+          for (int i = 0; i < BATCH; ++i)
+            raw[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) +
+                                                     __shfl_sync(0xffffffffu, q_off, (i0 + i) * RPI + lane / LPR) + 8 * c);
+#pragma unroll
+          for (int i = 0; i < BATCH; ++i) {
+            const int lr = wr + (i0 + i) * RPI + lane / LPR;  // row of the tile
+            const T2* e = reinterpret_cast<const T2*>(&raw[i]);
+            const float2 m2 = up2(__hmax2(__hmax2(__habs2(e[0]), __habs2(e[1])), __hmax2(__habs2(e[2]), __habs2(e[3]))));
+            float amax = fmaxf(m2.x, m2.y);  // NaN elements do not count
+#pragma unroll
+            for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            // 2^k with amax 2^k in [128, 256), inside fp32's normal range; a row
+            // with an infinity has no finite output and becomes NaN
+            const int k = amax > 0.f ? min(max(134 - (int)(__float_as_uint(amax) >> 23), -126), 126) : 0;
+            const float up = amax == INFINITY ? __int_as_float(0x7FFFFFFF) : __uint_as_float((uint32_t)(127 + k) << 23);
+            float2 v[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) v[x] = fmul2(up2(e[x]), make_float2(up, up));
+            uint2 terms[C::TERMS];
+            split_terms<C::TERMS>(v, terms);
+#pragma unroll
+            for (int x = 0; x < C::TERMS; ++x)
+              *reinterpret_cast<uint2*>(qs + x * C::QTERM + (c >> 4) * (128 * 128) + unit_offset(lr, (c >> 1) & 7) + (c & 1) * 8) = terms[x];
+            const int got = __shfl_sync(0xffffffffu, k, (lane % RPI) * LPR);  // row i * RPI + lane % RPI
+            if (lane / RPI == i0 + i) mine = got;
+          }
         }
-        // 2^k with amax 2^k in [128, 256), inside fp32's normal range
-        const int k = amax > 0.f ? min(max(134 - (int)(__float_as_uint(amax) >> 23), -126), 126) : 0;
-        const float up = __uint_as_float((uint32_t)(127 + k) << 23);
-        c2 *= __uint_as_float((uint32_t)(127 - k) << 23);
-#pragma unroll 2
-        for (int c = 0; c < D / 16; ++c) {
-          float v[16];
-          load8(q + 16 * c, v);
-          load8(q + 16 * c + 8, v + 8);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] = live ? v[i] * up : 0.f;
-          uint2 lo[C::TERMS], hi[C::TERMS];
-          split_terms<C::TERMS>(v, lo);
-          split_terms<C::TERMS>(v + 8, hi);
-#pragma unroll
-          for (int i = 0; i < C::TERMS; ++i)
-            *reinterpret_cast<uint4*>(qs + i * C::QTERM + (c >> 3) * (128 * 128) + unit_offset(t, c & 7)) =
-                make_uint4(lo[i].x, lo[i].y, hi[i].x, hi[i].y);
-        }
+        c2 *= __uint_as_float((uint32_t)(127 - mine) << 23);
         fence_proxy_async_smem();
         mbar_arrive(q_full);
       }
@@ -513,24 +535,39 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
       if (ok) {
         const float inv = l == 0.f ? 0.f : 1.f / l;  // a NaN sum stays NaN
         const int64_t part = ((int64_t)slot * a.h_k + h) * C::ROWS + w * 128 + t;
-        T* o = static_cast<T*>(a.o) + (int64_t)(q0 + tok) * a.o_stride_tok + hq * a.o_stride_head;
+        const int64_t o_off = (int64_t)(q0 + tok) * a.o_stride_tok + hq * a.o_stride_head;
+        // final rows go through shared memory (this warp's part of the Q tile,
+        // which no MMA reads any more), so that D / 8 lanes write a row
+        constexpr int LPR = D / 8, RPI = 32 / LPR;
+        unsigned char* stage = sm + w * C::QTILE + (warp & 3) * (32 * D * 2);
 #pragma unroll 1
-        for (int c = 0; c < D; c += 16) {
-          float v[16];
+        for (int c = 0; c < D; c += 32) {
+          float v[32];
           if (n > 0) {
-            tmem_ld16(o_addr + c, v);
+            tmem_ld32(o_addr + c, v);
             tmem_wait_ld();
           }
 #pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] = l == 0.f ? 0.f : v[i] * inv;
-          if (live && slot < 0) {
-            store8(o + c, v);
-            store8(o + c + 8, v + 8);
+          for (int i = 0; i < 32; ++i) v[i] = l == 0.f ? 0.f : v[i] * inv;
+          if (slot < 0) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8)
+              store8(reinterpret_cast<T*>(stage + lane * (D * 2) + ((((c + i) >> 3) ^ (lane & 7)) << 4)), v + i);
           } else if (live) {
 #pragma unroll
-            for (int i = 0; i < 16; i += 8) store8(a.o_part + part * D + c + i, v + i);
+            for (int i = 0; i < 32; i += 8) store8(a.o_part + part * D + c + i, v + i);
           }
           __syncwarp();  // the TMEM load is a whole-warp operation
+        }
+        if (slot < 0) {
+          const int rows_here = min(max(n_rows - (row0 + w * 128 + (warp & 3) * 32), 0), 32);
+#pragma unroll 4
+          for (int i = 0; i < 32 / RPI; ++i) {
+            const int r = i * RPI + lane / LPR;
+            const int64_t at_row = __shfl_sync(0xffffffffu, o_off, r);
+            const uint4 x = *reinterpret_cast<const uint4*>(stage + r * (D * 2) + (((lane % LPR) ^ (r & 7)) << 4));
+            if (r < rows_here) *reinterpret_cast<uint4*>(static_cast<T*>(a.o) + at_row + 8 * (lane % LPR)) = x;
+          }
         }
         if (live) {
           const float lse = l == 0.f ? -INFINITY : (log2f(l) - nm) * kLn2;
