@@ -60,6 +60,7 @@ namespace ba {
 using namespace sm100;
 
 constexpr uint64_t kWaitNs = 500000000ull;  // per wait; a tile takes microseconds
+constexpr int kPolyOf4 = 1;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kRaise = 15.f;  // the running maximum moves when a P' would pass 2^15 (f16's end is 2^16)
 
@@ -107,6 +108,24 @@ __device__ __forceinline__ void split_terms(float2* v, uint2* out) {
     }
     out[k] = make_uint2(c[0] | ((uint32_t)c[1] << 16), c[2] | ((uint32_t)c[3] << 16));
   }
+}
+
+// 2^x of two values, x <= 15, without the special-function unit: x = n + f with
+// |f| <= 1/2 (adding 1.5 * 2^23 rounds to n, in the low bits), 2^f by the
+// degree-4 polynomial through the Chebyshev nodes of [-1/2, 1/2] (relative
+// error 4e-6, under P's 2^-11), n into the exponent field. Below 2^-125 it
+// gives 2^-125, which is 0 in f16.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  const float2 magic = make_float2(12582912.f, 12582912.f), down = make_float2(-12582912.f, -12582912.f);
+  x = make_float2(fmaxf(x.x, -125.f), fmaxf(x.y, -125.f));
+  const float2 t = fadd2(x, magic), n = fadd2(t, down), f = fadd2(x, make_float2(-n.x, -n.y));
+  auto c = [](float v) { return make_float2(v, v); };
+  float2 p = ffma2(f, c(0.009666369f), c(0.055921976f));
+  p = ffma2(p, f, c(0.240223490f));
+  p = ffma2(p, f, c(0.693121045f));
+  p = ffma2(p, f, c(1.000000000f));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
 // two packed 16-bit values
@@ -516,7 +535,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const float2 d = s[16 * c + 8 * g + i];
-              const float2 e = make_float2(exp2_approx(d.x), exp2_approx(d.y));
+              const float2 e = i % 4 < kPolyOf4 ? exp2_poly(d) : make_float2(exp2_approx(d.x), exp2_approx(d.y));
               sum = fadd2(sum, e);
               p[8 * g + i] = f2_to_h2(e.x, e.y);
             }
@@ -533,6 +552,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
       if (ok) {
+        if (lim < base) l = 0.f;  // no key in this item (exp2_poly's zero is 2^-125)
         const float inv = l == 0.f ? 0.f : 1.f / l;  // a NaN sum stays NaN
         const int64_t part = ((int64_t)slot * a.h_k + h) * C::ROWS + w * 128 + t;
         const int64_t o_off = (int64_t)(q0 + tok) * a.o_stride_tok + hq * a.o_stride_head;
