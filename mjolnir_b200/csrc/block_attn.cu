@@ -4,8 +4,8 @@
 // A CTA takes one work item of one KV head: NT tiles of 128 rows -- a row is
 // (query token, head of the KV head's group), so a group shares every key read
 // -- and a range of key tiles of BN tokens. Warp roles:
-//   producer warps       one for K and the tile's block scales, one for V:
-//                        page-table walk, one TMA box per page
+//   producer warps       one for K, one for V and the tile's block scales: page-
+//                        table walk, one TMA box per page
 //   converter warpgroup  staged V codes e4m3 -> f16 (exact) into the MN-major
 //                        operand tiles
 //   MMA warps            one per row tile: S = Q K^T (kind::f8f6f4, K as
@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < KST; ++i) {
-      mbar_init(&k_full[i], 1);
+      mbar_init(&k_full[i], 2);  // K's copies, and the tile's scales
       mbar_init(&k_empty[i], na);
     }
     for (int i = 0; i < RST; ++i) {
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
     return -1;
   };
 
-  // Producer loop over one operand's ring: wait for the stage, `before`, then a
+  // Producer loop over one operand's ring: `before`, wait for the stage, then a
   // TMA box per page. Lane i < pages holds the table entry of the tile's page i
   // (a page may be larger than a tile: then the only box is a part of one).
   auto produce = [&](const CUtensorMap& map, int off, int stages, uint64_t* full, uint64_t* empty, auto before) {
@@ -265,9 +265,8 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
       const int page = page_of(next), where = page < 0 ? (int)a.num_pages : page;
       const int row = ps > BN ? (base + j * BN) & pmask : 0, s = j % stages;
       next = entries(j + 1);
-      ok = __all_sync(0xffffffffu, wait(&empty[s], j / stages + 1));
+      ok = before(j) && __all_sync(0xffffffffu, wait(&empty[s], j / stages + 1));
       if (!ok) break;
-      before(j);
       if (lane == 0) mbar_arrive_expect_tx(&full[s], C::RAW);
       __syncwarp();
       if (lane < pages) {
@@ -328,11 +327,14 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
       if (lead) mma_commit(drain);  // all issued MMAs complete before TMEM is released
       mbar_wait(drain, 0, &never_abort, kWaitNs);
     } else if (warp == 1) {
-      // -------------------------------------------------- producer: K and scales
+      // ------------------------------------------------------------ producer: K
+      produce(tmk, C::K_OFF, KST, k_full, k_empty, [](int) { return true; });
+    } else if (warp == 3) {
+      // -------------------------------------------------- producer: V and scales
       // Block scales of the tile's 16-token groups: lane i < BN / 16 looks the
       // page up two tiles ahead and reads the two exponents one tile ahead
       // (into registers that nothing combines before their tile: a use of them
-      // would wait the memory round trip).
+      // would wait the memory round trip). They go with K's stage.
       auto group_entry = [&](int j) { return lane < BN / 16 ? entry_of(base + j * BN + lane * 16) : kNone; };
       unsigned char next_k = 127, next_v = 127;
       auto exponents = [&](int j, int p) {
@@ -348,19 +350,19 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
         sc_entry = group_entry(1);
         exponents(0, page_of(e0));
       }
-      produce(tmk, C::K_OFF, KST, k_full, k_empty, [&](int j) {
+      produce(tmv, C::R_OFF, RST, r_full, r_empty, [&](int j) {
+        if (!__all_sync(0xffffffffu, wait(&k_empty[j % KST], j / KST + 1))) return false;
         if (lane < BN / 16) {
           const int e = block_e(next_v);
           reinterpret_cast<float4*>(sm + C::SC_OFF)[(j % C::SC_SLOTS) * (BN / 16) + lane] =
               make_float4(block_scale(next_k), (float)(e - 127), __uint_as_float((uint32_t)(254 - e) << 23), 0.f);
         }
+        __syncwarp();  // the scales are written before lane 0 arrives
+        if (lane == 0) mbar_arrive(&k_full[j % KST]);
         exponents(j + 1, page_of(sc_entry));
         sc_entry = group_entry(j + 2);
-        __syncwarp();  // the scales are written before lane 0 arrives on k_full
+        return true;
       });
-    } else if (warp == 3) {
-      // ------------------------------------------------------------ producer: V
-      produce(tmv, C::R_OFF, RST, r_full, r_empty, [](int) {});
     }
     __syncwarp();
   } else if (warp < 8) {
