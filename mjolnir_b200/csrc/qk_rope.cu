@@ -9,73 +9,35 @@
 // (i, i + rot_dim / 2) those are the same chunk of both halves, so every
 // rotation is inside one thread and the row's sum of squares is the only
 // exchange.
-#include <type_traits>
-
-#include "common.cuh"
+#include "block_cache.cuh"
 
 namespace mj {
 
+// 8 elements of a row; vec: its address is 16-byte aligned
 template <typename T>
-struct Chunk;  // 8 elements
-template <>
-struct Chunk<float> {
-  static __device__ __forceinline__ void load(const float* p, float* v, bool vec) {
-    if (vec) {
-      const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
+__device__ __forceinline__ void load_chunk(const T* p, float* v, bool vec) {
+  if (vec) {
+    load8(p, v);
+  } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = p[i];
-    }
+    for (int i = 0; i < 8; ++i) v[i] = (float)p[i];
   }
-  static __device__ __forceinline__ void store(float* p, const float* v, bool vec) {
-    if (vec) {
-      reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) p[i] = v[i];
-    }
-  }
-};
+}
 template <typename T>
-struct Half8 {
-  static __device__ __forceinline__ float up(T x) {
-    if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) return __half2float(x);
-    else return __bfloat162float(x);
-  }
-  static __device__ __forceinline__ T down(float x) {
-    if constexpr (std::is_same<T, __half>::value) return __float2half_rn(x);
-    else return __float2bfloat16_rn(x);
-  }
-  static __device__ __forceinline__ void load(const T* p, float* v, bool vec) {
-    if (vec) {
-      const uint4 raw = *reinterpret_cast<const uint4*>(p);
-      const T* e = reinterpret_cast<const T*>(&raw);
+__device__ __forceinline__ void store_chunk(T* p, const float* v, bool vec) {
+  if (vec) {
+    store8(p, v);
+  } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = up(e[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = up(p[i]);
-    }
+    for (int i = 0; i < 8; ++i) p[i] = (T)v[i];
   }
-  static __device__ __forceinline__ void store(T* p, const float* v, bool vec) {
-    if (vec) {
-      uint4 raw;
-      T* e = reinterpret_cast<T*>(&raw);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = down(v[i]);
-      *reinterpret_cast<uint4*>(p) = raw;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) p[i] = down(v[i]);
-    }
-  }
-};
-template <>
-struct Chunk<__half> : Half8<__half> {};
-template <>
-struct Chunk<__nv_bfloat16> : Half8<__nv_bfloat16> {};
+}
+// 8 elements of a table of any of the three types
+__device__ __forceinline__ void load_table(const void* p, int64_t i, int dt, float* v, bool vec) {
+  if (dt == MJ_DT_BF16) load_chunk(static_cast<const __nv_bfloat16*>(p) + i, v, vec);
+  else if (dt == MJ_DT_FP16) load_chunk(static_cast<const __half*>(p) + i, v, vec);
+  else load_chunk(static_cast<const float*>(p) + i, v, vec);
+}
 
 __device__ __forceinline__ void rotate(float& a, float& b, float c, float s) {
   const float x = a * c - b * s;
@@ -83,87 +45,108 @@ __device__ __forceinline__ void rotate(float& a, float& b, float c, float s) {
   a = x;
 }
 
-// vec: every row and table address is 16-byte aligned (host-checked)
-template <typename T>
-__global__ void __launch_bounds__(256) qk_norm_rope_kernel(mj_qk_norm_rope_args a, int team_log2, bool vec) {
+// A team takes HG heads of one token's Q, or of its K: the cosines, sines and
+// weights of its two chunks stay in registers for all of them, and the heads'
+// loads are in flight together.
+// vec: every row address is 16-byte aligned; vec_w, vec_cs: the weights' and the
+// table's (host-checked)
+template <typename T, int HG>
+__global__ void __launch_bounds__(256) qk_norm_rope_kernel(mj_qk_norm_rope_args a, int team_log2, bool vec, bool vec_w, bool vec_cs) {
   griddep_wait();
   const int team = 1 << team_log2;
-  const int64_t row = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> team_log2;
+  const int64_t unit = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> team_log2;
   const int j = threadIdx.x & (team - 1);
-  const int heads = a.h_q + a.h_k;
-  const int64_t t = row / heads;
-  int h = (int)(row - t * heads);
-  const bool live = t < a.num_tokens;
+  const int qg = (a.h_q + HG - 1) / HG, groups = qg + (a.h_k + HG - 1) / HG;
+  const int64_t t = unit / groups;
+  int g = (int)(unit - t * groups);
   const int nc = a.head_size >> 3, r2 = a.rot_dim >> 4;  // chunks of a row, rotating chunk pairs
-  const bool is_k = h >= a.h_q;
-  if (is_k) h -= a.h_q;
-  const bool mine = live && 2 * j < nc;
+  const bool is_k = g >= qg;
+  if (is_k) g -= qg;
+  const int h0 = g * HG, heads = min(HG, (is_k ? a.h_k : a.h_q) - h0);
+  const bool mine = t < a.num_tokens && 2 * j < nc;
   const int ca = a.interleaved || j >= r2 ? 2 * j : j, cb = a.interleaved || j >= r2 ? 2 * j + 1 : j + r2;
-  float x[8], y[8];
-  if (mine) {
-    const T* p = static_cast<const T*>(is_k ? a.k : a.q) + t * (is_k ? a.k_stride_tok : a.q_stride_tok) +
-                 h * (is_k ? a.k_stride_head : a.q_stride_head);
-    Chunk<T>::load(p + 8 * ca, x, vec);
-    Chunk<T>::load(p + 8 * cb, y, vec);
-  } else {
+  const bool turns = mine && r2 && (a.interleaved ? 16 * j < a.rot_dim : j < r2);
+  const int64_t pos = mine && r2 ? a.positions[t] : 0;
+  const bool bad = mine && r2 && (pos < 0 || pos >= a.num_positions);
+  if (bad && j == 0) flag(a.status, MJ_DEV_BAD_POSITION);
+  const int64_t st = is_k ? a.k_stride_tok : a.q_stride_tok, sh = is_k ? a.k_stride_head : a.q_stride_head;
+  const T* in = static_cast<const T*>(is_k ? a.k : a.q) + t * st + h0 * sh;
+  float x[HG][8], y[HG][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.f;
+  for (int h = 0; h < HG; ++h) {
+    if (mine && h < heads) {
+      load_chunk(in + h * sh + 8 * ca, x[h], vec);
+      load_chunk(in + h * sh + 8 * cb, y[h], vec);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[h][i] = y[h][i] = 0.f;
+    }
   }
-  // summed for every row: teams of one warp may differ in having a weight
-  float ss = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], fmaf(y[i], y[i], ss));
-  for (int o = team >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
   const void* w = is_k ? a.k_weight : a.q_weight;
-  if (w && mine) {
-    const float r = rsqrtf(ss / (float)a.head_size + a.eps);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[i] *= r * load_elem(w, 8 * ca + i, a.weight_dtype);
-      y[i] *= r * load_elem(w, 8 * cb + i, a.weight_dtype);
-    }
+  float wx[8], wy[8], c[8], s[8];
+  if (mine && w) {
+    load_table(w, 8 * ca, a.weight_dtype, wx, vec_w);
+    load_table(w, 8 * cb, a.weight_dtype, wy, vec_w);
   }
-  if (!mine) return;
-  if (r2) {
-    const int64_t pos = a.positions[t];
-    if (pos < 0 || pos >= a.num_positions) {
-      if (j == 0) flag(a.status, MJ_DEV_BAD_POSITION);
-      return;
-    }
-    const int64_t cs = pos * a.cos_sin_stride;
-    const int half = a.rot_dim >> 1;
-    if (a.interleaved) {
-      if (ca * 8 < a.rot_dim) {
+  if (turns && !bad) {  // a pair of chunks turns by 8 angles in either pairing
+    load_table(a.cos_sin, pos * a.cos_sin_stride + 8 * j, a.cos_sin_dtype, c, vec_cs);
+    load_table(a.cos_sin, pos * a.cos_sin_stride + (a.rot_dim >> 1) + 8 * j, a.cos_sin_dtype, s, vec_cs);
+  }
+  T* out = static_cast<T*>(is_k ? a.k_out : a.q_out) + t * (is_k ? a.ko_stride_tok : a.qo_stride_tok);
+  const int64_t oh = is_k ? a.ko_stride_head : a.qo_stride_head;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          rotate(x[2 * i], x[2 * i + 1], load_elem(a.cos_sin, cs + 4 * ca + i, a.cos_sin_dtype),
-                 load_elem(a.cos_sin, cs + half + 4 * ca + i, a.cos_sin_dtype));
+  for (int h = 0; h < HG; ++h) {
+    // summed for every row: teams of one warp may differ in having a weight
+    float ss = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          rotate(y[2 * i], y[2 * i + 1], load_elem(a.cos_sin, cs + 4 * cb + i, a.cos_sin_dtype),
-                 load_elem(a.cos_sin, cs + half + 4 * cb + i, a.cos_sin_dtype));
+    for (int i = 0; i < 8; ++i) ss = fmaf(x[h][i], x[h][i], fmaf(y[h][i], y[h][i], ss));
+    for (int o = team >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (!mine || bad || h >= heads) continue;
+    if (w) {
+      const float r = rsqrtf(ss / (float)a.head_size + a.eps);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[h][i] *= r * wx[i];
+        y[h][i] *= r * wy[i];
       }
-    } else if (j < r2) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        rotate(x[i], y[i], load_elem(a.cos_sin, cs + 8 * j + i, a.cos_sin_dtype),
-               load_elem(a.cos_sin, cs + half + 8 * j + i, a.cos_sin_dtype));
     }
+    if (turns) {
+      if (a.interleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          rotate(x[h][2 * i], x[h][2 * i + 1], c[i], s[i]);
+          rotate(y[h][2 * i], y[h][2 * i + 1], c[4 + i], s[4 + i]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) rotate(x[h][i], y[h][i], c[i], s[i]);
+      }
+    }
+    store_chunk(out + (h0 + h) * oh + 8 * ca, x[h], vec);
+    store_chunk(out + (h0 + h) * oh + 8 * cb, y[h], vec);
   }
-  T* o = static_cast<T*>(is_k ? a.k_out : a.q_out) + t * (is_k ? a.ko_stride_tok : a.qo_stride_tok) +
-         h * (is_k ? a.ko_stride_head : a.qo_stride_head);
-  Chunk<T>::store(o + 8 * ca, x, vec);
-  Chunk<T>::store(o + 8 * cb, y, vec);
+}
+
+template <typename T>
+static cudaError_t launch_t(const mj_qk_norm_rope_args& a, bool vec, cudaStream_t stream) {
+  int team_log2 = 0;
+  while ((16 << team_log2) < a.head_size) ++team_log2;
+  const int64_t cs = a.cos_sin_dtype == MJ_DT_FP32 ? 4 : 2;
+  const bool vec_w = (uintptr_t)a.q_weight % 16 == 0 && (uintptr_t)a.k_weight % 16 == 0;
+  const bool vec_cs = (uintptr_t)a.cos_sin % 16 == 0 && a.cos_sin_stride * cs % 16 == 0;
+  auto grid = [&](int hg) {
+    const int64_t units = a.num_tokens * ((a.h_q + hg - 1) / hg + (a.h_k + hg - 1) / hg);
+    return dim3((unsigned)(((units << team_log2) + 255) / 256));
+  };
+  if ((a.num_tokens * (a.h_q + a.h_k) << team_log2) >= (int64_t)1 << 19)
+    return launch_kernel(qk_norm_rope_kernel<T, 4>, grid(4), dim3(256), 0, stream, a, team_log2, vec, vec_w, vec_cs);
+  return launch_kernel(qk_norm_rope_kernel<T, 1>, grid(1), dim3(256), 0, stream, a, team_log2, vec, vec_w, vec_cs);
 }
 
 cudaError_t launch_qk_norm_rope(const mj_qk_norm_rope_args& a, bool vec, cudaStream_t stream) {
-  int team_log2 = 0;
-  while ((16 << team_log2) < a.head_size) ++team_log2;
-  const int64_t threads = a.num_tokens * (a.h_q + a.h_k) << team_log2;
-  const dim3 grid((unsigned)((threads + 255) / 256));
-  if (a.dtype == MJ_DT_FP32) return launch_kernel(qk_norm_rope_kernel<float>, grid, dim3(256), 0, stream, a, team_log2, vec);
-  if (a.dtype == MJ_DT_FP16) return launch_kernel(qk_norm_rope_kernel<__half>, grid, dim3(256), 0, stream, a, team_log2, vec);
-  return launch_kernel(qk_norm_rope_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, a, team_log2, vec);
+  if (a.dtype == MJ_DT_FP32) return launch_t<float>(a, vec, stream);
+  if (a.dtype == MJ_DT_FP16) return launch_t<__half>(a, vec, stream);
+  return launch_t<__nv_bfloat16>(a, vec, stream);
 }
 
 }  // namespace mj

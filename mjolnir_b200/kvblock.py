@@ -191,8 +191,12 @@ class BlockAttention:
 
     The leading sequences of a step that share one query length of at most
     ``max_q_len`` tokens (a batch's decodes, which schedulers put first) run on
-    the decode kernel, the others on the kernel for chunks: one query token of
-    a group of 4 heads fills 4 of the chunk kernel's 256 rows."""
+    the decode kernel while their rows per KV head fit one of its jobs: 48, or
+    16 at head size 256. Beyond, and for the other sequences, the kernel for
+    chunks runs, whose row tiles are 128 (8 KV heads of 128, 16 sequences of
+    8K: 4 rows 75 us against 155, 48 rows 132 against 157, 64 rows of 4 heads
+    154 against 114; head size 256, 4 heads: 12 rows 92 against 135, 48 rows 214
+    against 141)."""
 
     def __init__(self, *, num_heads: int, num_kv_heads: int, head_size: int, page_size: int, block_tokens: int = 16,
                  max_num_seqs: int = 256, max_num_tokens: int = 8192, max_q_len: int = 4, device: torch.device | str = "cuda"):
@@ -206,8 +210,12 @@ class BlockAttention:
         self.max_num_seqs, self.max_num_tokens = max_num_seqs, max_num_tokens
         self.device = torch.device(device)
         _lib.load()  # fail at construction, not at the first step
-        self.max_q_len = min(max_q_len, 64 // (num_heads // num_kv_heads))
+        self.max_q_len = min(max_q_len, (48 if head_size == 128 else 16) // (num_heads // num_kv_heads))
+        # the split merge as a launch of its own: inside the decode launch it costs
+        # more at every size measured (4 x 1000 tokens, 8 KV heads: 4 rows 17 us
+        # against 14, 16 rows 37 against 17)
         self.decode = None if self.max_q_len < 1 else DecodeRunner(
+            fused_merge=False,
             num_heads=num_heads, num_kv_heads=num_kv_heads, head_size=head_size, page_size=page_size,
             max_num_seqs=max_num_seqs, max_q_len=self.max_q_len, kv_format=f"fp8b{block_tokens}", kernel="tc", device=device)
         self.sm_count = torch.cuda.get_device_properties(self.device).multi_processor_count
