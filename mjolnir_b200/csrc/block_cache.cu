@@ -25,9 +25,10 @@ template <typename T, int D>
 __global__ void __launch_bounds__(128) block_write_kernel(mj_cache_write_args a, int lg, int tile) {
   griddep_wait();
   constexpr int CPR = D / 8;  // 8-element chunks of a row
+  constexpr int NB = 16 / sizeof(T);
   __shared__ int members_all[4][128];
   const int wid = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int* members = members_all[wid];  // run's tokens, as offsets from its first
+  int* members = members_all[wid];  // the run's tokens, as (offset from its first) << 7 | row of the block
   const int64_t tiles = (a.num_tokens + tile - 1) / tile;
   const int64_t w = blockIdx.x * (int64_t)4 + wid;
   if (w >= tiles * a.h_k * 2) return;  // whole warps
@@ -65,6 +66,8 @@ __global__ void __launch_bounds__(128) block_write_kernel(mj_cache_write_args a,
       if (lane == 0) flag(a.status, MJ_DEV_BAD_PAGE);
       continue;
     }
+    const int64_t at_scale = page * ssp + sub * ssb;
+    const unsigned char old_byte = scales[at_scale];  // (on its way while the run is read)
     // the run: its tokens in order, and which rows of the block they fill
     int count = 0;
     uint32_t rows[4] = {0, 0, 0, 0};
@@ -77,8 +80,8 @@ __global__ void __launch_bounds__(128) block_write_kernel(mj_cache_write_args a,
       const uint32_t in = __ballot_sync(0xffffffffu, same) & before;
       const bool take = (in >> lane) & 1u;
       const int at = count + __popc(in & ((1u << lane) - 1u));
-      if (take && at < G) members[at] = (int)(u - tb);
-      const int r = take ? (int)(s & (G - 1)) : 0;
+      const int r = (int)(s & (G - 1));
+      if (take && at < G) members[at] = (int)(u - tb) << 7 | r;
 #pragma unroll
       for (int k = 0; k < 4; ++k) rows[k] |= __reduce_or_sync(0xffffffffu, take && (r >> 5) == k ? 1u << (r & 31) : 0u);
       count += __popc(in);
@@ -86,26 +89,40 @@ __global__ void __launch_bounds__(128) block_write_kernel(mj_cache_write_args a,
     }
     if (count > G) count = G;
     __syncwarp();
-    float amax = 0.f;
-    for (int c = lane; c < count * CPR; c += 32) {
-      float v[8];
-      load8(src + (tb + members[c / CPR]) * st + (c % CPR) * 8, v);
+    // The run's chunks in batches of NB a lane, whose loads are in flight
+    // together; a run of one batch stays in registers, a longer one is read
+    // again (from L2) for its codes.
+    const int total = count * CPR;
+    Raw8<T> v[NB];
+    auto fetch = [&](int c0) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float m = fabsf(v[i]);
-        amax = m <= 3.402823466e38f ? fmaxf(amax, m) : amax;  // finite values only
+      for (int i = 0; i < NB; ++i) {
+        const int c = min(c0 + 32 * i, total - 1);  // lanes past the end repeat the last chunk
+        v[i].load(src + (tb + (members[c / CPR] >> 7)) * st + (c % CPR) * 8, true);
+      }
+    };
+    float amax = 0.f;
+    for (int c0 = lane; c0 - lane < total; c0 += 32 * NB) {
+      fetch(c0);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        float x[8];
+        v[i].get(x);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float m = fabsf(x[k]);
+          amax = m <= 3.402823466e38f ? fmaxf(amax, m) : amax;  // finite values only
+        }
       }
     }
     amax = warp_allmax(amax);
-    unsigned char* sb = scales + page * ssp + sub * ssb;
     int e = block_exponent(amax);
-    const bool opened = rows[0] & 1u;
     unsigned char* base = cache + page * sp + (int64_t)(sub << lg) * sr;
-    if (!opened) {
-      const int old = min(max((int)*sb, MJ_BLOCK_E_MIN), MJ_BLOCK_E_MAX);
-      __syncwarp();
+    if (!(rows[0] & 1u)) {  // not opened by this call
+      const int old = block_e(old_byte);
       if (e > old) {  // the rows already there follow
         const float f = __uint_as_float((uint32_t)(127 + old - e) << 23);
+#pragma unroll 4
         for (int c = lane; c < G * CPR; c += 32) {
           const int r = c / CPR;
           if ((rows[r >> 5] >> (r & 31)) & 1u) continue;
@@ -117,13 +134,18 @@ __global__ void __launch_bounds__(128) block_write_kernel(mj_cache_write_args a,
         e = old;
       }
     }
-    if (lane == 0) *sb = (unsigned char)e;
+    __syncwarp();  // every lane has its copy of the old byte
+    if (lane == 0) scales[at_scale] = (unsigned char)e;
     const float inv = __uint_as_float((uint32_t)(254 - e) << 23);  // 2^(127 - e)
-    for (int c = lane; c < count * CPR; c += 32) {
-      const int64_t u = tb + members[c / CPR];
-      float v[8];
-      load8(src + u * st + (c % CPR) * 8, v);
-      *reinterpret_cast<uint2*>(base + (slots[u] & (G - 1)) * sr + (c % CPR) * 8) = quantize8(v, inv);
+    for (int c0 = lane; c0 - lane < total; c0 += 32 * NB) {
+      if (total > 32 * NB) fetch(c0);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int c = c0 + 32 * i;
+        float x[8];
+        v[i].get(x);
+        if (c < total) *reinterpret_cast<uint2*>(base + (members[c / CPR] & 127) * sr + (c % CPR) * 8) = quantize8(x, inv);
+      }
     }
     __syncwarp();  // members is rewritten for the next block
   }
@@ -131,7 +153,12 @@ __global__ void __launch_bounds__(128) block_write_kernel(mj_cache_write_args a,
 
 template <typename T>
 static cudaError_t write_t(const mj_cache_write_args& a, int lg, cudaStream_t stream) {
-  const int tile = 16;
+  // A warp looks through `tile` tokens for the runs that begin there. A prompt's
+  // tokens begin one run in 16 or more, a decode step's one each: small calls
+  // take single tokens, so that a step's rows are not written one after another
+  // (128 rows of 8 heads: 22 us with 16).
+  int tile = 16;
+  while (tile > 1 && (a.num_tokens + tile - 1) / tile * a.h_k * 2 < 2048) tile >>= 1;
   const int64_t warps = (a.num_tokens + tile - 1) / tile * a.h_k * 2;
   const dim3 grid((unsigned)((warps + 3) / 4));
   if (a.head_size == 256) return launch_kernel(block_write_kernel<T, 256>, grid, dim3(128), 0, stream, a, lg, tile);
@@ -172,21 +199,31 @@ __global__ void __launch_bounds__(256) block_read_kernel(mj_block_read_args a, i
     return;
   }
   const int h0 = (int)(w % groups) * 8, h1 = min(h0 + 8, a.h_k);
-  constexpr int CPR = D / 8;
-  for (int c = lane; c < (h1 - h0) * 2 * CPR; c += 32) {
-    const int h = h0 + c / (2 * CPR), side = (c / CPR) & 1, at = (c % CPR) * 8;
-    const unsigned char* in = static_cast<const unsigned char*>(side ? a.v_cache : a.k_cache) +
-                              page * (side ? a.v_stride_page : a.k_stride_page) + r * (side ? a.v_stride_row : a.k_stride_row) +
-                              h * (side ? a.v_stride_head : a.k_stride_head) + at;
-    const unsigned char* sc = static_cast<const unsigned char*>(side ? a.v_scales : a.k_scales) +
-                              page * (side ? a.vs_stride_page : a.ks_stride_page) +
-                              (r >> lg) * (side ? a.vs_stride_block : a.ks_stride_block) +
-                              h * (side ? a.vs_stride_head : a.ks_stride_head);
-    T* out = static_cast<T*>(side ? a.v_out : a.k_out) + row * (side ? a.vo_stride_tok : a.ko_stride_tok) +
-             h * (side ? a.vo_stride_head : a.ko_stride_head) + at;
-    float v[8];
-    dequantize8(*reinterpret_cast<const uint2*>(in), block_scale(*sc), v);
-    store8(out, v);
+  constexpr int CPR = D / 8, NB = 4;
+  const unsigned char* kc = static_cast<const unsigned char*>(a.k_cache) + page * a.k_stride_page + r * a.k_stride_row;
+  const unsigned char* vc = static_cast<const unsigned char*>(a.v_cache) + page * a.v_stride_page + r * a.v_stride_row;
+  const unsigned char* ks = static_cast<const unsigned char*>(a.k_scales) + page * a.ks_stride_page + (r >> lg) * a.ks_stride_block;
+  const unsigned char* vs = static_cast<const unsigned char*>(a.v_scales) + page * a.vs_stride_page + (r >> lg) * a.vs_stride_block;
+  T* ko = static_cast<T*>(a.k_out) + row * a.ko_stride_tok;
+  T* vo = static_cast<T*>(a.v_out) + row * a.vo_stride_tok;
+  const int total = (h1 - h0) * 2 * CPR;
+  for (int c0 = lane; c0 < total; c0 += 32 * NB) {
+    uint2 codes[NB];
+    unsigned char e[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {  // every load of the batch in flight
+      const int c = min(c0 + 32 * i, total - 1), h = h0 + c / (2 * CPR), side = (c / CPR) & 1;
+      codes[i] = *reinterpret_cast<const uint2*>((side ? vc + h * a.v_stride_head : kc + h * a.k_stride_head) + (c % CPR) * 8);
+      e[i] = *(side ? vs + h * a.vs_stride_head : ks + h * a.ks_stride_head);
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int c = c0 + 32 * i, h = h0 + c / (2 * CPR), side = (c / CPR) & 1;
+      if (c >= total) break;
+      float v[8];
+      dequantize8(codes[i], block_scale(e[i]), v);
+      store8((side ? vo + h * a.vo_stride_head : ko + h * a.ko_stride_head) + (c % CPR) * 8, v);
+    }
   }
 }
 

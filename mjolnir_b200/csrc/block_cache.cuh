@@ -60,6 +60,26 @@ __device__ __forceinline__ void store8(__half* p, const float* v) {
   *reinterpret_cast<uint4*>(p) = raw;
 }
 
+// 8 elements of a row as they are in memory
+template <typename T>
+struct Raw8 {
+  uint4 v[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p, bool vec) {
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else {
+      T* e = reinterpret_cast<T*>(v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = p[i];
+    }
+  }
+  __device__ __forceinline__ void get(float* x) const {
+    const T* e = reinterpret_cast<const T*>(v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)e[i];
+  }
+};
 // 8 values times f -> e4m3 codes: nearest even, saturating, NaN stays NaN
 __device__ __forceinline__ uint2 quantize8(const float* v, float f) {
   uint16_t c[4];

@@ -48,10 +48,9 @@ __device__ __forceinline__ void rotate(float& a, float& b, float c, float s) {
 // A team takes HG heads of one token's Q, or of its K: the cosines, sines and
 // weights of its two chunks stay in registers for all of them, and the heads'
 // loads are in flight together.
-// vec: every row address is 16-byte aligned; vec_w, vec_cs: the weights' and the
-// table's (host-checked)
-template <typename T, int HG>
-__global__ void __launch_bounds__(256) qk_norm_rope_kernel(mj_qk_norm_rope_args a, int team_log2, bool vec, bool vec_w, bool vec_cs) {
+// VEC: every row, weight and table address is 16-byte aligned (host-checked)
+template <typename T, int HG, bool VEC>
+__global__ void __launch_bounds__(256) qk_norm_rope_kernel(mj_qk_norm_rope_args a, int team_log2) {
   griddep_wait();
   const int team = 1 << team_log2;
   const int64_t unit = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> team_log2;
@@ -71,76 +70,84 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(mj_qk_norm_rope_args 
   if (bad && j == 0) flag(a.status, MJ_DEV_BAD_POSITION);
   const int64_t st = is_k ? a.k_stride_tok : a.q_stride_tok, sh = is_k ? a.k_stride_head : a.q_stride_head;
   const T* in = static_cast<const T*>(is_k ? a.k : a.q) + t * st + h0 * sh;
-  float x[HG][8], y[HG][8];
+  // a missing head's or thread's chunks repeat ones that are there, and are not stored
+  Raw8<T> rx[HG], ry[HG];
+  if (t < a.num_tokens) {
+    const int at = 2 * j < nc ? 1 : 0;
 #pragma unroll
-  for (int h = 0; h < HG; ++h) {
-    if (mine && h < heads) {
-      load_chunk(in + h * sh + 8 * ca, x[h], vec);
-      load_chunk(in + h * sh + 8 * cb, y[h], vec);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[h][i] = y[h][i] = 0.f;
+    for (int h = 0; h < HG; ++h) {
+      const T* row = in + (h < heads ? h : 0) * sh;
+      rx[h].load(row + 8 * ca * at, VEC);
+      ry[h].load(row + 8 * cb * at, VEC);
     }
   }
   const void* w = is_k ? a.k_weight : a.q_weight;
   float wx[8], wy[8], c[8], s[8];
   if (mine && w) {
-    load_table(w, 8 * ca, a.weight_dtype, wx, vec_w);
-    load_table(w, 8 * cb, a.weight_dtype, wy, vec_w);
+    load_table(w, 8 * ca, a.weight_dtype, wx, VEC);
+    load_table(w, 8 * cb, a.weight_dtype, wy, VEC);
   }
   if (turns && !bad) {  // a pair of chunks turns by 8 angles in either pairing
-    load_table(a.cos_sin, pos * a.cos_sin_stride + 8 * j, a.cos_sin_dtype, c, vec_cs);
-    load_table(a.cos_sin, pos * a.cos_sin_stride + (a.rot_dim >> 1) + 8 * j, a.cos_sin_dtype, s, vec_cs);
+    load_table(a.cos_sin, pos * a.cos_sin_stride + 8 * j, a.cos_sin_dtype, c, VEC);
+    load_table(a.cos_sin, pos * a.cos_sin_stride + (a.rot_dim >> 1) + 8 * j, a.cos_sin_dtype, s, VEC);
   }
   T* out = static_cast<T*>(is_k ? a.k_out : a.q_out) + t * (is_k ? a.ko_stride_tok : a.qo_stride_tok);
   const int64_t oh = is_k ? a.ko_stride_head : a.qo_stride_head;
 #pragma unroll
   for (int h = 0; h < HG; ++h) {
     // summed for every row: teams of one warp may differ in having a weight
-    float ss = 0.f;
+    float x[8], y[8], ss = 0.f;
+    rx[h].get(x);
+    ry[h].get(y);
+    if (mine) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(x[h][i], x[h][i], fmaf(y[h][i], y[h][i], ss));
+      for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], fmaf(y[i], y[i], ss));
+    }
     for (int o = team >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     if (!mine || bad || h >= heads) continue;
     if (w) {
       const float r = rsqrtf(ss / (float)a.head_size + a.eps);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        x[h][i] *= r * wx[i];
-        y[h][i] *= r * wy[i];
+        x[i] *= r * wx[i];
+        y[i] *= r * wy[i];
       }
     }
     if (turns) {
       if (a.interleaved) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          rotate(x[h][2 * i], x[h][2 * i + 1], c[i], s[i]);
-          rotate(y[h][2 * i], y[h][2 * i + 1], c[4 + i], s[4 + i]);
+          rotate(x[2 * i], x[2 * i + 1], c[i], s[i]);
+          rotate(y[2 * i], y[2 * i + 1], c[4 + i], s[4 + i]);
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) rotate(x[h][i], y[h][i], c[i], s[i]);
+        for (int i = 0; i < 8; ++i) rotate(x[i], y[i], c[i], s[i]);
       }
     }
-    store_chunk(out + (h0 + h) * oh + 8 * ca, x[h], vec);
-    store_chunk(out + (h0 + h) * oh + 8 * cb, y[h], vec);
+    store_chunk(out + (h0 + h) * oh + 8 * ca, x, VEC);
+    store_chunk(out + (h0 + h) * oh + 8 * cb, y, VEC);
   }
 }
 
+// heads of a thread in large calls: 8192 tokens x 40 heads take 63 us with one,
+// 54 with two, 43 with four and 68 with eight (213 registers)
+constexpr int kHeads = 4;
 template <typename T>
 static cudaError_t launch_t(const mj_qk_norm_rope_args& a, bool vec, cudaStream_t stream) {
   int team_log2 = 0;
   while ((16 << team_log2) < a.head_size) ++team_log2;
   const int64_t cs = a.cos_sin_dtype == MJ_DT_FP32 ? 4 : 2;
-  const bool vec_w = (uintptr_t)a.q_weight % 16 == 0 && (uintptr_t)a.k_weight % 16 == 0;
-  const bool vec_cs = (uintptr_t)a.cos_sin % 16 == 0 && a.cos_sin_stride * cs % 16 == 0;
+  vec = vec && (uintptr_t)a.q_weight % 16 == 0 && (uintptr_t)a.k_weight % 16 == 0 && (uintptr_t)a.cos_sin % 16 == 0 &&
+        a.cos_sin_stride * cs % 16 == 0;
   auto grid = [&](int hg) {
     const int64_t units = a.num_tokens * ((a.h_q + hg - 1) / hg + (a.h_k + hg - 1) / hg);
     return dim3((unsigned)(((units << team_log2) + 255) / 256));
   };
+  if (!vec) return launch_kernel(qk_norm_rope_kernel<T, 1, false>, grid(1), dim3(256), 0, stream, a, team_log2);
   if ((a.num_tokens * (a.h_q + a.h_k) << team_log2) >= (int64_t)1 << 19)
-    return launch_kernel(qk_norm_rope_kernel<T, 4>, grid(4), dim3(256), 0, stream, a, team_log2, vec, vec_w, vec_cs);
-  return launch_kernel(qk_norm_rope_kernel<T, 1>, grid(1), dim3(256), 0, stream, a, team_log2, vec, vec_w, vec_cs);
+    return launch_kernel(qk_norm_rope_kernel<T, kHeads, true>, grid(kHeads), dim3(256), 0, stream, a, team_log2);
+  return launch_kernel(qk_norm_rope_kernel<T, 1, true>, grid(1), dim3(256), 0, stream, a, team_log2);
 }
 
 cudaError_t launch_qk_norm_rope(const mj_qk_norm_rope_args& a, bool vec, cudaStream_t stream) {
