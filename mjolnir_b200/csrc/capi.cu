@@ -318,7 +318,7 @@ int mj_block_write(const mj_cache_write_args* args, void* stream) {
   bool ok = aligned(a.key, 16) && aligned(a.value, 16);
   for (int64_t s : {a.key_stride_tok, a.key_stride_head, a.value_stride_tok, a.value_stride_head}) ok = ok && (s * es) % 16 == 0;
   if (!ok) return fail(MJ_ERR_UNSUPPORTED, "mj_block_write: key / value rows must be 16-byte aligned");
-  if (a.num_tokens > INT32_MAX || a.num_tokens * a.h_k > (int64_t)1 << 33) return fail(MJ_ERR_UNSUPPORTED, "mj_block_write: too many rows");
+  if (a.num_tokens >= 1 << 24 || a.h_k > 1024) return fail(MJ_ERR_UNSUPPORTED, "mj_block_write: too many rows");
   return cuda_status(mj::launch_block_write(a, (cudaStream_t)stream), "mj_block_write launch");
 }
 
@@ -329,8 +329,8 @@ int mj_block_read(const mj_block_read_args* args, void* stream) {
   const int64_t st[6] = {a.k_stride_page, a.k_stride_row, a.k_stride_head, a.v_stride_page, a.v_stride_row, a.v_stride_head};
   const int64_t ss[6] = {a.ks_stride_page, a.ks_stride_block, a.ks_stride_head, a.vs_stride_page, a.vs_stride_block, a.vs_stride_head};
   if (const char* why = block_cache_problem(a.head_size, a.kv_format, a.page_size, a.h_k, a.num_pages, a.k_cache, a.v_cache,
-                                            st, a.k_scales, a.v_scales, ss, 8))
-    return fail(MJ_ERR_UNSUPPORTED, "mj_block_read: %s (head_size %d, kv_format %d, page_size %d; 8-byte aligned rows)", why,
+                                            st, a.k_scales, a.v_scales, ss, 16))
+    return fail(MJ_ERR_UNSUPPORTED, "mj_block_read: %s (head_size %d, kv_format %d, page_size %d; 16-byte aligned rows)", why,
                 a.head_size, a.kv_format, a.page_size);
   if (a.out_dtype < MJ_DT_BF16 || a.out_dtype > MJ_DT_FP32) return fail(MJ_ERR_INVALID, "mj_block_read: out_dtype %d", a.out_dtype);
   if (a.num_seqs == 0 || a.num_rows == 0) {
