@@ -54,20 +54,12 @@ def _format(block_tokens: int, page_size: int, head_size: int) -> int:
     return _lib.BLOCK_FORMATS[block_tokens]
 
 
-def _strides(t: torch.Tensor) -> tuple:
-    """Strides of the first three dims; a dim of extent 1 may carry any."""
-    st, sh = t.stride(), t.shape
-    if 1 in sh:
-        st = [0 if n == 1 else x for n, x in zip(sh, st)]
-    return st[0], st[1], st[2]
-
-
 def _cache(k_cache, v_cache, k_scales, v_scales) -> tuple:
-    """Checks cache and scale views; returns (shape, kv_format, the six code
-    strides, the six scale strides)."""
+    """Checks cache and scale views; returns (shape, kv_format, device index,
+    the six code strides, the six scale strides)."""
     shape, sshape = k_cache.shape, k_scales.shape
-    if len(shape) != 4 or v_cache.shape != shape or k_cache.itemsize != 1 or v_cache.itemsize != 1 or (
-            k_cache.stride(3) != 1 or v_cache.stride(3) != 1):
+    ks, vs, kss, vss = k_cache.stride(), v_cache.stride(), k_scales.stride(), v_scales.stride()
+    if len(shape) != 4 or v_cache.shape != shape or k_cache.itemsize != 1 or v_cache.itemsize != 1 or ks[3] != 1 or vs[3] != 1:
         raise ValueError(f"k_cache {tuple(shape)} {k_cache.dtype} and v_cache {tuple(v_cache.shape)} {v_cache.dtype} must be "
                          "(pages, page_size, h_k, d) byte views with contiguous rows")
     pages, page_size, h_k, d = shape
@@ -76,8 +68,12 @@ def _cache(k_cache, v_cache, k_scales, v_scales) -> tuple:
         raise ValueError(f"k_scales {tuple(sshape)} {k_scales.dtype} and v_scales {tuple(v_scales.shape)} {v_scales.dtype} must "
                          f"be ({pages}, {page_size} / G, {h_k}) byte views")
     kv_format = _format(page_size // sshape[1], page_size, d)
-    _on(k_cache.device, v_cache, k_scales, v_scales)
-    return shape, kv_format, _strides(k_cache) + _strides(v_cache), _strides(k_scales) + _strides(v_scales)
+    dev = k_cache.get_device()
+    _on(dev, v_cache, k_scales, v_scales)
+    st = (ks[0], ks[1], ks[2], vs[0], vs[1], vs[2])
+    if pages == 1 or h_k == 1:  # a dim of extent 1 may carry any stride
+        st = tuple(0 if n == 1 else x for n, x in zip((*shape[:3], *shape[:3]), st))
+    return shape, kv_format, dev, st, (kss[0], kss[1], kss[2], vss[0], vss[1], vss[2])
 
 
 def _rows(name: str, t: torch.Tensor, h_k: int, d: int) -> tuple:
@@ -88,10 +84,11 @@ def _rows(name: str, t: torch.Tensor, h_k: int, d: int) -> tuple:
     return st[0], st[1]
 
 
-def _on(device: torch.device, *tensors) -> None:
+def _on(dev: int, *tensors) -> None:
+    """Every tensor that is there is on the device of this index (-1: the CPU)."""
     for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"every tensor must be on {device}, got {t.device}")
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"every tensor must be on {'cuda:%d' % dev if dev >= 0 else 'the CPU'}, got {t.device}")
 
 
 def write(
@@ -111,7 +108,7 @@ def write(
     T = slot_mapping.shape[0]
     if T == 0:
         return
-    (pages, page_size, h_k, d), kv_format, st, ss = _cache(k_cache, v_cache, k_scales, v_scales)
+    (pages, page_size, h_k, d), kv_format, dev, st, ss = _cache(k_cache, v_cache, k_scales, v_scales)
     kt, vt = _rows("key", key, h_k, d), _rows("value", value, h_k, d)
     if key.shape[0] < T or value.shape[0] < T:
         raise ValueError("fewer key / value rows than slots")
@@ -119,7 +116,7 @@ def write(
         raise TypeError("key and value must share a dtype")
     if slot_mapping.dim() != 1 or slot_mapping.dtype not in (torch.int64, torch.int32):
         raise TypeError("slot_mapping must be a 1-D int64")
-    _on(k_cache.device, key, value, slot_mapping, status)
+    _on(dev, key, value, slot_mapping, status)
     slots = slot_mapping
     if slots.dtype != torch.int64 or not slots.is_contiguous():
         slots = slots.to(torch.int64).contiguous()
@@ -127,7 +124,7 @@ def write(
         key.data_ptr(), value.data_ptr(), dtype_code(key.dtype), T, h_k, d, *kt, *vt, k_cache.data_ptr(), v_cache.data_ptr(),
         *st, pages, page_size, kv_format, slots.data_ptr(), None, 0, None, 0, _ptr(status),
         k_scales.data_ptr(), v_scales.data_ptr(), *ss)
-    call(_lib.block_write, a, k_cache.device)
+    call(_lib.block_write, a, dev)
 
 
 def _table(block_table: torch.Tensor, num_seqs: int) -> None:
@@ -151,7 +148,7 @@ def read(
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """Read tokens ``starts[s] ..`` of each sequence into rows ``offsets[s] ..
     offsets[s + 1] - 1`` of the outputs; returns ``(k_out, v_out)``."""
-    (pages, page_size, h_k, d), kv_format, st, ss = _cache(k_cache, v_cache, k_scales, v_scales)
+    (pages, page_size, h_k, d), kv_format, dev, st, ss = _cache(k_cache, v_cache, k_scales, v_scales)
     n = starts.shape[0]
     for name, t, m in (("starts", starts, n), ("offsets", offsets, n + 1)):
         if t.dtype != torch.int32 or t.shape != (m,) or not t.is_contiguous():
@@ -160,12 +157,12 @@ def read(
     ko, vo = _rows("k_out", k_out, h_k, d), _rows("v_out", v_out, h_k, d)
     if v_out.shape != k_out.shape or v_out.dtype != k_out.dtype:
         raise ValueError("k_out and v_out must share a shape and dtype")
-    _on(k_cache.device, block_table, starts, offsets, k_out, v_out, status)
+    _on(dev, block_table, starts, offsets, k_out, v_out, status)
     a = _lib.BlockReadArgs(
         k_cache.data_ptr(), v_cache.data_ptr(), *st, k_scales.data_ptr(), v_scales.data_ptr(), *ss, pages, page_size, h_k, d,
         kv_format, block_table.data_ptr(), block_table.stride(0), block_table.shape[1], starts.data_ptr(), offsets.data_ptr(),
         n, k_out.shape[0], k_out.data_ptr(), v_out.data_ptr(), dtype_code(k_out.dtype), *ko, *vo, _ptr(status))
-    call(_lib.block_read, a, k_cache.device)
+    call(_lib.block_read, a, dev)
     return k_out, v_out
 
 
@@ -245,7 +242,7 @@ class BlockAttention:
         _table(block_table, len(q))
         if seq_lens.dtype != torch.int32 or seq_lens.dim() != 1 or seq_lens.shape[0] < len(q) or not seq_lens.is_contiguous():
             raise ValueError("seq_lens must be a contiguous int32 tensor of every sequence")
-        _on(self.status.device, block_table, seq_lens)
+        _on(self.status.get_device(), block_table, seq_lens)
         decode, few = None, 0
         if q and 1 <= q[0] <= self.max_q_len:
             few = next((i for i, x in enumerate(q) if x != q[0]), len(q))
@@ -276,7 +273,7 @@ class BlockAttention:
         softmax_scale: float,
         lse: torch.Tensor | None = None,  # optional (tokens, h_q) fp32
     ) -> torch.Tensor:
-        (pages, page_size, h_k, d), kv_format, st, ss = _cache(k_cache, v_cache, k_scales, v_scales)
+        (pages, page_size, h_k, d), kv_format, dev, st, ss = _cache(k_cache, v_cache, k_scales, v_scales)
         if (page_size, kv_format, h_k, d) != (self.page_size, self.kv_format, self.h_k, self.d):
             raise ValueError(f"a cache of pages {page_size}, format {kv_format}, {h_k} heads of {d} is not this runner's")
         qs, os_ = _rows("query", query, self.h_q, d), _rows("out", out, self.h_q, d)
@@ -288,8 +285,7 @@ class BlockAttention:
         if lse is not None and (lse.dtype != torch.float32 or lse.shape[0] < tokens or lse.shape[1:] != (self.h_q,)
                                 or not lse.is_contiguous()):
             raise ValueError("lse must be a contiguous fp32 (tokens, h_q)")
-        dev = self.status.device
-        _on(dev, query, out, k_cache, lse)
+        _on(dev, self.status, query, out, lse)
         bt, scale, causal = plan.block_table, float(softmax_scale), int(plan.causal)
         cache = (k_cache.data_ptr(), v_cache.data_ptr(), *st)
         scales = (k_scales.data_ptr(), v_scales.data_ptr())

@@ -31,7 +31,7 @@ def qk_norm_rope(
     """Normalise and rotate Q and K; returns ``(q_out, k_out)``. A position
     outside the table flags ``MJ_DEV_BAD_POSITION`` in ``status`` and leaves
     its token's output rows as they were."""
-    shape, dtype, dev = q.shape, q.dtype, q.device
+    shape, dtype, dev = q.shape, q.dtype, q.get_device()
     if len(shape) != 3 or len(k.shape) != 3:
         raise ValueError(f"q {tuple(shape)} and k {tuple(k.shape)} must be (tokens, heads, head_size)")
     T, h_q, d = shape
@@ -39,9 +39,9 @@ def qk_norm_rope(
     if k.shape[0] != T or k.shape[2] != d or k.dtype != dtype:
         raise ValueError(f"k {tuple(k.shape)} {k.dtype} does not match q {tuple(shape)} {dtype}")
     if q_out is None:
-        q_out = torch.empty(shape, dtype=dtype, device=dev)
+        q_out = torch.empty(shape, dtype=dtype, device=q.device)
     if k_out is None:
-        k_out = torch.empty(k.shape, dtype=dtype, device=dev)
+        k_out = torch.empty(k.shape, dtype=dtype, device=q.device)
     if q_out.shape != shape or q_out.dtype != dtype or k_out.shape != k.shape or k_out.dtype != dtype:
         raise ValueError(f"q_out {tuple(q_out.shape)} {q_out.dtype} / k_out {tuple(k_out.shape)} {k_out.dtype} do not match q and k")
     qs, ks, qos, kos = q.stride(), k.stride(), q_out.stride(), k_out.stride()
@@ -60,8 +60,8 @@ def qk_norm_rope(
     if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
         raise ValueError(f"norm weights must share a dtype, got {q_weight.dtype} and {k_weight.dtype}")
     for t in (k, q_out, k_out, positions, cos_sin, q_weight, k_weight, status):
-        if t is not None and t.device != dev:
-            raise ValueError(f"every tensor must be on {dev}, got {t.device}")
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"every tensor must be on {q.device}, got {t.device}")
     call(_lib.qk_norm_rope, _lib.QkNormRopeArgs(
         q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), dtype_code(dtype), T, h_q, h_k, d, cos_sin.shape[1],
         int(interleaved), qs[0], qs[1], ks[0], ks[1], qos[0], qos[1], kos[0], kos[1], positions.data_ptr(), cos_sin.data_ptr(),

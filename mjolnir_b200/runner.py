@@ -235,11 +235,13 @@ def _stream(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def call(entry, args, device: torch.device) -> None:
-    """Run a library entry point on ``device``'s current stream, with that
-    device current."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        entry(args, _stream(device))
+def call(entry, args, device: int) -> None:
+    """Run a library entry point on the current stream of the device of this
+    index, with that device current."""
+    if device < 0:
+        raise ValueError("the kernels take CUDA tensors")
+    if device == torch._C._cuda_getDevice():
+        entry(args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
             entry(args, _stream(device))

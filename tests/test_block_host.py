@@ -137,3 +137,58 @@ def test_c_entries_refuse():
     a.dtype, a.k_stride_row = _lib.MJ_DT_BF16, 24
     with pytest.raises(_lib.MjolnirError, match="alignment"):
         _lib.block_attention(a, 0)
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(3, 2, 128)
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        kvblock.write(x, x, *_cache(), torch.arange(3))
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        qkrope.qk_norm_rope(x, x, torch.zeros(3, dtype=torch.int64), torch.zeros(4, 128))
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_plan_covers_every_row_and_tile_once(seed):
+    import random
+
+    import numpy as np
+
+    r = random.Random(seed)
+    for _ in range(200):
+        n = r.randint(0, 12)
+        q = [r.choice([0, 1, 5, 70, 1500, r.randint(0, 400)]) for _ in range(n)]
+        kv = [max(0, x + r.choice([-2, 0, 0, 40, 9000])) for x in q]
+        h_k, h_r, d, causal = r.choice([1, 2, 8]), r.choice([1, 3, 4, 6]), r.choice([128, 256]), r.random() < 0.7
+        slots = r.choice([0, 2 * -(-148 // h_k)])
+        work, merges = np.zeros((20000, 8), np.int32), np.zeros((max(1, slots), 4), np.int32)
+        nw, nm, ns = _lib.block_plan(q, kv, h_k * h_r, h_k, d, causal, 148, slots, work, merges)
+        assert ns <= slots
+        rows, items = 128 if d == 256 else 256, {}
+        for s, r0, tb, te, slot, *_ in work[:nw].tolist():
+            items.setdefault((s, r0), []).append((tb, te, slot))
+        assert set(items) == {(s, r0) for s in range(n) for r0 in range(0, q[s] * h_r, rows)}
+        used = []
+        for (s, r0), pieces in items.items():
+            pieces.sort()
+            last = kv[s] - q[s] + (min(r0 + rows, q[s] * h_r) - 1) // h_r if causal else kv[s] - 1
+            assert pieces[0][0] == 0 and pieces[-1][1] == (last // 64 + 1 if last >= 0 else 0)
+            assert all(a[1] == b[0] for a, b in zip(pieces, pieces[1:]))
+            got = [p[2] for p in pieces]
+            if len(pieces) == 1:
+                assert got == [-1]
+                continue
+            used += got
+            assert [m[2:] for m in merges[:nm].tolist() if m[:2] == [s, r0]] == [[got[0], len(got)]]
+        assert sorted(used) == list(range(ns))
+
+
+def test_plan_refuses():
+    import numpy as np
+
+    work, merges = np.zeros((2, 8), np.int32), np.zeros((1, 4), np.int32)
+    with pytest.raises(_lib.MjolnirError, match="capacity"):
+        _lib.block_plan([1, 1, 1], [5, 5, 5], 4, 1, 128, True, 148, 0, work, merges)
+    with pytest.raises(_lib.MjolnirError, match="length"):
+        _lib.block_plan([1], [-5], 4, 1, 128, True, 148, 0, work, merges)
+    with pytest.raises(_lib.MjolnirError, match="invalid"):
+        _lib.block_plan([1], [5], 4, 3, 128, True, 148, 0, work, merges)
