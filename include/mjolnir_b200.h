@@ -10,6 +10,9 @@
  *                   (fp8-e4m3, or e2m3 packed 4 codes per 3 bytes)
  *   mj_decode       paged split-KV decode attention over that cache
  *   mj_combine      log-sum-exp merge of the split-KV partials
+ * and, around a cache whose scales are chosen per block of tokens as it is
+ * written (no counterpart in the reference): mj_qk_norm_rope, mj_block_write,
+ * mj_block_read, mj_block_plan and mj_block_attention.
  *
  * Reference interfaces these replace (GoBrrr-ai/mjolnir, src/mjolnir/mjolnir/):
  *   mj_cache_write  kvfp6.py:218-254 `write_kv` (e2m3) and the fp8 write

@@ -283,7 +283,7 @@ int mj_qk_norm_rope(const mj_qk_norm_rope_args* args, void* stream) {
   if (a.rot_dim && (!a.positions || !a.cos_sin || a.num_positions <= 0))
     return fail(MJ_ERR_INVALID, "mj_qk_norm_rope: rotation needs positions and the cos / sin table");
   if (!(a.eps >= 0.f)) return fail(MJ_ERR_INVALID, "mj_qk_norm_rope: eps %g", (double)a.eps);
-  if (a.num_tokens * (a.h_q + a.h_k) > (int64_t)1 << 34) return fail(MJ_ERR_UNSUPPORTED, "mj_qk_norm_rope: too many rows");
+  if (a.num_tokens >= 1 << 30 || a.num_tokens * (a.h_q + a.h_k) > (int64_t)1 << 33) return fail(MJ_ERR_UNSUPPORTED, "mj_qk_norm_rope: too many rows");
   // 16-byte accesses where every row allows them
   const int64_t es = a.dtype == MJ_DT_FP32 ? 4 : 2;
   bool vec = true;
@@ -343,7 +343,7 @@ int mj_block_read(const mj_block_read_args* args, void* stream) {
   bool ok = aligned(a.k_out, 16) && aligned(a.v_out, 16);
   for (int64_t s : {a.ko_stride_tok, a.ko_stride_head, a.vo_stride_tok, a.vo_stride_head}) ok = ok && (s * es) % 16 == 0;
   if (!ok) return fail(MJ_ERR_UNSUPPORTED, "mj_block_read: output rows must be 16-byte aligned");
-  if (a.num_rows > INT32_MAX) return fail(MJ_ERR_UNSUPPORTED, "mj_block_read: too many rows");
+  if (a.num_rows > INT32_MAX || a.num_rows * a.h_k > (int64_t)1 << 34) return fail(MJ_ERR_UNSUPPORTED, "mj_block_read: too many rows");
   return cuda_status(mj::launch_block_read(a, (cudaStream_t)stream), "mj_block_read launch");
 }
 

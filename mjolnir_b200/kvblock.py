@@ -184,7 +184,9 @@ class BlockPlan:
 
 class BlockAttention:
     """Attention over a block-scaled cache for steps of any mix of lengths:
-    single tokens, drafts and prompt chunks behind cached contexts.
+    single tokens, drafts and prompt chunks behind cached contexts. A runner
+    owns its plan buffers and split partials, so its calls belong to one
+    stream at a time.
 
     The leading sequences of a step that share one query length of at most
     ``max_q_len`` tokens (a batch's decodes, which schedulers put first) run on

@@ -189,3 +189,40 @@ def test_pages_past_32_bit_offsets():
             outs.append(r.run(plan, q, torch.empty_like(q), *v, 128**-0.5))
             r.check_status()
         assert torch.equal(outs[0], outs[1]) and math.isfinite(outs[0].float().sum().item())
+
+
+@pytest.mark.parametrize("merge", [True, False])
+@pytest.mark.parametrize("d,h_q,page,block,q_len", [(128, 4, 16, 16, 1), (128, 8, 64, 64, 2), (128, 8, 128, 128, 7), (256, 6, 128, 32, 3)])
+def test_decode_runner_on_block_formats(merge, d, h_q, page, block, q_len):
+    """The formats through DecodeRunner itself: split merge inside the decode launch, or as a launch of its own."""
+    from mjolnir_b200.runner import DecodeRunner
+
+    c = Cache([2000, 77, 1], h_k=1, d=d, page=page, block=block, seed=q_len)
+    r = DecodeRunner(num_heads=h_q, num_kv_heads=1, head_size=d, page_size=page, max_num_seqs=3, max_q_len=q_len,
+                     kv_format=f"fp8b{block}", fused_merge=merge)
+    q = torch.randn(3 * q_len, h_q, d, generator=c.g).to(torch.bfloat16)
+    q[0, 1, 3] = float("nan")
+    plan = r.plan(c.lens, 3, q_len, c.table.cuda(), torch.tensor(c.lens, dtype=torch.int32).cuda())
+    assert plan.with_reduction
+    out, one = torch.empty(3 * q_len, h_q, d, dtype=torch.bfloat16, device="cuda"), torch.ones(1, device="cuda")
+    r.run(plan, q.cuda(), out, *c.args[:2], one, one, d**-0.5, k_scales=c.args[2], v_scales=c.args[3])
+    torch.cuda.synchronize()
+    r.check_status()
+    want, _, mag = attention_plain(c, q, [q_len] * 3, d**-0.5)
+    fine = torch.ones(3 * q_len, h_q, dtype=torch.bool)
+    fine[0, 1] = False
+    assert torch.isnan(out[0, 1]).all()
+    assert_attention(out.cpu()[fine], want[fine], mag[fine])
+    with pytest.raises(ValueError, match="needs k_scales"):
+        r.run(plan, q.cuda(), out, *c.args[:2], one, one, d**-0.5)
+
+
+def test_the_example_runs():
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, os.path.join(root, "examples", "block_cache.py")], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
+    assert "1942 tokens of 2 sequences" in r.stdout
