@@ -128,6 +128,13 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
                      __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
+// the largest of three; NaN if one is
+__device__ __forceinline__ float nan_max3(float x, float y, float z) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(x), "f"(y), "f"(z));
+  return m;
+}
+
 // two packed 16-bit values
 __device__ __forceinline__ float2 up2(__nv_bfloat162 v) { return __bfloat1622float2(v); }
 __device__ __forceinline__ float2 up2(__half2 v) { return __half22float2(v); }
@@ -158,6 +165,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::MISC_OFF);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + C::MISC_OFF + 4);
   int& never_abort = *reinterpret_cast<int*>(sm + C::MISC_OFF + 8);
+  volatile int* nan_v = reinterpret_cast<volatile int*>(sm + C::MISC_OFF + 12);
   if (reinterpret_cast<uintptr_t>(sm) & 1023) {  // uniform: nothing taken yet
     if (threadIdx.x == 0) flag(a.status, MJ_DEV_BAD_SPLIT);
     return;
@@ -203,6 +211,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
     mbar_init(drain, na);
     *abort_flag = 0;
     never_abort = 0;
+    *nan_v = 0;
     fence_mbar_init();
   }
   if (warp == 1 && lane == 0) {
@@ -235,6 +244,13 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
   // phase of that pair's barriers
   auto s_col = [&](int w, int j) { return (uint32_t)(w * 128 + (j & 1) * BN); };
   auto at = [&](int w, int j) { return 2 * w + (j & 1); };
+
+  // The first key tile that some row of the item sees only part of. From there
+  // on NaN codes of V reach the product as zeros (P = 0 times NaN would be NaN
+  // in the rows that do not see them), and if there was one, the epilogue makes
+  // those elements NaN in the rows that do.
+  const int item_lim = a.causal ? L - n_tok + row0 / h_r : L - 1;
+  const int j_part = max(item_lim + 1 - tb * BN, 0) / BN;
 
   // Page-table walk. An entry is loaded before it is needed and checked then:
   // checking it at once would wait a memory round trip.
@@ -386,6 +402,12 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
         d[i] = *reinterpret_cast<const uint4*>(raw + unit_offset(r, 4 * (blk & 1) + quad));
         if (r >= rows) d[i] = make_uint4(0, 0, 0, 0);
       }
+      if (j >= j_part) {
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) any |= drop_nan_codes(d[i]);
+        if (any) *nan_v = 1;  // before this tile's arrival on v_full
+      }
       if (!wait(&v_empty[j % VST], j / VST + 1)) return false;
       unsigned char* out = sm + C::V_OFF + (j % VST) * C::VTILE + blk * (BN * 128);
 #pragma unroll
@@ -503,11 +525,14 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
         }
         float mx4[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mx4[i] = fmaxf(s[i].x, s[i].y);
+        for (int i = 0; i < 4; ++i) mx4[i] = s[i].x;
 #pragma unroll
-        for (int i = 4; i < BN / 2; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], fmaxf(s[i].x, s[i].y));
-        float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-        if (__any_sync(0xffffffffu, j == 0 || mx > kRaise)) {
+        for (int i = 4; i < BN / 2; ++i) mx4[i & 3] = nan_max3(mx4[i & 3], s[i].x, s[i - 4].y);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx4[i] = nan_max3(mx4[i], s[BN / 2 - 4 + i].y, mx4[0]);
+        float mx = nan_max3(mx4[1], mx4[2], mx4[3]);
+        if (__any_sync(0xffffffffu, j == 0 || !(mx <= kRaise))) {
+          if (isnan(mx)) l = mx;  // a NaN score: so is the row (exp2_poly would lose it)
           const float up = (j == 0 ? mx > -INFINITY : mx > kRaise) ? -mx : 0.f;  // added to nm
           nm += up;
 #pragma unroll
@@ -551,9 +576,11 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
       }
       // ---- epilogue: O / l of this row
       if (ok && n > 0) ok = wait(&o_full[at(w, n - 1)], (n - 1) >> 1);
+      if (ok && n > 0) ok = wait(&v_full[(n - 1) % VST], (n - 1) / VST);  // long complete: orders the read of nan_v
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
       if (ok) {
+        const bool nans = *nan_v != 0;
         if (lim < base) l = 0.f;  // no key in this item (exp2_poly's zero is 2^-125)
         const float inv = l == 0.f ? 0.f : 1.f / l;  // a NaN sum stays NaN
         const int64_t part = ((int64_t)slot * a.h_k + h) * C::ROWS + w * 128 + t;
@@ -571,6 +598,17 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
           }
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = l == 0.f ? 0.f : v[i] * inv;
+          if (nans)  // rare
+#pragma unroll 1
+            for (int key = base + j_part * BN; key <= min(lim, base + n * BN - 1); ++key) {
+              const int pg = page_of(entry_of(key));
+              if (pg < 0) continue;
+              const uint32_t* code = reinterpret_cast<const uint32_t*>(static_cast<const unsigned char*>(a.v_cache) + pg * a.v_stride_page +
+                                                                       (key & pmask) * a.v_stride_row + h * a.v_stride_head + c);
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (nan_codes(__ldg(code + i / 4)) >> (8 * (i % 4)) & 0x80u) v[i] = __int_as_float(0x7FFFFFFF);
+            }
           if (slot < 0) {
 #pragma unroll
             for (int i = 0; i < 32; i += 8)
@@ -622,7 +660,7 @@ __global__ void __launch_bounds__(256) block_merge_kernel(const __grid_constant_
   if (R >= (a.q_start[e.x + 1] - q0) * h_r || e.w <= 0) return;
   const int64_t step = (int64_t)a.h_k * ROWS, first = ((int64_t)e.z * a.h_k + h) * ROWS + r;
   float mx = -INFINITY;
-  for (int s = 0; s < e.w; ++s) mx = fmaxf(mx, a.lse_part[first + s * step]);
+  for (int s = 0; s < e.w; ++s) mx = nan_max(mx, a.lse_part[first + s * step]);  // a NaN partial makes its row NaN
   float o[E], l = 0.f;
 #pragma unroll
   for (int i = 0; i < E; ++i) o[i] = 0.f;

@@ -80,6 +80,19 @@ struct Raw8 {
     for (int i = 0; i < 8; ++i) x[i] = (float)e[i];
   }
 };
+// 0x80 in every byte of w that is a NaN code (0x7F or 0xFF)
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
+// 16 codes with NaN made zero; true if one was
+__device__ __forceinline__ bool drop_nan_codes(uint4& c) {
+  const uint32_t x = nan_codes(c.x), y = nan_codes(c.y), z = nan_codes(c.z), w = nan_codes(c.w);
+  if (!(x | y | z | w)) return false;
+  c.x &= ~((x >> 7) * 0xFFu);
+  c.y &= ~((y >> 7) * 0xFFu);
+  c.z &= ~((z >> 7) * 0xFFu);
+  c.w &= ~((w >> 7) * 0xFFu);
+  return true;
+}
+
 // 8 values times f -> e4m3 codes: nearest even, saturating, NaN stays NaN
 __device__ __forceinline__ uint2 quantize8(const float* v, float f) {
   uint16_t c[4];

@@ -392,6 +392,7 @@ __global__ void __launch_bounds__(Cfg<FMT, NQP, NWG, CVTW, DH>::THREADS, Cfg<FMT
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::MISC_OFF);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + C::MISC_OFF + 4);
   int& never_abort = *reinterpret_cast<int*>(sm + C::MISC_OFF + 8);  // no one sets it: drains wait on time only
+  volatile int* nan_job = reinterpret_cast<volatile int*>(sm + C::MISC_OFF + 16);  // [4], block formats
   float* lred_all = reinterpret_cast<float*>(sm + C::MISC_OFF + 64);  // [NWG][4][NQP]
 
   if (threadIdx.x == 0) {
@@ -420,6 +421,8 @@ __global__ void __launch_bounds__(Cfg<FMT, NQP, NWG, CVTW, DH>::THREADS, Cfg<FMT
     mbar_init(b.k_ready + S, 1);  // "never": nothing arrives on it (the abort-path probe)
     *abort_flag = 0;
     never_abort = 0;
+    if constexpr (Fmt<FMT>::BLOCK)
+      for (int i = 0; i < 4; ++i) nan_job[i] = 0;
     fence_mbar_init();
   }
   if constexpr (Fmt<FMT>::SCALED) {
@@ -512,12 +515,13 @@ __global__ void __launch_bounds__(Cfg<FMT, NQP, NWG, CVTW, DH>::THREADS, Cfg<FMT
 
   // ---------------------------------------- V conversion / tail zero (thread ct)
   auto convert_role = [&](const int ct) {
-    int it = 0;
+    int it = 0, jobs = 0;
     bool ok = true;
     for (int p = blockIdx.x; ok && p < total_jobs; p += gridDim.x) {
       int seq, tb, te, split, h, g;
       if (!job(p, seq, tb, te, split, h, g)) continue;
       const int L = a.seq_lens[seq];
+      ++jobs;
       for (int tile = tb; tile < te; ++tile, ++it) {
         const int st = it % S;
         if constexpr (Fmt<FMT>::SCALED) {
@@ -579,6 +583,26 @@ __global__ void __launch_bounds__(Cfg<FMT, NQP, NWG, CVTW, DH>::THREADS, Cfg<FMT
               for (int c = r0 * 8 + ct; c < kTileRows * 8; c += C::CVT_ROLE)
                 *reinterpret_cast<uint4*>(vb + vchunk(c)) = make_uint4(0, 0, 0, 0);
             }
+          }
+          // Block formats: so would the NaN codes of a draft's own tokens poison
+          // the queries before them. They become zeros here, and the epilogue
+          // makes their elements NaN in the rows that see them.
+          if constexpr (Fmt<FMT>::BLOCK) {
+            const int r0 = max(valid - a.q_len + 1, 0), r1 = min(valid, kTileRows);
+            bool any = false;
+            if (r0 < r1)
+              for (int dh = 0; dh < DH; ++dh) {
+                unsigned char* vb = vbuf(st, dh);
+                for (int c = r0 * 8 + ct; c < r1 * 8; c += C::CVT_ROLE) {
+                  uint4* q = reinterpret_cast<uint4*>(vb + vchunk(c));
+                  uint4 codes = *q;
+                  if (drop_nan_codes(codes)) {
+                    *q = codes;
+                    any = true;
+                  }
+                }
+              }
+            if (any) nan_job[jobs & 3] = jobs;  // this role is at most two jobs ahead of the epilogue
           }
         }
         fence_proxy_async_smem();
@@ -1185,6 +1209,8 @@ __global__ void __launch_bounds__(Cfg<FMT, NQP, NWG, CVTW, DH>::THREADS, Cfg<FMT
 #pragma unroll
           for (int k = 0; k < 8 && c + k < NQP; ++k) orow[dh][c + k] = hv[k] + mv[k] * 0.0625f + lv[k] * 0.00390625f;
         }
+      bool nans = false;
+      if constexpr (Fmt<FMT>::BLOCK) nans = nan_job[jc & 3] == jc;
       tc_fence_before();
       mbar_arrive(b.o_free);  // the next job's first PV may overwrite O
       if (named_bar_or(bar_id, 128, *abort_flag != 0)) {
@@ -1210,6 +1236,20 @@ __global__ void __launch_bounds__(Cfg<FMT, NQP, NWG, CVTW, DH>::THREADS, Cfg<FMT
             const float lt = lred[r] + lred[NQP + r] + lred[2 * NQP + r] + lred[3 * NQP + r];
             if constexpr (Fmt<FMT>::BLOCK) o[r] = lt == 0.f ? 0.f : orow[dh][r] * (vscale / lt);  // NaN sums stay NaN; lt may pass 2^126
             else o[r] = lt > 0.f ? orow[dh][r] * __fdividef(vscale, lt) : 0.f;
+          }
+          if constexpr (Fmt<FMT>::BLOCK) {
+            if (nans)  // rare: NaN codes of V among the draft's own tokens
+#pragma unroll 1
+              for (int key = max(max(L - q_len + 1, 0), tb * kTileRows); key < min(L, te * kTileRows); ++key) {
+                const int pg = __ldg(a.block_table + (int64_t)seq * a.block_table_stride + key / a.page_size);
+                if (pg < 0 || pg >= a.num_pages) continue;
+                const unsigned char code = __ldg(static_cast<const unsigned char*>(a.v_cache) + pg * a.v_stride_page +
+                                                 (key & (a.page_size - 1)) * a.v_stride_row + h * a.v_stride_head + e);
+                if ((code & 0x7F) == 0x7F)
+#pragma unroll
+                  for (int r = 0; r < NQP; ++r)
+                    if (key <= lim_of(r)) o[r] = __int_as_float(0x7FFFFFFF);
+              }
           }
           if (final_out && a.o_mul) {
             float om[NQP];

@@ -115,6 +115,45 @@ def test_nan_query_stays_in_its_row():
     assert_attention(got.cpu()[fine], want[fine], mag[fine])
 
 
+@pytest.mark.parametrize("d,h_q,q_len,ctx,positions", [
+    (128, 8, 150, 300, (449, 301, 420, 5)), (128, 8, 4, 300, (303, 301)), (128, 8, 3, 125, (127, 126)),
+    (256, 4, 90, 0, (0, 89, 60)), (256, 4, 4, 126, (127, 129)), (128, 4, 1, 200, (200, 17)),
+    (128, 8, 4, 9000, (9001, 9003)), (128, 8, 64, 5000, (5063, 5001, 4990))])
+@pytest.mark.parametrize("causal", [True, False])
+def test_nan_values_reach_only_the_rows_that_see_them(d, h_q, q_len, ctx, positions, causal):
+    """K and V hold NaN at a few tokens: K's make the rows that see them NaN,
+    V's only their own elements; rows before them are as without them."""
+    c = Cache([q_len + ctx], h_k=2, d=d, seed=ctx + q_len)
+    q = torch.randn(q_len, h_q, d, generator=c.g).to(torch.bfloat16)
+    want, _, mag = attention_plain(c, q, [q_len], d**-0.5, causal=causal)
+    nan = torch.zeros(q_len, h_q, d, dtype=torch.bool)
+    limit = torch.arange(ctx, ctx + q_len) if causal else torch.full((q_len,), ctx + q_len - 1)
+    for i, at in enumerate(positions):
+        page, row = int(c.table[0, at // c.page]), at % c.page
+        c.kv[1][page, row, 0, 3 + 31 * i] = 0x7F if i % 2 else 0xFF
+        nan[limit >= at, : h_q // 2, 3 + 31 * i] = True
+    key = positions[0]
+    c.kv[0][int(c.table[0, key // c.page]), key % c.page, 1, 2] = 0x7F
+    nan[limit >= key, h_q // 2:] = True
+    got, _ = _run(c, q, [q_len], causal=causal)
+    got = got.cpu()
+    assert torch.equal(torch.isnan(got), nan)
+    assert_attention(got[~nan], want[~nan], mag[~nan])
+
+
+@pytest.mark.parametrize("q_len", [1, 40])
+def test_nan_query_over_a_split_context(q_len):
+    c = Cache([20000], h_k=1, seed=q_len)
+    q = torch.randn(q_len, 2, 128, generator=c.g).to(torch.bfloat16)
+    q[0, 1, 100] = float("nan")
+    got, _ = _run(c, q, [q_len])
+    want, _, mag = attention_plain(c, q, [q_len], 128**-0.5)
+    assert torch.isnan(got[0, 1]).all()
+    fine = torch.ones(q_len, 2, dtype=torch.bool)
+    fine[0, 1] = False
+    assert_attention(got.cpu()[fine], want[fine], mag[fine])
+
+
 def test_bad_page_is_flagged():
     from mjolnir_b200 import _lib, kvblock
 
