@@ -6,6 +6,8 @@
 // rounds), so a block filled token by token holds what one write of all its
 // tokens would. e4m3 is a floating type: the shared exponent costs no
 // precision until a value is 2^14 below its block's largest.
+#include <limits.h>
+
 #include "block_cache.cuh"
 
 namespace mj {
@@ -35,8 +37,9 @@ __global__ void __launch_bounds__(128) block_write_kernel(mj_cache_write_args a,
   const int64_t w = blockIdx.x * (int64_t)4 + wid;
   if (w >= tiles * a.h_k * 2) return;  // whole warps
   const int side = (int)(w & 1);
-  const int h = (int)((w >> 1) % a.h_k);
-  const int64_t t0 = ((w >> 1) / a.h_k) * tile;
+  const uint32_t at = (uint32_t)(w >> 1);  // below 2^32: the grid's blocks are counted in 31 bits
+  const int h = (int)(at % (uint32_t)a.h_k);
+  const int64_t t0 = (int64_t)(at / (uint32_t)a.h_k) * tile;
   const int64_t* slots = a.slot_mapping;
   const T* src = static_cast<const T*>(side ? a.value : a.key) + h * (side ? a.value_stride_head : a.key_stride_head);
   const int64_t st = side ? a.value_stride_tok : a.key_stride_tok;
@@ -61,9 +64,9 @@ __global__ void __launch_bounds__(128) block_write_kernel(mj_cache_write_args a,
   for (uint32_t todo = __ballot_sync(0xffffffffu, first); todo; todo &= todo - 1) {
     const int64_t tb = t0 + __ffs(todo) - 1;
     const int64_t block = slots[tb] >> lg;
-    const int per_page = a.page_size >> lg;
-    const int64_t page = block / per_page;
-    const int sub = (int)(block % per_page);
+    const int lgp = 31 - __clz(a.page_size >> lg);  // blocks of a page, a power of two
+    const int64_t page = block >> lgp;
+    const int sub = (int)block & ((1 << lgp) - 1);
     if (page >= a.num_pages) {
       if (lane == 0) flag(a.status, MJ_DEV_BAD_PAGE);
       continue;
@@ -181,29 +184,38 @@ cudaError_t launch_block_write(const mj_cache_write_args& a, cudaStream_t stream
 // page are looked up once, then each pass moves 512 codes (K and V of two heads
 // at head_size 128), four passes in flight.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) block_read_kernel(mj_block_read_args a, int lg) {
+__global__ void __launch_bounds__(256) block_read_kernel(mj_block_read_args a, int lg, bool wide) {
   griddep_wait();
   const int lane = threadIdx.x & 31;
-  const int groups = (a.h_k + 7) / 8;
-  const int64_t w = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5;
-  const int64_t row = w / groups;
-  if (row >= a.num_rows || row >= a.offsets[a.num_seqs]) return;
-  int lo = 0, hi = a.num_seqs - 1;  // the last sequence whose rows begin at or before this one
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.offsets[mid] <= row) lo = mid;
-    else hi = mid - 1;
+  const int64_t row = blockIdx.x * (int64_t)8 + (threadIdx.x >> 5);
+  if (row >= a.num_rows) return;  // whole warps
+  const int end = a.offsets[a.num_seqs];
+  // The last sequence whose rows begin at or before this one: 32 of the offsets
+  // at a time, each lane's start with it (one memory round trip up to 32 sequences).
+  int lo = 0, len = a.num_seqs;
+  int64_t pos;
+  for (;;) {
+    const int step = (len + 31) / 32, i = lane * step;
+    const bool in = i < len;
+    const int off = in ? a.offsets[lo + i] : INT_MAX, begin = in ? a.starts[lo + i] : 0;
+    const uint32_t at = __ballot_sync(0xffffffffu, off <= row);
+    const int k = at ? 31 - __clz(at) : 0;
+    lo += k * step;
+    pos = row - __shfl_sync(0xffffffffu, off, k) + __shfl_sync(0xffffffffu, begin, k);
+    if (step == 1) break;
+    len = min(step, len - k * step);
   }
-  const int64_t pos = row - a.offsets[lo] + a.starts[lo];
-  const int64_t col = pos / a.page_size;
-  const int r = (int)(pos % a.page_size);
+  if (row >= end) return;
+  const int lgp = 31 - __clz(a.page_size);  // a power of two
+  const int64_t col = pos >> lgp;
+  const int r = (int)pos & (a.page_size - 1);
   int page = -1;
   if (pos >= 0 && col < a.block_table_cols) page = a.block_table[lo * a.block_table_stride + col];
   if (page < 0 || page >= a.num_pages) {
     if (lane == 0) flag(a.status, MJ_DEV_BAD_PAGE);
     return;
   }
-  const int h0 = (int)(w % groups) * 8, h1 = min(h0 + 8, a.h_k);
+  const int h0 = blockIdx.y * 8, h1 = min(h0 + 8, a.h_k);
   constexpr int CPR = D / 16, NB = 4;
   const unsigned char* kc = static_cast<const unsigned char*>(a.k_cache) + page * a.k_stride_page + r * a.k_stride_row;
   const unsigned char* vc = static_cast<const unsigned char*>(a.v_cache) + page * a.v_stride_page + r * a.v_stride_row;
@@ -227,21 +239,29 @@ __global__ void __launch_bounds__(256) block_read_kernel(mj_block_read_args a, i
       if (c >= total) break;
       T* out = (side ? vo + h * a.vo_stride_head : ko + h * a.ko_stride_head) + (c % CPR) * 16;
       const float f = block_scale(e[i]);
-      float v[8];
+      float v[16];
       dequantize8(make_uint2(codes[i].x, codes[i].y), f, v);
-      store8(out, v);
-      dequantize8(make_uint2(codes[i].z, codes[i].w), f, v);
-      store8(out + 8, v);
+      dequantize8(make_uint2(codes[i].z, codes[i].w), f, v + 8);
+      if (wide) {
+        uint4 raw[sizeof(T)];
+        store8(reinterpret_cast<T*>(raw), v);
+        store8(reinterpret_cast<T*>(raw) + 8, v + 8);
+#pragma unroll
+        for (int x = 0; x < (int)sizeof(T); x += 2) store32(reinterpret_cast<uint4*>(out) + x, raw[x], raw[x + 1]);
+      } else {
+        store8(out, v);
+        store8(out + 8, v + 8);
+      }
     }
   }
 }
 
 template <typename T>
 static cudaError_t read_t(const mj_block_read_args& a, int lg, cudaStream_t stream) {
-  const int64_t warps = a.num_rows * ((a.h_k + 7) / 8);
-  const dim3 grid((unsigned)((warps + 7) / 8));
-  if (a.head_size == 256) return launch_kernel(block_read_kernel<T, 256>, grid, dim3(256), 0, stream, a, lg);
-  return launch_kernel(block_read_kernel<T, 128>, grid, dim3(256), 0, stream, a, lg);
+  const dim3 grid((unsigned)((a.num_rows + 7) / 8), (unsigned)((a.h_k + 7) / 8));
+  const bool wide = ((uintptr_t)a.k_out | (uintptr_t)a.v_out | ((a.ko_stride_tok | a.ko_stride_head | a.vo_stride_tok | a.vo_stride_head) * sizeof(T))) % 32 == 0;
+  if (a.head_size == 256) return launch_kernel(block_read_kernel<T, 256>, grid, dim3(256), 0, stream, a, lg, wide);
+  return launch_kernel(block_read_kernel<T, 128>, grid, dim3(256), 0, stream, a, lg, wide);
 }
 
 cudaError_t launch_block_read(const mj_block_read_args& a, cudaStream_t stream) {

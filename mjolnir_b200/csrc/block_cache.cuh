@@ -59,6 +59,12 @@ __device__ __forceinline__ void store8(__half* p, const float* v) {
   for (int i = 0; i < 4; ++i) e[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
   *reinterpret_cast<uint4*>(p) = raw;
 }
+// 32 bytes at a 32-byte aligned address
+__device__ __forceinline__ void store32(void* p, uint4 a, uint4 b) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x),
+               "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
+}
 
 // 8 elements of a row as they are in memory
 template <typename T>

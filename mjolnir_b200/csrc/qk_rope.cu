@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(mj_qk_norm_rope_args 
   const int64_t unit = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> team_log2;
   const int j = threadIdx.x & (team - 1);
   const int qg = (a.h_q + HG - 1) / HG, groups = qg + (a.h_k + HG - 1) / HG;
-  const int64_t t = unit / groups;
+  const int64_t t = unit >> 32 ? unit / groups : (uint32_t)unit / (uint32_t)groups;  // a 64-bit division is a long routine
   int g = (int)(unit - t * groups);
   const int nc = a.head_size >> 3, r2 = a.rot_dim >> 4;  // chunks of a row, rotating chunk pairs
   const bool is_k = g >= qg;
