@@ -184,7 +184,7 @@ cudaError_t launch_block_write(const mj_cache_write_args& a, cudaStream_t stream
 // page are looked up once, then each pass moves 512 codes (K and V of two heads
 // at head_size 128), four passes in flight.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) block_read_kernel(mj_block_read_args a, int lg, bool wide) {
+__global__ void __launch_bounds__(256, 4) block_read_kernel(mj_block_read_args a, int lg, bool wide) {
   griddep_wait();
   const int lane = threadIdx.x & 31;
   const int64_t row = blockIdx.x * (int64_t)8 + (threadIdx.x >> 5);

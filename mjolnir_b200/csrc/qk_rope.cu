@@ -13,6 +13,8 @@
 
 namespace mj {
 
+using namespace sm100;
+
 // 8 elements of a row; vec: its address is 16-byte aligned
 template <typename T>
 __device__ __forceinline__ void load_chunk(const T* p, float* v, bool vec) {
@@ -50,7 +52,7 @@ __device__ __forceinline__ void rotate(float& a, float& b, float c, float s) {
 // loads are in flight together.
 // VEC: every row, weight and table address is 16-byte aligned (host-checked)
 template <typename T, int HG, bool VEC>
-__global__ void __launch_bounds__(256) qk_norm_rope_kernel(mj_qk_norm_rope_args a, int team_log2) {
+__global__ void __launch_bounds__(128) qk_norm_rope_kernel(mj_qk_norm_rope_args a, int team_log2) {
   griddep_wait();
   const int team = 1 << team_log2;
   const int64_t unit = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> team_log2;
@@ -66,8 +68,6 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(mj_qk_norm_rope_args 
   const int ca = a.interleaved || j >= r2 ? 2 * j : j, cb = a.interleaved || j >= r2 ? 2 * j + 1 : j + r2;
   const bool turns = mine && r2 && (a.interleaved ? 16 * j < a.rot_dim : j < r2);
   const int64_t pos = mine && r2 ? a.positions[t] : 0;
-  const bool bad = mine && r2 && (pos < 0 || pos >= a.num_positions);
-  if (bad && j == 0) flag(a.status, MJ_DEV_BAD_POSITION);
   const int64_t st = is_k ? a.k_stride_tok : a.q_stride_tok, sh = is_k ? a.k_stride_head : a.q_stride_head;
   const T* in = static_cast<const T*>(is_k ? a.k : a.q) + t * st + h0 * sh;
   // a missing head's or thread's chunks repeat ones that are there, and are not stored
@@ -81,52 +81,60 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(mj_qk_norm_rope_args 
       ry[h].load(row + 8 * cb * at, VEC);
     }
   }
+  auto f = [](float2* p) { return reinterpret_cast<float*>(p); };
   const void* w = is_k ? a.k_weight : a.q_weight;
-  float wx[8], wy[8], c[8], s[8];
+  float2 wx[4], wy[4], c[4], s[4];  // packed pairs: half the instructions
   if (mine && w) {
-    load_table(w, 8 * ca, a.weight_dtype, wx, VEC);
-    load_table(w, 8 * cb, a.weight_dtype, wy, VEC);
+    load_table(w, 8 * ca, a.weight_dtype, f(wx), VEC);
+    load_table(w, 8 * cb, a.weight_dtype, f(wy), VEC);
   }
+  const bool bad = mine && r2 && (pos < 0 || pos >= a.num_positions);
+  if (bad && j == 0) flag(a.status, MJ_DEV_BAD_POSITION);  // (looked at once the rows are on their way)
   if (turns && !bad) {  // a pair of chunks turns by 8 angles in either pairing
-    load_table(a.cos_sin, pos * a.cos_sin_stride + 8 * j, a.cos_sin_dtype, c, VEC);
-    load_table(a.cos_sin, pos * a.cos_sin_stride + (a.rot_dim >> 1) + 8 * j, a.cos_sin_dtype, s, VEC);
+    load_table(a.cos_sin, pos * a.cos_sin_stride + 8 * j, a.cos_sin_dtype, f(c), VEC);
+    load_table(a.cos_sin, pos * a.cos_sin_stride + (a.rot_dim >> 1) + 8 * j, a.cos_sin_dtype, f(s), VEC);
   }
   T* out = static_cast<T*>(is_k ? a.k_out : a.q_out) + t * (is_k ? a.ko_stride_tok : a.qo_stride_tok);
   const int64_t oh = is_k ? a.ko_stride_head : a.qo_stride_head;
 #pragma unroll
   for (int h = 0; h < HG; ++h) {
     // summed for every row: teams of one warp may differ in having a weight
-    float x[8], y[8], ss = 0.f;
-    rx[h].get(x);
-    ry[h].get(y);
+    float2 x[4], y[4], sq = make_float2(0.f, 0.f);
+    rx[h].get(f(x));
+    ry[h].get(f(y));
     if (mine) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], fmaf(y[i], y[i], ss));
+      for (int i = 0; i < 4; ++i) sq = ffma2(x[i], x[i], ffma2(y[i], y[i], sq));
     }
+    float ss = sq.x + sq.y;
     for (int o = team >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     if (!mine || bad || h >= heads) continue;
     if (w) {
       const float r = rsqrtf(ss / (float)a.head_size + a.eps);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i] *= r * wx[i];
-        y[i] *= r * wy[i];
+      for (int i = 0; i < 4; ++i) {
+        x[i] = fmul2(x[i], fmul2(make_float2(r, r), wx[i]));
+        y[i] = fmul2(y[i], fmul2(make_float2(r, r), wy[i]));
       }
     }
     if (turns) {
       if (a.interleaved) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          rotate(x[2 * i], x[2 * i + 1], c[i], s[i]);
-          rotate(y[2 * i], y[2 * i + 1], c[4 + i], s[4 + i]);
+          rotate(x[i].x, x[i].y, f(c)[i], f(s)[i]);
+          rotate(y[i].x, y[i].y, f(c)[4 + i], f(s)[4 + i]);
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) rotate(x[i], y[i], c[i], s[i]);
+        for (int i = 0; i < 4; ++i) {
+          const float2 t = ffma2(x[i], c[i], fmul2(y[i], make_float2(-s[i].x, -s[i].y)));
+          y[i] = ffma2(y[i], c[i], fmul2(x[i], s[i]));
+          x[i] = t;
+        }
       }
     }
-    store_chunk(out + (h0 + h) * oh + 8 * ca, x, VEC);
-    store_chunk(out + (h0 + h) * oh + 8 * cb, y, VEC);
+    store_chunk(out + (h0 + h) * oh + 8 * ca, f(x), VEC);
+    store_chunk(out + (h0 + h) * oh + 8 * cb, f(y), VEC);
   }
 }
 
@@ -142,12 +150,12 @@ static cudaError_t launch_t(const mj_qk_norm_rope_args& a, bool vec, cudaStream_
         a.cos_sin_stride * cs % 16 == 0;
   auto grid = [&](int hg) {
     const int64_t units = a.num_tokens * ((a.h_q + hg - 1) / hg + (a.h_k + hg - 1) / hg);
-    return dim3((unsigned)(((units << team_log2) + 255) / 256));
+    return dim3((unsigned)(((units << team_log2) + 127) / 128));
   };
-  if (!vec) return launch_kernel(qk_norm_rope_kernel<T, 1, false>, grid(1), dim3(256), 0, stream, a, team_log2);
+  if (!vec) return launch_kernel(qk_norm_rope_kernel<T, 1, false>, grid(1), dim3(128), 0, stream, a, team_log2);
   if ((a.num_tokens * (a.h_q + a.h_k) << team_log2) >= (int64_t)1 << 19)
-    return launch_kernel(qk_norm_rope_kernel<T, kHeads, true>, grid(kHeads), dim3(256), 0, stream, a, team_log2);
-  return launch_kernel(qk_norm_rope_kernel<T, 1, true>, grid(1), dim3(256), 0, stream, a, team_log2);
+    return launch_kernel(qk_norm_rope_kernel<T, kHeads, true>, grid(kHeads), dim3(128), 0, stream, a, team_log2);
+  return launch_kernel(qk_norm_rope_kernel<T, 1, true>, grid(1), dim3(128), 0, stream, a, team_log2);
 }
 
 cudaError_t launch_qk_norm_rope(const mj_qk_norm_rope_args& a, bool vec, cudaStream_t stream) {
