@@ -103,7 +103,10 @@ __device__ __forceinline__ bool drop_nan_codes(uint4& c) {
 __device__ __forceinline__ uint2 quantize8(const float* v, float f) {
   uint16_t c[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) c[i] = sm100::f2_to_e4m3x2(v[2 * i] * f, v[2 * i + 1] * f);
+  for (int i = 0; i < 4; ++i) {
+    const float2 x = sm100::fmul2(make_float2(v[2 * i], v[2 * i + 1]), make_float2(f, f));
+    c[i] = sm100::f2_to_e4m3x2(x.x, x.y);
+  }
   return make_uint2(c[0] | ((uint32_t)c[1] << 16), c[2] | ((uint32_t)c[3] << 16));
 }
 __device__ __forceinline__ void dequantize8(uint2 codes, float f, float* v) {

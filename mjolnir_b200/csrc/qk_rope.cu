@@ -34,12 +34,31 @@ __device__ __forceinline__ void store_chunk(T* p, const float* v, bool vec) {
     for (int i = 0; i < 8; ++i) p[i] = (T)v[i];
   }
 }
-// 8 elements of a table of any of the three types
-__device__ __forceinline__ void load_table(const void* p, int64_t i, int dt, float* v, bool vec) {
-  if (dt == MJ_DT_BF16) load_chunk(static_cast<const __nv_bfloat16*>(p) + i, v, vec);
-  else if (dt == MJ_DT_FP16) load_chunk(static_cast<const __half*>(p) + i, v, vec);
-  else load_chunk(static_cast<const float*>(p) + i, v, vec);
-}
+// 8 elements of a table of any of the three types: as they are in memory, so
+// that several are on their way before one is used, then as floats
+struct RawTable {
+  uint4 v[2];
+  __device__ __forceinline__ void load(const void* p, int64_t i, int dt, bool vec) {
+    const char* q = static_cast<const char*>(p) + i * (dt == MJ_DT_FP32 ? 4 : 2);
+    if (vec) {
+      v[0] = reinterpret_cast<const uint4*>(q)[0];
+      if (dt == MJ_DT_FP32) v[1] = reinterpret_cast<const uint4*>(q)[1];
+    } else if (dt == MJ_DT_FP32) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) reinterpret_cast<uint32_t*>(v)[k] = reinterpret_cast<const uint32_t*>(q)[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) reinterpret_cast<uint16_t*>(v)[k] = reinterpret_cast<const uint16_t*>(q)[k];
+    }
+  }
+  __device__ __forceinline__ void get(int dt, float* x) const {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      x[k] = dt == MJ_DT_BF16   ? (float)reinterpret_cast<const __nv_bfloat16*>(v)[k]
+             : dt == MJ_DT_FP16 ? (float)reinterpret_cast<const __half*>(v)[k]
+                                : reinterpret_cast<const float*>(v)[k];
+  }
+};
 
 __device__ __forceinline__ void rotate(float& a, float& b, float c, float s) {
   const float x = a * c - b * s;
@@ -47,15 +66,21 @@ __device__ __forceinline__ void rotate(float& a, float& b, float c, float s) {
   a = x;
 }
 
+// What bounds it: memory latency. A warp's rows, position, weights and cosines
+// are four groups of loads, of which only the cosines wait for another
+// (the position); five CTAs of 128 threads an SM keep 20 warps of them in
+// flight (4: 39.9 us for 8192 tokens x 40 heads of 128, 5: 35.4, 4.9 TB/s; 6,
+// with spills: 46). A ring of cp.async stages in persistent CTAs took 62.
 // A team takes HG heads of one token's Q, or of its K: the cosines, sines and
 // weights of its two chunks stay in registers for all of them, and the heads'
 // loads are in flight together.
 // VEC: every row, weight and table address is 16-byte aligned (host-checked)
-template <typename T, int HG, bool VEC>
-__global__ void __launch_bounds__(128) qk_norm_rope_kernel(mj_qk_norm_rope_args a, int team_log2) {
+// TL: log2 of a team's threads
+template <typename T, int HG, bool VEC, int TL>
+__global__ void __launch_bounds__(128, 5) qk_norm_rope_kernel(mj_qk_norm_rope_args a, float inv_d) {
   griddep_wait();
-  const int team = 1 << team_log2;
-  const int64_t unit = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> team_log2;
+  constexpr int team = 1 << TL;
+  const int64_t unit = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> TL;
   const int j = threadIdx.x & (team - 1);
   const int qg = (a.h_q + HG - 1) / HG, groups = qg + (a.h_k + HG - 1) / HG;
   const int64_t t = unit >> 32 ? unit / groups : (uint32_t)unit / (uint32_t)groups;  // a 64-bit division is a long routine
@@ -84,16 +109,21 @@ __global__ void __launch_bounds__(128) qk_norm_rope_kernel(mj_qk_norm_rope_args 
   auto f = [](float2* p) { return reinterpret_cast<float*>(p); };
   const void* w = is_k ? a.k_weight : a.q_weight;
   float2 wx[4], wy[4], c[4], s[4];  // packed pairs: half the instructions
+  RawTable raw[2], turn[2];
   if (mine && w) {
-    load_table(w, 8 * ca, a.weight_dtype, f(wx), VEC);
-    load_table(w, 8 * cb, a.weight_dtype, f(wy), VEC);
+    raw[0].load(w, 8 * ca, a.weight_dtype, VEC);
+    raw[1].load(w, 8 * cb, a.weight_dtype, VEC);
   }
   const bool bad = mine && r2 && (pos < 0 || pos >= a.num_positions);
   if (bad && j == 0) flag(a.status, MJ_DEV_BAD_POSITION);  // (looked at once the rows are on their way)
   if (turns && !bad) {  // a pair of chunks turns by 8 angles in either pairing
-    load_table(a.cos_sin, pos * a.cos_sin_stride + 8 * j, a.cos_sin_dtype, f(c), VEC);
-    load_table(a.cos_sin, pos * a.cos_sin_stride + (a.rot_dim >> 1) + 8 * j, a.cos_sin_dtype, f(s), VEC);
+    turn[0].load(a.cos_sin, pos * a.cos_sin_stride + 8 * j, a.cos_sin_dtype, VEC);
+    turn[1].load(a.cos_sin, pos * a.cos_sin_stride + (a.rot_dim >> 1) + 8 * j, a.cos_sin_dtype, VEC);
   }
+  raw[0].get(a.weight_dtype, f(wx));
+  raw[1].get(a.weight_dtype, f(wy));
+  turn[0].get(a.cos_sin_dtype, f(c));
+  turn[1].get(a.cos_sin_dtype, f(s));
   T* out = static_cast<T*>(is_k ? a.k_out : a.q_out) + t * (is_k ? a.ko_stride_tok : a.qo_stride_tok);
   const int64_t oh = is_k ? a.ko_stride_head : a.qo_stride_head;
 #pragma unroll
@@ -107,10 +137,11 @@ __global__ void __launch_bounds__(128) qk_norm_rope_kernel(mj_qk_norm_rope_args 
       for (int i = 0; i < 4; ++i) sq = ffma2(x[i], x[i], ffma2(y[i], y[i], sq));
     }
     float ss = sq.x + sq.y;
+#pragma unroll
     for (int o = team >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     if (!mine || bad || h >= heads) continue;
     if (w) {
-      const float r = rsqrtf(ss / (float)a.head_size + a.eps);
+      const float r = rsqrtf(fmaf(ss, inv_d, a.eps));
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         x[i] = fmul2(x[i], fmul2(make_float2(r, r), wx[i]));
@@ -138,30 +169,34 @@ __global__ void __launch_bounds__(128) qk_norm_rope_kernel(mj_qk_norm_rope_args 
   }
 }
 
-// heads of a thread in large calls: 8192 tokens x 40 heads take 63 us with one,
-// 54 with two, 43 with four and 68 with eight (213 registers)
+// Heads of a thread in large calls: 8192 tokens x 40 heads took 63 us with one,
+// 54 with two, 43 with four and 68 with eight (213 registers) when this was
+// chosen; now 43 with two, 35 with four, 39 with five. Below 2^19 threads one
+// head a thread fills more of the GPU (32 tokens: 2.2 us).
 constexpr int kHeads = 4;
-template <typename T>
+template <typename T, int TL>
 static cudaError_t launch_t(const mj_qk_norm_rope_args& a, bool vec, cudaStream_t stream) {
-  int team_log2 = 0;
-  while ((16 << team_log2) < a.head_size) ++team_log2;
+  if constexpr (TL < 5) {
+    if (a.head_size > 16 << TL) return launch_t<T, TL + 1>(a, vec, stream);
+  }
   const int64_t cs = a.cos_sin_dtype == MJ_DT_FP32 ? 4 : 2;
   vec = vec && (uintptr_t)a.q_weight % 16 == 0 && (uintptr_t)a.k_weight % 16 == 0 && (uintptr_t)a.cos_sin % 16 == 0 &&
         a.cos_sin_stride * cs % 16 == 0;
   auto grid = [&](int hg) {
     const int64_t units = a.num_tokens * ((a.h_q + hg - 1) / hg + (a.h_k + hg - 1) / hg);
-    return dim3((unsigned)(((units << team_log2) + 127) / 128));
+    return dim3((unsigned)(((units << TL) + 127) / 128));
   };
-  if (!vec) return launch_kernel(qk_norm_rope_kernel<T, 1, false>, grid(1), dim3(128), 0, stream, a, team_log2);
-  if ((a.num_tokens * (a.h_q + a.h_k) << team_log2) >= (int64_t)1 << 19)
-    return launch_kernel(qk_norm_rope_kernel<T, kHeads, true>, grid(kHeads), dim3(128), 0, stream, a, team_log2);
-  return launch_kernel(qk_norm_rope_kernel<T, 1, true>, grid(1), dim3(128), 0, stream, a, team_log2);
+  const float inv_d = 1.f / (float)a.head_size;
+  if (!vec) return launch_kernel(qk_norm_rope_kernel<T, 1, false, TL>, grid(1), dim3(128), 0, stream, a, inv_d);
+  if ((a.num_tokens * (a.h_q + a.h_k) << TL) >= (int64_t)1 << 19)
+    return launch_kernel(qk_norm_rope_kernel<T, kHeads, true, TL>, grid(kHeads), dim3(128), 0, stream, a, inv_d);
+  return launch_kernel(qk_norm_rope_kernel<T, 1, true, TL>, grid(1), dim3(128), 0, stream, a, inv_d);
 }
 
 cudaError_t launch_qk_norm_rope(const mj_qk_norm_rope_args& a, bool vec, cudaStream_t stream) {
-  if (a.dtype == MJ_DT_FP32) return launch_t<float>(a, vec, stream);
-  if (a.dtype == MJ_DT_FP16) return launch_t<__half>(a, vec, stream);
-  return launch_t<__nv_bfloat16>(a, vec, stream);
+  if (a.dtype == MJ_DT_FP32) return launch_t<float, 0>(a, vec, stream);
+  if (a.dtype == MJ_DT_FP16) return launch_t<__half, 0>(a, vec, stream);
+  return launch_t<__nv_bfloat16, 0>(a, vec, stream);
 }
 
 }  // namespace mj
