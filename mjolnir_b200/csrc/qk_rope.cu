@@ -77,7 +77,7 @@ __device__ __forceinline__ void rotate(float& a, float& b, float c, float s) {
 // VEC: every row, weight and table address is 16-byte aligned (host-checked)
 // TL: log2 of a team's threads
 template <typename T, int HG, bool VEC, int TL>
-__global__ void __launch_bounds__(128, 5) qk_norm_rope_kernel(mj_qk_norm_rope_args a, float inv_d) {
+__global__ void __launch_bounds__(128, sizeof(T) == 4 ? 3 : 5) qk_norm_rope_kernel(mj_qk_norm_rope_args a, float inv_d) {
   griddep_wait();
   constexpr int team = 1 << TL;
   const int64_t unit = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> TL;
