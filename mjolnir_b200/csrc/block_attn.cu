@@ -18,9 +18,16 @@
 //                        online softmax in base 2, P back to TMEM as f16
 // S is double-buffered in TMEM (64 keys a tile, two buffers and O of both row
 // tiles fill its 512 columns): the next tile's product runs beside this one's
-// softmax, so a softmax warpgroup finds its next scores waiting. With 128 keys
-// and one buffer it waited for the previous product and the next one, two
-// thousand cycles of each tile's five.
+// softmax, so a softmax warpgroup finds its next scores waiting (8192 tokens of
+// 32 / 8 heads of 128: 641 us with 128 keys a tile and one buffer, 614 so).
+//
+// What bounds it: the softmax warps. Such a prompt takes 520 to 590 us (its
+// 550 GFLOP at 0.93 to 1.06 PFLOP/s, by the clock that a run's power leaves),
+// five chunks of 1.5K tokens behind 6K 500 to 540. A tile of 64 keys costs
+// 1,312 cycles of tensor work and 1,024 of exponentials on the special-function
+// unit, hence the polynomial for a quarter of them (587 -> 572 us; for half,
+// 630); two softmax warps on a scheduler hide little of each other's latency,
+// and four with half a row each did no better (586 to 601).
 //
 // Q enters as TERMS e4m3 terms of its row scaled by a power of two to [128,
 // 256): hi + mid holds bf16's 8 bits, a third term f16's 11; what is lost is
@@ -488,9 +495,8 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
         fence_proxy_async_smem();
         mbar_arrive(q_full);
       }
-      // nm: minus the running maximum; a
-      // row that sees no key of the first tile sees none at all (keys are a
-      // prefix) and keeps P = 0. l: the row sum.
+      // nm: minus the running maximum; a row that sees no key of the first tile
+      // sees none at all (keys are a prefix) and keeps P = 0. l: the row sum.
       float nm = 0.f, l = 0.f;
       bool ok = true;
       const uint32_t o_addr = C::O_COL + w * 128 + lane_base;

