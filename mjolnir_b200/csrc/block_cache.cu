@@ -15,6 +15,13 @@
 
 namespace mj {
 
+// Pages need not be powers of two, and a 64-bit division is a long routine: a
+// quotient x / n is the high half of x * ceil(2^64 / n), exact while x * n <
+// 2^64 and never too small. Blocks of a page: n <= 2^16, x < 2^47; rows of a
+// page: n <= 2^20, x < 2^33. For n = 1 the multiplier wraps to 0.
+static uint64_t reciprocal(int n) { return ~0ull / (uint64_t)n + 1; }
+__device__ __forceinline__ int64_t quotient(int64_t x, uint64_t rec) { return rec ? (int64_t)__umul64hi((uint64_t)x, rec) : x; }
+
 // The smallest e with amax <= 448 * 2^(e - 127), 448 = 1.75 * 2^8.
 __device__ __forceinline__ int block_exponent(float amax) {
   const uint32_t u = __float_as_uint(amax);
@@ -61,7 +68,7 @@ __device__ __forceinline__ float max_abs(const Raw8<T> (&v)[NB]) {
 // call's warps more room: 13K tokens 28.6 us with 8, 25.7 with 16, a step of 128
 // rows 4.8 and 6.3, before the magnitudes were compared in pairs; now 22.1 and 4.1)
 template <typename T, int D, int NB>
-__global__ void __launch_bounds__(128) block_write_kernel(mj_cache_write_args a, int lg, int tile) {
+__global__ void __launch_bounds__(128) block_write_kernel(mj_cache_write_args a, int lg, int tile, uint64_t per_page) {
   griddep_wait();
   constexpr int CPR = D / 8;  // 8-element chunks of a row
   __shared__ int members_all[4][128];
@@ -98,9 +105,8 @@ __global__ void __launch_bounds__(128) block_write_kernel(mj_cache_write_args a,
   for (uint32_t todo = __ballot_sync(0xffffffffu, first); todo; todo &= todo - 1) {
     const int64_t tb = t0 + __ffs(todo) - 1;
     const int64_t block = slots[tb] >> lg;
-    const int lgp = 31 - __clz(a.page_size >> lg);  // blocks of a page, a power of two
-    const int64_t page = block >> lgp;
-    const int sub = (int)block & ((1 << lgp) - 1);
+    const int64_t page = quotient(block, per_page);
+    const int sub = (int)(block - page * (a.page_size >> lg));
     if (page >= a.num_pages) {
       if (lane == 0) flag(a.status, MJ_DEV_BAD_PAGE);
       continue;
@@ -206,7 +212,7 @@ static cudaError_t write_t(const mj_cache_write_args& a, int lg, cudaStream_t st
   auto kern = a.head_size == 256 ? tile < 16 ? block_write_kernel<T, 256, NB> : block_write_kernel<T, 256, 2 * NB>
               : tile < 16        ? block_write_kernel<T, 128, NB>
                                  : block_write_kernel<T, 128, 2 * NB>;
-  return launch_kernel(kern, grid, dim3(128), 0, stream, a, lg, tile);
+  return launch_kernel(kern, grid, dim3(128), 0, stream, a, lg, tile, reciprocal(a.page_size >> lg));
 }
 
 cudaError_t launch_block_write(const mj_cache_write_args& a, cudaStream_t stream) {
@@ -222,7 +228,7 @@ cudaError_t launch_block_write(const mj_cache_write_args& a, cudaStream_t stream
 // heads take 67 us, 5.9 TB/s, at four CTAs an SM (at the three that the
 // registers gave by themselves 74, at six 73 with spills; two passes in flight 73).
 template <typename T, int D>
-__global__ void __launch_bounds__(256, 4) block_read_kernel(mj_block_read_args a, int lg, bool wide) {
+__global__ void __launch_bounds__(256, 4) block_read_kernel(mj_block_read_args a, int lg, bool wide, uint64_t per_page) {
   griddep_wait();
   const int lane = threadIdx.x & 31;
   const int64_t row = blockIdx.x * (int64_t)8 + (threadIdx.x >> 5);
@@ -244,9 +250,8 @@ __global__ void __launch_bounds__(256, 4) block_read_kernel(mj_block_read_args a
     len = min(step, len - k * step);
   }
   if (row >= end) return;
-  const int lgp = 31 - __clz(a.page_size);  // a power of two
-  const int64_t col = pos >> lgp;
-  const int r = (int)pos & (a.page_size - 1);
+  const int64_t col = quotient(pos, per_page);
+  const int r = (int)(pos - col * a.page_size);
   int page = -1;
   if (pos >= 0 && col < a.block_table_cols) page = a.block_table[lo * a.block_table_stride + col];
   if (page < 0 || page >= a.num_pages) {
@@ -297,9 +302,10 @@ __global__ void __launch_bounds__(256, 4) block_read_kernel(mj_block_read_args a
 template <typename T>
 static cudaError_t read_t(const mj_block_read_args& a, int lg, cudaStream_t stream) {
   const dim3 grid((unsigned)((a.num_rows + 7) / 8), (unsigned)((a.h_k + 7) / 8));
+  const uint64_t rec = reciprocal(a.page_size);
   const bool wide = ((uintptr_t)a.k_out | (uintptr_t)a.v_out | ((a.ko_stride_tok | a.ko_stride_head | a.vo_stride_tok | a.vo_stride_head) * sizeof(T))) % 32 == 0;
-  if (a.head_size == 256) return launch_kernel(block_read_kernel<T, 256>, grid, dim3(256), 0, stream, a, lg, wide);
-  return launch_kernel(block_read_kernel<T, 128>, grid, dim3(256), 0, stream, a, lg, wide);
+  if (a.head_size == 256) return launch_kernel(block_read_kernel<T, 256>, grid, dim3(256), 0, stream, a, lg, wide, rec);
+  return launch_kernel(block_read_kernel<T, 128>, grid, dim3(256), 0, stream, a, lg, wide, rec);
 }
 
 cudaError_t launch_block_read(const mj_block_read_args& a, cudaStream_t stream) {
