@@ -581,6 +581,9 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
         mbar_arrive(&p_full[at(w, j)]);
       }
       // ---- epilogue: O / l of this row
+      // Staging below goes over the Q tile, whose rows other warps write too. The
+      // last product is behind all of them; without a key tile there is none.
+      if (n == 0) ok = wait(q_full, 0);
       if (ok && n > 0) ok = wait(&o_full[at(w, n - 1)], (n - 1) >> 1);
       if (ok && n > 0) ok = wait(&v_full[(n - 1) % VST], (n - 1) / VST);  // long complete: orders the read of nan_v
       ok = __all_sync(0xffffffffu, ok);
