@@ -59,7 +59,7 @@ extern "C" {
 /* device status word codes (written by kernels into args->status, if given) */
 #define MJ_DEV_OK 0
 #define MJ_DEV_BAD_PAGE 1    /* block-table entry or slot page outside [0, num_pages) */
-#define MJ_DEV_BAD_SPLIT 2   /* work item split >= max_splits or seq >= part_seqs */
+#define MJ_DEV_BAD_SPLIT 2   /* work item split >= max_splits or seq >= part_seqs; a block-attention item or merge out of range */
 #define MJ_DEV_TIMEOUT 3     /* a bounded wait in a pipelined kernel gave up */
 #define MJ_DEV_BAD_POSITION 4 /* a position outside the cos / sin table */
 

@@ -189,7 +189,8 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
   const int h_r = a.h_q / a.h_k;
   const int q0 = a.q_start[seq], n_tok = a.q_start[seq + 1] - q0, L = a.seq_lens[seq];
   const int n_rows = n_tok * h_r;
-  if (row0 < 0 || row0 >= n_rows || q0 < 0 || q0 + (int64_t)n_tok > a.num_tokens || slot >= a.num_slots) {
+  if (row0 < 0 || row0 >= n_rows || q0 < 0 || n_tok < 0 || q0 + (int64_t)n_tok > a.num_tokens || slot >= a.num_slots ||
+      tb < 0 || it0.w > INT_MAX / BN - 2) {
     if (threadIdx.x == 0) flag(a.status, MJ_DEV_BAD_SPLIT);  // uniform: nothing taken yet
     return;
   }
@@ -665,8 +666,17 @@ __global__ void __launch_bounds__(256) block_merge_kernel(const __grid_constant_
   const int64_t m = wi / ROWS / a.h_k;
   if (m >= a.num_merges) return;
   const int4 e = reinterpret_cast<const int4*>(a.merges)[m];
-  const int h_r = a.h_q / a.h_k, q0 = a.q_start[e.x], R = e.y + r;
-  if (R >= (a.q_start[e.x + 1] - q0) * h_r || e.w <= 0) return;
+  if (e.w <= 0) return;
+  if (e.x < 0 || e.x >= a.num_seqs || e.y < 0 || e.z < 0 || e.w > a.num_slots - e.z) {  // uniform in the warp
+    if (lane == 0) flag(a.status, MJ_DEV_BAD_SPLIT);
+    return;
+  }
+  const int h_r = a.h_q / a.h_k, q0 = a.q_start[e.x], n_tok = a.q_start[e.x + 1] - q0;
+  if (q0 < 0 || n_tok < 0 || q0 + (int64_t)n_tok > a.num_tokens) {
+    if (lane == 0) flag(a.status, MJ_DEV_BAD_SPLIT);
+    return;
+  }
+  if (r >= n_tok * h_r - e.y) return;
   const int64_t step = (int64_t)a.h_k * ROWS, first = ((int64_t)e.z * a.h_k + h) * ROWS + r;
   float mx = -INFINITY;
   for (int s = 0; s < e.w; ++s) mx = nan_max(mx, a.lse_part[first + s * step]);  // a NaN partial makes its row NaN
@@ -688,7 +698,7 @@ __global__ void __launch_bounds__(256) block_merge_kernel(const __grid_constant_
       }
     }
   }
-  const int hq = h * h_r + R % h_r;
+  const int R = e.y + r, hq = h * h_r + R % h_r;
   const int64_t tok = q0 + R / h_r;
   T* out = static_cast<T*>(a.o) + tok * a.o_stride_tok + hq * a.o_stride_head;
   const float inv = l == 0.f ? 0.f : 1.f / l;
