@@ -85,7 +85,8 @@ extern "C" {
  * code * 2^(e - 127). Written by mj_block_write, read by mj_block_read,
  * mj_block_attention and mj_decode. Writers produce e in
  * [MJ_BLOCK_E_MIN, MJ_BLOCK_E_MAX]; readers take a byte outside as the nearest
- * of the two. */
+ * of the two. Pages, rows or heads that share their codes (a stride of 0) are
+ * read by mj_block_read only; mj_block_write refuses shared scales too. */
 #define MJ_KV_FP8_B16 5
 #define MJ_KV_FP8_B32 6
 #define MJ_KV_FP8_B64 7

@@ -263,6 +263,15 @@ static const char* block_cache_problem(int head_size, int kv_format, int page_si
   return nullptr;
 }
 
+// True where a stride of 0 lets pages, rows (blocks) or heads share their bytes.
+// In the codes the tensor maps cannot hold that, and a write would race with itself.
+static bool shared_bytes(const int64_t* strides, int64_t pages, int64_t rows, int64_t heads) {
+  const int64_t n[3] = {pages, rows, heads};
+  for (int i = 0; i < 6; ++i)
+    if (n[i % 3] > 1 && !strides[i]) return true;
+  return false;
+}
+
 int mj_qk_norm_rope(const mj_qk_norm_rope_args* args, void* stream) {
   if (!args) return fail(MJ_ERR_INVALID, "mj_qk_norm_rope: null args");
   const mj_qk_norm_rope_args& a = *args;
@@ -319,6 +328,9 @@ int mj_block_write(const mj_cache_write_args* args, void* stream) {
   for (int64_t s : {a.key_stride_tok, a.key_stride_head, a.value_stride_tok, a.value_stride_head}) ok = ok && (s * es) % 16 == 0;
   if (!ok) return fail(MJ_ERR_UNSUPPORTED, "mj_block_write: key / value rows must be 16-byte aligned");
   if (a.num_tokens >= 1 << 24 || a.h_k > 1024) return fail(MJ_ERR_UNSUPPORTED, "mj_block_write: too many rows");
+  if (shared_bytes(st, a.num_pages, a.page_size, a.h_k) ||
+      shared_bytes(ss, a.num_pages, a.page_size >> mj::block_log2(a.kv_format), a.h_k))
+    return fail(MJ_ERR_UNSUPPORTED, "mj_block_write: a cache or scale stride of 0");
   return cuda_status(mj::launch_block_write(a, (cudaStream_t)stream), "mj_block_write launch");
 }
 
@@ -377,6 +389,7 @@ int mj_block_attention(const mj_block_attn_args* args, void* stream) {
       (a.num_merges && (!a.merges || !aligned(a.merges, 16))) || (a.num_slots && (!a.o_part || !a.lse_part || !aligned(a.o_part, 16))))
     return fail(MJ_ERR_INVALID, "mj_block_attention: plan or partial buffers");
   if ((int64_t)a.num_work * a.h_k > (int64_t)INT32_MAX) return fail(MJ_ERR_UNSUPPORTED, "mj_block_attention: too many work items");
+  if (shared_bytes(st, a.num_pages, a.page_size, a.h_k)) return fail(MJ_ERR_UNSUPPORTED, "mj_block_attention: a cache stride of 0");
   return cuda_status(mj::launch_block_attention(a, (cudaStream_t)stream), "mj_block_attention launch");
 }
 

@@ -70,6 +70,9 @@ const char* tc_ineligible(const mj_decode_args& a) {
   for (int i = 0; i < 6; ++i)
     if (st[i] % (int64_t)al) return "KV stride alignment";
   if (a.k_stride_row == 0 || a.v_stride_row == 0) return "row stride";
+  // heads or pages that share their bytes: the tensor maps cannot hold a stride of 0
+  if (a.h_k > 1 && (!a.k_stride_head || !a.v_stride_head)) return "head stride";
+  if (a.num_pages > 1 && (!a.k_stride_page || !a.v_stride_page)) return "page stride";
   if (!encode_fn()) return "cuTensorMapEncodeTiled unavailable";
   return nullptr;
 }
