@@ -242,6 +242,9 @@ class BlockAttention:
         if len(q) != len(kv) or min(q, default=0) < 0 or min(kv, default=0) < 0:
             raise ValueError("query_lens and seq_lens_cpu must pair up, without negative lengths")
         _table(block_table, len(q))
+        longest = max((x for x, n in zip(kv, q) if n), default=0)
+        if longest > block_table.shape[1] * self.page_size:  # the decode kernel knows no end of a table's row
+            raise ValueError(f"{longest} tokens of a sequence are more than block_table's {block_table.shape[1]} pages of {self.page_size}")
         if seq_lens.dtype != torch.int32 or seq_lens.dim() != 1 or seq_lens.shape[0] < len(q) or not seq_lens.is_contiguous():
             raise ValueError("seq_lens must be a contiguous int32 tensor of every sequence")
         _on(self.status.get_device(), block_table, seq_lens)
