@@ -231,10 +231,16 @@ class BlockAttention:
         self.one = torch.ones(1, dtype=torch.float32, device=self.device)
 
     def plan(self, query_lens, seq_lens_cpu, block_table: torch.Tensor, seq_lens: torch.Tensor,
-             causal: bool = True) -> BlockPlan:
+             causal: bool = True, fixed_grid: bool = False) -> BlockPlan:
         """Plan a step: ``query_lens[s]`` new tokens of each sequence, which
         are the last of its ``seq_lens[s]`` tokens. The device ``seq_lens``
-        (int32) are what the kernels mask with."""
+        (int32) are what the kernels mask with.
+
+        A CUDA graph captured over :meth:`run` holds the launches of its plan:
+        it replays that plan only. With ``fixed_grid`` the launches do not
+        depend on the lengths, so the graph replays any later plan with
+        ``fixed_grid`` of as many sequences and the same query length; only
+        steps that the decode kernel serves whole have that form."""
         q = [int(x) for x in query_lens]
         if len(q) > self.max_num_seqs or sum(q) > self.max_num_tokens:
             raise ValueError(f"{len(q)} sequences / {sum(q)} tokens beyond the runner's capacity")
@@ -251,7 +257,10 @@ class BlockAttention:
         decode, few = None, 0
         if q and 1 <= q[0] <= self.max_q_len:
             few = next((i for i, x in enumerate(q) if x != q[0]), len(q))
-            decode = self.decode.plan(kv, few, q[0], block_table, seq_lens, causal=causal)
+            if not fixed_grid or few == len(q):
+                decode = self.decode.plan(kv, few, q[0], block_table, seq_lens, causal=causal, fixed_grid=fixed_grid)
+        if fixed_grid and (few < len(q) or not q):
+            raise ValueError(f"fixed_grid: a step of one query length of 1 to {self.max_q_len} tokens, got {q[:8]}")
         if few == len(q):
             return BlockPlan(q, sum(q), block_table, seq_lens, None, None, None, 0, causal, decode)
         n, (m0, w0) = len(q), self._at
