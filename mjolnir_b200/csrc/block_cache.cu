@@ -58,6 +58,17 @@ __device__ __forceinline__ float max_abs(const Raw8<T> (&v)[NB]) {
   return fmaxf(fmaxf((float)m[0].x, (float)m[0].y), 0.f);
 }
 
+// Skipped tokens are passed 256 at a time, their loads in flight together (a
+// token, or 32, a memory round trip: 8K of them before the first kept one 632 us,
+// behind the last 77; so 15 and 23). True if any of the 256 from u on is kept,
+// or the first or the last token of all where the 256 pass that end.
+__device__ __forceinline__ bool any_kept(const int64_t* slots, int64_t u, int64_t num_tokens, int lane) {
+  int sign = -1;  // the high words hold the sign
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sign &= reinterpret_cast<const int*>(slots + min(max(u + 32 * i + lane, (int64_t)0), num_tokens - 1))[1];
+  return __any_sync(0xffffffffu, sign >= 0);
+}
+
 // One warp per (tile of tokens, KV head, side). A lane per token finds the
 // tokens that begin a block's run in slot_mapping; the warp then takes those
 // blocks in turn: the run's largest magnitude, the scale, the codes, and (only
@@ -90,18 +101,24 @@ __global__ void __launch_bounds__(128) block_write_kernel(mj_cache_write_args a,
   const int64_t ssp = side ? a.vs_stride_page : a.ks_stride_page, ssb = side ? a.vs_stride_row : a.ks_stride_row;
   const int G = 1 << lg;
 
-  // lane i < tile: does token t0 + i begin its block's run?
-  bool first = false;
+  // lane i < tile: does token t0 + i begin its block's run? The kept token before
+  // it is in the tile, but for the tile's first one, whose `far` one is looked
+  // for 32 tokens at a time (lane 0 the nearest; the first 32 come with the tile).
   const int64_t t = t0 + lane;
-  if (lane < tile && t < a.num_tokens) {
-    const int64_t s = slots[t];
-    first = s >= 0;
-    if (first) {
-      int64_t u = t - 1;
-      while (u >= 0 && slots[u] < 0) --u;
-      first = u < 0 || (slots[u] >> lg) != (s >> lg);
-    }
+  int64_t far = t0 > lane ? slots[t0 - 1 - lane] : -1;
+  const int64_t mine = lane < tile && t < a.num_tokens ? slots[t] : -1;
+  const uint32_t kept = __ballot_sync(0xffffffffu, mine >= 0);
+  if (!kept) return;  // whole warps
+  uint32_t found = __ballot_sync(0xffffffffu, far >= 0);
+  for (int64_t u = t0 - 32; !found && u > 0; u -= 32) {
+    while (u > 0 && !any_kept(slots, u - 256, a.num_tokens, lane)) u -= 256;
+    far = u > lane ? slots[u - 1 - lane] : -1;
+    found = __ballot_sync(0xffffffffu, far >= 0);
   }
+  far = __shfl_sync(0xffffffffu, far, found ? __ffs(found) - 1 : 0);
+  const uint32_t below = kept & ((1u << lane) - 1u);
+  const int64_t near = __shfl_sync(0xffffffffu, mine, below ? 31 - __clz(below) : 0);
+  const bool first = mine >= 0 && (mine >> lg) != ((below ? near : far) >> lg);
   for (uint32_t todo = __ballot_sync(0xffffffffu, first); todo; todo &= todo - 1) {
     const int64_t tb = t0 + __ffs(todo) - 1;
     const int64_t block = slots[tb] >> lg;
@@ -131,6 +148,8 @@ __global__ void __launch_bounds__(128) block_write_kernel(mj_cache_write_args a,
       for (int k = 0; k < 4; ++k) rows[k] |= __reduce_or_sync(0xffffffffu, take && (r >> 5) == k ? 1u << (r & 31) : 0u);
       count += __popc(in);
       if (stop || count >= G) break;
+      if (!in)
+        while (u0 + 32 < a.num_tokens && !any_kept(slots, u0 + 32, a.num_tokens, lane)) u0 += 256;
     }
     if (count > G) count = G;
     __syncwarp();
