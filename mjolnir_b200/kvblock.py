@@ -81,7 +81,7 @@ def _rows(name: str, t: torch.Tensor, h_k: int, d: int) -> tuple:
     shape, st = t.shape, t.stride()
     if len(shape) != 3 or shape[1] != h_k or shape[2] != d or st[2] != 1:
         raise ValueError(f"{name} {tuple(shape)} is not (rows, {h_k}, {d}) with contiguous rows")
-    return st[0], st[1]
+    return st[0] if shape[0] > 1 else 0, st[1] if h_k > 1 else 0  # a dim of extent 1 may carry any stride
 
 
 def _on(dev: int, *tensors) -> None:
