@@ -18,29 +18,7 @@ __device__ __forceinline__ int block_e(unsigned char b) {
 }
 __device__ __forceinline__ float block_scale(unsigned char b) { return __uint_as_float((uint32_t)block_e(b) << 23); }
 
-// 8 elements, 16-byte aligned for the 16-bit types and fp32
-__device__ __forceinline__ void load8(const float* p, float* v) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-}
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float* v) {
-  const uint4 raw = *reinterpret_cast<const uint4*>(p);
-  const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&raw);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __bfloat1622float2(e[i]);
-    v[2 * i] = f.x, v[2 * i + 1] = f.y;
-  }
-}
-__device__ __forceinline__ void load8(const __half* p, float* v) {
-  const uint4 raw = *reinterpret_cast<const uint4*>(p);
-  const __half2* e = reinterpret_cast<const __half2*>(&raw);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(e[i]);
-    v[2 * i] = f.x, v[2 * i + 1] = f.y;
-  }
-}
+// 8 elements to a 16-byte aligned address
 __device__ __forceinline__ void store8(float* p, const float* v) {
   reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
   reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);

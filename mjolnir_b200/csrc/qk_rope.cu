@@ -17,15 +17,6 @@ using namespace sm100;
 
 // 8 elements of a row; vec: its address is 16-byte aligned
 template <typename T>
-__device__ __forceinline__ void load_chunk(const T* p, float* v, bool vec) {
-  if (vec) {
-    load8(p, v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (float)p[i];
-  }
-}
-template <typename T>
 __device__ __forceinline__ void store_chunk(T* p, const float* v, bool vec) {
   if (vec) {
     store8(p, v);
