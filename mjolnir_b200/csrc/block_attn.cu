@@ -40,7 +40,13 @@
 // a z exceeds it by 15: moving it means waiting for the last product and
 // rescaling O in TMEM, two thousand cycles of a tile's softmax, and a warp pays
 // for each of its 32 rows (a threshold of 8 did so on most tiles of random
-// scores). f16 holds P' down to 2^-25 of the maximum.
+// scores).
+// P' enters the product as f16 (an exact product would take two), the row sum in
+// fp32: 11 bits down to 2^-14 of the maximum, steps of 2^-24 of it below. With
+// bf16 outputs their own rounding hides that; fp16 outputs are 2.7e-4 from 64
+// bits where fp32 arithmetic leaves 2.1e-4. The maximum counts V's scales: an
+// element that one block holds zeros in loses bits of a block whose V scale is
+// more than 2^14 below that one's, and all of them beyond 2^25.
 //
 // Every mbarrier wait is bounded; on a timeout the CTA flags MJ_DEV_TIMEOUT,
 // all roles stop, the copies and MMAs in flight complete and TMEM is freed.
