@@ -160,10 +160,14 @@ __global__ void __launch_bounds__(128, sizeof(T) == 4 ? 3 : 5) qk_norm_rope_kern
   }
 }
 
-// Heads of a thread in large calls: 8192 tokens x 40 heads took 63 us with one,
-// 54 with two, 43 with four and 68 with eight (213 registers) when this was
-// chosen; now 43 with two, 35 with four, 39 with five. Below 2^19 threads one
-// head a thread fills more of the GPU (32 tokens: 2.2 us).
+// Heads of a thread: four in large calls (8192 tokens x 40 heads 35 us; with two
+// 43, with five 39; 6553 tokens 29, with one 37), one in small ones, to fill the
+// GPU. The edge in 16 bits, one head and four, 40 heads of 128: 2^17 threads 3.2 and 3.6 us, 2^18
+// 5.2 and 4.6, 2^18.9 9.7 and 8.5; in fp32 2^18.5 11.6 and 12.4, 2^20 26.4 and
+// 25.7. Q's and K's heads go to fours each for itself, and the places of a four
+// that no head takes cost as much as heads: at 2^20 threads 1 + 1 heads 19.9 us
+// with one and 31.1 with four, 4 + 1 20.0 and 21.1, 6 + 2 19.8 and 20.5, 8 + 1
+// 20.2 and 19.2. So four where there are at most 4 / 3 places a head.
 constexpr int kHeads = 4;
 template <typename T, int TL>
 static cudaError_t launch_t(const mj_qk_norm_rope_args& a, bool vec, cudaStream_t stream) {
@@ -179,7 +183,8 @@ static cudaError_t launch_t(const mj_qk_norm_rope_args& a, bool vec, cudaStream_
   };
   const float inv_d = 1.f / (float)a.head_size;
   if (!vec) return launch_kernel(qk_norm_rope_kernel<T, 1, false, TL>, grid(1), dim3(128), 0, stream, a, inv_d);
-  if ((a.num_tokens * (a.h_q + a.h_k) << TL) >= (int64_t)1 << 19)
+  const int64_t heads = (int64_t)a.h_q + a.h_k, places = kHeads * (((int64_t)a.h_q + kHeads - 1) / kHeads + ((int64_t)a.h_k + kHeads - 1) / kHeads);
+  if ((a.num_tokens * heads << TL) >= (int64_t)1 << (sizeof(T) == 4 ? 19 : 18) && 3 * places <= 4 * heads)
     return launch_kernel(qk_norm_rope_kernel<T, kHeads, true, TL>, grid(kHeads), dim3(128), 0, stream, a, inv_d);
   return launch_kernel(qk_norm_rope_kernel<T, 1, true, TL>, grid(1), dim3(128), 0, stream, a, inv_d);
 }
