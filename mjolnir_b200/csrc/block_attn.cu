@@ -21,9 +21,12 @@
 // softmax, so a softmax warpgroup finds its next scores waiting (8192 tokens of
 // 32 / 8 heads of 128: 641 us with 128 keys a tile and one buffer, 614 so).
 //
-// What bounds it: the softmax warps. Such a prompt takes 520 to 590 us (its
-// 550 GFLOP at 0.93 to 1.06 PFLOP/s, by the clock that a run's power leaves),
-// five chunks of 1.5K tokens behind 6K 500 to 540. A tile of 64 keys costs
+// What bounds it: the softmax warps. Such a prompt takes 535 to 605 us in a graph
+// (its 550 GFLOP at 0.91 to 1.03 PFLOP/s, by the clock that a run's power leaves:
+// 582 us at a median of 1845 MHz, 1965 without a load), five chunks of 1.5K
+// tokens behind 6K 495 to 555, a prompt of 4K at head size 256 and 24 / 4 heads
+// 260 (0.79 PFLOP/s). The figures below for variants are medians of runs among
+// one another; differences under 3 % are within that spread. A tile of 64 keys costs
 // 1,312 cycles of tensor work and 1,024 of exponentials on the special-function
 // unit, hence the polynomial for a quarter of them (587 -> 572 us; for half,
 // 630); two softmax warps on a scheduler hide little of each other's latency,

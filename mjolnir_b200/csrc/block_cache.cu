@@ -74,10 +74,11 @@ __device__ __forceinline__ bool any_kept(const int64_t* slots, int64_t u, int64_
 // blocks in turn: the run's largest magnitude, the scale, the codes, and (only
 // where an open block's scale grew) the rows already there.
 // What bounds it: memory latency (slots, then the rows, then the codes) beside
-// two passes of arithmetic over the rows: 13K tokens of 8 heads 22.1 us, 3.5 TB/s.
+// two passes of arithmetic over the rows: 13K tokens of 8 heads 21.5 us, 3.6 TB/s
+// (from fp32 28.2 us, 4.1 TB/s).
 // NB: chunks of a lane in flight (16 read a run of 32 rows at once; 8 leave a small
 // call's warps more room: 13K tokens 28.6 us with 8, 25.7 with 16, a step of 128
-// rows 4.8 and 6.3, before the magnitudes were compared in pairs; now 22.1 and 4.1)
+// rows 4.8 and 6.3, before the magnitudes were compared in pairs; now 21.5 and 4.1)
 template <typename T, int D, int NB>
 __global__ void __launch_bounds__(128) block_write_kernel(mj_cache_write_args a, int lg, int tile, uint64_t per_page) {
   griddep_wait();
@@ -222,7 +223,10 @@ static cudaError_t write_t(const mj_cache_write_args& a, int lg, cudaStream_t st
   // A warp looks through `tile` tokens for the runs that begin there. A prompt's
   // tokens begin one run in 16 or more, a decode step's one each: small calls
   // take single tokens, so that a step's rows are not written one after another
-  // (128 rows of 8 heads: 22 us with 16).
+  // (128 rows of 8 heads: 22 us with 16). The slots do not tell the host which it
+  // is; 2,048 warps favour the step. A limit of 1,024, 2,048 and 4,096 warps: a
+  // step of 128 rows 4.7, 4.0 and 4.0 us, of 512 12.4, 9.4 and 9.9; a prompt of
+  // 1000 tokens 5.9, 6.8 and 8.3, of 2000 5.8, 7.7 and 9.2, of 4000 7.5, 7.5, 11.1.
   int tile = 16;
   while (tile > 1 && (a.num_tokens + tile - 1) / tile * a.h_k * 2 < 2048) tile >>= 1;
   const int64_t warps = (a.num_tokens + tile - 1) / tile * a.h_k * 2;
@@ -244,7 +248,7 @@ cudaError_t launch_block_write(const mj_cache_write_args& a, cudaStream_t stream
 // One warp per (output row, group of up to 8 KV heads): the row's sequence and
 // page are looked up once, then each pass moves 512 codes (K and V of two heads
 // at head_size 128), four passes in flight. Bound by memory: 66K tokens of 8
-// heads take 67 us, 5.9 TB/s, at four CTAs an SM (at the three that the
+// heads take 67 us, 5.9 TB/s (to fp32 114 us, 6.4 TB/s), at four CTAs an SM (at the three that the
 // registers gave by themselves 74, at six 73 with spills; two passes in flight 73).
 template <typename T, int D>
 __global__ void __launch_bounds__(256, 4) block_read_kernel(mj_block_read_args a, int lg, bool wide, uint64_t per_page) {

@@ -60,8 +60,9 @@ __device__ __forceinline__ void rotate(float& a, float& b, float c, float s) {
 // What bounds it: memory latency. A warp's rows, position, weights and cosines
 // are four groups of loads, of which only the cosines wait for another
 // (the position); five CTAs of 128 threads an SM keep 20 warps of them in
-// flight (4: 39.9 us for 8192 tokens x 40 heads of 128, 5: 35.4, 4.9 TB/s; 6,
-// with spills: 46). A ring of cp.async stages in persistent CTAs took 62.
+// flight (4: 39.9 us for 8192 tokens x 40 heads of 128, 5: 35.5, 4.8 TB/s, with
+// one or two registers of the 16-bit variants spilled; 6, with more: 46). In fp32
+// the same call is bound by memory, 55 us, 6.2 TB/s. A ring of cp.async stages in persistent CTAs took 62.
 // A team takes HG heads of one token's Q, or of its K: the cosines, sines and
 // weights of its two chunks stay in registers for all of them, and the heads'
 // loads are in flight together.

@@ -192,10 +192,11 @@ class BlockAttention:
     ``max_q_len`` tokens (a batch's decodes, which schedulers put first) run on
     the decode kernel while their rows per KV head fit one of its jobs: 48, or
     16 at head size 256. Beyond, and for the other sequences, the kernel for
-    chunks runs, whose row tiles are 128 (8 KV heads of 128, 16 sequences of
-    8K: 4 rows 75 us against 155, 48 rows 132 against 157, 64 rows of 4 heads
-    154 against 114; head size 256, 4 heads: 12 rows 92 against 135, 48 rows 214
-    against 141)."""
+    chunks runs, whose row tiles are 128. 16 sequences of 8K in a graph, decode
+    kernel and chunk kernel: 8 KV heads of 128, 4 rows 48 and 142 us, 16 rows 66
+    and 143, 48 rows 107 and 144; 4 KV heads of 128, 48 rows 65 and 101, 64 rows
+    134 and 101; 4 KV heads of 256, 6 rows 51 and 117, 16 rows 72 and 118, 18 rows
+    133 and 118, 48 rows 198 and 122."""
 
     def __init__(self, *, num_heads: int, num_kv_heads: int, head_size: int, page_size: int, block_tokens: int = 16,
                  max_num_seqs: int = 256, max_num_tokens: int = 8192, max_q_len: int = 4, device: torch.device | str = "cuda"):
