@@ -46,7 +46,7 @@
 // scores).
 // P' enters the product as f16 (an exact product would take two), the row sum in
 // fp32: 11 bits down to 2^-14 of the maximum, steps of 2^-24 of it below. With
-// bf16 outputs their own rounding hides that; fp16 outputs are 2.7e-4 from 64
+// bf16 outputs their own rounding hides that; fp16 outputs are 2.5e-4 to 3e-4 from 64
 // bits where fp32 arithmetic leaves 2.1e-4. The maximum counts V's scales: an
 // element that one block holds zeros in loses bits of a block whose V scale is
 // more than 2^14 below that one's, and all of them beyond 2^25.
