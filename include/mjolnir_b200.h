@@ -62,6 +62,7 @@ extern "C" {
 #define MJ_DEV_BAD_SPLIT 2   /* work item split >= max_splits or seq >= part_seqs; a block-attention item or merge out of range */
 #define MJ_DEV_TIMEOUT 3     /* a bounded wait in a pipelined kernel gave up */
 #define MJ_DEV_BAD_POSITION 4 /* a position outside the cos / sin table */
+#define MJ_DEV_BAD_LENGTH 5  /* a sequence's length or query rows beyond the tensors that hold them */
 
 /* KV formats. e2m3 / e3m2: 6-bit codes (sign | exponent | mantissa, biases
  * 1 / 3, maxima 7.5 / 28, no inf or NaN) packed 4 per 3 bytes little-endian;
@@ -378,6 +379,20 @@ typedef struct mj_qk_norm_rope_args {
 
 int mj_qk_norm_rope(const mj_qk_norm_rope_args* args, void* stream);
 
+/* The same with a position on each of several axes (time, height and width of
+ * images and video): angle i of token t takes its cosine and sine from table
+ * row positions[axis[i] * axis_stride + t]. A position outside the table on
+ * any axis, used by an angle or not, flags MJ_DEV_BAD_POSITION and leaves
+ * that token's rows untouched. */
+#define MJ_ROPE_AXES 4
+typedef struct mj_rope_axes {
+  int num_axes;             /* 1 .. MJ_ROPE_AXES */
+  int64_t axis_stride;      /* elements between the axes' rows of positions */
+  unsigned char axis[256];  /* the axis of each of the rot_dim / 2 angles */
+} mj_rope_axes;
+
+int mj_qk_norm_rope_axes(const mj_qk_norm_rope_args* args, const mj_rope_axes* axes, void* stream);
+
 /* ------------------------------------------------------------------------ */
 /* Quantising write into a block-scaled cache (kv_format MJ_KV_FP8_B16 ..     */
 /* _B128 of a mj_cache_write_args; k_scale / v_scale and their modes are not  */
@@ -485,6 +500,90 @@ int mj_block_attention(const mj_block_attn_args* args, void* stream);
 int mj_block_plan(const int32_t* query_lens, const int32_t* seq_lens, int num_seqs, int h_q, int h_k, int head_size,
                   int causal, int sm_count, int max_slots, int32_t* work_out, int work_capacity, int32_t* merges_out,
                   int merges_capacity, int* num_work, int* num_merges, int* num_slots);
+
+/* ------------------------------------------------------------------------ */
+/* The attention weight that each cached token receives in a step, added up   */
+/* per KV head. Query rows offsets[s] .. offsets[s + 1] - 1 are the last n_s   */
+/* tokens of sequence s (seq_lens[s] INCLUDES them); query i of n_s sees keys */
+/* 0 .. seq_lens[s] - n_s + i. For every key j of the sequence                */
+/*   weights[s][h][j] = old + sum of exp(softmax_scale q_i . k_j - lse_i)     */
+/* over the query heads of KV head h and the queries that see j, the last     */
+/* `window` ones only where window > 0. old is what the tensor held, but 0 at */
+/* this step's own tokens, j >= seq_lens[s] - n_s. A row whose lse is -inf    */
+/* (it saw no key) adds nothing; a row whose lse is NaN makes the keys it     */
+/* sees NaN. Entries from seq_lens[s] on are left as they were. The sums are  */
+/* taken in a fixed order. A key whose page is outside [0, num_pages) flags   */
+/* MJ_DEV_BAD_PAGE, its entry is unspecified. A sequence longer than          */
+/* weights_cols or than the block table's row, or whose offsets do not lie in */
+/* [0, num_rows], flags MJ_DEV_BAD_LENGTH and is left out.                    */
+typedef struct mj_block_weigh_args {
+  const void* q;                /* (num_rows, h_q, head_size), head dim contiguous, 16-byte aligned rows */
+  int dtype;                    /* MJ_DT_BF16 or MJ_DT_FP16 */
+  int64_t q_stride_tok, q_stride_head; /* elements */
+  const float* lse;             /* (num_rows, h_q) natural-log sum-exp, contiguous */
+  int64_t num_rows;
+  int num_seqs, h_q, h_k, head_size; /* head_size 128 or 256 */
+  int page_size, kv_format;     /* page 16, 32, 64 or 128; MJ_KV_FP8_B16 .. _B128 */
+  const void* k_cache;          /* logical (num_pages, page_size, h_k, head_size) e4m3 codes */
+  int64_t k_stride_page, k_stride_row, k_stride_head;    /* bytes */
+  const void* k_scales;         /* logical (num_pages, page_size / G, h_k) exponent bytes */
+  int64_t ks_stride_page, ks_stride_block, ks_stride_head; /* bytes */
+  int64_t num_pages;
+  const int32_t* block_table; int64_t block_table_stride; int block_table_cols;
+  const int32_t* offsets;       /* (num_seqs + 1,), ascending from 0 */
+  const int32_t* seq_lens;      /* (num_seqs,) */
+  float* weights;               /* (num_seqs, h_k, weights_cols), last dim contiguous */
+  int64_t w_stride_seq, w_stride_head; /* elements */
+  int64_t weights_cols;
+  float softmax_scale;
+  int window;                   /* 0 = every query */
+  int32_t* status;              /* optional device status word (MJ_DEV_*) */
+} mj_block_weigh_args;
+
+int mj_block_weigh(const mj_block_weigh_args* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Tokens dropped from a block-scaled cache by their weights. Of a sequence   */
+/* of L = seq_lens[s] > budget tokens every KV head keeps its last `recent`   */
+/* tokens and the budget - recent others of the largest weights (of equal     */
+/* ones, those of the lowest index; NaN counts as larger than all). Kept      */
+/* tokens move, in their order, to positions 0 .. budget - 1 of the sequence, */
+/* in its own pages, and their weights with them; kept[s][h][i] is the token  */
+/* that position i received. A block takes the smallest e in [95, 159] that   */
+/* the finite values of its kept rows need, as a write of these rows would,   */
+/* and codes become e4m3(code * 2^(e_old - e)), NaN stays NaN. Rows and       */
+/* weights from budget on are left as they were. Shorter sequences are left   */
+/* alone: kept is 0 .. L - 1, then -1. new_lens[s] = min(L, budget).          */
+/* A sequence longer than weights_cols or than the block table's row, or of   */
+/* negative length, flags MJ_DEV_BAD_LENGTH, one with a page outside          */
+/* [0, num_pages) MJ_DEV_BAD_PAGE: it is left alone, its kept are -1 and its  */
+/* new length is its old one. Pages belong to one sequence of the call: where */
+/* they do not, their contents are unspecified.                               */
+typedef struct mj_block_evict_args {
+  void* k_cache;                /* logical (num_pages, page_size, h_k, head_size) e4m3 codes, 16-byte aligned rows */
+  void* v_cache;
+  int64_t k_stride_page, k_stride_row, k_stride_head; /* bytes */
+  int64_t v_stride_page, v_stride_row, v_stride_head; /* bytes */
+  void* k_scales;               /* logical (num_pages, page_size / G, h_k) exponent bytes */
+  void* v_scales;
+  int64_t ks_stride_page, ks_stride_block, ks_stride_head; /* bytes */
+  int64_t vs_stride_page, vs_stride_block, vs_stride_head; /* bytes */
+  int64_t num_pages;
+  int page_size, h_k, head_size; /* any page that the block divides; head_size 128 or 256 */
+  int kv_format;                /* MJ_KV_FP8_B16 .. _B128 */
+  const int32_t* block_table; int64_t block_table_stride; int block_table_cols;
+  const int32_t* seq_lens;      /* (num_seqs,) */
+  int num_seqs;
+  float* weights;               /* (num_seqs, h_k, weights_cols), last dim contiguous */
+  int64_t w_stride_seq, w_stride_head; /* elements */
+  int64_t weights_cols;
+  int budget, recent;           /* 0 <= recent <= budget */
+  int32_t* new_lens;            /* (num_seqs,), not seq_lens itself */
+  int32_t* kept;                /* (num_seqs, h_k, budget) */
+  int32_t* status;              /* optional device status word (MJ_DEV_*) */
+} mj_block_evict_args;
+
+int mj_block_evict(const mj_block_evict_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -24,6 +24,7 @@ MJ_DEV_BAD_PAGE = 1
 MJ_DEV_BAD_SPLIT = 2
 MJ_DEV_TIMEOUT = 3
 MJ_DEV_BAD_POSITION = 4
+MJ_DEV_BAD_LENGTH = 5
 
 MJ_KV_FP8_E4M3 = 0
 MJ_KV_E2M3 = 1
@@ -54,7 +55,8 @@ MJ_SCALE_SEQ_HEAD = 3
 EXPORTED = ("mj_last_error", "mj_abi_version", "mj_row_bytes", "mj_cache_write", "mj_decode", "mj_combine",
             "mj_decode_noalloc", "mj_decode_kernel", "mj_expand_pages", "mj_plan_split_kv", "mj_create", "mj_plan",
             "mj_runner_fill", "mj_runner_status", "mj_destroy", "mj_tc_fallbacks", "mj_qk_norm_rope", "mj_block_write",
-            "mj_block_read", "mj_block_attention", "mj_block_plan")
+            "mj_block_read", "mj_block_attention", "mj_block_plan", "mj_qk_norm_rope_axes",
+            "mj_block_weigh", "mj_block_evict")
 
 _i64, _i32, _vp, _f32 = C.c_int64, C.c_int, C.c_void_p, C.c_float
 
@@ -144,6 +146,13 @@ class QkNormRopeArgs(C.Structure):
     ]
 
 
+ROPE_AXES = 4
+
+
+class RopeAxes(C.Structure):
+    _fields_ = [("num_axes", _i32), ("axis_stride", _i64), ("axis", C.c_ubyte * 256)]
+
+
 _BLOCK_CACHE_FIELDS = [
     ("k_stride_page", _i64), ("k_stride_row", _i64), ("k_stride_head", _i64),
     ("v_stride_page", _i64), ("v_stride_row", _i64), ("v_stride_head", _i64),
@@ -179,6 +188,28 @@ class BlockAttnArgs(C.Structure):
         ("softmax_scale", _f32), ("causal", _i32),
         ("work", _vp), ("num_work", _i32), ("merges", _vp), ("num_merges", _i32),
         ("o_part", _vp), ("lse_part", _vp), ("num_slots", _i32), ("status", _vp),
+    ]
+
+
+class BlockWeighArgs(C.Structure):
+    _fields_ = [
+        ("q", _vp), ("dtype", _i32), ("q_stride_tok", _i64), ("q_stride_head", _i64), ("lse", _vp), ("num_rows", _i64),
+        ("num_seqs", _i32), ("h_q", _i32), ("h_k", _i32), ("head_size", _i32), ("page_size", _i32), ("kv_format", _i32),
+        ("k_cache", _vp), ("k_stride_page", _i64), ("k_stride_row", _i64), ("k_stride_head", _i64),
+        ("k_scales", _vp), ("ks_stride_page", _i64), ("ks_stride_block", _i64), ("ks_stride_head", _i64),
+        ("num_pages", _i64), ("block_table", _vp), ("block_table_stride", _i64), ("block_table_cols", _i32),
+        ("offsets", _vp), ("seq_lens", _vp), ("weights", _vp), ("w_stride_seq", _i64), ("w_stride_head", _i64),
+        ("weights_cols", _i64), ("softmax_scale", _f32), ("window", _i32), ("status", _vp),
+    ]
+
+
+class BlockEvictArgs(C.Structure):
+    _fields_ = [
+        ("k_cache", _vp), ("v_cache", _vp), *_BLOCK_CACHE_FIELDS,
+        ("page_size", _i32), ("h_k", _i32), ("head_size", _i32), ("kv_format", _i32),
+        ("block_table", _vp), ("block_table_stride", _i64), ("block_table_cols", _i32),
+        ("seq_lens", _vp), ("num_seqs", _i32), ("weights", _vp), ("w_stride_seq", _i64), ("w_stride_head", _i64),
+        ("weights_cols", _i64), ("budget", _i32), ("recent", _i32), ("new_lens", _vp), ("kept", _vp), ("status", _vp),
     ]
 
 
@@ -221,9 +252,12 @@ def load():
         lib.mj_expand_pages.argtypes = [C.POINTER(ExpandArgs), _vp]
         lib.mj_expand_pages.restype = C.c_int
         for fn, args in (("mj_qk_norm_rope", QkNormRopeArgs), ("mj_block_write", CacheWriteArgs),
-                         ("mj_block_read", BlockReadArgs), ("mj_block_attention", BlockAttnArgs)):
+                         ("mj_block_read", BlockReadArgs), ("mj_block_attention", BlockAttnArgs),
+                         ("mj_block_weigh", BlockWeighArgs), ("mj_block_evict", BlockEvictArgs)):
             getattr(lib, fn).argtypes = [C.POINTER(args), _vp]
             getattr(lib, fn).restype = C.c_int
+        lib.mj_qk_norm_rope_axes.argtypes = [C.POINTER(QkNormRopeArgs), C.POINTER(RopeAxes), _vp]
+        lib.mj_qk_norm_rope_axes.restype = C.c_int
         _pi = C.POINTER(C.c_int32)
         lib.mj_plan_split_kv.argtypes = [_pi, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                                          C.c_float, _pi, C.c_int, _pi, C.POINTER(C.c_int), C.POINTER(C.c_int)]
@@ -285,6 +319,10 @@ def qk_norm_rope(args: QkNormRopeArgs, stream: int) -> None:
     check(load().mj_qk_norm_rope(C.byref(args), _vp(stream)))
 
 
+def qk_norm_rope_axes(args: tuple[QkNormRopeArgs, RopeAxes], stream: int) -> None:
+    check(load().mj_qk_norm_rope_axes(C.byref(args[0]), C.byref(args[1]), _vp(stream)))
+
+
 def block_write(args: CacheWriteArgs, stream: int) -> None:
     check(load().mj_block_write(C.byref(args), _vp(stream)))
 
@@ -295,6 +333,14 @@ def block_read(args: BlockReadArgs, stream: int) -> None:
 
 def block_attention(args: BlockAttnArgs, stream: int) -> None:
     check(load().mj_block_attention(C.byref(args), _vp(stream)))
+
+
+def block_weigh(args: BlockWeighArgs, stream: int) -> None:
+    check(load().mj_block_weigh(C.byref(args), _vp(stream)))
+
+
+def block_evict(args: BlockEvictArgs, stream: int) -> None:
+    check(load().mj_block_evict(C.byref(args), _vp(stream)))
 
 
 def block_plan(query_lens, seq_lens, h_q: int, h_k: int, head_size: int, causal: bool, sm_count: int, max_slots: int,

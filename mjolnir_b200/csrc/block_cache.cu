@@ -22,13 +22,6 @@ namespace mj {
 static uint64_t reciprocal(int n) { return ~0ull / (uint64_t)n + 1; }
 __device__ __forceinline__ int64_t quotient(int64_t x, uint64_t rec) { return rec ? (int64_t)__umul64hi((uint64_t)x, rec) : x; }
 
-// The smallest e with amax <= 448 * 2^(e - 127), 448 = 1.75 * 2^8.
-__device__ __forceinline__ int block_exponent(float amax) {
-  const uint32_t u = __float_as_uint(amax);
-  const int e = (int)(u >> 23) - 8 + ((u & 0x7FFFFFu) > 0x600000u);
-  return min(max(e, MJ_BLOCK_E_MIN), MJ_BLOCK_E_MAX);
-}
-
 // The largest magnitude of a lane's chunks, NaN left out. 16-bit values are
 // compared in pairs: two instructions a pair.
 template <int NB>

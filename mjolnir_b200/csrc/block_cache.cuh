@@ -18,6 +18,13 @@ __device__ __forceinline__ int block_e(unsigned char b) {
 }
 __device__ __forceinline__ float block_scale(unsigned char b) { return __uint_as_float((uint32_t)block_e(b) << 23); }
 
+// The smallest e with amax <= 448 * 2^(e - 127), 448 = 1.75 * 2^8.
+__device__ __forceinline__ int block_exponent(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  const int e = (int)(u >> 23) - 8 + ((u & 0x7FFFFFu) > 0x600000u);
+  return min(max(e, MJ_BLOCK_E_MIN), MJ_BLOCK_E_MAX);
+}
+
 // 8 elements to a 16-byte aligned address
 __device__ __forceinline__ void store8(float* p, const float* v) {
   reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);

@@ -15,10 +15,12 @@ cudaError_t launch_combine(const mj_decode_args& a, cudaStream_t stream);
 cudaError_t launch_decode_tc(const mj_decode_args& a, cudaStream_t stream, bool* handled, bool dry);
 const char* tc_ineligible(const mj_decode_args& a);
 cudaError_t launch_expand_pages(const mj_expand_args& a, cudaStream_t stream);
-cudaError_t launch_qk_norm_rope(const mj_qk_norm_rope_args& a, bool vec, cudaStream_t stream);
+cudaError_t launch_qk_norm_rope(const mj_qk_norm_rope_args& a, const mj_rope_axes* axes, bool vec, cudaStream_t stream);
 cudaError_t launch_block_write(const mj_cache_write_args& a, cudaStream_t stream);
 cudaError_t launch_block_read(const mj_block_read_args& a, cudaStream_t stream);
 cudaError_t launch_block_attention(const mj_block_attn_args& a, cudaStream_t stream);
+cudaError_t launch_block_weigh(const mj_block_weigh_args& a, cudaStream_t stream);
+cudaError_t launch_block_evict(const mj_block_evict_args& a, cudaStream_t stream);
 }  // namespace mj
 
 static thread_local char g_err[512] = "";
@@ -272,7 +274,7 @@ static bool shared_bytes(const int64_t* strides, int64_t pages, int64_t rows, in
   return false;
 }
 
-int mj_qk_norm_rope(const mj_qk_norm_rope_args* args, void* stream) {
+static int norm_rope(const mj_qk_norm_rope_args* args, const mj_rope_axes* axes, void* stream) {
   if (!args) return fail(MJ_ERR_INVALID, "mj_qk_norm_rope: null args");
   const mj_qk_norm_rope_args& a = *args;
   if (a.num_tokens < 0 || a.h_q < 0 || a.h_k < 0)
@@ -283,6 +285,13 @@ int mj_qk_norm_rope(const mj_qk_norm_rope_args* args, void* stream) {
     return fail(MJ_ERR_UNSUPPORTED, "mj_qk_norm_rope: rot_dim %d (a multiple of 16, at most head_size)", a.rot_dim);
   for (int dt : {a.dtype, a.cos_sin_dtype, a.weight_dtype})
     if (dt < MJ_DT_BF16 || dt > MJ_DT_FP32) return fail(MJ_ERR_INVALID, "mj_qk_norm_rope: dtype %d", dt);
+  if (axes) {
+    if (axes->num_axes < 1 || axes->num_axes > MJ_ROPE_AXES)
+      return fail(MJ_ERR_UNSUPPORTED, "mj_qk_norm_rope_axes: %d axes (1 to %d)", axes->num_axes, MJ_ROPE_AXES);
+    for (int i = 0; i < a.rot_dim / 2; ++i)
+      if (axes->axis[i] >= axes->num_axes)
+        return fail(MJ_ERR_INVALID, "mj_qk_norm_rope_axes: angle %d on axis %d of %d", i, axes->axis[i], axes->num_axes);
+  }
   if (a.num_tokens == 0 || a.h_q + a.h_k == 0) {
     g_err[0] = 0;
     return MJ_OK;
@@ -304,7 +313,14 @@ int mj_qk_norm_rope(const mj_qk_norm_rope_args* args, void* stream) {
     vec = vec && aligned(a.k, 16) && aligned(a.k_out, 16);
     for (int64_t s : {a.k_stride_tok, a.k_stride_head, a.ko_stride_tok, a.ko_stride_head}) vec = vec && (s * es) % 16 == 0;
   }
-  return cuda_status(mj::launch_qk_norm_rope(a, vec, (cudaStream_t)stream), "mj_qk_norm_rope launch");
+  return cuda_status(mj::launch_qk_norm_rope(a, axes, vec, (cudaStream_t)stream), "mj_qk_norm_rope launch");
+}
+
+int mj_qk_norm_rope(const mj_qk_norm_rope_args* args, void* stream) { return norm_rope(args, nullptr, stream); }
+
+int mj_qk_norm_rope_axes(const mj_qk_norm_rope_args* args, const mj_rope_axes* axes, void* stream) {
+  if (!axes) return fail(MJ_ERR_INVALID, "mj_qk_norm_rope_axes: null axes");
+  return norm_rope(args, axes, stream);
 }
 
 int mj_block_write(const mj_cache_write_args* args, void* stream) {
@@ -391,6 +407,69 @@ int mj_block_attention(const mj_block_attn_args* args, void* stream) {
   if ((int64_t)a.num_work * a.h_k > (int64_t)INT32_MAX) return fail(MJ_ERR_UNSUPPORTED, "mj_block_attention: too many work items");
   if (shared_bytes(st, a.num_pages, a.page_size, a.h_k)) return fail(MJ_ERR_UNSUPPORTED, "mj_block_attention: a cache stride of 0");
   return cuda_status(mj::launch_block_attention(a, (cudaStream_t)stream), "mj_block_attention launch");
+}
+
+int mj_block_weigh(const mj_block_weigh_args* args, void* stream) {
+  if (!args) return fail(MJ_ERR_INVALID, "mj_block_weigh: null args");
+  const mj_block_weigh_args& a = *args;
+  if (a.num_seqs < 0 || a.num_rows < 0 || a.h_k <= 0 || a.h_q <= 0 || a.h_q % a.h_k || a.window < 0)
+    return fail(MJ_ERR_INVALID, "mj_block_weigh: num_seqs %d num_rows %lld h_q %d h_k %d window %d", a.num_seqs,
+                (long long)a.num_rows, a.h_q, a.h_k, a.window);
+  const int64_t st[6] = {a.k_stride_page, a.k_stride_row, a.k_stride_head, a.k_stride_page, a.k_stride_row, a.k_stride_head};
+  const int64_t ss[6] = {a.ks_stride_page, a.ks_stride_block, a.ks_stride_head, a.ks_stride_page, a.ks_stride_block, a.ks_stride_head};
+  if (const char* why = block_cache_problem(a.head_size, a.kv_format, a.page_size, a.h_k, a.num_pages, a.k_cache, a.k_cache,
+                                            st, a.k_scales, a.k_scales, ss, 16))
+    return fail(MJ_ERR_UNSUPPORTED, "mj_block_weigh: %s (head_size %d, kv_format %d, page_size %d; 16-byte aligned rows)", why,
+                a.head_size, a.kv_format, a.page_size);
+  if (a.page_size != 16 && a.page_size != 32 && a.page_size != 64 && a.page_size != 128)
+    return fail(MJ_ERR_UNSUPPORTED, "mj_block_weigh: page_size %d (16, 32, 64 or 128)", a.page_size);
+  if (a.dtype != MJ_DT_BF16 && a.dtype != MJ_DT_FP16)
+    return fail(MJ_ERR_UNSUPPORTED, "mj_block_weigh: dtype %d (bf16 or fp16)", a.dtype);
+  if (a.num_seqs == 0 || a.num_rows == 0) {
+    g_err[0] = 0;
+    return MJ_OK;
+  }
+  if (!a.q || !a.lse || !a.block_table || a.block_table_cols <= 0 || !a.offsets || !a.seq_lens || !a.weights)
+    return fail(MJ_ERR_INVALID, "mj_block_weigh: null pointer argument");
+  if (a.weights_cols < 0 || a.w_stride_seq < 0 || a.w_stride_head < 0)
+    return fail(MJ_ERR_INVALID, "mj_block_weigh: weights of %lld columns", (long long)a.weights_cols);
+  if ((a.num_seqs > 1 && !a.w_stride_seq) || (a.h_k > 1 && !a.w_stride_head))
+    return fail(MJ_ERR_UNSUPPORTED, "mj_block_weigh: a weights stride of 0");
+  if (!aligned(a.q, 16) || a.q_stride_tok % 8 || a.q_stride_head % 8 || a.q_stride_tok < 0 || a.q_stride_head < 0)
+    return fail(MJ_ERR_UNSUPPORTED, "mj_block_weigh: q rows must be 16-byte aligned");
+  if (a.num_rows * a.h_q > (int64_t)INT32_MAX || a.num_seqs > 1 << 20) return fail(MJ_ERR_UNSUPPORTED, "mj_block_weigh: too many rows");
+  if (shared_bytes(st, a.num_pages, a.page_size, a.h_k)) return fail(MJ_ERR_UNSUPPORTED, "mj_block_weigh: a cache stride of 0");
+  return cuda_status(mj::launch_block_weigh(a, (cudaStream_t)stream), "mj_block_weigh launch");
+}
+
+int mj_block_evict(const mj_block_evict_args* args, void* stream) {
+  if (!args) return fail(MJ_ERR_INVALID, "mj_block_evict: null args");
+  const mj_block_evict_args& a = *args;
+  if (a.num_seqs < 0 || a.budget < 0 || a.recent < 0 || a.recent > a.budget)
+    return fail(MJ_ERR_INVALID, "mj_block_evict: num_seqs %d budget %d recent %d", a.num_seqs, a.budget, a.recent);
+  const int64_t st[6] = {a.k_stride_page, a.k_stride_row, a.k_stride_head, a.v_stride_page, a.v_stride_row, a.v_stride_head};
+  const int64_t ss[6] = {a.ks_stride_page, a.ks_stride_block, a.ks_stride_head, a.vs_stride_page, a.vs_stride_block, a.vs_stride_head};
+  if (const char* why = block_cache_problem(a.head_size, a.kv_format, a.page_size, a.h_k, a.num_pages, a.k_cache, a.v_cache,
+                                            st, a.k_scales, a.v_scales, ss, 16))
+    return fail(MJ_ERR_UNSUPPORTED, "mj_block_evict: %s (head_size %d, kv_format %d, page_size %d; 16-byte aligned rows)", why,
+                a.head_size, a.kv_format, a.page_size);
+  if (a.num_seqs == 0) {
+    g_err[0] = 0;
+    return MJ_OK;
+  }
+  if (!a.block_table || a.block_table_cols <= 0 || !a.seq_lens || !a.weights || !a.new_lens || (a.budget && !a.kept))
+    return fail(MJ_ERR_INVALID, "mj_block_evict: null pointer argument");
+  if (a.weights_cols < 0 || a.weights_cols > INT32_MAX || a.w_stride_seq < 0 || a.w_stride_head < 0)
+    return fail(MJ_ERR_INVALID, "mj_block_evict: weights of %lld columns", (long long)a.weights_cols);
+  if ((a.num_seqs > 1 && !a.w_stride_seq) || (a.h_k > 1 && !a.w_stride_head))
+    return fail(MJ_ERR_UNSUPPORTED, "mj_block_evict: a weights stride of 0");
+  if (a.new_lens < a.seq_lens + a.num_seqs && a.seq_lens < a.new_lens + a.num_seqs)
+    return fail(MJ_ERR_INVALID, "mj_block_evict: new_lens overlaps seq_lens, which every KV head reads");
+  if ((int64_t)a.num_seqs * a.h_k > 1 << 24 || a.budget > 1 << 24) return fail(MJ_ERR_UNSUPPORTED, "mj_block_evict: too many rows");
+  if (shared_bytes(st, a.num_pages, a.page_size, a.h_k) ||
+      shared_bytes(ss, a.num_pages, a.page_size >> mj::block_log2(a.kv_format), a.h_k))
+    return fail(MJ_ERR_UNSUPPORTED, "mj_block_evict: a cache or scale stride of 0");
+  return cuda_status(mj::launch_block_evict(a, (cudaStream_t)stream), "mj_block_evict launch");
 }
 
 }  // extern "C"

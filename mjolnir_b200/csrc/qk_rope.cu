@@ -9,6 +9,8 @@
 // (i, i + rot_dim / 2) those are the same chunk of both halves, so every
 // rotation is inside one thread and the row's sum of squares is the only
 // exchange.
+#include <type_traits>
+
 #include "block_cache.cuh"
 
 namespace mj {
@@ -25,6 +27,9 @@ __device__ __forceinline__ void store_chunk(T* p, const float* v, bool vec) {
     for (int i = 0; i < 8; ++i) p[i] = (T)v[i];
   }
 }
+// Without axes: every angle turns by positions[token].
+struct NoAxes {};
+
 // 8 elements of a table of any of the three types: as they are in memory, so
 // that several are on their way before one is used, then as floats
 struct RawTable {
@@ -41,6 +46,11 @@ struct RawTable {
 #pragma unroll
       for (int k = 0; k < 8; ++k) reinterpret_cast<uint16_t*>(v)[k] = reinterpret_cast<const uint16_t*>(q)[k];
     }
+  }
+  // element k (a constant) alone
+  __device__ __forceinline__ void load_one(const void* p, int64_t i, int k, int dt) {
+    if (dt == MJ_DT_FP32) reinterpret_cast<uint32_t*>(v)[k] = static_cast<const uint32_t*>(p)[i];
+    else reinterpret_cast<uint16_t*>(v)[k] = static_cast<const uint16_t*>(p)[i];
   }
   __device__ __forceinline__ void get(int dt, float* x) const {
 #pragma unroll
@@ -68,8 +78,13 @@ __device__ __forceinline__ void rotate(float& a, float& b, float c, float s) {
 // loads are in flight together.
 // VEC: every row, weight and table address is 16-byte aligned (host-checked)
 // TL: log2 of a team's threads
-template <typename T, int HG, bool VEC, int TL>
-__global__ void __launch_bounds__(128, sizeof(T) == 4 ? 3 : 5) qk_norm_rope_kernel(mj_qk_norm_rope_args a, float inv_d) {
+// AX: mj_rope_axes, or NoAxes. With axes a token has a position on each, all of
+// them loaded and checked by every thread of the token; a thread's 8 angles
+// that follow one axis come from its table row in vectors, others one by one.
+template <typename T, int HG, bool VEC, int TL, typename AX>
+__global__ void __launch_bounds__(128, sizeof(T) == 4 ? 3 : 5)
+    qk_norm_rope_kernel(mj_qk_norm_rope_args a, float inv_d, const __grid_constant__ AX ax) {
+  constexpr bool kAxes = !std::is_same<AX, NoAxes>::value;
   griddep_wait();
   constexpr int team = 1 << TL;
   const int64_t unit = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> TL;
@@ -84,7 +99,12 @@ __global__ void __launch_bounds__(128, sizeof(T) == 4 ? 3 : 5) qk_norm_rope_kern
   const bool mine = t < a.num_tokens && 2 * j < nc;
   const int ca = a.interleaved || j >= r2 ? 2 * j : j, cb = a.interleaved || j >= r2 ? 2 * j + 1 : j + r2;
   const bool turns = mine && r2 && (a.interleaved ? 16 * j < a.rot_dim : j < r2);
-  const int64_t pos = mine && r2 ? a.positions[t] : 0;
+  int64_t pos = mine && r2 ? a.positions[t] : 0;
+  int64_t more[MJ_ROPE_AXES - 1];  // positions on the axes after the first
+  if constexpr (kAxes) {
+#pragma unroll
+    for (int x = 1; x < MJ_ROPE_AXES; ++x) more[x - 1] = mine && x < ax.num_axes ? a.positions[x * ax.axis_stride + t] : 0;
+  }
   const int64_t st = is_k ? a.k_stride_tok : a.q_stride_tok, sh = is_k ? a.k_stride_head : a.q_stride_head;
   const T* in = static_cast<const T*>(is_k ? a.k : a.q) + t * st + h0 * sh;
   // a missing head's or thread's chunks repeat ones that are there, and are not stored
@@ -106,11 +126,39 @@ __global__ void __launch_bounds__(128, sizeof(T) == 4 ? 3 : 5) qk_norm_rope_kern
     raw[0].load(w, 8 * ca, a.weight_dtype, VEC);
     raw[1].load(w, 8 * cb, a.weight_dtype, VEC);
   }
-  const bool bad = mine && r2 && (pos < 0 || pos >= a.num_positions);
+  bool bad = mine && r2 && (pos < 0 || pos >= a.num_positions);
+  if constexpr (kAxes) {
+#pragma unroll
+    for (int x = 0; x < MJ_ROPE_AXES - 1; ++x) bad |= more[x] < 0 || more[x] >= a.num_positions;
+  }
   if (bad && j == 0) flag(a.status, MJ_DEV_BAD_POSITION);  // (looked at once the rows are on their way)
   if (turns && !bad) {  // a pair of chunks turns by 8 angles in either pairing
-    turn[0].load(a.cos_sin, pos * a.cos_sin_stride + 8 * j, a.cos_sin_dtype, VEC);
-    turn[1].load(a.cos_sin, pos * a.cos_sin_stride + (a.rot_dim >> 1) + 8 * j, a.cos_sin_dtype, VEC);
+    bool one = true;
+    if constexpr (kAxes) {
+      const uint2 axis = *reinterpret_cast<const uint2*>(ax.axis + 8 * j);
+      auto on = [&](int k) {  // the position of angle k of the 8
+        const uint32_t x = (k < 4 ? axis.x : axis.y) >> (8 * (k & 3)) & 0xFFu;
+        int64_t p = pos;
+#pragma unroll
+        for (uint32_t i = 1; i < MJ_ROPE_AXES; ++i) p = x == i ? more[i - 1] : p;
+        return p;
+      };
+      one = axis.x == axis.y && axis.x == (axis.x & 0xFFu) * 0x01010101u;
+      if (one) {
+        pos = on(0);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int64_t at = on(k) * a.cos_sin_stride + 8 * j + k;
+          turn[0].load_one(a.cos_sin, at, k, a.cos_sin_dtype);
+          turn[1].load_one(a.cos_sin, at + (a.rot_dim >> 1), k, a.cos_sin_dtype);
+        }
+      }
+    }
+    if (one) {
+      turn[0].load(a.cos_sin, pos * a.cos_sin_stride + 8 * j, a.cos_sin_dtype, VEC);
+      turn[1].load(a.cos_sin, pos * a.cos_sin_stride + (a.rot_dim >> 1) + 8 * j, a.cos_sin_dtype, VEC);
+    }
   }
   raw[0].get(a.weight_dtype, f(wx));
   raw[1].get(a.weight_dtype, f(wy));
@@ -170,10 +218,10 @@ __global__ void __launch_bounds__(128, sizeof(T) == 4 ? 3 : 5) qk_norm_rope_kern
 // with one and 31.1 with four, 4 + 1 20.0 and 21.1, 6 + 2 19.8 and 20.5, 8 + 1
 // 20.2 and 19.2. So four where there are at most 4 / 3 places a head.
 constexpr int kHeads = 4;
-template <typename T, int TL>
-static cudaError_t launch_t(const mj_qk_norm_rope_args& a, bool vec, cudaStream_t stream) {
+template <typename T, int TL, typename AX>
+static cudaError_t launch_t(const mj_qk_norm_rope_args& a, const AX& ax, bool vec, cudaStream_t stream) {
   if constexpr (TL < 5) {
-    if (a.head_size > 16 << TL) return launch_t<T, TL + 1>(a, vec, stream);
+    if (a.head_size > 16 << TL) return launch_t<T, TL + 1>(a, ax, vec, stream);
   }
   const int64_t cs = a.cos_sin_dtype == MJ_DT_FP32 ? 4 : 2;
   vec = vec && (uintptr_t)a.q_weight % 16 == 0 && (uintptr_t)a.k_weight % 16 == 0 && (uintptr_t)a.cos_sin % 16 == 0 &&
@@ -183,17 +231,22 @@ static cudaError_t launch_t(const mj_qk_norm_rope_args& a, bool vec, cudaStream_
     return dim3((unsigned)(((units << TL) + 127) / 128));
   };
   const float inv_d = 1.f / (float)a.head_size;
-  if (!vec) return launch_kernel(qk_norm_rope_kernel<T, 1, false, TL>, grid(1), dim3(128), 0, stream, a, inv_d);
+  if (!vec) return launch_kernel(qk_norm_rope_kernel<T, 1, false, TL, AX>, grid(1), dim3(128), 0, stream, a, inv_d, ax);
   const int64_t heads = (int64_t)a.h_q + a.h_k, places = kHeads * (((int64_t)a.h_q + kHeads - 1) / kHeads + ((int64_t)a.h_k + kHeads - 1) / kHeads);
   if ((a.num_tokens * heads << TL) >= (int64_t)1 << (sizeof(T) == 4 ? 19 : 18) && 3 * places <= 4 * heads)
-    return launch_kernel(qk_norm_rope_kernel<T, kHeads, true, TL>, grid(kHeads), dim3(128), 0, stream, a, inv_d);
-  return launch_kernel(qk_norm_rope_kernel<T, 1, true, TL>, grid(1), dim3(128), 0, stream, a, inv_d);
+    return launch_kernel(qk_norm_rope_kernel<T, kHeads, true, TL, AX>, grid(kHeads), dim3(128), 0, stream, a, inv_d, ax);
+  return launch_kernel(qk_norm_rope_kernel<T, 1, true, TL, AX>, grid(1), dim3(128), 0, stream, a, inv_d, ax);
 }
 
-cudaError_t launch_qk_norm_rope(const mj_qk_norm_rope_args& a, bool vec, cudaStream_t stream) {
-  if (a.dtype == MJ_DT_FP32) return launch_t<float, 0>(a, vec, stream);
-  if (a.dtype == MJ_DT_FP16) return launch_t<__half, 0>(a, vec, stream);
-  return launch_t<__nv_bfloat16, 0>(a, vec, stream);
+template <typename AX>
+static cudaError_t launch(const mj_qk_norm_rope_args& a, const AX& ax, bool vec, cudaStream_t stream) {
+  if (a.dtype == MJ_DT_FP32) return launch_t<float, 0>(a, ax, vec, stream);
+  if (a.dtype == MJ_DT_FP16) return launch_t<__half, 0>(a, ax, vec, stream);
+  return launch_t<__nv_bfloat16, 0>(a, ax, vec, stream);
+}
+
+cudaError_t launch_qk_norm_rope(const mj_qk_norm_rope_args& a, const mj_rope_axes* ax, bool vec, cudaStream_t stream) {
+  return ax && a.rot_dim ? launch(a, *ax, vec, stream) : launch(a, NoAxes(), vec, stream);
 }
 
 }  // namespace mj

@@ -12,7 +12,11 @@ functions take logical views -- codes ``(pages, page_size, h_k, d)``, exponents
 * :func:`write` -- quantise new K / V rows into the cache;
 * :func:`read` -- cached tokens back as contiguous rows;
 * :class:`BlockAttention` -- attention of ragged query chunks (and of single
-  tokens) over the cache.
+  tokens) over the cache;
+* :func:`weigh` -- the attention weight that each cached token received, added
+  up over steps;
+* :func:`evict` -- the tokens of least weight dropped, the others moved
+  together.
 """
 
 from __future__ import annotations
@@ -164,6 +168,112 @@ def read(
         n, k_out.shape[0], k_out.data_ptr(), v_out.data_ptr(), dtype_code(k_out.dtype), *ko, *vo, _ptr(status))
     call(_lib.block_read, a, dev)
     return k_out, v_out
+
+
+def _weights(weights: torch.Tensor, num_seqs: int, h_k: int) -> tuple:
+    """(sequence, head) strides of checked weights."""
+    shape, st = weights.shape, weights.stride()
+    if weights.dtype != torch.float32 or len(shape) != 3 or shape[0] < num_seqs or shape[1] != h_k or (shape[2] > 1 and st[2] != 1):
+        raise ValueError(f"weights must be fp32 (>= {num_seqs}, {h_k}, tokens) with contiguous rows, got {weights.dtype} {tuple(shape)}")
+    return st[0] if num_seqs > 1 else 0, st[1] if h_k > 1 else 0
+
+
+def _side(k_cache: torch.Tensor, k_scales: torch.Tensor) -> tuple:
+    """K's part of :func:`_cache`."""
+    shape, kv_format, dev, st, ss = _cache(k_cache, k_cache, k_scales, k_scales)
+    return shape, kv_format, dev, st[:3], ss[:3]
+
+
+def weigh(
+    query: torch.Tensor,  # (>= offsets[-1], h_q, d) bf16 / fp16, 16-byte aligned rows
+    lse: torch.Tensor,  # (>= offsets[-1], h_q) fp32, contiguous: natural-log sum-exp of the step's attention
+    k_cache: torch.Tensor,  # (pages, page_size, h_k, d) byte view
+    k_scales: torch.Tensor,  # (pages, page_size / G, h_k) byte view
+    block_table: torch.Tensor,  # (>= n, blocks) int32
+    offsets: torch.Tensor,  # (n + 1,) int32: the query rows of each sequence, ascending from 0
+    seq_lens: torch.Tensor,  # (n,) int32, the step's tokens included
+    weights: torch.Tensor,  # (>= n, h_k, tokens) fp32, any sequence and head strides, updated in place
+    softmax_scale: float,
+    *,
+    window: int = 0,
+    status: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Add the causal attention weight that each cached token received in a
+    step, ``exp(scale q.k - lse)`` over the queries and heads of its KV head
+    that see it, to ``weights``; the step's own tokens start from 0. Query rows
+    ``offsets[s] .. offsets[s + 1] - 1`` are the last tokens of sequence ``s``,
+    as :meth:`BlockAttention.run` takes them, which leaves their ``lse``. With
+    ``window`` only the last that many queries of each sequence count. Entries
+    from ``seq_lens[s]`` on are left as they were. Returns ``weights``.
+
+    The lengths are read on the device alone: a captured CUDA graph replays the
+    call for whatever they hold then."""
+    (pages, page_size, h_k, d), kv_format, dev, st, ss = _side(k_cache, k_scales)
+    n = seq_lens.shape[0] if seq_lens.dim() == 1 else -1
+    for name, t, m in (("seq_lens", seq_lens, n), ("offsets", offsets, n + 1)):
+        if t.dtype != torch.int32 or t.shape != (m,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 ({m if n >= 0 else 'n'},), got {t.dtype} {tuple(t.shape)}")
+    _table(block_table, n)
+    h_q = query.shape[1] if query.dim() == 3 else 0
+    qs, ws = _rows("query", query, h_q, d), _weights(weights, n, h_k)
+    if h_q < 1 or h_q % h_k:
+        raise ValueError(f"query heads {h_q} must be a multiple of the cache's {h_k}")
+    dt = dtype_code(query.dtype)
+    if dt == _lib.MJ_DT_FP32:
+        raise TypeError(f"query must be bf16 or fp16, got {query.dtype}")
+    if lse.dtype != torch.float32 or lse.dim() != 2 or lse.shape[1] != h_q or not lse.is_contiguous():
+        raise ValueError(f"lse must be a contiguous fp32 (rows, {h_q}), got {lse.dtype} {tuple(lse.shape)}")
+    if window < 0:
+        raise ValueError(f"window {window}")
+    _on(dev, query, lse, block_table, offsets, seq_lens, weights, status)
+    call(_lib.block_weigh, _lib.BlockWeighArgs(
+        query.data_ptr(), dt, *qs, lse.data_ptr(), min(query.shape[0], lse.shape[0]), n, h_q, h_k, d, page_size, kv_format,
+        k_cache.data_ptr(), *st, k_scales.data_ptr(), *ss, pages, block_table.data_ptr(), block_table.stride(0),
+        block_table.shape[1], offsets.data_ptr(), seq_lens.data_ptr(), weights.data_ptr(), *ws, weights.shape[2],
+        float(softmax_scale), int(window), _ptr(status)), dev)
+    return weights
+
+
+def evict(
+    weights: torch.Tensor,  # (>= n, h_k, tokens) fp32, any sequence and head strides; kept ones move
+    k_cache: torch.Tensor,  # (pages, page_size, h_k, d) byte views, updated in place
+    v_cache: torch.Tensor,
+    k_scales: torch.Tensor,  # (pages, page_size / G, h_k) byte views, updated in place
+    v_scales: torch.Tensor,
+    block_table: torch.Tensor,  # (>= n, blocks) int32
+    seq_lens: torch.Tensor,  # (n,) int32
+    new_lens: torch.Tensor,  # (n,) int32, written; not seq_lens itself
+    kept: torch.Tensor,  # (n, h_k, budget) int32, written: the token that each position received
+    *,
+    recent: int = 0,
+    status: torch.Tensor | None = None,
+) -> None:
+    """Cut every sequence of more than ``budget = kept.shape[2]`` tokens down to
+    it: each KV head keeps the last ``recent`` tokens and the others of the
+    largest ``weights`` (of equal ones the earliest), in their order at
+    positions ``0 .. budget - 1`` of the sequence's own pages, as a write of
+    these rows would leave them, and their weights likewise. The pages behind
+    are free. Shorter sequences are left alone (``kept`` ends in -1). A page
+    that several sequences hold must not be in the call. K keeps the rotation
+    of its old position: new tokens go on counting from the length without
+    evictions."""
+    (pages, page_size, h_k, d), kv_format, dev, st, ss = _cache(k_cache, v_cache, k_scales, v_scales)
+    n = seq_lens.shape[0] if seq_lens.dim() == 1 else -1
+    for name, t in (("seq_lens", seq_lens), ("new_lens", new_lens)):
+        if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 ({n if n >= 0 else 'n'},), got {t.dtype} {tuple(t.shape)}")
+    if kept.dtype != torch.int32 or kept.dim() != 3 or kept.shape[:2] != (n, h_k) or not kept.is_contiguous():
+        raise ValueError(f"kept must be a contiguous int32 ({n}, {h_k}, budget), got {kept.dtype} {tuple(kept.shape)}")
+    budget = kept.shape[2]
+    if not 0 <= recent <= budget:
+        raise ValueError(f"recent {recent} of a budget of {budget}")
+    _table(block_table, n)
+    ws = _weights(weights, n, h_k)
+    _on(dev, weights, block_table, seq_lens, new_lens, kept, status)
+    call(_lib.block_evict, _lib.BlockEvictArgs(
+        k_cache.data_ptr(), v_cache.data_ptr(), *st, k_scales.data_ptr(), v_scales.data_ptr(), *ss, pages, page_size, h_k, d,
+        kv_format, block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), n,
+        weights.data_ptr(), *ws, weights.shape[2], budget, int(recent), new_lens.data_ptr(), kept.data_ptr(), _ptr(status)), dev)
 
 
 @dataclass
