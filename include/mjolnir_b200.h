@@ -471,10 +471,12 @@ typedef struct mj_block_attn_args {
   float softmax_scale;
   int causal;
   /* The plan (mj_block_plan writes it on the host): num_work items of 8 int32
-   * (seq, first row, tile begin, tile end, partial slot or -1, 0, 0, 0). A
+   * (seq, first row, tile begin, tile end, partial slot or -1, span, 0, 0). A
    * row is (query token, head of the KV head's group), token-major; an item
    * covers MJ_BLOCK_ROWS(head_size) rows from its first and the keys of its
-   * tiles of MJ_BLOCK_KEYS. Items with a slot leave normalised
+   * tiles of MJ_BLOCK_KEYS. span = 0: rows of sequence seq. span > 0: rows of
+   * sequences seq .. seq + span - 1 taken together, all of which see every key
+   * of the item's tiles, which are read from the pages of sequence seq. Items with a slot leave normalised
    * partials in o_part / lse_part at [slot][KV head][row]; num_merges entries
    * of 4 int32 (seq, first row, first slot, slots) say which to join. */
   const int32_t* work; int num_work;
@@ -500,6 +502,46 @@ int mj_block_attention(const mj_block_attn_args* args, void* stream);
 int mj_block_plan(const int32_t* query_lens, const int32_t* seq_lens, int num_seqs, int h_q, int h_k, int head_size,
                   int causal, int sm_count, int max_slots, int32_t* work_out, int work_capacity, int32_t* merges_out,
                   int merges_capacity, int* num_work, int* num_merges, int* num_slots);
+
+/* Host plan of a step whose sequences share cached prefixes. A group is
+ * (first sequence, sequences, tokens): the first `tokens` (a multiple of 128)
+ * tokens of its sequences are the same ones, in the same pages, and every query
+ * of theirs sees all of them. Their keys become items of the group's rows
+ * (span > 0), the keys behind them items of each sequence from decode_seqs on;
+ * the sequences before it have theirs from mj_decode, which left
+ * decode_pieces[s] partials (0: its output is final). Groups come in ascending
+ * order and do not overlap. joins_out: joins_capacity x 12 int32 for
+ * mj_block_join, num_rows rows in all. MJ_ERR_UNSUPPORTED when a capacity is
+ * too small. Pure host code, no CUDA call. */
+int mj_block_shared_plan(const int32_t* query_lens, const int32_t* seq_lens, int num_seqs, int decode_seqs,
+                         const int32_t* decode_pieces, const int32_t* groups, int num_groups, int h_q, int h_k,
+                         int head_size, int causal, int sm_count, int max_slots, int32_t* work_out, int work_capacity,
+                         int32_t* joins_out, int joins_capacity, int* num_work, int* num_joins, int* num_rows,
+                         int* num_slots);
+
+/* Joins the partials of a step's rows, weights e^(lse - largest), into O and
+ * LSE. An entry of 12 int32 is (seq, first row, rows, rows of the entries
+ * before it; first own slot, own partials, first shared slot, shared partials;
+ * first row's place among its group's rows, 0, 0, 0). Own partials are slots of
+ * o_part, or with first own slot -1 those that mj_decode left in d_part. A
+ * row's place p among the group's rows is row p % R of shared slots first +
+ * p / R * partials + 0, 1, ..., R = MJ_BLOCK_ROWS. Rows without partials are
+ * left as they were. */
+typedef struct mj_block_join_args {
+  int num_seqs, h_q, h_k, head_size; /* head_size 128 or 256 */
+  int dtype;                         /* MJ_DT_BF16 or MJ_DT_FP16 */
+  void* o; int64_t o_stride_tok, o_stride_head; /* elements */
+  float* lse;                        /* optional (num_tokens, h_q) */
+  int64_t num_tokens;
+  const int32_t* q_start;            /* (num_seqs + 1,) */
+  const int32_t* joins; int num_joins; int num_rows;
+  const float* o_part; const float* lse_part; int num_slots; /* as mj_block_attention leaves them */
+  const float* d_part; const float* d_lse_part;              /* as mj_decode leaves them */
+  int max_splits, part_seqs;
+  int32_t* status;                   /* optional device status word (MJ_DEV_*) */
+} mj_block_join_args;
+
+int mj_block_join(const mj_block_join_args* args, void* stream);
 
 /* ------------------------------------------------------------------------ */
 /* The attention weight that each cached token receives in a step, added up   */

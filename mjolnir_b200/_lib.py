@@ -56,7 +56,7 @@ EXPORTED = ("mj_last_error", "mj_abi_version", "mj_row_bytes", "mj_cache_write",
             "mj_decode_noalloc", "mj_decode_kernel", "mj_expand_pages", "mj_plan_split_kv", "mj_create", "mj_plan",
             "mj_runner_fill", "mj_runner_status", "mj_destroy", "mj_tc_fallbacks", "mj_qk_norm_rope", "mj_block_write",
             "mj_block_read", "mj_block_attention", "mj_block_plan", "mj_qk_norm_rope_axes",
-            "mj_block_weigh", "mj_block_evict")
+            "mj_block_weigh", "mj_block_evict", "mj_block_shared_plan", "mj_block_join")
 
 _i64, _i32, _vp, _f32 = C.c_int64, C.c_int, C.c_void_p, C.c_float
 
@@ -191,6 +191,15 @@ class BlockAttnArgs(C.Structure):
     ]
 
 
+class BlockJoinArgs(C.Structure):
+    _fields_ = [
+        ("num_seqs", _i32), ("h_q", _i32), ("h_k", _i32), ("head_size", _i32), ("dtype", _i32),
+        ("o", _vp), ("o_stride_tok", _i64), ("o_stride_head", _i64), ("lse", _vp), ("num_tokens", _i64), ("q_start", _vp),
+        ("joins", _vp), ("num_joins", _i32), ("num_rows", _i32), ("o_part", _vp), ("lse_part", _vp), ("num_slots", _i32),
+        ("d_part", _vp), ("d_lse_part", _vp), ("max_splits", _i32), ("part_seqs", _i32), ("status", _vp),
+    ]
+
+
 class BlockWeighArgs(C.Structure):
     _fields_ = [
         ("q", _vp), ("dtype", _i32), ("q_stride_tok", _i64), ("q_stride_head", _i64), ("lse", _vp), ("num_rows", _i64),
@@ -253,7 +262,8 @@ def load():
         lib.mj_expand_pages.restype = C.c_int
         for fn, args in (("mj_qk_norm_rope", QkNormRopeArgs), ("mj_block_write", CacheWriteArgs),
                          ("mj_block_read", BlockReadArgs), ("mj_block_attention", BlockAttnArgs),
-                         ("mj_block_weigh", BlockWeighArgs), ("mj_block_evict", BlockEvictArgs)):
+                         ("mj_block_weigh", BlockWeighArgs), ("mj_block_evict", BlockEvictArgs),
+                         ("mj_block_join", BlockJoinArgs)):
             getattr(lib, fn).argtypes = [C.POINTER(args), _vp]
             getattr(lib, fn).restype = C.c_int
         lib.mj_qk_norm_rope_axes.argtypes = [C.POINTER(QkNormRopeArgs), C.POINTER(RopeAxes), _vp]
@@ -264,6 +274,9 @@ def load():
         lib.mj_plan_split_kv.restype = C.c_int
         lib.mj_block_plan.argtypes = [_pi, _pi, *[C.c_int] * 7, _pi, C.c_int, _pi, C.c_int, *[C.POINTER(C.c_int)] * 3]
         lib.mj_block_plan.restype = C.c_int
+        lib.mj_block_shared_plan.argtypes = [_pi, _pi, C.c_int, C.c_int, _pi, _pi, *[C.c_int] * 7, _pi, C.c_int, _pi, C.c_int,
+                                             *[C.POINTER(C.c_int)] * 4]
+        lib.mj_block_shared_plan.restype = C.c_int
         lib.mj_create.argtypes = [C.c_int] * 10
         lib.mj_create.restype = _vp
         lib.mj_plan.argtypes = [_vp, _pi, C.c_int, C.c_int, C.c_int, C.c_int, _vp]
@@ -356,6 +369,25 @@ def block_plan(query_lens, seq_lens, h_q: int, h_k: int, head_size: int, causal:
                                sm_count, max_slots, work.ctypes.data_as(_pi), len(work), merges.ctypes.data_as(_pi),
                                len(merges), *[C.byref(x) for x in n]))
     return n[0].value, n[1].value, n[2].value
+
+
+def block_join(args: BlockJoinArgs, stream: int) -> None:
+    check(load().mj_block_join(C.byref(args), _vp(stream)))
+
+
+def block_shared_plan(query_lens, seq_lens, decode_pieces, groups, h_q: int, h_k: int, head_size: int, causal: bool,
+                      sm_count: int, max_slots: int, work, joins) -> tuple[int, int, int, int]:
+    """mj_block_shared_plan into the int32 arrays ``work`` (n, 8) and ``joins``
+    (m, 12): (work items, joins, joined rows, partial slots)."""
+    import numpy as np
+
+    q, kv, pieces, gr = (np.ascontiguousarray(x, dtype=np.int32) for x in (query_lens, seq_lens, decode_pieces, groups))
+    p = lambda x: x.ctypes.data_as(C.POINTER(C.c_int32))  # noqa: E731
+    n = [C.c_int(0) for _ in range(4)]
+    check(load().mj_block_shared_plan(p(q), p(kv), len(q), len(pieces), p(pieces), p(gr), gr.size // 3, h_q, h_k, head_size,
+                                      int(causal), sm_count, max_slots, p(work), len(work), p(joins), len(joins),
+                                      *[C.byref(x) for x in n]))
+    return n[0].value, n[1].value, n[2].value, n[3].value
 
 
 def plan_split_kv(seq_lens, h_k: int, n_q_tiles: int, sm_count: int, ctas_per_sm: int = 1, max_splits: int = 16,

@@ -194,12 +194,17 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
     if (threadIdx.x == 0) flag(a.status, MJ_DEV_BAD_SPLIT);
     return;
   }
-  const int seq = it0.x, row0 = it0.y, tb = it0.z, slot = item[1].x;
+  const int seq = it0.x, row0 = it0.y, tb = it0.z, slot = item[1].x, span = item[1].y;
+  if (span < 0 || span > a.num_seqs - seq || it0.w > INT_MAX / BN - 2) {
+    if (threadIdx.x == 0) flag(a.status, MJ_DEV_BAD_SPLIT);
+    return;
+  }
   const int h_r = a.h_q / a.h_k;
-  const int q0 = a.q_start[seq], n_tok = a.q_start[seq + 1] - q0, L = a.seq_lens[seq];
+  // rows of several sequences over the prefix that they share: all see all of the item's keys
+  const bool causal = a.causal && !span;
+  const int q0 = a.q_start[seq], n_tok = a.q_start[seq + max(span, 1)] - q0, L = span ? it0.w * BN : a.seq_lens[seq];
   const int n_rows = n_tok * h_r;
-  if (row0 < 0 || row0 >= n_rows || q0 < 0 || n_tok < 0 || q0 + (int64_t)n_tok > a.num_tokens || slot >= a.num_slots ||
-      tb < 0 || it0.w > INT_MAX / BN - 2) {
+  if (row0 < 0 || row0 >= n_rows || q0 < 0 || n_tok < 0 || q0 + (int64_t)n_tok > a.num_tokens || slot >= a.num_slots || tb < 0) {
     if (threadIdx.x == 0) flag(a.status, MJ_DEV_BAD_SPLIT);  // uniform: nothing taken yet
     return;
   }
@@ -266,7 +271,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
   // on NaN codes of V reach the product as zeros (P = 0 times NaN would be NaN
   // in the rows that do not see them), and if there was one, the epilogue makes
   // those elements NaN in the rows that do.
-  const int item_lim = a.causal ? L - n_tok + row0 / h_r : L - 1;
+  const int item_lim = causal ? L - n_tok + row0 / h_r : L - 1;
   const int j_part = max(item_lim + 1 - tb * BN, 0) / BN;
 
   // Page-table walk. An entry is loaded before it is needed and checked then:
@@ -456,7 +461,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
       const int R = row0 + w * 128 + t;
       const bool live = R < n_rows;
       const int tok = min(R, n_rows - 1) / h_r, hq = h * h_r + min(R, n_rows - 1) % h_r;
-      const int lim = !live ? -1 : a.causal ? L - n_tok + tok : L - 1;  // the last key this row sees
+      const int lim = !live ? -1 : causal ? L - n_tok + tok : L - 1;  // the last key this row sees
       // the first row of the warp sees the fewest keys
       const int warp_lim = __shfl_sync(0xffffffffu, lim, 0);
       // ---- Q: the warp's rows in TERMS e4m3 terms into the K-major tiles. D / 8
@@ -716,6 +721,96 @@ __global__ void __launch_bounds__(256) block_merge_kernel(const __grid_constant_
   if (a.lse && lane == 0) a.lse[tok * a.h_q + hq] = l == 0.f ? -INFINITY : mx + logf(l);
 }
 
+// Joins the partials of the rows of a step whose sequences share prefixes: a
+// row's own (of its sequence's keys behind the prefix, from this file's kernel
+// or from the decode kernel) and its group's. A warp per (row, KV head); 32
+// entries at a time are searched for the row's.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) block_join_kernel(const __grid_constant__ mj_block_join_args a) {
+  griddep_wait();
+  constexpr int ROWS = MJ_BLOCK_ROWS(D), E = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int64_t wi = blockIdx.x * (int64_t)8 + (threadIdx.x >> 5);
+  const int h = (int)(wi % a.h_k);
+  const int64_t row = wi / a.h_k;
+  if (row >= a.num_rows) return;  // whole warps
+  const int4* entries = reinterpret_cast<const int4*>(a.joins);
+  int lo = 0, len = a.num_joins;
+  while (len > 1) {  // the last entry that begins at or before this row
+    const int step = (len + 31) / 32, i = lane * step;
+    const uint32_t at = __ballot_sync(0xffffffffu, i < len && entries[3 * (lo + min(i, len - 1))].w <= row);
+    const int k = at ? 31 - __clz(at) : 0;
+    lo += k * step;
+    len = min(step, len - k * step);
+  }
+  const int4 e = entries[3 * lo], parts = entries[3 * lo + 1];
+  const int r = (int)row - e.w, R = e.y + r, place = entries[3 * lo + 2].x + r;
+  const int own = parts.y, shared = parts.w;
+  bool bad = e.x < 0 || e.x >= a.num_seqs || r < 0 || r >= e.z || e.y < 0 || own < 0 || shared < 0 || place < 0;
+  const int h_r = a.h_q / a.h_k;
+  int q0 = 0, n_rows = 0;
+  if (!bad) {
+    q0 = a.q_start[e.x];
+    const int n_tok = a.q_start[e.x + 1] - q0;
+    n_rows = n_tok * h_r;
+    bad = q0 < 0 || n_tok < 0 || q0 + (int64_t)n_tok > a.num_tokens || R >= n_rows || own + shared > 4096;
+    if (parts.x >= 0) bad |= own > a.num_slots - parts.x || r >= ROWS;
+    else bad |= own > a.max_splits || (own && (e.x >= a.part_seqs || !a.d_part));
+    if (shared) bad |= parts.z < 0 || parts.z + (int64_t)(place / ROWS + 1) * shared > a.num_slots;
+  }
+  if (bad) {  // uniform in the warp
+    if (lane == 0) flag(a.status, MJ_DEV_BAD_SPLIT);
+    return;
+  }
+  if (own + shared == 0) return;
+  // partial k: its row index in the buffers of its kind
+  const int64_t own0 = parts.x >= 0 ? ((int64_t)parts.x * a.h_k + h) * ROWS + r : ((int64_t)e.x * a.h_k + h) * n_rows + R;
+  const int64_t own_step = parts.x >= 0 ? (int64_t)a.h_k * ROWS : (int64_t)a.part_seqs * a.h_k * n_rows;
+  const int64_t sh0 = (((int64_t)parts.z + (int64_t)(place / ROWS) * shared) * a.h_k + h) * ROWS + place % ROWS;
+  const float *own_o = parts.x >= 0 ? a.o_part : a.d_part, *own_lse = parts.x >= 0 ? a.lse_part : a.d_lse_part;
+  auto lse_of = [&](int k) { return k < own ? own_lse[own0 + k * own_step] : a.lse_part[sh0 + (int64_t)(k - own) * a.h_k * ROWS]; };
+  float mx = -INFINITY;
+  for (int k = lane; k < own + shared; k += 32) mx = nan_max(mx, lse_of(k));  // a NaN partial makes its row NaN
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = nan_max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  float o[E], l = 0.f;
+#pragma unroll
+  for (int i = 0; i < E; ++i) o[i] = 0.f;
+  if (mx != -INFINITY) {
+    for (int k0 = 0; k0 < own + shared; k0 += 32) {
+      const float wl = k0 + lane < own + shared ? __expf(lse_of(k0 + lane) - mx) : 0.f;
+      const int n = min(32, own + shared - k0);
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const int k = k0 + i;
+        const float w = __shfl_sync(0xffffffffu, wl, i);
+        const float* p = k < own ? own_o + (own0 + k * own_step) * D : a.o_part + (sh0 + (int64_t)(k - own) * a.h_k * ROWS) * D;
+        l += w;
+#pragma unroll
+        for (int c = 0; c < E / 4; ++c) {
+          const float4 v = reinterpret_cast<const float4*>(p)[32 * c + lane];
+          o[4 * c] = fmaf(w, v.x, o[4 * c]);
+          o[4 * c + 1] = fmaf(w, v.y, o[4 * c + 1]);
+          o[4 * c + 2] = fmaf(w, v.z, o[4 * c + 2]);
+          o[4 * c + 3] = fmaf(w, v.w, o[4 * c + 3]);
+        }
+      }
+    }
+  }
+  const int hq = h * h_r + R % h_r;
+  const int64_t tok = q0 + R / h_r;
+  T* out = static_cast<T*>(a.o) + tok * a.o_stride_tok + hq * a.o_stride_head;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int c = 0; c < E / 4; ++c) {
+    alignas(8) T v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (T)(o[4 * c + i] * inv);
+    *reinterpret_cast<uint2*>(out + 128 * c + 4 * lane) = *reinterpret_cast<const uint2*>(v);
+  }
+  if (a.lse && lane == 0) a.lse[tok * a.h_q + hq] = l == 0.f ? -INFINITY : mx + logf(l);
+}
+
 constexpr int kMaxDevices = 64;
 
 // One operand's codes as (128 codes, 128-code halves of a row, page rows, KV
@@ -770,6 +865,17 @@ cudaError_t launch_block_attention(const mj_block_attn_args& a, cudaStream_t str
   if (a.dtype == MJ_DT_FP16)
     return a.head_size == 256 ? ba::launch_t<__half, 256>(a, stream) : ba::launch_t<__half, 128>(a, stream);
   return a.head_size == 256 ? ba::launch_t<__nv_bfloat16, 256>(a, stream) : ba::launch_t<__nv_bfloat16, 128>(a, stream);
+}
+
+template <typename T>
+static cudaError_t join_t(const mj_block_join_args& a, cudaStream_t stream) {
+  const int64_t warps = (int64_t)a.num_rows * a.h_k;
+  auto kern = a.head_size == 256 ? ba::block_join_kernel<T, 256> : ba::block_join_kernel<T, 128>;
+  return launch_kernel(kern, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, stream, a);
+}
+
+cudaError_t launch_block_join(const mj_block_join_args& a, cudaStream_t stream) {
+  return a.dtype == MJ_DT_FP16 ? join_t<__half>(a, stream) : join_t<__nv_bfloat16>(a, stream);
 }
 
 }  // namespace mj

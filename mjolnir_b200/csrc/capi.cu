@@ -19,6 +19,7 @@ cudaError_t launch_qk_norm_rope(const mj_qk_norm_rope_args& a, const mj_rope_axe
 cudaError_t launch_block_write(const mj_cache_write_args& a, cudaStream_t stream);
 cudaError_t launch_block_read(const mj_block_read_args& a, cudaStream_t stream);
 cudaError_t launch_block_attention(const mj_block_attn_args& a, cudaStream_t stream);
+cudaError_t launch_block_join(const mj_block_join_args& a, cudaStream_t stream);
 cudaError_t launch_block_weigh(const mj_block_weigh_args& a, cudaStream_t stream);
 cudaError_t launch_block_evict(const mj_block_evict_args& a, cudaStream_t stream);
 }  // namespace mj
@@ -407,6 +408,29 @@ int mj_block_attention(const mj_block_attn_args* args, void* stream) {
   if ((int64_t)a.num_work * a.h_k > (int64_t)INT32_MAX) return fail(MJ_ERR_UNSUPPORTED, "mj_block_attention: too many work items");
   if (shared_bytes(st, a.num_pages, a.page_size, a.h_k)) return fail(MJ_ERR_UNSUPPORTED, "mj_block_attention: a cache stride of 0");
   return cuda_status(mj::launch_block_attention(a, (cudaStream_t)stream), "mj_block_attention launch");
+}
+
+int mj_block_join(const mj_block_join_args* args, void* stream) {
+  if (!args) return fail(MJ_ERR_INVALID, "mj_block_join: null args");
+  const mj_block_join_args& a = *args;
+  if (a.num_seqs < 0 || a.num_tokens < 0 || a.h_k <= 0 || a.h_q <= 0 || a.h_q % a.h_k || a.num_joins < 0 || a.num_rows < 0 ||
+      a.num_slots < 0 || a.max_splits < 0 || a.part_seqs < 0)
+    return fail(MJ_ERR_INVALID, "mj_block_join: num_seqs %d num_tokens %lld h_q %d h_k %d num_joins %d num_rows %d", a.num_seqs,
+                (long long)a.num_tokens, a.h_q, a.h_k, a.num_joins, a.num_rows);
+  if (a.head_size != 128 && a.head_size != 256) return fail(MJ_ERR_UNSUPPORTED, "mj_block_join: head_size %d (128 or 256)", a.head_size);
+  if (a.dtype != MJ_DT_BF16 && a.dtype != MJ_DT_FP16)
+    return fail(MJ_ERR_UNSUPPORTED, "mj_block_join: dtype %d (bf16 or fp16)", a.dtype);
+  if (a.num_seqs == 0 || a.num_tokens == 0 || a.num_joins == 0 || a.num_rows == 0) {
+    g_err[0] = 0;
+    return MJ_OK;
+  }
+  if (!a.o || !a.q_start || !a.joins || !aligned(a.joins, 16) || (a.num_slots && (!a.o_part || !a.lse_part || !aligned(a.o_part, 16))) ||
+      (a.d_part && (!a.d_lse_part || !aligned(a.d_part, 16))))
+    return fail(MJ_ERR_INVALID, "mj_block_join: plan or partial buffers");
+  if (!aligned(a.o, 16) || a.o_stride_tok % 8 || a.o_stride_head % 8)
+    return fail(MJ_ERR_UNSUPPORTED, "mj_block_join: o rows must be 16-byte aligned");
+  if ((int64_t)a.num_rows * a.h_k > (int64_t)INT32_MAX) return fail(MJ_ERR_UNSUPPORTED, "mj_block_join: too many rows");
+  return cuda_status(mj::launch_block_join(a, (cudaStream_t)stream), "mj_block_join launch");
 }
 
 int mj_block_weigh(const mj_block_weigh_args* args, void* stream) {

@@ -204,6 +204,130 @@ int mj_block_plan(const int32_t* query_lens, const int32_t* seq_lens, int num_se
   return MJ_OK;
 }
 
+int mj_block_shared_plan(const int32_t* query_lens, const int32_t* seq_lens, int num_seqs, int decode_seqs,
+                         const int32_t* decode_pieces, const int32_t* groups, int num_groups, int h_q, int h_k,
+                         int head_size, int causal, int sm_count, int max_slots, int32_t* work_out, int work_capacity,
+                         int32_t* joins_out, int joins_capacity, int* num_work, int* num_joins, int* num_rows,
+                         int* num_slots) {
+  if (num_seqs < 0 || decode_seqs < 0 || decode_seqs > num_seqs || num_groups < 0 || h_k <= 0 || h_q <= 0 || h_q % h_k ||
+      (head_size != 128 && head_size != 256) || sm_count <= 0 || max_slots < 0 || (num_seqs && (!query_lens || !seq_lens)) ||
+      (decode_seqs && !decode_pieces) || (num_groups && !groups) || work_capacity < 0 || joins_capacity < 0 ||
+      (work_capacity && !work_out) || (joins_capacity && !joins_out) || !num_work || !num_joins || !num_rows || !num_slots)
+    return mj::set_last_error(MJ_ERR_INVALID, "mj_block_shared_plan: invalid argument");
+  constexpr int kMinPiece = 8;
+  const int h_r = h_q / h_k, rows = MJ_BLOCK_ROWS(head_size), keys = MJ_BLOCK_KEYS;
+  struct Block {  // of a sequence's rows, or of a group's
+    int32_t seq, row0, t0, t1, span;
+    bool slotted;  // leaves partials even in one piece
+    int32_t group, pieces, slot;
+  };
+  try {
+    for (int s = 0; s < num_seqs; ++s)
+      if (query_lens[s] < 0 || seq_lens[s] < 0 || (int64_t)query_lens[s] * h_r > INT32_MAX)
+        return mj::set_last_error(MJ_ERR_INVALID, "mj_block_shared_plan: a length");
+    for (int s = 0; s < decode_seqs; ++s)
+      if (decode_pieces[s] < 0) return mj::set_last_error(MJ_ERR_INVALID, "mj_block_shared_plan: decode_pieces");
+    std::vector<int32_t> group_of(num_seqs, -1);
+    std::vector<int64_t> group_rows(num_groups, 0), place(num_seqs, 0);
+    std::vector<Block> blocks;
+    for (int g = 0, end = 0; g < num_groups; ++g) {
+      const int32_t first = groups[3 * g], count = groups[3 * g + 1], tokens = groups[3 * g + 2];
+      if (first < end || count < 1 || count > num_seqs - first || tokens <= 0 || tokens % 128)
+        return mj::set_last_error(MJ_ERR_INVALID, "mj_block_shared_plan: a group");
+      end = first + count;
+      for (int s = first; s < end; ++s) {
+        if (query_lens[s] && (causal ? (int64_t)seq_lens[s] - query_lens[s] : seq_lens[s]) < tokens)
+          return mj::set_last_error(MJ_ERR_INVALID, "mj_block_shared_plan: a query before the end of its group's tokens");
+        group_of[s] = g;
+        place[s] = group_rows[g];
+        group_rows[g] += (int64_t)query_lens[s] * h_r;
+      }
+      if (group_rows[g] > INT32_MAX) return mj::set_last_error(MJ_ERR_INVALID, "mj_block_shared_plan: a length");
+      for (int64_t r = 0; r < group_rows[g]; r += rows)
+        blocks.push_back({first, (int32_t)r, 0, tokens / keys, count, true, g, 1, -1});
+    }
+    const size_t of_groups = blocks.size();
+    for (int s = decode_seqs; s < num_seqs; ++s) {
+      const int64_t n = query_lens[s], L = seq_lens[s], all = n * h_r;
+      const int t0 = group_of[s] < 0 ? 0 : groups[3 * group_of[s] + 2] / keys;
+      for (int64_t r = 0; r < all; r += rows) {
+        const int64_t last = causal ? L - n + (std::min(r + rows, all) - 1) / h_r : L - 1;  // last key seen
+        const int t1 = last < 0 ? 0 : (int32_t)(last / keys + 1);
+        blocks.push_back({s, (int32_t)r, t0, std::max(t0, t1), 0, group_of[s] >= 0, -1, 1, -1});
+      }
+    }
+    // an equal share of the step's key tiles per SM; larger where that needs more slots than there are
+    int64_t total = 0;
+    for (const Block& b : blocks) total += b.t1 - b.t0;
+    int64_t bound = std::max<int64_t>(kMinPiece, ceil_div(total * h_k, sm_count)), slots = 0;
+    for (;; bound *= 2) {
+      slots = 0;
+      bool whole = true;
+      for (Block& b : blocks) {
+        b.pieces = b.t1 - b.t0 > bound ? (int32_t)ceil_div(b.t1 - b.t0, bound) : 1;
+        whole = whole && b.pieces == 1;
+        slots += b.pieces > 1 || b.slotted ? b.pieces : 0;
+      }
+      if (slots <= max_slots) break;
+      if (whole) return mj::set_last_error(MJ_ERR_UNSUPPORTED, "mj_block_shared_plan: more partials than max_slots");
+    }
+    int64_t nw = 0, ns = 0;
+    for (Block& b : blocks) {
+      nw += b.pieces;
+      if (b.pieces > 1 || b.slotted) {
+        b.slot = (int32_t)ns;
+        ns += b.pieces;
+      }
+    }
+    if (nw > work_capacity) return mj::set_last_error(MJ_ERR_UNSUPPORTED, "mj_block_shared_plan: more items than the capacity");
+    // joins: every sequence with rows, by its own blocks
+    std::vector<int32_t> shared_first(num_groups, -1), shared_pieces(num_groups, 0);
+    for (size_t i = of_groups; i-- > 0;) {
+      shared_first[blocks[i].group] = blocks[i].slot;
+      shared_pieces[blocks[i].group] = blocks[i].pieces;
+    }
+    int64_t nj = 0, nr = 0;
+    bool room = true;
+    auto join = [&](int s, int64_t row0, int64_t count, int first, int pieces) {
+      if (nj >= joins_capacity) {
+        room = false;
+        return;
+      }
+      const int g = group_of[s];
+      const int32_t e[12] = {s, (int32_t)row0, (int32_t)count, (int32_t)nr, first, pieces, g < 0 ? -1 : shared_first[g],
+                             g < 0 ? 0 : shared_pieces[g], g < 0 ? 0 : (int32_t)(place[s] + row0), 0, 0, 0};
+      std::copy(e, e + 12, joins_out + 12 * nj++);
+      nr += count;
+    };
+    for (int s = 0; s < decode_seqs; ++s)
+      if (query_lens[s]) join(s, 0, (int64_t)query_lens[s] * h_r, -1, decode_pieces[s]);
+    for (size_t i = of_groups; i < blocks.size(); ++i) {
+      const Block& b = blocks[i];
+      if (b.slot >= 0) join(b.seq, b.row0, std::min<int64_t>(rows, (int64_t)query_lens[b.seq] * h_r - b.row0), b.slot, b.pieces);
+    }
+    if (!room) return mj::set_last_error(MJ_ERR_UNSUPPORTED, "mj_block_shared_plan: more joins than the capacity");
+    if (nr > INT32_MAX) return mj::set_last_error(MJ_ERR_INVALID, "mj_block_shared_plan: a length");
+    std::stable_sort(blocks.begin(), blocks.end(), [](const Block& x, const Block& y) {
+      return (int64_t)(x.t1 - x.t0) * y.pieces > (int64_t)(y.t1 - y.t0) * x.pieces;
+    });
+    int64_t at = 0;
+    for (const Block& b : blocks)
+      for (int i = 0; i < b.pieces; ++i) {  // pieces of equal length, to a tile
+        const int64_t t = b.t1 - b.t0;
+        const int32_t w[8] = {b.seq, b.row0, (int32_t)(b.t0 + t * i / b.pieces), (int32_t)(b.t0 + t * (i + 1) / b.pieces),
+                              b.slot < 0 ? -1 : b.slot + i, b.span, 0, 0};
+        std::copy(w, w + 8, work_out + 8 * at++);
+      }
+    *num_work = (int)nw;
+    *num_joins = (int)nj;
+    *num_rows = (int)nr;
+    *num_slots = (int)ns;
+  } catch (const std::exception&) {
+    return mj::set_last_error(MJ_ERR_INVALID, "mj_block_shared_plan: out of memory");
+  }
+  return MJ_OK;
+}
+
 // ---- runner handle --------------------------------------------------------
 
 // the tensor-core kernel's rows per job (48; 16 at head_size 256) and CTAs

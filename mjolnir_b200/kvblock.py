@@ -27,9 +27,11 @@ import numpy as np
 import torch
 
 from . import _lib
+from .plan import TILE_ROWS
 from .runner import DecodeRunner, StepPlan, _ptr, call, dtype_code
 
 HEAD_SIZES = (128, 256)
+SHARED_BLOCKS = 64  # row blocks of sequences behind a shared prefix that a step has room for
 BLOCK_TOKENS = tuple(_lib.BLOCK_FORMATS)
 
 
@@ -290,6 +292,8 @@ class BlockPlan:
     num_slots: int
     causal: bool = True
     decode: StepPlan | None = None  # the leading sequences that the decode kernel serves
+    joins: torch.Tensor | None = None  # (entries, 12) int32, device: rows whose sequences share a prefix
+    num_rows: int = 0  # rows that the entries join
 
 
 class BlockAttention:
@@ -336,13 +340,21 @@ class BlockAttention:
         # the plan: q_start | merges | work, one fixed-address buffer and one copy a step
         self._at = (-(-(max_num_seqs + 1) // 4) * 4, -(-(max_num_seqs + 1) // 4) * 4 + 4 * self.max_slots)
         self.plan_buf = torch.zeros(self._at[1] + 8 * self.max_work, dtype=torch.int32, device=self.device)
+        # steps with shared prefixes: q_start | joins | work in a buffer of their own, made
+        # with the partials by the first such plan. Every row of a group has a partial over
+        # the prefix, and behind a chunk kernel's one of its own: room for this many row
+        # blocks, beside the partials that splitting asks for
+        self.max_shared_slots = self.max_slots + 2 * min(max_num_seqs, SHARED_BLOCKS)
+        self.max_items = self.max_work + self.max_shared_slots - self.max_slots
+        self._shared_at = (self._at[0], self._at[0] + 12 * (max_num_seqs + self.max_work))
+        self.shared_buf = self.shared_o_part = self.shared_lse_part = None
         self.o_part = torch.empty(self.max_slots * num_kv_heads * self.rows * head_size, dtype=torch.float32, device=self.device)
         self.lse_part = torch.empty(self.max_slots * num_kv_heads * self.rows, dtype=torch.float32, device=self.device)
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self.one = torch.ones(1, dtype=torch.float32, device=self.device)
 
     def plan(self, query_lens, seq_lens_cpu, block_table: torch.Tensor, seq_lens: torch.Tensor,
-             causal: bool = True, fixed_grid: bool = False) -> BlockPlan:
+             causal: bool = True, fixed_grid: bool = False, shared=()) -> BlockPlan:
         """Plan a step: ``query_lens[s]`` new tokens of each sequence, which
         are the last of its ``seq_lens[s]`` tokens. The device ``seq_lens``
         (int32) are what the kernels mask with.
@@ -351,7 +363,15 @@ class BlockAttention:
         it replays that plan only. With ``fixed_grid`` the launches do not
         depend on the lengths, so the graph replays any later plan with
         ``fixed_grid`` of as many sequences and the same query length; only
-        steps that the decode kernel serves whole have that form."""
+        steps that the decode kernel serves whole have that form.
+
+        ``shared`` names prefixes that sequences have in common, as ``(first
+        sequence, number of sequences, tokens)``: the first ``tokens`` tokens of
+        these neighbouring sequences are the same ones, in the same pages of
+        ``block_table`` (the first of them is read for all). Their keys are then
+        read once for the whole group. The result is the same as without, but
+        for the order of its sums. A graph with ``fixed_grid`` replays later
+        plans that share alike."""
         q = [int(x) for x in query_lens]
         if len(q) > self.max_num_seqs or sum(q) > self.max_num_tokens:
             raise ValueError(f"{len(q)} sequences / {sum(q)} tokens beyond the runner's capacity")
@@ -368,10 +388,18 @@ class BlockAttention:
         decode, few = None, 0
         if q and 1 <= q[0] <= self.max_q_len:
             few = next((i for i, x in enumerate(q) if x != q[0]), len(q))
+        groups = self._groups(shared, q, kv, few, causal)
+        starts = [0] * len(q)
+        for first, count, tokens in groups:
+            starts[first:first + count] = [tokens if n else 0 for n in q[first:first + count]]
+        if few:
             if not fixed_grid or few == len(q):
-                decode = self.decode.plan(kv, few, q[0], block_table, seq_lens, causal=causal, fixed_grid=fixed_grid)
+                decode = self.decode.plan(kv, few, q[0], block_table, seq_lens, causal=causal, fixed_grid=fixed_grid,
+                                          starts=starts[:few] if groups else None)
         if fixed_grid and (few < len(q) or not q):
             raise ValueError(f"fixed_grid: a step of one query length of 1 to {self.max_q_len} tokens, got {q[:8]}")
+        if groups:
+            return self._plan_shared(q, kv, groups, starts, few, decode, block_table, seq_lens, causal)
         if few == len(q):
             return BlockPlan(q, sum(q), block_table, seq_lens, None, None, None, 0, causal, decode)
         n, (m0, w0) = len(q), self._at
@@ -385,6 +413,49 @@ class BlockAttention:
         self.plan_buf[:used].copy_(stage[:used], non_blocking=True)
         return BlockPlan(q, sum(q), block_table, seq_lens, self.plan_buf[:n + 1], self.plan_buf[w0:used].view(-1, 8),
                          self.plan_buf[m0:m0 + 4 * nm].view(-1, 4), slots, causal, decode)
+
+    def _groups(self, shared, q: list[int], kv: list[int], few: int, causal: bool) -> list[tuple[int, int, int]]:
+        """The groups worth a shared read, with the tokens that every query of
+        theirs sees, in whole tiles of the decode kernel."""
+        groups, end = [], 0
+        for first, count, tokens in sorted((int(a), int(b), int(c)) for a, b, c in shared):
+            if first < end or count < 1 or first + count > len(q) or tokens < 0:
+                raise ValueError(f"shared: ({first}, {count}, {tokens}) is not (first sequence, sequences, tokens) of {len(q)} sequences "
+                                 "apart from the other groups")
+            end = first + count
+            seen = [kv[s] - (q[s] if causal else 0) for s in range(first, end) if q[s]]
+            tokens = min([tokens, kv[first], *seen]) // TILE_ROWS * TILE_ROWS
+            if len(seen) > 1 and tokens > 0:
+                groups.append((first, count, tokens))
+        # every row block of a group, and of its sequences on the chunk kernel, takes a slot
+        room, h_r, kept = self.max_shared_slots, self.h_q // self.h_k, []
+        for first, count, tokens in groups:
+            rows = [n * h_r for n in q[first:first + count]]
+            room -= -(-sum(rows) // self.rows) + sum(-(-n // self.rows) for n in rows[max(few - first, 0):])
+            if room < 0:
+                break
+            kept.append((first, count, tokens))
+        return kept
+
+    def _plan_shared(self, q, kv, groups, starts, few, decode, block_table, seq_lens, causal) -> BlockPlan:
+        n, (j0, w0) = len(q), self._shared_at
+        if self.shared_buf is None:
+            part = self.max_shared_slots * self.h_k * self.rows
+            self.shared_buf = torch.zeros(w0 + 8 * self.max_items, dtype=torch.int32, device=self.device)
+            self.shared_o_part = torch.empty(part * self.d, dtype=torch.float32, device=self.device)
+            self.shared_lse_part = torch.empty(part, dtype=torch.float32, device=self.device)
+        stage = torch.empty(self.shared_buf.shape[0], dtype=torch.int32, pin_memory=True)
+        host = stage.numpy()
+        host[0] = 0
+        np.cumsum(q, out=host[1:n + 1])
+        work, joins = host[w0:].reshape(-1, 8), host[j0:w0].reshape(-1, 12)
+        pieces = [p if p > 1 or starts[s] else 0 for s, p in enumerate(decode.pieces)] if few else []
+        nw, nj, rows, slots = _lib.block_shared_plan(q, kv, pieces, groups, self.h_q, self.h_k, self.d, causal, self.sm_count,
+                                                     self.max_shared_slots, work, joins)
+        used = w0 + 8 * nw
+        self.shared_buf[:used].copy_(stage[:used], non_blocking=True)
+        return BlockPlan(q, sum(q), block_table, seq_lens, self.shared_buf[:n + 1], self.shared_buf[w0:used].view(-1, 8),
+                         self.shared_buf[:0].view(-1, 4), slots, causal, decode, self.shared_buf[j0:j0 + 12 * nj].view(-1, 12), rows)
 
     def run(
         self,
@@ -421,15 +492,25 @@ class BlockAttention:
                 p.num_seqs, p.q_len, self.h_q, h_k, d, page_size, kv_format, query.data_ptr(), dt, *qs, out.data_ptr(), dt,
                 *os_, *cache, pages, bt.data_ptr(), bt.stride(0), plan.seq_lens.data_ptr(), p.work.data_ptr(), p.num_work,
                 p.n_splits.data_ptr(), r.max_splits, r.o_part.data_ptr(), r.lse_part.data_ptr(), self.max_num_seqs, _ptr(lse),
-                one, _lib.MJ_SCALE_TENSOR, one, _lib.MJ_SCALE_TENSOR, None, None, scale, causal, int(p.with_reduction),
+                one, _lib.MJ_SCALE_TENSOR, one, _lib.MJ_SCALE_TENSOR, None, None, scale, causal,
+                int(p.with_reduction and plan.joins is None),
                 r.kernel, r.status.data_ptr(), r.merge_counters.data_ptr() if r.merges(p) else None, *scales, *ss, 0), dev)
+        part = (self.o_part, self.lse_part) if plan.joins is None else (self.shared_o_part, self.shared_lse_part)
+        part = (part[0].data_ptr(), part[1].data_ptr())
         if plan.work is not None:
             call(_lib.block_attention, _lib.BlockAttnArgs(
                 len(plan.query_lens), self.h_q, h_k, d, page_size, kv_format, dt, query.data_ptr(), *qs, out.data_ptr(), *os_,
                 tokens, *cache, *scales, *ss, pages, bt.data_ptr(), bt.stride(0), bt.shape[1], plan.seq_lens.data_ptr(),
                 plan.q_start.data_ptr(), _ptr(lse), scale, causal, plan.work.data_ptr(), plan.work.shape[0],
-                plan.merges.data_ptr(), plan.merges.shape[0], self.o_part.data_ptr(), self.lse_part.data_ptr(),
+                plan.merges.data_ptr(), plan.merges.shape[0], *part,
                 plan.num_slots, self.status.data_ptr()), dev)
+        if plan.joins is not None:
+            r = self.decode
+            d_part = (r.o_part.data_ptr(), r.lse_part.data_ptr(), r.max_splits) if plan.decode is not None else (None, None, 0)
+            call(_lib.block_join, _lib.BlockJoinArgs(
+                len(plan.query_lens), self.h_q, h_k, d, dt, out.data_ptr(), *os_, _ptr(lse), tokens, plan.q_start.data_ptr(),
+                plan.joins.data_ptr(), plan.joins.shape[0], plan.num_rows, *part,
+                plan.num_slots, *d_part, self.max_num_seqs, self.status.data_ptr()), dev)
         return out
 
     def check_status(self) -> None:

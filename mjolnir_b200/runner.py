@@ -58,6 +58,7 @@ class StepPlan:
     num_chunks: int
     causal: bool = True
     tile_jobs: int = 0  # 128-row KV tiles x KV heads the step reads
+    pieces: list[int] | None = None  # partials that each sequence's items leave
 
 
 # ---------------------------------------------------------------------------
@@ -362,18 +363,24 @@ class DecodeRunner:
         margin: int = 0,
         causal: bool = True,
         fixed_grid: bool = False,
+        starts=None,
     ) -> StepPlan:
         """CPU plan + async copy into the persistent device buffers. ``margin``
         plans every sequence that many tokens longer (the kernel masks with the
         device ``seq_lens``, so the plan stays valid while they grow).
         ``fixed_grid`` launches the padded capacity (empty items exit at once)
         so a captured CUDA graph replays any later plan; otherwise the grid is
-        the plan's real item count."""
+        the plan's real item count. ``starts`` (multiples of 128, at most the
+        lengths) leaves the first tokens of sequences out: those with a start
+        leave partials even in one piece, for the caller to join with theirs."""
         if not (1 <= q_len <= self.max_q_len and num_seqs <= self.max_num_seqs):
             raise ValueError(f"q_len {q_len} / num_seqs {num_seqs} beyond the runner's capacity")
         lens = [int(x) + margin for x in list(seq_lens_cpu)[:num_seqs]]
+        starts = [0] * num_seqs if starts is None else [int(x) for x in starts]
+        if any(x % TILE_ROWS or not 0 <= x <= max(0, n) for x, n in zip(starts, lens)) or len(starts) != num_seqs:
+            raise ValueError(f"starts must be multiples of {TILE_ROWS} up to the lengths, got {starts[:8]}")
         p = plan_split_kv(
-            lens,
+            [n - x for n, x in zip(lens, starts)],
             self.h_k,
             self.n_tiles(q_len),
             self.sm_count,
@@ -382,8 +389,16 @@ class DecodeRunner:
             pad_to=self._cap,
             rebalance=self.rebalance,
         )
-        work_h = torch.from_numpy(p.work_array()).pin_memory() if self.device.type == "cuda" else torch.from_numpy(p.work_array())
-        ns_h = torch.tensor(p.n_splits, dtype=torch.int32)
+        work_h, pieces = torch.from_numpy(p.work_array()), p.n_splits
+        if any(starts):
+            if self.max_splits < 2:
+                raise ValueError("starts need a runner of at least two splits")
+            at = torch.tensor([x // TILE_ROWS for x in starts], dtype=torch.int32)[work_h[:, 0].long()]
+            work_h[:, 1:3] += torch.where(work_h[:, 2] > work_h[:, 1], at, 0)[:, None]
+            pieces = [max(n, 2) if x else n for n, x in zip(pieces, starts)]
+        if self.device.type == "cuda":
+            work_h = work_h.pin_memory()
+        ns_h = torch.tensor(pieces, dtype=torch.int32)
         if self.device.type == "cuda":
             ns_h = ns_h.pin_memory()
         self.work_buf.copy_(work_h, non_blocking=True)
@@ -404,7 +419,8 @@ class DecodeRunner:
             chunk_tiles=p.chunk_tiles,
             num_chunks=real,
             causal=causal or q_len == 1,
-            tile_jobs=sum(-(-L // 128) for L in lens) * self.h_k,
+            tile_jobs=sum(-(-(n - x) // 128) for n, x in zip(lens, starts)) * self.h_k,
+            pieces=p.n_splits,
         )
 
     # ---------------------------------------------------------------- launch
