@@ -1,63 +1,548 @@
 // The attention weight that each cached token receives in a step, added up per
-// KV head: w[s][h][j] += sum over the rows (query, head of the group) that see
-// key j of exp(scale q . k_j - lse).
+// KV head, on the 5th-generation tensor cores (sm_100a):
+// w[s][h][j] += sum over the rows (query, head of the group) that see key j of
+// exp(scale q . k_j - lse).
+//
+// The scores are computed with the keys in the rows of the product, S^T = K Q^T:
+// a lane of TMEM is a key, so a thread adds up its own key's weights in
+// registers, no two threads meet, and the order of every sum is fixed. A job is
+// (sequence, KV head, tile of 128 keys): its K tile stays, the query rows that
+// see it stream past in tiles of N.
+//
+// Both operands are 16 bits wide. Q enters as it is, by TMA; K's e4m3 codes are
+// exact in either type, so the products are exact, and the block scales, one a
+// key, go into the exponent with the softmax scale. (fp8 products would need Q
+// in three e4m3 terms to leave an fp32 sum its precision.)
+//
+// Jobs need no plan: one warp of each CTA walks the sequences' lengths on the
+// device, so a captured graph replays for whatever they hold. Persistent CTAs
+// take the jobs in rounds, every other round in reverse: a prompt's first keys
+// are seen by all its rows, its last by few.
+//
+// Warp roles: 0 K (page walk, TMA, block scales), 1 Q (TMA) and its lse, 2 MMA,
+// 3 the jobs; 4-7 convert K's codes; 8-15 two warpgroups that take the S tiles
+// in turn and add up. Every mbarrier wait is bounded; on a timeout the CTA flags
+// MJ_DEV_TIMEOUT, all roles stop, copies and MMAs in flight complete and TMEM is
+// freed.
+#include <limits.h>
 #include <math.h>
+
+#include <atomic>
+#include <mutex>
+#include <type_traits>
+
+#include <cuda.h>
 
 #include "block_cache.cuh"
 
 namespace mj {
 
-// One warp per key: the row of K in registers, then every query row that sees it.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) block_weigh_kernel(const __grid_constant__ mj_block_weigh_args a, int lg, int blocks) {
-  griddep_wait();
-  constexpr int E = D / 32;  // elements of a lane
-  const int lane = threadIdx.x & 31;
-  const int x = blockIdx.x % blocks, sh = blockIdx.x / blocks, h = sh % a.h_k, seq = sh / a.h_k;
-  const int q0 = a.offsets[seq], q1 = a.offsets[seq + 1], L = a.seq_lens[seq], n = q1 - q0;
-  if (q0 < 0 || n < 0 || q1 > a.num_rows || L < 0 || L > a.weights_cols || L > (int64_t)a.block_table_cols * a.page_size) {
-    if (threadIdx.x == 0) flag(a.status, MJ_DEV_BAD_LENGTH);
+std::mutex& tc_init_mutex();
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn tensor_map_encoder();
+
+namespace bw {
+
+using namespace sm100;
+
+constexpr uint64_t kWaitNs = 500000000ull;  // per wait; a tile takes microseconds
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int KEYS = 128, JOBS = 8, THREADS = 512;
+
+// What a role needs to know of a job. The K warp adds the scales.
+struct Job {
+  int seq, h, kt, L, n, q0, t0, tiles;  // seq < 0: no more; t0: the first query that counts and sees a key
+  float scale[KEYS / 16];
+};
+
+template <typename T, int D, int N>
+struct Cfg {
+  static constexpr int RAW = KEYS * D, K16 = 2 * RAW, QST = N * D * 2;  // a tile's codes; as 16 bits; a tile of Q rows
+  static constexpr bool WIDE = N >= 64;
+  // stages of K codes, of K in 16 bits, of Q
+  static constexpr int RS = WIDE ? 2 : D == 256 ? 4 : 6, KS = D == 256 ? 1 : 2, QS = WIDE ? 3 : 4;
+  static constexpr int SB = 4;  // S buffers in TMEM, each with its columns' lse
+  static constexpr int K_OFF = 0, R_OFF = K_OFF + KS * K16, Q_OFF = R_OFF + RS * RAW, Z_OFF = Q_OFF + QS * QST;
+  static constexpr int RED_OFF = Z_OFF + SB * N * 4, JOB_OFF = RED_OFF + KEYS * 4, BAR_OFF = JOB_OFF + JOBS * (int)sizeof(Job);
+  static constexpr int NBARS = 2 * (RS + KS + QS + SB + JOBS + 1) + 1;
+  static constexpr int MISC_OFF = BAR_OFF + NBARS * 8;
+  static constexpr int SMEM = MISC_OFF + 16;
+  static_assert(SMEM <= 232448, "shared memory of a CTA");
+  static_assert(JOBS >= 3, "the K warp looks two jobs ahead");
+};
+
+// 16 codes -> 16 values of T (exact)
+template <typename T>
+__device__ __forceinline__ void widen16(uint4 c, uint32_t* o) {
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (std::is_same<T, __half>::value) {
+      o[2 * k] = e4m3x2_to_h2((uint16_t)w[k]);
+      o[2 * k + 1] = e4m3x2_to_h2((uint16_t)(w[k] >> 16));
+    } else {
+      const float2 a = e4m3x2_to_f2((uint16_t)w[k]), b = e4m3x2_to_f2((uint16_t)(w[k] >> 16));
+      const __nv_bfloat162 x = __floats2bfloat162_rn(a.x, a.y), y = __floats2bfloat162_rn(b.x, b.y);
+      o[2 * k] = *reinterpret_cast<const uint32_t*>(&x);
+      o[2 * k + 1] = *reinterpret_cast<const uint32_t*>(&y);
+    }
+  }
+}
+
+// byte offset of 16-byte unit u of row r in a [rows][128 bytes] swizzled block
+__device__ __forceinline__ uint32_t unit_offset(uint32_t r, uint32_t u) { return r * 128 + ((u ^ (r & 7)) << 4); }
+
+template <typename T, int D, int N>
+__global__ void __launch_bounds__(THREADS, 1)
+    block_weigh_kernel(const __grid_constant__ mj_block_weigh_args a, int lg, int hb, int tb, int ht,
+                       const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmq) {
+  using C = Cfg<T, D, N>;
+  constexpr int RS = C::RS, KS = C::KS, QS = C::QS, SB = C::SB;
+  extern __shared__ __align__(1024) unsigned char sm[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::BAR_OFF);
+  uint64_t *r_full = bars, *r_empty = r_full + RS, *k_full = r_empty + RS, *k_empty = k_full + KS, *q_full = k_empty + KS,
+           *q_empty = q_full + QS, *s_full = q_empty + QS, *s_empty = s_full + SB, *j_full = s_empty + SB, *j_empty = j_full + JOBS,
+           *red_full = j_empty + JOBS, *red_empty = red_full + 1, *drain = red_empty + 1;
+  Job* jobs = reinterpret_cast<Job*>(sm + C::JOB_OFF);
+  float* red = reinterpret_cast<float*>(sm + C::RED_OFF);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::MISC_OFF);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + C::MISC_OFF + 4);
+  int& never_abort = *reinterpret_cast<int*>(sm + C::MISC_OFF + 8);
+  if (reinterpret_cast<uintptr_t>(sm) & 1023) {  // uniform: nothing taken yet
+    if (threadIdx.x == 0) flag(a.status, MJ_DEV_BAD_SPLIT);
     return;
   }
-  const int h_r = a.h_q / a.h_k, first = a.window ? max(n - a.window, 0) : 0;
-  float* w = a.weights + seq * a.w_stride_seq + h * a.w_stride_head;
-  for (int j = x * 8 + (threadIdx.x >> 5); j < L; j += blocks * 8) {
-    const int page = a.block_table[seq * a.block_table_stride + j / a.page_size], r = j % a.page_size;
-    if (page < 0 || page >= a.num_pages) {
-      if (lane == 0) flag(a.status, MJ_DEV_BAD_PAGE);
-      continue;
-    }
-    const unsigned char* row = static_cast<const unsigned char*>(a.k_cache) + page * a.k_stride_page + r * a.k_stride_row + h * a.k_stride_head;
-    const float f = block_scale(static_cast<const unsigned char*>(a.k_scales)[page * a.ks_stride_page + (r >> lg) * a.ks_stride_block + h * a.ks_stride_head]);
-    float k[E];
-#pragma unroll
-    for (int i = 0; i < E; ++i) k[i] = e4m3_value(row[lane * E + i]) * f;
-    float sum = 0.f;
-    for (int t = max(first, j - (L - n)); t < n; ++t)
-      for (int g = 0; g < h_r; ++g) {
-        const int hq = h * h_r + g;
-        const T* q = static_cast<const T*>(a.q) + (int64_t)(q0 + t) * a.q_stride_tok + hq * a.q_stride_head + lane * E;
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < E; ++i) s = fmaf((float)q[i], k[i], s);
-        s = warp_allsum(s);
-        const float z = a.lse[(int64_t)(q0 + t) * a.h_q + hq];
-        if (z != -INFINITY) sum += expf(s * a.softmax_scale - z);
-      }
-    if (lane == 0) w[j] = (j >= L - n ? 0.f : w[j]) + sum;
+  griddep_wait();
+  if (threadIdx.x == 0) {
+    auto init = [](uint64_t* b, int n, int count) {
+      for (int i = 0; i < n; ++i) mbar_init(b + i, count);
+    };
+    init(r_full, RS, 1);
+    init(r_empty, RS, 128);
+    init(k_full, KS, 128);
+    init(k_empty, KS, 1);
+    init(q_full, QS, 1);
+    init(q_empty, QS, 1);
+    init(s_full, SB, 2);  // the product, and its issuer (who saw the job's scales and the rows' lse)
+    init(s_empty, SB, 128);
+    init(j_full, JOBS, 1);
+    init(j_empty, JOBS, 3 + 4 + 8);  // the K, Q and MMA warps, those that convert, those that add up
+    init(red_full, 1, 128);
+    init(red_empty, 1, 128);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    never_abort = 0;
+    fence_mbar_init();
   }
+  // rows of a Q stage that no box fills stay zero
+  for (int i = threadIdx.x; i < QS * C::QST / 16; i += THREADS) reinterpret_cast<uint4*>(sm + C::Q_OFF)[i] = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
+  if (warp == 0 && lane == 0) {
+    prefetch_tmap(&tmk);
+    prefetch_tmap(&tmq);
+  }
+  if (warp == 2) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (*tmem_slot != 0) {  // uniform, and cannot happen: all 512 columns
+    if (threadIdx.x == 0) flag(a.status, MJ_DEV_BAD_SPLIT);
+    if (warp == 2) tmem_dealloc(*tmem_slot, 512);
+    return;
+  }
+  auto wait = [&](uint64_t* bar, int phase) {
+    if (mbar_wait(bar, (uint32_t)phase & 1u, abort_flag, kWaitNs)) return true;
+    if (!*abort_flag) {
+      *abort_flag = 1;
+      flag(a.status, MJ_DEV_TIMEOUT);
+    }
+    return false;
+  };
+  // whole warps: every lane leaves with its warp
+  auto wait_warp = [&](uint64_t* bar, int phase) { return __all_sync(0xffffffffu, wait(bar, phase)) != 0; };
+  // job i of this CTA, once it is there; false at the end
+  auto next_job = [&](int i) { return wait_warp(&j_full[i % JOBS], i / JOBS) && jobs[i % JOBS].seq >= 0; };
+  auto done_job = [&](int i) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&j_empty[i % JOBS]);
+  };
+
+  if (warp == 3) {
+    // ------------------------------------------------------------------ the jobs
+    // 32 sequences at a time: lane i has the jobs of sequence s0 + i, and of those before it
+    int s0 = -32, i = 0;
+    int64_t base = 0, total = 0, before = 0, count = 0;
+    int L = 0, n = 0, q0 = 0;
+    bool ok = true;
+    for (int64_t round = 0; ok; ++round, ++i) {
+      const int64_t p = round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+      bool more = true;
+      while (p >= base + total) {
+        base += total;
+        s0 += 32;
+        if (s0 >= a.num_seqs) {
+          more = false;
+          break;
+        }
+        const int s = s0 + lane;
+        count = 0;
+        if (s < a.num_seqs) {
+          q0 = a.offsets[s];
+          n = a.offsets[s + 1] - q0;
+          L = a.seq_lens[s];
+          if (q0 < 0 || n < 0 || q0 + (int64_t)n > a.num_rows || L < 0 || L > a.weights_cols ||
+              L > (int64_t)a.block_table_cols * a.page_size || L > INT_MAX - 2 * KEYS)
+            flag(a.status, MJ_DEV_BAD_LENGTH);
+          else if (n) count = (int64_t)((L + KEYS - 1) / KEYS) * a.h_k;
+        }
+        before = count;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int64_t x = __shfl_up_sync(0xffffffffu, before, o);
+          if (lane >= o) before += x;
+        }
+        total = __shfl_sync(0xffffffffu, before, 31);
+        before -= count;
+      }
+      ok = wait_warp(&j_empty[i % JOBS], i / JOBS + 1);
+      if (!ok) break;
+      Job& j = jobs[i % JOBS];
+      if (!more) {
+        if (lane == 0) {
+          j.seq = -1;
+          mbar_arrive(&j_full[i % JOBS]);
+        }
+        break;
+      }
+      const int64_t at = p - base - before;
+      if (at >= 0 && at < count) {  // one lane: tiles of keys, and the heads of each, in turn
+        const int kt = (int)(at / a.h_k), first = a.window ? max(n - a.window, 0) : 0;
+        const int t0 = min(max(first, kt * KEYS - (L - n)), n);
+        j.seq = s0 + lane;
+        j.h = (int)(at % a.h_k);
+        j.kt = kt;
+        j.L = L;
+        j.n = n;
+        j.q0 = q0;
+        j.t0 = t0;
+        j.tiles = (n - t0 + tb - 1) / tb * ht;
+        mbar_arrive(&j_full[i % JOBS]);
+      }
+      __syncwarp();
+    }
+  } else if (warp == 0) {
+    // -------------------------------------------------------- K: codes and scales
+    // Lane i < 8 looks up the page of the tile's 16-token group i two jobs ahead
+    // and reads its exponent one job ahead (a use at once would wait for memory).
+    constexpr int kNone = INT_MIN;
+    const uint64_t policy = l2_policy_evict_normal();
+    const int ps = a.page_size, per = max(ps / 16, 1), pages = KEYS / ps, G = KEYS / 16;
+    auto entry_of = [&](const Job& j) {
+      const int pos = j.kt * KEYS + lane * 16;
+      return lane < G && pos < j.L ? __ldg(a.block_table + j.seq * a.block_table_stride + pos / ps) : kNone;
+    };
+    auto exponent_of = [&](const Job& j, int page) -> unsigned char {
+      if (page < 0) return 127;
+      const int row = (j.kt * KEYS + lane * 16) % ps;
+      return __ldg(static_cast<const unsigned char*>(a.k_scales) + page * a.ks_stride_page + (row >> lg) * a.ks_stride_block + j.h * a.ks_stride_head);
+    };
+    auto page_of = [&](int e) {  // -1: no such token, or a bad entry
+      if ((unsigned)e < (uint64_t)a.num_pages) return e;
+      if (e != kNone) flag(a.status, MJ_DEV_BAD_PAGE);
+      return -1;
+    };
+    bool here = next_job(0), ahead = here && next_job(1), ok = true;
+    int e0 = here ? entry_of(jobs[0]) : kNone, e1 = ahead ? entry_of(jobs[1 % JOBS]) : kNone;
+    int page = page_of(e0);
+    unsigned char ex = here ? exponent_of(jobs[0], page) : 127;
+    int i = 0;
+    for (; here; ++i) {
+      Job& j = jobs[i % JOBS];
+      const int page1 = page_of(e1);
+      const unsigned char ex1 = ahead ? exponent_of(jobs[(i + 1) % JOBS], page1) : 127;
+      const bool ahead2 = ahead && next_job(i + 2);
+      e1 = ahead2 ? entry_of(jobs[(i + 2) % JOBS]) : kNone;
+      ok = wait_warp(&r_empty[i % RS], i / RS + 1);
+      if (!ok) break;
+      if (lane < G) j.scale[lane] = block_scale(ex);
+      __syncwarp();
+      if (lane == 0) mbar_arrive_expect_tx(&r_full[i % RS], C::RAW);
+      __syncwarp();
+      const int pg = __shfl_sync(0xffffffffu, page, (lane * per) % 32);
+      if (lane < pages) {
+#pragma unroll
+        for (int dh = 0; dh < D / 128; ++dh)  // an absent page is read out of range: zeros
+          tma_load_5d(sm + C::R_OFF + (i % RS) * C::RAW + dh * (KEYS * 128) + lane * ps * 128, &tmk, &r_full[i % RS], 0, dh, 0, j.h,
+                      pg < 0 ? (int)a.num_pages : pg, policy);
+      }
+      done_job(i);
+      page = page1;
+      ex = ex1;
+      here = ahead;
+      ahead = ahead2;
+    }
+    for (int x = max(i - RS, 0); x < i; ++x) mbar_wait(&r_full[x % RS], (x / RS) & 1, &never_abort, kWaitNs);  // copies in flight land
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ Q and its lse
+    // Column c of a tile is (token c / hb, head c % hb of the tile's). The lse are
+    // loaded a tile ahead.
+    constexpr int PER = (N + 31) / 32;
+    const int h_r = a.h_q / a.h_k;
+    const uint64_t policy = l2_policy_evict_normal();
+    float z[PER], z1[PER];
+    auto load = [&](const Job& j, int tile, float* out) {
+      const int tok = j.t0 + tile / ht * tb, head = tile % ht * hb;
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        const int c = lane + 32 * k, t = tok + c / hb, g = head + c % hb;
+        out[k] = c < hb * tb && t < j.n && g < h_r ? __ldg(a.lse + (int64_t)(j.q0 + t) * a.h_q + j.h * h_r + g) : -INFINITY;
+      }
+    };
+    bool here = next_job(0);
+    int i = 0, tile = 0, it = 0;
+    if (here) load(jobs[0], 0, z);
+    while (here) {
+      const Job& j = jobs[i % JOBS];
+      const bool last = tile + 1 == j.tiles;
+      bool more = true;
+      if (last) more = next_job(i + 1);
+      if (more) load(last ? jobs[(i + 1) % JOBS] : j, last ? 0 : tile + 1, z1);
+      const int s = it % QS;
+      if (!wait_warp(&q_empty[s], it / QS + 1) || !wait_warp(&s_empty[it % SB], it / SB + 1)) break;
+      float* zs = reinterpret_cast<float*>(sm + C::Z_OFF) + it % SB * N;
+#pragma unroll
+      for (int k = 0; k < PER; ++k)  // a row without keys adds nothing
+        if (lane + 32 * k < N) zs[lane + 32 * k] = z[k] == -INFINITY ? -INFINITY : -z[k] * kLog2e;
+      __syncwarp();
+      if (lane == 0) mbar_arrive_expect_tx(&q_full[s], (D / 64) * 128 * hb * tb);
+      __syncwarp();
+      if (lane < D / 64)
+        tma_load_4d(sm + C::Q_OFF + s * C::QST + lane * (N * 128), &tmq, &q_full[s], lane * 64, tile % ht * hb, j.h,
+                    j.q0 + j.t0 + tile / ht * tb, policy);
+      ++it;
+      if (last) {
+        done_job(i);
+        ++i;
+        tile = 0;
+        here = more;
+      } else {
+        ++tile;
+      }
+#pragma unroll
+      for (int k = 0; k < PER; ++k) z[k] = z1[k];
+    }
+    for (int x = max(it - QS, 0); x < it; ++x) mbar_wait(&q_full[x % QS], (x / QS) & 1, &never_abort, kWaitNs);
+  } else if (warp == 2) {
+    // ---------------------------------------------------------------------- MMA
+    constexpr uint32_t idesc = std::is_same<T, __half>::value ? idesc_f16(0, 0, N) : idesc_bf16(0, 0, N);
+    const bool lead = elect_one();
+    int it = 0;
+    bool ok = true;
+    for (int i = 0; ok && next_job(i); ++i) {
+      const int tiles = jobs[i % JOBS].tiles;
+      ok = wait_warp(&k_full[i % KS], i / KS);
+      const uint64_t k = smem_desc_sw128(smem_addr(sm + C::K_OFF + (i % KS) * C::K16), 16, 1024);
+      for (int tile = 0; ok && tile < tiles; ++tile, ++it) {
+        const int b = it % SB, s = it % QS;
+        ok = wait_warp(&q_full[s], it / QS) && wait_warp(&s_empty[b], it / SB + 1);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t q = smem_desc_sw128(smem_addr(sm + C::Q_OFF + s * C::QST), 16, 1024);
+        if (lead) {
+#pragma unroll
+          for (int x = 0; x < D / 16; ++x)  // 16 head-dim elements a step
+            mma_f16(b * N, k + x / 4 * (KEYS * 8) + x % 4 * 2, q + x / 4 * (N * 8) + x % 4 * 2, idesc, x > 0);
+          mma_commit(&s_full[b]);
+          mbar_arrive(&s_full[b]);
+          mma_commit(&q_empty[s]);
+          if (tile + 1 == tiles) mma_commit(&k_empty[i % KS]);
+        }
+        __syncwarp();
+      }
+      done_job(i);
+    }
+    if (lead) mma_commit(drain);  // all issued MMAs complete before TMEM is released
+    mbar_wait(drain, 0, &never_abort, kWaitNs);
+  } else if (warp < 8) {
+    // ------------------------------------------------------------ codes -> 16 bits
+    // Thread ct takes 16-code chunk 4 blk + quad of rows r0, r0 + STEP, ...: eight
+    // neighbouring threads are four chunks of a 64-element block in rows r and
+    // r ^ 5, so that both their staged reads and their stores cover all banks.
+    const int ct = threadIdx.x - 128;
+    constexpr int BLOCKS = D / 64, STEP = 32 / BLOCKS, NC = KEYS / STEP, BATCH = 8;
+    const int quad = ct & 3, blk = (ct >> 3) % BLOCKS, pr = (ct >> 3) / BLOCKS;
+    const int r0 = ((pr & 3) ^ ((ct >> 2) & 1 ? 5 : 0)) + (pr & ~3) * 2;
+    for (int i = 0; next_job(i); ++i) {
+      if (!wait_warp(&r_full[i % RS], i / RS) || !wait_warp(&k_empty[i % KS], i / KS + 1)) break;
+      const unsigned char* raw = sm + C::R_OFF + (i % RS) * C::RAW + (blk >> 1) * (KEYS * 128);
+      unsigned char* out = sm + C::K_OFF + (i % KS) * C::K16 + blk * (KEYS * 128);
+#pragma unroll 1
+      for (int x0 = 0; x0 < NC; x0 += BATCH) {
+        uint4 d[BATCH];
+#pragma unroll
+        for (int x = 0; x < BATCH; ++x) d[x] = *reinterpret_cast<const uint4*>(raw + unit_offset(r0 + (x0 + x) * STEP, 4 * (blk & 1) + quad));
+#pragma unroll
+        for (int x = 0; x < BATCH; ++x) {
+          uint32_t o[8];
+          widen16<T>(d[x], o);
+          *reinterpret_cast<uint4*>(out + unit_offset(r0 + (x0 + x) * STEP, 2 * quad)) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(out + unit_offset(r0 + (x0 + x) * STEP, 2 * quad + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
+        }
+      }
+      // the stage is free once every value read from it went through the stores above
+      mbar_arrive(&r_empty[i % RS]);
+      fence_proxy_async_smem();
+      mbar_arrive(&k_full[i % KS]);
+      done_job(i);
+    }
+  } else {
+    // ------------------------------------------------------------------ the sums
+    const int wg = (warp - 8) >> 2, t = threadIdx.x & 127;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    int it = 0, joined = 0;
+    bool ok = true;
+    for (int i = 0; ok && next_job(i); ++i) {
+      const Job& j = jobs[i % JOBS];
+      const int tiles = j.tiles, key = j.kt * KEYS + t, ahead = j.L - j.n, t0 = j.t0, n = j.n;
+      float* w = a.weights + j.seq * a.w_stride_seq + j.h * a.w_stride_head + key;
+      // the warpgroup of the job's first tile writes its weights
+      const bool writes = (it & 1) == wg;
+      float old = 0.f;
+      if (writes && key < j.L && key < ahead) old = *w;
+      float sum = 0.f, low = 0.f, c2 = 0.f;  // the sum and what its rounding lost
+      for (int tile = 0; tile < tiles; ++tile, ++it) {
+        if ((it & 1) != wg) continue;
+        const int b = it % SB;
+        ok = wait_warp(&s_full[b], it / SB);
+        if (!ok) break;
+        tc_fence_after();
+        if (tile < 2) c2 = a.softmax_scale * kLog2e * j.scale[t >> 4];
+        // columns of queries that are there and see the key
+        const int tok = t0 + tile / ht * tb;
+        const int c_lo = max(key - ahead - tok, 0) * hb, c_hi = min(n - tok, tb) * hb;
+        const bool partial = tok + tb > n || j.kt * KEYS + KEYS - 1 > ahead + tok;  // uniform
+        const float4* zs = reinterpret_cast<const float4*>(sm + C::Z_OFF + b * N * 4);
+        float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        constexpr int W = N < 32 ? N : 32;
+#pragma unroll 1
+        for (int c = 0; c < N; c += W) {
+          float2 v[W / 2];
+          if (W == 32) tmem_ld32(b * N + c + lane_base, reinterpret_cast<float*>(v));
+          else tmem_ld16(b * N + c + lane_base, reinterpret_cast<float*>(v));
+          tmem_wait_ld();
+#pragma unroll
+          for (int x = 0; x < W / 4; ++x) {
+            const float4 z = zs[c / 4 + x];
+            float2 e0 = ffma2(v[2 * x], make_float2(c2, c2), make_float2(z.x, z.y));
+            float2 e1 = ffma2(v[2 * x + 1], make_float2(c2, c2), make_float2(z.z, z.w));
+            if (partial) {
+              const int c0 = c + 4 * x;
+              e0.x = c0 >= c_lo && c0 < c_hi ? e0.x : -INFINITY;
+              e0.y = c0 + 1 >= c_lo && c0 + 1 < c_hi ? e0.y : -INFINITY;
+              e1.x = c0 + 2 >= c_lo && c0 + 2 < c_hi ? e1.x : -INFINITY;
+              e1.y = c0 + 3 >= c_lo && c0 + 3 < c_hi ? e1.y : -INFINITY;
+            }
+            part[0] = fadd2(part[0], make_float2(exp2_approx(e0.x), exp2_approx(e0.y)));
+            part[1] = fadd2(part[1], make_float2(exp2_approx(e1.x), exp2_approx(e1.y)));
+          }
+        }
+        tc_fence_before();
+        mbar_arrive(&s_empty[b]);
+        const float p = (part[0].x + part[0].y) + (part[1].x + part[1].y) + low, next = sum + p;
+        low = p - (next - sum);
+        sum = next;
+      }
+      if (!ok) break;
+      if (tiles > 1) {  // the other warpgroup's part
+        if (!writes) {
+          ok = wait_warp(red_empty, joined + 1);
+          if (!ok) break;
+          red[t] = sum;
+          mbar_arrive(red_full);
+        } else {
+          ok = wait_warp(red_full, joined);
+          if (!ok) break;
+          sum += red[t];
+          mbar_arrive(red_empty);
+        }
+        ++joined;
+      }
+      if (writes && key < j.L) *w = old + sum;
+      done_job(i);
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc(0, 512);
+  }
+}
+
+constexpr int kMaxDevices = 64;
+
+template <typename T, int D, int N>
+static cudaError_t launch_t(const mj_block_weigh_args& a, cudaStream_t stream) {
+  using C = Cfg<T, D, N>;
+  auto kern = block_weigh_kernel<T, D, N>;
+  static std::atomic<int> ready[kMaxDevices];  // SMs of the device, once the kernel is prepared on it
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+  int sms = ready[dev].load(std::memory_order_acquire);
+  if (!sms) {
+    std::lock_guard<std::mutex> lock(tc_init_mutex());
+    if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM)) != cudaSuccess) return e;
+    if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
+    ready[dev].store(sms, std::memory_order_release);
+  }
+  auto fn = tensor_map_encoder();
+  if (!fn) return cudaErrorNotSupported;
+  CUtensorMap mk, mq;
+  {  // codes as (128 codes, 128-code halves of a row, page rows, KV heads, pages), boxes of one page's rows
+    cuuint64_t dims[5] = {128, (cuuint64_t)(D / 128), (cuuint64_t)a.page_size, (cuuint64_t)a.h_k, (cuuint64_t)a.num_pages};
+    // a dimension of extent 1 never moves its coordinate: any legal stride
+    cuuint64_t strides[4] = {128, (cuuint64_t)(a.k_stride_row ? a.k_stride_row : 16), (cuuint64_t)(a.k_stride_head ? a.k_stride_head : 16),
+                             (cuuint64_t)(a.k_stride_page ? a.k_stride_page : 16)};
+    cuuint32_t box[5] = {128, 1, (cuuint32_t)a.page_size, 1, 1}, estr[5] = {1, 1, 1, 1, 1};
+    if (fn(&mk, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<void*>(a.k_cache), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return cudaErrorInvalidValue;
+  }
+  // a tile of Q rows: tb tokens of hb heads of a group, or, of a larger group, N heads of one token
+  const int h_r = a.h_q / a.h_k, hb = h_r < N ? h_r : N, tb = N / hb, ht = (h_r + hb - 1) / hb;
+  {  // rows as (elements, heads of a group, groups, tokens)
+    const cuuint64_t head = a.h_q > 1 ? a.q_stride_head * 2 : 16, tok = a.num_rows > 1 ? a.q_stride_tok * 2 : 16;
+    cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)h_r, (cuuint64_t)a.h_k, (cuuint64_t)a.num_rows}, strides[3] = {head, head * h_r, tok};
+    cuuint32_t box[4] = {64, (cuuint32_t)hb, 1, (cuuint32_t)tb}, estr[4] = {1, 1, 1, 1};
+    if (fn(&mq, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(a.q),
+           dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return cudaErrorInvalidValue;
+  }
+  return launch_kernel(kern, dim3((unsigned)sms), dim3(THREADS), C::SMEM, stream, a, block_log2(a.kv_format), hb, tb, ht, mk, mq);
 }
 
 template <typename T>
-static cudaError_t weigh_t(const mj_block_weigh_args& a, cudaStream_t stream) {
-  const int blocks = 64;
-  const dim3 grid((unsigned)(a.num_seqs * a.h_k * blocks));
-  auto kern = a.head_size == 256 ? block_weigh_kernel<T, 256> : block_weigh_kernel<T, 128>;
-  return launch_kernel(kern, grid, dim3(256), 0, stream, a, block_log2(a.kv_format), blocks);
+static cudaError_t launch_d(const mj_block_weigh_args& a, cudaStream_t stream) {
+  // rows of a sequence and KV head that count, on average
+  const int64_t all = a.num_rows * (a.h_q / a.h_k), most = a.window ? (int64_t)a.num_seqs * a.window * (a.h_q / a.h_k) : all;
+  const bool few = (all < most ? all : most) <= (int64_t)32 * a.num_seqs;
+  if (a.head_size == 256) return few ? launch_t<T, 256, 16>(a, stream) : launch_t<T, 256, 64>(a, stream);
+  return few ? launch_t<T, 128, 16>(a, stream) : launch_t<T, 128, 128>(a, stream);
 }
 
+}  // namespace bw
+
 cudaError_t launch_block_weigh(const mj_block_weigh_args& a, cudaStream_t stream) {
-  return a.dtype == MJ_DT_FP16 ? weigh_t<__half>(a, stream) : weigh_t<__nv_bfloat16>(a, stream);
+  return a.dtype == MJ_DT_FP16 ? bw::launch_d<__half>(a, stream) : bw::launch_d<__nv_bfloat16>(a, stream);
 }
 
 }  // namespace mj

@@ -461,6 +461,8 @@ int mj_block_weigh(const mj_block_weigh_args* args, void* stream) {
     return fail(MJ_ERR_UNSUPPORTED, "mj_block_weigh: a weights stride of 0");
   if (!aligned(a.q, 16) || a.q_stride_tok % 8 || a.q_stride_head % 8 || a.q_stride_tok < 0 || a.q_stride_head < 0)
     return fail(MJ_ERR_UNSUPPORTED, "mj_block_weigh: q rows must be 16-byte aligned");
+  if ((a.num_rows > 1 && !a.q_stride_tok) || (a.h_q > 1 && !a.q_stride_head))
+    return fail(MJ_ERR_UNSUPPORTED, "mj_block_weigh: a q stride of 0");
   if (a.num_rows * a.h_q > (int64_t)INT32_MAX || a.num_seqs > 1 << 20) return fail(MJ_ERR_UNSUPPORTED, "mj_block_weigh: too many rows");
   if (shared_bytes(st, a.num_pages, a.page_size, a.h_k)) return fail(MJ_ERR_UNSUPPORTED, "mj_block_weigh: a cache stride of 0");
   return cuda_status(mj::launch_block_weigh(a, (cudaStream_t)stream), "mj_block_weigh launch");

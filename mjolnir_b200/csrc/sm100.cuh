@@ -288,6 +288,16 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uin
       : "memory");
 }
 
+// kind::f16, both operands in shared memory, of one 16-bit type.
+__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // One lane of a converged warp. A warp that runs an issue loop as a whole and
 // issues through this keeps the loop's addresses and descriptors in uniform
 // registers; in a one-thread branch each MMA first moves them there.
@@ -319,6 +329,11 @@ __host__ __device__ constexpr uint32_t idesc_f8f6f4(uint32_t a_fmt, uint32_t b_f
 // Instruction descriptor for kind::f16 on f16 operands, fp32 accumulator, M = 128.
 __host__ __device__ constexpr uint32_t idesc_f16(uint32_t a_major, uint32_t b_major, uint32_t n) {
   return (1u << 4) | (a_major << 15) | (b_major << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+// The same on bf16 operands.
+__host__ __device__ constexpr uint32_t idesc_bf16(uint32_t a_major, uint32_t b_major, uint32_t n) {
+  return idesc_f16(a_major, b_major, n) | (1u << 7) | (1u << 10);
 }
 
 // Shared-memory matrix descriptor, 128-byte swizzle, sm_100 version 1.
