@@ -19,9 +19,9 @@
 // take the jobs in rounds, every other round in reverse: a prompt's first keys
 // are seen by all its rows, its last by few.
 //
-// Warp roles: 0 K (page walk, TMA, block scales), 1 Q (TMA) and its lse, 2 MMA,
-// 3 the jobs; 4-7 convert K's codes; 8-15 two warpgroups that take the S tiles
-// in turn and add up. Every mbarrier wait is bounded; on a timeout the CTA flags
+// Warp roles: 0 K (page walk, TMA, block scales), 1 Q (TMA), 2 MMA,
+// 3 the jobs; then warpgroups that convert K's codes, in turn, and warpgroups that
+// take the S tiles in turn and add up. Every mbarrier wait is bounded; on a timeout the CTA flags
 // MJ_DEV_TIMEOUT, all roles stop, copies and MMAs in flight complete and TMEM is
 // freed.
 #include <limits.h>
@@ -49,28 +49,44 @@ using namespace sm100;
 
 constexpr uint64_t kWaitNs = 500000000ull;  // per wait; a tile takes microseconds
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int KEYS = 128, JOBS = 8, THREADS = 512;
+constexpr int KEYS = 128;
+
+// Tiles of keys of a job, at most: where few rows see them, a job's lookups and
+// its descriptor serve several.
+template <int N>
+constexpr int kTiles = N >= 64 ? 1 : 4;
 
 // What a role needs to know of a job. The K warp adds the scales.
 struct Job {
-  int seq, h, kt, L, n, q0, t0, tiles;  // seq < 0: no more; t0: the first query that counts and sees a key
-  float scale[KEYS / 16];
+  int seq, h, kt, nk, L, n, q0;  // seq < 0: no more; nk tiles of keys from kt on
+  int t0[4], tiles[4];           // of each: the first query that counts and sees one of them, tiles of rows from it on
+  float scale[4 * (KEYS / 16)];
 };
 
 template <typename T, int D, int N>
 struct Cfg {
   static constexpr int RAW = KEYS * D, K16 = 2 * RAW, QST = N * D * 2;  // a tile's codes; as 16 bits; a tile of Q rows
   static constexpr bool WIDE = N >= 64;
+  // Warpgroups that convert K's codes, and that add up. Many rows: the
+  // exponentials bound it, and two or four warps on a scheduler must hide one
+  // another's latency (8192 tokens, 32 / 8 heads: 376 us with two warpgroups, 341
+  // with four). Few rows: every tile of keys is converted for one product.
+  static constexpr int CWGS = WIDE || D == 256 ? 1 : 2, WGS = WIDE ? 4 : 2, THREADS = 128 * (1 + CWGS + WGS);
   // stages of K codes, of K in 16 bits, of Q
-  static constexpr int RS = WIDE ? 2 : D == 256 ? 4 : 6, KS = D == 256 ? 1 : 2, QS = WIDE ? 3 : 4;
-  static constexpr int SB = 4;  // S buffers in TMEM, each with its columns' lse
+  static constexpr int RS = WIDE ? (D == 256 ? 1 : 2) : D == 256 ? 3 : 8, KS = D == 256 ? 1 : 2, QS = WIDE ? 3 : 4;
+  static constexpr int SB = 4;  // S buffers in TMEM; a warpgroup that adds up has three of its columns' lse
+  static constexpr int JOBS = 4;
+  static constexpr int PAIRS = WGS * (WGS - 1);  // of a warpgroup that writes weights and one that adds its part
   static constexpr int K_OFF = 0, R_OFF = K_OFF + KS * K16, Q_OFF = R_OFF + RS * RAW, Z_OFF = Q_OFF + QS * QST;
-  static constexpr int RED_OFF = Z_OFF + SB * N * 4, JOB_OFF = RED_OFF + KEYS * 4, BAR_OFF = JOB_OFF + JOBS * (int)sizeof(Job);
-  static constexpr int NBARS = 2 * (RS + KS + QS + SB + JOBS + 1) + 1;
+  static constexpr int RED_OFF = Z_OFF + 3 * WGS * N * 4, JOB_OFF = RED_OFF + PAIRS * KEYS * 4, BAR_OFF = JOB_OFF + JOBS * (int)sizeof(Job);
+  static constexpr int NBARS = 2 * (RS + KS + QS + SB + JOBS + PAIRS) + WGS + 1;
   static constexpr int MISC_OFF = BAR_OFF + NBARS * 8;
   static constexpr int SMEM = MISC_OFF + 16;
   static_assert(SMEM <= 232448, "shared memory of a CTA");
   static_assert(JOBS >= 3, "the K warp looks two jobs ahead");
+  // a buffer is always waited for by the same warpgroup, whose waits are in order:
+  // another's could take an older phase of the same parity for its own
+  static_assert(RS % CWGS == 0 && KS % CWGS == 0 && SB % WGS == 0, "buffers of a warpgroup");
 };
 
 // 16 codes -> 16 values of T (exact)
@@ -95,17 +111,17 @@ __device__ __forceinline__ void widen16(uint4 c, uint32_t* o) {
 __device__ __forceinline__ uint32_t unit_offset(uint32_t r, uint32_t u) { return r * 128 + ((u ^ (r & 7)) << 4); }
 
 template <typename T, int D, int N>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
     block_weigh_kernel(const __grid_constant__ mj_block_weigh_args a, int lg, int hb, int tb, int ht,
                        const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmq) {
   using C = Cfg<T, D, N>;
-  constexpr int RS = C::RS, KS = C::KS, QS = C::QS, SB = C::SB;
+  constexpr int RS = C::RS, KS = C::KS, QS = C::QS, SB = C::SB, JOBS = C::JOBS, CWGS = C::CWGS, WGS = C::WGS;
   extern __shared__ __align__(1024) unsigned char sm[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::BAR_OFF);
   uint64_t *r_full = bars, *r_empty = r_full + RS, *k_full = r_empty + RS, *k_empty = k_full + KS, *q_full = k_empty + KS,
            *q_empty = q_full + QS, *s_full = q_empty + QS, *s_empty = s_full + SB, *j_full = s_empty + SB, *j_empty = j_full + JOBS,
-           *red_full = j_empty + JOBS, *red_empty = red_full + 1, *drain = red_empty + 1;
+           *red_full = j_empty + JOBS, *red_empty = red_full + C::PAIRS, *z_full = red_empty + C::PAIRS, *drain = z_full + WGS;
   Job* jobs = reinterpret_cast<Job*>(sm + C::JOB_OFF);
   float* red = reinterpret_cast<float*>(sm + C::RED_OFF);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::MISC_OFF);
@@ -126,19 +142,20 @@ __global__ void __launch_bounds__(THREADS, 1)
     init(k_empty, KS, 1);
     init(q_full, QS, 1);
     init(q_empty, QS, 1);
-    init(s_full, SB, 2);  // the product, and its issuer (who saw the job's scales and the rows' lse)
+    init(s_full, SB, 2);  // the product, and its issuer (who saw the job's scales)
     init(s_empty, SB, 128);
     init(j_full, JOBS, 1);
-    init(j_empty, JOBS, 3 + 4 + 8);  // the K, Q and MMA warps, those that convert, those that add up
-    init(red_full, 1, 128);
-    init(red_empty, 1, 128);
+    init(j_empty, JOBS, 3 + 4 * (CWGS + WGS));  // the K, Q and MMA warps, those that convert, those that add up
+    init(red_full, C::PAIRS, 128);
+    init(red_empty, C::PAIRS, 128);
+    init(z_full, WGS, 128);
     mbar_init(drain, 1);
     *abort_flag = 0;
     never_abort = 0;
     fence_mbar_init();
   }
   // rows of a Q stage that no box fills stay zero
-  for (int i = threadIdx.x; i < QS * C::QST / 16; i += THREADS) reinterpret_cast<uint4*>(sm + C::Q_OFF)[i] = make_uint4(0, 0, 0, 0);
+  for (int i = threadIdx.x; i < QS * C::QST / 16; i += C::THREADS) reinterpret_cast<uint4*>(sm + C::Q_OFF)[i] = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
   if (warp == 0 && lane == 0) {
     prefetch_tmap(&tmk);
@@ -175,10 +192,35 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   if (warp == 3) {
     // ------------------------------------------------------------------ the jobs
-    // 32 sequences at a time: lane i has the jobs of sequence s0 + i, and of those before it
+    // 32 sequences at a time: lane i has the key tiles of sequence s0 + i
+    int L = 0, n = 0, q0 = 0;
+    auto tiles_of = [&](int s, bool complain) {
+      if (s >= a.num_seqs) return 0;
+      q0 = a.offsets[s];
+      n = a.offsets[s + 1] - q0;
+      L = a.seq_lens[s];
+      if (q0 < 0 || n < 0 || q0 + (int64_t)n > a.num_rows || L < 0 || L > a.weights_cols ||
+          L > (int64_t)a.block_table_cols * a.page_size || L > INT_MAX - 8 * KEYS) {
+        if (complain) flag(a.status, MJ_DEV_BAD_LENGTH);
+        return 0;
+      }
+      return n ? (L + KEYS - 1) / KEYS : 0;
+    };
+    // Tiles a job: as many as leave every CTA two jobs (each costs its lookups'
+    // latency; a few jobs more than CTAs leave some of them idle).
+    int per = 1;
+    if (kTiles<N> > 1) {
+      int64_t tiles = 0;
+      for (int s = lane; s - lane < a.num_seqs && tiles * a.h_k < 2ll * kTiles<N> * gridDim.x; s += 32) {
+        int x = tiles_of(s, false);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        tiles += x;
+      }
+      while (per < kTiles<N> && tiles * a.h_k >= 4ll * per * gridDim.x) per *= 2;
+    }
     int s0 = -32, i = 0;
     int64_t base = 0, total = 0, before = 0, count = 0;
-    int L = 0, n = 0, q0 = 0;
     bool ok = true;
     for (int64_t round = 0; ok; ++round, ++i) {
       const int64_t p = round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
@@ -190,17 +232,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           more = false;
           break;
         }
-        const int s = s0 + lane;
-        count = 0;
-        if (s < a.num_seqs) {
-          q0 = a.offsets[s];
-          n = a.offsets[s + 1] - q0;
-          L = a.seq_lens[s];
-          if (q0 < 0 || n < 0 || q0 + (int64_t)n > a.num_rows || L < 0 || L > a.weights_cols ||
-              L > (int64_t)a.block_table_cols * a.page_size || L > INT_MAX - 2 * KEYS)
-            flag(a.status, MJ_DEV_BAD_LENGTH);
-          else if (n) count = (int64_t)((L + KEYS - 1) / KEYS) * a.h_k;
-        }
+        count = (int64_t)((tiles_of(s0 + lane, true) + per - 1) / per) * a.h_k;
         before = count;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -221,35 +253,37 @@ __global__ void __launch_bounds__(THREADS, 1)
         break;
       }
       const int64_t at = p - base - before;
-      if (at >= 0 && at < count) {  // one lane: tiles of keys, and the heads of each, in turn
-        const int kt = (int)(at / a.h_k), first = a.window ? max(n - a.window, 0) : 0;
-        const int t0 = min(max(first, kt * KEYS - (L - n)), n);
+      if (at >= 0 && at < count) {  // one lane: groups of key tiles, and the heads of each, in turn
+        const int64_t group = at >> 32 ? at / a.h_k : (uint32_t)at / (uint32_t)a.h_k;  // a 64-bit division is a long routine
         j.seq = s0 + lane;
-        j.h = (int)(at % a.h_k);
-        j.kt = kt;
+        j.h = (int)(at - group * a.h_k);
+        j.kt = (int)group * per;
+        j.nk = min(per, (L + KEYS - 1) / KEYS - j.kt);
         j.L = L;
         j.n = n;
         j.q0 = q0;
-        j.t0 = t0;
-        j.tiles = (n - t0 + tb - 1) / tb * ht;
+        for (int x = 0; x < j.nk; ++x) {
+          j.t0[x] = max(a.window ? max(n - a.window, 0) : 0, (j.kt + x) * KEYS - (L - n));
+          j.tiles[x] = (n - j.t0[x] + tb - 1) / tb * ht;
+        }
         mbar_arrive(&j_full[i % JOBS]);
       }
       __syncwarp();
     }
   } else if (warp == 0) {
     // -------------------------------------------------------- K: codes and scales
-    // Lane i < 8 looks up the page of the tile's 16-token group i two jobs ahead
-    // and reads its exponent one job ahead (a use at once would wait for memory).
+    // Lane i looks up the page of the job's 16-token group i two jobs ahead and
+    // reads its exponent one job ahead (a use at once would wait for memory).
     constexpr int kNone = INT_MIN;
     const uint64_t policy = l2_policy_evict_normal();
-    const int ps = a.page_size, per = max(ps / 16, 1), pages = KEYS / ps, G = KEYS / 16;
+    const int ps = a.page_size, lps = 31 - __clz(ps), groups = max(ps / 16, 1), pages = KEYS / ps;
     auto entry_of = [&](const Job& j) {
       const int pos = j.kt * KEYS + lane * 16;
-      return lane < G && pos < j.L ? __ldg(a.block_table + j.seq * a.block_table_stride + pos / ps) : kNone;
+      return lane < j.nk * (KEYS / 16) && pos < j.L ? __ldg(a.block_table + j.seq * a.block_table_stride + (pos >> lps)) : kNone;
     };
     auto exponent_of = [&](const Job& j, int page) -> unsigned char {
       if (page < 0) return 127;
-      const int row = (j.kt * KEYS + lane * 16) % ps;
+      const int row = (j.kt * KEYS + lane * 16) & (ps - 1);
       return __ldg(static_cast<const unsigned char*>(a.k_scales) + page * a.ks_stride_page + (row >> lg) * a.ks_stride_block + j.h * a.ks_stride_head);
     };
     auto page_of = [&](int e) {  // -1: no such token, or a bad entry
@@ -261,127 +295,122 @@ __global__ void __launch_bounds__(THREADS, 1)
     int e0 = here ? entry_of(jobs[0]) : kNone, e1 = ahead ? entry_of(jobs[1 % JOBS]) : kNone;
     int page = page_of(e0);
     unsigned char ex = here ? exponent_of(jobs[0], page) : 127;
-    int i = 0;
-    for (; here; ++i) {
+    int i = 0, u = 0;
+    for (; ok && here; ++i) {
       Job& j = jobs[i % JOBS];
+      const int nk = j.nk, h = j.h;
+      j.scale[lane] = block_scale(ex);
       const int page1 = page_of(e1);
       const unsigned char ex1 = ahead ? exponent_of(jobs[(i + 1) % JOBS], page1) : 127;
       const bool ahead2 = ahead && next_job(i + 2);
       e1 = ahead2 ? entry_of(jobs[(i + 2) % JOBS]) : kNone;
-      ok = wait_warp(&r_empty[i % RS], i / RS + 1);
-      if (!ok) break;
-      if (lane < G) j.scale[lane] = block_scale(ex);
-      __syncwarp();
-      if (lane == 0) mbar_arrive_expect_tx(&r_full[i % RS], C::RAW);
-      __syncwarp();
-      const int pg = __shfl_sync(0xffffffffu, page, (lane * per) % 32);
-      if (lane < pages) {
+      __syncwarp();  // the scales are written before lane 0 arrives
+      for (int x = 0; x < nk; ++x, ++u) {
+        ok = wait_warp(&r_empty[u % RS], u / RS + 1);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&r_full[u % RS], C::RAW);
+        __syncwarp();
+        const int pg = __shfl_sync(0xffffffffu, page, (x * (KEYS / 16) + lane * groups) & 31);
+        if (lane < pages) {
 #pragma unroll
-        for (int dh = 0; dh < D / 128; ++dh)  // an absent page is read out of range: zeros
-          tma_load_5d(sm + C::R_OFF + (i % RS) * C::RAW + dh * (KEYS * 128) + lane * ps * 128, &tmk, &r_full[i % RS], 0, dh, 0, j.h,
-                      pg < 0 ? (int)a.num_pages : pg, policy);
+          for (int dh = 0; dh < D / 128; ++dh)  // an absent page is read out of range: zeros
+            tma_load_5d(sm + C::R_OFF + (u % RS) * C::RAW + dh * (KEYS * 128) + lane * ps * 128, &tmk, &r_full[u % RS], 0, dh, 0, h,
+                        pg < 0 ? (int)a.num_pages : pg, policy);
+        }
       }
+      if (!ok) break;
       done_job(i);
       page = page1;
       ex = ex1;
       here = ahead;
       ahead = ahead2;
     }
-    for (int x = max(i - RS, 0); x < i; ++x) mbar_wait(&r_full[x % RS], (x / RS) & 1, &never_abort, kWaitNs);  // copies in flight land
+    for (int x = max(u - RS, 0); x < u; ++x) mbar_wait(&r_full[x % RS], (x / RS) & 1, &never_abort, kWaitNs);  // copies in flight land
   } else if (warp == 1) {
-    // ------------------------------------------------------------ Q and its lse
-    // Column c of a tile is (token c / hb, head c % hb of the tile's). The lse are
-    // loaded a tile ahead.
-    constexpr int PER = (N + 31) / 32;
+    // ------------------------------------------------------------------------- Q
+    // Column c of a tile is (token c / hb, head c % hb of the tile's).
     const int h_r = a.h_q / a.h_k;
     const uint64_t policy = l2_policy_evict_normal();
-    float z[PER], z1[PER];
-    auto load = [&](const Job& j, int tile, float* out) {
-      const int tok = j.t0 + tile / ht * tb, head = tile % ht * hb;
-#pragma unroll
-      for (int k = 0; k < PER; ++k) {
-        const int c = lane + 32 * k, t = tok + c / hb, g = head + c % hb;
-        out[k] = c < hb * tb && t < j.n && g < h_r ? __ldg(a.lse + (int64_t)(j.q0 + t) * a.h_q + j.h * h_r + g) : -INFINITY;
-      }
-    };
-    bool here = next_job(0);
-    int i = 0, tile = 0, it = 0;
-    if (here) load(jobs[0], 0, z);
-    while (here) {
+    int it = 0;
+    bool ok = true;
+    for (int i = 0; ok && next_job(i); ++i) {
       const Job& j = jobs[i % JOBS];
-      const bool last = tile + 1 == j.tiles;
-      bool more = true;
-      if (last) more = next_job(i + 1);
-      if (more) load(last ? jobs[(i + 1) % JOBS] : j, last ? 0 : tile + 1, z1);
-      const int s = it % QS;
-      if (!wait_warp(&q_empty[s], it / QS + 1) || !wait_warp(&s_empty[it % SB], it / SB + 1)) break;
-      float* zs = reinterpret_cast<float*>(sm + C::Z_OFF) + it % SB * N;
-#pragma unroll
-      for (int k = 0; k < PER; ++k)  // a row without keys adds nothing
-        if (lane + 32 * k < N) zs[lane + 32 * k] = z[k] == -INFINITY ? -INFINITY : -z[k] * kLog2e;
-      __syncwarp();
-      if (lane == 0) mbar_arrive_expect_tx(&q_full[s], (D / 64) * 128 * hb * tb);
-      __syncwarp();
-      if (lane < D / 64)
-        tma_load_4d(sm + C::Q_OFF + s * C::QST + lane * (N * 128), &tmq, &q_full[s], lane * 64, tile % ht * hb, j.h,
-                    j.q0 + j.t0 + tile / ht * tb, policy);
-      ++it;
-      if (last) {
-        done_job(i);
-        ++i;
-        tile = 0;
-        here = more;
-      } else {
-        ++tile;
-      }
-#pragma unroll
-      for (int k = 0; k < PER; ++k) z[k] = z1[k];
+      const int nk = j.nk, h = j.h, n = j.n, q0 = j.q0;
+      for (int x = 0; ok && x < nk; ++x)
+        for (int tok = j.t0[x], head = 0; tok < n; ++it) {
+          const int s = it % QS;
+          ok = wait_warp(&q_empty[s], it / QS + 1);
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(&q_full[s], (D / 64) * 128 * hb * tb);
+          __syncwarp();
+          if (lane < D / 64) tma_load_4d(sm + C::Q_OFF + s * C::QST + lane * (N * 128), &tmq, &q_full[s], lane * 64, head, h, q0 + tok, policy);
+          head += hb;
+          if (head >= h_r) {
+            head = 0;
+            tok += tb;
+          }
+        }
+      if (ok) done_job(i);
     }
-    for (int x = max(it - QS, 0); x < it; ++x) mbar_wait(&q_full[x % QS], (x / QS) & 1, &never_abort, kWaitNs);
+    for (int y = max(it - QS, 0); y < it; ++y) mbar_wait(&q_full[y % QS], (y / QS) & 1, &never_abort, kWaitNs);
   } else if (warp == 2) {
     // ---------------------------------------------------------------------- MMA
     constexpr uint32_t idesc = std::is_same<T, __half>::value ? idesc_f16(0, 0, N) : idesc_bf16(0, 0, N);
     const bool lead = elect_one();
-    int it = 0;
+    int it = 0, u = 0;
     bool ok = true;
+    auto ready = [&]() { return wait_warp(&q_full[it % QS], it / QS) && wait_warp(&s_empty[it % SB], it / SB + 1); };  // tile `it`
     for (int i = 0; ok && next_job(i); ++i) {
-      const int tiles = jobs[i % JOBS].tiles;
-      ok = wait_warp(&k_full[i % KS], i / KS);
-      const uint64_t k = smem_desc_sw128(smem_addr(sm + C::K_OFF + (i % KS) * C::K16), 16, 1024);
-      for (int tile = 0; ok && tile < tiles; ++tile, ++it) {
-        const int b = it % SB, s = it % QS;
-        ok = wait_warp(&q_full[s], it / QS) && wait_warp(&s_empty[b], it / SB + 1);
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t q = smem_desc_sw128(smem_addr(sm + C::Q_OFF + s * C::QST), 16, 1024);
-        if (lead) {
+      const Job& j = jobs[i % JOBS];
+      for (int x = 0, nk = j.nk; ok && x < nk; ++x, ++u) {
+        const int tiles = j.tiles[x];
+        ok = wait_warp(&k_full[u % KS], u / KS) && ready();
+        const uint64_t k = smem_desc_sw128(smem_addr(sm + C::K_OFF + (u % KS) * C::K16), 16, 1024);
+        for (int tile = 0; ok && tile < tiles; ++tile) {
+          const int b = it % SB, s = it % QS;
+          tc_fence_after();
+          const uint64_t q = smem_desc_sw128(smem_addr(sm + C::Q_OFF + s * C::QST), 16, 1024);
+          auto steps = [&](auto half) {  // 16 head-dim elements a step
+            constexpr int H = decltype(half)::value;
+            if (lead) {
 #pragma unroll
-          for (int x = 0; x < D / 16; ++x)  // 16 head-dim elements a step
-            mma_f16(b * N, k + x / 4 * (KEYS * 8) + x % 4 * 2, q + x / 4 * (N * 8) + x % 4 * 2, idesc, x > 0);
-          mma_commit(&s_full[b]);
-          mbar_arrive(&s_full[b]);
-          mma_commit(&q_empty[s]);
-          if (tile + 1 == tiles) mma_commit(&k_empty[i % KS]);
+              for (int y = H * (D / 32); y < (H + 1) * (D / 32); ++y)
+                mma_f16(b * N, k + y / 4 * (KEYS * 8) + y % 4 * 2, q + y / 4 * (N * 8) + y % 4 * 2, idesc, y > 0);
+            }
+          };
+          steps(std::integral_constant<int, 0>());
+          // the waits for the next tile pass while these products run
+          ++it;
+          if (tile + 1 < tiles) ok = ready();
+          steps(std::integral_constant<int, 1>());
+          if (lead) {
+            mma_commit(&s_full[b]);
+            mbar_arrive(&s_full[b]);
+            mma_commit(&q_empty[s]);
+            if (tile + 1 == tiles) mma_commit(&k_empty[u % KS]);
+          }
+          __syncwarp();
         }
-        __syncwarp();
       }
-      done_job(i);
+      if (ok) done_job(i);
     }
     if (lead) mma_commit(drain);  // all issued MMAs complete before TMEM is released
     mbar_wait(drain, 0, &never_abort, kWaitNs);
-  } else if (warp < 8) {
+  } else if (warp < 4 + 4 * CWGS) {
     // ------------------------------------------------------------ codes -> 16 bits
     // Thread ct takes 16-code chunk 4 blk + quad of rows r0, r0 + STEP, ...: eight
     // neighbouring threads are four chunks of a 64-element block in rows r and
     // r ^ 5, so that both their staged reads and their stores cover all banks.
-    const int ct = threadIdx.x - 128;
-    constexpr int BLOCKS = D / 64, STEP = 32 / BLOCKS, NC = KEYS / STEP, BATCH = 8;
+    const int ct = threadIdx.x & 127, cwg = (warp - 4) >> 2;
+    constexpr int BLOCKS = D / 64, STEP = 32 / BLOCKS, NC = KEYS / STEP, BATCH = 4;
     const int quad = ct & 3, blk = (ct >> 3) % BLOCKS, pr = (ct >> 3) / BLOCKS;
     const int r0 = ((pr & 3) ^ ((ct >> 2) & 1 ? 5 : 0)) + (pr & ~3) * 2;
-    for (int i = 0; next_job(i); ++i) {
-      if (!wait_warp(&r_full[i % RS], i / RS) || !wait_warp(&k_empty[i % KS], i / KS + 1)) break;
-      const unsigned char* raw = sm + C::R_OFF + (i % RS) * C::RAW + (blk >> 1) * (KEYS * 128);
-      unsigned char* out = sm + C::K_OFF + (i % KS) * C::K16 + blk * (KEYS * 128);
+    int u = 0;
+    bool ok = true;
+    auto convert = [&]() {
+      if (!wait_warp(&r_full[u % RS], u / RS) || !wait_warp(&k_empty[u % KS], u / KS + 1)) return false;
+      const unsigned char* raw = sm + C::R_OFF + (u % RS) * C::RAW + (blk >> 1) * (KEYS * 128);
+      unsigned char* out = sm + C::K_OFF + (u % KS) * C::K16 + blk * (KEYS * 128);
 #pragma unroll 1
       for (int x0 = 0; x0 < NC; x0 += BATCH) {
         uint4 d[BATCH];
@@ -396,85 +425,142 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
       // the stage is free once every value read from it went through the stores above
-      mbar_arrive(&r_empty[i % RS]);
+      mbar_arrive(&r_empty[u % RS]);
       fence_proxy_async_smem();
-      mbar_arrive(&k_full[i % KS]);
-      done_job(i);
+      mbar_arrive(&k_full[u % KS]);
+      return true;
+    };
+    for (int i = 0; ok && next_job(i); ++i) {
+      const int nk = jobs[i % JOBS].nk;
+#pragma unroll 1
+      for (int x = 0; ok && x < nk; ++x, ++u)
+        if (CWGS == 1 || u % CWGS == cwg) ok = convert();
+      if (ok) done_job(i);
     }
   } else {
     // ------------------------------------------------------------------ the sums
-    const int wg = (warp - 8) >> 2, t = threadIdx.x & 127;
+    const int wg = (warp - 4 - 4 * CWGS) >> 2, t = threadIdx.x & 127;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    int it = 0, joined = 0;
+    const int h_r = a.h_q / a.h_k;
+    // The lse of this warpgroup's tiles, by buffer: a tile's are stored while the
+    // one before is added up, which warps that lag behind may still be at the
+    // start of; so three.
+    float* const zbuf = reinterpret_cast<float*>(sm + C::Z_OFF) + wg * (3 * N);
+    int z_stored = 0, z_seen = 0;
+    // this thread's column: its lse in tile `tile` of the queries from t0 on
+    const int z_tok = t < hb * tb ? t / hb : INT_MAX / 2, z_head = t % hb;
+    auto tok_of = [&](int t0, int tile) { return t0 + (ht == 1 ? tile : tile / ht) * tb; };
+    auto load_lse = [&](const Job& j, int t0, int tile) {
+      const int tok = tok_of(t0, tile), head = ht == 1 ? z_head : tile % ht * hb + z_head;
+      return z_tok < j.n - tok && head < h_r ? __ldg(a.lse + (int64_t)(j.q0 + tok + z_tok) * a.h_q + j.h * h_r + head) : -INFINITY;
+    };
+    auto store_lse = [&](float z) {
+      if (t < N) zbuf[z_stored % 3 * N + t] = z == -INFINITY ? -INFINITY : -z * kLog2e;  // a row without keys adds nothing
+      mbar_arrive(&z_full[wg]);
+      ++z_stored;
+    };
+    // This key's weights of the tile in S buffer b, columns [c_lo, c_hi) of it where
+    // PART: the next columns are on their way from TMEM while these are added up.
+    auto add_up = [&](auto part, int b, float c2, int c_lo, int c_hi) {
+      constexpr bool PART = decltype(part)::value;
+      const float4* zs = reinterpret_cast<const float4*>(zbuf + (z_seen + 2) % 3 * N);
+      const uint32_t s_addr = b * N + lane_base;
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)}, v[2][8];
+      tmem_ld16(s_addr, reinterpret_cast<float*>(v[0]));
+#pragma unroll
+      for (int c = 0; c < N; c += 16) {
+        float2* const now = v[c / 16 & 1];
+        tmem_wait_ld();
+        if (c + 16 < N) tmem_ld16(s_addr + c + 16, reinterpret_cast<float*>(v[c / 16 + 1 & 1]));
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          if (PART && c + 4 * x >= c_hi) break;  // uniform
+          const float4 z = zs[c / 4 + x];
+          float2 e[2] = {ffma2(now[2 * x], make_float2(c2, c2), make_float2(z.x, z.y)),
+                         ffma2(now[2 * x + 1], make_float2(c2, c2), make_float2(z.z, z.w))};
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            if (PART) {
+              const int c0 = c + 4 * x + 2 * y;
+              e[y].x = c0 >= c_lo && c0 < c_hi ? e[y].x : -INFINITY;
+              e[y].y = c0 + 1 >= c_lo && c0 + 1 < c_hi ? e[y].y : -INFINITY;
+            }
+            sum[y] = fadd2(sum[y], make_float2(exp2_approx(e[y].x), exp2_approx(e[y].y)));
+          }
+        }
+      }
+      return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+    };
+    int it = 0, gave[WGS] = {}, took[WGS] = {};  // tiles; parts given at each place, and taken from it
     bool ok = true;
     for (int i = 0; ok && next_job(i); ++i) {
       const Job& j = jobs[i % JOBS];
-      const int tiles = j.tiles, key = j.kt * KEYS + t, ahead = j.L - j.n, t0 = j.t0, n = j.n;
-      float* w = a.weights + j.seq * a.w_stride_seq + j.h * a.w_stride_head + key;
-      // the warpgroup of the job's first tile writes its weights
-      const bool writes = (it & 1) == wg;
-      float old = 0.f;
-      if (writes && key < j.L && key < ahead) old = *w;
-      float sum = 0.f, low = 0.f, c2 = 0.f;  // the sum and what its rounding lost
-      for (int tile = 0; tile < tiles; ++tile, ++it) {
-        if ((it & 1) != wg) continue;
-        const int b = it % SB;
-        ok = wait_warp(&s_full[b], it / SB);
-        if (!ok) break;
-        tc_fence_after();
-        if (tile < 2) c2 = a.softmax_scale * kLog2e * j.scale[t >> 4];
-        // columns of queries that are there and see the key
-        const int tok = t0 + tile / ht * tb;
-        const int c_lo = max(key - ahead - tok, 0) * hb, c_hi = min(n - tok, tb) * hb;
-        const bool partial = tok + tb > n || j.kt * KEYS + KEYS - 1 > ahead + tok;  // uniform
-        const float4* zs = reinterpret_cast<const float4*>(sm + C::Z_OFF + b * N * 4);
-        float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        constexpr int W = N < 32 ? N : 32;
+      const int ahead = j.L - j.n, n = j.n, nk = j.nk, L = j.L;
+      int z_at = -1;  // the first query of the tile whose lse this warpgroup has, where it is its keys' only one
 #pragma unroll 1
-        for (int c = 0; c < N; c += W) {
-          float2 v[W / 2];
-          if (W == 32) tmem_ld32(b * N + c + lane_base, reinterpret_cast<float*>(v));
-          else tmem_ld16(b * N + c + lane_base, reinterpret_cast<float*>(v));
-          tmem_wait_ld();
+      for (int x = 0; x < nk; ++x) {
+        const int key = (j.kt + x) * KEYS + t, t0 = j.t0[x], tiles = j.tiles[x];
+        // The warpgroups take the tiles in turn; this one has the unit's tiles
+        // place, place + WGS, ... The first place writes the weights.
+        const int place = (wg - it) & (WGS - 1), it0 = it;
+        it += tiles;
+        if (place >= tiles) continue;
+        float* w = a.weights + j.seq * a.w_stride_seq + j.h * a.w_stride_head + key;
+        float old = 0.f;
+        if (place == 0 && key < min(L, ahead)) old = *w;
+        const bool again = tiles == 1 && z_at == t0;
+        z_at = tiles == 1 ? t0 : -1;
+        float z = 0.f;
+        if (!again) {
+          store_lse(load_lse(j, t0, place));
+          if (place + WGS < tiles) z = load_lse(j, t0, place + WGS);
+        }
+        float sum = 0.f, low = 0.f, c2 = 0.f;  // the sum, and what its rounding lost
+#pragma unroll 1
+        for (int tile = place; tile < tiles; tile += WGS) {
+          if (!again) ok = wait_warp(&z_full[wg], z_seen++);
+          if (tile + WGS < tiles) {  // the lse of this warpgroup's next tile, and the load of the one's behind it
+            store_lse(z);
+            if (tile + 2 * WGS < tiles) z = load_lse(j, t0, tile + 2 * WGS);
+          }
+          const int b = (it0 + tile) % SB;
+          ok = ok && wait_warp(&s_full[b], (it0 + tile) / SB);
+          if (!ok) break;
+          tc_fence_after();
+          if (tile == place) c2 = a.softmax_scale * kLog2e * j.scale[x * (KEYS / 16) + (t >> 4)];
+          // columns of queries that are there and see the key
+          const int tok = tok_of(t0, tile), c_lo = max(key - ahead - tok, 0) * hb, c_hi = min(n - tok, tb) * hb;
+          const bool part = N == 16 || tok + tb > n || key - t + KEYS - 1 > ahead + tok;  // uniform; few columns: always
+          const float p = (part ? add_up(std::true_type(), b, c2, c_lo, c_hi) : add_up(std::false_type(), b, c2, 0, 0)) + low, next = sum + p;
+          tc_fence_before();
+          mbar_arrive(&s_empty[b]);
+          low = p - (next - sum);
+          sum = next;
+        }
+        if (!ok) break;
+        // the other places' parts, in their order; every pair of warpgroups has a buffer
 #pragma unroll
-          for (int x = 0; x < W / 4; ++x) {
-            const float4 z = zs[c / 4 + x];
-            float2 e0 = ffma2(v[2 * x], make_float2(c2, c2), make_float2(z.x, z.y));
-            float2 e1 = ffma2(v[2 * x + 1], make_float2(c2, c2), make_float2(z.z, z.w));
-            if (partial) {
-              const int c0 = c + 4 * x;
-              e0.x = c0 >= c_lo && c0 < c_hi ? e0.x : -INFINITY;
-              e0.y = c0 + 1 >= c_lo && c0 + 1 < c_hi ? e0.y : -INFINITY;
-              e1.x = c0 + 2 >= c_lo && c0 + 2 < c_hi ? e1.x : -INFINITY;
-              e1.y = c0 + 3 >= c_lo && c0 + 3 < c_hi ? e1.y : -INFINITY;
-            }
-            part[0] = fadd2(part[0], make_float2(exp2_approx(e0.x), exp2_approx(e0.y)));
-            part[1] = fadd2(part[1], make_float2(exp2_approx(e1.x), exp2_approx(e1.y)));
+        for (int y = 1; y < WGS; ++y) {
+          if (tiles <= y || (place != 0 && place != y)) continue;
+          const int pair = (place == 0 ? wg : (wg - y) & (WGS - 1)) * (WGS - 1) + y - 1;
+          if (place == y) {
+            ok = ok && wait_warp(&red_empty[pair], gave[y] + 1);
+            if (!ok) break;
+            red[pair * KEYS + t] = sum;
+            mbar_arrive(&red_full[pair]);
+            ++gave[y];
+          } else {
+            ok = ok && wait_warp(&red_full[pair], took[y]);
+            if (!ok) break;
+            sum += red[pair * KEYS + t];
+            mbar_arrive(&red_empty[pair]);
+            ++took[y];
           }
         }
-        tc_fence_before();
-        mbar_arrive(&s_empty[b]);
-        const float p = (part[0].x + part[0].y) + (part[1].x + part[1].y) + low, next = sum + p;
-        low = p - (next - sum);
-        sum = next;
+        if (!ok) break;
+        if (place == 0 && key < L) *w = old + sum;
       }
-      if (!ok) break;
-      if (tiles > 1) {  // the other warpgroup's part
-        if (!writes) {
-          ok = wait_warp(red_empty, joined + 1);
-          if (!ok) break;
-          red[t] = sum;
-          mbar_arrive(red_full);
-        } else {
-          ok = wait_warp(red_full, joined);
-          if (!ok) break;
-          sum += red[t];
-          mbar_arrive(red_empty);
-        }
-        ++joined;
-      }
-      if (writes && key < j.L) *w = old + sum;
-      done_job(i);
+      if (ok) done_job(i);
     }
     tc_fence_before();
   }
@@ -527,7 +613,7 @@ static cudaError_t launch_t(const mj_block_weigh_args& a, cudaStream_t stream) {
            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
       return cudaErrorInvalidValue;
   }
-  return launch_kernel(kern, dim3((unsigned)sms), dim3(THREADS), C::SMEM, stream, a, block_log2(a.kv_format), hb, tb, ht, mk, mq);
+  return launch_kernel(kern, dim3((unsigned)sms), dim3(C::THREADS), C::SMEM, stream, a, block_log2(a.kv_format), hb, tb, ht, mk, mq);
 }
 
 template <typename T>
