@@ -19,9 +19,10 @@
 // take the jobs in rounds, every other round in reverse: a prompt's first keys
 // are seen by all its rows, its last by few.
 //
-// Warp roles: 0 K (page walk, TMA, block scales), 1 Q (TMA), 2 MMA,
-// 3 the jobs; then warpgroups that convert K's codes, in turn, and warpgroups that
-// take the S tiles in turn and add up. Every mbarrier wait is bounded; on a timeout the CTA flags
+// Warp roles: 0 K (page walk, TMA, block scales; where few rows see a tile, four
+// warps of their own behind the others), 1 Q (TMA), 2 MMA, 3 the jobs; then
+// warpgroups that convert K's codes, in turn, and warpgroups that take the S tiles
+// in turn and add up. Every mbarrier wait is bounded; on a timeout the CTA flags
 // MJ_DEV_TIMEOUT, all roles stop, copies and MMAs in flight complete and TMEM is
 // freed.
 #include <limits.h>
@@ -60,6 +61,7 @@ constexpr int kTiles = N >= 64 ? 1 : 4;
 struct Job {
   int seq, h, kt, nk, L, n, q0;  // seq < 0: no more; nk tiles of keys from kt on
   int t0[4], tiles[4];           // of each: the first query that counts and sees one of them, tiles of rows from it on
+  int one;                       // they have one tile of rows, the same
   float scale[4 * (KEYS / 16)];
 };
 
@@ -71,11 +73,14 @@ struct Cfg {
   // exponentials bound it, and two or four warps on a scheduler must hide one
   // another's latency (8192 tokens, 32 / 8 heads: 376 us with two warpgroups, 341
   // with four). Few rows: every tile of keys is converted for one product.
-  static constexpr int CWGS = WIDE || D == 256 ? 1 : 2, WGS = WIDE ? 4 : 2, THREADS = 128 * (1 + CWGS + WGS);
+  static constexpr int CWGS = WIDE ? 1 : 2, WGS = WIDE ? 4 : 2;
+  // Warps that fetch K. A lane's copies are issued one after another, over 100
+  // cycles each; with pages of 16 a tile has eight, and HBM has brought it in 700.
+  static constexpr int KWARPS = WIDE ? 1 : 4, K0 = WIDE ? 0 : 4 * (1 + CWGS + WGS), THREADS = 128 * (1 + CWGS + WGS) + (WIDE ? 0 : 128);
   // stages of K codes, of K in 16 bits, of Q
-  static constexpr int RS = WIDE ? (D == 256 ? 1 : 2) : D == 256 ? 3 : 8, KS = D == 256 ? 1 : 2, QS = WIDE ? 3 : 4;
+  static constexpr int RS = WIDE ? (D == 256 ? 1 : 2) : D == 256 ? 2 : 4, KS = WIDE ? (D == 256 ? 1 : 2) : D == 256 ? 2 : 4, QS = D == 256 ? 2 : WIDE ? 3 : 4;
   static constexpr int SB = 4;  // S buffers in TMEM; a warpgroup that adds up has three of its columns' lse
-  static constexpr int JOBS = 4;
+  static constexpr int JOBS = WIDE ? 4 : 8;
   static constexpr int PAIRS = WGS * (WGS - 1);  // of a warpgroup that writes weights and one that adds its part
   static constexpr int K_OFF = 0, R_OFF = K_OFF + KS * K16, Q_OFF = R_OFF + RS * RAW, Z_OFF = Q_OFF + QS * QST;
   static constexpr int RED_OFF = Z_OFF + 3 * WGS * N * 4, JOB_OFF = RED_OFF + PAIRS * KEYS * 4, BAR_OFF = JOB_OFF + JOBS * (int)sizeof(Job);
@@ -145,7 +150,7 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
     init(s_full, SB, 2);  // the product, and its issuer (who saw the job's scales)
     init(s_empty, SB, 128);
     init(j_full, JOBS, 1);
-    init(j_empty, JOBS, 3 + 4 * (CWGS + WGS));  // the K, Q and MMA warps, those that convert, those that add up
+    init(j_empty, JOBS, 2 + C::KWARPS + 4 * (CWGS + WGS));  // the Q, MMA and K warps, those that convert, those that add up
     init(red_full, C::PAIRS, 128);
     init(red_empty, C::PAIRS, 128);
     init(z_full, WGS, 128);
@@ -266,16 +271,19 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
           j.t0[x] = max(a.window ? max(n - a.window, 0) : 0, (j.kt + x) * KEYS - (L - n));
           j.tiles[x] = (n - j.t0[x] + tb - 1) / tb * ht;
         }
+        j.one = j.tiles[0] == 1 && j.t0[j.nk - 1] == j.t0[0];  // (t0 grows with x)
         mbar_arrive(&j_full[i % JOBS]);
       }
       __syncwarp();
     }
-  } else if (warp == 0) {
+  } else if (warp >= C::K0 && warp < C::K0 + C::KWARPS) {
     // -------------------------------------------------------- K: codes and scales
+    // Every K warp looks up all pages and copies its share of each tile's.
     // Lane i looks up the page of the job's 16-token group i two jobs ahead and
     // reads its exponent one job ahead (a use at once would wait for memory).
     constexpr int kNone = INT_MIN;
     const uint64_t policy = l2_policy_evict_normal();
+    const int kw = warp - C::K0;
     const int ps = a.page_size, lps = 31 - __clz(ps), groups = max(ps / 16, 1), pages = KEYS / ps;
     auto entry_of = [&](const Job& j) {
       const int pos = j.kt * KEYS + lane * 16;
@@ -299,7 +307,7 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
     for (; ok && here; ++i) {
       Job& j = jobs[i % JOBS];
       const int nk = j.nk, h = j.h;
-      j.scale[lane] = block_scale(ex);
+      if (kw == 0) j.scale[lane] = block_scale(ex);
       const int page1 = page_of(e1);
       const unsigned char ex1 = ahead ? exponent_of(jobs[(i + 1) % JOBS], page1) : 127;
       const bool ahead2 = ahead && next_job(i + 2);
@@ -308,10 +316,10 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
       for (int x = 0; x < nk; ++x, ++u) {
         ok = wait_warp(&r_empty[u % RS], u / RS + 1);
         if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(&r_full[u % RS], C::RAW);
+        if (kw == 0 && lane == 0) mbar_arrive_expect_tx(&r_full[u % RS], C::RAW);  // (whichever comes first, this or another warp's copies)
         __syncwarp();
         const int pg = __shfl_sync(0xffffffffu, page, (x * (KEYS / 16) + lane * groups) & 31);
-        if (lane < pages) {
+        if (lane < pages && lane % C::KWARPS == kw) {
 #pragma unroll
           for (int dh = 0; dh < D / 128; ++dh)  // an absent page is read out of range: zeros
             tma_load_5d(sm + C::R_OFF + (u % RS) * C::RAW + dh * (KEYS * 128) + lane * ps * 128, &tmk, &r_full[u % RS], 0, dh, 0, h,
@@ -335,7 +343,7 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
     bool ok = true;
     for (int i = 0; ok && next_job(i); ++i) {
       const Job& j = jobs[i % JOBS];
-      const int nk = j.nk, h = j.h, n = j.n, q0 = j.q0;
+      const int nk = j.one ? 1 : j.nk, h = j.h, n = j.n, q0 = j.q0;
       for (int x = 0; ok && x < nk; ++x)
         for (int tok = j.t0[x], head = 0; tok < n; ++it) {
           const int s = it % QS;
@@ -357,45 +365,61 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
     // ---------------------------------------------------------------------- MMA
     constexpr uint32_t idesc = std::is_same<T, __half>::value ? idesc_f16(0, 0, N) : idesc_bf16(0, 0, N);
     const bool lead = elect_one();
-    int it = 0, u = 0;
+    int it = 0, u = 0, iq = 0;  // S tiles, K tiles, Q tiles
     bool ok = true;
-    auto ready = [&]() { return wait_warp(&q_full[it % QS], it / QS) && wait_warp(&s_empty[it % SB], it / SB + 1); };  // tile `it`
     for (int i = 0; ok && next_job(i); ++i) {
       const Job& j = jobs[i % JOBS];
-      for (int x = 0, nk = j.nk; ok && x < nk; ++x, ++u) {
-        const int tiles = j.tiles[x];
-        ok = wait_warp(&k_full[u % KS], u / KS) && ready();
-        const uint64_t k = smem_desc_sw128(smem_addr(sm + C::K_OFF + (u % KS) * C::K16), 16, 1024);
-        for (int tile = 0; ok && tile < tiles; ++tile) {
-          const int b = it % SB, s = it % QS;
-          tc_fence_after();
-          const uint64_t q = smem_desc_sw128(smem_addr(sm + C::Q_OFF + s * C::QST), 16, 1024);
-          auto steps = [&](auto half) {  // 16 head-dim elements a step
-            constexpr int H = decltype(half)::value;
-            if (lead) {
-#pragma unroll
-              for (int y = H * (D / 32); y < (H + 1) * (D / 32); ++y)
-                mma_f16(b * N, k + y / 4 * (KEYS * 8) + y % 4 * 2, q + y / 4 * (N * 8) + y % 4 * 2, idesc, y > 0);
-            }
-          };
-          steps(std::integral_constant<int, 0>());
-          // the waits for the next tile pass while these products run
-          ++it;
-          if (tile + 1 < tiles) ok = ready();
-          steps(std::integral_constant<int, 1>());
+      const int nk = j.nk;
+      const bool one = j.one;
+      int x = 0, tile = 0, tiles = j.tiles[0];
+      // everything that the tile at hand needs
+      auto ready = [&]() {
+        return (tile > 0 || wait_warp(&k_full[u % KS], u / KS)) && ((one && x > 0) || wait_warp(&q_full[iq % QS], iq / QS)) &&
+               wait_warp(&s_empty[it % SB], it / SB + 1);
+      };
+      ok = ready();
+      while (ok && x < nk) {
+        const int b = it % SB, s = iq % QS, ku = u % KS;
+        const bool last_k = tile + 1 == tiles, last_q = !one || x + 1 == nk;  // uses of the K tile, of the Q tile
+        tc_fence_after();
+        const uint64_t k = smem_desc_sw128(smem_addr(sm + C::K_OFF + ku * C::K16), 16, 1024);
+        const uint64_t q = smem_desc_sw128(smem_addr(sm + C::Q_OFF + s * C::QST), 16, 1024);
+        auto steps = [&](auto half) {  // 16 head-dim elements a step
+          constexpr int H = decltype(half)::value;
           if (lead) {
-            mma_commit(&s_full[b]);
-            mbar_arrive(&s_full[b]);
-            mma_commit(&q_empty[s]);
-            if (tile + 1 == tiles) mma_commit(&k_empty[u % KS]);
+#pragma unroll
+            for (int y = H * (D / 32); y < (H + 1) * (D / 32); ++y)
+              mma_f16(b * N, k + y / 4 * (KEYS * 8) + y % 4 * 2, q + y / 4 * (N * 8) + y % 4 * 2, idesc, y > 0);
           }
-          __syncwarp();
+        };
+        steps(std::integral_constant<int, 0>());
+        // The waits for the keys' next tile pass while these products run. Not those
+        // for other keys: this tile's K buffer would be free only after they are there.
+        ++it;
+        iq += last_q;
+        ++tile;
+        if (last_k) {
+          tile = 0;
+          ++u;
+          if (++x < nk) tiles = j.tiles[x];
         }
+        if (!last_k) ok = ready();
+        steps(std::integral_constant<int, 1>());
+        if (lead) {
+          mma_commit(&s_full[b]);
+          mbar_arrive(&s_full[b]);
+          if (last_q) mma_commit(&q_empty[s]);
+          if (last_k) mma_commit(&k_empty[ku]);
+        }
+        __syncwarp();
+        if (last_k && x < nk) ok = ready();
       }
       if (ok) done_job(i);
     }
     if (lead) mma_commit(drain);  // all issued MMAs complete before TMEM is released
     mbar_wait(drain, 0, &never_abort, kWaitNs);
+  } else if (warp == 0) {
+    // (K has warps of its own)
   } else if (warp < 4 + 4 * CWGS) {
     // ------------------------------------------------------------ codes -> 16 bits
     // Thread ct takes 16-code chunk 4 blk + quad of rows r0, r0 + STEP, ...: eight
@@ -621,7 +645,7 @@ static cudaError_t launch_d(const mj_block_weigh_args& a, cudaStream_t stream) {
   // rows of a sequence and KV head that count, on average
   const int64_t all = a.num_rows * (a.h_q / a.h_k), most = a.window ? (int64_t)a.num_seqs * a.window * (a.h_q / a.h_k) : all;
   const bool few = (all < most ? all : most) <= (int64_t)32 * a.num_seqs;
-  if (a.head_size == 256) return few ? launch_t<T, 256, 16>(a, stream) : launch_t<T, 256, 64>(a, stream);
+  if (a.head_size == 256) return few ? launch_t<T, 256, 16>(a, stream) : launch_t<T, 256, 96>(a, stream);
   return few ? launch_t<T, 128, 16>(a, stream) : launch_t<T, 128, 128>(a, stream);
 }
 
