@@ -15,13 +15,6 @@
 
 namespace mj {
 
-// Pages need not be powers of two, and a 64-bit division is a long routine: a
-// quotient x / n is the high half of x * ceil(2^64 / n), exact while x * n <
-// 2^64 and never too small. Blocks of a page: n <= 2^16, x < 2^47; rows of a
-// page: n <= 2^20, x < 2^33. For n = 1 the multiplier wraps to 0.
-static uint64_t reciprocal(int n) { return ~0ull / (uint64_t)n + 1; }
-__device__ __forceinline__ int64_t quotient(int64_t x, uint64_t rec) { return rec ? (int64_t)__umul64hi((uint64_t)x, rec) : x; }
-
 // The largest magnitude of a lane's chunks, NaN left out. 16-bit values are
 // compared in pairs: two instructions a pair.
 template <int NB>

@@ -25,6 +25,13 @@ __device__ __forceinline__ int block_exponent(float amax) {
   return min(max(e, MJ_BLOCK_E_MIN), MJ_BLOCK_E_MAX);
 }
 
+// Pages need not be powers of two, and a 64-bit division is a long routine: a
+// quotient x / n is the high half of x * ceil(2^64 / n), exact while x * n <
+// 2^64 and never too small. Blocks of a page: n <= 2^16, x < 2^47; rows of a
+// page: n <= 2^20, x < 2^33. For n = 1 the multiplier wraps to 0.
+inline uint64_t reciprocal(int n) { return ~0ull / (uint64_t)n + 1; }
+__device__ __forceinline__ int64_t quotient(int64_t x, uint64_t rec) { return rec ? (int64_t)__umul64hi((uint64_t)x, rec) : x; }
+
 // 8 elements to a 16-byte aligned address
 __device__ __forceinline__ void store8(float* p, const float* v) {
   reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);

@@ -4,40 +4,40 @@
 // A cluster of CTAs takes one (sequence, KV head).
 // 1. The m-th largest weight (m = budget - recent) by radix selection: weights
 //    as unsigned keys of the same order, three passes over 11, 11 and 10 of
-//    their bits, each a histogram of the keys that agree so far.
+//    their bits, each a histogram of the keys that agree so far. Every CTA adds
+//    up the cluster's histograms for itself, in vectors.
 // 2. The kept tokens in order: those above that key, the first of those equal
-//    to it, the recent ones. A CTA takes a contiguous part of the tokens; what
-//    the parts before it keep is summed over the cluster.
+//    to it, the recent ones. A CTA takes a contiguous part of the tokens, a
+//    thread a contiguous part of that; what the parts before it keep is summed
+//    over the block, then over the cluster.
 // 3. The rows move. Position i receives token kept[i] >= i, so a step that
 //    reads all its tokens before it writes, and steps in ascending order, work
 //    in place: rows from i on are not read by the steps before. A step is 128
 //    positions a CTA, whole blocks of scales; the cluster's barrier lies
 //    between its reads and its writes, and the next step's reads (of rows that
-//    this one's writes are below) are on their way meanwhile.
+//    this one's writes are below) are on their way into registers meanwhile.
 #include <cooperative_groups.h>
 #include <math.h>
+
+#include <algorithm>
+#include <atomic>
+#include <mutex>
 
 #include "block_cache.cuh"
 
 namespace mj {
+
+std::mutex& tc_init_mutex();
 
 namespace cg = cooperative_groups;
 using namespace sm100;
 
 namespace ev {
 
-constexpr int THREADS = 512, WARPS = THREADS / 32;
-constexpr int STEP = 128;    // positions of a CTA's step
-constexpr int BINS = 2048;   // of a radix pass
-
-__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
+constexpr int STEP = 128;   // positions of a CTA's step
+constexpr int AHEAD = 8;    // steps whose positions are looked up together
+constexpr int BINS = 2048;  // of a radix pass
+constexpr int PER = 8;      // tokens of a thread in a segment of the selection
 
 // Weights in their order as unsigned keys; -0 is 0, NaN above all.
 __device__ __forceinline__ uint32_t key_of(float w) {
@@ -46,20 +46,28 @@ __device__ __forceinline__ uint32_t key_of(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// A position's source and destination: page and row of each
+struct Move {
+  int src_page, src_row, dst_page, dst_row;
+};
+
 template <int D>
-struct Smem {
-  unsigned char rows[2][STEP][2 * D];  // a step's K | V rows
-  float w[2][STEP];
-  unsigned char e[2][2][STEP];         // [buffer][side]: their exponent bytes
-  int hist[BINS];
-  int e_new[2][STEP / 16];             // [side][block]
-  int scan[WARPS + 1];
-  int pick[2];                         // a radix pass's bin, and how many are above it
-  int parts[2];                        // this CTA's tokens above the threshold, and equal to it
-  int bad;
+struct Cfg {
+  static constexpr int THREADS = D == 256 ? 1024 : 512, WARPS = THREADS / 32;  // a thread has four 16-byte chunks of a step
+  struct Smem {
+    Move moves[AHEAD * STEP];
+    float w[AHEAD * STEP];
+    unsigned char e[2][AHEAD * STEP];  // [side]: exponent bytes of the sources
+    int hist[3][BINS];                 // of the passes
+    int amax[3][2][STEP / 16];         // [step % 3][side][block]: largest magnitude of its rows, as bits
+    int scan[WARPS + 1];
+    int pick[2];                       // a pass's bin, and how many are above it
+    int parts[2];                      // this CTA's tokens above the threshold, and equal to it
+  };
 };
 
 // Inclusive sums over the block; `total` of all of them.
+template <int WARPS>
 __device__ __forceinline__ int block_scan(int v, int* scan, int& total) {
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
 #pragma unroll
@@ -70,37 +78,46 @@ __device__ __forceinline__ int block_scan(int v, int* scan, int& total) {
   __syncthreads();  // scan's last readers are done
   if (lane == 31) scan[wid] = v;
   __syncthreads();
-  int below = 0;
-  total = 0;
+  int x = lane < WARPS ? scan[lane] : 0;
 #pragma unroll
-  for (int i = 0; i < WARPS; ++i) {
-    const int x = scan[i];
-    below += i < wid ? x : 0;
-    total += x;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
   }
-  return v + below;
+  total = __shfl_sync(0xffffffffu, x, 31);
+  const int below = __shfl_sync(0xffffffffu, x, wid ? wid - 1 : 0);
+  return v + (wid ? below : 0);
+}
+
+// the largest magnitude code of 16, NaN left out
+__device__ __forceinline__ uint32_t max_code(uint4 c) {
+  drop_nan_codes(c);
+  uint32_t m = __vmaxu4(__vmaxu4(c.x & 0x7F7F7F7Fu, c.y & 0x7F7F7F7Fu), __vmaxu4(c.z & 0x7F7F7F7Fu, c.w & 0x7F7F7F7Fu));
+  m = __vmaxu4(m, m >> 16);
+  return max(m & 0xFFu, m >> 8 & 0xFFu);
 }
 
 template <int D>
-__global__ void __launch_bounds__(THREADS) block_evict_kernel(const __grid_constant__ mj_block_evict_args a, int lg) {
+__global__ void __launch_bounds__(Cfg<D>::THREADS, D == 256 ? 1 : 2)
+    block_evict_kernel(const __grid_constant__ mj_block_evict_args a, int lg, uint64_t per_page) {
+  constexpr int THREADS = Cfg<D>::THREADS, WARPS = Cfg<D>::WARPS, SEG = PER * THREADS;
   extern __shared__ __align__(16) unsigned char raw[];
-  Smem<D>& sm = *reinterpret_cast<Smem<D>*>(raw);
+  auto& sm = *reinterpret_cast<typename Cfg<D>::Smem*>(raw);
   auto cluster = cg::this_cluster();
   const int CL = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int job = blockIdx.x / CL, h = job % a.h_k, seq = job / a.h_k;
-  const int t = threadIdx.x, lane = t & 31, wid = t >> 5;
+  const int t = threadIdx.x;
   griddep_wait();
   const int L = a.seq_lens[seq], budget = a.budget;
   int32_t* kept = a.kept + ((int64_t)seq * a.h_k + h) * budget;
   const bool cut = L > budget;
-  const int64_t G = 1 << lg;
   // pages that hold a token, looked at before anything is written; the same
   // answer in every CTA and for every head
   const int32_t* table = a.block_table + seq * a.block_table_stride;
   bool bad = L < 0 || L > a.weights_cols || L > (int64_t)a.block_table_cols * a.page_size;
   if (bad && t == 0 && rank == 0) flag(a.status, MJ_DEV_BAD_LENGTH);
   if (!bad && cut) {
-    const int pages = (int)((L + (int64_t)a.page_size - 1) / a.page_size);
+    const int pages = (int)quotient(L - 1, per_page) + 1;
     int missing = 0;
     for (int i = t; i < pages; i += THREADS) missing |= (unsigned)table[i] >= (uint64_t)a.num_pages;
     bad = __syncthreads_or(missing);
@@ -117,32 +134,53 @@ __global__ void __launch_bounds__(THREADS) block_evict_kernel(const __grid_const
   // ---- 1. the threshold
   const int M = L - a.recent, m = budget - a.recent;  // 0 <= m < M
   const int part = (M + CL - 1) / CL, t0 = min(rank * part, M), t1 = min(t0 + part, M);
+  // this thread's tokens of the segment that begins at s0; of a part of one
+  // segment they stay in registers for all passes
+  uint32_t key[PER];
+  const int per = min((part + THREADS - 1) / THREADS, PER), seg = per * THREADS;
+  auto load_keys = [&](int s0) {
+#pragma unroll
+    for (int x = 0; x < PER; ++x) {
+      const int i = s0 + t * per + x;
+      key[x] = x < per && i < t1 ? key_of(w[i]) : 0u;
+    }
+  };
+  // tokens of them that are there
+  auto count_of = [&](int s0) { return min(max(t1 - s0 - t * per, 0), per); };
   uint32_t prefix = 0;  // the threshold's bits so far
   int above = 0;        // keys that are larger than any with these bits
   if (m > 0) {
+    for (int i = t; i < 3 * BINS; i += THREADS) sm.hist[0][i] = 0;
+    load_keys(t0);
+    __syncthreads();
     int shift = 32;
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
       const int bits = pass < 2 ? 11 : 10;
       const uint32_t known = pass ? ~0u << shift : 0u;
       shift -= bits;
-      for (int i = t; i < BINS; i += THREADS) sm.hist[i] = 0;
-      __syncthreads();
-      for (int i = t0 + t; i < t1; i += THREADS) {
-        const uint32_t k = key_of(w[i]);
-        if ((k & known) == prefix) atomicAdd(&sm.hist[(k >> shift) & ((1u << bits) - 1u)], 1);
+      int* hist = sm.hist[pass];
+      for (int s0 = t0; s0 < t1; s0 += seg) {
+        if (part > seg) load_keys(s0);
+        const int n = count_of(s0);
+#pragma unroll
+        for (int x = 0; x < PER; ++x)
+          if (x < n && (key[x] & known) == prefix) atomicAdd(&hist[(key[x] >> shift) & ((1u << bits) - 1u)], 1);
       }
       cluster.sync();
-      // four bins a thread, from the largest down
-      int c[4], sum = 0;
+      // four bins a thread, from the largest down; all CTAs' on their way together
+      int c[4] = {0, 0, 0, 0};
+      if (t < BINS / 4) {
+        int4 v[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        c[i] = 0;
-        for (int r = 0; r < CL; ++r) c[i] += cluster.map_shared_rank(sm.hist, r)[BINS - 1 - (4 * t + i)];
-        sum += c[i];
+        for (int r = 0; r < 8; ++r)
+          v[r] = r < CL ? reinterpret_cast<const int4*>(cluster.map_shared_rank(hist, r))[BINS / 4 - 1 - t] : make_int4(0, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) c[0] += v[r].w, c[1] += v[r].z, c[2] += v[r].y, c[3] += v[r].x;
       }
       int total;
-      int before = block_scan(sum, sm.scan, total) - sum + above;
+      const int sum = c[0] + c[1] + c[2] + c[3];
+      int before = block_scan<WARPS>(sum, sm.scan, total) - sum + above;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (before < m && before + c[i] >= m) {
@@ -151,25 +189,31 @@ __global__ void __launch_bounds__(THREADS) block_evict_kernel(const __grid_const
         }
         before += c[i];
       }
-      cluster.sync();  // histograms are read, the pick is written
+      __syncthreads();
       prefix |= (uint32_t)sm.pick[0] << shift;
       above = sm.pick[1];
-      __syncthreads();
     }
   }
   const int ties = m - above;  // tokens of exactly the threshold's key to keep
 
   // ---- 2. the kept tokens, in order
   if (m > 0) {
-    int gt = 0, eq = 0;
-    for (int i = t0 + t; i < t1; i += THREADS) {
-      const uint32_t k = key_of(w[i]);
-      gt += k > prefix;
-      eq += k == prefix;
+    auto tally = [&](int s0) {  // above the threshold in the low half, equal to it in the high half
+      const int n = count_of(s0);
+      int v = 0;
+#pragma unroll
+      for (int x = 0; x < PER; ++x) v += x < n ? (key[x] > prefix) + ((key[x] == prefix) << 16) : 0;
+      return v;
+    };
+    int n_gt = 0, n_eq = 0, mine = 0, incl = 0;
+    for (int s0 = t0; s0 < t1; s0 += seg) {
+      if (part > seg) load_keys(s0);
+      int total;
+      mine = tally(s0);
+      incl = block_scan<WARPS>(mine, sm.scan, total);
+      n_gt += total & 0xFFFF;
+      n_eq += total >> 16;
     }
-    int n_gt, n_eq;
-    block_scan(gt, sm.scan, n_gt);
-    block_scan(eq, sm.scan, n_eq);
     if (t == 0) {
       sm.parts[0] = n_gt;
       sm.parts[1] = n_eq;
@@ -180,98 +224,135 @@ __global__ void __launch_bounds__(THREADS) block_evict_kernel(const __grid_const
       base_gt += cluster.map_shared_rank(sm.parts, r)[0];
       base_eq += cluster.map_shared_rank(sm.parts, r)[1];
     }
-    for (int i0 = t0; i0 < t1; i0 += THREADS) {
-      const int i = i0 + t;
-      const uint32_t k = i < t1 ? key_of(w[i]) : 0u;
-      const int is_gt = i < t1 && k > prefix, is_eq = i < t1 && k == prefix;
-      int s_gt, s_eq;
-      const int up_gt = block_scan(is_gt, sm.scan, s_gt) + base_gt, up_eq = block_scan(is_eq, sm.scan, s_eq) + base_eq;
-      if (is_gt || (is_eq && up_eq <= ties)) kept[up_gt + min(up_eq, ties) - 1] = i;
-      base_gt += s_gt;
-      base_eq += s_eq;
+    for (int s0 = t0; s0 < t1; s0 += seg) {
+      if (part > seg) {
+        int total;
+        load_keys(s0);
+        mine = tally(s0);
+        incl = block_scan<WARPS>(mine, sm.scan, total);
+        n_gt = total & 0xFFFF;
+        n_eq = total >> 16;
+      }
+      const int n = count_of(s0);
+      int gt = base_gt + (incl & 0xFFFF) - (mine & 0xFFFF), eq = base_eq + (incl >> 16) - (mine >> 16);
+#pragma unroll
+      for (int x = 0; x < PER; ++x) {
+        if (x >= n) break;
+        if (key[x] > prefix || (key[x] == prefix && eq < ties)) kept[gt + min(eq, ties)] = s0 + t * per + x;
+        gt += key[x] > prefix;
+        eq += key[x] == prefix;
+      }
+      base_gt += n_gt;
+      base_eq += n_eq;
     }
   }
   for (int i = rank * THREADS + t; i < a.recent; i += CL * THREADS) kept[m + i] = M + i;
   cluster.sync();
 
   // ---- 3. the rows move
-  constexpr int CPR = 2 * D / 16;  // 16-byte chunks of a K | V row
+  constexpr int SIDE = D / 16, CPR = 2 * SIDE;  // 16-byte chunks of a K or V row, of both
+  static_assert(STEP * CPR == 4 * THREADS, "four chunks a thread");
   const int steps = (budget + STEP * CL - 1) / (STEP * CL);
-  auto fetch = [&](int step) {
-    const int p0 = (step * CL + rank) * STEP, b = step & 1, count = min(max(budget - p0, 0), STEP);
-    for (int c = t; c < count * CPR; c += THREADS) {
-      const int i = c / CPR, u = c % CPR, src = kept[p0 + i], row = src % a.page_size, side = u >= CPR / 2;
-      const int page = table[src / a.page_size];
-      const unsigned char* from = side ? static_cast<const unsigned char*>(a.v_cache) + page * a.v_stride_page + row * a.v_stride_row + h * a.v_stride_head
-                                       : static_cast<const unsigned char*>(a.k_cache) + page * a.k_stride_page + row * a.k_stride_row + h * a.k_stride_head;
-      cp_async16(&sm.rows[b][i][u * 16], from + (u % (CPR / 2)) * 16);
-      if (u % (CPR / 2) == 0)
-        sm.e[b][side][i] = side ? static_cast<const unsigned char*>(a.v_scales)[page * a.vs_stride_page + (row >> lg) * a.vs_stride_block + h * a.vs_stride_head]
-                                : static_cast<const unsigned char*>(a.k_scales)[page * a.ks_stride_page + (row >> lg) * a.ks_stride_block + h * a.ks_stride_head];
-      if (u == 0) sm.w[b][i] = w[src];
+  const int u = t % CPR, side = u / SIDE;  // this thread's chunk of its four rows t / CPR, + 32, + 64, + 96
+  const int64_t sp = side ? a.v_stride_page : a.k_stride_page, sr = side ? a.v_stride_row : a.k_stride_row;
+  const int64_t ssp = side ? a.vs_stride_page : a.ks_stride_page, ssb = side ? a.vs_stride_block : a.ks_stride_block;
+  unsigned char* cache = static_cast<unsigned char*>(side ? a.v_cache : a.k_cache) + h * (side ? a.v_stride_head : a.k_stride_head) + u % SIDE * 16;
+  unsigned char* scales = static_cast<unsigned char*>(side ? a.v_scales : a.k_scales) + h * (side ? a.vs_stride_head : a.ks_stride_head);
+  auto first_of = [&](int step) { return (step * CL + rank) * STEP; };
+  // positions of the steps from `step` on: where they come from and go to, the
+  // sources' exponents and weights
+  auto look_up = [&](int step) {
+    for (int x = t; x < AHEAD * STEP; x += THREADS) {
+      const int p = first_of(step + x / STEP) + x % STEP;
+      if (step + x / STEP >= steps || p >= budget) break;
+      const int src = kept[p], sc = (int)quotient(src, per_page), dc = (int)quotient(p, per_page);
+      const Move v = {table[sc], src - sc * a.page_size, table[dc], p - dc * a.page_size};
+      sm.moves[x] = v;
+      sm.w[x] = w[src];
+      const int b = v.src_row >> lg;
+      sm.e[0][x] = static_cast<const unsigned char*>(a.k_scales)[v.src_page * a.ks_stride_page + b * a.ks_stride_block + h * a.ks_stride_head];
+      sm.e[1][x] = static_cast<const unsigned char*>(a.v_scales)[v.src_page * a.vs_stride_page + b * a.vs_stride_block + h * a.vs_stride_head];
     }
-    cp_async_commit();
   };
-  fetch(0);
+  uint4 now[4], next[4];
+  auto fetch = [&](int step, uint4* v) {
+    const int count = budget - first_of(step);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int i = t / CPR + x * (STEP / 4), at = step % AHEAD * STEP + i;
+      v[x] = make_uint4(0, 0, 0, 0);
+      if (step < steps && i < count) v[x] = *reinterpret_cast<const uint4*>(cache + sm.moves[at].src_page * sp + sm.moves[at].src_row * sr);
+    }
+  };
+  if (t < 3 * 2 * (STEP / 16)) sm.amax[0][0][t] = 0;
 #pragma unroll 1
   for (int step = 0; step < steps; ++step) {
-    const int p0 = (step * CL + rank) * STEP, b = step & 1, count = min(max(budget - p0, 0), STEP);
-    if (step + 1 < steps) fetch(step + 1);
-    else cp_async_commit();
-    cp_async_wait<1>();
-    __syncthreads();
-    // a block's exponent: the largest finite magnitude of its rows times their scales, by a warp per (side, block)
-    const int blocks = (int)((count + G - 1) >> lg);
-    for (int x = wid; x < 2 * blocks; x += WARPS) {
-      const int side = x / blocks, blk = x % blocks, r1 = min((blk + 1) << lg, count);
-      float amax = 0.f;
-      for (int c = lane; c < (r1 - (blk << lg)) * (D / 16); c += 32) {
-        const int i = (blk << lg) + c / (D / 16);
-        const uint4 q = *reinterpret_cast<const uint4*>(&sm.rows[b][i][side * D + (c % (D / 16)) * 16]);
-        const uint32_t v[4] = {q.x, q.y, q.z, q.w};
-        uint32_t most = 0;
+    if (step % AHEAD == 0) {  // (the last step has ended behind a barrier)
+      look_up(step);
+      __syncthreads();
+      fetch(step, now);
+    }
+    if ((step + 1) % AHEAD) fetch(step + 1, next);
+    const int p0 = first_of(step), count = budget - p0;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const uint32_t mag = v[k >> 2] >> (8 * (k & 3)) & 0x7Fu;
-          most = mag == 0x7Fu ? most : max(most, mag);
-        }
-        amax = fmaxf(amax, e4m3x2_to_f2((uint16_t)most).x * block_scale(sm.e[b][side][i]));
-      }
-      amax = warp_allmax(amax);
-      if (lane == 0) sm.e_new[side][blk] = block_exponent(amax);
+    for (int x = 0; x < 4; ++x) {  // the largest magnitudes of the step's blocks: by rows, then blocks
+      const int i = t / CPR + x * (STEP / 4), at = step % AHEAD * STEP + i;
+      uint32_t most = max_code(now[x]);
+#pragma unroll
+      for (int o = SIDE / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+      if (u % SIDE == 0 && i < count) atomicMax(&sm.amax[step % 3][side][i >> lg], __float_as_int(e4m3x2_to_f2((uint16_t)most).x * block_scale(sm.e[side][at])));
     }
     cluster.sync();  // every CTA of the cluster has read this step's tokens
-    for (int c = t; c < count * CPR; c += THREADS) {
-      const int i = c / CPR, u = c % CPR, pos = p0 + i, row = pos % a.page_size, side = u >= CPR / 2;
-      const int page = table[pos / a.page_size], e = sm.e_new[side][i >> lg];
-      const float f = __uint_as_float((uint32_t)(127 + block_e(sm.e[b][side][i]) - e) << 23);
-      uint4 q = *reinterpret_cast<const uint4*>(&sm.rows[b][i][u * 16]);
-      q = make_uint4(scale4(q.x, f), scale4(q.y, f), scale4(q.z, f), scale4(q.w, f));
-      unsigned char* to = side ? static_cast<unsigned char*>(a.v_cache) + page * a.v_stride_page + row * a.v_stride_row + h * a.v_stride_head
-                               : static_cast<unsigned char*>(a.k_cache) + page * a.k_stride_page + row * a.k_stride_row + h * a.k_stride_head;
-      *reinterpret_cast<uint4*>(to + (u % (CPR / 2)) * 16) = q;
-      if (u % (CPR / 2) == 0 && (i & (G - 1)) == 0) {
-        if (side) static_cast<unsigned char*>(a.v_scales)[page * a.vs_stride_page + (row >> lg) * a.vs_stride_block + h * a.vs_stride_head] = (unsigned char)e;
-        else static_cast<unsigned char*>(a.k_scales)[page * a.ks_stride_page + (row >> lg) * a.ks_stride_block + h * a.ks_stride_head] = (unsigned char)e;
+    if (t < 2 * (STEP / 16)) sm.amax[(step + 2) % 3][0][t] = 0;  // (read last before that barrier, and next behind another)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int i = t / CPR + x * (STEP / 4), at = step % AHEAD * STEP + i;
+      if (i < count) {
+        const Move v = sm.moves[at];
+        const int e = block_exponent(__int_as_float(sm.amax[step % 3][side][i >> lg]));
+        const float f = __uint_as_float((uint32_t)(127 + block_e(sm.e[side][at]) - e) << 23);
+        *reinterpret_cast<uint4*>(cache + v.dst_page * sp + v.dst_row * sr) =
+            make_uint4(scale4(now[x].x, f), scale4(now[x].y, f), scale4(now[x].z, f), scale4(now[x].w, f));
+        if (u % SIDE == 0 && (i & ((1 << lg) - 1)) == 0) scales[v.dst_page * ssp + (v.dst_row >> lg) * ssb] = (unsigned char)e;
       }
-      if (u == 0) w[pos] = sm.w[b][i];
+      now[x] = next[x];
     }
-    __syncthreads();  // this step's buffers are free
+    if (t < STEP && t < count) w[p0 + t] = sm.w[step % AHEAD * STEP + t];
+    if ((step + 1) % AHEAD == 0) __syncthreads();  // the looked-up positions are done with
   }
   cluster.sync();  // (no CTA leaves while another reads its shared memory)
 }
 
+constexpr int kMaxDevices = 64;
+
 template <int D>
 static cudaError_t launch_t(const mj_block_evict_args& a, cudaStream_t stream) {
   auto kern = block_evict_kernel<D>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem<D>));
+  constexpr int smem = (int)sizeof(typename Cfg<D>::Smem);
+  static std::atomic<int> ready[kMaxDevices];  // CTAs that the device holds at once, once the kernel is prepared on it
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+  int room = ready[dev].load(std::memory_order_acquire);
+  if (!room) {
+    std::lock_guard<std::mutex> lock(tc_init_mutex());
+    int sms = 0, per_sm = 0;
+    if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return e;
+    if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
+    if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, Cfg<D>::THREADS, smem)) != cudaSuccess) return e;
+    room = std::max(1, sms * per_sm);
+    ready[dev].store(room, std::memory_order_release);
+  }
+  // CTAs of a cluster: as many as fill the GPU once and find work, in steps of the
+  // rows that stay or segments of the weights
+  const int64_t jobs = (int64_t)a.num_seqs * a.h_k;
   int cl = 1;
-  while (cl < 8 && a.num_seqs * a.h_k * cl < 296 && cl * STEP < a.budget) cl *= 2;
+  while (cl < 8 && 2 * cl * jobs <= room && (cl * STEP < a.budget || (int64_t)cl * PER * Cfg<D>::THREADS < a.weights_cols)) cl *= 2;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.num_seqs * a.h_k * cl));
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = sizeof(Smem<D>);
+  cfg.gridDim = dim3((unsigned)(jobs * cl));
+  cfg.blockDim = dim3(Cfg<D>::THREADS);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -281,7 +362,7 @@ static cudaError_t launch_t(const mj_block_evict_args& a, cudaStream_t stream) {
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, kern, a, block_log2(a.kv_format));
+  return cudaLaunchKernelEx(&cfg, kern, a, block_log2(a.kv_format), reciprocal(a.page_size));
 }
 
 }  // namespace ev
