@@ -7,9 +7,9 @@
 //    their bits, each a histogram of the keys that agree so far. Every CTA adds
 //    up the cluster's histograms for itself, in vectors.
 // 2. The kept tokens in order: those above that key, the first of those equal
-//    to it, the recent ones. A CTA takes a contiguous part of the tokens, a
-//    thread a contiguous part of that; what the parts before it keep is summed
-//    over the block, then over the cluster.
+//    to it, the recent ones. A CTA takes a contiguous part of the tokens, a warp
+//    a contiguous part of that; what the parts before it keep is summed over the
+//    block, then over the cluster.
 // 3. The rows move. Position i receives token kept[i] >= i, so a step that
 //    reads all its tokens before it writes, and steps in ascending order, work
 //    in place: rows from i on are not read by the steps before. A step is 128
@@ -37,7 +37,7 @@ namespace ev {
 constexpr int STEP = 128;   // positions of a CTA's step
 constexpr int AHEAD = 8;    // steps whose positions are looked up together
 constexpr int BINS = 2048;  // of a radix pass
-constexpr int PER = 8;      // tokens of a thread in a segment of the selection
+constexpr int KEYS = 8192;  // tokens whose keys fit a CTA's shared memory
 
 // Weights in their order as unsigned keys; -0 is 0, NaN above all.
 __device__ __forceinline__ uint32_t key_of(float w) {
@@ -46,37 +46,33 @@ __device__ __forceinline__ uint32_t key_of(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// A position's source and destination: page and row of each
-struct Move {
-  int src_page, src_row, dst_page, dst_row;
-};
-
 template <int D>
 struct Cfg {
   static constexpr int THREADS = D == 256 ? 1024 : 512, WARPS = THREADS / 32;  // a thread has four 16-byte chunks of a step
   struct Smem {
-    Move moves[AHEAD * STEP];
+    // of the positions looked up, by side: the rows that they come from and go to
+    const unsigned char* src[2][AHEAD * STEP];
+    unsigned char* dst[2][AHEAD * STEP];
+    unsigned char* scale[2][AHEAD * STEP / 16];  // destinations' exponent bytes, by 16 positions
     float w[AHEAD * STEP];
-    unsigned char e[2][AHEAD * STEP];  // [side]: exponent bytes of the sources
-    int hist[3][BINS];                 // of the passes
-    int amax[3][2][STEP / 16];         // [step % 3][side][block]: largest magnitude of its rows, as bits
-    int scan[WARPS + 1];
-    int pick[2];                       // a pass's bin, and how many are above it
-    int parts[2];                      // this CTA's tokens above the threshold, and equal to it
+    unsigned char e[2][AHEAD * STEP];            // exponent bytes of the sources
+    uint32_t f[2][STEP];                         // a step's two factors of a row, as f16
+    int hist[3][BINS];                           // of the passes
+    uint32_t key[KEYS];
+    int amax[3][2][STEP / 16];                   // [step % 3][side][block]: largest magnitude of its rows, as bits
+    int scan[WARPS];
+    int pick[2];                                 // a pass's bin, and how many are above it
+    int parts[2];                                // this CTA's tokens above the threshold, and equal to it
   };
 };
 
-// Inclusive sums over the block; `total` of all of them.
+// Sums over the warps before this one of a value that is the same in a warp's
+// lanes; `total` over all.
 template <int WARPS>
-__device__ __forceinline__ int block_scan(int v, int* scan, int& total) {
+__device__ __forceinline__ int warps_before(int v, int* scan, int& total) {
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += x;
-  }
   __syncthreads();  // scan's last readers are done
-  if (lane == 31) scan[wid] = v;
+  if (lane == 0) scan[wid] = v;
   __syncthreads();
   int x = lane < WARPS ? scan[lane] : 0;
 #pragma unroll
@@ -86,27 +82,65 @@ __device__ __forceinline__ int block_scan(int v, int* scan, int& total) {
   }
   total = __shfl_sync(0xffffffffu, x, 31);
   const int below = __shfl_sync(0xffffffffu, x, wid ? wid - 1 : 0);
-  return v + (wid ? below : 0);
+  return wid ? below : 0;
 }
 
-// the largest magnitude code of 16, NaN left out
-__device__ __forceinline__ uint32_t max_code(uint4 c) {
-  drop_nan_codes(c);
-  uint32_t m = __vmaxu4(__vmaxu4(c.x & 0x7F7F7F7Fu, c.y & 0x7F7F7F7Fu), __vmaxu4(c.z & 0x7F7F7F7Fu, c.w & 0x7F7F7F7Fu));
-  m = __vmaxu4(m, m >> 16);
-  return max(m & 0xFFu, m >> 8 & 0xFFu);
+// the largest magnitude of 16 codes, NaN left out
+__device__ __forceinline__ float max_abs16(uint4 c) {
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  __half2 m[2];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t h = e4m3x2_to_h2((uint16_t)(w[i >> 1] >> (16 * (i & 1))));
+    const __half2 x = __habs2(*reinterpret_cast<const __half2*>(&h));
+    m[i & 1] = i < 2 ? x : __hmax2(m[i & 1], x);
+  }
+  m[0] = __hmax2(m[0], m[1]);
+  return fmaxf(fmaxf((float)m[0].x, (float)m[0].y), 0.f);
 }
+
+// 4 codes times two powers of two, as codes, in f16: there a product below 2^-21
+// may round, but is 0 as a code all the same
+__device__ __forceinline__ uint32_t shift4(uint32_t codes, __half2 f, __half2 g) {
+  uint32_t out[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t h = e4m3x2_to_h2((uint16_t)(codes >> (16 * i)));
+    const __half2 x = __hmul2(__hmul2(*reinterpret_cast<const __half2*>(&h), f), g);
+    uint16_t c;
+    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(c) : "r"(*reinterpret_cast<const uint32_t*>(&x)));
+    out[i] = c;
+  }
+  return out[0] | out[1] << 16;
+}
+// The cluster's barrier between a step's reads and its writes, in two halves.
+// Nothing that one CTA writes there is read by another: it only has to come after
+// the reads (a release would also wait for the writes of the step before). A
+// store that depends on their values, and never happens, stands before it.
+__device__ __forceinline__ void cluster_arrive(float not_negative, int* smem) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.lt.f32 p, %0, 0f00000000;\n\t"
+      "@p st.shared.u32 [%1], 0;\n\t"
+      "barrier.cluster.arrive.relaxed.aligned;\n\t}" ::"f"(not_negative),
+      "r"(smem_addr(smem))
+      : "memory");
+}
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// 2^k for -24 <= k <= 15
+__device__ __forceinline__ uint32_t h_exp2(int k) { return k < -14 ? 1u << (k + 24) : (uint32_t)(15 + k) << 10; }
 
 template <int D>
 __global__ void __launch_bounds__(Cfg<D>::THREADS, D == 256 ? 1 : 2)
     block_evict_kernel(const __grid_constant__ mj_block_evict_args a, int lg, uint64_t per_page) {
-  constexpr int THREADS = Cfg<D>::THREADS, WARPS = Cfg<D>::WARPS, SEG = PER * THREADS;
+  constexpr int THREADS = Cfg<D>::THREADS, WARPS = Cfg<D>::WARPS;
   extern __shared__ __align__(16) unsigned char raw[];
   auto& sm = *reinterpret_cast<typename Cfg<D>::Smem*>(raw);
   auto cluster = cg::this_cluster();
   const int CL = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int job = blockIdx.x / CL, h = job % a.h_k, seq = job / a.h_k;
-  const int t = threadIdx.x;
+  const int t = threadIdx.x, lane = t & 31, wid = t >> 5;
   griddep_wait();
   const int L = a.seq_lens[seq], budget = a.budget;
   int32_t* kept = a.kept + ((int64_t)seq * a.h_k + h) * budget;
@@ -133,25 +167,19 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, D == 256 ? 1 : 2)
 
   // ---- 1. the threshold
   const int M = L - a.recent, m = budget - a.recent;  // 0 <= m < M
-  const int part = (M + CL - 1) / CL, t0 = min(rank * part, M), t1 = min(t0 + part, M);
-  // this thread's tokens of the segment that begins at s0; of a part of one
-  // segment they stay in registers for all passes
-  uint32_t key[PER];
-  const int per = min((part + THREADS - 1) / THREADS, PER), seg = per * THREADS;
-  auto load_keys = [&](int s0) {
-#pragma unroll
-    for (int x = 0; x < PER; ++x) {
-      const int i = s0 + t * per + x;
-      key[x] = x < per && i < t1 ? key_of(w[i]) : 0u;
-    }
-  };
-  // tokens of them that are there
-  auto count_of = [&](int s0) { return min(max(t1 - s0 - t * per, 0), per); };
+  // Few enough tokens, and every CTA looks through all of them: that costs less
+  // than exchanging histograms.
+  const bool alone = M <= KEYS;
+  const int part = alone ? M : (M + CL - 1) / CL, t0 = alone ? 0 : min(rank * part, M), n = min(part, M - t0);
+  const bool held = part <= KEYS;  // keys are made once
+  auto key_at = [&](int i) { return held ? sm.key[i] : key_of(w[t0 + i]); };
   uint32_t prefix = 0;  // the threshold's bits so far
   int above = 0;        // keys that are larger than any with these bits
   if (m > 0) {
-    for (int i = t; i < 3 * BINS; i += THREADS) sm.hist[0][i] = 0;
-    load_keys(t0);
+    for (int i = t; i < 3 * BINS / 4; i += THREADS) reinterpret_cast<int4*>(sm.hist[0])[i] = make_int4(0, 0, 0, 0);
+    if (held)
+#pragma unroll 8
+      for (int i = t; i < n; i += THREADS) sm.key[i] = key_of(w[t0 + i]);
     __syncthreads();
     int shift = 32;
 #pragma unroll 1
@@ -160,17 +188,19 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, D == 256 ? 1 : 2)
       const uint32_t known = pass ? ~0u << shift : 0u;
       shift -= bits;
       int* hist = sm.hist[pass];
-      for (int s0 = t0; s0 < t1; s0 += seg) {
-        if (part > seg) load_keys(s0);
-        const int n = count_of(s0);
-#pragma unroll
-        for (int x = 0; x < PER; ++x)
-          if (x < n && (key[x] & known) == prefix) atomicAdd(&hist[(key[x] >> shift) & ((1u << bits) - 1u)], 1);
+#pragma unroll 4
+      for (int i = t; i < n; i += THREADS) {
+        const uint32_t k = key_at(i);
+        if ((k & known) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1u)], 1);
       }
-      cluster.sync();
+      if (alone) __syncthreads();
+      else cluster.sync();
       // four bins a thread, from the largest down; all CTAs' on their way together
       int c[4] = {0, 0, 0, 0};
-      if (t < BINS / 4) {
+      if (t < BINS / 4 && alone) {
+        const int4 v = reinterpret_cast<const int4*>(hist)[BINS / 4 - 1 - t];
+        c[0] = v.w, c[1] = v.z, c[2] = v.y, c[3] = v.x;
+      } else if (t < BINS / 4) {
         int4 v[8];
 #pragma unroll
         for (int r = 0; r < 8; ++r)
@@ -178,9 +208,13 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, D == 256 ? 1 : 2)
 #pragma unroll
         for (int r = 0; r < 8; ++r) c[0] += v[r].w, c[1] += v[r].z, c[2] += v[r].y, c[3] += v[r].x;
       }
-      int total;
-      const int sum = c[0] + c[1] + c[2] + c[3];
-      int before = block_scan<WARPS>(sum, sm.scan, total) - sum + above;
+      int total, sum = c[0] + c[1] + c[2] + c[3], before = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += x;
+      }
+      before += warps_before<WARPS>(__shfl_sync(0xffffffffu, before, 31), sm.scan, total) - sum + above;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (before < m && before + c[i] >= m) {
@@ -196,82 +230,89 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, D == 256 ? 1 : 2)
   }
   const int ties = m - above;  // tokens of exactly the threshold's key to keep
 
-  // ---- 2. the kept tokens, in order
+  // ---- 2. the kept tokens, in order (by one that knows all: those of its own steps)
+  auto mine_to_write = [&](int p) { return !alone || (p / STEP & (CL - 1)) == rank; };
   if (m > 0) {
-    auto tally = [&](int s0) {  // above the threshold in the low half, equal to it in the high half
-      const int n = count_of(s0);
-      int v = 0;
-#pragma unroll
-      for (int x = 0; x < PER; ++x) v += x < n ? (key[x] > prefix) + ((key[x] == prefix) << 16) : 0;
-      return v;
-    };
-    int n_gt = 0, n_eq = 0, mine = 0, incl = 0;
-    for (int s0 = t0; s0 < t1; s0 += seg) {
-      if (part > seg) load_keys(s0);
-      int total;
-      mine = tally(s0);
-      incl = block_scan<WARPS>(mine, sm.scan, total);
-      n_gt += total & 0xFFFF;
-      n_eq += total >> 16;
+    // a warp has consecutive tokens, [begin, end) of the part
+    const int chunk = ((n + WARPS - 1) / WARPS + 31) & ~31, begin = min(wid * chunk, n), end = min(begin + chunk, n);
+    int gt = 0, eq = 0;
+#pragma unroll 2
+    for (int i0 = begin; i0 < end; i0 += 32) {
+      const uint32_t k = i0 + lane < end ? key_at(i0 + lane) : 0u;
+      gt += __popc(__ballot_sync(0xffffffffu, i0 + lane < end && k > prefix));
+      eq += __popc(__ballot_sync(0xffffffffu, i0 + lane < end && k == prefix));
     }
-    if (t == 0) {
-      sm.parts[0] = n_gt;
-      sm.parts[1] = n_eq;
-    }
-    cluster.sync();
-    int base_gt = 0, base_eq = 0;
-    for (int r = 0; r < rank; ++r) {
-      base_gt += cluster.map_shared_rank(sm.parts, r)[0];
-      base_eq += cluster.map_shared_rank(sm.parts, r)[1];
-    }
-    for (int s0 = t0; s0 < t1; s0 += seg) {
-      if (part > seg) {
-        int total;
-        load_keys(s0);
-        mine = tally(s0);
-        incl = block_scan<WARPS>(mine, sm.scan, total);
-        n_gt = total & 0xFFFF;
-        n_eq = total >> 16;
+    int n_gt, n_eq;
+    gt = warps_before<WARPS>(gt, sm.scan, n_gt);
+    eq = warps_before<WARPS>(eq, sm.scan, n_eq);
+    if (!alone) {
+      if (t == 0) {
+        sm.parts[0] = n_gt;
+        sm.parts[1] = n_eq;
       }
-      const int n = count_of(s0);
-      int gt = base_gt + (incl & 0xFFFF) - (mine & 0xFFFF), eq = base_eq + (incl >> 16) - (mine >> 16);
-#pragma unroll
-      for (int x = 0; x < PER; ++x) {
-        if (x >= n) break;
-        if (key[x] > prefix || (key[x] == prefix && eq < ties)) kept[gt + min(eq, ties)] = s0 + t * per + x;
-        gt += key[x] > prefix;
-        eq += key[x] == prefix;
+      cluster.sync();
+      for (int r = 0; r < rank; ++r) {
+        gt += cluster.map_shared_rank(sm.parts, r)[0];
+        eq += cluster.map_shared_rank(sm.parts, r)[1];
       }
-      base_gt += n_gt;
-      base_eq += n_eq;
+    }
+#pragma unroll 2
+    for (int i0 = begin; i0 < end; i0 += 32) {
+      const int i = i0 + lane;
+      const uint32_t k = i < end ? key_at(i) : 0u, below = (1u << lane) - 1u;
+      const bool is_gt = i < end && k > prefix, is_eq = i < end && k == prefix;
+      const uint32_t all_gt = __ballot_sync(0xffffffffu, is_gt), all_eq = __ballot_sync(0xffffffffu, is_eq);
+      const int my_eq = eq + __popc(all_eq & below), p = gt + __popc(all_gt & below) + min(my_eq, ties);
+      if ((is_gt || (is_eq && my_eq < ties)) && mine_to_write(p)) kept[p] = t0 + i;
+      gt += __popc(all_gt);
+      eq += __popc(all_eq);
     }
   }
-  for (int i = rank * THREADS + t; i < a.recent; i += CL * THREADS) kept[m + i] = M + i;
-  cluster.sync();
+  if (alone) {
+    for (int i = t; i < a.recent; i += THREADS)
+      if (mine_to_write(m + i)) kept[m + i] = M + i;
+    __syncthreads();
+  } else {
+    for (int i = rank * THREADS + t; i < a.recent; i += CL * THREADS) kept[m + i] = M + i;
+    cluster.sync();
+  }
 
   // ---- 3. the rows move
   constexpr int SIDE = D / 16, CPR = 2 * SIDE;  // 16-byte chunks of a K or V row, of both
   static_assert(STEP * CPR == 4 * THREADS, "four chunks a thread");
   const int steps = (budget + STEP * CL - 1) / (STEP * CL);
   const int u = t % CPR, side = u / SIDE;  // this thread's chunk of its four rows t / CPR, + 32, + 64, + 96
-  const int64_t sp = side ? a.v_stride_page : a.k_stride_page, sr = side ? a.v_stride_row : a.k_stride_row;
-  const int64_t ssp = side ? a.vs_stride_page : a.ks_stride_page, ssb = side ? a.vs_stride_block : a.ks_stride_block;
-  unsigned char* cache = static_cast<unsigned char*>(side ? a.v_cache : a.k_cache) + h * (side ? a.v_stride_head : a.k_stride_head) + u % SIDE * 16;
-  unsigned char* scales = static_cast<unsigned char*>(side ? a.v_scales : a.k_scales) + h * (side ? a.vs_stride_head : a.ks_stride_head);
   auto first_of = [&](int step) { return (step * CL + rank) * STEP; };
   // positions of the steps from `step` on: where they come from and go to, the
   // sources' exponents and weights
   auto look_up = [&](int step) {
-    for (int x = t; x < AHEAD * STEP; x += THREADS) {
-      const int p = first_of(step + x / STEP) + x % STEP;
-      if (step + x / STEP >= steps || p >= budget) break;
-      const int src = kept[p], sc = (int)quotient(src, per_page), dc = (int)quotient(p, per_page);
-      const Move v = {table[sc], src - sc * a.page_size, table[dc], p - dc * a.page_size};
-      sm.moves[x] = v;
-      sm.w[x] = w[src];
-      const int b = v.src_row >> lg;
-      sm.e[0][x] = static_cast<const unsigned char*>(a.k_scales)[v.src_page * a.ks_stride_page + b * a.ks_stride_block + h * a.ks_stride_head];
-      sm.e[1][x] = static_cast<const unsigned char*>(a.v_scales)[v.src_page * a.vs_stride_page + b * a.vs_stride_block + h * a.vs_stride_head];
+    constexpr int N = AHEAD * STEP / THREADS;
+    int p[N], src[N];
+    bool in[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int x = t + i * THREADS;
+      p[i] = first_of(step + x / STEP) + x % STEP;
+      in[i] = step + x / STEP < steps && p[i] < budget;
+      src[i] = in[i] ? kept[p[i]] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (!in[i]) continue;
+      const int x = t + i * THREADS, sc = (int)quotient(src[i], per_page), dc = (int)quotient(p[i], per_page);
+      const int64_t s_page = table[sc], s_row = src[i] - sc * a.page_size, d_page = table[dc], d_row = p[i] - dc * a.page_size;
+      sm.w[x] = w[src[i]];
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const int64_t sp = y ? a.v_stride_page : a.k_stride_page, sr = y ? a.v_stride_row : a.k_stride_row;
+        const int64_t ssp = y ? a.vs_stride_page : a.ks_stride_page, ssb = y ? a.vs_stride_block : a.ks_stride_block;
+        unsigned char* cache = static_cast<unsigned char*>(y ? a.v_cache : a.k_cache) + h * (y ? a.v_stride_head : a.k_stride_head);
+        unsigned char* scales = static_cast<unsigned char*>(y ? a.v_scales : a.k_scales) + h * (y ? a.vs_stride_head : a.ks_stride_head);
+        sm.src[y][x] = cache + s_page * sp + s_row * sr;
+        sm.dst[y][x] = cache + d_page * sp + d_row * sr;
+        sm.e[y][x] = scales[s_page * ssp + (s_row >> lg) * ssb];
+        if (x % 16 == 0) sm.scale[y][x / 16] = scales + d_page * ssp + (d_row >> lg) * ssb;
+      }
     }
   };
   uint4 now[4], next[4];
@@ -281,7 +322,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, D == 256 ? 1 : 2)
     for (int x = 0; x < 4; ++x) {
       const int i = t / CPR + x * (STEP / 4), at = step % AHEAD * STEP + i;
       v[x] = make_uint4(0, 0, 0, 0);
-      if (step < steps && i < count) v[x] = *reinterpret_cast<const uint4*>(cache + sm.moves[at].src_page * sp + sm.moves[at].src_row * sr);
+      if (step < steps && i < count) v[x] = *reinterpret_cast<const uint4*>(sm.src[side][at] + u % SIDE * 16);
     }
   };
   if (t < 3 * 2 * (STEP / 16)) sm.amax[0][0][t] = 0;
@@ -293,31 +334,42 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, D == 256 ? 1 : 2)
       fetch(step, now);
     }
     if ((step + 1) % AHEAD) fetch(step + 1, next);
-    const int p0 = first_of(step), count = budget - p0;
+    const int count = budget - first_of(step);
+    float most[4];  // of the chunks: once they are known, this step's tokens have been read
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {  // the largest magnitudes of the step's blocks: by rows, then blocks
+    for (int x = 0; x < 4; ++x) most[x] = max_abs16(now[x]);
+    cluster_arrive((most[0] + most[1]) + (most[2] + most[3]), sm.pick);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {  // of the rows, then the blocks
       const int i = t / CPR + x * (STEP / 4), at = step % AHEAD * STEP + i;
-      uint32_t most = max_code(now[x]);
 #pragma unroll
-      for (int o = SIDE / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-      if (u % SIDE == 0 && i < count) atomicMax(&sm.amax[step % 3][side][i >> lg], __float_as_int(e4m3x2_to_f2((uint16_t)most).x * block_scale(sm.e[side][at])));
+      for (int o = SIDE / 2; o > 0; o >>= 1) most[x] = fmaxf(most[x], __shfl_xor_sync(0xffffffffu, most[x], o));
+      if (u % SIDE == 0 && i < count) atomicMax(&sm.amax[step % 3][side][i >> lg], __float_as_int(most[x] * block_scale(sm.e[side][at])));
     }
-    cluster.sync();  // every CTA of the cluster has read this step's tokens
+    __syncthreads();
     if (t < 2 * (STEP / 16)) sm.amax[(step + 2) % 3][0][t] = 0;  // (read last before that barrier, and next behind another)
+    cluster_wait();  // every CTA of the cluster has read this step's tokens
+    if (t < 2 * STEP && t % STEP < count) {  // a row's side each: its block's exponent, and its codes' way there
+      const int i = t % STEP, y = t / STEP, at = step % AHEAD * STEP + i;
+      const int e = block_exponent(__int_as_float(sm.amax[step % 3][y][i >> lg]));
+      // from -24 down every code becomes 0; above 15 (then all are tiny) in two steps
+      const int k = max(block_e(sm.e[y][at]) - e, -24);
+      sm.f[y][i] = h_exp2(min(k, 15)) | h_exp2(min(max(k - 15, 0), 15)) << 16;
+      if ((i & ((1 << lg) - 1)) == 0) *sm.scale[y][at / 16] = (unsigned char)e;
+    }
+    __syncthreads();
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       const int i = t / CPR + x * (STEP / 4), at = step % AHEAD * STEP + i;
       if (i < count) {
-        const Move v = sm.moves[at];
-        const int e = block_exponent(__int_as_float(sm.amax[step % 3][side][i >> lg]));
-        const float f = __uint_as_float((uint32_t)(127 + block_e(sm.e[side][at]) - e) << 23);
-        *reinterpret_cast<uint4*>(cache + v.dst_page * sp + v.dst_row * sr) =
-            make_uint4(scale4(now[x].x, f), scale4(now[x].y, f), scale4(now[x].z, f), scale4(now[x].w, f));
-        if (u % SIDE == 0 && (i & ((1 << lg) - 1)) == 0) scales[v.dst_page * ssp + (v.dst_row >> lg) * ssb] = (unsigned char)e;
+        const uint32_t fg = sm.f[side][i];
+        const __half2 f = __half2half2(__ushort_as_half((unsigned short)fg)), g = __half2half2(__ushort_as_half((unsigned short)(fg >> 16)));
+        *reinterpret_cast<uint4*>(sm.dst[side][at] + u % SIDE * 16) =
+            make_uint4(shift4(now[x].x, f, g), shift4(now[x].y, f, g), shift4(now[x].z, f, g), shift4(now[x].w, f, g));
       }
       now[x] = next[x];
     }
-    if (t < STEP && t < count) w[p0 + t] = sm.w[step % AHEAD * STEP + t];
+    if (t < STEP && t < count) w[first_of(step) + t] = sm.w[step % AHEAD * STEP + t];
     if ((step + 1) % AHEAD == 0) __syncthreads();  // the looked-up positions are done with
   }
   cluster.sync();  // (no CTA leaves while another reads its shared memory)
@@ -348,7 +400,7 @@ static cudaError_t launch_t(const mj_block_evict_args& a, cudaStream_t stream) {
   // rows that stay or segments of the weights
   const int64_t jobs = (int64_t)a.num_seqs * a.h_k;
   int cl = 1;
-  while (cl < 8 && 2 * cl * jobs <= room && (cl * STEP < a.budget || (int64_t)cl * PER * Cfg<D>::THREADS < a.weights_cols)) cl *= 2;
+  while (cl < 8 && 2 * cl * jobs <= room && (cl * STEP < a.budget || (int64_t)cl * KEYS < a.weights_cols)) cl *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(jobs * cl));
   cfg.blockDim = dim3(Cfg<D>::THREADS);
