@@ -519,10 +519,18 @@ int mj_block_shared_plan(const int32_t* query_lens, const int32_t* seq_lens, int
                          int32_t* joins_out, int joins_capacity, int* num_work, int* num_joins, int* num_rows,
                          int* num_slots);
 
+/* Whether a step takes less time with its groups than without, by a model of both
+ * (mj_block_shared_plan's items and the join against mj_block_plan's, and what
+ * the decode kernel reads): *worth = 0 or 1. Pure host code. */
+int mj_block_shared_worth(const int32_t* query_lens, const int32_t* seq_lens, int num_seqs, int decode_seqs,
+                          const int32_t* groups, int num_groups, int h_q, int h_k, int head_size, int causal,
+                          int sm_count, int max_slots, int* worth);
+
 /* Joins the partials of a step's rows, weights e^(lse - largest), into O and
  * LSE. An entry of 12 int32 is (seq, first row, rows, rows of the entries
  * before it; first own slot, own partials, first shared slot, shared partials;
- * first row's place among its group's rows, 0, 0, 0). Own partials are slots of
+ * first row's place among its group's rows, first query row and query rows of
+ * the sequence, 0). Own partials are slots of
  * o_part, or with first own slot -1 those that mj_decode left in d_part. A
  * row's place p among the group's rows is row p % R of shared slots first +
  * p / R * partials + 0, 1, ..., R = MJ_BLOCK_ROWS. Rows without partials are
@@ -533,7 +541,6 @@ typedef struct mj_block_join_args {
   void* o; int64_t o_stride_tok, o_stride_head; /* elements */
   float* lse;                        /* optional (num_tokens, h_q) */
   int64_t num_tokens;
-  const int32_t* q_start;            /* (num_seqs + 1,) */
   const int32_t* joins; int num_joins; int num_rows;
   const float* o_part; const float* lse_part; int num_slots; /* as mj_block_attention leaves them */
   const float* d_part; const float* d_lse_part;              /* as mj_decode leaves them */

@@ -56,7 +56,8 @@ EXPORTED = ("mj_last_error", "mj_abi_version", "mj_row_bytes", "mj_cache_write",
             "mj_decode_noalloc", "mj_decode_kernel", "mj_expand_pages", "mj_plan_split_kv", "mj_create", "mj_plan",
             "mj_runner_fill", "mj_runner_status", "mj_destroy", "mj_tc_fallbacks", "mj_qk_norm_rope", "mj_block_write",
             "mj_block_read", "mj_block_attention", "mj_block_plan", "mj_qk_norm_rope_axes",
-            "mj_block_weigh", "mj_block_evict", "mj_block_shared_plan", "mj_block_join")
+            "mj_block_weigh", "mj_block_evict", "mj_block_shared_plan", "mj_block_shared_worth",
+            "mj_block_join")
 
 _i64, _i32, _vp, _f32 = C.c_int64, C.c_int, C.c_void_p, C.c_float
 
@@ -194,7 +195,7 @@ class BlockAttnArgs(C.Structure):
 class BlockJoinArgs(C.Structure):
     _fields_ = [
         ("num_seqs", _i32), ("h_q", _i32), ("h_k", _i32), ("head_size", _i32), ("dtype", _i32),
-        ("o", _vp), ("o_stride_tok", _i64), ("o_stride_head", _i64), ("lse", _vp), ("num_tokens", _i64), ("q_start", _vp),
+        ("o", _vp), ("o_stride_tok", _i64), ("o_stride_head", _i64), ("lse", _vp), ("num_tokens", _i64),
         ("joins", _vp), ("num_joins", _i32), ("num_rows", _i32), ("o_part", _vp), ("lse_part", _vp), ("num_slots", _i32),
         ("d_part", _vp), ("d_lse_part", _vp), ("max_splits", _i32), ("part_seqs", _i32), ("status", _vp),
     ]
@@ -277,6 +278,8 @@ def load():
         lib.mj_block_shared_plan.argtypes = [_pi, _pi, C.c_int, C.c_int, _pi, _pi, *[C.c_int] * 7, _pi, C.c_int, _pi, C.c_int,
                                              *[C.POINTER(C.c_int)] * 4]
         lib.mj_block_shared_plan.restype = C.c_int
+        lib.mj_block_shared_worth.argtypes = [_pi, _pi, C.c_int, C.c_int, _pi, *[C.c_int] * 7, C.POINTER(C.c_int)]
+        lib.mj_block_shared_worth.restype = C.c_int
         lib.mj_create.argtypes = [C.c_int] * 10
         lib.mj_create.restype = _vp
         lib.mj_plan.argtypes = [_vp, _pi, C.c_int, C.c_int, C.c_int, C.c_int, _vp]
@@ -388,6 +391,19 @@ def block_shared_plan(query_lens, seq_lens, decode_pieces, groups, h_q: int, h_k
                                       int(causal), sm_count, max_slots, p(work), len(work), p(joins), len(joins),
                                       *[C.byref(x) for x in n]))
     return n[0].value, n[1].value, n[2].value, n[3].value
+
+
+def block_shared_worth(query_lens, seq_lens, decode_seqs: int, groups, h_q: int, h_k: int, head_size: int, causal: bool,
+                       sm_count: int, max_slots: int) -> bool:
+    """mj_block_shared_worth: whether the step takes less time with its groups."""
+    import numpy as np
+
+    q, kv, gr = (np.ascontiguousarray(x, dtype=np.int32) for x in (query_lens, seq_lens, groups))
+    p = lambda x: x.ctypes.data_as(C.POINTER(C.c_int32))  # noqa: E731
+    n = C.c_int(0)
+    check(load().mj_block_shared_worth(p(q), p(kv), len(q), decode_seqs, p(gr), gr.size // 3, h_q, h_k, head_size, int(causal),
+                                       sm_count, max_slots, C.byref(n)))
+    return bool(n.value)
 
 
 def plan_split_kv(seq_lens, h_k: int, n_q_tiles: int, sm_count: int, ctas_per_sm: int = 1, max_splits: int = 16,

@@ -613,6 +613,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
         // which no MMA reads any more), so that D / 8 lanes write a row
         constexpr int LPR = D / 8, RPI = 32 / LPR;
         unsigned char* stage = sm + w * C::QTILE + (warp & 3) * (32 * D * 2);
+        const int rows_here = min(max(n_rows - (row0 + w * 128 + (warp & 3) * 32), 0), 32);
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           float v[32];
@@ -637,14 +638,22 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
 #pragma unroll
             for (int i = 0; i < 32; i += 8)
               store8(reinterpret_cast<T*>(stage + lane * (D * 2) + ((((c + i) >> 3) ^ (lane & 7)) << 4)), v + i);
-          } else if (live) {
+          } else {  // partials the same way, 32 columns at a time: eight lanes a row
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) store8(a.o_part + part * D + c + i, v + i);
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<float4*>(stage + lane * 128 + (((i >> 2) ^ (lane & 7)) << 4)) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            __syncwarp();
+            const int64_t first = part - lane;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              const int r = i + lane / 8;
+              const float4 x = *reinterpret_cast<const float4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+              if (r < rows_here) *reinterpret_cast<float4*>(a.o_part + (first + r) * D + c + 4 * (lane & 7)) = x;
+            }
           }
-          __syncwarp();  // the TMEM load is a whole-warp operation
+          __syncwarp();  // the TMEM load is a whole-warp operation, and the staged rows have been read
         }
         if (slot < 0) {
-          const int rows_here = min(max(n_rows - (row0 + w * 128 + (warp & 3) * 32), 0), 32);
 #pragma unroll 4
           for (int i = 0; i < 32 / RPI; ++i) {
             const int r = i * RPI + lane / LPR;
@@ -743,21 +752,14 @@ __global__ void __launch_bounds__(256) block_join_kernel(const __grid_constant__
     lo += k * step;
     len = min(step, len - k * step);
   }
-  const int4 e = entries[3 * lo], parts = entries[3 * lo + 1];
-  const int r = (int)row - e.w, R = e.y + r, place = entries[3 * lo + 2].x + r;
-  const int own = parts.y, shared = parts.w;
-  bool bad = e.x < 0 || e.x >= a.num_seqs || r < 0 || r >= e.z || e.y < 0 || own < 0 || shared < 0 || place < 0;
-  const int h_r = a.h_q / a.h_k;
-  int q0 = 0, n_rows = 0;
-  if (!bad) {
-    q0 = a.q_start[e.x];
-    const int n_tok = a.q_start[e.x + 1] - q0;
-    n_rows = n_tok * h_r;
-    bad = q0 < 0 || n_tok < 0 || q0 + (int64_t)n_tok > a.num_tokens || R >= n_rows || own + shared > 4096;
-    if (parts.x >= 0) bad |= own > a.num_slots - parts.x || r >= ROWS;
-    else bad |= own > a.max_splits || (own && (e.x >= a.part_seqs || !a.d_part));
-    if (shared) bad |= parts.z < 0 || parts.z + (int64_t)(place / ROWS + 1) * shared > a.num_slots;
-  }
+  const int4 e = entries[3 * lo], parts = entries[3 * lo + 1], more = entries[3 * lo + 2];
+  const int r = (int)row - e.w, R = e.y + r, place = more.x + r, own = parts.y, shared = parts.w;
+  const int h_r = a.h_q / a.h_k, q0 = more.y, n_rows = more.z * h_r;
+  bool bad = e.x < 0 || e.x >= a.num_seqs || r < 0 || r >= e.z || e.y < 0 || own < 0 || shared < 0 || place < 0 || own > 4096 ||
+             shared > 4096 || q0 < 0 || more.z < 0 || q0 + (int64_t)more.z > a.num_tokens || R >= n_rows;
+  if (parts.x >= 0) bad |= own > a.num_slots - parts.x || r >= ROWS;
+  else bad |= own > a.max_splits || (own && (e.x >= a.part_seqs || !a.d_part));
+  if (shared) bad |= parts.z < 0 || parts.z + (int64_t)(place / ROWS + 1) * shared > a.num_slots;
   if (bad) {  // uniform in the warp
     if (lane == 0) flag(a.status, MJ_DEV_BAD_SPLIT);
     return;
@@ -780,7 +782,7 @@ __global__ void __launch_bounds__(256) block_join_kernel(const __grid_constant__
     for (int k0 = 0; k0 < own + shared; k0 += 32) {
       const float wl = k0 + lane < own + shared ? __expf(lse_of(k0 + lane) - mx) : 0.f;
       const int n = min(32, own + shared - k0);
-#pragma unroll 4
+#pragma unroll (32 / E)
       for (int i = 0; i < n; ++i) {
         const int k = k0 + i;
         const float w = __shfl_sync(0xffffffffu, wl, i);

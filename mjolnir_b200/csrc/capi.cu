@@ -424,7 +424,7 @@ int mj_block_join(const mj_block_join_args* args, void* stream) {
     g_err[0] = 0;
     return MJ_OK;
   }
-  if (!a.o || !a.q_start || !a.joins || !aligned(a.joins, 16) || (a.num_slots && (!a.o_part || !a.lse_part || !aligned(a.o_part, 16))) ||
+  if (!a.o || !a.joins || !aligned(a.joins, 16) || (a.num_slots && (!a.o_part || !a.lse_part || !aligned(a.o_part, 16))) ||
       (a.d_part && (!a.d_lse_part || !aligned(a.d_part, 16))))
     return fail(MJ_ERR_INVALID, "mj_block_join: plan or partial buffers");
   if (!aligned(a.o, 16) || a.o_stride_tok % 8 || a.o_stride_head % 8)

@@ -21,6 +21,7 @@
 #include <algorithm>
 #include <cmath>
 #include <exception>
+#include <functional>
 #include <set>
 #include <vector>
 
@@ -204,6 +205,154 @@ int mj_block_plan(const int32_t* query_lens, const int32_t* seq_lens, int num_se
   return MJ_OK;
 }
 
+}  // extern "C"
+
+// Rows of a sequence, or of a group, with the key tiles [t0, t1) that they see.
+namespace {
+struct SharedBlock {
+  int32_t seq, row0, t0, t1, span;
+  bool slotted;  // leaves partials even in one piece
+  int32_t group, pieces, slot;
+};
+constexpr int kMinPiece = 8;
+
+int64_t pieces_of(const SharedBlock& b, int64_t bound) { return b.t1 - b.t0 > bound ? ceil_div(b.t1 - b.t0, bound) : 1; }
+
+// What blocks cut in pieces of at most `bound` tiles take, in tiles of a CTA's
+// time: CTAs (an item and KV head each, longest first, as many at once as there
+// are SMs) a round its longest item and as much as 12 tiles for its beginning and
+// end, a piece of the row that has most of them 0.3 in the join. Negative: more
+// than max_slots partials.
+double cost_of(const std::vector<SharedBlock>& blocks, int64_t bound, int h_k, int sm_count, int64_t max_slots,
+               std::vector<int32_t>& lengths) {
+  int64_t slots = 0, most = 0;
+  lengths.clear();
+  for (const SharedBlock& b : blocks) {
+    const int64_t pieces = pieces_of(b, bound);
+    slots += pieces > 1 || b.slotted ? pieces : 0;
+    most = std::max(most, pieces);
+    lengths.insert(lengths.end(), (size_t)pieces, ceil_div(b.t1 - b.t0, pieces));
+  }
+  if (slots > max_slots) return -1.0;
+  std::sort(lengths.begin(), lengths.end(), std::greater<int32_t>());
+  double cost = most > 1 ? 0.3 * most : 0.0;
+  for (size_t first = 0; first < lengths.size() * h_k; first += sm_count) cost += lengths[first / h_k] + 12.0;
+  return cost;
+}
+
+// The bound of the least cost among those that cut the longest block in 1, 2, ...
+// pieces (0: none has so few partials). 64 sequences behind 16K tokens of 8 KV
+// heads: 55 us with 19 pieces, two rounds on 148 SMs, 30 with 18.
+int64_t best_bound(const std::vector<SharedBlock>& blocks, int h_k, int sm_count, int64_t max_slots, double* cost) {
+  std::vector<int32_t> lengths;
+  int64_t longest = 1, best = 0;
+  for (const SharedBlock& b : blocks) longest = std::max<int64_t>(longest, b.t1 - b.t0);
+  for (int64_t k = 1; k <= sm_count; ++k) {
+    const int64_t bound = std::max<int64_t>(kMinPiece, ceil_div(longest, k));
+    const double c = cost_of(blocks, bound, h_k, sm_count, max_slots, lengths);
+    if (c < 0.0) break;  // more pieces would need no fewer
+    if (!best || c < *cost) {
+      best = bound;
+      *cost = c;
+    }
+    if (bound <= kMinPiece) break;
+  }
+  return best;
+}
+
+// A step whose sequences share prefixes: blocks of the groups' rows first, then
+// those of the sequences from decode_seqs on. Empty message: fine.
+struct SharedStep {
+  std::vector<SharedBlock> blocks;
+  size_t of_groups = 0;
+  std::vector<int32_t> group_of, start;  // of a sequence: its group or -1, its first query row
+  std::vector<int64_t> place, group_rows;  // its first row's place among its group's, a group's rows
+};
+
+const char* shared_step(SharedStep& st, const int32_t* query_lens, const int32_t* seq_lens, int num_seqs, int decode_seqs,
+                        const int32_t* groups, int num_groups, int h_r, int head_size, int causal) {
+  const int rows = MJ_BLOCK_ROWS(head_size), keys = MJ_BLOCK_KEYS;
+  st.group_of.assign(num_seqs, -1);
+  st.start.assign(num_seqs + 1, 0);
+  st.place.assign(num_seqs, 0);
+  st.group_rows.assign(num_groups, 0);
+  int64_t rows_before = 0;
+  for (int s = 0; s < num_seqs; ++s) {
+    if (query_lens[s] < 0 || seq_lens[s] < 0) return "a length";
+    rows_before += query_lens[s];
+    if (rows_before * h_r > INT32_MAX) return "a length";
+    st.start[s + 1] = (int32_t)rows_before;
+  }
+  for (int g = 0, end = 0; g < num_groups; ++g) {
+    const int32_t first = groups[3 * g], count = groups[3 * g + 1], tokens = groups[3 * g + 2];
+    if (first < end || count < 1 || count > num_seqs - first || tokens <= 0 || tokens % 128) return "a group";
+    end = first + count;
+    for (int s = first; s < end; ++s) {
+      if (query_lens[s] && (causal ? (int64_t)seq_lens[s] - query_lens[s] : seq_lens[s]) < tokens)
+        return "a query before the end of its group's tokens";
+      st.group_of[s] = g;
+      st.place[s] = st.group_rows[g];
+      st.group_rows[g] += (int64_t)query_lens[s] * h_r;
+    }
+    for (int64_t r = 0; r < st.group_rows[g]; r += rows) st.blocks.push_back({first, (int32_t)r, 0, tokens / keys, count, true, g, 1, -1});
+  }
+  st.of_groups = st.blocks.size();
+  for (int s = decode_seqs; s < num_seqs; ++s) {
+    const int64_t n = query_lens[s], L = seq_lens[s], all = n * h_r;
+    const int t0 = st.group_of[s] < 0 ? 0 : groups[3 * st.group_of[s] + 2] / keys;
+    for (int64_t r = 0; r < all; r += rows) {
+      const int64_t last = causal ? L - n + (std::min(r + rows, all) - 1) / h_r : L - 1;  // last key seen
+      const int t1 = last < 0 ? 0 : (int32_t)(last / keys + 1);
+      st.blocks.push_back({s, (int32_t)r, t0, std::max(t0, t1), 0, st.group_of[s] >= 0, -1, 1, -1});
+    }
+  }
+  return nullptr;
+}
+}  // namespace
+
+extern "C" {
+
+int mj_block_shared_worth(const int32_t* query_lens, const int32_t* seq_lens, int num_seqs, int decode_seqs,
+                          const int32_t* groups, int num_groups, int h_q, int h_k, int head_size, int causal,
+                          int sm_count, int max_slots, int* worth) {
+  if (num_seqs < 0 || decode_seqs < 0 || decode_seqs > num_seqs || num_groups < 0 || h_k <= 0 || h_q <= 0 || h_q % h_k ||
+      (head_size != 128 && head_size != 256) || sm_count <= 0 || max_slots < 0 || (num_seqs && (!query_lens || !seq_lens)) ||
+      (num_groups && !groups) || !worth)
+    return mj::set_last_error(MJ_ERR_INVALID, "mj_block_shared_worth: invalid argument");
+  *worth = 0;
+  try {
+    SharedStep with, without;
+    for (int i = 0; i < 2; ++i)
+      if (const char* why = shared_step(i ? with : without, query_lens, seq_lens, num_seqs, decode_seqs, groups, i ? num_groups : 0,
+                                        h_q / h_k, head_size, causal)) {
+        char msg[128];
+        snprintf(msg, sizeof(msg), "mj_block_shared_worth: %s", why);
+        return mj::set_last_error(MJ_ERR_INVALID, msg);
+      }
+    if (with.of_groups == 0) return MJ_OK;
+    double a = 0.0, b = 0.0;
+    if (!best_bound(with.blocks, h_k, sm_count, max_slots, &a)) return MJ_OK;
+    int64_t total = 0;
+    for (const SharedBlock& x : without.blocks) total += x.t1 - x.t0;
+    std::vector<int32_t> lengths;
+    if (total) b = cost_of(without.blocks, std::max<int64_t>(kMinPiece, ceil_div(total * h_k, sm_count)), h_k, sm_count, INT64_MAX, lengths);
+    // In the time of a tile HBM moves 6.8 MB: of keys and values to the decode
+    // kernel, of partials to and from the join, whose launch takes that of 6.
+    const double row = (double)h_k * head_size / 6.8e6;
+    for (int s = 0; s < decode_seqs; ++s) {
+      const int g = with.group_of[s];
+      b += 2 * row * seq_lens[s];
+      a += 2 * row * (seq_lens[s] - (g >= 0 && query_lens[s] ? groups[3 * g + 2] : 0));
+    }
+    a += 6.0;
+    for (int g = 0; g < num_groups; ++g) a += 2 * 4 * 2 * row * with.group_rows[g];
+    *worth = a < b;
+  } catch (const std::exception&) {
+    return mj::set_last_error(MJ_ERR_INVALID, "mj_block_shared_worth: out of memory");
+  }
+  return MJ_OK;
+}
+
 int mj_block_shared_plan(const int32_t* query_lens, const int32_t* seq_lens, int num_seqs, int decode_seqs,
                          const int32_t* decode_pieces, const int32_t* groups, int num_groups, int h_q, int h_k,
                          int head_size, int causal, int sm_count, int max_slots, int32_t* work_out, int work_capacity,
@@ -214,65 +363,23 @@ int mj_block_shared_plan(const int32_t* query_lens, const int32_t* seq_lens, int
       (decode_seqs && !decode_pieces) || (num_groups && !groups) || work_capacity < 0 || joins_capacity < 0 ||
       (work_capacity && !work_out) || (joins_capacity && !joins_out) || !num_work || !num_joins || !num_rows || !num_slots)
     return mj::set_last_error(MJ_ERR_INVALID, "mj_block_shared_plan: invalid argument");
-  constexpr int kMinPiece = 8;
-  const int h_r = h_q / h_k, rows = MJ_BLOCK_ROWS(head_size), keys = MJ_BLOCK_KEYS;
-  struct Block {  // of a sequence's rows, or of a group's
-    int32_t seq, row0, t0, t1, span;
-    bool slotted;  // leaves partials even in one piece
-    int32_t group, pieces, slot;
-  };
+  const int h_r = h_q / h_k, rows = MJ_BLOCK_ROWS(head_size);
   try {
-    for (int s = 0; s < num_seqs; ++s)
-      if (query_lens[s] < 0 || seq_lens[s] < 0 || (int64_t)query_lens[s] * h_r > INT32_MAX)
-        return mj::set_last_error(MJ_ERR_INVALID, "mj_block_shared_plan: a length");
+    SharedStep st;
+    if (const char* why = shared_step(st, query_lens, seq_lens, num_seqs, decode_seqs, groups, num_groups, h_r, head_size, causal)) {
+      char msg[128];
+      snprintf(msg, sizeof(msg), "mj_block_shared_plan: %s", why);
+      return mj::set_last_error(MJ_ERR_INVALID, msg);
+    }
     for (int s = 0; s < decode_seqs; ++s)
       if (decode_pieces[s] < 0) return mj::set_last_error(MJ_ERR_INVALID, "mj_block_shared_plan: decode_pieces");
-    std::vector<int32_t> group_of(num_seqs, -1);
-    std::vector<int64_t> group_rows(num_groups, 0), place(num_seqs, 0);
-    std::vector<Block> blocks;
-    for (int g = 0, end = 0; g < num_groups; ++g) {
-      const int32_t first = groups[3 * g], count = groups[3 * g + 1], tokens = groups[3 * g + 2];
-      if (first < end || count < 1 || count > num_seqs - first || tokens <= 0 || tokens % 128)
-        return mj::set_last_error(MJ_ERR_INVALID, "mj_block_shared_plan: a group");
-      end = first + count;
-      for (int s = first; s < end; ++s) {
-        if (query_lens[s] && (causal ? (int64_t)seq_lens[s] - query_lens[s] : seq_lens[s]) < tokens)
-          return mj::set_last_error(MJ_ERR_INVALID, "mj_block_shared_plan: a query before the end of its group's tokens");
-        group_of[s] = g;
-        place[s] = group_rows[g];
-        group_rows[g] += (int64_t)query_lens[s] * h_r;
-      }
-      if (group_rows[g] > INT32_MAX) return mj::set_last_error(MJ_ERR_INVALID, "mj_block_shared_plan: a length");
-      for (int64_t r = 0; r < group_rows[g]; r += rows)
-        blocks.push_back({first, (int32_t)r, 0, tokens / keys, count, true, g, 1, -1});
-    }
-    const size_t of_groups = blocks.size();
-    for (int s = decode_seqs; s < num_seqs; ++s) {
-      const int64_t n = query_lens[s], L = seq_lens[s], all = n * h_r;
-      const int t0 = group_of[s] < 0 ? 0 : groups[3 * group_of[s] + 2] / keys;
-      for (int64_t r = 0; r < all; r += rows) {
-        const int64_t last = causal ? L - n + (std::min(r + rows, all) - 1) / h_r : L - 1;  // last key seen
-        const int t1 = last < 0 ? 0 : (int32_t)(last / keys + 1);
-        blocks.push_back({s, (int32_t)r, t0, std::max(t0, t1), 0, group_of[s] >= 0, -1, 1, -1});
-      }
-    }
-    // an equal share of the step's key tiles per SM; larger where that needs more slots than there are
-    int64_t total = 0;
-    for (const Block& b : blocks) total += b.t1 - b.t0;
-    int64_t bound = std::max<int64_t>(kMinPiece, ceil_div(total * h_k, sm_count)), slots = 0;
-    for (;; bound *= 2) {
-      slots = 0;
-      bool whole = true;
-      for (Block& b : blocks) {
-        b.pieces = b.t1 - b.t0 > bound ? (int32_t)ceil_div(b.t1 - b.t0, bound) : 1;
-        whole = whole && b.pieces == 1;
-        slots += b.pieces > 1 || b.slotted ? b.pieces : 0;
-      }
-      if (slots <= max_slots) break;
-      if (whole) return mj::set_last_error(MJ_ERR_UNSUPPORTED, "mj_block_shared_plan: more partials than max_slots");
-    }
+    std::vector<SharedBlock>& blocks = st.blocks;
+    double cost = 0.0;
+    const int64_t bound = best_bound(blocks, h_k, sm_count, max_slots, &cost);
+    if (!bound) return mj::set_last_error(MJ_ERR_UNSUPPORTED, "mj_block_shared_plan: more partials than max_slots");
     int64_t nw = 0, ns = 0;
-    for (Block& b : blocks) {
+    for (SharedBlock& b : blocks) {
+      b.pieces = (int32_t)pieces_of(b, bound);
       nw += b.pieces;
       if (b.pieces > 1 || b.slotted) {
         b.slot = (int32_t)ns;
@@ -282,7 +389,7 @@ int mj_block_shared_plan(const int32_t* query_lens, const int32_t* seq_lens, int
     if (nw > work_capacity) return mj::set_last_error(MJ_ERR_UNSUPPORTED, "mj_block_shared_plan: more items than the capacity");
     // joins: every sequence with rows, by its own blocks
     std::vector<int32_t> shared_first(num_groups, -1), shared_pieces(num_groups, 0);
-    for (size_t i = of_groups; i-- > 0;) {
+    for (size_t i = st.of_groups; i-- > 0;) {
       shared_first[blocks[i].group] = blocks[i].slot;
       shared_pieces[blocks[i].group] = blocks[i].pieces;
     }
@@ -293,25 +400,24 @@ int mj_block_shared_plan(const int32_t* query_lens, const int32_t* seq_lens, int
         room = false;
         return;
       }
-      const int g = group_of[s];
+      const int g = st.group_of[s];
       const int32_t e[12] = {s, (int32_t)row0, (int32_t)count, (int32_t)nr, first, pieces, g < 0 ? -1 : shared_first[g],
-                             g < 0 ? 0 : shared_pieces[g], g < 0 ? 0 : (int32_t)(place[s] + row0), 0, 0, 0};
+                             g < 0 ? 0 : shared_pieces[g], g < 0 ? 0 : (int32_t)(st.place[s] + row0), st.start[s], query_lens[s], 0};
       std::copy(e, e + 12, joins_out + 12 * nj++);
       nr += count;
     };
     for (int s = 0; s < decode_seqs; ++s)
       if (query_lens[s]) join(s, 0, (int64_t)query_lens[s] * h_r, -1, decode_pieces[s]);
-    for (size_t i = of_groups; i < blocks.size(); ++i) {
-      const Block& b = blocks[i];
+    for (size_t i = st.of_groups; i < blocks.size(); ++i) {
+      const SharedBlock& b = blocks[i];
       if (b.slot >= 0) join(b.seq, b.row0, std::min<int64_t>(rows, (int64_t)query_lens[b.seq] * h_r - b.row0), b.slot, b.pieces);
     }
     if (!room) return mj::set_last_error(MJ_ERR_UNSUPPORTED, "mj_block_shared_plan: more joins than the capacity");
-    if (nr > INT32_MAX) return mj::set_last_error(MJ_ERR_INVALID, "mj_block_shared_plan: a length");
-    std::stable_sort(blocks.begin(), blocks.end(), [](const Block& x, const Block& y) {
+    std::stable_sort(blocks.begin(), blocks.end(), [](const SharedBlock& x, const SharedBlock& y) {
       return (int64_t)(x.t1 - x.t0) * y.pieces > (int64_t)(y.t1 - y.t0) * x.pieces;
     });
     int64_t at = 0;
-    for (const Block& b : blocks)
+    for (const SharedBlock& b : blocks)
       for (int i = 0; i < b.pieces; ++i) {  // pieces of equal length, to a tile
         const int64_t t = b.t1 - b.t0;
         const int32_t w[8] = {b.seq, b.row0, (int32_t)(b.t0 + t * i / b.pieces), (int32_t)(b.t0 + t * (i + 1) / b.pieces),

@@ -8,6 +8,15 @@ from tests.block_helpers import Cache, assert_attention, attention_plain
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def share(monkeypatch, request):
+    """Small steps are not worth sharing: these tests share all the same."""
+    from mjolnir_b200 import kvblock
+
+    if request.node.name != "test_sharing_where_it_pays":
+        monkeypatch.setattr(kvblock.BlockAttention, "_worth", lambda self, *a: True)
+
+
 class Shared(Cache):
     """A cache whose groups (first, count, tokens) have their first whole pages in common."""
 
@@ -95,6 +104,16 @@ def test_many_sequences(q_lens):
     groups = [(0, len(q_lens), 4096)]
     c = Shared([4096 + n + 5 * i for i, n in enumerate(q_lens)], groups, h_k=2, seed=len(q_lens))
     check(c, q_lens, groups, 16)
+
+
+def test_sharing_where_it_pays():
+    """The plan's own choice: many sequences behind a long prefix share, a few behind a short one do not."""
+    for q_len in (1, 20):
+        groups = [(0, 3, 256)]
+        check(Shared([300, 290, 310], groups, seed=4), [q_len] * 3, groups, 8, shares=False)
+        n = 40 if q_len == 1 else 8
+        groups = [(0, n, 4096)]
+        check(Shared([4096 + q_len + i for i in range(n)], groups, h_k=8, page=64, seed=5), [q_len] * n, groups, 32)
 
 
 def test_not_causal():

@@ -115,6 +115,18 @@ def test_plan_refuses():
         plan([-1], [200], [], [])
 
 
+def test_worth():
+    """Many short rows behind a long prefix: yes. Few, short prefixes, or rows that fill their tiles alone: no."""
+    worth = lambda q, tokens, own=200, few=0, h_k=8, d=128: _lib.block_shared_worth(  # noqa: E731
+        q, [tokens + own + x for x in q], few, [(0, len(q), tokens)], 4 * h_k, h_k, d, True, 148, 166)
+    assert worth([1] * 64, 16384, few=64) and worth([24] * 16, 4096) and worth([3] * 16, 4096, d=256, h_k=4)
+    assert not worth([1] * 4, 16384, few=4) and not worth([24] * 2, 1024) and not worth([500] * 8, 1024) and not worth([0, 0], 4096)
+    with pytest.raises(_lib.MjolnirError, match="a group"):
+        _lib.block_shared_worth([1], [200], 0, [(0, 2, 128)], 4, 1, 128, True, 148, 10)
+    with pytest.raises(_lib.MjolnirError, match="invalid"):
+        _lib.block_shared_worth([1], [200], 2, [(0, 1, 128)], 4, 1, 128, True, 148, 10)
+
+
 def test_join_refuses():
     j = _lib.BlockJoinArgs()
     j.num_seqs, j.num_tokens, j.h_q, j.h_k = 1, 1, 3, 2
@@ -135,6 +147,7 @@ def test_groups_are_checked():
     from mjolnir_b200 import kvblock
 
     r = object.__new__(kvblock.BlockAttention)
+    r._worth = lambda *a: True
     r.h_q, r.h_k, r.rows, r.max_shared_slots = 8, 2, 256, 40
     q, kv = [1, 1, 1, 50], [1000, 900, 1500, 800]
     ok = lambda *g: r._groups(g, q, kv, 3, True)  # noqa: E731
