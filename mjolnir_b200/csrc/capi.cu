@@ -293,6 +293,7 @@ static int norm_rope(const mj_qk_norm_rope_args* args, const mj_rope_axes* axes,
       if (axes->axis[i] >= axes->num_axes)
         return fail(MJ_ERR_INVALID, "mj_qk_norm_rope_axes: angle %d on axis %d of %d", i, axes->axis[i], axes->num_axes);
   }
+  if (axes && a.num_positions > INT32_MAX) return fail(MJ_ERR_UNSUPPORTED, "mj_qk_norm_rope_axes: too many positions");
   if (a.num_tokens == 0 || a.h_q + a.h_k == 0) {
     g_err[0] = 0;
     return MJ_OK;

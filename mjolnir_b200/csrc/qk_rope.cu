@@ -78,9 +78,9 @@ __device__ __forceinline__ void rotate(float& a, float& b, float c, float s) {
 // loads are in flight together.
 // VEC: every row, weight and table address is 16-byte aligned (host-checked)
 // TL: log2 of a team's threads
-// AX: mj_rope_axes, or NoAxes. With axes a token has a position on each, all of
-// them loaded and checked by every thread of the token; a thread's 8 angles
-// that follow one axis come from its table row in vectors, others one by one.
+// AX: mj_rope_axes, or NoAxes. With axes a token has a position on each, which the
+// team's first threads load and hand round; a thread's 8 angles that follow one
+// axis come from its table row in vectors, others one by one.
 template <typename T, int HG, bool VEC, int TL, typename AX>
 __global__ void __launch_bounds__(128, sizeof(T) == 4 ? 3 : 5)
     qk_norm_rope_kernel(mj_qk_norm_rope_args a, float inv_d, const __grid_constant__ AX ax) {
@@ -99,11 +99,14 @@ __global__ void __launch_bounds__(128, sizeof(T) == 4 ? 3 : 5)
   const bool mine = t < a.num_tokens && 2 * j < nc;
   const int ca = a.interleaved || j >= r2 ? 2 * j : j, cb = a.interleaved || j >= r2 ? 2 * j + 1 : j + r2;
   const bool turns = mine && r2 && (a.interleaved ? 16 * j < a.rot_dim : j < r2);
-  int64_t pos = mine && r2 ? a.positions[t] : 0;
-  int64_t more[MJ_ROPE_AXES - 1];  // positions on the axes after the first
+  // with axes, a thread's are those on axis j, j + team, ...; (one, but in teams of less than four)
+  constexpr int NP = kAxes && team < MJ_ROPE_AXES ? MJ_ROPE_AXES / team : 1;
+  int64_t pos[NP];
   if constexpr (kAxes) {
 #pragma unroll
-    for (int x = 1; x < MJ_ROPE_AXES; ++x) more[x - 1] = mine && x < ax.num_axes ? a.positions[x * ax.axis_stride + t] : 0;
+    for (int i = 0; i < NP; ++i) pos[i] = t < a.num_tokens && r2 && j + i * team < ax.num_axes ? a.positions[(j + i * team) * ax.axis_stride + t] : 0;
+  } else {
+    pos[0] = mine && r2 ? a.positions[t] : 0;
   }
   const int64_t st = is_k ? a.k_stride_tok : a.q_stride_tok, sh = is_k ? a.k_stride_head : a.q_stride_head;
   const T* in = static_cast<const T*>(is_k ? a.k : a.q) + t * st + h0 * sh;
@@ -126,39 +129,44 @@ __global__ void __launch_bounds__(128, sizeof(T) == 4 ? 3 : 5)
     raw[0].load(w, 8 * ca, a.weight_dtype, VEC);
     raw[1].load(w, 8 * cb, a.weight_dtype, VEC);
   }
-  bool bad = mine && r2 && (pos < 0 || pos >= a.num_positions);
+  bool bad = false;  // (looked at once the rows are on their way)
+#pragma unroll
+  for (int i = 0; i < NP; ++i) bad |= r2 && t < a.num_tokens && (kAxes || mine) && (pos[i] < 0 || pos[i] >= a.num_positions);
+  if constexpr (kAxes) bad = __ballot_sync(0xffffffffu, bad) >> (threadIdx.x & 31 & ~(team - 1)) & (uint32_t)((1ull << team) - 1);
+  if (bad && j == 0) flag(a.status, MJ_DEV_BAD_POSITION);
   if constexpr (kAxes) {
+    uint2 axis = make_uint2(0, 0);
+    if (turns) axis = *reinterpret_cast<const uint2*>(ax.axis + 8 * j);
+    auto on = [&](int k) {  // the position of angle k of the 8: every lane asks
+      const int x = (k < 4 ? axis.x : axis.y) >> (8 * (k & 3)) & 0xFFu;
+      int p = __shfl_sync(0xffffffffu, (int)pos[0], x % team, team);
 #pragma unroll
-    for (int x = 0; x < MJ_ROPE_AXES - 1; ++x) bad |= more[x] < 0 || more[x] >= a.num_positions;
-  }
-  if (bad && j == 0) flag(a.status, MJ_DEV_BAD_POSITION);  // (looked at once the rows are on their way)
-  if (turns && !bad) {  // a pair of chunks turns by 8 angles in either pairing
-    bool one = true;
-    if constexpr (kAxes) {
-      const uint2 axis = *reinterpret_cast<const uint2*>(ax.axis + 8 * j);
-      auto on = [&](int k) {  // the position of angle k of the 8
-        const uint32_t x = (k < 4 ? axis.x : axis.y) >> (8 * (k & 3)) & 0xFFu;
-        int64_t p = pos;
+      for (int i = 1; i < NP; ++i) {
+        const int q = __shfl_sync(0xffffffffu, (int)pos[i], x % team, team);
+        if (x / team == i) p = q;
+      }
+      return (int64_t)p;
+    };
+    const bool use = turns && !bad;
+    if (__all_sync(0xffffffffu, axis.x == axis.y && axis.x == (axis.x & 0xFFu) * 0x01010101u)) {
+      const int64_t at = on(0) * a.cos_sin_stride + 8 * j;
+      if (use) {
+        turn[0].load(a.cos_sin, at, a.cos_sin_dtype, VEC);
+        turn[1].load(a.cos_sin, at + (a.rot_dim >> 1), a.cos_sin_dtype, VEC);
+      }
+    } else {
 #pragma unroll
-        for (uint32_t i = 1; i < MJ_ROPE_AXES; ++i) p = x == i ? more[i - 1] : p;
-        return p;
-      };
-      one = axis.x == axis.y && axis.x == (axis.x & 0xFFu) * 0x01010101u;
-      if (one) {
-        pos = on(0);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int64_t at = on(k) * a.cos_sin_stride + 8 * j + k;
+      for (int k = 0; k < 8; ++k) {
+        const int64_t at = on(k) * a.cos_sin_stride + 8 * j + k;
+        if (use) {
           turn[0].load_one(a.cos_sin, at, k, a.cos_sin_dtype);
           turn[1].load_one(a.cos_sin, at + (a.rot_dim >> 1), k, a.cos_sin_dtype);
         }
       }
     }
-    if (one) {
-      turn[0].load(a.cos_sin, pos * a.cos_sin_stride + 8 * j, a.cos_sin_dtype, VEC);
-      turn[1].load(a.cos_sin, pos * a.cos_sin_stride + (a.rot_dim >> 1) + 8 * j, a.cos_sin_dtype, VEC);
-    }
+  } else if (turns && !bad) {  // a pair of chunks turns by 8 angles in either pairing
+    turn[0].load(a.cos_sin, pos[0] * a.cos_sin_stride + 8 * j, a.cos_sin_dtype, VEC);
+    turn[1].load(a.cos_sin, pos[0] * a.cos_sin_stride + (a.rot_dim >> 1) + 8 * j, a.cos_sin_dtype, VEC);
   }
   raw[0].get(a.weight_dtype, f(wx));
   raw[1].get(a.weight_dtype, f(wy));
