@@ -69,17 +69,22 @@ template <typename T, int D, int N>
 struct Cfg {
   static constexpr int RAW = KEYS * D, K16 = 2 * RAW, QST = N * D * 2;  // a tile's codes; as 16 bits; a tile of Q rows
   static constexpr bool WIDE = N >= 64;
+  // CTAs of an SM: a CTA's roles wait for one another more than they work where few
+  // rows see a tile, so two (at head size 256 their shared memory allows one).
+  static constexpr int CTAS = !WIDE && D == 128 ? 2 : 1;
   // Warpgroups that convert K's codes, and that add up. Many rows: the
   // exponentials bound it, and two or four warps on a scheduler must hide one
   // another's latency (8192 tokens, 32 / 8 heads: 376 us with two warpgroups, 341
   // with four). Few rows: every tile of keys is converted for one product.
-  static constexpr int CWGS = WIDE ? 1 : 2, WGS = WIDE ? 4 : 2;
+  static constexpr int CWGS = WIDE || CTAS == 2 ? 1 : 2, WGS = WIDE ? 4 : CTAS == 2 ? 1 : 2;
   // Warps that fetch K. A lane's copies are issued one after another, over 100
-  // cycles each; with pages of 16 a tile has eight, and HBM has brought it in 700.
-  static constexpr int KWARPS = WIDE ? 1 : 4, K0 = WIDE ? 0 : 4 * (1 + CWGS + WGS), THREADS = 128 * (1 + CWGS + WGS) + (WIDE ? 0 : 128);
+  // cycles each; with pages of 16 a tile has eight.
+  static constexpr int KWARPS = WIDE || CTAS == 2 ? 1 : 4, K0 = KWARPS == 1 ? 0 : 4 * (1 + CWGS + WGS), THREADS = 128 * (1 + CWGS + WGS) + (KWARPS == 1 ? 0 : 128);
   // stages of K codes, of K in 16 bits, of Q
-  static constexpr int RS = WIDE ? (D == 256 ? 1 : 2) : D == 256 ? 2 : 4, KS = WIDE ? (D == 256 ? 1 : 2) : D == 256 ? 2 : 4, QS = D == 256 ? 2 : WIDE ? 3 : 4;
+  static constexpr int RS = WIDE && D == 256 ? 1 : 2, KS = WIDE && D == 256 ? 1 : 2, QS = D == 256 || !WIDE ? 2 : 3;
   static constexpr int SB = 4;  // S buffers in TMEM; a warpgroup that adds up has three of its columns' lse
+  static constexpr int TMEM_COLS = CTAS == 2 ? 64 : 512;
+  static_assert(SB * N <= TMEM_COLS, "S buffers");
   static constexpr int JOBS = WIDE ? 4 : 8;
   static constexpr int PAIRS = WGS * (WGS - 1);  // of a warpgroup that writes weights and one that adds its part
   static constexpr int K_OFF = 0, R_OFF = K_OFF + KS * K16, Q_OFF = R_OFF + RS * RAW, Z_OFF = Q_OFF + QS * QST;
@@ -87,7 +92,7 @@ struct Cfg {
   static constexpr int NBARS = 2 * (RS + KS + QS + SB + JOBS + PAIRS) + WGS + 1;
   static constexpr int MISC_OFF = BAR_OFF + NBARS * 8;
   static constexpr int SMEM = MISC_OFF + 16;
-  static_assert(SMEM <= 232448, "shared memory of a CTA");
+  static_assert(SMEM + 1024 <= 233472 / CTAS, "shared memory of a CTA");  // (1 KB of each is the system's)
   static_assert(JOBS >= 3, "the K warp looks two jobs ahead");
   // a buffer is always waited for by the same warpgroup, whose waits are in order:
   // another's could take an older phase of the same parity for its own
@@ -116,7 +121,7 @@ __device__ __forceinline__ void widen16(uint4 c, uint32_t* o) {
 __device__ __forceinline__ uint32_t unit_offset(uint32_t r, uint32_t u) { return r * 128 + ((u ^ (r & 7)) << 4); }
 
 template <typename T, int D, int N>
-__global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
+__global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, Cfg<T, D, N>::CTAS)
     block_weigh_kernel(const __grid_constant__ mj_block_weigh_args a, int lg, int hb, int tb, int ht,
                        const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmq) {
   using C = Cfg<T, D, N>;
@@ -167,17 +172,13 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
     prefetch_tmap(&tmq);
   }
   if (warp == 2) {
-    tmem_alloc(tmem_slot, 512);
+    tmem_alloc(tmem_slot, C::TMEM_COLS);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (*tmem_slot != 0) {  // uniform, and cannot happen: all 512 columns
-    if (threadIdx.x == 0) flag(a.status, MJ_DEV_BAD_SPLIT);
-    if (warp == 2) tmem_dealloc(*tmem_slot, 512);
-    return;
-  }
+  const uint32_t tmem = *tmem_slot;
   auto wait = [&](uint64_t* bar, int phase) {
     if (mbar_wait(bar, (uint32_t)phase & 1u, abort_flag, kWaitNs)) return true;
     if (!*abort_flag) {
@@ -389,7 +390,7 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
           if (lead) {
 #pragma unroll
             for (int y = H * (D / 32); y < (H + 1) * (D / 32); ++y)
-              mma_f16(b * N, k + y / 4 * (KEYS * 8) + y % 4 * 2, q + y / 4 * (N * 8) + y % 4 * 2, idesc, y > 0);
+              mma_f16(tmem + b * N, k + y / 4 * (KEYS * 8) + y % 4 * 2, q + y / 4 * (N * 8) + y % 4 * 2, idesc, y > 0);
           }
         };
         steps(std::integral_constant<int, 0>());
@@ -488,7 +489,7 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
     auto add_up = [&](auto part, int b, float c2, int c_lo, int c_hi) {
       constexpr bool PART = decltype(part)::value;
       const float4* zs = reinterpret_cast<const float4*>(zbuf + (z_seen + 2) % 3 * N);
-      const uint32_t s_addr = b * N + lane_base;
+      const uint32_t s_addr = tmem + b * N + lane_base;
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)}, v[2][8];
       tmem_ld16(s_addr, reinterpret_cast<float*>(v[0]));
 #pragma unroll
@@ -591,7 +592,7 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
   __syncthreads();
   if (warp == 2) {
     tc_fence_after();
-    tmem_dealloc(0, 512);
+    tmem_dealloc(tmem, C::TMEM_COLS);
   }
 }
 
@@ -601,17 +602,18 @@ template <typename T, int D, int N>
 static cudaError_t launch_t(const mj_block_weigh_args& a, cudaStream_t stream) {
   using C = Cfg<T, D, N>;
   auto kern = block_weigh_kernel<T, D, N>;
-  static std::atomic<int> ready[kMaxDevices];  // SMs of the device, once the kernel is prepared on it
+  static std::atomic<int> ready[kMaxDevices];  // CTAs that the device holds at once, once the kernel is prepared on it
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
-  int sms = ready[dev].load(std::memory_order_acquire);
-  if (!sms) {
+  int ctas = ready[dev].load(std::memory_order_acquire);
+  if (!ctas) {
     std::lock_guard<std::mutex> lock(tc_init_mutex());
     if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM)) != cudaSuccess) return e;
-    if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
-    ready[dev].store(sms, std::memory_order_release);
+    if ((e = cudaDeviceGetAttribute(&ctas, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
+    ctas *= C::CTAS;
+    ready[dev].store(ctas, std::memory_order_release);
   }
   auto fn = tensor_map_encoder();
   if (!fn) return cudaErrorNotSupported;
@@ -637,7 +639,7 @@ static cudaError_t launch_t(const mj_block_weigh_args& a, cudaStream_t stream) {
            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
       return cudaErrorInvalidValue;
   }
-  return launch_kernel(kern, dim3((unsigned)sms), dim3(C::THREADS), C::SMEM, stream, a, block_log2(a.kv_format), hb, tb, ht, mk, mq);
+  return launch_kernel(kern, dim3((unsigned)ctas), dim3(C::THREADS), C::SMEM, stream, a, block_log2(a.kv_format), hb, tb, ht, mk, mq);
 }
 
 template <typename T>
