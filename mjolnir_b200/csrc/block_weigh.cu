@@ -242,6 +242,14 @@ __device__ __forceinline__ void fetch_keys(const C& cta, int lg, const CUtensorM
 // byte offset of 16-byte unit u of row r in a [rows][128 bytes] swizzled block
 __device__ __forceinline__ uint32_t unit_offset(uint32_t r, uint32_t u) { return r * 128 + ((u ^ (r & 7)) << 4); }
 
+// A key's weight, which one thread writes: a token of the step begins at 0. The
+// others are added to where they are, in L2: a load would be waited for, some
+// 2000 cycles a tile.
+__device__ __forceinline__ void put(float* w, float sum, bool begins) {
+  if (begins) *w = sum;
+  else atomicAdd(w, sum);
+}
+
 // ------------------------------------------------------------- many rows a tile
 template <typename T, int D, int N>
 struct Cfg {
@@ -517,8 +525,6 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
         continue;
       }
       float* w = a.weights + j.seq * a.w_stride_seq + j.h * a.w_stride_head + key;
-      float old = 0.f;
-      if (place == 0 && key < min(L, ahead)) old = *w;
       float z = 0.f;
       store_lse(load_lse(j, t0, place));
       if (place + WGS < tiles) z = load_lse(j, t0, place + WGS);
@@ -565,7 +571,7 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
         }
       }
       if (!ok) break;
-      if (place == 0 && key < L) *w = old + sum;
+      if (place == 0 && key < L) put(w, sum, key >= ahead);
       done_job(i);
     }
     tc_fence_before();
@@ -789,7 +795,6 @@ __global__ void __launch_bounds__(Few<D>::THREADS, Few<D>::CTAS)
 #pragma unroll 1
       for (int x = 0; ok && x < nk; ++x, w += KEYS) {
         const int key = (j.kt + x) * KEYS + t, tiles = j.tiles[x];
-        const float old = key < min(L, ahead) ? *w : 0.f;
         float sum = 0.f, low = 0.f;  // the sum, and what its rounding lost
         int tok = j.t0[x], head = 0;
 #pragma unroll 1
@@ -833,7 +838,7 @@ __global__ void __launch_bounds__(Few<D>::THREADS, Few<D>::CTAS)
             tok += tb;
           }
         }
-        if (ok && key < L) *w = old + sum;
+        if (ok && key < L) put(w, sum, key >= ahead);
       }
       if (ok) cta.done_job(i);
     }
@@ -876,8 +881,10 @@ static bool key_map(CUtensorMap* m, const mj_block_weigh_args& a) {
   cuuint64_t strides[4] = {128, (cuuint64_t)(a.k_stride_row ? a.k_stride_row : 16), (cuuint64_t)(a.k_stride_head ? a.k_stride_head : 16),
                            (cuuint64_t)(a.k_stride_page ? a.k_stride_page : 16)};
   cuuint32_t box[5] = {128, 1, (cuuint32_t)a.page_size, 1, 1}, estr[5] = {1, 1, 1, 1, 1};
+  // 128 bytes at a time into L2: behind a row's 128 of K lie V's, which nobody reads
+  // (32 x 8K single tokens: 53 us with 256)
   return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<void*>(a.k_cache), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename T, int D, int N>
