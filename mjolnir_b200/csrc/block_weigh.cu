@@ -261,7 +261,7 @@ struct Cfg {
   // stages of K codes, of K in 16 bits, of Q
   static constexpr int RS = D == 256 ? 1 : 2, KS = D == 256 ? 1 : 2, QS = D == 256 ? 2 : 3;
   static constexpr int SB = 4;  // S buffers in TMEM; a warpgroup that adds up has three of its columns' lse
-  static constexpr int JOBS = 4;
+  static constexpr int JOBS = 16;  // (K is fetched for jobs that far ahead: 8 sequences of 6K, 64 rows 57 us with 4, 42 with 16)
   static constexpr int PAIRS = WGS * (WGS - 1);  // of a warpgroup that writes weights and one that adds its part
   static constexpr int K_OFF = 0, R_OFF = K_OFF + KS * K16, Q_OFF = R_OFF + RS * RAW, Z_OFF = Q_OFF + QS * QST;
   static constexpr int RED_OFF = Z_OFF + 3 * WGS * N * 4, JOB_OFF = RED_OFF + PAIRS * KEYS * 4, BAR_OFF = JOB_OFF + JOBS * (int)sizeof(Job);
@@ -927,10 +927,13 @@ static cudaError_t launch_few(const mj_block_weigh_args& a, cudaStream_t stream)
 
 template <typename T>
 static cudaError_t launch_d(const mj_block_weigh_args& a, cudaStream_t stream) {
-  // Queries that count and rows of a KV head, on average over the sequences: up to
-  // 32 rows of 4 queries the kernel for few (more queries may be one sequence's).
+  // The kernel for few rows where the sequences' rows, on average, are one tile of
+  // its 16, and their queries at most 4 (more may be one sequence's). It makes Q's
+  // terms again for every tile of keys where there are more: 8 sequences of 6K, 16
+  // rows 24 us, 32 rows 65 and with the other kernel 51, 64 rows 120 and 57.
   const int64_t most = a.window ? (int64_t)a.num_seqs * a.window : a.num_rows, tokens = a.num_rows < most ? a.num_rows : most;
-  const bool few = tokens <= 4 * (int64_t)a.num_seqs && tokens * (a.h_q / a.h_k) <= 32 * (int64_t)a.num_seqs;
+  const int h_r = a.h_q / a.h_k, fit = h_r > 16 ? 0 : 16 / h_r < 4 ? 16 / h_r : 4;
+  const bool few = tokens <= (int64_t)fit * a.num_seqs;
   if (few) return a.head_size == 256 ? launch_few<T, 256>(a, stream) : launch_few<T, 128>(a, stream);
   return a.head_size == 256 ? launch_t<T, 256, 96>(a, stream) : launch_t<T, 128, 128>(a, stream);
 }
