@@ -261,6 +261,13 @@ struct Cfg {
   // stages of K codes, of K in 16 bits, of Q
   static constexpr int RS = D == 256 ? 1 : 2, KS = D == 256 ? 1 : 2, QS = D == 256 ? 2 : 3;
   static constexpr int SB = 4;  // S buffers in TMEM; a warpgroup that adds up has three of its columns' lse
+  // The tensor cores cut off what a step's sum has below fp32's last place. Over
+  // the 16 steps of fp16 products at head size 256 weights came out 6.6e-7 too
+  // small (1.2e-6 from 64 bits, plain fp32 arithmetic 3.7e-7), so there each half of
+  // the head dim has a sum of its own.
+  static constexpr bool SPLIT = std::is_same<T, __half>::value && D == 256;
+  static constexpr int SN = SPLIT ? 2 * N : N;
+  static_assert(SB * SN <= 512, "S buffers");
   static constexpr int JOBS = 16;  // (K is fetched for jobs that far ahead: 8 sequences of 6K, 64 rows 57 us with 4, 42 with 16)
   static constexpr int PAIRS = WGS * (WGS - 1);  // of a warpgroup that writes weights and one that adds its part
   static constexpr int K_OFF = 0, R_OFF = K_OFF + KS * K16, Q_OFF = R_OFF + RS * RAW, Z_OFF = Q_OFF + QS * QST;
@@ -406,7 +413,8 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
           if (lead) {
 #pragma unroll
             for (int y = H * (D / 32); y < (H + 1) * (D / 32); ++y)
-              mma_f16(tmem + b * N, k + y / 4 * (KEYS * 8) + y % 4 * 2, q + y / 4 * (N * 8) + y % 4 * 2, idesc, y > 0);
+              mma_f16(tmem + b * C::SN + (C::SPLIT ? H * N : 0), k + y / 4 * (KEYS * 8) + y % 4 * 2, q + y / 4 * (N * 8) + y % 4 * 2, idesc,
+                      y > (C::SPLIT ? H * (D / 32) : 0));
           }
         };
         steps(std::integral_constant<int, 0>());
@@ -484,13 +492,17 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
     auto add_up = [&](auto part, int b, float c2, int c_lo, int c_hi) {
       constexpr bool PART = decltype(part)::value;
       const float4* zs = reinterpret_cast<const float4*>(zbuf + (z_seen + 2) % 3 * N);
-      const uint32_t s_addr = tmem + b * N + lane_base;
-      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)}, v[2][8];
+      const uint32_t s_addr = tmem + b * C::SN + lane_base;
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)}, v[2][8], more[C::SPLIT ? 8 : 1];
       tmem_ld16(s_addr, reinterpret_cast<float*>(v[0]));
 #pragma unroll
       for (int c = 0; c < N; c += 16) {
         float2* const now = v[c / 16 & 1];
+        if (C::SPLIT) tmem_ld16(s_addr + N + c, reinterpret_cast<float*>(more));
         tmem_wait_ld();
+        if (C::SPLIT)
+#pragma unroll
+          for (int x = 0; x < 8; ++x) now[x] = fadd2(now[x], more[C::SPLIT ? x : 0]);
         if (c + 16 < N) tmem_ld16(s_addr + c + 16, reinterpret_cast<float*>(v[c / 16 + 1 & 1]));
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
@@ -935,7 +947,8 @@ static cudaError_t launch_d(const mj_block_weigh_args& a, cudaStream_t stream) {
   const int h_r = a.h_q / a.h_k, fit = h_r > 16 ? 0 : 16 / h_r < 4 ? 16 / h_r : 4;
   const bool few = tokens <= (int64_t)fit * a.num_seqs;
   if (few) return a.head_size == 256 ? launch_few<T, 256>(a, stream) : launch_few<T, 128>(a, stream);
-  return a.head_size == 256 ? launch_t<T, 256, 96>(a, stream) : launch_t<T, 128, 128>(a, stream);
+  constexpr int N256 = std::is_same<T, __half>::value ? 64 : 96;  // (fp16's two sums of 96 do not fit TMEM)
+  return a.head_size == 256 ? launch_t<T, 256, N256>(a, stream) : launch_t<T, 128, 128>(a, stream);
 }
 
 }  // namespace bw
