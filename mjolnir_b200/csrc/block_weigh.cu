@@ -93,10 +93,15 @@ struct Cta {
   }
 };
 
+// The sequences that a launch takes: those with lo to hi queries that count.
+struct Take {
+  int lo, hi;
+};
+
 // The warp that finds the CTA's jobs: up to TILES tiles of keys of one KV head.
 // 32 sequences at a time, lane i has the key tiles of sequence s0 + i.
 template <int TILES, class C>
-__device__ __forceinline__ void find_jobs(const C& cta, int tb, int ht) {
+__device__ __forceinline__ void find_jobs(const C& cta, Take take, int tb, int ht) {
   const mj_block_weigh_args& a = cta.a;
   const int lane = cta.lane;
   int L = 0, n = 0, q0 = 0;
@@ -110,7 +115,8 @@ __device__ __forceinline__ void find_jobs(const C& cta, int tb, int ht) {
       if (complain) flag(a.status, MJ_DEV_BAD_LENGTH);
       return 0;
     }
-    return n ? (L + KEYS - 1) / KEYS : 0;
+    const int m = a.window && a.window < n ? a.window : n;
+    return m && m >= take.lo && m <= take.hi ? (L + KEYS - 1) / KEYS : 0;
   };
   // Tiles a job: as many as leave every CTA two jobs (each costs its lookups'
   // latency; a few jobs more than CTAs leave some of them idle).
@@ -301,7 +307,7 @@ __device__ __forceinline__ void widen16(uint4 c, uint32_t* o) {
 
 template <typename T, int D, int N>
 __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
-    block_weigh_kernel(const __grid_constant__ mj_block_weigh_args a, int lg, int hb, int tb, int ht,
+    block_weigh_kernel(const __grid_constant__ mj_block_weigh_args a, Take take, int lg, int hb, int tb, int ht,
                        const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmq) {
   using C = Cfg<T, D, N>;
   constexpr int RS = C::RS, KS = C::KS, QS = C::QS, SB = C::SB, JOBS = C::JOBS, WGS = C::WGS;
@@ -364,7 +370,7 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
   auto done_job = [&](int i) { cta.done_job(i); };
 
   if (warp == 3) {
-    find_jobs<1>(cta, tb, ht);
+    find_jobs<1>(cta, take, tb, ht);
   } else if (warp == 0) {
     fetch_keys<D, RS>(cta, lg, tmk, sm + C::R_OFF, r_full, r_empty);
   } else if (warp == 1) {
@@ -621,7 +627,7 @@ struct Few {
 
 template <typename T, int D>
 __global__ void __launch_bounds__(Few<D>::THREADS, Few<D>::CTAS)
-    block_weigh_few_kernel(const __grid_constant__ mj_block_weigh_args a, int lg, int hb, int tb, int ht, const __grid_constant__ CUtensorMap tmk) {
+    block_weigh_few_kernel(const __grid_constant__ mj_block_weigh_args a, Take take, int lg, int tb, const __grid_constant__ CUtensorMap tmk) {
   using C = Few<D>;
   constexpr int RS = C::RS, QS = C::QS, SB = C::SB, JOBS = C::JOBS, N = C::N, R = C::R;
   extern __shared__ __align__(1024) unsigned char sm[];
@@ -672,12 +678,12 @@ __global__ void __launch_bounds__(Few<D>::THREADS, Few<D>::CTAS)
   const int h_r = a.h_q / a.h_k;
 
   if (warp == 3) {
-    find_jobs<4>(cta, tb, ht);
+    find_jobs<4>(cta, take, tb, 1);
   } else if (warp == 0) {
     fetch_keys<D, RS>(cta, lg, tmk, sm + C::R_OFF, r_full, r_empty);
   } else if (warp == 1) {
     // ------------------------------------------------------------------------- Q
-    // Row r of a tile is (token r / hb, head r % hb of the tile's). D / 8 lanes read
+    // Row r of a tile is (token r / h_r, head r % h_r of the group). D / 8 lanes read
     // a row; a pass is the rows that a warp reads at once.
     constexpr int LPR = D / 8, RPP = 32 / LPR, PASSES = R / RPP;
     const int c = lane % LPR, row_of_lane = lane / LPR;
@@ -689,15 +695,15 @@ __global__ void __launch_bounds__(Few<D>::THREADS, Few<D>::CTAS)
 #pragma unroll 1
       for (int x = 0; ok && x < nk; ++x)
 #pragma unroll 1
-        for (int tok = j.t0[x], head = 0; tok < n; ++iq) {
-          const int count = min(hb, h_r - head) * min(tb, n - tok), s = iq % QS;
+        for (int tok = j.t0[x]; tok < n; tok += tb, ++iq) {
+          const int count = h_r * min(tb, n - tok), s = iq % QS;
           uint4 raw[PASSES];
           float z[PASSES];
 #pragma unroll
           for (int p = 0; p < PASSES; ++p) {
             const int r = p * RPP + row_of_lane;
             if (r < count) {
-              const int64_t t = q0 + tok + r / hb, hq = h0 + head + r % hb;
+              const int64_t t = q0 + tok + r / h_r, hq = h0 + r % h_r;
               raw[p] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + t * a.q_stride_tok + hq * a.q_stride_head + 8 * c);
               z[p] = __ldg(a.lse + t * a.h_q + hq);
             }
@@ -745,11 +751,6 @@ __global__ void __launch_bounds__(Few<D>::THREADS, Few<D>::CTAS)
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(&q_full[s]);
-          head += hb;
-          if (head >= h_r) {
-            head = 0;
-            tok += tb;
-          }
         }
       if (ok) cta.done_job(i);
     }
@@ -808,16 +809,16 @@ __global__ void __launch_bounds__(Few<D>::THREADS, Few<D>::CTAS)
       for (int x = 0; ok && x < nk; ++x, w += KEYS) {
         const int key = (j.kt + x) * KEYS + t, tiles = j.tiles[x];
         float sum = 0.f, low = 0.f;  // the sum, and what its rounding lost
-        int tok = j.t0[x], head = 0;
+        int tok = j.t0[x];
 #pragma unroll 1
-        for (int tile = 0; tile < tiles; ++tile, ++it) {
+        for (int tile = 0; tile < tiles; ++tile, tok += tb, ++it) {
           const int b = it % SB, s = iq % QS;
           ok = cta.wait_warp(&s_full[b], it / SB);
           if (!ok) break;
           tc_fence_after();
           const float scale = j.scale[x * (KEYS / 16) + (t >> 4)];
           // rows of queries that are there and see the key
-          const int r_lo = max(key - ahead - tok, 0) * hb, r_hi = min(min(n - tok, tb) * hb, h_r - head + (tb - 1) * hb);
+          const int r_lo = max(key - ahead - tok, 0) * h_r, r_hi = min(n - tok, tb) * h_r;
           float p = 0.f;
 #pragma unroll
           for (int r0 = 0; r0 < R; r0 += 8) {
@@ -844,11 +845,6 @@ __global__ void __launch_bounds__(Few<D>::THREADS, Few<D>::CTAS)
           const float next = sum + p;
           low = p - (next - sum);
           sum = next;
-          head += hb;
-          if (head >= h_r) {
-            head = 0;
-            tok += tb;
-          }
         }
         if (ok && key < L) put(w, sum, key >= ahead);
       }
@@ -900,7 +896,7 @@ static bool key_map(CUtensorMap* m, const mj_block_weigh_args& a) {
 }
 
 template <typename T, int D, int N>
-static cudaError_t launch_t(const mj_block_weigh_args& a, cudaStream_t stream) {
+static cudaError_t launch_t(const mj_block_weigh_args& a, Take take, cudaStream_t stream) {
   using C = Cfg<T, D, N>;
   auto kern = block_weigh_kernel<T, D, N>;
   static std::atomic<int> ready[kMaxDevices];
@@ -920,11 +916,11 @@ static cudaError_t launch_t(const mj_block_weigh_args& a, cudaStream_t stream) {
                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
       return cudaErrorInvalidValue;
   }
-  return launch_kernel(kern, dim3((unsigned)grid), dim3(C::THREADS), C::SMEM, stream, a, block_log2(a.kv_format), hb, tb, ht, mk, mq);
+  return launch_kernel(kern, dim3((unsigned)grid), dim3(C::THREADS), C::SMEM, stream, a, take, block_log2(a.kv_format), hb, tb, ht, mk, mq);
 }
 
 template <typename T, int D>
-static cudaError_t launch_few(const mj_block_weigh_args& a, cudaStream_t stream) {
+static cudaError_t launch_few(const mj_block_weigh_args& a, Take take, cudaStream_t stream) {
   using C = Few<D>;
   auto kern = block_weigh_few_kernel<T, D>;
   static std::atomic<int> ready[kMaxDevices];
@@ -933,22 +929,30 @@ static cudaError_t launch_few(const mj_block_weigh_args& a, cudaStream_t stream)
   if (e != cudaSuccess) return e;
   CUtensorMap mk;
   if (!key_map(&mk, a)) return cudaErrorInvalidValue;
-  const int h_r = a.h_q / a.h_k, hb = h_r < C::R ? h_r : C::R, tb = C::R / hb, ht = (h_r + hb - 1) / hb;
-  return launch_kernel(kern, dim3((unsigned)grid), dim3(C::THREADS), C::SMEM, stream, a, block_log2(a.kv_format), hb, tb, ht, mk);
+  return launch_kernel(kern, dim3((unsigned)grid), dim3(C::THREADS), C::SMEM, stream, a, take, block_log2(a.kv_format), C::R / (a.h_q / a.h_k), mk);
 }
 
 template <typename T>
 static cudaError_t launch_d(const mj_block_weigh_args& a, cudaStream_t stream) {
-  // The kernel for few rows where the sequences' rows, on average, are one tile of
-  // its 16, and their queries at most 4 (more may be one sequence's). It makes Q's
-  // terms again for every tile of keys where there are more: 8 sequences of 6K, 16
-  // rows 24 us, 32 rows 65 and with the other kernel 51, 64 rows 120 and 57.
+  // The kernel for few rows takes the sequences whose rows are one tile of its 16:
+  // of more it would make Q's terms again for every tile of keys (8 sequences of
+  // 6K, 16 rows 24 us, 32 rows 65 and with the other kernel 51, 64 rows 120 and
+  // 57). The lengths are the device's, so where there may be both, both are
+  // launched: 64 single tokens of 8K beside a chunk of 512 take BOTH_US, with the kernel
+  // for many rows alone 435, a chunk of 190 beside them with the one for few alone
+  // 717. With no more tokens than sequences all are taken to be single ones.
   const int64_t most = a.window ? (int64_t)a.num_seqs * a.window : a.num_rows, tokens = a.num_rows < most ? a.num_rows : most;
-  const int h_r = a.h_q / a.h_k, fit = h_r > 16 ? 0 : 16 / h_r < 4 ? 16 / h_r : 4;
-  const bool few = tokens <= (int64_t)fit * a.num_seqs;
-  if (few) return a.head_size == 256 ? launch_few<T, 256>(a, stream) : launch_few<T, 128>(a, stream);
-  constexpr int N256 = std::is_same<T, __half>::value ? 64 : 96;  // (fp16's two sums of 96 do not fit TMEM)
-  return a.head_size == 256 ? launch_t<T, 256, N256>(a, stream) : launch_t<T, 128, 128>(a, stream);
+  const int h_r = a.h_q / a.h_k, fit = 16 / h_r;
+  const bool few = fit && (a.num_seqs > 1 || tokens <= fit),
+             many = !few || (tokens > a.num_seqs && tokens > fit);
+  if (many) {
+    constexpr int N256 = std::is_same<T, __half>::value ? 64 : 96;  // (fp16's two sums of 96 do not fit TMEM)
+    const Take take = {few ? fit + 1 : 0, INT_MAX};
+    const cudaError_t e = a.head_size == 256 ? launch_t<T, 256, N256>(a, take, stream) : launch_t<T, 128, 128>(a, take, stream);
+    if (e != cudaSuccess || !few) return e;
+  }
+  const Take take = {0, many ? fit : INT_MAX};
+  return a.head_size == 256 ? launch_few<T, 256>(a, take, stream) : launch_few<T, 128>(a, take, stream);
 }
 
 }  // namespace bw
