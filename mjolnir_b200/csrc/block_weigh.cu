@@ -93,9 +93,13 @@ struct Cta {
   }
 };
 
-// The sequences that a launch takes: those with lo to hi queries that count.
+// The sequences that a launch takes: those with lo to hi queries that count. Of
+// two launches the second begins while the first runs, which let it once all that
+// both read was there; it waits for the first before it ends, for whatever follows
+// waits for the second alone. No two sequences share a weight.
 struct Take {
   int lo, hi;
+  bool both;
 };
 
 // The warp that finds the CTA's jobs: up to TILES tiles of keys of one KV head.
@@ -327,6 +331,7 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
     return;
   }
   griddep_wait();
+  if (take.both) griddep_launch_dependents();
   if (threadIdx.x == 0) {
     auto init = [](uint64_t* b, int n, int count) {
       for (int i = 0; i < n; ++i) mbar_init(b + i, count);
@@ -644,7 +649,7 @@ __global__ void __launch_bounds__(Few<D>::THREADS, Few<D>::CTAS)
     if (threadIdx.x == 0) flag(a.status, MJ_DEV_BAD_SPLIT);
     return;
   }
-  griddep_wait();
+  if (!take.both) griddep_wait();
   if (threadIdx.x == 0) {
     auto init = [](uint64_t* b, int n, int count) {
       for (int i = 0; i < n; ++i) mbar_init(b + i, count);
@@ -857,6 +862,7 @@ __global__ void __launch_bounds__(Few<D>::THREADS, Few<D>::CTAS)
     tc_fence_after();
     tmem_dealloc(tmem, C::TMEM_COLS);
   }
+  if (take.both) griddep_wait();
 }
 
 constexpr int kMaxDevices = 64;
@@ -938,20 +944,21 @@ static cudaError_t launch_d(const mj_block_weigh_args& a, cudaStream_t stream) {
   // of more it would make Q's terms again for every tile of keys (8 sequences of
   // 6K, 16 rows 24 us, 32 rows 65 and with the other kernel 51, 64 rows 120 and
   // 57). The lengths are the device's, so where there may be both, both are
-  // launched: 64 single tokens of 8K beside a chunk of 512 take BOTH_US, with the kernel
-  // for many rows alone 435, a chunk of 190 beside them with the one for few alone
-  // 717. With no more tokens than sequences all are taken to be single ones.
+  // launched: 64 single tokens of 8K beside a chunk of 512 take 151 us, with the
+  // kernel for many rows alone 435; beside a chunk of 190 127, with the one for few
+  // alone 717. (A launch that finds nothing costs 4 us.) With no more tokens than
+  // sequences all are taken to be single ones.
   const int64_t most = a.window ? (int64_t)a.num_seqs * a.window : a.num_rows, tokens = a.num_rows < most ? a.num_rows : most;
   const int h_r = a.h_q / a.h_k, fit = 16 / h_r;
   const bool few = fit && (a.num_seqs > 1 || tokens <= fit),
              many = !few || (tokens > a.num_seqs && tokens > fit);
   if (many) {
     constexpr int N256 = std::is_same<T, __half>::value ? 64 : 96;  // (fp16's two sums of 96 do not fit TMEM)
-    const Take take = {few ? fit + 1 : 0, INT_MAX};
+    const Take take = {few ? fit + 1 : 0, INT_MAX, few};
     const cudaError_t e = a.head_size == 256 ? launch_t<T, 256, N256>(a, take, stream) : launch_t<T, 128, 128>(a, take, stream);
     if (e != cudaSuccess || !few) return e;
   }
-  const Take take = {0, many ? fit : INT_MAX};
+  const Take take = {0, many ? fit : INT_MAX, many};
   return a.head_size == 256 ? launch_few<T, 256>(a, take, stream) : launch_few<T, 128>(a, take, stream);
 }
 
