@@ -208,3 +208,28 @@ def test_twice_at_once():
         assert torch.equal(kept.cpu(), want_k) and torch.equal(wd.cpu(), want_w)
         for side in range(2):
             assert np.array_equal(c.kv[side].cpu().numpy(), codes[side]) and np.array_equal(c.sc[side].cpu().numpy(), exps[side])
+
+
+def test_more_heads_than_the_gpu_holds():
+    lens = [40 + 3 * i for i in range(120)]
+    check(Cache(lens, h_k=3, seed=11), 64, 7)
+
+
+@pytest.mark.parametrize("d,n,budget", [(256, 1, 9000), (256, 2, 700), (128, 3, 1024), (128, 5, 1025)])
+def test_long_of_several_sequences(d, n, budget):
+    """Tokens beyond those whose keys a CTA holds, in every size of cluster."""
+    check(Cache([20000 + 61 * i for i in range(n)], h_k=1 if n < 3 else 4, d=d, page=64, block=64, seed=n + d), budget, 64)
+
+
+def test_weights_heads_outermost():
+    from mjolnir_b200 import kvblock
+
+    c = Cache([300, 90], h_k=2, seed=12)
+    w = torch.rand(2, 2, 300, generator=c.g)
+    wd = w.transpose(0, 1).contiguous().cuda().transpose(0, 1)
+    new, kept = torch.zeros(2, dtype=torch.int32, device="cuda"), torch.zeros(2, 2, 100, dtype=torch.int32, device="cuda")
+    kvblock.evict(wd, *c.args, c.table.cuda(), torch.tensor(c.lens, dtype=torch.int32, device="cuda"), new, kept, recent=3)
+    codes, exps, want_w, want_k = evict_plain(c, w, 100, 3)
+    assert torch.equal(kept.cpu(), want_k) and torch.equal(wd.cpu(), want_w)
+    for side in range(2):
+        assert np.array_equal(c.kv[side].cpu().numpy(), codes[side]) and np.array_equal(c.sc[side].cpu().numpy(), exps[side])
