@@ -434,6 +434,16 @@ int mj_block_join(const mj_block_join_args* args, void* stream) {
   return cuda_status(mj::launch_block_join(a, (cudaStream_t)stream), "mj_block_join launch");
 }
 
+// Whether rows of `cols` elements of an (n0, n1) array share some, whose dims lie one outside the other.
+static bool rows_overlap(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t cols) {
+  if (n0 > 1 && n1 > 1) {
+    const bool swap = s0 < s1;
+    const int64_t outer = swap ? s1 : s0, inner = swap ? s0 : s1, n = swap ? n0 : n1;
+    return inner < cols || outer < (__int128)inner * (n - 1) + cols;
+  }
+  return (n0 > 1 && s0 < cols) || (n1 > 1 && s1 < cols);
+}
+
 int mj_block_weigh(const mj_block_weigh_args* args, void* stream) {
   if (!args) return fail(MJ_ERR_INVALID, "mj_block_weigh: null args");
   const mj_block_weigh_args& a = *args;
@@ -458,8 +468,8 @@ int mj_block_weigh(const mj_block_weigh_args* args, void* stream) {
     return fail(MJ_ERR_INVALID, "mj_block_weigh: null pointer argument");
   if (a.weights_cols < 0 || a.w_stride_seq < 0 || a.w_stride_head < 0)
     return fail(MJ_ERR_INVALID, "mj_block_weigh: weights of %lld columns", (long long)a.weights_cols);
-  if ((a.num_seqs > 1 && !a.w_stride_seq) || (a.h_k > 1 && !a.w_stride_head))
-    return fail(MJ_ERR_UNSUPPORTED, "mj_block_weigh: a weights stride of 0");
+  if (rows_overlap(a.num_seqs, a.w_stride_seq, a.h_k, a.w_stride_head, a.weights_cols))
+    return fail(MJ_ERR_UNSUPPORTED, "mj_block_weigh: a weights stride by which rows share elements");
   if (!aligned(a.q, 16) || a.q_stride_tok % 8 || a.q_stride_head % 8 || a.q_stride_tok < 0 || a.q_stride_head < 0)
     return fail(MJ_ERR_UNSUPPORTED, "mj_block_weigh: q rows must be 16-byte aligned");
   if ((a.num_rows > 1 && !a.q_stride_tok) || (a.h_q > 1 && !a.q_stride_head))
@@ -486,10 +496,10 @@ int mj_block_evict(const mj_block_evict_args* args, void* stream) {
   }
   if (!a.block_table || a.block_table_cols <= 0 || !a.seq_lens || !a.weights || !a.new_lens || (a.budget && !a.kept))
     return fail(MJ_ERR_INVALID, "mj_block_evict: null pointer argument");
-  if (a.weights_cols < 0 || a.weights_cols > INT32_MAX || a.w_stride_seq < 0 || a.w_stride_head < 0)
+  if (a.weights_cols < 0 || a.weights_cols > INT32_MAX - 65536 || a.w_stride_seq < 0 || a.w_stride_head < 0)
     return fail(MJ_ERR_INVALID, "mj_block_evict: weights of %lld columns", (long long)a.weights_cols);
-  if ((a.num_seqs > 1 && !a.w_stride_seq) || (a.h_k > 1 && !a.w_stride_head))
-    return fail(MJ_ERR_UNSUPPORTED, "mj_block_evict: a weights stride of 0");
+  if (rows_overlap(a.num_seqs, a.w_stride_seq, a.h_k, a.w_stride_head, a.weights_cols))
+    return fail(MJ_ERR_UNSUPPORTED, "mj_block_evict: a weights stride by which rows share elements");
   if (a.new_lens < a.seq_lens + a.num_seqs && a.seq_lens < a.new_lens + a.num_seqs)
     return fail(MJ_ERR_INVALID, "mj_block_evict: new_lens overlaps seq_lens, which every KV head reads");
   if ((int64_t)a.num_seqs * a.h_k > 1 << 24 || a.budget > 1 << 24) return fail(MJ_ERR_UNSUPPORTED, "mj_block_evict: too many rows");

@@ -150,3 +150,20 @@ def test_c_entries_refuse():
     e.w_stride_seq = 8
     with pytest.raises(_lib.MjolnirError, match="stride of 0"):
         _lib.block_evict(e, 0)
+
+
+@pytest.mark.parametrize("n,h_k,seq,head,good", [
+    (3, 2, 20, 10, True), (3, 2, 10, 30, True), (3, 2, 19, 10, False), (3, 2, 10, 29, False), (3, 2, 10, 10, False),
+    (3, 2, 20, 9, False), (3, 1, 10, 0, True), (3, 1, 9, 0, False), (1, 2, 0, 10, True), (1, 2, 0, 9, False), (1, 1, 0, 0, True),
+    (3, 2, 2**62, 10, True), (3, 2, 2**62, 2**62 - 1, False),
+])
+def test_rows_of_weights_share_nothing(n, h_k, seq, head, good):
+    """The strides pass, and the next check refuses; or they do not."""
+    one = ctypes.create_string_buffer(1024)
+    at = (ctypes.addressof(one) + 255) // 256 * 256
+    e = _lib.BlockEvictArgs()
+    e.num_seqs, e.budget, e.h_k, e.head_size, e.page_size, e.num_pages, e.kv_format = n, 4, h_k, 128, 16, 1, _lib.BLOCK_FORMATS[16]
+    e.k_cache = e.v_cache = e.k_scales = e.v_scales = e.block_table = e.weights = e.kept = e.seq_lens = e.new_lens = at
+    e.block_table_cols, e.weights_cols, e.w_stride_seq, e.w_stride_head = 1, 10, seq, head
+    with pytest.raises(_lib.MjolnirError, match="new_lens overlaps" if good else "weights stride"):
+        _lib.block_evict(e, 0)

@@ -253,3 +253,56 @@ def test_on_another_stream():
             fresh[s, :, L - 1] = True  # the step's own token starts anew each time
         total = torch.where(fresh, want, 3 * want)
         assert ((w.cpu().double() - total).abs() <= 4 * tol).all()
+
+
+@pytest.mark.parametrize("d,h_q,h_k,page", [(128, 8, 2, 16), (256, 5, 1, 64), (128, 16, 1, 32)])
+@pytest.mark.parametrize("window", [0, 3])
+def test_single_tokens_beside_chunks(d, h_q, h_k, page, window):
+    """A sequence of few rows and one of many go different ways in one call; more than 32 sequences."""
+    q_lens = [1, 140, 1, 0, 4, 1, 17, 2] + [1] * 30 + [3, 66]
+    ctx = [300, 5, 128, 12, 0, 700, 255, 40] + [9 * i for i in range(30)] + [127, 400]
+    check(Cache([a + b for a, b in zip(q_lens, ctx)], h_k=h_k, d=d, page=page, seed=d + window), q_lens, h_q, window=window)
+
+
+def test_no_more_tokens_than_sequences():
+    """All taken for single ones, yet one has most of them."""
+    check(Cache([90, 300, 0, 7] + [0] * 200, h_k=2, seed=21), [1, 150, 0, 2] + [0] * 200, 8)
+
+
+def test_graph_whose_sequences_change_places():
+    """Captured with a chunk and single tokens, replayed with the chunk elsewhere, grown or gone."""
+    from mjolnir_b200 import kvblock
+
+    c = Cache([400, 300, 500], h_k=2, seed=22)
+    q = torch.randn(120, 8, 128, generator=c.g).bfloat16()
+    qd, table, lens = q.cuda(), c.table.cuda(), torch.tensor(c.lens, dtype=torch.int32, device="cuda")
+    ld, offsets, w = torch.zeros(120, 8, device="cuda"), offsets_of([1, 70, 1]), torch.zeros(3, 2, 500, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    kvblock.weigh(qd, ld, c.kv[0], c.sc[0], table, offsets, lens, w, 128**-0.5)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        kvblock.weigh(qd, ld, c.kv[0], c.sc[0], table, offsets, lens, w, 128**-0.5)
+    for q_lens in ([1, 70, 1], [70, 1, 1], [1, 1, 1], [60, 0, 60], [4, 5, 3]):
+        n = sum(q_lens)
+        lse = attention_plain(c, q[:n], q_lens, 128**-0.5)[1].float()
+        ld[:n] = lse.cuda()
+        offsets.copy_(offsets_of(q_lens))
+        w.zero_()
+        graph.replay()
+        want, tol = weigh_plain(c, q[:n], lse, q_lens, torch.zeros(3, 2, 500), 128**-0.5)
+        assert ((w.cpu().double() - want).abs() <= tol).all(), q_lens
+
+
+def test_heads_outermost():
+    """Weights as (heads, sequences, tokens) in memory, K's views of a cache whose heads are outermost too."""
+    from mjolnir_b200 import kvblock
+
+    c = Cache([260, 45], h_k=2, seed=23)
+    q = torch.randn(31, 6, 128, generator=c.g).bfloat16()
+    lse = attention_plain(c, q, [30, 1], 128**-0.5)[1].float()
+    k = c.kv[0].permute(2, 0, 1, 3).contiguous().permute(1, 2, 0, 3)
+    e = c.sc[0].permute(2, 0, 1).contiguous().permute(1, 2, 0)
+    w = torch.zeros(2, 2, 260, device="cuda").transpose(0, 1)
+    kvblock.weigh(q.cuda(), lse.cuda(), k, e, c.table.cuda(), offsets_of([30, 1]), torch.tensor(c.lens, dtype=torch.int32, device="cuda"), w, 128**-0.5)
+    want, tol = weigh_plain(c, q, lse, [30, 1], torch.zeros(2, 2, 260), 128**-0.5)
+    assert ((w.cpu().double() - want).abs() <= tol).all()
