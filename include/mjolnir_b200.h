@@ -560,11 +560,13 @@ int mj_block_join(const mj_block_join_args* args, void* stream);
 /* `window` ones only where window > 0. old is what the tensor held, but 0 at */
 /* this step's own tokens, j >= seq_lens[s] - n_s. A row whose lse is -inf    */
 /* (it saw no key) adds nothing; a row whose lse is NaN makes the keys it     */
-/* sees NaN. Entries from seq_lens[s] on are left as they were. The sums are  */
-/* taken in a fixed order. A key whose page is outside [0, num_pages) flags   */
-/* MJ_DEV_BAD_PAGE, its entry is unspecified. A sequence longer than          */
-/* weights_cols or than the block table's row, or whose offsets do not lie in */
-/* [0, num_rows], flags MJ_DEV_BAD_LENGTH and is left out.                    */
+/* sees NaN, as does one with NaN elements; what one with infinite elements   */
+/* adds is unspecified (0, an infinity or NaN). Entries from seq_lens[s] on    */
+/* are left as they were. The sums are taken in a fixed order. A key whose    */
+/* page is outside [0, num_pages) flags MJ_DEV_BAD_PAGE, its entry is         */
+/* unspecified. A sequence longer than weights_cols or than the block table's */
+/* row, or whose offsets do not lie in [0, num_rows], flags MJ_DEV_BAD_LENGTH */
+/* and is left out. Rows of weights share no element.                         */
 typedef struct mj_block_weigh_args {
   const void* q;                /* (num_rows, h_q, head_size), head dim contiguous, 16-byte aligned rows */
   int dtype;                    /* MJ_DT_BF16 or MJ_DT_FP16 */

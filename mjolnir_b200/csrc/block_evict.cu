@@ -16,6 +16,11 @@
 //    positions a CTA, whole blocks of scales; the cluster's barrier lies
 //    between its reads and its writes, and the next step's reads (of rows that
 //    this one's writes are below) are on their way into registers meanwhile.
+//
+// What bounds it: latency. Every pass of the selection and every step of the move
+// waits for memory or for the cluster, and there are few of either a CTA. 4
+// sequences of 1.1K tokens cut to 1K, 8 KV heads of 128: 13 us, 8.7 MB; 16 of 8K
+// cut to 2K: 49 us, 2.8 TB/s of what has to move; one of 60K cut to 8K 41 us.
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -168,7 +173,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, D == 256 ? 1 : 2)
   // ---- 1. the threshold
   const int M = L - a.recent, m = budget - a.recent;  // 0 <= m < M
   // Few enough tokens, and every CTA looks through all of them: that costs less
-  // than exchanging histograms.
+  // than exchanging histograms (4 sequences of 1.1K tokens 14.7 us, with the
+  // exchange 26.9; 16 of 8K 49.5 and 49.8).
   const bool alone = M <= KEYS;
   const int part = alone ? M : (M + CL - 1) / CL, t0 = alone ? 0 : min(rank * part, M), n = min(part, M - t0);
   const bool held = part <= KEYS;  // keys are made once

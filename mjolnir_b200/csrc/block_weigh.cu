@@ -5,26 +5,38 @@
 //
 // The scores are computed with the keys in the rows of the product, S^T = K Q^T:
 // a lane of TMEM is a key, so a thread adds up its own key's weights in
-// registers, no two threads meet, and the order of every sum is fixed. A job is
-// (sequence, KV head, tile of 128 keys): its K tile stays, the query rows that
-// see it stream past in tiles of N.
+// registers, no two threads meet, and the order of every sum is fixed: one thread
+// writes an entry, once a call. A job is (sequence, KV head, tile of 128 keys): its
+// K tile stays, the query rows that see it stream past in tiles of N. The block
+// scales, one a key, go into the exponent with the softmax scale.
 //
-// Both operands are 16 bits wide. Q enters as it is, by TMA; K's e4m3 codes are
-// exact in either type, so the products are exact, and the block scales, one a
-// key, go into the exponent with the softmax scale. (fp8 products would need Q
-// in three e4m3 terms to leave an fp32 sum its precision.)
+// Two kernels, by the rows that see a tile. Where they are many, both operands are
+// 16 bits wide: Q enters as it is, by TMA, and K's e4m3 codes are converted, exactly,
+// once for all rows. Where they are few, K enters as stored and Q in three e4m3
+// terms: then reading K is all there is to do, and converting it cost more than
+// reading it.
+//
+// What bounds them. Many: the exponentials, one an (row, key) pair, 16 a clock and
+// SM. A prompt of 8192 tokens, 32 / 8 heads of 128, takes 333 us at 1965 MHz and 345
+// to 360 at the clocks that its power leaves (275 GFLOP at 0.77 to 0.83 PFLOP/s);
+// its exponentials alone are 240 us, the product 170. An eighth of them in
+// arithmetic took 309 us at full clock but 346 under the power limit, and windows
+// 7 % longer: not kept. At head size 256 a few sequences leave SMs idle, since a
+// job's rows are not split: 4096 tokens of 24 / 4 heads 257 us, 128 jobs of up to
+// 256 tiles. Few: HBM. 32 single tokens behind 8K, 32 / 8 heads of 128 (192 MB),
+// 37 us, 5.1 TB/s; head size 256, 16 behind 8K, 23 us, 4.1 TB/s; four behind 1000
+// tokens 6.9 us, which is one job's latency.
 //
 // Jobs need no plan: one warp of each CTA walks the sequences' lengths on the
 // device, so a captured graph replays for whatever they hold. Persistent CTAs
 // take the jobs in rounds, every other round in reverse: a prompt's first keys
 // are seen by all its rows, its last by few.
 //
-// Warp roles: 0 K (page walk, TMA, block scales; where few rows see a tile, four
-// warps of their own behind the others), 1 Q (TMA), 2 MMA, 3 the jobs; then
-// warpgroups that convert K's codes, in turn, and warpgroups that take the S tiles
-// in turn and add up. Every mbarrier wait is bounded; on a timeout the CTA flags
-// MJ_DEV_TIMEOUT, all roles stop, copies and MMAs in flight complete and TMEM is
-// freed.
+// Warp roles: 0 K (page walk, TMA, block scales), 1 Q (TMA; of few rows their
+// terms), 2 MMA, 3 the jobs; then, of many rows, a warpgroup that converts K's
+// codes, and those that take the S tiles in turn and add up. Every mbarrier wait
+// is bounded; on a timeout the CTA flags MJ_DEV_TIMEOUT, all roles stop, copies and
+// MMAs in flight complete and TMEM is freed.
 #include <limits.h>
 #include <math.h>
 
@@ -123,7 +135,9 @@ __device__ __forceinline__ void find_jobs(const C& cta, Take take, int tb, int h
     return m && m >= take.lo && m <= take.hi ? (L + KEYS - 1) / KEYS : 0;
   };
   // Tiles a job: as many as leave every CTA two jobs (each costs its lookups'
-  // latency; a few jobs more than CTAs leave some of them idle).
+  // latency; a few jobs more than CTAs leave some of them idle). 32 single tokens
+  // behind 8K: 59 us with one tile a job, 37 with four; four behind 1000 tokens 6.6
+  // and 8.2.
   int per = 1;
   if (TILES > 1) {
     int64_t tiles = 0;

@@ -306,3 +306,19 @@ def test_heads_outermost():
     kvblock.weigh(q.cuda(), lse.cuda(), k, e, c.table.cuda(), offsets_of([30, 1]), torch.tensor(c.lens, dtype=torch.int32, device="cuda"), w, 128**-0.5)
     want, tol = weigh_plain(c, q, lse, [30, 1], torch.zeros(2, 2, 260), 128**-0.5)
     assert ((w.cpu().double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("q_lens", [[1, 2, 1], [1, 90, 1]])
+def test_rows_that_are_not_finite(q_lens, d):
+    """A row with a NaN makes the keys it sees NaN, one with an infinity at most touches them; nothing else."""
+    c = Cache([200, 200, 140], h_k=2, d=d, seed=24)
+    q = torch.randn(sum(q_lens), 8, d, generator=c.g).bfloat16()
+    lse = attention_plain(c, q, q_lens, d**-0.5)[1].float()
+    old = torch.zeros(3, 2, 200)
+    want, tol = weigh_plain(c, q, lse, q_lens, old, d**-0.5)
+    q[0, 1, 7], q[1, 6, 9] = math.nan, math.inf
+    got, status = run(c, q.cuda(), lse.cuda(), q_lens, old, d**-0.5)
+    ok = (got.double() - want).abs() <= tol
+    sees = 200 - q_lens[1] + 1  # of the row with the infinity
+    assert status == 0 and torch.isnan(got[0, 0]).all() and ok[0, 1].all() and ok[1, 0].all() and ok[1, 1, sees:].all() and ok[2].all()
