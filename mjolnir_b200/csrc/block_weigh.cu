@@ -21,9 +21,7 @@
 // to 360 at the clocks that its power leaves (275 GFLOP at 0.77 to 0.83 PFLOP/s);
 // its exponentials alone are 240 us, the product 170. An eighth of them in
 // arithmetic took 309 us at full clock but 346 under the power limit, and windows
-// 7 % longer: not kept. At head size 256 a few sequences leave SMs idle, since a
-// job's rows are not split: 4096 tokens of 24 / 4 heads 257 us, 128 jobs of up to
-// 256 tiles. Few: HBM. 32 single tokens behind 8K, 32 / 8 heads of 128 (192 MB),
+// 7 % longer: not kept. Few: HBM. 32 single tokens behind 8K, 32 / 8 heads of 128 (192 MB),
 // 37 us, 5.1 TB/s; head size 256, 16 behind 8K, 23 us, 4.1 TB/s; four behind 1000
 // tokens 6.9 us, which is one job's latency.
 //
@@ -69,6 +67,8 @@ struct Job {
   int seq, h, kt, nk, L, n, q0;  // seq < 0: no more; nk tiles of keys from kt on
   int t0[4], tiles[4];           // of each: the first query that counts and sees one of them, tiles of rows from it on
   int one;                       // they have one tile of rows, the same
+  int parts;                     // CTAs of a cluster that share the job: of its tiles of rows, CTA r has r, r + parts, ... (`tiles`
+                                 // counts each CTA's; those of some may lie behind the last row)
   float scale[4 * (KEYS / 16)];
 };
 
@@ -115,9 +115,10 @@ struct Take {
 };
 
 // The warp that finds the CTA's jobs: up to TILES tiles of keys of one KV head.
-// 32 sequences at a time, lane i has the key tiles of sequence s0 + i.
-template <int TILES, class C>
-__device__ __forceinline__ void find_jobs(const C& cta, Take take, int tb, int ht) {
+// 32 sequences at a time, lane i has the key tiles of sequence s0 + i. The CTAs of
+// a cluster take their own jobs, or share one where there are too few.
+template <int TILES, bool SHARE, class C>
+__device__ __forceinline__ void find_jobs(const C& cta, Take take, int tb, int ht, int cluster) {
   const mj_block_weigh_args& a = cta.a;
   const int lane = cta.lane;
   int L = 0, n = 0, q0 = 0;
@@ -149,10 +150,44 @@ __device__ __forceinline__ void find_jobs(const C& cta, Take take, int tb, int h
     }
     while (per < TILES && tiles * a.h_k >= 4ll * per * gridDim.x) per *= 2;
   }
+  int parts = 1;
+  if (SHARE) {
+    // What takes longer, in tiles of rows: a job as many and 3 more for its keys, a
+    // shared one its share and 5 more. Jobs before the step's first tokens have all
+    // its rows, the others ever fewer; a lane adds up those of one worker.
+    int jobs = 0, full = 0, rows = 0;
+    for (int s = lane; s - lane < a.num_seqs && jobs < 1 << 20; s += 32) {
+      const int x = tiles_of(s, false);
+      if (x) {
+        jobs += min(x, 1 << 20);
+        full += min(max(L - n, 0) / KEYS, 1 << 20);
+        rows = max(rows, (min(n, a.window ? a.window : n) + tb - 1) / tb * ht);
+      }
+    }
+    jobs = __reduce_add_sync(0xffffffffu, min(jobs, 1 << 20));
+    full = __reduce_add_sync(0xffffffffu, min(full, 1 << 20));
+    rows = __reduce_max_sync(0xffffffffu, rows);
+    if ((int64_t)jobs * a.h_k <= 3 * (int)gridDim.x) {
+      jobs *= a.h_k;
+      full *= a.h_k;
+      const float fall = jobs > full ? 1.f / (float)(jobs - full) : 0.f;
+      auto time_of = [&](int share, float more) {
+        const int w = (int)gridDim.x / share, at = lane * (w - 1) / 31;
+        float sum = 0.f;
+        for (int r = 0; r * w < jobs; ++r) {
+          const int job = r * w + (r & 1 ? w - 1 - at : at);
+          if (job < jobs) sum += more + ceilf((float)rows * (job < full ? 1.f : 1.f - (float)(job - full) * fall) / (float)share);
+        }
+        return __reduce_max_sync(0xffffffffu, (uint32_t)sum);
+      };
+      if (time_of(cluster, 5.f) < time_of(1, 3.f)) parts = cluster;
+    }
+  }
+  const int workers = (int)gridDim.x / parts, me = (int)blockIdx.x / parts;
   int s0 = -32, i = 0;
   int64_t base = 0, total = 0, before = 0, count = 0;
   for (int64_t round = 0;; ++round, ++i) {
-    const int64_t p = round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+    const int64_t p = round * workers + (round & 1 ? workers - 1 - me : me);
     bool more = true;
     while (p >= base + total) {
       base += total;
@@ -192,8 +227,10 @@ __device__ __forceinline__ void find_jobs(const C& cta, Take take, int tb, int h
       j.q0 = q0;
       for (int x = 0; x < j.nk; ++x) {
         j.t0[x] = max(a.window ? max(n - a.window, 0) : 0, (j.kt + x) * KEYS - (L - n));
-        j.tiles[x] = (n - j.t0[x] + tb - 1) / tb * ht;
+        const int tiles = (n - j.t0[x] + tb - 1) / tb * ht;
+        j.tiles[x] = parts > 1 ? (tiles + parts - 1) / parts : tiles;
       }
+      j.parts = parts;
       j.one = j.tiles[0] == 1 && j.t0[j.nk - 1] == j.t0[0];  // (t0 grows with x)
       mbar_arrive(&cta.j_full[i % C::JOBS]);
     }
@@ -274,6 +311,42 @@ __device__ __forceinline__ void put(float* w, float sum, bool begins) {
   else atomicAdd(w, sum);
 }
 
+// ---- what CTAs of a cluster say to one another
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// `p` of CTA `rank`'s shared memory
+__device__ __forceinline__ uint32_t at_rank(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void store_there(uint32_t at, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory"); }
+__device__ __forceinline__ void arrive_there(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// For a phase that another CTA's threads complete; bounded as mbar_wait.
+__device__ __forceinline__ bool wait_others(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  const uint64_t t0 = globaltimer();
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_addr(bar)), "r"(parity), "r"(20000u)
+        : "memory");
+    if (ok) return true;
+    if (*abort_flag || globaltimer() - t0 > kWaitNs) return false;
+  }
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // ------------------------------------------------------------- many rows a tile
 template <typename T, int D, int N>
 struct Cfg {
@@ -293,10 +366,12 @@ struct Cfg {
   static constexpr int SN = SPLIT ? 2 * N : N;
   static_assert(SB * SN <= 512, "S buffers");
   static constexpr int JOBS = 16;  // (K is fetched for jobs that far ahead: 8 sequences of 6K, 64 rows 57 us with 4, 42 with 16)
+  static constexpr int PARTS = 8;  // CTAs of a cluster, at most; each but the first has a buffer in that one for each warpgroup's sums
   static constexpr int PAIRS = WGS * (WGS - 1);  // of a warpgroup that writes weights and one that adds its part
   static constexpr int K_OFF = 0, R_OFF = K_OFF + KS * K16, Q_OFF = R_OFF + RS * RAW, Z_OFF = Q_OFF + QS * QST;
-  static constexpr int RED_OFF = Z_OFF + 3 * WGS * N * 4, JOB_OFF = RED_OFF + PAIRS * KEYS * 4, BAR_OFF = JOB_OFF + JOBS * (int)sizeof(Job);
-  static constexpr int NBARS = 2 * (RS + KS + QS + SB + JOBS + PAIRS) + WGS + 1;
+  static constexpr int RED_OFF = Z_OFF + 3 * WGS * N * 4, X_OFF = RED_OFF + PAIRS * KEYS * 4;
+  static constexpr int JOB_OFF = X_OFF + (PARTS - 1) * WGS * KEYS * 4, BAR_OFF = JOB_OFF + JOBS * (int)sizeof(Job);
+  static constexpr int NBARS = 2 * (RS + KS + QS + SB + JOBS + PAIRS) + WGS + 1 + PARTS * WGS;
   static constexpr int MISC_OFF = BAR_OFF + NBARS * 8;
   static constexpr int SMEM = MISC_OFF + 16;
   static_assert(SMEM <= 232448, "shared memory of a CTA");
@@ -323,9 +398,10 @@ __device__ __forceinline__ void widen16(uint4 c, uint32_t* o) {
   }
 }
 
-template <typename T, int D, int N>
+// SHARE: for clusters
+template <typename T, int D, int N, bool SHARE>
 __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
-    block_weigh_kernel(const __grid_constant__ mj_block_weigh_args a, Take take, int lg, int hb, int tb, int ht,
+    block_weigh_kernel(const __grid_constant__ mj_block_weigh_args a, Take take, int cluster, int lg, int hb, int tb, int ht,
                        const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmq) {
   using C = Cfg<T, D, N>;
   constexpr int RS = C::RS, KS = C::KS, QS = C::QS, SB = C::SB, JOBS = C::JOBS, WGS = C::WGS;
@@ -334,7 +410,8 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::BAR_OFF);
   uint64_t *r_full = bars, *r_empty = r_full + RS, *k_full = r_empty + RS, *k_empty = k_full + KS, *q_full = k_empty + KS,
            *q_empty = q_full + QS, *s_full = q_empty + QS, *s_empty = s_full + SB, *j_full = s_empty + SB, *j_empty = j_full + JOBS,
-           *red_full = j_empty + JOBS, *red_empty = red_full + C::PAIRS, *z_full = red_empty + C::PAIRS, *drain = z_full + WGS;
+           *red_full = j_empty + JOBS, *red_empty = red_full + C::PAIRS, *z_full = red_empty + C::PAIRS, *drain = z_full + WGS,
+           *x_full = drain + 1, *x_empty = x_full + (C::PARTS - 1) * WGS;
   Job* jobs = reinterpret_cast<Job*>(sm + C::JOB_OFF);
   float* red = reinterpret_cast<float*>(sm + C::RED_OFF);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::MISC_OFF);
@@ -363,6 +440,8 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
     init(red_full, C::PAIRS, 128);
     init(red_empty, C::PAIRS, 128);
     init(z_full, WGS, 128);
+    init(x_full, (C::PARTS - 1) * WGS, 128);
+    init(x_empty, WGS, 128);
     mbar_init(drain, 1);
     *abort_flag = 0;
     never_abort = 0;
@@ -380,40 +459,36 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
     tmem_relinquish();
   }
   tc_fence_before();
-  __syncthreads();
+  if (SHARE) cluster_sync();  // (nobody arrives at a barrier that is not there yet)
+  else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  const uint32_t rank = SHARE ? cluster_rank() : 0;
   const Cta<JOBS> cta{a, jobs, j_full, j_empty, abort_flag, &never_abort, lane};
   auto wait_warp = [&](uint64_t* bar, int phase) { return cta.wait_warp(bar, phase); };
   auto next_job = [&](int i) { return cta.next_job(i); };
   auto done_job = [&](int i) { cta.done_job(i); };
 
   if (warp == 3) {
-    find_jobs<1>(cta, take, tb, ht);
+    find_jobs<1, SHARE>(cta, take, tb, ht, cluster);
   } else if (warp == 0) {
     fetch_keys<D, RS>(cta, lg, tmk, sm + C::R_OFF, r_full, r_empty);
   } else if (warp == 1) {
     // ------------------------------------------------------------------------- Q
     // Column c of a tile is (token c / hb, head c % hb of the tile's).
-    const int h_r = a.h_q / a.h_k;
     const uint64_t policy = l2_policy_evict_normal();
     int it = 0;
     bool ok = true;
     for (int i = 0; ok && next_job(i); ++i) {
       const Job& j = jobs[i % JOBS];
-      const int h = j.h, n = j.n, q0 = j.q0;
-      for (int tok = j.t0[0], head = 0; tok < n; ++it) {
-        const int s = it % QS;
+      const int h = j.h, q0 = j.q0 + j.t0[0], tiles = j.tiles[0], parts = SHARE ? j.parts : 1;
+      for (int tile = 0, at = parts > 1 ? rank : 0; tile < tiles; ++tile, at += parts, ++it) {
+        const int s = it % QS, tok = (ht == 1 ? at : at / ht) * tb, head = ht == 1 ? 0 : at % ht * hb;  // (rows behind the last tensor row: zeros)
         ok = wait_warp(&q_empty[s], it / QS + 1);
         if (!ok) break;
         if (lane == 0) mbar_arrive_expect_tx(&q_full[s], (D / 64) * 128 * hb * tb);
         __syncwarp();
         if (lane < D / 64) tma_load_4d(sm + C::Q_OFF + s * C::QST + lane * (N * 128), &tmq, &q_full[s], lane * 64, head, h, q0 + tok, policy);
-        head += hb;
-        if (head >= h_r) {
-          head = 0;
-          tok += tb;
-        }
       }
       if (ok) done_job(i);
     }
@@ -502,9 +577,10 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
     int z_stored = 0, z_seen = 0;
     // this thread's column: its lse in tile `tile` of the queries from t0 on
     const int z_tok = t < hb * tb ? t / hb : INT_MAX / 2, z_head = t % hb;
-    auto tok_of = [&](int t0, int tile) { return t0 + (ht == 1 ? tile : tile / ht) * tb; };
+    int parts = 1, part0 = 0;  // of the job: its CTAs, and this one's place
+    auto tok_of = [&](int t0, int tile) { return t0 + (ht == 1 ? tile * parts + part0 : (tile * parts + part0) / ht) * tb; };
     auto load_lse = [&](const Job& j, int t0, int tile) {
-      const int tok = tok_of(t0, tile), head = ht == 1 ? z_head : tile % ht * hb + z_head;
+      const int tok = tok_of(t0, tile), head = ht == 1 ? z_head : (tile * parts + part0) % ht * hb + z_head;
       return z_tok < j.n - tok && head < h_r ? __ldg(a.lse + (int64_t)(j.q0 + tok + z_tok) * a.h_q + j.h * h_r + head) : -INFINITY;
     };
     auto store_lse = [&](float z) {
@@ -549,10 +625,15 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
       return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
     };
     int it = 0, gave[WGS] = {}, took[WGS] = {};  // tiles; parts given at each place, and taken from it
+    int x_jobs = 0;                              // shared jobs whose sums came together in this warpgroup
     bool ok = true;
     for (int i = 0; ok && next_job(i); ++i) {
       const Job& j = jobs[i % JOBS];
       const int ahead = j.L - j.n, n = j.n, L = j.L, key = j.kt * KEYS + t, t0 = j.t0[0], tiles = j.tiles[0];
+      if (SHARE) {
+        parts = j.parts;
+        part0 = parts > 1 ? rank : 0;
+      }
       // The warpgroups take the tiles in turn; this one has the job's tiles
       // place, place + WGS, ... The first place writes the weights.
       const int place = (wg - it) & (WGS - 1), it0 = it;
@@ -608,7 +689,37 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
         }
       }
       if (!ok) break;
-      if (place == 0 && key < L) put(w, sum, key >= ahead);
+      if (SHARE && place == 0 && parts > 1) {
+        // The other CTAs' sums, in their order. All have as many tiles, so it is the
+        // same warpgroup's everywhere, and each has a buffer and barriers of its own.
+        auto wait_x = [&](uint64_t* bar, int phase) {
+          const bool there = wait_others(bar, (uint32_t)phase & 1u, abort_flag);
+          if (!there && !*abort_flag) {
+            *abort_flag = 1;
+            flag(a.status, MJ_DEV_TIMEOUT);
+          }
+          return __all_sync(0xffffffffu, there) != 0;
+        };
+        float* const xbuf = reinterpret_cast<float*>(sm + C::X_OFF);
+        if (rank) {
+          const int b = ((int)rank - 1) * WGS + wg;
+          ok = wait_x(&x_empty[wg], x_jobs + 1);
+          if (!ok) break;
+          store_there(at_rank(xbuf + b * KEYS + t, 0), sum);
+          arrive_there(at_rank(&x_full[b], 0));
+        } else {
+          for (int r = 1; r < parts; ++r) {
+            const int b = (r - 1) * WGS + wg;
+            ok = wait_x(&x_full[b], x_jobs);
+            if (!ok) break;
+            sum += xbuf[b * KEYS + t];
+            arrive_there(at_rank(&x_empty[wg], r));
+          }
+          if (!ok) break;
+        }
+        ++x_jobs;
+      }
+      if (place == 0 && (!SHARE || part0 == 0) && key < L) put(w, sum, key >= ahead);
       done_job(i);
     }
     tc_fence_before();
@@ -618,6 +729,7 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  if (SHARE) cluster_sync();  // no CTA leaves while another may write to its shared memory
 }
 
 // -------------------------------------------------------------- few rows a tile
@@ -697,7 +809,7 @@ __global__ void __launch_bounds__(Few<D>::THREADS, Few<D>::CTAS)
   const int h_r = a.h_q / a.h_k;
 
   if (warp == 3) {
-    find_jobs<4>(cta, take, tb, 1);
+    find_jobs<4, false>(cta, take, tb, 1, 1);
   } else if (warp == 0) {
     fetch_keys<D, RS>(cta, lg, tmk, sm + C::R_OFF, r_full, r_empty);
   } else if (warp == 1) {
@@ -881,10 +993,10 @@ __global__ void __launch_bounds__(Few<D>::THREADS, Few<D>::CTAS)
 
 constexpr int kMaxDevices = 64;
 
-// The current device, and how many CTAs of a kernel it holds at once (prepared on
-// first use).
+// How many CTAs of a kernel the current device holds at once, in clusters
+// (prepared on first use).
 template <class Kernel>
-static cudaError_t prepare(Kernel kern, int smem, int ctas, std::atomic<int>* ready, int* grid) {
+static cudaError_t prepare(Kernel kern, int threads, int smem, int ctas, int cluster, std::atomic<int>* ready, int* grid) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
@@ -895,6 +1007,21 @@ static cudaError_t prepare(Kernel kern, int smem, int ctas, std::atomic<int>* re
     if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return e;
     if ((e = cudaDeviceGetAttribute(grid, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
     *grid *= ctas;
+    if (cluster > 1) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3((unsigned)cluster);
+      cfg.blockDim = dim3((unsigned)threads);
+      cfg.dynamicSmemBytes = (size_t)smem;
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeClusterDimension;
+      at[0].val.clusterDim.x = (unsigned)cluster;
+      at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+      cfg.attrs = at;
+      cfg.numAttrs = 1;
+      int clusters = 0;
+      if ((e = cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg)) != cudaSuccess) return e;
+      *grid = clusters > 1 ? clusters * cluster : cluster;
+    }
     ready[dev].store(*grid, std::memory_order_release);
   }
   return cudaSuccess;
@@ -918,10 +1045,21 @@ static bool key_map(CUtensorMap* m, const mj_block_weigh_args& a) {
 template <typename T, int D, int N>
 static cudaError_t launch_t(const mj_block_weigh_args& a, Take take, cudaStream_t stream) {
   using C = Cfg<T, D, N>;
-  auto kern = block_weigh_kernel<T, D, N>;
-  static std::atomic<int> ready[kMaxDevices];
+  // CTAs of a cluster, which share a job's rows where there are too few jobs (4096
+  // tokens of 24 / 4 heads of 256 144 us, without 257; 2000 behind 2000 of 6 / 1 heads
+  // 28 and 73). One where there cannot be too few, or where the rows are few tiles,
+  // for looking costs (500 tokens behind 7000, 8 / 2 heads, 22.6 and 19.9 us). Two
+  // otherwise, which fill all SMs; four or eight, which leave 16 and 28 of 148 out,
+  // where the weights are too short for as many jobs.
+  const int64_t most = a.window && a.window < a.num_rows ? a.window : a.num_rows, tiles = (most * (a.h_q / a.h_k) + N - 1) / N;
+  const int64_t least_jobs = (a.num_rows + KEYS - 1) / KEYS * a.h_k, most_jobs = (a.weights_cols + KEYS - 1) / KEYS * a.num_seqs * a.h_k;
+  int level = tiles < 4 || least_jobs >= 300 ? 0 : most_jobs > 60 ? 1 : most_jobs > 15 ? 2 : 3;
+  static_assert(1 << 3 <= C::PARTS, "buffers of a cluster's sums");
+  const int cluster = 1 << level;
+  auto kern = cluster > 1 ? block_weigh_kernel<T, D, N, true> : block_weigh_kernel<T, D, N, false>;
+  static std::atomic<int> ready[4][kMaxDevices];
   int grid = 0;
-  const cudaError_t e = prepare(kern, C::SMEM, 1, ready, &grid);
+  cudaError_t e = prepare(kern, C::THREADS, C::SMEM, 1, cluster, ready[level], &grid);
   if (e != cudaSuccess) return e;
   CUtensorMap mk, mq;
   if (!key_map(&mk, a)) return cudaErrorInvalidValue;
@@ -936,7 +1074,20 @@ static cudaError_t launch_t(const mj_block_weigh_args& a, Take take, cudaStream_
                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
       return cudaErrorInvalidValue;
   }
-  return launch_kernel(kern, dim3((unsigned)grid), dim3(C::THREADS), C::SMEM, stream, a, take, block_log2(a.kv_format), hb, tb, ht, mk, mq);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(C::THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)cluster;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, a, take, cluster, block_log2(a.kv_format), hb, tb, ht, mk, mq);
 }
 
 template <typename T, int D>
@@ -945,7 +1096,7 @@ static cudaError_t launch_few(const mj_block_weigh_args& a, Take take, cudaStrea
   auto kern = block_weigh_few_kernel<T, D>;
   static std::atomic<int> ready[kMaxDevices];
   int grid = 0;
-  const cudaError_t e = prepare(kern, C::SMEM, C::CTAS, ready, &grid);
+  const cudaError_t e = prepare(kern, C::THREADS, C::SMEM, C::CTAS, 1, ready, &grid);
   if (e != cudaSuccess) return e;
   CUtensorMap mk;
   if (!key_map(&mk, a)) return cudaErrorInvalidValue;

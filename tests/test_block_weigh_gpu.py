@@ -322,3 +322,40 @@ def test_rows_that_are_not_finite(q_lens, d):
     ok = (got.double() - want).abs() <= tol
     sees = 200 - q_lens[1] + 1  # of the row with the infinity
     assert status == 0 and torch.isnan(got[0, 0]).all() and ok[0, 1].all() and ok[1, 0].all() and ok[1, 1, sees:].all() and ok[2].all()
+
+
+@pytest.mark.parametrize("lens,q_lens,d,h_q,h_k,window", [
+    ([1000], [1000], 128, 6, 1, 0), ([700], [100], 128, 6, 1, 0), ([2600], [700], 128, 5, 1, 0), ([2600], [701], 256, 6, 1, 100),
+    ([1200, 900, 40], [1200, 300, 40], 128, 8, 4, 0), ([1500], [1500], 256, 6, 3, 0), ([150, 300], [60, 90], 128, 257, 1, 0),
+    ([3000, 1, 800], [600, 1, 800], 128, 12, 2, 0), ([900, 300, 0, 5], [900, 300, 0, 5], 128, 12, 3, 200), ([400], [399], 128, 40, 1, 0),
+])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_few_jobs_of_many_rows(lens, q_lens, d, h_q, h_k, window, dtype):
+    """Jobs whose rows the CTAs of a cluster share: two, four and eight, with and without a tile for each; the same bits every time."""
+    c = Cache(lens, h_k=h_k, d=d, page=32, seed=sum(lens) + h_q)
+    state = c.g.get_state()
+    first = check(c, q_lens, h_q, dtype, window)
+    c.g.set_state(state)
+    again = check(c, q_lens, h_q, dtype, window)
+    assert torch.equal(first, again)
+
+
+def test_shared_jobs_of_two_calls_at_once():
+    from mjolnir_b200 import kvblock
+
+    c = Cache([900, 500], h_k=2, seed=25)
+    q_lens = [900, 400]
+    q = torch.randn(1300, 8, 128, generator=c.g).bfloat16()
+    lse = attention_plain(c, q, q_lens, 128**-0.5)[1].float()
+    args = (q.cuda(), lse.cuda(), c.kv[0], c.sc[0], c.table.cuda(), offsets_of(q_lens), torch.tensor(c.lens, dtype=torch.int32, device="cuda"))
+    outs = [torch.zeros(2, 2, 900, device="cuda") for _ in range(3)]
+    torch.cuda.synchronize()
+    for w in outs:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(4):
+                w.zero_()
+                kvblock.weigh(*args, w, 128**-0.5)
+    torch.cuda.synchronize()
+    want, tol = weigh_plain(c, q, lse, q_lens, torch.zeros(2, 2, 900), 128**-0.5)
+    for w in outs:
+        assert ((w.cpu().double() - want).abs() <= tol).all()
