@@ -182,8 +182,17 @@ def _weights(weights: torch.Tensor, num_seqs: int, h_k: int) -> tuple:
 
 def _side(k_cache: torch.Tensor, k_scales: torch.Tensor) -> tuple:
     """K's part of :func:`_cache`."""
-    shape, kv_format, dev, st, ss = _cache(k_cache, k_cache, k_scales, k_scales)
-    return shape, kv_format, dev, st[:3], ss[:3]
+    shape, sshape, st, ss = k_cache.shape, k_scales.shape, k_cache.stride(), k_scales.stride()
+    if len(shape) != 4 or k_cache.itemsize != 1 or st[3] != 1:
+        raise ValueError(f"k_cache {tuple(shape)} {k_cache.dtype} must be a (pages, page_size, h_k, d) byte view with contiguous rows")
+    pages, page_size, h_k, d = shape
+    if len(sshape) != 3 or k_scales.itemsize != 1 or sshape[0] != pages or sshape[2] != h_k or sshape[1] < 1 or page_size % sshape[1]:
+        raise ValueError(f"k_scales {tuple(sshape)} {k_scales.dtype} must be a ({pages}, {page_size} / G, {h_k}) byte view")
+    kv_format = _format(page_size // sshape[1], page_size, d)
+    st = st[:3]
+    if pages == 1 or h_k == 1:  # a dim of extent 1 may carry any stride
+        st = tuple(0 if n == 1 else x for n, x in zip(shape, st))
+    return shape, kv_format, k_cache.get_device(), st, ss
 
 
 def weigh(
@@ -212,24 +221,26 @@ def weigh(
     call for whatever they hold then."""
     (pages, page_size, h_k, d), kv_format, dev, st, ss = _side(k_cache, k_scales)
     n = seq_lens.shape[0] if seq_lens.dim() == 1 else -1
-    for name, t, m in (("seq_lens", seq_lens, n), ("offsets", offsets, n + 1)):
-        if t.dtype != torch.int32 or t.shape != (m,) or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous int32 ({m if n >= 0 else 'n'},), got {t.dtype} {tuple(t.shape)}")
+    if (seq_lens.dtype != torch.int32 or n < 0 or not seq_lens.is_contiguous() or offsets.dtype != torch.int32
+            or offsets.shape != (n + 1,) or not offsets.is_contiguous()):
+        raise ValueError(f"seq_lens and offsets must be contiguous int32 (n,) and (n + 1,), got {seq_lens.dtype} {tuple(seq_lens.shape)} "
+                         f"and {offsets.dtype} {tuple(offsets.shape)}")
     _table(block_table, n)
-    h_q = query.shape[1] if query.dim() == 3 else 0
+    q_shape, l_shape = query.shape, lse.shape
+    h_q = q_shape[1] if len(q_shape) == 3 else 0
     qs, ws = _rows("query", query, h_q, d), _weights(weights, n, h_k)
     if h_q < 1 or h_q % h_k:
         raise ValueError(f"query heads {h_q} must be a multiple of the cache's {h_k}")
     dt = dtype_code(query.dtype)
     if dt == _lib.MJ_DT_FP32:
         raise TypeError(f"query must be bf16 or fp16, got {query.dtype}")
-    if lse.dtype != torch.float32 or lse.dim() != 2 or lse.shape[1] != h_q or not lse.is_contiguous():
-        raise ValueError(f"lse must be a contiguous fp32 (rows, {h_q}), got {lse.dtype} {tuple(lse.shape)}")
+    if lse.dtype != torch.float32 or len(l_shape) != 2 or l_shape[1] != h_q or not lse.is_contiguous():
+        raise ValueError(f"lse must be a contiguous fp32 (rows, {h_q}), got {lse.dtype} {tuple(l_shape)}")
     if window < 0:
         raise ValueError(f"window {window}")
-    _on(dev, query, lse, block_table, offsets, seq_lens, weights, status)
+    _on(dev, k_scales, query, lse, block_table, offsets, seq_lens, weights, status)
     call(_lib.block_weigh, _lib.BlockWeighArgs(
-        query.data_ptr(), dt, *qs, lse.data_ptr(), min(query.shape[0], lse.shape[0]), n, h_q, h_k, d, page_size, kv_format,
+        query.data_ptr(), dt, *qs, lse.data_ptr(), min(q_shape[0], l_shape[0]), n, h_q, h_k, d, page_size, kv_format,
         k_cache.data_ptr(), *st, k_scales.data_ptr(), *ss, pages, block_table.data_ptr(), block_table.stride(0),
         block_table.shape[1], offsets.data_ptr(), seq_lens.data_ptr(), weights.data_ptr(), *ws, weights.shape[2],
         float(softmax_scale), int(window), _ptr(status)), dev)

@@ -62,28 +62,29 @@ def qk_norm_rope(
     """Normalise and rotate Q and K; returns ``(q_out, k_out)``. A position
     outside the table, on any axis, flags ``MJ_DEV_BAD_POSITION`` in ``status``
     and leaves its token's output rows as they were."""
-    shape, dtype, dev = q.shape, q.dtype, q.get_device()
-    if len(shape) != 3 or len(k.shape) != 3:
-        raise ValueError(f"q {tuple(shape)} and k {tuple(k.shape)} must be (tokens, heads, head_size)")
+    shape, k_shape, dtype, dev = q.shape, k.shape, q.dtype, q.get_device()
+    if len(shape) != 3 or len(k_shape) != 3:
+        raise ValueError(f"q {tuple(shape)} and k {tuple(k_shape)} must be (tokens, heads, head_size)")
     T, h_q, d = shape
-    h_k = k.shape[1]
-    if k.shape[0] != T or k.shape[2] != d or k.dtype != dtype:
-        raise ValueError(f"k {tuple(k.shape)} {k.dtype} does not match q {tuple(shape)} {dtype}")
+    h_k = k_shape[1]
+    if k_shape[0] != T or k_shape[2] != d or k.dtype != dtype:
+        raise ValueError(f"k {tuple(k_shape)} {k.dtype} does not match q {tuple(shape)} {dtype}")
     if q_out is None:
         q_out = torch.empty(shape, dtype=dtype, device=q.device)
     if k_out is None:
-        k_out = torch.empty(k.shape, dtype=dtype, device=q.device)
-    if q_out.shape != shape or q_out.dtype != dtype or k_out.shape != k.shape or k_out.dtype != dtype:
+        k_out = torch.empty(k_shape, dtype=dtype, device=q.device)
+    if q_out.shape != shape or q_out.dtype != dtype or k_out.shape != k_shape or k_out.dtype != dtype:
         raise ValueError(f"q_out {tuple(q_out.shape)} {q_out.dtype} / k_out {tuple(k_out.shape)} {k_out.dtype} do not match q and k")
     qs, ks, qos, kos = q.stride(), k.stride(), q_out.stride(), k_out.stride()
     if qs[2] != 1 or ks[2] != 1 or qos[2] != 1 or kos[2] != 1:
         raise ValueError("the head dim of q, k and the outputs must be contiguous")
-    if positions.dtype != torch.int64 or positions.shape[positions.dim() - 1:] != (T,) or (T > 1 and positions.stride(-1) != 1) or (
-            positions.dim() != (1 if axes is None else 2)):
+    ps, pst = positions.shape, positions.stride()
+    if positions.dtype != torch.int64 or len(ps) != (1 if axes is None else 2) or ps[-1] != T or (T > 1 and pst[-1] != 1):
         raise ValueError(f"positions must be an int64 {f'({T},)' if axes is None else f'(axes, {T})'} with contiguous rows, got "
                          f"{positions.dtype} {tuple(positions.shape)}")
-    if cos_sin.dim() != 2 or (cos_sin.shape[1] > 1 and cos_sin.stride(1) != 1):
-        raise ValueError(f"cos_sin must be (positions, rot_dim) with contiguous rows, got {tuple(cos_sin.shape)}")
+    cs, cst = cos_sin.shape, cos_sin.stride()
+    if len(cs) != 2 or (cs[1] > 1 and cst[1] != 1):
+        raise ValueError(f"cos_sin must be (positions, rot_dim) with contiguous rows, got {tuple(cs)}")
     w_dtype = torch.float32
     for w in (q_weight, k_weight):
         if w is not None:
@@ -97,13 +98,13 @@ def qk_norm_rope(
             raise ValueError(f"every tensor must be on {q.device}, got {t.device}")
     entry, more = _lib.qk_norm_rope, None
     if axes is not None:
-        n = positions.shape[0]
-        more = _lib.RopeAxes(n, positions.stride(0) if n > 1 else 0, _axes(tuple(axes), n, cos_sin.shape[1]))
+        n = ps[0]
+        more = _lib.RopeAxes(n, pst[0] if n > 1 else 0, _axes(tuple(axes), n, cs[1]))
         entry = _lib.qk_norm_rope_axes
     a = _lib.QkNormRopeArgs(
-        q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), dtype_code(dtype), T, h_q, h_k, d, cos_sin.shape[1],
+        q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), dtype_code(dtype), T, h_q, h_k, d, cs[1],
         int(interleaved), qs[0], qs[1], ks[0], ks[1], qos[0], qos[1], kos[0], kos[1], positions.data_ptr(), cos_sin.data_ptr(),
-        dtype_code(cos_sin.dtype), cos_sin.stride(0), cos_sin.shape[0], _ptr(q_weight), _ptr(k_weight), dtype_code(w_dtype),
+        dtype_code(cos_sin.dtype), cst[0], cs[0], _ptr(q_weight), _ptr(k_weight), dtype_code(w_dtype),
         float(eps), _ptr(status))
     call(entry, a if more is None else (a, more), dev)
     return q_out, k_out
