@@ -114,6 +114,16 @@ struct Take {
   bool both;
 };
 
+// Of two launches, one that has none leaves before it takes anything.
+__device__ __forceinline__ bool has_any(const mj_block_weigh_args& a, Take take) {
+  int any = 0;
+  for (int s = threadIdx.x; s < a.num_seqs; s += blockDim.x) {
+    const int n = a.offsets[s + 1] - a.offsets[s], m = a.window && a.window < n ? a.window : n;
+    any |= (m >= take.lo && m <= take.hi) || n < 0;  // (that is complained of)
+  }
+  return __syncthreads_or(any) != 0;
+}
+
 // The warp that finds the CTA's jobs: up to TILES tiles of keys of one KV head.
 // 32 sequences at a time, lane i has the key tiles of sequence s0 + i. The CTAs of
 // a cluster take their own jobs, or share one where there are too few.
@@ -133,7 +143,7 @@ __device__ __forceinline__ void find_jobs(const C& cta, Take take, int tb, int h
       return 0;
     }
     const int m = a.window && a.window < n ? a.window : n;
-    return m && m >= take.lo && m <= take.hi ? (L + KEYS - 1) / KEYS : 0;
+    return m >= take.lo && m <= take.hi ? (L + KEYS - 1) / KEYS : 0;
   };
   // Tiles a job: as many as leave every CTA two jobs (each costs its lookups'
   // latency; a few jobs more than CTAs leave some of them idle). 32 single tokens
@@ -422,7 +432,10 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
     return;
   }
   griddep_wait();
-  if (take.both) griddep_launch_dependents();
+  if (take.both) {
+    griddep_launch_dependents();
+    if (!has_any(a, take)) return;  // (every CTA of a cluster)
+  }
   if (threadIdx.x == 0) {
     auto init = [](uint64_t* b, int n, int count) {
       for (int i = 0; i < n; ++i) mbar_init(b + i, count);
@@ -775,7 +788,12 @@ __global__ void __launch_bounds__(Few<D>::THREADS, Few<D>::CTAS)
     if (threadIdx.x == 0) flag(a.status, MJ_DEV_BAD_SPLIT);
     return;
   }
-  if (!take.both) griddep_wait();
+  if (!take.both) {
+    griddep_wait();
+  } else if (!has_any(a, take)) {
+    griddep_wait();
+    return;
+  }
   if (threadIdx.x == 0) {
     auto init = [](uint64_t* b, int n, int count) {
       for (int i = 0; i < n; ++i) mbar_init(b + i, count);
@@ -1053,7 +1071,7 @@ static cudaError_t launch_t(const mj_block_weigh_args& a, Take take, cudaStream_
   // where the weights are too short for as many jobs.
   const int64_t most = a.window && a.window < a.num_rows ? a.window : a.num_rows, tiles = (most * (a.h_q / a.h_k) + N - 1) / N;
   const int64_t least_jobs = (a.num_rows + KEYS - 1) / KEYS * a.h_k, most_jobs = (a.weights_cols + KEYS - 1) / KEYS * a.num_seqs * a.h_k;
-  int level = tiles < 4 || least_jobs >= 300 ? 0 : most_jobs > 60 ? 1 : most_jobs > 15 ? 2 : 3;
+  int level = tiles < 8 || least_jobs >= 300 ? 0 : most_jobs > 60 ? 1 : most_jobs > 15 ? 2 : 3;
   static_assert(1 << 3 <= C::PARTS, "buffers of a cluster's sums");
   const int cluster = 1 << level;
   auto kern = cluster > 1 ? block_weigh_kernel<T, D, N, true> : block_weigh_kernel<T, D, N, false>;
@@ -1109,9 +1127,9 @@ static cudaError_t launch_d(const mj_block_weigh_args& a, cudaStream_t stream) {
   // of more it would make Q's terms again for every tile of keys (8 sequences of
   // 6K, 16 rows 24 us, 32 rows 65 and with the other kernel 51, 64 rows 120 and
   // 57). The lengths are the device's, so where there may be both, both are
-  // launched: 64 single tokens of 8K beside a chunk of 512 take 151 us, with the
-  // kernel for many rows alone 435; beside a chunk of 190 127, with the one for few
-  // alone 717. (A launch that finds nothing costs 4 us.) With no more tokens than
+  // launched: 64 single tokens of 8K beside a chunk of 512 take 155 us, with the
+  // kernel for many rows alone 435; beside a chunk of 190 131, with the one for few
+  // alone 717. (A launch that finds nothing costs 2 us.) With no more tokens than
   // sequences all are taken to be single ones.
   const int64_t most = a.window ? (int64_t)a.num_seqs * a.window : a.num_rows, tokens = a.num_rows < most ? a.num_rows : most;
   const int h_r = a.h_q / a.h_k, fit = 16 / h_r;
@@ -1119,11 +1137,11 @@ static cudaError_t launch_d(const mj_block_weigh_args& a, cudaStream_t stream) {
              many = !few || (tokens > a.num_seqs && tokens > fit);
   if (many) {
     constexpr int N256 = std::is_same<T, __half>::value ? 64 : 96;  // (fp16's two sums of 96 do not fit TMEM)
-    const Take take = {few ? fit + 1 : 0, INT_MAX, few};
+    const Take take = {few ? fit + 1 : 1, INT_MAX, few};
     const cudaError_t e = a.head_size == 256 ? launch_t<T, 256, N256>(a, take, stream) : launch_t<T, 128, 128>(a, take, stream);
     if (e != cudaSuccess || !few) return e;
   }
-  const Take take = {0, many ? fit : INT_MAX, many};
+  const Take take = {1, many ? fit : INT_MAX, many};
   return a.head_size == 256 ? launch_few<T, 256>(a, take, stream) : launch_few<T, 128>(a, take, stream);
 }
 

@@ -359,3 +359,24 @@ def test_shared_jobs_of_two_calls_at_once():
     want, tol = weigh_plain(c, q, lse, q_lens, torch.zeros(2, 2, 900), 128**-0.5)
     for w in outs:
         assert ((w.cpu().double() - want).abs() <= tol).all()
+
+
+def test_offsets_that_fall():
+    """Flagged, whichever kernel the others go to; they are done all the same."""
+    from mjolnir_b200 import _lib, kvblock
+
+    c = Cache([50, 60, 70], h_k=1, seed=26)
+    q = torch.randn(40, 4, 128, generator=c.g).bfloat16()
+    for offsets, ok in (([0, 1, 0, 0], 0), ([5, 0, 0, 0], None), ([0, 30, 29, 29], 0), ([0, 0, 30, 29], 1)):
+        lse, status, w = torch.zeros(40, 4), torch.zeros(1, dtype=torch.int32, device="cuda"), torch.zeros(3, 1, 70, device="cuda")
+        if ok is not None:
+            n = offsets[ok + 1] - offsets[ok]
+            rows = [n if s == ok else 0 for s in range(3)]
+            lse[offsets[ok]:offsets[ok] + n] = attention_plain(c, q[offsets[ok]:offsets[ok] + n], rows, 128**-0.5)[1].float()
+        kvblock.weigh(q.cuda(), lse.cuda(), c.kv[0], c.sc[0], c.table.cuda(), torch.tensor(offsets, dtype=torch.int32, device="cuda"),
+                      torch.tensor(c.lens, dtype=torch.int32, device="cuda"), w, 128**-0.5, status=status)
+        assert int(status) == _lib.MJ_DEV_BAD_LENGTH
+        want, tol = torch.zeros(3, 1, 70, dtype=torch.float64), torch.zeros(3, 1, 70, dtype=torch.float64)
+        if ok is not None:
+            want, tol = weigh_plain(c, q[offsets[ok]:], lse[offsets[ok]:], rows, torch.zeros(3, 1, 70), 128**-0.5)
+        assert ((w.cpu().double() - want).abs() <= tol).all()
