@@ -28,7 +28,8 @@
 // Jobs need no plan: one warp of each CTA walks the sequences' lengths on the
 // device, so a captured graph replays for whatever they hold. Persistent CTAs
 // take the jobs in rounds, every other round in reverse: a prompt's first keys
-// are seen by all its rows, its last by few.
+// are seen by all its rows, its last by few. Where there are too few jobs, the CTAs
+// of a cluster share the rows of one and its first CTA adds up their sums, in order.
 //
 // Warp roles: 0 K (page walk, TMA, block scales), 1 Q (TMA; of few rows their
 // terms), 2 MMA, 3 the jobs; then, of many rows, a warpgroup that converts K's

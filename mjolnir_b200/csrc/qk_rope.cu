@@ -82,8 +82,8 @@ __device__ __forceinline__ void rotate(float& a, float& b, float c, float s) {
 // team's first threads load and hand round; a thread's 8 angles that follow one
 // axis come from its table row in vectors, others one by one. It is bound as
 // without axes, by HBM and how many rows are on their way: 8192 tokens of 32 / 8
-// heads of 128 on three alternating axes 40 us, 4.3 TB/s (one position a token 35;
-// positions loaded by every thread 47), 16 tokens 2.8 us, a launch.
+// heads of 128 on three axes in turn 40 us, 4.3 TB/s (one position a token 35;
+// positions loaded by every thread 47), 32 tokens 2.8 us, a launch.
 template <typename T, int HG, bool VEC, int TL, typename AX>
 __global__ void __launch_bounds__(128, sizeof(T) == 4 ? 3 : 5)
     qk_norm_rope_kernel(mj_qk_norm_rope_args a, float inv_d, const __grid_constant__ AX ax) {
