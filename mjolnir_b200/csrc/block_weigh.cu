@@ -787,6 +787,7 @@ __global__ void __launch_bounds__(Few<D>::THREADS, Few<D>::CTAS)
   int& never_abort = *reinterpret_cast<int*>(sm + C::MISC_OFF + 8);
   if (reinterpret_cast<uintptr_t>(sm) & 1023) {  // uniform: nothing taken yet
     if (threadIdx.x == 0) flag(a.status, MJ_DEV_BAD_SPLIT);
+    griddep_wait();
     return;
   }
   if (!take.both) {
