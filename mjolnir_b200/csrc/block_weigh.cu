@@ -178,7 +178,7 @@ __device__ __forceinline__ void find_jobs(const C& cta, Take take, int tb, int h
     jobs = __reduce_add_sync(0xffffffffu, min(jobs, 1 << 20));
     full = __reduce_add_sync(0xffffffffu, min(full, 1 << 20));
     rows = __reduce_max_sync(0xffffffffu, rows);
-    if ((int64_t)jobs * a.h_k <= 3 * (int)gridDim.x) {
+    if ((int64_t)jobs * a.h_k <= 3 * (int)gridDim.x) {  // (more even out by themselves)
       jobs *= a.h_k;
       full *= a.h_k;
       const float fall = jobs > full ? 1.f / (float)(jobs - full) : 0.f;
@@ -1067,10 +1067,11 @@ static cudaError_t launch_t(const mj_block_weigh_args& a, Take take, cudaStream_
   using C = Cfg<T, D, N>;
   // CTAs of a cluster, which share a job's rows where there are too few jobs (4096
   // tokens of 24 / 4 heads of 256 144 us, without 257; 2000 behind 2000 of 6 / 1 heads
-  // 28 and 73). One where there cannot be too few, or where the rows are few tiles,
-  // for looking costs (500 tokens behind 7000, 8 / 2 heads, 22.6 and 19.9 us). Two
-  // otherwise, which fill all SMs; four or eight, which leave 16 and 28 of 148 out,
-  // where the weights are too short for as many jobs.
+  // 28 and 73). One where there cannot be too few (300 are two an SM), or where the
+  // rows are few tiles, for looking costs (500 tokens behind 7000, 8 / 2 heads, 22.6
+  // and 19.9 us). Two otherwise, which fill all SMs; four or eight, which leave 16 and
+  // 28 of 148 out, where the weights are too short for 60 or 15 jobs, fewer than half, or
+  // an eighth, of the SMs.
   const int64_t most = a.window && a.window < a.num_rows ? a.window : a.num_rows, tiles = (most * (a.h_q / a.h_k) + N - 1) / N;
   const int64_t least_jobs = (a.num_rows + KEYS - 1) / KEYS * a.h_k, most_jobs = (a.weights_cols + KEYS - 1) / KEYS * a.num_seqs * a.h_k;
   int level = tiles < 8 || least_jobs >= 300 ? 0 : most_jobs > 60 ? 1 : most_jobs > 15 ? 2 : 3;
