@@ -1069,12 +1069,14 @@ static cudaError_t launch_t(const mj_block_weigh_args& a, Take take, cudaStream_
   // tokens of 24 / 4 heads of 256 144 us, without 257; 2000 behind 2000 of 6 / 1 heads
   // 28 and 73). One where there cannot be too few (300 are two an SM), or where the
   // rows are few tiles, for looking costs (500 tokens behind 7000, 8 / 2 heads, 22.6
-  // and 19.9 us). Two otherwise, which fill all SMs; four or eight, which leave 16 and
-  // 28 of 148 out, where the weights are too short for 60 or 15 jobs, fewer than half, or
-  // an eighth, of the SMs.
+  // and 19.9 us). Two otherwise, which fill all SMs. Four or eight, which leave 16 and
+  // 28 of 148 out, where the weights are too short for more jobs than the 33 or 15
+  // clusters: 600 tokens of 6 heads, 15 jobs 28.8, 21.2, 17.2 and 15.8 us with one,
+  // two, four and eight, 24 jobs 28.8, 21.1, 17.2 and 22.5, 36 jobs 29.5, 21.3, 23.3
+  // and 29.3, 80 jobs, where none share, 29.5 and 31 to 32.
   const int64_t most = a.window && a.window < a.num_rows ? a.window : a.num_rows, tiles = (most * (a.h_q / a.h_k) + N - 1) / N;
   const int64_t least_jobs = (a.num_rows + KEYS - 1) / KEYS * a.h_k, most_jobs = (a.weights_cols + KEYS - 1) / KEYS * a.num_seqs * a.h_k;
-  int level = tiles < 8 || least_jobs >= 300 ? 0 : most_jobs > 60 ? 1 : most_jobs > 15 ? 2 : 3;
+  int level = tiles < 8 || least_jobs >= 300 ? 0 : most_jobs > 33 ? 1 : most_jobs > 15 ? 2 : 3;
   static_assert(1 << 3 <= C::PARTS, "buffers of a cluster's sums");
   const int cluster = 1 << level;
   auto kern = cluster > 1 ? block_weigh_kernel<T, D, N, true> : block_weigh_kernel<T, D, N, false>;
