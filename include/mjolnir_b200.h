@@ -471,12 +471,14 @@ typedef struct mj_block_attn_args {
   float softmax_scale;
   int causal;
   /* The plan (mj_block_plan writes it on the host): num_work items of 8 int32
-   * (seq, first row, tile begin, tile end, partial slot or -1, span, 0, 0). A
+   * (seq, first row, tile begin, tile end, partial slot or -1, span, rest, 0). A
    * row is (query token, head of the KV head's group), token-major; an item
    * covers MJ_BLOCK_ROWS(head_size) rows from its first and the keys of its
    * tiles of MJ_BLOCK_KEYS. span = 0: rows of sequence seq. span > 0: rows of
    * sequences seq .. seq + span - 1 taken together, all of which see every key
-   * of the item's tiles, which are read from the pages of sequence seq. Items with a slot leave normalised
+   * of the item's tiles, which are read from the pages of sequence seq. rest = 1:
+   * in fp16 launches without merges the item's weights hold 22 bits instead of 11.
+   * Items with a slot leave normalised
    * partials in o_part / lse_part at [slot][KV head][row]; num_merges entries
    * of 4 int32 (seq, first row, first slot, slots) say which to join. */
   const int32_t* work; int num_work;

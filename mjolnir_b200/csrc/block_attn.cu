@@ -57,7 +57,12 @@
 // items of its own, or the decode kernel's, and block_join_kernel puts a row's
 // partials together. 64 single tokens behind 16K tokens, 32 / 8 heads of 128: 59 us
 // (the prefix 30, 144 CTAs in one round; own keys in the decode kernel 22), each
-// sequence by itself 330.
+// sequence by itself 330. Rows that the decode kernel serves without the group keep
+// its precision where the output shows it: of an fp16 group with such rows P enters
+// as f16 and what that lost, as f16 too, over the other half of S: 22 bits, in
+// steps of 2^-25 of the maximum at least (64 fp16 tokens behind 16K 2.12e-4 from 64
+// bits, as without the group, for 2.82e-4 with P in 11 bits; 62.5 us for 57.5).
+// bf16 outputs are 1.67e-3 off either way.
 //
 // Every mbarrier wait is bounded; on a timeout the CTA flags MJ_DEV_TIMEOUT,
 // all roles stop, the copies and MMAs in flight complete and TMEM is freed.
@@ -173,7 +178,8 @@ struct Pair<__nv_bfloat16> {
   typedef __nv_bfloat162 type;
 };
 
-template <typename T, int D>
+// REST: for launches of items whose weights are held in two terms, beside others
+template <typename T, int D, bool REST>
 __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
     block_attn_kernel(const __grid_constant__ mj_block_attn_args a, int lg, const __grid_constant__ CUtensorMap tmk,
                       const __grid_constant__ CUtensorMap tmv) {
@@ -207,6 +213,7 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
     if (threadIdx.x == 0) flag(a.status, MJ_DEV_BAD_SPLIT);
     return;
   }
+  const bool rest = REST && item[1].z != 0;
   const int h_r = a.h_q / a.h_k;
   // rows of several sequences over the prefix that they share: all see all of the item's keys
   const bool causal = a.causal && !span;
@@ -366,6 +373,9 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
 #pragma unroll
           for (int i = 0; i < BN / 16; ++i)
             mma_f16_ts(C::O_COL + w * 128, s_col(w, j) + i * 8, v + i * 128, idesc, j > 0 || i > 0);
+          if (rest)
+#pragma unroll
+            for (int i = 0; i < BN / 16; ++i) mma_f16_ts(C::O_COL + w * 128, s_col(w, j) + BN / 2 + i * 8, v + i * 128, idesc, 1);
           mma_commit(&o_full[at(w, j)]);
           mma_commit(&v_empty[j % VST]);
         }
@@ -582,22 +592,42 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
             }
           }
         }
+        if (!rest) {
 #pragma unroll
-        for (int c = 0; c < BN / 32; ++c) {  // 32 keys: 16 columns of P
-          uint32_t p[16];
+          for (int c = 0; c < BN / 32; ++c) {  // 32 keys: 16 columns of P
+            uint32_t p[16];
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
+            for (int g = 0; g < 2; ++g) {
+              float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float2 d = s[16 * c + 8 * g + i];
+                const float2 e = i % 4 < kPolyOf4 ? exp2_poly(d) : make_float2(exp2_approx(d.x), exp2_approx(d.y));
+                sum = fadd2(sum, e);
+                p[8 * g + i] = f2_to_h2(e.x, e.y);
+              }
+              l = fmaf(sum.x + sum.y, sc[2 * c + g].z, l);
+            }
+            tmem_st16(s_addr + 16 * c, p);
+          }
+        } else {  // and what its rounding left, in the other half of S
+#pragma unroll
+          for (int g = 0; g < BN / 16; ++g) {
+            uint32_t p[8], lost[8];
             float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              const float2 d = s[16 * c + 8 * g + i];
+              const float2 d = s[8 * g + i];
               const float2 e = i % 4 < kPolyOf4 ? exp2_poly(d) : make_float2(exp2_approx(d.x), exp2_approx(d.y));
               sum = fadd2(sum, e);
-              p[8 * g + i] = f2_to_h2(e.x, e.y);
+              p[i] = f2_to_h2(e.x, e.y);
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p[i])), r = fadd2(e, make_float2(-f.x, -f.y));
+              lost[i] = f2_to_h2(r.x, r.y);
             }
-            l = fmaf(sum.x + sum.y, sc[2 * c + g].z, l);
+            l = fmaf(sum.x + sum.y, sc[g].z, l);
+            tmem_st8(s_addr + 8 * g, reinterpret_cast<const float*>(p));
+            tmem_st8(s_addr + BN / 2 + 8 * g, reinterpret_cast<const float*>(lost));
           }
-          tmem_st16(s_addr + 16 * c, p);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -842,10 +872,10 @@ static bool make_map(CUtensorMap* m, const void* base, int64_t s_page, int64_t s
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool REST>
 static cudaError_t launch_t(const mj_block_attn_args& a, cudaStream_t stream) {
   using C = Cfg<T, D>;
-  auto kern = block_attn_kernel<T, D>;
+  auto kern = block_attn_kernel<T, D, REST>;
   static std::atomic<int> ready[kMaxDevices];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -873,10 +903,16 @@ static cudaError_t launch_t(const mj_block_attn_args& a, cudaStream_t stream) {
 
 }  // namespace ba
 
+template <typename T, bool REST>
+static cudaError_t attention_t(const mj_block_attn_args& a, cudaStream_t stream) {
+  return a.head_size == 256 ? ba::launch_t<T, 256, REST>(a, stream) : ba::launch_t<T, 128, REST>(a, stream);
+}
+
 cudaError_t launch_block_attention(const mj_block_attn_args& a, cudaStream_t stream) {
-  if (a.dtype == MJ_DT_FP16)
-    return a.head_size == 256 ? ba::launch_t<__half, 256>(a, stream) : ba::launch_t<__half, 128>(a, stream);
-  return a.head_size == 256 ? ba::launch_t<__nv_bfloat16, 256>(a, stream) : ba::launch_t<__nv_bfloat16, 128>(a, stream);
+  if (a.dtype != MJ_DT_FP16) return attention_t<__nv_bfloat16, false>(a, stream);
+  // partials that nothing here merges are for mj_block_join: items of groups among
+  // them (the code for those costs prompts of fp16 1 %)
+  return a.num_slots && !a.num_merges ? attention_t<__half, true>(a, stream) : attention_t<__half, false>(a, stream);
 }
 
 template <typename T>

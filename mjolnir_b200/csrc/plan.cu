@@ -212,6 +212,7 @@ namespace {
 struct SharedBlock {
   int32_t seq, row0, t0, t1, span;
   bool slotted;  // leaves partials even in one piece
+  bool rest;     // P in two terms: rows that the decode kernel serves without the group
   int32_t group, pieces, slot;
 };
 constexpr int kMinPiece = 8;
@@ -294,7 +295,7 @@ const char* shared_step(SharedStep& st, const int32_t* query_lens, const int32_t
       st.place[s] = st.group_rows[g];
       st.group_rows[g] += (int64_t)query_lens[s] * h_r;
     }
-    for (int64_t r = 0; r < st.group_rows[g]; r += rows) st.blocks.push_back({first, (int32_t)r, 0, tokens / keys, count, true, g, 1, -1});
+    for (int64_t r = 0; r < st.group_rows[g]; r += rows) st.blocks.push_back({first, (int32_t)r, 0, tokens / keys, count, true, first < decode_seqs, g, 1, -1});
   }
   st.of_groups = st.blocks.size();
   for (int s = decode_seqs; s < num_seqs; ++s) {
@@ -303,7 +304,7 @@ const char* shared_step(SharedStep& st, const int32_t* query_lens, const int32_t
     for (int64_t r = 0; r < all; r += rows) {
       const int64_t last = causal ? L - n + (std::min(r + rows, all) - 1) / h_r : L - 1;  // last key seen
       const int t1 = last < 0 ? 0 : (int32_t)(last / keys + 1);
-      st.blocks.push_back({s, (int32_t)r, t0, std::max(t0, t1), 0, st.group_of[s] >= 0, -1, 1, -1});
+      st.blocks.push_back({s, (int32_t)r, t0, std::max(t0, t1), 0, st.group_of[s] >= 0, false, -1, 1, -1});
     }
   }
   return nullptr;
@@ -421,7 +422,7 @@ int mj_block_shared_plan(const int32_t* query_lens, const int32_t* seq_lens, int
       for (int i = 0; i < b.pieces; ++i) {  // pieces of equal length, to a tile
         const int64_t t = b.t1 - b.t0;
         const int32_t w[8] = {b.seq, b.row0, (int32_t)(b.t0 + t * i / b.pieces), (int32_t)(b.t0 + t * (i + 1) / b.pieces),
-                              b.slot < 0 ? -1 : b.slot + i, b.span, 0, 0};
+                              b.slot < 0 ? -1 : b.slot + i, b.span, b.rest, 0};
         std::copy(w, w + 8, work_out + 8 * at++);
       }
     *num_work = (int)nw;

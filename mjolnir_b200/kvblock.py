@@ -381,8 +381,11 @@ class BlockAttention:
         these neighbouring sequences are the same ones, in the same pages of
         ``block_table`` (the first of them is read for all). Their keys are then
         read once for the whole group where that takes less time. The result is
-        the same as without, but for the order of its sums. A graph with ``fixed_grid`` replays later
-        plans that share alike."""
+        the same as without, but for the order of its sums and, of single tokens
+        and drafts in bf16, for weights over the prefix of 11 bits (the other
+        sequences' have as many without it), which is under the rounding of
+        their outputs. A graph with ``fixed_grid`` replays later plans that
+        share alike."""
         q = [int(x) for x in query_lens]
         if len(q) > self.max_num_seqs or sum(q) > self.max_num_tokens:
             raise ValueError(f"{len(q)} sequences / {sum(q)} tokens beyond the runner's capacity")
