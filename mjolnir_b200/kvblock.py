@@ -384,8 +384,9 @@ class BlockAttention:
         the same as without, but for the order of its sums and, of single tokens
         and drafts in bf16, for weights over the prefix of 11 bits (the other
         sequences' have as many without it), which is under the rounding of
-        their outputs. A graph with ``fixed_grid`` replays later plans that
-        share alike."""
+        their outputs. A graph with ``fixed_grid`` replays later plans of the
+        same ``shared``: whether and how they share then follows from the
+        arguments alone, and every query has to see all the tokens named."""
         q = [int(x) for x in query_lens]
         if len(q) > self.max_num_seqs or sum(q) > self.max_num_tokens:
             raise ValueError(f"{len(q)} sequences / {sum(q)} tokens beyond the runner's capacity")
@@ -402,7 +403,7 @@ class BlockAttention:
         decode, few = None, 0
         if q and 1 <= q[0] <= self.max_q_len:
             few = next((i for i, x in enumerate(q) if x != q[0]), len(q))
-        groups = self._groups(shared, q, kv, few, causal)
+        groups = self._groups(shared, q, kv, few, causal, fixed_grid)
         starts = [0] * len(q)
         for first, count, tokens in groups:
             starts[first:first + count] = [tokens if n else 0 for n in q[first:first + count]]
@@ -428,9 +429,10 @@ class BlockAttention:
         return BlockPlan(q, sum(q), block_table, seq_lens, self.plan_buf[:n + 1], self.plan_buf[w0:used].view(-1, 8),
                          self.plan_buf[m0:m0 + 4 * nm].view(-1, 4), slots, causal, decode)
 
-    def _groups(self, shared, q: list[int], kv: list[int], few: int, causal: bool) -> list[tuple[int, int, int]]:
+    def _groups(self, shared, q: list[int], kv: list[int], few: int, causal: bool, fixed_grid: bool = False) -> list[tuple[int, int, int]]:
         """The groups worth a shared read, with the tokens that every query of
-        theirs sees, in whole tiles of the decode kernel."""
+        theirs sees, in whole tiles of the decode kernel. With ``fixed_grid``
+        they follow from ``q`` and ``shared`` alone."""
         groups, end = [], 0
         for first, count, tokens in sorted((int(a), int(b), int(c)) for a, b, c in shared):
             if first < end or count < 1 or first + count > len(q) or tokens < 0:
@@ -438,7 +440,10 @@ class BlockAttention:
                                  "apart from the other groups")
             end = first + count
             seen = [kv[s] - (q[s] if causal else 0) for s in range(first, end) if q[s]]
-            tokens = min([tokens, kv[first], *seen]) // TILE_ROWS * TILE_ROWS
+            named, tokens = tokens // TILE_ROWS * TILE_ROWS, min([tokens, kv[first], *seen]) // TILE_ROWS * TILE_ROWS
+            if fixed_grid and tokens < named and len(seen) > 1:
+                raise ValueError(f"shared: some query of sequences {first} to {end - 1} sees fewer than the group's tokens: with fixed_grid "
+                                 "every one has to, whatever the step")
             if len(seen) > 1 and tokens > 0:
                 groups.append((first, count, tokens))
         # every row block of a group, and of its sequences on the chunk kernel, takes a slot
@@ -449,6 +454,10 @@ class BlockAttention:
             if room < 0:
                 break
             kept.append((first, count, tokens))
+        if fixed_grid:  # the gain does not depend on the keys behind the prefix
+            kv = list(q)
+            for first, count, tokens in kept:
+                kv[first:first + count] = [tokens + n for n in q[first:first + count]]
         return kept if kept and self._worth(q, kv, few, kept, causal) else []
 
     def _worth(self, q: list[int], kv: list[int], few: int, groups, causal: bool) -> bool:
