@@ -450,10 +450,10 @@ class BlockAttention:
         room, h_r, kept = self.max_shared_slots, self.h_q // self.h_k, []
         for first, count, tokens in groups:
             rows = [n * h_r for n in q[first:first + count]]
-            room -= -(-sum(rows) // self.rows) + sum(-(-n // self.rows) for n in rows[max(few - first, 0):])
-            if room < 0:
-                break
-            kept.append((first, count, tokens))
+            need = -(-sum(rows) // self.rows) + sum(-(-n // self.rows) for n in rows[max(few - first, 0):])
+            if need <= room:
+                room -= need
+                kept.append((first, count, tokens))
         if fixed_grid:  # the gain does not depend on the keys behind the prefix
             kv = list(q)
             for first, count, tokens in kept:
