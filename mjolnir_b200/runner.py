@@ -376,11 +376,14 @@ class DecodeRunner:
         if not (1 <= q_len <= self.max_q_len and num_seqs <= self.max_num_seqs):
             raise ValueError(f"q_len {q_len} / num_seqs {num_seqs} beyond the runner's capacity")
         lens = [int(x) + margin for x in list(seq_lens_cpu)[:num_seqs]]
-        starts = [0] * num_seqs if starts is None else [int(x) for x in starts]
-        if any(x % TILE_ROWS or not 0 <= x <= max(0, n) for x, n in zip(starts, lens)) or len(starts) != num_seqs:
-            raise ValueError(f"starts must be multiples of {TILE_ROWS} up to the lengths, got {starts[:8]}")
+        own = lens  # tokens that the items cover
+        if starts is not None:
+            starts = [int(x) for x in starts]
+            if len(starts) != num_seqs or any(x % TILE_ROWS or not 0 <= x <= max(0, n) for x, n in zip(starts, lens)):
+                raise ValueError(f"starts must be multiples of {TILE_ROWS} up to the lengths, got {starts[:8]}")
+            own = [n - x for n, x in zip(lens, starts)]
         p = plan_split_kv(
-            [n - x for n, x in zip(lens, starts)],
+            own,
             self.h_k,
             self.n_tiles(q_len),
             self.sm_count,
@@ -390,7 +393,7 @@ class DecodeRunner:
             rebalance=self.rebalance,
         )
         work_h, pieces = torch.from_numpy(p.work_array()), p.n_splits
-        if any(starts):
+        if starts is not None and any(starts):
             if self.max_splits < 2:
                 raise ValueError("starts need a runner of at least two splits")
             at = torch.tensor([x // TILE_ROWS for x in starts], dtype=torch.int32)[work_h[:, 0].long()]
@@ -419,7 +422,7 @@ class DecodeRunner:
             chunk_tiles=p.chunk_tiles,
             num_chunks=real,
             causal=causal or q_len == 1,
-            tile_jobs=sum(-(-(n - x) // 128) for n, x in zip(lens, starts)) * self.h_k,
+            tile_jobs=sum(-(-L // 128) for L in own) * self.h_k,
             pieces=p.n_splits,
         )
 
