@@ -31,7 +31,8 @@ from .plan import TILE_ROWS
 from .runner import DecodeRunner, StepPlan, _ptr, call, dtype_code
 
 HEAD_SIZES = (128, 256)
-SHARED_BLOCKS = 64  # row blocks of sequences behind a shared prefix that a step has room for
+SHARED_BLOCKS = 64  # row blocks of sequences behind a shared prefix that a step has room for,
+SHARED_BYTES = 1 << 27  # while their partials take no more than this
 BLOCK_TOKENS = tuple(_lib.BLOCK_FORMATS)
 
 
@@ -321,10 +322,15 @@ class BlockAttention:
     kernel and chunk kernel: 8 KV heads of 128, 4 rows 48 and 142 us, 16 rows 66
     and 143, 48 rows 107 and 144; 4 KV heads of 128, 48 rows 65 and 101, 64 rows
     134 and 101; 4 KV heads of 256, 6 rows 51 and 117, 16 rows 72 and 118, 18 rows
-    133 and 118, 48 rows 198 and 122."""
+    133 and 118, 48 rows 198 and 122.
+
+    Split partials take some 40 MB. Steps that share prefixes have others, of up
+    to 185 MB, which the first such plan allocates, or with ``shared_prefixes``
+    the constructor."""
 
     def __init__(self, *, num_heads: int, num_kv_heads: int, head_size: int, page_size: int, block_tokens: int = 16,
-                 max_num_seqs: int = 256, max_num_tokens: int = 8192, max_q_len: int = 4, device: torch.device | str = "cuda"):
+                 max_num_seqs: int = 256, max_num_tokens: int = 8192, max_q_len: int = 4, shared_prefixes: bool = False,
+                 device: torch.device | str = "cuda"):
         if num_heads % num_kv_heads:
             raise ValueError("num_heads must be a multiple of num_kv_heads")
         if page_size not in (16, 32, 64, 128):
@@ -351,14 +357,15 @@ class BlockAttention:
         # the plan: q_start | merges | work, one fixed-address buffer and one copy a step
         self._at = (-(-(max_num_seqs + 1) // 4) * 4, -(-(max_num_seqs + 1) // 4) * 4 + 4 * self.max_slots)
         self.plan_buf = torch.zeros(self._at[1] + 8 * self.max_work, dtype=torch.int32, device=self.device)
-        # steps with shared prefixes: q_start | joins | work in a buffer of their own, made
-        # with the partials by the first such plan. Every row of a group has a partial over
-        # the prefix, and behind a chunk kernel's one of its own: room for this many row
-        # blocks, beside the partials that splitting asks for
-        self.max_shared_slots = self.max_slots + 2 * min(max_num_seqs, SHARED_BLOCKS)
+        # steps with shared prefixes: q_start | joins | work in a buffer of their own, and
+        # partials. Every row of a group has a partial over the prefix, and behind a chunk
+        # kernel's one of its own: room for this many row blocks, beside the partials that
+        # splitting asks for
+        per_slot = num_kv_heads * self.rows * head_size * 4
+        self.max_shared_slots = self.max_slots + min(2 * min(max_num_seqs, SHARED_BLOCKS), SHARED_BYTES // per_slot)
         self.max_items = self.max_work + self.max_shared_slots - self.max_slots
         self._shared_at = (self._at[0], self._at[0] + 12 * (max_num_seqs + self.max_work))
-        self.shared_buf = self.shared_o_part = self.shared_lse_part = None
+        self.shared = self._shared_buffers() if shared_prefixes else None
         self.o_part = torch.empty(self.max_slots * num_kv_heads * self.rows * head_size, dtype=torch.float32, device=self.device)
         self.lse_part = torch.empty(self.max_slots * num_kv_heads * self.rows, dtype=torch.float32, device=self.device)
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
@@ -379,7 +386,8 @@ class BlockAttention:
         ``shared`` names prefixes that sequences have in common, as ``(first
         sequence, number of sequences, tokens)``: the first ``tokens`` tokens of
         these neighbouring sequences are the same ones, in the same pages of
-        ``block_table`` (the first of them is read for all). Their keys are then
+        ``block_table`` (the first of them is read for all). A sequence is in one
+        group at most, also where prefixes stand behind others. Their keys are then
         read once for the whole group where that takes less time. The result is
         the same as without, but for the order of its sums and, of single tokens
         and drafts in bf16, for weights over the prefix of 11 bits (the other
@@ -468,14 +476,19 @@ class BlockAttention:
         behind 4K: 2 sequences 23 and 21 us, 4 28 and 43, 32 81 and 139."""
         return _lib.block_shared_worth(q, kv, few, groups, self.h_q, self.h_k, self.d, causal, self.sm_count, self.max_shared_slots)
 
+    def _shared_buffers(self) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Plan, output and log-sum-exp partials of steps that share."""
+        rows = self.max_shared_slots * self.h_k * self.rows
+        return (torch.zeros(self._shared_at[1] + 8 * self.max_items, dtype=torch.int32, device=self.device),
+                torch.empty(rows * self.d, dtype=torch.float32, device=self.device),
+                torch.empty(rows, dtype=torch.float32, device=self.device))
+
     def _plan_shared(self, q, kv, groups, starts, few, decode, block_table, seq_lens, causal) -> BlockPlan:
         n, (j0, w0) = len(q), self._shared_at
-        if self.shared_buf is None:
-            part = self.max_shared_slots * self.h_k * self.rows
-            self.shared_buf = torch.zeros(w0 + 8 * self.max_items, dtype=torch.int32, device=self.device)
-            self.shared_o_part = torch.empty(part * self.d, dtype=torch.float32, device=self.device)
-            self.shared_lse_part = torch.empty(part, dtype=torch.float32, device=self.device)
-        stage = torch.empty(self.shared_buf.shape[0], dtype=torch.int32, pin_memory=True)
+        if self.shared is None:
+            self.shared = self._shared_buffers()
+        buf = self.shared[0]
+        stage = torch.empty(buf.shape[0], dtype=torch.int32, pin_memory=True)
         host = stage.numpy()
         host[0] = 0
         np.cumsum(q, out=host[1:n + 1])
@@ -484,9 +497,9 @@ class BlockAttention:
         nw, nj, rows, slots = _lib.block_shared_plan(q, kv, pieces, groups, self.h_q, self.h_k, self.d, causal, self.sm_count,
                                                      self.max_shared_slots, work, joins)
         used = w0 + 8 * nw
-        self.shared_buf[:used].copy_(stage[:used], non_blocking=True)
-        return BlockPlan(q, sum(q), block_table, seq_lens, self.shared_buf[:n + 1], self.shared_buf[w0:used].view(-1, 8),
-                         self.shared_buf[:0].view(-1, 4), slots, causal, decode, self.shared_buf[j0:j0 + 12 * nj].view(-1, 12), rows)
+        buf[:used].copy_(stage[:used], non_blocking=True)
+        return BlockPlan(q, sum(q), block_table, seq_lens, buf[:n + 1], buf[w0:used].view(-1, 8),
+                         buf[:0].view(-1, 4), slots, causal, decode, buf[j0:j0 + 12 * nj].view(-1, 12), rows)
 
     def run(
         self,
@@ -526,7 +539,7 @@ class BlockAttention:
                 one, _lib.MJ_SCALE_TENSOR, one, _lib.MJ_SCALE_TENSOR, None, None, scale, causal,
                 int(p.with_reduction and plan.joins is None),
                 r.kernel, r.status.data_ptr(), r.merge_counters.data_ptr() if r.merges(p) else None, *scales, *ss, 0), dev)
-        part = (self.o_part, self.lse_part) if plan.joins is None else (self.shared_o_part, self.shared_lse_part)
+        part = (self.o_part, self.lse_part) if plan.joins is None else self.shared[1:]
         part = (part[0].data_ptr(), part[1].data_ptr())
         if plan.work is not None:
             call(_lib.block_attention, _lib.BlockAttnArgs(
