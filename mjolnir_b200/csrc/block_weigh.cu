@@ -1067,23 +1067,32 @@ static cudaError_t launch_t(const mj_block_weigh_args& a, Take take, cudaStream_
   using C = Cfg<T, D, N>;
   // CTAs of a cluster, which share a job's rows where there are too few jobs (4096
   // tokens of 24 / 4 heads of 256 144 us, without 257; 2000 behind 2000 of 6 / 1 heads
-  // 28 and 73). One where there cannot be too few (300 are two an SM), or where the
-  // rows are few tiles, for looking costs (500 tokens behind 7000, 8 / 2 heads, 22.6
-  // and 19.9 us). Two otherwise, which fill all SMs. Four or eight, which leave 16 and
-  // 28 of 148 out, where the weights are too short for more jobs than the 33 or 15
-  // clusters: 600 tokens of 6 heads, 15 jobs 28.8, 21.2, 17.2 and 15.8 us with one,
-  // two, four and eight, 24 jobs 28.8, 21.1, 17.2 and 22.5, 36 jobs 29.5, 21.3, 23.3
-  // and 29.3, 80 jobs, where none share, 29.5 and 31 to 32.
+  // 28 and 73). One where the rows are few tiles, for looking costs (500 tokens behind
+  // 7000, 8 / 2 heads, 22.6 and 19.9 us), or where they are enough for two jobs an SM,
+  // as far as the tensor's rows tell (16 prompts of 512, 32 / 8 heads, 68 us, in
+  // clusters 72; 500 tokens in a buffer of 8192 rows 20.3, in clusters 14.7). Two
+  // otherwise, which fill all SMs. Four or eight, which on 148 SMs leave 16 and 28
+  // out, where the weights are too short for more jobs than there are such clusters
+  // (33 and 15; weights wider than their sequences take two): 600 tokens of 6 heads,
+  // 15 jobs 28.8, 21.2, 17.2 and 15.8 us with one, two, four and eight, 24 jobs 28.8,
+  // 21.1, 17.2 and 22.5, 36 jobs 29.5, 21.3, 23.3 and 29.3, 80 jobs, where none share,
+  // 29.5 and 31 to 32.
   const int64_t most = a.window && a.window < a.num_rows ? a.window : a.num_rows, tiles = (most * (a.h_q / a.h_k) + N - 1) / N;
-  const int64_t least_jobs = (a.num_rows + KEYS - 1) / KEYS * a.h_k, most_jobs = (a.weights_cols + KEYS - 1) / KEYS * a.num_seqs * a.h_k;
-  int level = tiles < 8 || least_jobs >= 300 ? 0 : most_jobs > 33 ? 1 : most_jobs > 15 ? 2 : 3;
-  static_assert(1 << 3 <= C::PARTS, "buffers of a cluster's sums");
-  const int cluster = 1 << level;
-  auto kern = cluster > 1 ? block_weigh_kernel<T, D, N, true> : block_weigh_kernel<T, D, N, false>;
+  const int64_t row_jobs = (a.num_rows + KEYS - 1) / KEYS * a.h_k, most_jobs = (a.weights_cols + KEYS - 1) / KEYS * a.num_seqs * a.h_k;
+  auto kern = block_weigh_kernel<T, D, N, false>;
   static std::atomic<int> ready[4][kMaxDevices];
-  int grid = 0;
-  cudaError_t e = prepare(kern, C::THREADS, C::SMEM, 1, cluster, ready[level], &grid);
+  int grid = 0, level = 0;  // log2 of a cluster's CTAs
+  cudaError_t e = prepare(kern, C::THREADS, C::SMEM, 1, 1, ready[0], &grid);
   if (e != cudaSuccess) return e;
+  if (tiles >= 8 && row_jobs < 2 * grid) {
+    static_assert(1 << 3 <= C::PARTS, "buffers of a cluster's sums");
+    kern = block_weigh_kernel<T, D, N, true>;
+    for (level = 3;; --level) {
+      if ((e = prepare(kern, C::THREADS, C::SMEM, 1, 1 << level, ready[level], &grid)) != cudaSuccess) return e;
+      if (level == 1 || most_jobs <= grid >> level) break;
+    }
+  }
+  const int cluster = 1 << level;
   CUtensorMap mk, mq;
   if (!key_map(&mk, a)) return cudaErrorInvalidValue;
   // a tile of Q rows: tb tokens of hb heads of a group, or, of a larger group, N heads of one token
