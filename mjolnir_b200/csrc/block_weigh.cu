@@ -1143,12 +1143,13 @@ static cudaError_t launch_d(const mj_block_weigh_args& a, cudaStream_t stream) {
   // 57). The lengths are the device's, so where there may be both, both are
   // launched: 64 single tokens of 8K beside a chunk of 512 take 155 us, with the
   // kernel for many rows alone 435; beside a chunk of 190 131, with the one for few
-  // alone 717. (A launch that finds nothing costs 2 us.) With no more tokens than
-  // sequences all are taken to be single ones.
+  // alone 717. (A launch that finds nothing costs 2 us: windows no longer than the
+  // tile need none: 4 of each of 8 x 300 tokens behind 6K 24 us, with it 28.) With no
+  // more tokens than sequences all are taken to be single ones.
   const int64_t most = a.window ? (int64_t)a.num_seqs * a.window : a.num_rows, tokens = a.num_rows < most ? a.num_rows : most;
   const int h_r = a.h_q / a.h_k, fit = 16 / h_r;
   const bool few = fit && (a.num_seqs > 1 || tokens <= fit),
-             many = !few || (tokens > a.num_seqs && tokens > fit);
+             many = !few || (tokens > a.num_seqs && tokens > fit && !(a.window && a.window <= fit));
   if (many) {
     constexpr int N256 = std::is_same<T, __half>::value ? 64 : 96;  // (fp16's two sums of 96 do not fit TMEM)
     const Take take = {few ? fit + 1 : 1, INT_MAX, few};

@@ -1,0 +1,43 @@
+"""What a call of kvblock.weigh launches, and arguments at the ends of their ranges."""
+
+import pytest
+import torch
+
+from tests.block_helpers import Cache
+
+pytestmark = pytest.mark.gpu
+
+
+def step(lens, q_lens, h_q=8, h_k=2, rows=None, seed=1, cols=None):
+    """(arguments of weigh but the weights, weights)"""
+    c = Cache(lens, h_k=h_k, seed=seed)
+    rows = rows or sum(q_lens)
+    q = torch.randn(rows, h_q, 128, generator=c.g).bfloat16().cuda()
+    lse = (torch.randn(rows, h_q, generator=c.g) + 5).cuda()
+    at = torch.tensor([sum(q_lens[:i]) for i in range(len(q_lens) + 1)], dtype=torch.int32).cuda()
+    lens = torch.tensor(lens, dtype=torch.int32).cuda()
+    return (q, lse, c.kv[0], c.sc[0], c.table.cuda(), at, lens), torch.rand(len(q_lens), h_k, cols or max(c.lens), generator=c.g).cuda()
+
+
+def launches(call):
+    """The kernels of a call, from the graph that it is captured into."""
+    from cuda.bindings import runtime
+
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        call()
+    err, _, count = runtime.cudaGraphGetNodes(graph.raw_cuda_graph())
+    assert int(err) == 0
+    return count
+
+
+@pytest.mark.parametrize("q_lens,window,want", [([30, 40], 0, 2), ([30, 40], 5, 2), ([30, 40], 4, 1), ([30, 40], 1, 1), ([1, 1], 0, 1), ([40], 0, 1),
+                                                ([40], 4, 1), ([3], 0, 1)])
+def test_a_launch_that_cannot_find_a_sequence_is_left_out(q_lens, window, want):
+    """Sequences of at most 4 queries (16 rows of 4 heads) have one kernel, those of more the other."""
+    from mjolnir_b200 import kvblock
+
+    args, w = step([300 + n for n in q_lens], q_lens)
+    assert launches(lambda: kvblock.weigh(*args, w, 0.1, window=window)) == want
