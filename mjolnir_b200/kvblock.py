@@ -244,7 +244,7 @@ def weigh(
         query.data_ptr(), dt, *qs, lse.data_ptr(), min(q_shape[0], l_shape[0]), n, h_q, h_k, d, page_size, kv_format,
         k_cache.data_ptr(), *st, k_scales.data_ptr(), *ss, pages, block_table.data_ptr(), block_table.stride(0),
         block_table.shape[1], offsets.data_ptr(), seq_lens.data_ptr(), weights.data_ptr(), *ws, weights.shape[2],
-        float(softmax_scale), int(window), _ptr(status)), dev)
+        float(softmax_scale), min(int(window), 2**31 - 1), _ptr(status)), dev)  # (ctypes would cut off what is above)
     return weights
 
 

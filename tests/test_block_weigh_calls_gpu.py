@@ -41,3 +41,12 @@ def test_a_launch_that_cannot_find_a_sequence_is_left_out(q_lens, window, want):
 
     args, w = step([300 + n for n in q_lens], q_lens)
     assert launches(lambda: kvblock.weigh(*args, w, 0.1, window=window)) == want
+
+
+@pytest.mark.parametrize("window", [2**31 - 1, 2**31, 2**32, 2**32 + 1, 2**40 + 3])
+def test_windows_beyond_32_bits_are_every_query(window):
+    from mjolnir_b200 import kvblock
+
+    args, w = step([200, 90, 61], [40, 3, 60])
+    want = kvblock.weigh(*args, w.clone(), 0.1)
+    assert torch.equal(kvblock.weigh(*args, w.clone(), 0.1, window=window), want)
