@@ -115,12 +115,19 @@ struct Take {
   bool both;
 };
 
-// Of two launches, one that has none leaves before it takes anything.
-__device__ __forceinline__ bool has_any(const mj_block_weigh_args& a, Take take) {
+// A sequence that the call complains of: n queries from q0 on, L tokens.
+__device__ __forceinline__ bool out_of_range(const mj_block_weigh_args& a, int q0, int n, int L) {
+  const int64_t room = (int64_t)a.block_table_cols * a.page_size;
+  return (q0 < 0) | (n < 0) | (q0 + (int64_t)n > a.num_rows) | (L < 0) | (L > a.weights_cols) | (L > room) | (L > INT_MAX - 8 * KEYS);
+}
+
+// Of two launches, one that has none leaves before it takes anything; the first
+// stays where there is something to complain of.
+__device__ __forceinline__ bool has_any(const mj_block_weigh_args& a, Take take, bool first) {
   int any = 0;
   for (int s = threadIdx.x; s < a.num_seqs; s += blockDim.x) {
-    const int n = a.offsets[s + 1] - a.offsets[s], m = a.window && a.window < n ? a.window : n;
-    any |= (m >= take.lo && m <= take.hi) || n < 0;  // (that is complained of)
+    const int q0 = a.offsets[s], n = a.offsets[s + 1] - q0, L = first ? a.seq_lens[s] : 0, m = a.window && a.window < n ? a.window : n;
+    any |= (m >= take.lo && m <= take.hi) | (first && out_of_range(a, q0, n, L));  // (the loads wait once)
   }
   return __syncthreads_or(any) != 0;
 }
@@ -138,8 +145,7 @@ __device__ __forceinline__ void find_jobs(const C& cta, Take take, int tb, int h
     q0 = a.offsets[s];
     n = a.offsets[s + 1] - q0;
     L = a.seq_lens[s];
-    if (q0 < 0 || n < 0 || q0 + (int64_t)n > a.num_rows || L < 0 || L > a.weights_cols ||
-        L > (int64_t)a.block_table_cols * a.page_size || L > INT_MAX - 8 * KEYS) {
+    if (out_of_range(a, q0, n, L)) {
       if (complain) flag(a.status, MJ_DEV_BAD_LENGTH);
       return 0;
     }
@@ -435,7 +441,7 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
   griddep_wait();
   if (take.both) {
     griddep_launch_dependents();
-    if (!has_any(a, take)) return;  // (every CTA of a cluster)
+    if (!has_any(a, take, true)) return;  // (every CTA of a cluster)
   }
   if (threadIdx.x == 0) {
     auto init = [](uint64_t* b, int n, int count) {
@@ -792,7 +798,7 @@ __global__ void __launch_bounds__(Few<D>::THREADS, Few<D>::CTAS)
   }
   if (!take.both) {
     griddep_wait();
-  } else if (!has_any(a, take)) {
+  } else if (!has_any(a, take, false)) {
     griddep_wait();
     return;
   }

@@ -50,3 +50,17 @@ def test_windows_beyond_32_bits_are_every_query(window):
     args, w = step([200, 90, 61], [40, 3, 60])
     want = kvblock.weigh(*args, w.clone(), 0.1)
     assert torch.equal(kvblock.weigh(*args, w.clone(), 0.1, window=window), want)
+
+
+@pytest.mark.parametrize("rows", [40, 3])
+@pytest.mark.parametrize("lens,at", [([500, 90], [0, 0, 0]), ([90, 500], [0, 0, 0]), ([90, -1], [0, 0, 0]), ([90, 90], [99, 99, 99]), ([90, 90], [0, 0, -2]),
+                                     ([90, 90], [-1, -1, -1])])
+def test_lengths_and_offsets_out_of_range_are_flagged_without_queries_too(lens, at, rows):
+    """Whatever the call launches (rows for both kernels, or for one)."""
+    from mjolnir_b200 import _lib, kvblock
+
+    args, w = step([90, 90], [rows - 1, 1], cols=100)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    before = w.clone()
+    kvblock.weigh(*args[:5], torch.tensor(at, dtype=torch.int32).cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), w, 0.1, status=status)
+    assert status.item() == _lib.MJ_DEV_BAD_LENGTH and torch.equal(w, before)
