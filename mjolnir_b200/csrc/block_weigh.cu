@@ -756,8 +756,9 @@ __global__ void __launch_bounds__(Cfg<T, D, N>::THREADS, 1)
 // Where a step's sequences have a few rows each, K is read for little arithmetic,
 // and converting it would cost more than multiplying it. So K enters the product
 // as stored, and Q, once a job, as three e4m3 terms of its row scaled by a power
-// of two to [128, 256): x = hi + mid / 16 + lo / 256, 12 bits and more of it down
-// to 2^-18 of the row's largest element (bf16 and fp16 have 8 and 11). The terms
+// of two to [128, 256): x = hi + mid / 16 + lo / 256, in steps of 2^-17 at least. So
+// bf16 elements (8 bits) are exact down to 2^-17 of the row's largest, fp16 ones (11)
+// down to 2^-14, and what is below is off by 2^-25 of the largest at most. The terms
 // are columns of their own, joined in fp32. Several CTAs an SM: their roles wait
 // more than they work. (With K converted to 16 bits, two CTAs an SM, 32 x 8K
 // single tokens of 32 / 8 heads took 58 us, with one 71.)
