@@ -19,8 +19,8 @@
 //
 // What bounds it: latency. Every pass of the selection and every step of the move
 // waits for memory or for the cluster, and there are few of either a CTA. 4
-// sequences of 1.1K tokens cut to 1K, 8 KV heads of 128: 13 us, 8.7 MB; 16 of 8K
-// cut to 2K: 49 us, 2.8 TB/s of what has to move; one of 60K cut to 8K 41 us.
+// sequences of 1.1K tokens cut to 1K, 8 KV heads of 128: 13.4 us, 8.7 MB; 16 of 8K
+// cut to 2K: 48.3 us, 2.9 TB/s of what has to move; one of 60K cut to 8K 42.5 us.
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -118,32 +118,31 @@ __device__ __forceinline__ uint32_t shift4(uint32_t codes, __half2 f, __half2 g)
   }
   return out[0] | out[1] << 16;
 }
-// The cluster's barrier between a step's reads and its writes, in two halves.
-// Nothing that one CTA writes there is read by another: it only has to come after
-// the reads (a release would also wait for the writes of the step before). A
-// store that depends on their values, and never happens, stands before it.
-__device__ __forceinline__ void cluster_arrive(float not_negative, int* smem) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.lt.f32 p, %0, 0f00000000;\n\t"
-      "@p st.shared.u32 [%1], 0;\n\t"
-      "barrier.cluster.arrive.relaxed.aligned;\n\t}" ::"f"(not_negative),
-      "r"(smem_addr(smem))
-      : "memory");
-}
+// The cluster's barrier between a step's reads and its writes, in two halves: what
+// the CTAs read before they arrive they have read before one that waited writes.
+// Only a release orders reads before it; it waits for the writes of the step before
+// too (16 x 8K cut to 2K 48.3 us; with a relaxed arrival, whose order nothing
+// promises, 45.9).
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// Keeps the computation of x >= 0 before what follows: a store that never happens.
+__device__ __forceinline__ void settle(float x, int* smem) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.f32 p, %0, 0f00000000;\n\t@p st.shared.u32 [%1], 0;\n\t}" ::"f"(x), "r"(smem_addr(smem)) : "memory");
+}
 
 // 2^k for -24 <= k <= 15
 __device__ __forceinline__ uint32_t h_exp2(int k) { return k < -14 ? 1u << (k + 24) : (uint32_t)(15 + k) << 10; }
 
-template <int D>
+// SHARE: CTAs of a cluster share a job
+template <int D, bool SHARE>
 __global__ void __launch_bounds__(Cfg<D>::THREADS, D == 256 ? 1 : 2)
     block_evict_kernel(const __grid_constant__ mj_block_evict_args a, int lg, uint64_t per_page) {
   constexpr int THREADS = Cfg<D>::THREADS, WARPS = Cfg<D>::WARPS;
   extern __shared__ __align__(16) unsigned char raw[];
   auto& sm = *reinterpret_cast<typename Cfg<D>::Smem*>(raw);
   auto cluster = cg::this_cluster();
-  const int CL = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int CL = SHARE ? (int)cluster.num_blocks() : 1, rank = SHARE ? (int)cluster.block_rank() : 0;
   const int job = blockIdx.x / CL, h = job % a.h_k, seq = job / a.h_k;
   const int t = threadIdx.x, lane = t & 31, wid = t >> 5;
   griddep_wait();
@@ -341,10 +340,11 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, D == 256 ? 1 : 2)
     }
     if ((step + 1) % AHEAD) fetch(step + 1, next);
     const int count = budget - first_of(step);
-    float most[4];  // of the chunks: once they are known, this step's tokens have been read
+    float most[4];  // of the chunks
 #pragma unroll
     for (int x = 0; x < 4; ++x) most[x] = max_abs16(now[x]);
-    cluster_arrive((most[0] + most[1]) + (most[2] + most[3]), sm.pick);
+    settle((most[0] + most[1]) + (most[2] + most[3]), sm.pick);  // (behind the barrier's halves they cost 16 x 8K 2 us)
+    if (SHARE) cluster_arrive();
 #pragma unroll
     for (int x = 0; x < 4; ++x) {  // of the rows, then the blocks
       const int i = t / CPR + x * (STEP / 4), at = step % AHEAD * STEP + i;
@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, D == 256 ? 1 : 2)
     }
     __syncthreads();
     if (t < 2 * (STEP / 16)) sm.amax[(step + 2) % 3][0][t] = 0;  // (read last before that barrier, and next behind another)
-    cluster_wait();  // every CTA of the cluster has read this step's tokens
+    if (SHARE) cluster_wait();  // every CTA of the cluster has read this step's tokens
     if (t < 2 * STEP && t % STEP < count) {  // a row's side each: its block's exponent, and its codes' way there
       const int i = t % STEP, y = t / STEP, at = step % AHEAD * STEP + i;
       const int e = block_exponent(__int_as_float(sm.amax[step % 3][y][i >> lg]));
@@ -385,7 +385,6 @@ constexpr int kMaxDevices = 64;
 
 template <int D>
 static cudaError_t launch_t(const mj_block_evict_args& a, cudaStream_t stream) {
-  auto kern = block_evict_kernel<D>;
   constexpr int smem = (int)sizeof(typename Cfg<D>::Smem);
   static std::atomic<int> ready[kMaxDevices];  // CTAs that the device holds at once, once the kernel is prepared on it
   int dev = 0;
@@ -396,9 +395,10 @@ static cudaError_t launch_t(const mj_block_evict_args& a, cudaStream_t stream) {
   if (!room) {
     std::lock_guard<std::mutex> lock(tc_init_mutex());
     int sms = 0, per_sm = 0;
-    if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return e;
+    if ((e = cudaFuncSetAttribute(block_evict_kernel<D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return e;
+    if ((e = cudaFuncSetAttribute(block_evict_kernel<D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return e;
     if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
-    if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, Cfg<D>::THREADS, smem)) != cudaSuccess) return e;
+    if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, block_evict_kernel<D, true>, Cfg<D>::THREADS, smem)) != cudaSuccess) return e;
     room = std::max(1, sms * per_sm);
     ready[dev].store(room, std::memory_order_release);
   }
@@ -413,6 +413,7 @@ static cudaError_t launch_t(const mj_block_evict_args& a, cudaStream_t stream) {
   const int one_each = room / (D == 256 ? 1 : 2);
   int cl = 1;
   while (cl < 8 && 2 * cl * jobs <= room && ((2 * cl * jobs <= one_each ? cl : 2 * cl) * STEP < a.budget || (int64_t)cl * KEYS < a.weights_cols)) cl *= 2;
+  auto kern = cl > 1 ? block_evict_kernel<D, true> : block_evict_kernel<D, false>;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(jobs * cl));
   cfg.blockDim = dim3(Cfg<D>::THREADS);
