@@ -133,9 +133,13 @@ __global__ void __launch_bounds__(128, sizeof(T) == 4 ? 3 : 5)
     raw[1].load(w, 8 * cb, a.weight_dtype, VEC);
   }
   bool bad = false;  // (looked at once the rows are on their way)
+  if constexpr (kAxes) {
 #pragma unroll
-  for (int i = 0; i < NP; ++i) bad |= r2 && t < a.num_tokens && (kAxes || mine) && (pos[i] < 0 || pos[i] >= a.num_positions);
-  if constexpr (kAxes) bad = __ballot_sync(0xffffffffu, bad) >> (threadIdx.x & 31 & ~(team - 1)) & (uint32_t)((1ull << team) - 1);
+    for (int i = 0; i < NP; ++i) bad |= r2 && t < a.num_tokens && (pos[i] < 0 || pos[i] >= a.num_positions);
+    bad = __ballot_sync(0xffffffffu, bad) >> (threadIdx.x & 31 & ~(team - 1)) & (uint32_t)((1ull << team) - 1);
+  } else {
+    bad = mine && r2 && (pos[0] < 0 || pos[0] >= a.num_positions);
+  }
   if (bad && j == 0) flag(a.status, MJ_DEV_BAD_POSITION);
   if constexpr (kAxes) {
     uint2 axis = make_uint2(0, 0);
