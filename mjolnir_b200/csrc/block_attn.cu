@@ -676,7 +676,14 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
 #pragma unroll
             for (int i = 0; i < 32; i += 8)
               store8(reinterpret_cast<T*>(stage + lane * (D * 2) + ((((c + i) >> 3) ^ (lane & 7)) << 4)), v + i);
-          } else {  // partials the same way, 32 columns at a time: eight lanes a row
+          } else if (rows_here < 32) {
+            // partials of a few rows as they are (16 drafts of 18 rows behind 8K, 4 KV
+            // heads of 256, bf16 92.1 us, staged 93.8; all of a warp's, 16 tokens of 96
+            // rows behind 30K, 45.1 so and 41.4 staged)
+            if (live)
+#pragma unroll
+              for (int i = 0; i < 32; i += 8) store8(a.o_part + part * D + c + i, v + i);
+          } else {  // of whole warps staged, 32 columns at a time: eight lanes a row
 #pragma unroll
             for (int i = 0; i < 32; i += 4)
               *reinterpret_cast<float4*>(stage + lane * 128 + (((i >> 2) ^ (lane & 7)) << 4)) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
@@ -685,8 +692,8 @@ __global__ void __launch_bounds__(Cfg<T, D>::THREADS, 1)
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
               const int r = i + lane / 8;
-              const float4 x = *reinterpret_cast<const float4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-              if (r < rows_here) *reinterpret_cast<float4*>(a.o_part + (first + r) * D + c + 4 * (lane & 7)) = x;
+              *reinterpret_cast<float4*>(a.o_part + (first + r) * D + c + 4 * (lane & 7)) =
+                  *reinterpret_cast<const float4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
             }
           }
           __syncwarp();  // the TMEM load is a whole-warp operation, and the staged rows have been read
